@@ -29,7 +29,8 @@ LIB = os.path.join(LIBDIR, "libbatmobile_hip.so")
 NL_LIB = os.path.join(LIBDIR, "libbatteries_neighbor.so")
 EXT = os.path.join(PYDIR, "_batmobile" + sysconfig.get_config_var("EXT_SUFFIX"))
 
-HIP_SOURCES = ["sh.hip", "tp.hip", "mp.hip", "nl.hip", "graph.hip", "mace.hip"]
+HIP_SOURCES = ["sh.hip", "tp.hip", "mp.hip", "nl.hip", "graph.hip", "mace.hip",
+               "attention.hip", "block_norm.hip", "grad_clip.hip"]
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"
@@ -88,22 +89,23 @@ def build_ext(force=False):
     import torch
     from torch.utils import cpp_extension
 
-    src = os.path.join(CSRC, "binding.cpp")
-    if not (force or _stale(EXT, [src, LIB] + _headers())):
+    srcs = [os.path.join(CSRC, f) for f in ("binding.cpp", "binding_block.cpp")]
+    if not (force or _stale(EXT, srcs + [LIB] + _headers())):
         return EXT
     inc = cpp_extension.include_paths() + [os.path.join(ROCM, "include"), INCLUDE,
                                           sysconfig.get_paths()["include"]]
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", src, "-o", EXT,
-           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_batmobile",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           "-w"]
-    cmd += ["-I" + p for p in inc]
-    cmd += ["-L" + torch_lib, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python",
-            "-L" + LIBDIR, "-lbatmobile_hip", "-L" + os.path.join(ROCM, "lib"), "-lamdhip64",
-            "-Wl,-rpath,$ORIGIN/../lib", "-Wl,-rpath," + torch_lib]
-    _run(cmd)
+    flags = ["-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+             "-DTORCH_EXTENSION_NAME=_batmobile", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-w"] + ["-I" + p for p in inc]
+    objs = [os.path.join(BUILD, os.path.basename(f).replace(".cpp", ".o")) for f in srcs]
+    with cf.ThreadPoolExecutor(max_workers=2) as ex:
+        list(ex.map(_run, [["g++"] + flags + ["-c", f, "-o", o] for f, o in zip(srcs, objs)]))
+    _run(["g++", "-shared"] + objs + ["-o", EXT] + [
+        "-L" + torch_lib, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+        "-L" + LIBDIR, "-lbatmobile_hip", "-L" + os.path.join(ROCM, "lib"), "-lamdhip64",
+        "-Wl,-rpath,$ORIGIN/../lib", "-Wl,-rpath," + torch_lib])
     return EXT
 
 

@@ -18,6 +18,8 @@
 
 #include "batmobile_hip.h"
 
+void register_block_ops(pybind11::module_& m);  // binding_block.cpp
+
 namespace {
 
 void check_device(const torch::Tensor& t, const char* name) {
@@ -1133,6 +1135,7 @@ PYBIND11_MODULE(_batmobile, m) {
           py::arg("cutoff"), py::arg("order") = py::none(),
           "gradient of the MACE-style layer w.r.t. positions (extension); order as for "
           "mace_forward");
+    register_block_ops(m);
     m.def("selftest_mfma_16x16x4", &selftest_mfma_16x16x4, py::arg("A"), py::arg("B"),
           "D = A @ B through one v_mfma_f32_16x16x4f32 (lane-layout self test)");
     m.def("selftest_mfma_4x4x1_bcast", &selftest_mfma_4x4x1_bcast, py::arg("A"), py::arg("B"),

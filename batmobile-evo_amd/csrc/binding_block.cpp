@@ -1,0 +1,379 @@
+// The operators of an equivariant transformer block in the _batmobile extension (registered by
+// binding.cpp): attention over the edges of a graph, norms by degree with gate and residual,
+// gradient clipping.  No reference counterpart.  Host code only, over include/batmobile_hip.h.
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/extension.h>
+
+#include <cmath>
+#include <cstdint>
+#include <tuple>
+#include <vector>
+
+#include "batmobile_hip.h"
+
+namespace {
+
+using torch::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+hipStream_t stream_of(const Tensor& t) {
+    return c10::hip::getCurrentHIPStream(t.device().index()).stream();
+}
+
+void check_status(int rc, const char* what) {
+    if (rc == BATMOBILE_HIP_OK) return;
+    if (rc == BATMOBILE_HIP_ERR_ARG) TORCH_CHECK(false, what, ": invalid argument");
+    if (rc == BATMOBILE_HIP_ERR_WORKSPACE) TORCH_CHECK(false, what, ": workspace too small");
+    TORCH_CHECK(false, "HIP error in ", what, ": ", hipGetErrorString(static_cast<hipError_t>(rc)));
+}
+
+// 0 fp32, 1 bf16
+int dtype_of(const Tensor& t, const char* name) {
+    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(t.scalar_type() == torch::kFloat32 || t.scalar_type() == torch::kBFloat16, name,
+                " must be float32 or bfloat16");
+    return t.scalar_type() == torch::kBFloat16;
+}
+void check_like(const Tensor& t, const Tensor& as, const char* name) {
+    TORCH_CHECK(t.device() == as.device(), name, " must be on ", as.device());
+    TORCH_CHECK(t.scalar_type() == as.scalar_type(), name, " must have the type of the others");
+}
+void check_f32(const Tensor& t, const Tensor& as, const char* name) {
+    TORCH_CHECK(t.device() == as.device(), name, " must be on ", as.device());
+    TORCH_CHECK(t.scalar_type() == torch::kFloat32, name, " must be float32");
+}
+const int64_t* index_ptr(const Tensor& t, const Tensor& as, int64_t n, const char* name) {
+    TORCH_CHECK(t.device() == as.device(), name, " must be on ", as.device());
+    TORCH_CHECK(t.scalar_type() == torch::kInt64, name, " must be int64");
+    TORCH_CHECK(t.is_contiguous() && t.dim() == 1, name, " must be contiguous and 1D");
+    TORCH_CHECK(t.numel() == n, name, " must have ", n, " entries");
+    return t.data_ptr<int64_t>();
+}
+Tensor bytes_on(const Tensor& as, size_t n) {
+    return torch::empty({(int64_t)((n + 15) / 16 * 16)},
+                        torch::TensorOptions().dtype(torch::kUInt8).device(as.device()));
+}
+
+// ---------------------------------------------------------------------------
+// attention
+// ---------------------------------------------------------------------------
+
+// [n, heads, D] with dense heads, any stride of the rows
+Tensor dense_heads(const Tensor& t) {
+    if (t.size(0) <= 1 || t.numel() == 0) return t.contiguous();
+    if (t.stride(2) == 1 && (t.size(1) == 1 || t.stride(1) == t.size(2)) &&
+        t.stride(0) >= t.size(1) * t.size(2))
+        return t;
+    return t.contiguous();
+}
+
+struct AttnShape {
+    int dtype, H, Hkv, Dk, Dv;
+    int64_t n_dst, n_src, E;
+};
+
+AttnShape attn_shape(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias,
+                     int64_t E) {
+    AttnShape s;
+    s.dtype = dtype_of(q, "q");
+    TORCH_CHECK(q.dim() == 3, "q must be 3D [N_dst, H, Dk]");
+    TORCH_CHECK(k.dim() == 3, "k must be 3D [N_src, H_kv, Dk]");
+    TORCH_CHECK(v.dim() == 3, "v must be 3D [N_src, H_kv, Dv]");
+    check_like(k, q, "k");
+    check_like(v, q, "v");
+    s.n_dst = q.size(0), s.n_src = k.size(0), s.E = E;
+    TORCH_CHECK(v.size(0) == s.n_src, "k and v must have the same number of rows");
+    TORCH_CHECK(k.size(1) == v.size(1), "k and v must have the same number of heads");
+    TORCH_CHECK(q.size(1) > 0 && k.size(1) > 0 && q.size(1) % k.size(1) == 0,
+                "the heads of q must be a multiple of those of k and v");
+    TORCH_CHECK(q.size(2) == k.size(2), "q and k must have the same head size");
+    TORCH_CHECK(q.size(2) >= 1 && q.size(2) <= 256 && v.size(2) >= 1 && v.size(2) <= 256,
+                "head sizes must be in [1, 256]");
+    s.H = (int)q.size(1), s.Hkv = (int)k.size(1), s.Dk = (int)q.size(2), s.Dv = (int)v.size(2);
+    if (bias) {
+        check_f32(*bias, q, "bias");
+        TORCH_CHECK(bias->dim() == 2 && bias->size(0) == E && bias->size(1) == s.H,
+                    "bias must be [E, H]");
+    }
+    return s;
+}
+
+std::tuple<Tensor, Tensor> neighbor_attention(const Tensor& q_, const Tensor& k_, const Tensor& v_,
+                                              const OptTensor& bias_, const Tensor& row_ptr,
+                                              const Tensor& src, const OptTensor& eid,
+                                              double scale, bool keep_stats) {
+    const AttnShape s = attn_shape(q_, k_, v_, bias_, src.numel());
+    const c10::DeviceGuard guard(q_.device());
+    const Tensor q = dense_heads(q_), k = dense_heads(k_), v = dense_heads(v_);
+    Tensor bias;
+    if (bias_) bias = bias_->contiguous();
+    const int64_t* rp = index_ptr(row_ptr, q, s.n_dst + 1, "row_ptr");
+    const int64_t* col = index_ptr(src, q, s.E, "src");
+    const int64_t* ep = eid ? index_ptr(*eid, q, s.E, "edge_id") : nullptr;
+    Tensor out = torch::empty({s.n_dst, s.H, s.Dv}, q.options()), stats;
+    if (keep_stats) stats = torch::empty({s.n_dst, s.H, 2}, q.options().dtype(torch::kFloat32));
+    check_status(batteries_neighbor_attention(
+                     q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                     bias.defined() ? bias.data_ptr<float>() : nullptr, rp, col, ep,
+                     out.data_ptr(), keep_stats ? stats.data_ptr<float>() : nullptr, s.n_dst,
+                     s.n_src, s.E, s.H, s.Hkv, s.Dk, s.Dv, q.stride(0), k.stride(0), v.stride(0),
+                     (float)scale, s.dtype, stream_of(q)),
+                 "neighbor_attention");
+    return {out, stats};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> neighbor_attention_backward(
+    const Tensor& q_, const Tensor& k_, const Tensor& v_, const OptTensor& bias_,
+    const Tensor& stats, const Tensor& grad_, const Tensor& row_ptr, const Tensor& src,
+    const OptTensor& eid, const Tensor& src_ptr, const Tensor& src_dst, const Tensor& src_pos,
+    double scale, bool need_bias) {
+    const AttnShape s = attn_shape(q_, k_, v_, bias_, src.numel());
+    check_like(grad_, q_, "grad_out");
+    TORCH_CHECK(grad_.dim() == 3 && grad_.size(0) == s.n_dst && grad_.size(1) == s.H &&
+                    grad_.size(2) == s.Dv,
+                "grad_out must have the shape of the output");
+    check_f32(stats, q_, "stats");
+    TORCH_CHECK(stats.is_contiguous() && stats.numel() == s.n_dst * s.H * 2,
+                "stats must be [N_dst, H, 2]");
+    const c10::DeviceGuard guard(q_.device());
+    const Tensor q = dense_heads(q_), k = dense_heads(k_), v = dense_heads(v_),
+                 go = dense_heads(grad_);
+    Tensor bias, gbias;
+    if (bias_) bias = bias_->contiguous();
+    if (need_bias && bias_) gbias = torch::empty_like(bias);
+    const int64_t* rp = index_ptr(row_ptr, q, s.n_dst + 1, "row_ptr");
+    const int64_t* col = index_ptr(src, q, s.E, "src");
+    const int64_t* ep = eid ? index_ptr(*eid, q, s.E, "edge_id") : nullptr;
+    const int64_t* sp = index_ptr(src_ptr, q, s.n_src + 1, "src_ptr");
+    const int64_t* sd = index_ptr(src_dst, q, s.E, "src_dst");
+    const int64_t* ss = index_ptr(src_pos, q, s.E, "src_pos");
+    Tensor gq = torch::empty({s.n_dst, s.H, s.Dk}, q.options());
+    Tensor gk = torch::empty({s.n_src, s.Hkv, s.Dk}, q.options());
+    Tensor gv = torch::empty({s.n_src, s.Hkv, s.Dv}, q.options());
+    const size_t wsb = batteries_neighbor_attention_backward_workspace_bytes(s.E, s.H);
+    const Tensor ws = bytes_on(q, wsb);
+    check_status(
+        batteries_neighbor_attention_backward(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            bias.defined() ? bias.data_ptr<float>() : nullptr, stats.data_ptr<float>(),
+            go.data_ptr(), rp, col, ep, sp, sd, ss, gq.data_ptr(), gk.data_ptr(), gv.data_ptr(),
+            gbias.defined() ? gbias.data_ptr<float>() : nullptr, s.n_dst, s.n_src, s.E, s.H, s.Hkv,
+            s.Dk, s.Dv, q.stride(0), k.stride(0), v.stride(0), go.stride(0), (float)scale, s.dtype,
+            ws.data_ptr(), wsb, stream_of(q)),
+        "neighbor_attention_backward");
+    return {gq, gk, gv, gbias};
+}
+
+// ---------------------------------------------------------------------------
+// norms by degree
+// ---------------------------------------------------------------------------
+
+void check_features(const Tensor& x, const char* name) {
+    TORCH_CHECK(x.dim() == 3 && x.size(2) == 16, name, " must be 3D [N, C, 16]");
+    TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= 2048, name, " must have 1 to 2048 channels");
+}
+// contiguous and aligned for the kernels' 4-component loads
+Tensor rows4(const Tensor& t) {
+    const Tensor c = t.contiguous();
+    return reinterpret_cast<uintptr_t>(c.data_ptr()) & 15 ? c.clone(at::MemoryFormat::Contiguous)
+                                                          : c;
+}
+Tensor weight4(const Tensor& w, const Tensor& x, const char* name) {
+    check_f32(w, x, name);
+    TORCH_CHECK(w.dim() == 2 && w.size(0) == 4 && w.size(1) == x.size(1), name,
+                " must be [4, C]");
+    return w.contiguous();
+}
+void check_same(const Tensor& t, const Tensor& x, const char* name) {
+    check_like(t, x, name);
+    TORCH_CHECK(t.sizes() == x.sizes(), name, " must have the shape of x");
+}
+void* opt_ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+float* opt_f32(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+
+// (h, n, rs); y none: n = norm(x) alone, h undefined
+std::tuple<Tensor, Tensor, Tensor> gated_residual_norm(const Tensor& x_, const OptTensor& y_,
+                                                       const OptTensor& gate_,
+                                                       const OptTensor& scale_,
+                                                       const OptTensor& w_post_,
+                                                       const OptTensor& w_pre_, double eps,
+                                                       bool keep_stats) {
+    const int dt = dtype_of(x_, "x");
+    check_features(x_, "x");
+    TORCH_CHECK(y_ || w_pre_, "one of y and weight_pre is needed");
+    TORCH_CHECK(eps >= 0.0, "eps must not be negative");
+    const int64_t N = x_.size(0);
+    const int C = (int)x_.size(1);
+    const c10::DeviceGuard guard(x_.device());
+    const Tensor x = rows4(x_);
+    Tensor y, gate, scale, w_post, w_pre, h, n, rs;
+    if (y_) {
+        TORCH_CHECK(scale_ && w_post_, "y needs scale and weight_post");
+        check_same(*y_, x_, "y");
+        y = rows4(*y_);
+        check_f32(*scale_, x_, "scale");
+        TORCH_CHECK(scale_->dim() == 1 && scale_->size(0) == C, "scale must be [C]");
+        scale = scale_->contiguous();
+        w_post = weight4(*w_post_, x_, "weight_post");
+        if (gate_) {
+            check_like(*gate_, x_, "gate");
+            TORCH_CHECK(gate_->dim() == 3 && gate_->size(0) == N && gate_->size(1) == C &&
+                            gate_->size(2) == 4,
+                        "gate must be [N, C, 4]");
+            gate = gate_->contiguous();
+        }
+        h = torch::empty_like(x);
+    }
+    if (w_pre_) {
+        w_pre = weight4(*w_pre_, x_, "weight_pre");
+        n = torch::empty_like(x);
+    }
+    if (keep_stats) rs = torch::empty({N, 8}, x.options().dtype(torch::kFloat32));
+    // a tensor without elements has no address, which would read as "not given"
+    if (N > 0)
+        check_status(batteries_gated_residual_norm(x.data_ptr(), opt_ptr(y), opt_ptr(gate),
+                                                   opt_f32(scale), opt_f32(w_post),
+                                                   opt_f32(w_pre), opt_ptr(h), opt_ptr(n),
+                                                   opt_f32(rs), N, C, (float)eps, dt,
+                                                   stream_of(x)),
+                     "gated_residual_norm");
+    return {h, n, rs};
+}
+
+// (gx, gy, ggate, gscale, gw_post, gw_pre)
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> gated_residual_norm_backward(
+    const OptTensor& gh_, const OptTensor& gn_, const Tensor& h_, const OptTensor& y_,
+    const OptTensor& gate_, const OptTensor& scale_, const OptTensor& w_post_,
+    const OptTensor& w_pre_, const Tensor& rs) {
+    const int dt = dtype_of(h_, "h");
+    check_features(h_, "h");
+    const int64_t N = h_.size(0);
+    const int C = (int)h_.size(1);
+    TORCH_CHECK(y_ || w_pre_, "one of y and weight_pre is needed");
+    TORCH_CHECK(!w_pre_ || gn_, "weight_pre needs the gradient of n");
+    TORCH_CHECK(w_pre_ || gh_, "the gradient of h is needed");
+    check_f32(rs, h_, "rs");
+    TORCH_CHECK(rs.is_contiguous() && rs.numel() == N * 8, "rs must be [N, 8]");
+    const c10::DeviceGuard guard(h_.device());
+    const Tensor h = rows4(h_);
+    Tensor gh, gn, y, gate, scale, w_post, w_pre, gx, gy, ggate, gscale, gw_post, gw_pre;
+    gx = torch::empty_like(h);
+    if (gh_) check_same(*gh_, h_, "grad_h"), gh = rows4(*gh_);
+    if (w_pre_) {
+        check_same(*gn_, h_, "grad_n");
+        gn = rows4(*gn_);
+        w_pre = weight4(*w_pre_, h_, "weight_pre");
+        gw_pre = torch::empty_like(w_pre);
+    }
+    if (y_) {
+        TORCH_CHECK(scale_ && w_post_, "y needs scale and weight_post");
+        check_same(*y_, h_, "y");
+        y = rows4(*y_);
+        check_f32(*scale_, h_, "scale");
+        TORCH_CHECK(scale_->numel() == C, "scale must be [C]");
+        scale = scale_->contiguous();
+        w_post = weight4(*w_post_, h_, "weight_post");
+        gy = torch::empty_like(y);
+        gscale = torch::empty_like(scale);
+        gw_post = torch::empty_like(w_post);
+        if (gate_) {
+            check_like(*gate_, h_, "gate");
+            TORCH_CHECK(gate_->numel() == N * C * 4, "gate must be [N, C, 4]");
+            gate = gate_->contiguous();
+            ggate = torch::empty_like(gate);
+        }
+    }
+    if (N == 0) {
+        for (Tensor* t : {&gscale, &gw_post, &gw_pre})
+            if (t->defined()) t->zero_();
+        return {gx, gy, ggate, gscale, gw_post, gw_pre};
+    }
+    const size_t wsb = batteries_gated_residual_norm_backward_workspace_bytes(N, C);
+    const Tensor ws = bytes_on(h, wsb);
+    check_status(batteries_gated_residual_norm_backward(
+                     opt_ptr(gh), opt_ptr(gn), h.data_ptr(), opt_ptr(y), opt_ptr(gate),
+                     opt_f32(scale), opt_f32(w_post), opt_f32(w_pre), rs.data_ptr<float>(),
+                     gx.data_ptr(), opt_ptr(gy), opt_ptr(ggate), opt_f32(gscale),
+                     opt_f32(gw_post), opt_f32(gw_pre), N, C, dt, ws.data_ptr(), wsb,
+                     stream_of(h)),
+                 "gated_residual_norm_backward");
+    return {gx, gy, ggate, gscale, gw_post, gw_pre};
+}
+
+// ---------------------------------------------------------------------------
+// gradient clipping
+// ---------------------------------------------------------------------------
+
+// (norm, clipped): the norm as a tensor without dimensions; the clipped gradients in outs
+// (which may be the gradients) or in new tensors.  A strided view with gaps, or an out of
+// another layout than its gradient, goes through a dense copy.
+std::tuple<Tensor, std::vector<Tensor>> clip_grad_norm(
+    const std::vector<Tensor>& grads, double max_norm,
+    const c10::optional<std::vector<Tensor>>& outs) {
+    TORCH_CHECK(max_norm >= 0.0, "max_norm must not be negative");
+    TORCH_CHECK(!grads.empty(), "at least one tensor is needed");
+    TORCH_CHECK(!outs || outs->size() == grads.size(), "out must hold one tensor per gradient");
+    const torch::NoGradGuard no_grad;
+    const size_t n = grads.size();
+    std::vector<const void*> in(n);
+    std::vector<void*> out(n);
+    std::vector<int64_t> numel(n);
+    std::vector<int> dt(n);
+    std::vector<Tensor> dense(n), into(n);
+    TORCH_CHECK(grads[0].is_cuda(), "a gradient must be a CUDA tensor");
+    const c10::DeviceGuard guard(grads[0].device());
+    for (size_t i = 0; i < n; ++i) {
+        Tensor g = grads[i];
+        dt[i] = dtype_of(g, "a gradient");
+        TORCH_CHECK(g.device() == grads[0].device(), "the gradients must be on one device");
+        if (!g.is_non_overlapping_and_dense()) dense[i] = g = g.contiguous();
+        if (outs) {
+            const Tensor& o = (*outs)[i];
+            check_like(o, g, "out");
+            TORCH_CHECK(o.sizes() == g.sizes(), "out must have the shapes of the gradients");
+            if (o.strides() == g.strides()) into[i] = o;
+        }
+        if (!into[i].defined()) into[i] = torch::empty_like(g);
+        in[i] = g.data_ptr(), out[i] = into[i].data_ptr(), numel[i] = g.numel();
+    }
+    Tensor norm = torch::empty({}, grads[0].options().dtype(torch::kFloat32));
+    const size_t wsb = batteries_clip_grad_norm_workspace_bytes((int64_t)n);
+    const Tensor ws = bytes_on(grads[0], wsb);
+    check_status(batteries_clip_grad_norm(in.data(), out.data(), numel.data(), dt.data(),
+                                          (int64_t)n, (float)max_norm, norm.data_ptr<float>(),
+                                          ws.data_ptr(), wsb, stream_of(grads[0])),
+                 "clip_grad_norm");
+    if (!outs) return {norm, into};
+    for (size_t i = 0; i < n; ++i) {
+        Tensor o = (*outs)[i];
+        if (!o.is_same(into[i])) o.copy_(into[i]);
+    }
+    return {norm, *outs};
+}
+
+}  // namespace
+
+void register_block_ops(pybind11::module_& m) {
+    namespace py = pybind11;
+    m.def("neighbor_attention", &neighbor_attention, py::arg("q"), py::arg("k"), py::arg("v"),
+          py::arg("bias"), py::arg("row_ptr"), py::arg("src"), py::arg("edge_id"),
+          py::arg("scale"), py::arg("keep_stats") = false,
+          "softmax attention over the edges of each row -> (out, stats or None)");
+    m.def("neighbor_attention_backward", &neighbor_attention_backward, py::arg("q"), py::arg("k"),
+          py::arg("v"), py::arg("bias"), py::arg("stats"), py::arg("grad_out"),
+          py::arg("row_ptr"), py::arg("src"), py::arg("edge_id"), py::arg("src_ptr"),
+          py::arg("src_dst"), py::arg("src_pos"), py::arg("scale"), py::arg("need_bias") = true,
+          "(grad_q, grad_k, grad_v, grad_bias or None)");
+    m.def("gated_residual_norm", &gated_residual_norm, py::arg("x"), py::arg("y"),
+          py::arg("gate"), py::arg("scale"), py::arg("weight_post"), py::arg("weight_pre"),
+          py::arg("eps"), py::arg("keep_stats") = false,
+          "h = x + scale sigmoid(gate) norm(y), n = norm(h) -> (h, n, rs); y None: n = norm(x)");
+    m.def("gated_residual_norm_backward", &gated_residual_norm_backward, py::arg("grad_h"),
+          py::arg("grad_n"), py::arg("h"), py::arg("y"), py::arg("gate"), py::arg("scale"),
+          py::arg("weight_post"), py::arg("weight_pre"), py::arg("rs"),
+          "(grad_x, grad_y, grad_gate, grad_scale, grad_weight_post, grad_weight_pre)");
+    m.def("clip_grad_norm", &clip_grad_norm, py::arg("grads"), py::arg("max_norm"),
+          py::arg("out") = py::none(),
+          "(norm of all tensors together, the tensors scaled to max_norm)");
+}

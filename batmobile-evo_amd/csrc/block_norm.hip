@@ -1,0 +1,408 @@
+// Normalisation of node features [N, C, 16] by degree, alone and fused with the end of a block
+// (no reference counterpart).  Per row (atom) and degree l, components l^2 .. (l + 1)^2 - 1:
+//
+//   r_l(z) = (mean over channels and components of z^2 + eps)^-1/2
+//   norm(z; w)[c, lm] = w[l, c] r_l(z) z[c, lm]
+//   h = x + scale[c] sigmoid(gate[c, l]) norm(y; w_post)        (no gate: factor 1)
+//   n = norm(h; w_pre)
+//
+// which commutes with rotations: the factors are the same for all components of a degree.
+// Backward, with gh and gn the gradients of h and n, M_l = C (2 l + 1), f = scale sigmoid(gate):
+//
+//   V[c, l] = sum_m gn h                     gw_pre[l, c] = sum over atoms of r_l(h) V
+//   G = gh + r w_pre gn - h r^3 / M sum_c w_pre V          (gx = G)
+//   Z[c, l] = sum_m G y                      gw_post[l, c] = sum over atoms of f r_l(y) Z
+//   ggate = f (1 - sigmoid) w_post r_l(y) Z  gscale[c] = sum sigmoid w_post r_l(y) Z
+//   gy = r f w_post G - y r^3 / M sum_c f w_post Z
+//
+// Memory bound: each array is read or written once, a row lives in the registers of one wave
+// (up to 128 channels; 4 or 16 waves share a wider row).  A quad of lanes holds a channel, a
+// lane four of its components, so that every load and store is contiguous over the wave.  The
+// first of the four and the other three are each of one degree, and lane q of a quad does the
+// arithmetic per (channel, degree q): the quad's two partial sums per lane go to their degrees'
+// lanes, and the factors back, by quad permutes.
+#include "common.h"
+#include "batmobile_hip.h"
+
+namespace bmhip {
+
+constexpr int kNormMaxC = 2048;
+
+template <typename T>
+__device__ __forceinline__ float4 norm_ld4(const T* p);
+template <>
+__device__ __forceinline__ float4 norm_ld4<float>(const float* p) {
+    return *reinterpret_cast<const float4*>(p);
+}
+template <>
+__device__ __forceinline__ float4 norm_ld4<uint16_t>(const uint16_t* p) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    return make_float4(bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y));
+}
+__device__ __forceinline__ void norm_st4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+__device__ __forceinline__ void norm_st4(uint16_t* p, float4 v) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(bf16_pack(v.x, v.y), bf16_pack(v.z, v.w));
+}
+__device__ __forceinline__ float norm_ld(const float* p) { return *p; }
+__device__ __forceinline__ float norm_ld(const uint16_t* p) {
+    return __uint_as_float((uint32_t)*p << 16);
+}
+__device__ __forceinline__ void norm_st(float* p, float v) { *p = v; }
+__device__ __forceinline__ void norm_st(uint16_t* p, float v) {
+    *p = (uint16_t)(bf16_pack(v, 0.0f) & 0xffffu);
+}
+
+template <int S0, int S1, int S2, int S3>
+__device__ __forceinline__ float quad(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(
+        0, __float_as_int(v), S0 | (S1 << 2) | (S2 << 4) | (S3 << 6), 0xf, 0xf, true));
+}
+
+// Partial sums a (first component) and b (the other three) of the quad's lanes -> lane q: the
+// sum over the components of degree q (0 | 1..3 | 4..8 | 9..15 of the 16).
+__device__ __forceinline__ float to_degree(float a, float b, int q) {
+    const float ab = a + b, fb = quad<0, 0, 2, 2>(b), fab = quad<0, 0, 1, 0>(ab);
+    return q == 0 ? a : q == 1 ? fb : q == 2 ? fab + a : fb + ab;
+}
+// The factor of each lane's first and other components from the degrees' lanes.
+__device__ __forceinline__ float first_of(float f) { return quad<0, 2, 2, 3>(f); }
+__device__ __forceinline__ float others_of(float f) { return quad<1, 2, 3, 3>(f); }
+
+__device__ __forceinline__ float dot4(float4 a, float4 b, int q) {
+    return to_degree(a.x * b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, a.w * b.w)), q);
+}
+
+// Sum over the lanes of the same q, over the W waves of a row (every thread of the workgroup
+// takes part); the result in every lane of that q.  sh: two buffers used in turn.
+template <int W>
+__device__ __forceinline__ float row_sum(float v, float* sh, int& turn) {
+#pragma unroll
+    for (int o = 4; o < 64; o <<= 1) v += __shfl_xor(v, o);
+    if constexpr (W > 1) {
+        float* s = sh + turn * 4 * W;
+        turn ^= 1;
+        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+        if (lane < 4) s[w * 4 + lane] = v;
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) v += s[i * 4 + (lane & 3)];
+    }
+    return v;
+}
+
+struct NormArgs {
+    const void *x, *y, *gate, *gh, *gn, *h;
+    const float *scale, *w_post, *w_pre, *rs_in;
+    void *out_h, *out_n, *gx, *gy, *ggate;
+    float *rs, *part;                  // rs [N, 8]: 1/rms of y by degree, then of h
+    int64_t n;
+    int C;
+    float eps;
+};
+
+// Rows per workgroup: 4 (W = 1) or 1.  BLOCK: h = x + f norm(y) first; else h = x.
+template <typename T, int NV, int W, bool BLOCK, bool GATE, bool PRE>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_fwd_kernel(NormArgs a) {
+    __shared__ float sh[2 * 4 * W];
+    int turn = 0;
+    const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    if (row >= a.n) return;
+    const int t = W == 1 ? (threadIdx.x & 63) : threadIdx.x, q = t & 3;
+    const int64_t at = row * (int64_t)a.C * 16;
+    const float cnt = 1.0f / ((float)a.C * (float)(2 * q + 1));
+    float4 h[NV], y[NV];
+    float f[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * 64 * W + t) >> 2;
+        const bool in = c < a.C;
+        const int64_t o = at + (int64_t)(i * 64 * W + t) * 4;
+        h[i] = in ? norm_ld4((const T*)a.x + o) : make_float4(0, 0, 0, 0);
+        if constexpr (BLOCK) {
+            y[i] = in ? norm_ld4((const T*)a.y + o) : make_float4(0, 0, 0, 0);
+            f[i] = in ? a.scale[c] * a.w_post[q * a.C + c] : 0.0f;
+            if constexpr (GATE)
+                if (in) f[i] /= 1.0f + __expf(-norm_ld((const T*)a.gate + row * a.C * 4 +
+                                                        i * 64 * W + t));
+        }
+    }
+    if constexpr (BLOCK) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) s += dot4(y[i], y[i], q);
+        const float r = 1.0f / sqrtf(fmaf(row_sum<W>(s, sh, turn), cnt, a.eps));
+        if (a.rs && t < 4) a.rs[row * 8 + t] = r;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const float fa = first_of(f[i] * r), fb = others_of(f[i] * r);
+            h[i] = make_float4(fmaf(fa, y[i].x, h[i].x), fmaf(fb, y[i].y, h[i].y),
+                               fmaf(fb, y[i].z, h[i].z), fmaf(fb, y[i].w, h[i].w));
+            if (((i * 64 * W + t) >> 2) < a.C)
+                norm_st4((T*)a.out_h + at + (int64_t)(i * 64 * W + t) * 4, h[i]);
+        }
+    }
+    if constexpr (PRE) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) s += dot4(h[i], h[i], q);
+        const float r = 1.0f / sqrtf(fmaf(row_sum<W>(s, sh, turn), cnt, a.eps));
+        if (a.rs && t < 4) a.rs[row * 8 + 4 + t] = r;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * 64 * W + t) >> 2;
+            const float w = c < a.C ? a.w_pre[q * a.C + c] * r : 0.0f;
+            const float fa = first_of(w), fb = others_of(w);
+            if (c < a.C)
+                norm_st4((T*)a.out_n + at + (int64_t)(i * 64 * W + t) * 4,
+                         make_float4(fa * h[i].x, fb * h[i].y, fb * h[i].z, fb * h[i].w));
+        }
+    }
+}
+
+// Every workgroup takes rows blockIdx.x, + gridDim.x, ... (4 at a time for W = 1) and keeps its
+// share of the weights' gradients in registers: part [gridDim.x, 9 C] (pre [4][C], post [4][C],
+// scale [C]), summed by norm_weights_kernel in workgroup order.
+template <typename T, int NV, int W, bool BLOCK, bool GATE, bool PRE>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_bwd_kernel(NormArgs a) {
+    __shared__ float sh[2 * 4 * W];
+    __shared__ float red[W == 1 ? 4 * 64 : 1];
+    int turn = 0;
+    const int wave = threadIdx.x >> 6;
+    const int t = W == 1 ? (threadIdx.x & 63) : threadIdx.x, q = t & 3;
+    const float cnt = 1.0f / ((float)a.C * (float)(2 * q + 1));
+    float aw_pre[NV], aw_post[NV], a_scale[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) aw_pre[i] = aw_post[i] = a_scale[i] = 0.0f;
+    for (int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x; row < a.n;
+         row += W == 1 ? gridDim.x * 4 : gridDim.x) {
+        const int64_t at = row * (int64_t)a.C * 16;
+        float4 G[NV], h[NV], gn[NV];
+        float wp[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * 64 * W + t) >> 2;
+            const bool in = c < a.C;
+            const int64_t o = at + (int64_t)(i * 64 * W + t) * 4;
+            G[i] = h[i] = gn[i] = make_float4(0, 0, 0, 0);
+            wp[i] = 0.0f;
+            if (in) {
+                if (a.gh) G[i] = norm_ld4((const T*)a.gh + o);
+                if constexpr (PRE) {
+                    h[i] = norm_ld4((const T*)a.h + o);
+                    gn[i] = norm_ld4((const T*)a.gn + o);
+                    wp[i] = a.w_pre[q * a.C + c];
+                }
+            }
+        }
+        if constexpr (PRE) {
+            const float r = a.rs_in[row * 8 + 4 + q];
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const float v = dot4(gn[i], h[i], q);
+                aw_pre[i] = fmaf(r, v, aw_pre[i]);
+                s = fmaf(wp[i], v, s);
+            }
+            const float k = -row_sum<W>(s, sh, turn) * cnt * r * r * r;
+            const float ka = first_of(k), kb = others_of(k);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const float fa = first_of(wp[i] * r), fb = others_of(wp[i] * r);
+                G[i].x += fmaf(fa, gn[i].x, ka * h[i].x);
+                G[i].y += fmaf(fb, gn[i].y, kb * h[i].y);
+                G[i].z += fmaf(fb, gn[i].z, kb * h[i].z);
+                G[i].w += fmaf(fb, gn[i].w, kb * h[i].w);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (((i * 64 * W + t) >> 2) < a.C)
+                norm_st4((T*)a.gx + at + (int64_t)(i * 64 * W + t) * 4, G[i]);
+        if constexpr (BLOCK) {
+            const float r = a.rs_in[row * 8 + q];
+            float s = 0.0f, f[NV];
+            float4 y[NV];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (i * 64 * W + t) >> 2;
+                f[i] = 0.0f;
+                y[i] = make_float4(0, 0, 0, 0);
+                float sg = 1.0f, sc = 0.0f, w = 0.0f;
+                if (c < a.C) {
+                    y[i] = norm_ld4((const T*)a.y + at + (int64_t)(i * 64 * W + t) * 4);
+                    if constexpr (GATE)
+                        sg = 1.0f / (1.0f + __expf(-norm_ld((const T*)a.gate + row * a.C * 4 +
+                                                            i * 64 * W + t)));
+                    sc = a.scale[c];
+                    w = a.w_post[q * a.C + c];
+                }
+                const float z = dot4(G[i], y[i], q), rz = r * z;
+                f[i] = sc * sg * w;
+                s = fmaf(f[i], z, s);
+                aw_post[i] = fmaf(sc * sg, rz, aw_post[i]);
+                a_scale[i] = fmaf(sg * w, rz, a_scale[i]);
+                if constexpr (GATE)
+                    if (c < a.C)
+                        norm_st((T*)a.ggate + row * a.C * 4 + i * 64 * W + t,
+                                f[i] * (1.0f - sg) * rz);
+            }
+            const float k = -row_sum<W>(s, sh, turn) * cnt * r * r * r;
+            const float ka = first_of(k), kb = others_of(k);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const float fa = first_of(f[i] * r), fb = others_of(f[i] * r);
+                if (((i * 64 * W + t) >> 2) < a.C)
+                    norm_st4((T*)a.gy + at + (int64_t)(i * 64 * W + t) * 4,
+                             make_float4(fmaf(fa, G[i].x, ka * y[i].x),
+                                         fmaf(fb, G[i].y, kb * y[i].y),
+                                         fmaf(fb, G[i].z, kb * y[i].z),
+                                         fmaf(fb, G[i].w, kb * y[i].w)));
+            }
+        }
+    }
+    float* part = a.part + (int64_t)blockIdx.x * 9 * a.C;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            float v = k == 0 ? aw_pre[i] : k == 1 ? aw_post[i] : a_scale[i];
+            if (k == 0 && !PRE) continue;
+            if (k > 0 && !BLOCK) continue;
+            if (k == 2) v = v + quad<1, 0, 3, 2>(v), v = v + quad<2, 3, 0, 1>(v);
+            if constexpr (W == 1) {
+                __syncthreads();
+                red[wave * 64 + t] = v;
+                __syncthreads();
+                v = red[t] + red[64 + t] + red[128 + t] + red[192 + t];
+                if (wave != 0) continue;
+            }
+            const int c = (i * 64 * W + t) >> 2;
+            if (c >= a.C) continue;
+            if (k < 2) part[(k * 4 + q) * a.C + c] = v;
+            else if (q == 0) part[8 * a.C + c] = v;
+        }
+    }
+}
+
+// Column sums of part [rows, 9 C] over the workgroups' rows, in order: 16 columns a workgroup,
+// 16 threads a column, each over a contiguous run of the rows.
+__global__ __launch_bounds__(256) void norm_weights_kernel(const float* __restrict__ part,
+                                                           int rows, int C, float* gw_pre,
+                                                           float* gw_post, float* gscale) {
+    __shared__ float sh[16][17];
+    const int col = blockIdx.x * 16 + (threadIdx.x & 15), k = threadIdx.x >> 4;
+    const int per = (rows + 15) / 16;
+    float s = 0.0f;
+    const bool want = col < 9 * C && (col < 4 * C ? gw_pre != nullptr
+                                                  : col < 8 * C ? gw_post != nullptr
+                                                                : gscale != nullptr);
+    if (want)
+        for (int r = k * per; r < min(rows, (k + 1) * per); ++r) s += part[(int64_t)r * 9 * C + col];
+    sh[k][threadIdx.x & 15] = s;
+    __syncthreads();
+    if (k == 0 && want) {
+        s = 0.0f;
+        for (int i = 0; i < 16; ++i) s += sh[i][threadIdx.x];
+        if (col < 4 * C) gw_pre[col] = s;
+        else if (col < 8 * C) gw_post[col - 4 * C] = s;
+        else gscale[col - 8 * C] = s;
+    }
+}
+
+static int norm_bwd_blocks(int64_t n, int C) {
+    return (int)std::min<int64_t>(C <= 128 ? ceil_div(n, 4) : n, C <= 512 ? 1024 : 512);
+}
+
+template <typename T, int NV, int W, bool BLOCK, bool GATE, bool PRE>
+static void norm_launch(const NormArgs& a, bool bwd, hipStream_t s) {
+    const int threads = W == 1 ? 256 : 64 * W;
+    if (bwd)
+        norm_bwd_kernel<T, NV, W, BLOCK, GATE, PRE>
+            <<<norm_bwd_blocks(a.n, a.C), threads, 0, s>>>(a);
+    else
+        norm_fwd_kernel<T, NV, W, BLOCK, GATE, PRE>
+            <<<(unsigned)(W == 1 ? ceil_div(a.n, 4) : a.n), threads, 0, s>>>(a);
+}
+
+template <typename T, bool BLOCK, bool GATE, bool PRE>
+static void norm_pick(const NormArgs& a, bool bwd, hipStream_t s) {
+    if (a.C <= 16) norm_launch<T, 1, 1, BLOCK, GATE, PRE>(a, bwd, s);
+    else if (a.C <= 32) norm_launch<T, 2, 1, BLOCK, GATE, PRE>(a, bwd, s);
+    else if (a.C <= 64) norm_launch<T, 4, 1, BLOCK, GATE, PRE>(a, bwd, s);
+    else if (a.C <= 128) norm_launch<T, 8, 1, BLOCK, GATE, PRE>(a, bwd, s);
+    else if (a.C <= 512) norm_launch<T, 8, 4, BLOCK, GATE, PRE>(a, bwd, s);
+    else norm_launch<T, 8, 16, BLOCK, GATE, PRE>(a, bwd, s);
+}
+
+template <typename T>
+static void norm_run(const NormArgs& a, bool block, bool pre, bool bwd, hipStream_t s) {
+    if (!block) norm_pick<T, false, false, true>(a, bwd, s);
+    else if (a.gate && pre) norm_pick<T, true, true, true>(a, bwd, s);
+    else if (a.gate) norm_pick<T, true, true, false>(a, bwd, s);
+    else if (pre) norm_pick<T, true, false, true>(a, bwd, s);
+    else norm_pick<T, true, false, false>(a, bwd, s);
+}
+
+static bool norm_shape_ok(int64_t n, int C, int dtype) {
+    return n >= 0 && C > 0 && C <= kNormMaxC && (dtype == 0 || dtype == 1) &&
+           n < ((int64_t)1 << 31);
+}
+static bool aligned_to(std::initializer_list<const void*> ps, uintptr_t b) {
+    for (const void* p : ps)
+        if (reinterpret_cast<uintptr_t>(p) & (b - 1)) return false;
+    return true;
+}
+
+}  // namespace bmhip
+
+using namespace bmhip;
+
+extern "C" int batteries_gated_residual_norm(const void* x, const void* y, const void* gate,
+                                             const float* scale, const float* w_post,
+                                             const float* w_pre, void* h, void* n, float* rs,
+                                             int64_t N, int C, float eps, int dtype,
+                                             hipStream_t stream) {
+    if (!norm_shape_ok(N, C, dtype) || (!y && !w_pre) || (y && (!scale || !w_post || !h)) ||
+        (w_pre && !n))
+        return BM_ERR_ARG;
+    if (!aligned_to({x, y, h, n}, dtype == 0 ? 16 : 8)) return BM_ERR_ARG;
+    if (N == 0) return BM_OK;
+    NormArgs a{};
+    a.x = x; a.y = y; a.gate = gate; a.scale = scale; a.w_post = w_post; a.w_pre = w_pre;
+    a.out_h = h; a.out_n = n; a.rs = rs; a.n = N; a.C = C; a.eps = eps;
+    if (dtype == 0) norm_run<float>(a, y != nullptr, w_pre != nullptr, false, stream);
+    else norm_run<uint16_t>(a, y != nullptr, w_pre != nullptr, false, stream);
+    return (int)hipGetLastError();
+}
+
+extern "C" size_t batteries_gated_residual_norm_backward_workspace_bytes(int64_t N, int C) {
+    if (!norm_shape_ok(N, C, 0)) return 0;
+    return (size_t)norm_bwd_blocks(N, C) * 9 * (size_t)C * sizeof(float);
+}
+
+extern "C" int batteries_gated_residual_norm_backward(
+    const void* gh, const void* gn, const void* h, const void* y, const void* gate,
+    const float* scale, const float* w_post, const float* w_pre, const float* rs, void* gx,
+    void* gy, void* ggate, float* gscale, float* gw_post, float* gw_pre, int64_t N, int C,
+    int dtype, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    if (!norm_shape_ok(N, C, dtype) || (!y && !w_pre) || !gx ||
+        (y && (!scale || !w_post || !gy || !gscale || !gw_post)) || (gate && !ggate) ||
+        (w_pre && (!gn || !h || !gw_pre)) || (!w_pre && !gh))
+        return BM_ERR_ARG;
+    if (!aligned_to({gh, gn, h, y, gx, gy}, dtype == 0 ? 16 : 8)) return BM_ERR_ARG;
+    const size_t need = batteries_gated_residual_norm_backward_workspace_bytes(N, C);
+    if (workspace_bytes < need || (need && !workspace)) return BM_ERR_WORKSPACE;
+    NormArgs a{};
+    a.gh = gh; a.gn = gn; a.h = h; a.y = y; a.gate = gate; a.scale = scale; a.w_post = w_post;
+    a.w_pre = w_pre; a.rs_in = rs; a.gx = gx; a.gy = gy; a.ggate = ggate;
+    a.part = (float*)workspace; a.n = N; a.C = C;
+    if (N > 0) {
+        if (dtype == 0) norm_run<float>(a, y != nullptr, w_pre != nullptr, true, stream);
+        else norm_run<uint16_t>(a, y != nullptr, w_pre != nullptr, true, stream);
+    }
+    norm_weights_kernel<<<(unsigned)ceil_div(9 * (int64_t)C, 16), 256, 0, stream>>>(
+        a.part, N > 0 ? norm_bwd_blocks(N, C) : 0, C, w_pre ? gw_pre : nullptr,
+        y ? gw_post : nullptr, y ? gscale : nullptr);
+    return (int)hipGetLastError();
+}

@@ -61,6 +61,10 @@ from _batteries import (  # noqa: E402
 )
 from .graph import Graph  # noqa: E402
 from .mace import MACEInteraction, MaceLayerFunction  # noqa: E402
+from .attention import AttentionPlan, NeighborAttentionFunction, neighbor_attention  # noqa: E402
+from .block_norm import (  # noqa: E402
+    GatedResidualNormFunction, equivariant_norm, gated_residual_norm)
+from .grad_clip import clip_grad_norm, clip_grad_norm_  # noqa: E402
 
 # Autograd-compatible wrappers (reference __init__.py:35-44)
 from .autograd import (  # noqa: E402
@@ -112,4 +116,12 @@ __all__ = [
     "mace_backward",
     "MACEInteraction",
     "MaceLayerFunction",
+    "AttentionPlan",
+    "NeighborAttentionFunction",
+    "neighbor_attention",
+    "GatedResidualNormFunction",
+    "equivariant_norm",
+    "gated_residual_norm",
+    "clip_grad_norm",
+    "clip_grad_norm_",
 ]

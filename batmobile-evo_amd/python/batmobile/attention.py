@@ -1,0 +1,123 @@
+"""Softmax attention over the edges of a graph, with gradients.
+
+Not a reference API (the reference sums its messages).  For every destination i and head h,
+over the edges e: j -> i of the graph,
+
+    x_eh = scale <q[i, h], k[j, g]> + bias[e, h],  p = softmax over the row,
+    out[i, h] = sum_e p_eh v[j, g],                g = h // (H / H_kv)
+
+Equivariant features [N, C, 16] go in as heads of C / H channels, `x.view(N, H, C // H * 16)`:
+the product over a channel's 16 components does not change under rotations.
+"""
+import math
+
+import torch
+
+import _batmobile
+
+
+class AttentionPlan:
+    """The edges of a graph as the attention kernels take them, made once per graph.
+
+    src [E] int64 are the sources in the order of row_ptr [n_dst + 1] (edges grouped by
+    destination), ascending within a row.  order and src_order (permutations of the
+    destinations and of the sources; spatially near ones next to each other) only change the
+    speed.  from_edge_index takes edges in any order; bias rows are always in the caller's
+    order of the edges.  The arguments are checked on the GPU, which waits for it once.
+    """
+
+    def __init__(self, src, row_ptr, n_src=None, order=None, src_order=None, edge_id=None,
+                 validate=True):
+        self.src, self.row_ptr, self.edge_id = src, row_ptr, edge_id
+        self.order, self.src_order = order, src_order
+        self.n_dst = row_ptr.numel() - 1
+        self.n_src = self.n_dst if n_src is None else int(n_src)
+        self._source_side = None
+        if validate:
+            self._validate()
+
+    def _validate(self):
+        for name in ("src", "row_ptr", "edge_id", "order", "src_order"):
+            t = getattr(self, name)
+            if t is None and name not in ("src", "row_ptr"):
+                continue
+            if t.dtype != torch.int64 or t.dim() != 1 or not t.is_contiguous():
+                raise ValueError(f"AttentionPlan: {name} must be a contiguous int64 vector")
+            if t.device != self.src.device:
+                raise ValueError(f"AttentionPlan: {name} must be on the device of src")
+        e = self.src.numel()
+        step = self.row_ptr.diff()
+        ok = (step >= 0).all() & (self.row_ptr[0] == 0) & (self.row_ptr[-1] == e)
+        if e:
+            ok &= (self.src.min() >= 0) & (self.src.max() < self.n_src)
+        if not bool(ok):
+            raise ValueError("AttentionPlan: row_ptr must rise from 0 to E and src lie in "
+                             f"[0, {self.n_src})")
+        if e > 1:
+            first = torch.zeros(e + 1, dtype=torch.bool, device=self.src.device)
+            first[self.row_ptr] = True
+            if bool(((self.src[1:] < self.src[:-1]) & ~first[1:-1]).any()):
+                raise ValueError("AttentionPlan: src must ascend within a row (from_edge_index "
+                                 "takes edges in any order)")
+
+    @classmethod
+    def from_edge_index(cls, edge_index, n_dst, n_src=None, order=None, src_order=None):
+        """edge_index [2, E] (sources, destinations) in any order."""
+        if edge_index.dim() != 2 or edge_index.shape[0] != 2:
+            raise ValueError("AttentionPlan: edge_index must be [2, E]")
+        n_src = n_dst if n_src is None else n_src
+        src, dst = edge_index[0], edge_index[1]
+        if dst.numel() and not bool(((dst >= 0) & (dst < n_dst)).all()):
+            raise ValueError(f"AttentionPlan: destinations must lie in [0, {n_dst})")
+        edge_id = torch.argsort(dst * n_src + src, stable=True)
+        rows = torch.arange(n_dst + 1, device=dst.device)
+        row_ptr = torch.searchsorted(dst[edge_id], rows)
+        return cls(src[edge_id], row_ptr, n_src, order, src_order, edge_id)
+
+    def source_side(self):
+        """The edges grouped by source (for the backward; built on first use)."""
+        if self._source_side is None:
+            dst = torch.repeat_interleave(
+                torch.arange(self.n_dst, device=self.src.device), self.row_ptr.diff(),
+                output_size=self.src.numel())
+            by, pos = torch.sort(self.src, stable=True)
+            rows = torch.arange(self.n_src + 1, device=self.src.device)
+            self._source_side = (torch.searchsorted(by, rows), dst[pos], pos)
+        return self._source_side
+
+
+class NeighborAttentionFunction(torch.autograd.Function):
+    """out = attention(q, k, v, bias); the backward recomputes the probabilities."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, bias, plan, scale):
+        train = any(ctx.needs_input_grad[:4])
+        out, stats = _batmobile.neighbor_attention(q, k, v, bias, plan.row_ptr, plan.src,
+                                                   plan.edge_id, scale, train)
+        ctx.save_for_backward(q, k, v, bias, stats)
+        ctx.plan, ctx.scale = plan, scale
+        return out
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        q, k, v, bias, stats = ctx.saved_tensors
+        plan = ctx.plan
+        gq, gk, gv, gb = _batmobile.neighbor_attention_backward(
+            q, k, v, bias, stats, grad_out, plan.row_ptr, plan.src, plan.edge_id,
+            *plan.source_side(), ctx.scale, ctx.needs_input_grad[3])
+        return gq, gk, gv, gb, None, None
+
+
+def neighbor_attention(q, k, v, plan, bias=None, scale=None):
+    """Attention of each destination over its edges: out [n_dst, H, Dv].
+
+    q [n_dst, H, Dk], k [n_src, H_kv, Dk], v [n_src, H_kv, Dv] in float32 or bfloat16 (sums and
+    softmax in float32), H a multiple of H_kv, Dk and Dv up to 256; rows may be strided (slices
+    of one projection).  bias [E, H] float32: an edge with -inf is left out.  A row without an
+    edge gives zeros.  scale defaults to 1 / sqrt(Dk).  Gradients for q, k, v and bias.
+    """
+    if q.dim() == 3 and (q.shape[0] != plan.n_dst or k.shape[0] != plan.n_src):
+        raise RuntimeError(f"neighbor_attention: the plan has {plan.n_dst} destinations and "
+                           f"{plan.n_src} sources")
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
+    return NeighborAttentionFunction.apply(q, k, v, bias, plan, scale)

@@ -1,0 +1,24 @@
+"""Global norm of gradients and clipping, over many tensors in two kernels.
+
+Not a reference API.  norm = sqrt(sum over all tensors of g^2), summed in 64 bits; the
+gradients become g * min(1, max_norm / (norm + 1e-6)).  Nothing waits for the GPU: the norm is
+returned as a tensor.  float32 and bfloat16 tensors may be mixed.
+"""
+import torch
+
+import _batmobile
+
+
+def clip_grad_norm(grads, max_norm, out=None):
+    """(norm, clipped): the clipped gradients in `out` (a list like grads; None: new tensors)."""
+    return _batmobile.clip_grad_norm(grads, max_norm, out)
+
+
+def clip_grad_norm_(parameters, max_norm):
+    """Clips the gradients of `parameters` in place; returns their norm before clipping."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.zeros(())
+    return clip_grad_norm(grads, max_norm, grads)[0]

@@ -36,6 +36,8 @@ import torch
 
 import _batmobile
 
+from .attention import AttentionPlan
+
 
 class Graph:
     def __init__(self, positions, cell, cutoff, channels, self_loops=False, max_edges=None,
@@ -46,6 +48,7 @@ class Graph:
         self._rev = None
         self._fine_order = None
         self._order_w = None
+        self._attention = None
         self.n_atoms = positions.shape[0]
         self.channels = int(channels)
         cap = -1 if max_edges is None else int(max_edges)
@@ -133,6 +136,15 @@ class Graph:
             self.exact()
             self._rev = _batmobile.mace_reverse_edges(self.row_ptr, self.src)
         return self._rev
+
+    def attention_plan(self):
+        """The graph's edges for neighbor_attention, atoms in Morton order (built once)."""
+        if self._attention is None:
+            self.exact()
+            order = self.fine_order()
+            self._attention = AttentionPlan(self.src, self.row_ptr, self.n_atoms, order, order,
+                                            validate=False)
+        return self._attention
 
     def sh_tp_scatter(self, node_features, normalize=True, weights=None):
         """out[d] = sum_{e -> d} TP_simple(X[src_e], Y_lm(v_e)); one kernel, spatial schedule.

@@ -491,6 +491,74 @@ int batteries_mace_backward(const float* positions, const float* box, const floa
                             size_t workspace_bytes, hipStream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Softmax attention over the edges of a graph (no reference counterpart)
+ *
+ * Rows are destinations with their edges in row_ptr [n_dst + 1] order; col[e] is the source
+ * (ascending within a row) and eid[e] (NULL: e) the row of `bias` and `grad_bias` of edge e.
+ *   x_eh = scale <q[i,h], k[col e, h / (H / Hkv)]> + bias[eid e, h],   p = softmax over the row
+ *   out[i,h] = sum_e p_eh v[col e, h / (H / Hkv)]
+ * q [n_dst, H, Dk], k [n_src, Hkv, Dk], v [n_src, Hkv, Dv], out [n_dst, H, Dv] in fp32
+ * (dtype 0) or bf16 (dtype 1), the strides of their rows in elements; bias [E, H] fp32 or
+ * NULL.  An edge whose bias or logit is -inf is left out; a row without an edge gives 0.
+ * stats [n_dst, H, 2] (NULL: not kept): the maximum of x and the sum of exp(x - max), which
+ * the backward recomputes the probabilities from.  Dk, Dv <= 256.
+ * ------------------------------------------------------------------------- */
+int batteries_neighbor_attention(const void* q, const void* k, const void* v, const float* bias,
+                                 const int64_t* row_ptr, const int64_t* col, const int64_t* eid,
+                                 void* out, float* stats, int64_t n_dst, int64_t n_src,
+                                 int64_t n_edges, int H, int Hkv, int Dk, int Dv,
+                                 int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                 float scale, int dtype, hipStream_t stream);
+
+/* Gradients of the above: grad_q, grad_k, grad_v contiguous, grad_bias [E, H] or NULL.
+ * src_ptr [n_src + 1], src_dst [E], src_pos [E]: the edges grouped by source, destinations
+ * ascending, with each edge's position in the destinations' order. */
+size_t batteries_neighbor_attention_backward_workspace_bytes(int64_t n_edges, int H);
+int batteries_neighbor_attention_backward(
+    const void* q, const void* k, const void* v, const float* bias, const float* stats,
+    const void* grad_out, const int64_t* row_ptr, const int64_t* col, const int64_t* eid,
+    const int64_t* src_ptr, const int64_t* src_dst, const int64_t* src_pos, void* grad_q,
+    void* grad_k, void* grad_v, float* grad_bias, int64_t n_dst, int64_t n_src, int64_t n_edges,
+    int H, int Hkv, int Dk, int Dv, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+    int64_t go_stride, float scale, int dtype, void* workspace, size_t workspace_bytes,
+    hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Norms by degree of features [N, C, 16] (no reference counterpart)
+ *
+ * norm(z; w)[c, lm] = w[l, c] z[c, lm] / sqrt(mean over channels and the degree's components
+ * of z^2 + eps), w [4, C].
+ *   h = x + scale[c] sigmoid(gate[c, l]) norm(y; w_post),   n = norm(h; w_pre)
+ * y NULL: n = norm(x; w_pre) alone; gate NULL: factor 1; w_pre NULL: no n.  x, y, h, n
+ * [N, C, 16] and gate [N, C, 4] in fp32 (dtype 0; x, y, h, n 16-byte aligned) or bf16
+ * (dtype 1; 8-byte), the weights fp32.  rs [N, 8] (NULL: not kept) takes 1 / sqrt(...) of y
+ * and of h by degree, for the backward.  C <= 2048.
+ * ------------------------------------------------------------------------- */
+int batteries_gated_residual_norm(const void* x, const void* y, const void* gate,
+                                  const float* scale, const float* w_post, const float* w_pre,
+                                  void* h, void* n, float* rs, int64_t N, int C, float eps,
+                                  int dtype, hipStream_t stream);
+/* Gradients from gh (NULL: zero) and gn; h is the forward's h (x where y was NULL). */
+size_t batteries_gated_residual_norm_backward_workspace_bytes(int64_t N, int C);
+int batteries_gated_residual_norm_backward(
+    const void* gh, const void* gn, const void* h, const void* y, const void* gate,
+    const float* scale, const float* w_post, const float* w_pre, const float* rs, void* gx,
+    void* gy, void* ggate, float* gscale, float* gw_post, float* gw_pre, int64_t N, int C,
+    int dtype, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Global gradient norm and clipping (no reference counterpart)
+ *
+ * norm[0] = sqrt(sum over all tensors of g^2), out = g min(1, max_norm / (norm + 1e-6)).
+ * in, out (out[i] may be in[i]), numel and dtype (0 fp32, 1 bf16) are host arrays of
+ * n_tensors; the tensors are dense and aligned to their element.
+ * ------------------------------------------------------------------------- */
+size_t batteries_clip_grad_norm_workspace_bytes(int64_t n_tensors);
+int batteries_clip_grad_norm(const void* const* in, void* const* out, const int64_t* numel,
+                             const int* dtype, int64_t n_tensors, float max_norm, float* norm,
+                             void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Self test (no reference counterpart): D[16,16] = A[16,4] B[4,16] through one
  * v_mfma_f32_16x16x4f32 with the lane layout the kernels above assume.
  * ------------------------------------------------------------------------- */

@@ -1,0 +1,343 @@
+"""Attention over the edges of a graph on the GPU against the float64 oracle.
+
+Bounds (normwise, max|got - want| / max|want|).  fp32: a logit is a sum of up to 256 products,
+its error a few 2^-24 sqrt(256) = 1e-6 of its size (about 1), which the exponential passes on to
+the probabilities; outputs and gradients stay within 1e-5.  bf16: the results are rounded to 8
+bits (2^-9 = 2e-3 of the largest), the probabilities and their gradients possibly too before
+they meet the rows, whose weighted sum of absolute values is at most 3 times the largest result
+for these inputs: 8e-3.  The bias gradient is fp32 in either case: 1e-5.
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import block as ob
+
+from helpers import gen, normwise_err, periodic_box
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+BOUND = {"f32": 1e-5, "bf16": 8e-3}
+
+
+def _edges(degrees, m, seed, distinct=True):
+    """src ascending within rows of the given degrees, row_ptr."""
+    rng = np.random.default_rng(seed)
+    src = [np.sort(rng.permutation(m)[:d] if distinct else rng.integers(0, m, d)) for d in degrees]
+    row_ptr = np.concatenate([[0], np.cumsum(degrees)]).astype(np.int64)
+    return np.concatenate(src + [np.zeros(0)]).astype(np.int64), row_ptr
+
+
+def _inputs(n, m, e, h, kv, dk, dv, dtype, seed, bias=True):
+    g = gen(seed)
+    t = TYPES[dtype]
+    return {"q": torch.randn(n, h, dk, generator=g).to(t),
+            "k": torch.randn(m, kv, dk, generator=g).to(t),
+            "v": torch.randn(m, kv, dv, generator=g).to(t),
+            "bias": torch.randn(e, h, generator=g) if bias else None,
+            "go": torch.randn(n, h, dv, generator=g).to(t)}
+
+
+def _np(t):
+    return None if t is None else t.detach().cpu().double().numpy()
+
+
+def _run(dev, plan, t, scale=None):
+    """(out, grads) through autograd."""
+    import batmobile
+    leaf = {x: t[x].to(dev).requires_grad_(True) for x in ("q", "k", "v", "bias")
+            if t[x] is not None}
+    out = batmobile.neighbor_attention(leaf["q"], leaf["k"], leaf["v"], plan,
+                                       bias=leaf.get("bias"), scale=scale)
+    grads = torch.autograd.grad(out, list(leaf.values()), t["go"].to(dev))
+    torch.cuda.synchronize()
+    return out, dict(zip(leaf, grads))
+
+
+def _compare(out, grads, want, wgrads, dtype, what=""):
+    assert normwise_err(_np(out), want) <= BOUND[dtype], what
+    for name, got in grads.items():
+        bound = BOUND["f32" if name == "bias" else dtype]
+        assert normwise_err(_np(got), wgrads[name]) <= bound, (what, name)
+
+
+def _check(dev, src, row_ptr, m, t, dtype, order=None, src_order=None, scale=None):
+    import batmobile
+    plan = batmobile.AttentionPlan(torch.from_numpy(src).to(dev), torch.from_numpy(row_ptr).to(dev),
+                                   m, order, src_order)
+    out, grads = _run(dev, plan, t, scale)
+    want, wg = ob.attention(_np(t["q"]), _np(t["k"]), _np(t["v"]), src, row_ptr, _np(t["bias"]),
+                            scale, _np(t["go"]))
+    _compare(out, grads, want, wg, dtype)
+    return out, grads
+
+
+# one edge to rows longer than a tile's share of the work, empty rows between
+DEGREES = [0, 1, 2, 15, 16, 17, 31, 32, 33, 0, 64, 100, 5, 5, 5, 5, 0, 0, 3, 40, 1]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("h,kv,dk,dv", [(1, 1, 16, 16), (4, 4, 32, 32), (4, 2, 64, 64),
+                                        (8, 1, 24, 80), (2, 2, 128, 128), (3, 3, 7, 33),
+                                        (2, 1, 256, 256), (2, 2, 1, 130), (1, 1, 200, 1)])
+def test_sizes(dev, dtype, h, kv, dk, dv):
+    m = 150
+    src, row_ptr = _edges(DEGREES, m, 1)
+    t = _inputs(len(DEGREES), m, len(src), h, kv, dk, dv, dtype, 2)
+    out, grads = _check(dev, src, row_ptr, m, t, dtype)
+    empty = torch.tensor(DEGREES) == 0
+    assert not out[empty.to(dev)].any() and not grads["q"][empty.to(dev)].any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,m,degree", [(1, 1, 1), (1, 5000, 5000), (3, 3000, 2500),
+                                        (17, 400, 400), (40, 64, 64), (2, 10, 0)])
+def test_row_lengths(dev, dtype, n, m, degree):
+    """One edge, single long rows (a readout), dense rows, no edge at all; no bias."""
+    src, row_ptr = _edges([degree] * n, m, 3)
+    t = _inputs(n, m, len(src), 2, 2, 64, 64, dtype, 4, bias=False)
+    _check(dev, src, row_ptr, m, t, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_hub_among_short_rows(dev, dtype):
+    """One destination with 3001 edges among rows of 3, one source that every row reads."""
+    n, m = 50, 4000
+    degrees = [3] * n
+    degrees[20] = 3001
+    src, row_ptr = _edges(degrees, m, 5)
+    src[row_ptr[:-1]] = 0
+    t = _inputs(n, m, len(src), 4, 2, 48, 64, dtype, 6)
+    _check(dev, src, row_ptr, m, t, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_source_hub(dev, dtype):
+    """A source that 6000 destinations read: its gradients sum over a long row."""
+    n, m = 6000, 20
+    rng = np.random.default_rng(7)
+    src = np.stack([np.zeros(n), 1 + rng.integers(0, m - 1, n)], 1).astype(np.int64).reshape(-1)
+    row_ptr = np.arange(0, 2 * n + 1, 2, dtype=np.int64)
+    t = _inputs(n, m, len(src), 2, 2, 32, 32, dtype, 8)
+    _check(dev, src, row_ptr, m, t, dtype)
+
+
+@pytest.mark.parametrize("count", [2, 40, 700])
+def test_parallel_edges(dev, count):
+    """The same pair several times (periodic images), each edge with a bias of its own."""
+    n, m = 20, 30
+    src, row_ptr = _edges([12] * n, m, 9, distinct=False)
+    src = np.concatenate([np.sort(np.concatenate([src[a:b], np.full(count, 4)])) if i == 3 else
+                          src[a:b] for i, (a, b) in enumerate(zip(row_ptr[:-1], row_ptr[1:]))])
+    row_ptr = row_ptr + np.where(np.arange(n + 1) > 3, count, 0)
+    t = _inputs(n, m, len(src), 2, 2, 32, 48, "f32", 10)
+    _check(dev, src, row_ptr, m, t, "f32")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_graph_with_orders(dev, dtype):
+    """A periodic box through Graph.attention_plan: the order changes no result beyond the order
+    of summation, and channels as heads commute with the float64 oracle."""
+    import batmobile
+    n, c, h = 300, 8, 2
+    pos, cell = periodic_box(n, 11)
+    graph = batmobile.Graph(pos.to(dev), cell, 5.0, c)
+    src, row_ptr = graph.src.cpu().numpy(), graph.row_ptr.cpu().numpy()
+    t = _inputs(n, n, len(src), h, h, c // h * 16, c // h * 16, dtype, 12)
+    want, wg = ob.attention(_np(t["q"]), _np(t["k"]), _np(t["v"]), src, row_ptr, _np(t["bias"]),
+                            go=_np(t["go"]))
+    _compare(*_run(dev, graph.attention_plan(), t), want, wg, dtype)
+    _check(dev, src, row_ptr, n, t, dtype, torch.randperm(n, generator=gen(13)).to(dev),
+           torch.randperm(n, generator=gen(14)).to(dev))
+
+
+def test_edge_index_in_any_order(dev):
+    import batmobile
+    n, m, e, h = 60, 90, 900, 3
+    g = gen(15)
+    ei = torch.stack([torch.randint(0, m, (e,), generator=g), torch.randint(0, n, (e,), generator=g)])
+    t = _inputs(n, m, e, h, 1, 40, 24, "f32", 16)
+    out, grads = _run(dev, batmobile.AttentionPlan.from_edge_index(ei.to(dev), n, m), t)
+    by = np.lexsort((ei[0].numpy(), ei[1].numpy()))
+    row_ptr = np.searchsorted(ei[1].numpy()[by], np.arange(n + 1))
+    want, wg = ob.attention(_np(t["q"]), _np(t["k"]), _np(t["v"]), ei[0].numpy()[by], row_ptr,
+                            _np(t["bias"])[by], go=_np(t["go"]))
+    back = np.empty_like(wg["bias"])
+    back[by] = wg["bias"]
+    _compare(out, grads, want, dict(wg, bias=back), "f32")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_masks(dev, dtype):
+    """Bias of -inf on single edges, on whole rows, and the type's lowest value on edges and on a
+    whole row (there the probabilities are equal)."""
+    m = 80
+    src, row_ptr = _edges([10] * 20, m, 17)
+    t = _inputs(20, m, len(src), 2, 2, 32, 32, dtype, 18)
+    low = torch.finfo(torch.float32).min
+    b = t["bias"]
+    b[0:10] = -np.inf                 # row 0: nothing left
+    b[10:20, 1] = -np.inf             # row 1: nothing left for one head
+    b[20:30:3] = -np.inf
+    b[30:40] = low                    # row 3: all at the lowest value
+    b[40:50:2] = low
+    b[50:60:2] = low
+    b[51:60:2] = -np.inf              # row 5: lowest values or nothing
+    out, grads = _check(dev, src, row_ptr, m, t, dtype)
+    assert not out[0].any() and not out[1, 1].any() and not grads["bias"][0:10].any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_infinities_and_nan_stay_where_no_edge_leads(dev, dtype, value):
+    """A source with NaN or infinite keys and values, and a destination with such a query and
+    gradient: only rows and sources that share an unmasked edge with them may see it."""
+    n, m = 40, 40
+    src, row_ptr = _edges([9] * n, m, 19)
+    t = _inputs(n, m, len(src), 2, 2, 64, 64, dtype, 20)
+    dst = np.repeat(np.arange(n), 9)
+    bad_src, bad_dst = int(src[5 * 9]), 30
+    # every edge of the bad source but one row's, and of the bad destination, is masked
+    hit = ((src == bad_src) & (dst != 5)) | (dst == bad_dst)
+    t["bias"][torch.from_numpy(hit)] = -np.inf
+    t["k"][bad_src] = value
+    t["v"][bad_src, :, 3:40] = value
+    t["q"][bad_dst] = value
+    t["go"][bad_dst] = value
+    import batmobile
+    plan = batmobile.AttentionPlan(torch.from_numpy(src).to(dev),
+                                   torch.from_numpy(row_ptr).to(dev), m)
+    out, grads = _run(dev, plan, t)
+    rows = torch.arange(n) != 5
+    cols = torch.from_numpy(np.setdiff1d(np.arange(m), src[dst == 5]))
+    clean = {x: torch.nan_to_num(t[x].clone(), nan=0.0, posinf=0.0, neginf=0.0)
+             for x in ("q", "k", "v", "go")}
+    want, wg = ob.attention(_np(clean["q"]), _np(clean["k"]), _np(clean["v"]), src, row_ptr,
+                            _np(t["bias"]), go=_np(clean["go"]))
+    assert normwise_err(_np(out)[rows], want[rows]) <= BOUND[dtype]
+    assert normwise_err(_np(grads["q"])[rows], wg["q"][rows]) <= BOUND[dtype]
+    assert normwise_err(_np(grads["k"])[cols], wg["k"][cols]) <= BOUND[dtype]
+    assert normwise_err(_np(grads["v"])[cols], wg["v"][cols]) <= BOUND[dtype]
+    assert not np.isfinite(_np(out)[5]).all()
+
+
+def test_large_logits(dev):
+    """Logits of some thousands: the softmax is sharp, the maximum is taken off before the
+    exponential.  A logit of 1e4 carries an fp32 error of 1e-3 in the exponent, so rows are
+    compared through integers, whose products are exact."""
+    n, m = 20, 60
+    src, row_ptr = _edges([30] * n, m, 21)
+    t = _inputs(n, m, len(src), 1, 1, 16, 32, "f32", 22)
+    g = gen(23)
+    t["q"] = torch.randint(-30, 31, t["q"].shape, generator=g).float()
+    t["k"] = torch.randint(-30, 31, t["k"].shape, generator=g).float()
+    t["bias"] = torch.randint(-3, 4, t["bias"].shape, generator=g).float()
+    _check(dev, src, row_ptr, m, t, "f32", scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_strides_and_alignment(dev, dtype):
+    """q, k, v as slices of one projection, at odd element offsets, and with transposed heads."""
+    import batmobile
+    n, h, d = 70, 2, 32
+    src, row_ptr = _edges([12] * n, n, 24)
+    plan = batmobile.AttentionPlan(torch.from_numpy(src).to(dev), torch.from_numpy(row_ptr).to(dev))
+    t = _inputs(n, n, len(src), h, h, d, d, dtype, 25)
+    base, _ = _run(dev, plan, t)
+    qkv = torch.cat([t[x].reshape(n, -1) for x in "qkv"], 1).to(dev)
+    odd = torch.empty(n * 3 * h * d + 3, dtype=qkv.dtype, device=dev)[3:].view(n, -1)
+    odd.copy_(qkv)
+    for whole in (qkv, odd):
+        q, k, v = (x.view(n, h, d) for x in whole.chunk(3, 1))
+        out = batmobile.neighbor_attention(q, k, v, plan, bias=t["bias"].to(dev))
+        assert torch.equal(out, base)
+    tr = [t[x].to(dev).transpose(0, 1).contiguous().transpose(0, 1) for x in "qkv"]
+    assert torch.equal(batmobile.neighbor_attention(*tr, plan, bias=t["bias"].to(dev)), base)
+
+
+def test_gradient_against_differences(dev):
+    """Directional derivatives of the GPU's own fp32 output: step 1e-2, truncation of the order
+    of 1e-4 of the third derivative, rounding 1e-6 / 1e-2: 1e-3 of the gradient's norm."""
+    import batmobile
+    n, m = 30, 40
+    src, row_ptr = _edges([14] * n, m, 26)
+    plan = batmobile.AttentionPlan(torch.from_numpy(src).to(dev),
+                                   torch.from_numpy(row_ptr).to(dev), m)
+    t = _inputs(n, m, len(src), 4, 2, 20, 36, "f32", 27)
+    _, grads = _run(dev, plan, t)
+    go = t["go"].to(dev).double()
+    for name in ("q", "k", "v", "bias"):
+        d = grads[name] / grads[name].norm()
+
+        def f(step):
+            s = {x: t[x].to(dev) for x in ("q", "k", "v", "bias")}
+            s[name] = s[name] + step * d
+            return float((batmobile.neighbor_attention(s["q"], s["k"], s["v"], plan,
+                                                       bias=s["bias"]).double() * go).sum())
+        want = (f(1e-2) - f(-1e-2)) / 2e-2
+        got = float(grads[name].norm())
+        assert abs(got - want) <= 1e-3 * got, (name, got, want)
+
+
+def test_results_are_deterministic_and_follow_the_stream(dev):
+    """The same bits on another stream, right behind the work that makes the inputs."""
+    import batmobile
+    pos, cell = periodic_box(500, 28)
+    plan = batmobile.Graph(pos.to(dev), cell, 5.0, 8).attention_plan()
+    e = plan.src.numel()
+    t = _inputs(500, 500, e, 4, 2, 64, 64, "f32", 29)
+    a, ga = _run(dev, plan, t)
+    big = torch.randn(4096, 4096, device=dev)
+    stream = torch.cuda.Stream()
+    on = {x: t[x].to(dev) for x in t}
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for _ in range(5):
+            big = big @ big * 1e-3
+        late = {x: (v + 0 * big[0, 0].nan_to_num().to(v.dtype)) for x, v in on.items()}
+        b, gb = _run(dev, plan, late)
+    assert torch.equal(a, b)
+    for name in ga:
+        assert torch.equal(ga[name], gb[name]), name
+
+
+def test_refusals(dev):
+    import batmobile
+    src, row_ptr = _edges([3, 3], 5, 30)
+    s, r = torch.from_numpy(src).to(dev), torch.from_numpy(row_ptr).to(dev)
+    plan = batmobile.AttentionPlan(s, r, 5)
+    q = torch.zeros(2, 4, 8, device=dev)
+    k = torch.zeros(5, 2, 8, device=dev)
+    call = batmobile.neighbor_attention
+    with pytest.raises(RuntimeError, match="multiple"):
+        call(q, torch.zeros(5, 3, 8, device=dev), torch.zeros(5, 3, 8, device=dev), plan)
+    with pytest.raises(RuntimeError, match="head size"):
+        call(q, torch.zeros(5, 2, 9, device=dev), k, plan)
+    with pytest.raises(RuntimeError, match="256"):
+        call(q, k, torch.zeros(5, 2, 257, device=dev), plan)
+    with pytest.raises(RuntimeError, match="type"):
+        call(q, k.bfloat16(), k, plan)
+    with pytest.raises(RuntimeError, match="float32 or bfloat16"):
+        call(q.double(), k.double(), k.double(), plan)
+    with pytest.raises(RuntimeError, match="bias"):
+        call(q, k, k, plan, bias=torch.zeros(6, 3, device=dev))
+    with pytest.raises(RuntimeError, match="destinations"):
+        call(torch.zeros(3, 4, 8, device=dev), k, k, plan)
+    with pytest.raises(RuntimeError, match="must be on"):
+        call(q, k.cpu(), k, plan)
+    bad = s.clone()
+    bad[1] = 5
+    with pytest.raises(ValueError, match="lie in"):
+        batmobile.AttentionPlan(bad, r, 5)
+    with pytest.raises(ValueError, match="ascend"):
+        batmobile.AttentionPlan(torch.tensor([2, 1, 3, 0, 1, 2], device=dev), r, 5)
+    with pytest.raises(ValueError, match="ascend"):
+        batmobile.AttentionPlan(torch.tensor([2, 1, 0], device=dev),
+                                torch.tensor([0, 0, 3], device=dev), 5)
+    with pytest.raises(ValueError, match="row_ptr"):
+        batmobile.AttentionPlan(s, torch.tensor([0, 4, 3], device=dev), 5)
+    with pytest.raises(ValueError, match="int64"):
+        batmobile.AttentionPlan(s.int(), r, 5)
+    with pytest.raises(ValueError, match="destinations"):
+        batmobile.AttentionPlan.from_edge_index(torch.stack([s, s]), 2, 5)

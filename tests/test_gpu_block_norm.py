@@ -1,0 +1,305 @@
+"""Norms by degree with gate and residual, and gradient clipping, on the GPU against the float64
+oracle.
+
+Bounds (normwise).  fp32: a handful of roundings per element and sums of up to 2048 x 7 squares
+(1e-6): 3e-6; the weights' gradients are sums over all atoms, whose rounding grows like the root
+of their number against a sum that does so too: 1e-5.  bf16 features: results rounded to 8 bits,
+2^-9 of the largest, and n, gx formed from the rounded h in the backward: 6e-3 (three roundings).
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import block as ob
+
+from helpers import gen, normwise_err, random_rotation, wigner_d
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+BOUND = {"f32": 3e-6, "bf16": 6e-3}
+WEIGHT_BOUND = {"f32": 1e-5, "bf16": 6e-3}
+
+
+def _np(t):
+    return None if t is None else t.detach().cpu().double().numpy()
+
+
+def _inputs(n, c, dtype, seed):
+    g = gen(seed)
+    t = TYPES[dtype]
+    return {"x": torch.randn(n, c, 16, generator=g).to(t),
+            "y": (2 * torch.randn(n, c, 16, generator=g)).to(t),
+            "gate": torch.randn(n, c, 4, generator=g).to(t),
+            "scale": torch.randn(c, generator=g), "w_post": torch.randn(4, c, generator=g),
+            "w_pre": torch.randn(4, c, generator=g),
+            "gh": torch.randn(n, c, 16, generator=g).to(t),
+            "gn": torch.randn(n, c, 16, generator=g).to(t)}
+
+
+def _block(dev, t, gate=True, pre=True, seeds=("gh", "gn")):
+    import batmobile
+    names = ["x", "y", "scale", "w_post"] + (["gate"] if gate else []) + (["w_pre"] if pre else [])
+    leaf = {x: t[x].to(dev).requires_grad_(True) for x in names}
+    res = batmobile.gated_residual_norm(leaf["x"], leaf["y"], leaf.get("gate"), leaf["scale"],
+                                        leaf["w_post"], leaf.get("w_pre"))
+    h, n = res if pre else (res, None)
+    outs = [o for o, s in ((h, "gh"), (n, "gn")) if o is not None and s in seeds]
+    grads = torch.autograd.grad(outs, list(leaf.values()), [t[s].to(dev) for s in seeds])
+    return h, n, dict(zip(names, grads))
+
+
+def _check(got, want, dtype, weights=("scale", "w_post", "w_pre")):
+    for name, g in got.items():
+        bound = (WEIGHT_BOUND if name in weights else BOUND)[dtype]
+        assert normwise_err(_np(g), want[name]) <= bound, name
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,c", [(1, 1), (3, 5), (2, 16), (7, 17), (33, 32), (5, 48), (300, 64),
+                                 (9, 100), (4, 128), (3, 129), (6, 300), (2, 512), (2, 700),
+                                 (1, 2048)])
+def test_block_norm(dev, dtype, n, c):
+    t = _inputs(n, c, dtype, n + c)
+    h, nn, grads = _block(dev, t)
+    rh, rn, want = ob.gated_residual_norm(*[_np(t[x]) for x in ("x", "y", "gate", "scale", "w_post",
+                                                                "w_pre")],
+                                          gh=_np(t["gh"]), gn=_np(t["gn"]))
+    assert normwise_err(_np(h), rh) <= BOUND[dtype]
+    assert normwise_err(_np(nn), rn) <= BOUND[dtype]
+    _check(grads, want, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("gate,pre,seeds", [(False, True, ("gh", "gn")), (True, False, ("gh",)),
+                                            (False, False, ("gh",)), (True, True, ("gn",)),
+                                            (True, True, ("gh",))])
+def test_forms(dev, dtype, gate, pre, seeds):
+    """Without a gate, without the next norm, and with a gradient for one output only."""
+    t = _inputs(21, 40, dtype, 5)
+    h, nn, grads = _block(dev, t, gate, pre, seeds)
+    rh, rn, want = ob.gated_residual_norm(
+        _np(t["x"]), _np(t["y"]), _np(t["gate"]) if gate else None, _np(t["scale"]),
+        _np(t["w_post"]), _np(t["w_pre"]) if pre else None,
+        gh=_np(t["gh"]) if "gh" in seeds else None, gn=_np(t["gn"]) if "gn" in seeds else None)
+    assert normwise_err(_np(h), rh) <= BOUND[dtype]
+    if pre:
+        assert normwise_err(_np(nn), rn) <= BOUND[dtype]
+    if "gn" not in seeds and pre:
+        assert not grads.pop("w_pre").any()
+    _check(grads, want, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,c", [(1, 1), (5, 16), (130, 33), (4, 130), (2, 600)])
+def test_norm_alone(dev, dtype, n, c):
+    import batmobile
+    t = _inputs(n, c, dtype, 9)
+    x, w = t["x"].to(dev).requires_grad_(True), t["w_pre"].to(dev).requires_grad_(True)
+    out = batmobile.equivariant_norm(x, w)
+    gx, gw = torch.autograd.grad(out, [x, w], t["gn"].to(dev))
+    _, want, g = ob.gated_residual_norm(_np(t["x"]), None, None, None, None, _np(t["w_pre"]),
+                                        gn=_np(t["gn"]))
+    assert normwise_err(_np(out), want) <= BOUND[dtype]
+    _check({"x": gx, "w_pre": gw}, {"x": g["x"], "w_pre": g["w_pre"]}, dtype)
+
+
+def test_many_rows(dev):
+    """More rows than the backward's workgroups hold at once; a sample of rows, all weights."""
+    t = _inputs(9001, 24, "f32", 31)
+    h, nn, grads = _block(dev, t)
+    rh, rn, want = ob.gated_residual_norm(*[_np(t[x]) for x in ("x", "y", "gate", "scale", "w_post",
+                                                                "w_pre")],
+                                          gh=_np(t["gh"]), gn=_np(t["gn"]))
+    assert normwise_err(_np(nn), rn) <= BOUND["f32"]
+    _check(grads, want, "f32")
+
+
+def test_rows_without_rows_zeros_and_strides(dev):
+    import batmobile
+    w = torch.ones(4, 8, device=dev)
+    x = torch.zeros(0, 8, 16, device=dev, requires_grad=True)
+    out = batmobile.equivariant_norm(x, w.requires_grad_(True))
+    gx, gw = torch.autograd.grad(out, [x, w], torch.zeros_like(out))
+    assert out.shape == x.shape == gx.shape and not gw.any()
+    # a row of zeros: 0 / sqrt(eps) = 0, finite gradients
+    z = torch.zeros(2, 8, 16, device=dev, requires_grad=True)
+    n = batmobile.equivariant_norm(z, w)
+    (gz,) = torch.autograd.grad(n, [z], torch.ones_like(n))
+    assert not n.any() and torch.allclose(gz, torch.full_like(gz, 1e3), rtol=1e-5)
+    # a channel slice and an unaligned view give the results of their copies
+    wide = torch.randn(5, 24, 16, device=dev)
+    part = wide[:, 8:16]
+    assert torch.equal(batmobile.equivariant_norm(part, w),
+                       batmobile.equivariant_norm(part.contiguous(), w))
+    odd = torch.randn(5 * 8 * 16 + 1, device=dev)[1:].view(5, 8, 16)
+    assert torch.equal(batmobile.equivariant_norm(odd, w),
+                       batmobile.equivariant_norm(odd.clone(), w))
+
+
+def test_nan_and_infinities_stay_in_their_row(dev):
+    import batmobile
+    t = _inputs(12, 20, "f32", 41)
+    clean = _block(dev, t)
+    bad = dict(t, y=t["y"].clone())
+    bad["y"][3, 2, 5] = float("nan")
+    bad["y"][7, 0, 0] = float("inf")
+    got = _block(dev, bad)
+    rows = [i for i in range(12) if i not in (3, 7)]
+    for a, b in ((clean[0], got[0]), (clean[1], got[1]), (clean[2]["x"], got[2]["x"]),
+                 (clean[2]["y"], got[2]["y"]), (clean[2]["gate"], got[2]["gate"])):
+        assert torch.equal(a[rows], b[rows])
+    assert torch.isnan(got[0][3]).any()
+
+
+def test_rotation(dev):
+    """norm(D x) = D norm(x) for a rotation D of the components."""
+    import batmobile
+    t = _inputs(6, 12, "f32", 43)
+    d = torch.from_numpy(wigner_d(random_rotation(2)))
+    args = [t[x].to(dev) for x in ("gate", "scale", "w_post", "w_pre")]
+    a = batmobile.gated_residual_norm(t["x"].to(dev), t["y"].to(dev), *args)
+    b = batmobile.gated_residual_norm((t["x"].double() @ d.T).float().to(dev),
+                                      (t["y"].double() @ d.T).float().to(dev), *args)
+    for u, w in zip(a, b):
+        assert normwise_err(_np(w), _np(u) @ d.T.numpy()) <= 1e-5
+
+
+def test_gradient_against_differences(dev):
+    """Step 1e-2 along each gradient, as for the attention: 1e-3."""
+    import batmobile
+    t = _inputs(15, 10, "f32", 45)
+    _, _, grads = _block(dev, t)
+    for name, g in grads.items():
+        d = g / g.norm()
+
+        def f(step):
+            s = {x: v.to(dev) for x, v in t.items()}
+            s[name] = s[name] + step * d
+            h, n = batmobile.gated_residual_norm(s["x"], s["y"], s["gate"], s["scale"],
+                                                 s["w_post"], s["w_pre"])
+            return float((h.double() * s["gh"].double()).sum() +
+                         (n.double() * s["gn"].double()).sum())
+        want, got = (f(1e-2) - f(-1e-2)) / 2e-2, float(g.norm())
+        assert abs(got - want) <= 1e-3 * got, (name, got, want)
+
+
+def test_norm_refusals(dev):
+    import batmobile
+    x, w = torch.zeros(3, 4, 16, device=dev), torch.ones(4, 4, device=dev)
+    s = torch.ones(4, device=dev)
+    call = batmobile.gated_residual_norm
+    with pytest.raises(RuntimeError, match="16"):
+        batmobile.equivariant_norm(torch.zeros(3, 4, 9, device=dev), w)
+    with pytest.raises(RuntimeError, match=r"\[4, C\]"):
+        batmobile.equivariant_norm(x, torch.ones(4, 5, device=dev))
+    with pytest.raises(RuntimeError, match="float32 or bfloat16"):
+        batmobile.equivariant_norm(x.double(), w)
+    with pytest.raises(RuntimeError, match="float32"):
+        batmobile.equivariant_norm(x, w.bfloat16())
+    with pytest.raises(RuntimeError, match="shape of x"):
+        call(x, torch.zeros(3, 5, 16, device=dev), None, s, w, w)
+    with pytest.raises(RuntimeError, match="gate"):
+        call(x, x, torch.zeros(3, 4, 3, device=dev), s, w, w)
+    with pytest.raises(RuntimeError, match="scale"):
+        call(x, x, None, torch.ones(5, device=dev), w, w)
+    with pytest.raises(RuntimeError, match="type"):
+        call(x, x.bfloat16(), None, s, w, w)
+    with pytest.raises(RuntimeError, match="2048"):
+        batmobile.equivariant_norm(torch.zeros(1, 2049, 16, device=dev),
+                                   torch.ones(4, 2049, device=dev))
+
+
+# ---------------------------------------------------------------------------
+# clipping
+# ---------------------------------------------------------------------------
+
+def _grads(shapes, types, seed, size=1.0):
+    g = gen(seed)
+    return [(size * torch.randn(*s, generator=g)).to(TYPES[t]) for s, t in zip(shapes, types)]
+
+
+SHAPES = [(1,), (7,), (64,), (34, 8, 8), (0,), (3, 5, 7), (8193,), (100003,), (2, 4)]
+
+
+@pytest.mark.parametrize("types", [["f32"] * 9, ["bf16"] * 9, ["f32", "bf16"] * 4 + ["f32"]])
+@pytest.mark.parametrize("max_norm", [0.0, 1e-3, 1.0, 1e6])
+def test_clip(dev, types, max_norm):
+    """Clipped values: one rounding of the factor and one of the product, 2^-23 relative to the
+    largest (fp32), 2^-8 of it (bf16); the norm is summed in 64 bits: 1e-6."""
+    import batmobile
+    grads = _grads(SHAPES, types, 51)
+    norm, out = batmobile.clip_grad_norm([g.to(dev) for g in grads], max_norm)
+    rn, want = ob.clip([_np(g) for g in grads], max_norm)
+    assert abs(float(norm) - rn) <= 1e-6 * rn
+    for o, w, t in zip(out, want, types):
+        assert o.dtype == TYPES[t]
+        assert normwise_err(_np(o), w) <= (5e-7 if t == "f32" else 4e-3)
+
+
+def test_clip_many_tensors_and_extreme_values(dev):
+    """More tensors than a launch takes, values whose squares leave fp32's range either way."""
+    import batmobile
+    for size in (1e30, 1e-30):
+        grads = _grads([(50 + i,) for i in range(457)], ["f32"] * 457, 53, size)
+        norm, out = batmobile.clip_grad_norm([g.to(dev) for g in grads], size)
+        rn, want = ob.clip([_np(g) for g in grads], float(np.float32(size)))
+        assert abs(float(norm) - rn) <= 1e-6 * rn
+        for o, w in zip(out, want):     # 1e-30 * 1e-24 is 0 in fp32
+            assert normwise_err(_np(o), w.astype(np.float32)) <= 5e-7
+
+
+def test_clip_not_finite(dev):
+    """An infinite gradient gives an infinite norm and the factor 0 (0 * inf = NaN), NaN gives
+    NaN everywhere, as the formula says."""
+    import batmobile
+    a, b = torch.ones(5, device=dev), torch.ones(300, device=dev)
+    b[7] = float("inf")
+    norm, (ca, cb) = batmobile.clip_grad_norm([a, b], 1.0)
+    assert torch.isinf(norm) and not ca.any() and torch.isnan(cb[7]) and cb.nan_to_num().sum() == 0
+    b[7] = float("nan")
+    norm, (ca, cb) = batmobile.clip_grad_norm([a, b], 1.0)
+    assert torch.isnan(norm) and torch.isnan(ca).all() and torch.isnan(cb).all()
+
+
+def test_clip_in_place_layouts_and_streams(dev):
+    """In place on parameters: transposed and gapped gradients, one without a gradient; the
+    inputs made on another stream just before."""
+    import batmobile
+    g = gen(55)
+    vals = [torch.randn(6, 10, generator=g), torch.randn(31, generator=g),
+            torch.randn(9, 8, generator=g)]
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        p = [torch.nn.Parameter(torch.zeros(6, 10, device=dev)),
+             torch.nn.Parameter(torch.zeros(31, device=dev)),
+             torch.nn.Parameter(torch.zeros(9, 8, device=dev)),
+             torch.nn.Parameter(torch.zeros(4, device=dev))]
+        p[0].grad = vals[0].to(dev).t().contiguous().t()
+        p[1].grad = torch.zeros(62, device=dev)[::2]
+        p[1].grad.copy_(vals[1].to(dev))
+        p[2].grad = torch.zeros(73, device=dev)[1:].view(9, 8)
+        p[2].grad.copy_(vals[2].to(dev))
+        norm = batmobile.clip_grad_norm_(p, 0.5)
+    torch.cuda.synchronize()
+    rn, want = ob.clip([_np(v) for v in vals], 0.5)
+    assert abs(float(norm) - rn) <= 1e-6 * rn and p[3].grad is None
+    for q, w in zip(p, want):
+        assert normwise_err(_np(q.grad), w) <= 5e-7
+    # below the limit nothing changes, bit for bit
+    before = [q.grad.clone() for q in p[:3]]
+    batmobile.clip_grad_norm_(p, 10.0)
+    assert all(torch.equal(q.grad, b) for q, b in zip(p, before))
+
+
+def test_clip_refusals(dev):
+    import batmobile
+    a = torch.ones(4, device=dev)
+    with pytest.raises(RuntimeError, match="float32 or bfloat16"):
+        batmobile.clip_grad_norm([a.double()], 1.0)
+    with pytest.raises(RuntimeError, match="one tensor per"):
+        batmobile.clip_grad_norm([a], 1.0, [])
+    with pytest.raises(RuntimeError, match="shapes"):
+        batmobile.clip_grad_norm([a], 1.0, [torch.ones(5, device=dev)])
+    with pytest.raises(RuntimeError, match="type"):
+        batmobile.clip_grad_norm([a], 1.0, [a.bfloat16()])

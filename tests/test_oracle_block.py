@@ -1,0 +1,137 @@
+"""The block operators' float64 oracle against differences and its own invariants (CPU), and the
+refusals of the host entry points that need no GPU."""
+import ctypes
+import os
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import block as ob
+
+from helpers import random_rotation, wigner_d
+
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+STEP = 1e-6
+# central differences with step 1e-6 in float64: truncation ~1e-12, rounding ~1e-16 / 1e-6 times
+# the size of the sum (about 100)
+TOL = 1e-7
+
+
+def _graph(rng, n, m, degrees):
+    row_ptr = np.concatenate([[0], np.cumsum(degrees)])
+    src = np.concatenate([np.sort(rng.integers(0, m, d)) for d in degrees]) if sum(degrees) else \
+        np.zeros(0, np.int64)
+    return src.astype(np.int64), row_ptr.astype(np.int64)
+
+
+def _directional(f, args, grads, names, rng):
+    """f(args) -> scalar; the formula's directional derivative against the difference's."""
+    for name in names:
+        d = rng.normal(size=args[name].shape)
+        up, down = dict(args), dict(args)
+        up[name] = args[name] + STEP * d
+        down[name] = args[name] - STEP * d
+        want = (f(up) - f(down)) / (2 * STEP)
+        got = float((grads[name] * d)[np.isfinite(args[name])].sum())
+        assert abs(got - want) <= TOL * max(1.0, abs(want)), (name, got, want)
+
+
+@pytest.mark.parametrize("h,kv", [(2, 2), (4, 2)])
+def test_attention_gradients_against_differences(h, kv):
+    rng = np.random.default_rng(h)
+    src, row_ptr = _graph(rng, 5, 6, [3, 0, 1, 7, 4])
+    args = {"q": rng.normal(size=(5, h, 3)), "k": rng.normal(size=(6, kv, 3)),
+            "v": rng.normal(size=(6, kv, 5)), "bias": rng.normal(size=(15, h))}
+    args["bias"][[0, 3], 0] = -np.inf          # a masked edge, and a row with nothing left
+    go = rng.normal(size=(5, h, 5))
+
+    def f(a):
+        return float((ob.attention(a["q"], a["k"], a["v"], src, row_ptr, a["bias"]) * go).sum())
+
+    out, g = ob.attention(args["q"], args["k"], args["v"], src, row_ptr, args["bias"], go=go)
+    assert not out[1].any() and not out[2, 0].any()
+    _directional(f, args, g, ["q", "k", "v"], rng)
+    finite = dict(args, bias=np.where(np.isinf(args["bias"]), -50.0, args["bias"]))
+    _, g = ob.attention(finite["q"], finite["k"], finite["v"], src, row_ptr, finite["bias"], go=go)
+    _directional(f, finite, g, ["bias"], rng)
+
+
+@pytest.mark.parametrize("gated,pre", [(True, True), (False, True), (True, False)])
+def test_norm_gradients_against_differences(gated, pre):
+    rng = np.random.default_rng(5)
+    n, c = 3, 4
+    args = {"x": rng.normal(size=(n, c, 16)), "y": rng.normal(size=(n, c, 16)),
+            "scale": rng.normal(size=c), "w_post": rng.normal(size=(4, c))}
+    if gated:
+        args["gate"] = rng.normal(size=(n, c, 4))
+    if pre:
+        args["w_pre"] = rng.normal(size=(4, c))
+    gh, gn = rng.normal(size=(n, c, 16)), rng.normal(size=(n, c, 16))
+
+    def f(a):
+        h, nn = ob.gated_residual_norm(a["x"], a["y"], a.get("gate"), a["scale"], a["w_post"],
+                                       a.get("w_pre"))
+        return float((h * gh).sum() + ((nn * gn).sum() if pre else 0.0))
+
+    _, _, g = ob.gated_residual_norm(args["x"], args["y"], args.get("gate"), args["scale"],
+                                     args["w_post"], args.get("w_pre"), gh=gh,
+                                     gn=gn if pre else None)
+    _directional(f, args, g, list(args), rng)
+
+
+def test_norm_alone_gradient_and_rotation():
+    rng = np.random.default_rng(7)
+    x, w, gn = rng.normal(size=(3, 5, 16)), rng.normal(size=(4, 5)), rng.normal(size=(3, 5, 16))
+    _, n, g = ob.gated_residual_norm(x, None, None, None, None, w, gn=gn)
+    _directional(lambda a: float((ob.norm(a["x"], a["w_pre"])[0] * gn).sum()),
+                 {"x": x, "w_pre": w}, g, ["x", "w_pre"], rng)
+    d = wigner_d(random_rotation(3))
+    assert np.abs(ob.norm(x @ d.T, w)[0] - n @ d.T).max() <= 1e-12
+
+
+def test_clip_oracle():
+    norm, (a, b) = ob.clip([np.array([3.0]), np.array([[4.0]])], 1.0)
+    assert norm == 5.0 and abs(a[0] - 3 / (5 + 1e-6)) < 1e-15 and abs(b[0, 0] - 4 / (5 + 1e-6)) < 1e-15
+    assert ob.clip([np.array([3.0])], 10.0)[1][0][0] == 3.0
+
+
+def test_host_refusals_of_the_c_abi():
+    """Shapes and types that the kernels do not take end before any device call."""
+    lib = ctypes.CDLL(os.path.join(REPO, "batmobile-evo_amd", "lib", "libbatmobile_hip.so"))
+    p = ctypes.c_void_p(256)
+    i64 = ctypes.c_int64
+    norm = lib.batteries_gated_residual_norm
+    norm.argtypes = [ctypes.c_void_p] * 9 + [i64, ctypes.c_int, ctypes.c_float, ctypes.c_int,
+                                             ctypes.c_void_p]
+    assert norm(p, None, None, None, None, p, None, p, None, 5, 4096, 1e-6, 0, None) == -1
+    assert norm(p, None, None, None, None, p, None, p, None, 5, 8, 1e-6, 2, None) == -1
+    assert norm(p, None, None, None, None, None, None, None, None, 5, 8, 1e-6, 0, None) == -1
+    odd = ctypes.c_void_p(260)
+    assert norm(odd, None, None, None, None, p, None, p, None, 5, 8, 1e-6, 0, None) == -1
+    clip = lib.batteries_clip_grad_norm
+    clip.argtypes = [ctypes.c_void_p] * 4 + [i64, ctypes.c_float] + [ctypes.c_void_p] * 2 + \
+        [ctypes.c_size_t, ctypes.c_void_p]
+    ptrs = (ctypes.c_void_p * 1)(256)
+    n, dt = (i64 * 1)(10), (ctypes.c_int * 1)(3)
+    assert clip(ptrs, ptrs, n, dt, 1, 1.0, p, p, 1 << 20, None) == -1      # type
+    dt[0] = 0
+    assert clip(ptrs, ptrs, n, dt, 1, -1.0, p, p, 1 << 20, None) == -1     # max_norm
+    assert clip(ptrs, ptrs, n, dt, 1, 1.0, p, p, 16, None) == -2           # workspace
+
+
+def test_python_refusals(bm):
+    import batmobile
+    x = torch.zeros(3, 4, 16)
+    w = torch.ones(4, 4)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        batmobile.equivariant_norm(x, w)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        batmobile.clip_grad_norm([x], 1.0)
+    with pytest.raises(RuntimeError, match="at least one"):
+        batmobile.clip_grad_norm([], 1.0)
+    with pytest.raises(RuntimeError, match="negative"):
+        batmobile.clip_grad_norm([x], -1.0)
+    with pytest.raises(ValueError, match="edge_index"):
+        batmobile.AttentionPlan.from_edge_index(torch.zeros(3, 2, dtype=torch.long), 4)
+    assert float(batmobile.clip_grad_norm_([torch.zeros(3)], 1.0)) == 0.0
