@@ -30,7 +30,8 @@ NL_LIB = os.path.join(LIBDIR, "libbatteries_neighbor.so")
 EXT = os.path.join(PYDIR, "_batmobile" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 HIP_SOURCES = ["sh.hip", "tp.hip", "mp.hip", "nl.hip", "graph.hip", "mace.hip",
-               "attention.hip", "block_norm.hip", "grad_clip.hip"]
+               "attention.hip", "attention_bwd.hip", "attention_plan.hip", "block_norm.hip",
+               "grad_clip.hip"]
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"

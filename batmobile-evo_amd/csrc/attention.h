@@ -1,0 +1,382 @@
+// Tiles of the attention kernels (attention.hip, attention_bwd.hip, attention_plan.hip).
+//
+// A side of the graph (destinations with their sources, or sources with their destinations) is
+// cut into tiles of 16 rows, neighbours in space.  A tile's rows share many columns: the plan
+// lists the union of the columns, 32 to a chunk, with a 32-bit mask per row and chunk of the
+// edges that exist.  The kernels then take a chunk's 16 x 32 pairs as matrix products on the
+// matrix cores, so a column's data is read once per tile and head instead of once per edge (a
+// 5000-atom box with 28 neighbours: 448 edges of a tile lead to about 150 columns), and 5 of 6
+// products of a pair without an edge are thrown away, which costs less than reading the rows
+// again.  Edges of a row are numbered along the row: the k-th set bit of a row over the chunks
+// is its k-th edge, so the masks also give each pair's place in the arrays per edge.
+//
+// Every wave works on one (item, head): an item is a tile, or a part of one that has a long
+// row or many edges.  Nothing is shared between waves: the fragments come from global memory
+// in the layout the matrix instructions take.
+#pragma once
+#include "common.h"
+#include "batmobile_hip.h"
+
+namespace bmhip {
+
+constexpr int kAttnRows = 16;     // rows of a tile
+constexpr int kAttnCols = 32;     // columns of a chunk
+
+// ---------------------------------------------------------------------------
+// the plan of one side, in one int32 array
+// ---------------------------------------------------------------------------
+constexpr int kPlanHead = 16;     // items, parts, longest row, flags
+constexpr int kPlanItems = 0, kPlanParts = 1, kPlanBad = 2;
+
+struct PlanLayout {
+    int64_t tiles, max_items, max_chunks;
+    int64_t rows, tile_item, tile_chunk, tile_part, item_tile, items, base, masks, ids, total;
+};
+
+// An item takes up to 2048 edges and up to 256 of a row (512 if the row ends there).
+constexpr int kItemEdges = 2048, kItemRow = 256;
+
+inline PlanLayout plan_layout(int64_t n_rows, int64_t n_edges) {
+    PlanLayout p;
+    p.tiles = ceil_div(n_rows, kAttnRows);
+    p.max_items = p.tiles + n_edges / kItemEdges + n_edges / kItemRow;
+    p.max_chunks = n_edges / kAttnCols + p.max_items;
+    int64_t at = kPlanHead;
+    auto take = [&](int64_t n) {
+        const int64_t r = at;
+        at += (n + 15) / 16 * 16;   // 64-byte sections
+        return r;
+    };
+    p.rows = take(p.tiles * kAttnRows);
+    p.tile_item = take(p.tiles + 1);
+    p.tile_chunk = take(p.tiles + 1);
+    p.tile_part = take(p.tiles + 1);
+    p.items = take(p.max_items * 4);
+    p.base = take(p.max_items * kAttnRows);
+    p.masks = take(p.max_chunks * kAttnRows);
+    p.ids = take(p.max_chunks * kAttnCols);
+    p.total = at;
+    return p;
+}
+
+struct AttnSide {
+    const int* rows;          // [16 tiles], -1 past the end
+    const int* tile_part;     // [tiles + 1] first part
+    const int4* items;        // tile, first chunk, chunks, part (-1: the tile's only item)
+    const int* base;          // [16 items] each row's first edge in the item
+    const uint32_t* masks;    // [16 chunks]
+    const int* ids;           // [32 chunks] columns
+    const int* eid;           // edge -> its place in the arrays per edge (NULL: itself)
+    int n_items, n_tiles;
+};
+
+// The tile of part p, the tile's first part and their number.
+__device__ __forceinline__ int tile_of_part(const AttnSide& s, int p, int& first, int& parts) {
+    int lo = 0, hi = s.n_tiles - 1;
+    while (lo < hi) {
+        const int m = (lo + hi + 1) >> 1;
+        if (s.tile_part[m] <= p) lo = m; else hi = m - 1;
+    }
+    first = s.tile_part[lo];
+    parts = s.tile_part[lo + 1] - first;
+    return lo;
+}
+
+// The work unit of a wave: workgroup b runs on XCD b % 8, which takes a contiguous eighth of
+// the units, so that tiles that share columns meet in one L2.
+__device__ __forceinline__ int64_t attn_unit(int64_t n_units) {
+    const int64_t per = gridDim.x >> 3;
+    const int64_t b = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    const int64_t u = b * 4 + (threadIdx.x >> 6);
+    return u < n_units ? u : -1;
+}
+inline unsigned attn_grid(int64_t n_units) { return (unsigned)(ceil_div(n_units, 32) * 8); }
+
+// ---------------------------------------------------------------------------
+// Fragments.  l = lane, n = l % 16, g = l / 16.  A step takes kTiles tiles of 16 columns.
+//
+// Row form (the contraction runs along a row's components): lane l holds row n.
+//   bf16: components 32 s + 8 g + (0..7) in step s of v_mfma_f32_16x16x32_bf16
+//   fp32: components 16 s + 4 g + (0..3), one v_mfma_f32_16x16x4f32 for each of the four
+// Column form (the contraction runs over the step's columns j): lane l holds kW components
+// kW n + (0..) of a block of 16 kW, for kRowsPerLane columns; matrix product c of the block
+// takes component c of each, so that its row m is component kW m + c.
+//   bf16: columns 4 g + (0..3) and 16 + 4 g + (0..3), fp32: 4 g + (0..3)
+// The products are taken transposed, (columns) x (tile rows): lane l then has the pairs of tile
+// row n with columns 16 t + 4 g + r in tile t, element r, which is at once the layout that the
+// second product takes its factor in.  A result of the column form lies with tile row n in lane
+// l, components kW (4 g + r) + c of block b in acc[b kW + c][r].
+// ---------------------------------------------------------------------------
+template <typename T>
+struct Attn;
+
+template <>
+struct Attn<float> {
+    static constexpr int kTiles = 1, kRowsPerLane = 4, kSteps = 16, kAlign = 4;
+    using Vec = float4;                          // a row-form load
+    static __device__ __forceinline__ v4f rowprod(const float4& a, const float4& b, v4f acc) {
+        return mfma4(a, b, acc);
+    }
+};
+template <>
+struct Attn<uint16_t> {
+    static constexpr int kTiles = 2, kRowsPerLane = 8, kSteps = 32, kAlign = 8;
+    using Vec = v4u;
+    static __device__ __forceinline__ v4f rowprod(const v4u& a, const v4u& b, v4f acc) {
+        return mfma_bf16(a, b, acc);
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ const T* row_of(const void* p, int row, int64_t stride) {
+    return (const T*)p + (int64_t)row * stride;
+}
+
+// Row form of one row: D components of at most P, zero past D.
+template <typename T, int P>
+struct RowFrag {
+    static constexpr int kN = P / Attn<T>::kSteps;
+    typename Attn<T>::Vec v[kN];
+    __device__ __forceinline__ void load(const T* row, int D, int g) {
+#pragma unroll
+        for (int s = 0; s < kN; ++s) {
+            const int d = s * Attn<T>::kSteps + g * Attn<T>::kAlign;
+            typename Attn<T>::Vec z{};
+            if (d < D) z = *reinterpret_cast<const typename Attn<T>::Vec*>(row + d);
+            v[s] = z;
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int s = 0; s < kN; ++s) v[s] = typename Attn<T>::Vec{};
+    }
+};
+
+template <typename T, int P>
+__device__ __forceinline__ v4f row_product(const RowFrag<T, P>& a, const RowFrag<T, P>& b) {
+    // two chains: a chain of one accumulator would wait for every product
+    v4f x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < RowFrag<T, P>::kN; s += 2) {
+        x = Attn<T>::rowprod(a.v[s], b.v[s], x);
+        if (s + 1 < RowFrag<T, P>::kN) y = Attn<T>::rowprod(a.v[s + 1], b.v[s + 1], y);
+    }
+    return x + y;
+}
+
+// Column form of a step's columns: kW components a lane and block.
+template <typename T, int P>
+struct ColFrag;
+
+template <int P>
+struct ColFrag<float, P> {
+    static constexpr int kW = 4, kBlocks = P / 64, kAcc = kBlocks * kW;
+    float4 v[4][kBlocks];
+    template <typename F>
+    __device__ __forceinline__ void load(F&& row, int D, int n) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float* p = row(j);
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const int d = b * 64 + 4 * n;
+                v[j][b] = d < D ? *reinterpret_cast<const float4*>(p + d) : make_float4(0, 0, 0, 0);
+            }
+        }
+    }
+    // acc += (columns' components) x w, w[j] the factor of column j and tile row n
+    __device__ __forceinline__ void mac(const float* w, v4f* acc) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                acc[b * 4 + 0] = mfma1(v[j][b].x, w[j], acc[b * 4 + 0]);
+                acc[b * 4 + 1] = mfma1(v[j][b].y, w[j], acc[b * 4 + 1]);
+                acc[b * 4 + 2] = mfma1(v[j][b].z, w[j], acc[b * 4 + 2]);
+                acc[b * 4 + 3] = mfma1(v[j][b].w, w[j], acc[b * 4 + 3]);
+            }
+    }
+};
+
+template <int P>
+struct ColFrag<uint16_t, P> {
+    static constexpr int kW = P >= 128 ? 8 : 4, kBlocks = P / (16 * kW), kAcc = kBlocks * kW;
+    using Vec = unsigned __attribute__((ext_vector_type(kW / 2)));
+    Vec v[8][kBlocks];
+    template <typename F>
+    __device__ __forceinline__ void load(F&& row, int D, int n) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint16_t* p = row(j);
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const int d = b * 16 * kW + kW * n;
+                Vec z{};
+                if (d < D) z = *reinterpret_cast<const Vec*>(p + d);
+                v[j][b] = z;
+            }
+        }
+    }
+    // The factors as the sum of two bf16 values (16 bits): rounded to one they would add an
+    // error of the size of the result's own rounding.  The second product costs nothing next to
+    // reading the rows.
+    __device__ __forceinline__ void mac(const float* w, v4f* acc) const {
+        v4u hi, lo;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            hi[i] = bf16_pack(w[2 * i], w[2 * i + 1]);
+            lo[i] = bf16_pack(w[2 * i] - bf16_lo(hi[i]), w[2 * i + 1] - bf16_hi(hi[i]));
+        }
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int c = 0; c < kW; ++c) {
+                const unsigned sel = c & 1 ? 0x07060302u : 0x05040100u;
+                v4u a;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    a[i] = __builtin_amdgcn_perm(v[2 * i + 1][b][c / 2], v[2 * i][b][c / 2], sel);
+                acc[b * kW + c] = mfma_bf16(a, lo, acc[b * kW + c]);
+                acc[b * kW + c] = mfma_bf16(a, hi, acc[b * kW + c]);
+            }
+    }
+};
+
+__device__ __forceinline__ float attn_f32(float x) { return x; }
+__device__ __forceinline__ float attn_f32(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
+
+// The same sum with the columns of factor 0 left out, one column and component at a time: for
+// steps with infinities or NaN in a row that not every tile row has an edge to (0 times them
+// would be NaN).  Rare: it works on copies in memory, so that the callers' stay in registers.
+template <typename T, int P>
+__device__ __attribute__((noinline)) void mac_exact_mem(const float* w, const int* cols, float* acc,
+                                                        const T* base, int64_t stride, int D) {
+    constexpr int kW = ColFrag<T, P>::kW, kBlocks = ColFrag<T, P>::kBlocks;
+    const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+#pragma unroll 1
+    for (int j = 0; j < Attn<T>::kRowsPerLane; ++j)
+#pragma unroll 1
+        for (int gg = 0; gg < 4; ++gg) {
+            const float f = __shfl(w[j], gg * 16 + n);
+            const T* p = base + (int64_t)__shfl(cols[j], gg * 16) * stride;
+            if (f == 0.0f) continue;
+#pragma unroll 1
+            for (int i = 0; i < kBlocks * kW * 4; ++i) {
+                const int b = i / (kW * 4), c = i / 4 % kW, r = i % 4;
+                const int d = b * 16 * kW + kW * (4 * g + r) + c;
+                if (d < D) acc[i] = fmaf(f, attn_f32(p[d]), acc[i]);
+            }
+        }
+}
+template <typename T, int P>
+__device__ __forceinline__ void mac_exact(const float* w, const int* cols, v4f* acc, const T* base,
+                                          int64_t stride, int D) {
+    constexpr int kN = ColFrag<T, P>::kAcc, kR = Attn<T>::kRowsPerLane;
+    float t[kN * 4], tw[kR];
+    int tc[kR];
+#pragma unroll
+    for (int i = 0; i < kN * 4; ++i) t[i] = acc[i / 4][i % 4];
+#pragma unroll
+    for (int i = 0; i < kR; ++i) tw[i] = w[i], tc[i] = cols[i];
+    mac_exact_mem<T, P>(tw, tc, t, base, stride, D);
+#pragma unroll
+    for (int i = 0; i < kN * 4; ++i) acc[i / 4][i % 4] = t[i];
+}
+
+template <int N>
+__device__ __forceinline__ bool any_not_finite(const v4f* acc) {
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t = fmaf(acc[i][r], 0.0f, t);
+    return __any(t != 0.0f);
+}
+
+template <int W>
+__device__ __forceinline__ void attn_store_w(uint16_t* p, const float* v) {
+    if constexpr (W == 8)
+        *reinterpret_cast<v4u*>(p) = v4u{bf16_pack(v[0], v[1]), bf16_pack(v[2], v[3]),
+                                         bf16_pack(v[4], v[5]), bf16_pack(v[6], v[7])};
+    else
+        *reinterpret_cast<uint2*>(p) = make_uint2(bf16_pack(v[0], v[1]), bf16_pack(v[2], v[3]));
+}
+template <int W>
+__device__ __forceinline__ void attn_store_w(float* p, const float* v) {
+#pragma unroll
+    for (int i = 0; i < W; i += 4)
+        *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+}
+
+// f times a tile row's sums to its row of results (T, or fp32 for the parts of a cut tile).
+template <typename T, int P, typename O>
+__device__ __forceinline__ void store_rows(O* row, const v4f* acc, float f, int D, int g) {
+    constexpr int kW = ColFrag<T, P>::kW, kBlocks = ColFrag<T, P>::kBlocks;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int d = b * 16 * kW + kW * (4 * g + r);
+            float v[kW];
+#pragma unroll
+            for (int c = 0; c < kW; ++c) v[c] = acc[b * kW + c][r] * f;
+            if (d < D) attn_store_w<kW>(row + d, v);
+        }
+}
+
+// A step of an item: columns it * 16 kTiles .. of the item's chunks.
+template <typename T>
+struct Step {
+    int row[Attn<T>::kTiles];               // column whose row form this lane holds, per tile
+    int col[Attn<T>::kRowsPerLane];         // columns whose column form this lane holds
+    uint32_t mask;                          // tile row n: the step's edges, bit 16 t + 4 g + r
+    __device__ __forceinline__ void load(const AttnSide& s, int chunk, int it, int n, int g) {
+        constexpr int kT = Attn<T>::kTiles;
+        const int c = chunk + it * kT / 2, half = kT == 2 ? 0 : it & 1;
+        const int* ids = s.ids + (int64_t)c * kAttnCols + half * 16;
+        const uint32_t m = s.masks[(int64_t)c * kAttnRows + n];
+        mask = kT == 2 ? m : (m >> (half * 16)) & 0xffffu;
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+            row[t] = ids[16 * t + n];
+            const int4 q = *reinterpret_cast<const int4*>(ids + 16 * t + 4 * g);
+            col[4 * t] = q.x;
+            col[4 * t + 1] = q.y;
+            col[4 * t + 2] = q.z;
+            col[4 * t + 3] = q.w;
+        }
+    }
+    // place of pair (n, 16 t + 4 g + r) along row n's edges of this step
+    __device__ __forceinline__ int nth(int bit) const {
+        return __popc(mask & ((1u << bit) - 1u));
+    }
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+inline AttnSide side_args(const batmobile_attention_side& s, const int32_t* eid) {
+    const PlanLayout p = plan_layout(s.n_rows, s.n_edges);
+    AttnSide a;
+    a.rows = s.plan + p.rows;
+    a.tile_part = s.plan + p.tile_part;
+    a.items = reinterpret_cast<const int4*>(s.plan + p.items);
+    a.base = s.plan + p.base;
+    a.masks = reinterpret_cast<const uint32_t*>(s.plan + p.masks);
+    a.ids = s.plan + p.ids;
+    a.eid = eid;
+    a.n_items = s.n_items;
+    a.n_tiles = (int)p.tiles;
+    return a;
+}
+
+inline bool attn_shape_ok(const batmobile_attention_side& s, int H, int Hkv, int Dk, int Dv,
+                          int dtype) {
+    return s.n_rows >= 0 && s.n_cols >= 0 && s.n_edges >= 0 && (s.n_rows == 0 || s.plan) &&
+           s.n_items >= 0 && s.n_parts >= 0 && H > 0 && H <= 65535 && Hkv > 0 && H % Hkv == 0 &&
+           Dk > 0 && Dv > 0 && Dk <= 256 && Dv <= 256 && (dtype == 0 || dtype == 1) &&
+           (s.n_edges == 0 || s.n_cols > 0) && s.n_rows < INT32_MAX / 2 &&
+           s.n_edges < INT32_MAX / 4 &&
+           (int64_t)s.n_items * H < (int64_t)1 << 32;
+}
+
+}  // namespace bmhip

@@ -1,249 +1,253 @@
-// Softmax attention of every row (destination) over its neighbours (sources), forward and
-// backward, on the edge list of a graph (no reference counterpart: the reference sums its
-// messages, src/message_passing/fused_message_passing.cu).
+// Softmax attention of every row (destination) over its neighbours (sources) on the edges of a
+// graph, forward (no reference counterpart: the reference sums its messages,
+// src/message_passing/fused_message_passing.cu).
 //
 //   x_eh = scale <q[i,h], k[j,g]> + b[e,h]      edge e: j -> i, g = h / (H / H_kv)
 //   p_eh = exp(x_eh - m_ih) / l_ih              m, l: maximum and sum of exponentials over
-//                                               the edges of row i (b = -inf: no edge)
-//   o_ih = sum_e p_eh v[j,g]                    a row without an edge: o = 0
+//                                               the edges of row i
+//   o_ih = sum_e p_eh v[j,g]
 //
-// and, with go the gradient of o,
+// An edge whose b or x is -inf is left out; a row without an edge gives o = 0.
 //
-//   dp_eh = <go[i,h], v[j,g]>,  D_ih = sum_e p_eh dp_eh,  ds_eh = p_eh (dp_eh - D_ih)
-//   gb = ds,  gq[i,h] = scale sum_e ds k[j,g],  gk[j,g] = scale sum ds q[i,h],
-//   gv[j,g] = sum p go[i,h]
-//
-// One wave per (row, head): a lane holds components lane, lane + 64, ... of the head.
-#include "common.h"
-#include "batmobile_hip.h"
+// One pass over a tile's columns (attention.h) with the running maximum and sum.  x is formed in
+// natural units and the maximum taken off before the factor log2 e, so that a bias of the
+// type's lowest value does not become infinite.
+#include "attention.h"
 
 namespace bmhip {
 
-constexpr int kAttnMaxPer = 4;  // components per lane: head sizes up to 256
-
-template <typename T>
-__device__ __forceinline__ float attn_ld(const T* p);
-template <>
-__device__ __forceinline__ float attn_ld<float>(const float* p) { return *p; }
-template <>
-__device__ __forceinline__ float attn_ld<uint16_t>(const uint16_t* p) {
-    return __uint_as_float((uint32_t)*p << 16);
-}
-__device__ __forceinline__ void attn_st(float* p, float v) { *p = v; }
-__device__ __forceinline__ void attn_st(uint16_t* p, float v) {
-    *p = (uint16_t)(bf16_pack(v, 0.0f) & 0xffffu);
-}
-
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-
-struct AttnArgs {
-    const void *q, *k, *v, *go;
+struct AttnFwd {
+    AttnSide side;
+    const void *q, *k, *v;
     const float* bias;
-    const int64_t *row_ptr, *col, *eid;        // edges of a row: [row_ptr[i], row_ptr[i + 1])
-    const int64_t *src_ptr, *src_dst, *src_pos;  // of a source: its destinations, edge positions
-    void *out, *gq, *gk, *gv;
-    float *stats, *gbias;
-    float2* ws;                                // [E, H]: p, ds
-    int64_t n_dst, n_src, qs, ks, vs, gs;      // rows' strides in elements
-    int H, Hkv, Dk, Dv;
+    void* out;
+    float *stats;                          // [n_dst, H, 2]
+    float *part_o, *part_ml;               // [parts, H, 16, Dv], [parts, H, 16, 2]
+    int64_t qs, ks, vs;
+    int H, group, Dk, Dv;
     float scale;
 };
 
-template <typename T>
-__global__ __launch_bounds__(256) void attn_fwd_kernel(AttnArgs a) {
-    const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (u >= a.n_dst * a.H) return;
-    const int lane = threadIdx.x & 63, h = (int)(u % a.H), g = h / (a.H / a.Hkv);
-    const int64_t i = u / a.H;
-    const T* q = (const T*)a.q + i * a.qs + (int64_t)h * a.Dk;
-    float qr[kAttnMaxPer], o[kAttnMaxPer], m = -__builtin_inff(), l = 0.0f;
-    for (int c = 0; c < kAttnMaxPer; ++c) {
-        qr[c] = c * 64 + lane < a.Dk ? attn_ld(q + c * 64 + lane) : 0.0f;
-        o[c] = 0.0f;
+template <typename T, int KP, int VP>
+__global__ __launch_bounds__(256) void attn_fwd_kernel(AttnFwd a) {
+    constexpr int kT = Attn<T>::kTiles, kR = Attn<T>::kRowsPerLane;
+    constexpr float kInf = __builtin_inff();
+    const int64_t u = attn_unit((int64_t)a.side.n_items * a.H);
+    if (u < 0) return;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int item = (int)(u / a.H), h = (int)(u % a.H), kv = h / a.group;
+    const int4 it4 = a.side.items[item];
+    const int row = a.side.rows[it4.x * kAttnRows + n];
+    const int steps = it4.z * 2 / kT;
+    const T* kbase = (const T*)a.k + (int64_t)kv * a.Dk;
+    const T* vbase = (const T*)a.v + (int64_t)kv * a.Dv;
+    RowFrag<T, KP> q;
+    q.zero();
+    if (row >= 0) q.load(row_of<T>(a.q, row, a.qs) + (int64_t)h * a.Dk, a.Dk, g);
+
+    v4f acc[ColFrag<T, VP>::kAcc];
+    float m, l;
+    for (int exact = 0;; ++exact) {
+        m = -kInf;
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < ColFrag<T, VP>::kAcc; ++i) acc[i] = v4f{0, 0, 0, 0};
+        int edge = a.side.base[item * kAttnRows + n];
+        Step<T> st;
+        RowFrag<T, KP> kf[kT];
+        if (steps > 0) {
+            st.load(a.side, it4.y, 0, n, g);
+#pragma unroll
+            for (int t = 0; t < kT; ++t) kf[t].load(row_of<T>(kbase, st.row[t], a.ks), a.Dk, g);
+        }
+        for (int i = 0; i < steps; ++i) {
+            // loads in flight: this step's v and bias over the first product, the next step's
+            // k over the softmax and the second product
+            ColFrag<T, VP> vf;
+            vf.load([&](int j) { return row_of<T>(vbase, st.col[j], a.vs); }, a.Dv, n);
+            float b[4 * kT];
+#pragma unroll
+            for (int j = 0; j < 4 * kT; ++j) {
+                const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
+                b[j] = -kInf;
+                if ((st.mask >> bit) & 1) {
+                    b[j] = 0.0f;
+                    if (a.bias) {
+                        int e = edge + st.nth(bit);
+                        if (a.side.eid) e = a.side.eid[e];
+                        b[j] = a.bias[(int64_t)e * a.H + h];
+                    }
+                }
+            }
+            edge += __popc(st.mask);
+            Step<T> next;
+            next.load(a.side, it4.y, min(i + 1, steps - 1), n, g);
+            float x[4 * kT];
+#pragma unroll
+            for (int t = 0; t < kT; ++t) {
+                const v4f s = row_product<T, KP>(kf[t], q);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[4 * t + r] = s[r];
+            }
+#pragma unroll
+            for (int t = 0; t < kT; ++t) kf[t].load(row_of<T>(kbase, next.row[t], a.ks), a.Dk, g);
+            float top = m;
+#pragma unroll
+            for (int j = 0; j < 4 * kT; ++j) {
+                x[j] = b[j] == -kInf ? -kInf : fmaf(x[j], a.scale, b[j]);
+                top = fmaxf(top, x[j]);
+            }
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float ref = top == -kInf ? 0.0f : top;
+            if (__any(top > m)) {
+                const float f = exp2f((m - ref) * kLog2e);
+                l *= f;
+#pragma unroll
+                for (int j = 0; j < ColFrag<T, VP>::kAcc; ++j) acc[j] *= f;
+                m = top;
+            }
+            float p[4 * kT];
+#pragma unroll
+            for (int j = 0; j < 4 * kT; ++j) {
+                p[j] = exp2f((x[j] - ref) * kLog2e);
+                l += p[j];
+            }
+            if (exact) mac_exact<T, VP>(p, st.col, acc, vbase, a.vs, a.Dv);
+            else vf.mac(p, acc);
+            st = next;
+        }
+        // infinities or NaN: the sums once more, each row over its own edges alone
+        if (exact || !any_not_finite<ColFrag<T, VP>::kAcc>(acc)) break;
     }
-    for (int64_t e = a.row_ptr[i]; e < a.row_ptr[i + 1]; ++e) {
-        const int64_t j = a.col[e];
-        const float b = a.bias ? a.bias[(a.eid ? a.eid[e] : e) * a.H + h] : 0.0f;
-        if (b == -__builtin_inff()) continue;
-        const T* k = (const T*)a.k + j * a.ks + (int64_t)g * a.Dk;
-        float s = 0.0f;
-        for (int c = 0; c < kAttnMaxPer; ++c)
-            if (c * 64 + lane < a.Dk) s = fmaf(qr[c], attn_ld(k + c * 64 + lane), s);
-        const float x = wave_sum(s) * a.scale + b;
-        if (x == -__builtin_inff()) continue;
-        const float mn = fmaxf(m, x);
-        const float al = m == mn ? 1.0f : __expf(m - mn), p = __expf(x - mn);
-        m = mn;
-        l = l * al + p;
-        const T* v = (const T*)a.v + j * a.vs + (int64_t)g * a.Dv;
-        for (int c = 0; c < kAttnMaxPer; ++c)
-            if (c * 64 + lane < a.Dv) o[c] = fmaf(p, attn_ld(v + c * 64 + lane), o[c] * al);
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (row < 0) return;
+    if (it4.w >= 0) {
+        const int64_t at = ((int64_t)it4.w * a.H + h) * kAttnRows + n;
+        store_rows<T, VP>(a.part_o + at * a.Dv, acc, 1.0f, a.Dv, g);
+        if (g == 0) {
+            a.part_ml[at * 2] = m;
+            a.part_ml[at * 2 + 1] = l;
+        }
+        return;
     }
-    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-    T* out = (T*)a.out + (i * a.H + h) * (int64_t)a.Dv;
-    for (int c = 0; c < kAttnMaxPer; ++c)
-        if (c * 64 + lane < a.Dv) attn_st(out + c * 64 + lane, o[c] * inv);
-    if (a.stats && lane == 0) {
-        a.stats[u * 2] = m;
-        a.stats[u * 2 + 1] = l;
+    const int64_t at = (int64_t)row * a.H + h;
+    // l is 0 only without an edge; a NaN stays one
+    store_rows<T, VP>((T*)a.out + at * a.Dv, acc, l == 0.0f ? 0.0f : 1.0f / l, a.Dv, g);
+    if (a.stats && g == 0) {
+        a.stats[at * 2] = m;
+        a.stats[at * 2 + 1] = l;
     }
 }
 
-// gq, gbias and the edges' p and ds: a first pass over the row's edges for p, dp and D
+// Joins the parts of a cut tile, row by row: workgroup p of the parts takes rows p, p + parts of
+// its tile, ...; its waves take the parts in turn, a lane four components.
 template <typename T>
-__global__ __launch_bounds__(256) void attn_bwd_dst_kernel(AttnArgs a) {
-    const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (u >= a.n_dst * a.H) return;
-    const int lane = threadIdx.x & 63, h = (int)(u % a.H), g = h / (a.H / a.Hkv);
-    const int64_t i = u / a.H;
-    const T* q = (const T*)a.q + i * a.qs + (int64_t)h * a.Dk;
-    const T* go = (const T*)a.go + i * a.gs + (int64_t)h * a.Dv;
-    const float m = a.stats[u * 2], l = a.stats[u * 2 + 1];
-    float qr[kAttnMaxPer], gr[kAttnMaxPer], gq[kAttnMaxPer], D = 0.0f;
-    for (int c = 0; c < kAttnMaxPer; ++c) {
-        qr[c] = c * 64 + lane < a.Dk ? attn_ld(q + c * 64 + lane) : 0.0f;
-        gr[c] = c * 64 + lane < a.Dv ? attn_ld(go + c * 64 + lane) : 0.0f;
-        gq[c] = 0.0f;
-    }
-    const int64_t e0 = a.row_ptr[i], e1 = a.row_ptr[i + 1];
-    for (int64_t e = e0; e < e1; ++e) {
-        const int64_t j = a.col[e];
-        const float b = a.bias ? a.bias[(a.eid ? a.eid[e] : e) * a.H + h] : 0.0f;
-        float p = 0.0f, dp = 0.0f;
-        if (b != -__builtin_inff()) {
-            const T* k = (const T*)a.k + j * a.ks + (int64_t)g * a.Dk;
-            const T* v = (const T*)a.v + j * a.vs + (int64_t)g * a.Dv;
-            float s = 0.0f;
-            for (int c = 0; c < kAttnMaxPer; ++c) {
-                if (c * 64 + lane < a.Dk) s = fmaf(qr[c], attn_ld(k + c * 64 + lane), s);
-                if (c * 64 + lane < a.Dv) dp = fmaf(gr[c], attn_ld(v + c * 64 + lane), dp);
-            }
-            const float x = wave_sum(s) * a.scale + b;
-            dp = wave_sum(dp);
-            if (x != -__builtin_inff()) {
-                p = __expf(x - m) / l;
-                D += p * dp;
-            }
-        }
-        if (lane == 0) a.ws[e * a.H + h] = make_float2(p, dp);
-    }
-    __threadfence_block();
-    for (int64_t e = e0; e < e1; ++e) {
-        const float2 w = a.ws[e * a.H + h];
-        const float b = a.bias ? a.bias[(a.eid ? a.eid[e] : e) * a.H + h] : 0.0f;
-        const bool live = b != -__builtin_inff();
-        const float ds = live ? w.x * (w.y - D) : 0.0f;
-        const T* k = (const T*)a.k + a.col[e] * a.ks + (int64_t)g * a.Dk;
-        for (int c = 0; c < kAttnMaxPer; ++c)
-            if (live && c * 64 + lane < a.Dk)
-                gq[c] = fmaf(ds, attn_ld(k + c * 64 + lane), gq[c]);
-        if (lane == 0) {
-            a.ws[e * a.H + h].y = ds;
-            if (a.gbias) a.gbias[(a.eid ? a.eid[e] : e) * a.H + h] = ds;
-        }
-    }
-    T* out = (T*)a.gq + (i * a.H + h) * (int64_t)a.Dk;
-    for (int c = 0; c < kAttnMaxPer; ++c)
-        if (c * 64 + lane < a.Dk) attn_st(out + c * 64 + lane, gq[c] * a.scale);
-}
-
-// gk, gv of one source and key/value head
-template <typename T>
-__global__ __launch_bounds__(256) void attn_bwd_src_kernel(AttnArgs a) {
-    const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (u >= a.n_src * a.Hkv) return;
-    const int lane = threadIdx.x & 63, g = (int)(u % a.Hkv), G = a.H / a.Hkv;
-    const int64_t j = u / a.Hkv;
-    float gk[kAttnMaxPer], gv[kAttnMaxPer];
-    for (int c = 0; c < kAttnMaxPer; ++c) gk[c] = gv[c] = 0.0f;
-    for (int64_t t = a.src_ptr[j]; t < a.src_ptr[j + 1]; ++t) {
-        const int64_t i = a.src_dst[t], e = a.src_pos[t];
-        for (int h = g * G; h < g * G + G; ++h) {
-            const float b = a.bias ? a.bias[(a.eid ? a.eid[e] : e) * a.H + h] : 0.0f;
-            if (b == -__builtin_inff()) continue;
-            const float2 w = a.ws[e * a.H + h];
-            const T* q = (const T*)a.q + i * a.qs + (int64_t)h * a.Dk;
-            const T* go = (const T*)a.go + i * a.gs + (int64_t)h * a.Dv;
-            for (int c = 0; c < kAttnMaxPer; ++c) {
-                if (c * 64 + lane < a.Dk)
-                    gk[c] = fmaf(w.y, attn_ld(q + c * 64 + lane), gk[c]);
-                if (c * 64 + lane < a.Dv)
-                    gv[c] = fmaf(w.x, attn_ld(go + c * 64 + lane), gv[c]);
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnFwd a) {
+    __shared__ float sm[4], sl[4], so[4][256];
+    const int h = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    int first, parts;
+    const int tile = tile_of_part(a.side, blockIdx.x, first, parts);
+    for (int slot = (int)blockIdx.x - first; slot < kAttnRows; slot += parts) {
+        const int row = a.side.rows[tile * kAttnRows + slot];
+        if (row < 0) continue;
+        __syncthreads();
+        constexpr float kInf = __builtin_inff();
+        auto at = [&](int p) { return ((int64_t)(first + p) * a.H + h) * kAttnRows + slot; };
+        float m = -kInf;
+        for (int p = threadIdx.x; p < parts; p += 256) m = fmaxf(m, a.part_ml[at(p) * 2]);
+    #pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        if (lane == 0) sm[w] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+        const float ref = m == -kInf ? 0.0f : m;
+        float l = 0.0f, o[4] = {0, 0, 0, 0};
+        for (int p = w; p < parts; p += 4) {
+            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at(p) * 2);
+            const float f = exp2f((ml.x - ref) * kLog2e);
+            l = fmaf(ml.y, f, l);
+            if (4 * lane < a.Dv) {
+                const float4 x = *reinterpret_cast<const float4*>(a.part_o + at(p) * a.Dv + 4 * lane);
+                // a part without an edge of this row holds zeros, and the factor 0
+                o[0] = fmaf(x.x, f, o[0]);
+                o[1] = fmaf(x.y, f, o[1]);
+                o[2] = fmaf(x.z, f, o[2]);
+                o[3] = fmaf(x.w, f, o[3]);
             }
         }
-    }
-    T* ok = (T*)a.gk + (j * a.Hkv + g) * (int64_t)a.Dk;
-    T* ov = (T*)a.gv + (j * a.Hkv + g) * (int64_t)a.Dv;
-    for (int c = 0; c < kAttnMaxPer; ++c) {
-        if (c * 64 + lane < a.Dk) attn_st(ok + c * 64 + lane, gk[c] * a.scale);
-        if (c * 64 + lane < a.Dv) attn_st(ov + c * 64 + lane, gv[c]);
+        if (lane == 0) sl[w] = l;
+    #pragma unroll
+        for (int c = 0; c < 4; ++c) so[w][4 * lane + c] = o[c];
+        __syncthreads();
+        if (w != 0) continue;
+        l = sl[0] + sl[1] + sl[2] + sl[3];
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const int64_t to = (int64_t)row * a.H + h;
+    #pragma unroll
+        for (int c = 0; c < 4; ++c)
+            o[c] = (so[0][4 * lane + c] + so[1][4 * lane + c] + so[2][4 * lane + c] +
+                    so[3][4 * lane + c]) * inv;
+        if (4 * lane < a.Dv) attn_store_w<4>((T*)a.out + to * a.Dv + 4 * lane, o);
+        if (a.stats && lane == 0) {
+            a.stats[to * 2] = m;
+            a.stats[to * 2 + 1] = l;
+        }
     }
 }
 
-static bool attn_shape_ok(int64_t n_dst, int64_t n_src, int64_t n_edges, int H, int Hkv, int Dk,
-                          int Dv, int dtype) {
-    return n_dst >= 0 && n_src >= 0 && n_edges >= 0 && H > 0 && Hkv > 0 && H % Hkv == 0 &&
-           Dk > 0 && Dv > 0 && Dk <= 64 * kAttnMaxPer && Dv <= 64 * kAttnMaxPer &&
-           (n_edges == 0 || (n_src > 0 && n_dst > 0)) && (dtype == 0 || dtype == 1) &&
-           n_dst * (int64_t)H < ((int64_t)1 << 32) && n_src * (int64_t)Hkv < ((int64_t)1 << 32);
+template <typename T, int KP, int VP>
+static void attn_fwd_launch(const AttnFwd& a, hipStream_t s) {
+    attn_fwd_kernel<T, KP, VP><<<attn_grid((int64_t)a.side.n_items * a.H), 256, 0, s>>>(a);
+}
+template <typename T, int KP>
+static void attn_fwd_pick_v(const AttnFwd& a, hipStream_t s) {
+    if (a.Dv <= 64) attn_fwd_launch<T, KP, 64>(a, s);
+    else if (a.Dv <= 128) attn_fwd_launch<T, KP, 128>(a, s);
+    else attn_fwd_launch<T, KP, 256>(a, s);
+}
+template <typename T>
+static void attn_fwd_run(const AttnFwd& a, int parts, hipStream_t s) {
+    if (a.Dk <= 64) attn_fwd_pick_v<T, 64>(a, s);
+    else if (a.Dk <= 128) attn_fwd_pick_v<T, 128>(a, s);
+    else attn_fwd_pick_v<T, 256>(a, s);
+    if (parts)
+        attn_join_kernel<T><<<dim3((unsigned)parts, (unsigned)a.H), 256, 0, s>>>(a);
 }
 
 }  // namespace bmhip
 
 using namespace bmhip;
 
-extern "C" int batteries_neighbor_attention(
-    const void* q, const void* k, const void* v, const float* bias, const int64_t* row_ptr,
-    const int64_t* col, const int64_t* eid, void* out, float* stats, int64_t n_dst, int64_t n_src,
-    int64_t n_edges, int H, int Hkv, int Dk, int Dv, int64_t q_stride, int64_t k_stride,
-    int64_t v_stride, float scale, int dtype, hipStream_t stream) {
-    if (!attn_shape_ok(n_dst, n_src, n_edges, H, Hkv, Dk, Dv, dtype)) return BM_ERR_ARG;
-    if (n_dst == 0) return BM_OK;
-    AttnArgs a{};
-    a.q = q; a.k = k; a.v = v; a.bias = bias; a.row_ptr = row_ptr; a.col = col; a.eid = eid;
-    a.out = out; a.stats = stats; a.n_dst = n_dst; a.n_src = n_src; a.H = H; a.Hkv = Hkv;
-    a.Dk = Dk; a.Dv = Dv; a.qs = q_stride; a.ks = k_stride; a.vs = v_stride; a.scale = scale;
-    const unsigned grid = (unsigned)ceil_div(n_dst * H, 4);
-    if (dtype == 0) attn_fwd_kernel<float><<<grid, 256, 0, stream>>>(a);
-    else attn_fwd_kernel<uint16_t><<<grid, 256, 0, stream>>>(a);
-    return (int)hipGetLastError();
+extern "C" size_t batteries_neighbor_attention_workspace_bytes(int64_t n_parts, int H, int Dv) {
+    if (n_parts <= 0 || H <= 0 || Dv <= 0) return 0;
+    return (size_t)n_parts * H * kAttnRows * (Dv + 2) * sizeof(float);
 }
 
-extern "C" size_t batteries_neighbor_attention_backward_workspace_bytes(int64_t n_edges, int H) {
-    return (size_t)(n_edges > 0 ? n_edges : 0) * (size_t)H * sizeof(float2);
-}
-
-extern "C" int batteries_neighbor_attention_backward(
-    const void* q, const void* k, const void* v, const float* bias, const float* stats,
-    const void* grad_out, const int64_t* row_ptr, const int64_t* col, const int64_t* eid,
-    const int64_t* src_ptr, const int64_t* src_dst, const int64_t* src_pos, void* grad_q,
-    void* grad_k, void* grad_v, float* grad_bias, int64_t n_dst, int64_t n_src, int64_t n_edges,
-    int H, int Hkv, int Dk, int Dv, int64_t q_stride, int64_t k_stride, int64_t v_stride,
-    int64_t go_stride, float scale, int dtype, void* workspace, size_t workspace_bytes,
-    hipStream_t stream) {
-    if (!attn_shape_ok(n_dst, n_src, n_edges, H, Hkv, Dk, Dv, dtype)) return BM_ERR_ARG;
-    if (workspace_bytes < batteries_neighbor_attention_backward_workspace_bytes(n_edges, H) ||
-        (n_edges > 0 && !workspace))
-        return BM_ERR_WORKSPACE;
-    AttnArgs a{};
-    a.q = q; a.k = k; a.v = v; a.go = grad_out; a.bias = bias; a.row_ptr = row_ptr; a.col = col;
-    a.eid = eid; a.src_ptr = src_ptr; a.src_dst = src_dst; a.src_pos = src_pos;
-    a.gq = grad_q; a.gk = grad_k; a.gv = grad_v; a.gbias = grad_bias;
-    a.stats = const_cast<float*>(stats); a.ws = (float2*)workspace;
-    a.n_dst = n_dst; a.n_src = n_src; a.H = H; a.Hkv = Hkv; a.Dk = Dk; a.Dv = Dv;
-    a.qs = q_stride; a.ks = k_stride; a.vs = v_stride; a.gs = go_stride; a.scale = scale;
-    const unsigned gd = (unsigned)ceil_div(n_dst * H, 4), gs = (unsigned)ceil_div(n_src * Hkv, 4);
-    if (gd) {
-        if (dtype == 0) attn_bwd_dst_kernel<float><<<gd, 256, 0, stream>>>(a);
-        else attn_bwd_dst_kernel<uint16_t><<<gd, 256, 0, stream>>>(a);
-    }
-    if (gs) {
-        if (dtype == 0) attn_bwd_src_kernel<float><<<gs, 256, 0, stream>>>(a);
-        else attn_bwd_src_kernel<uint16_t><<<gs, 256, 0, stream>>>(a);
-    }
+extern "C" int batteries_neighbor_attention(const void* q, const void* k, const void* v,
+                                            const float* bias, const int32_t* edge_id,
+                                            const batmobile_attention_side* side, void* out,
+                                            float* stats, int H, int Hkv, int Dk, int Dv,
+                                            int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                            float scale, int dtype, void* workspace,
+                                            size_t workspace_bytes, hipStream_t stream) {
+    if (!side || !attn_shape_ok(*side, H, Hkv, Dk, Dv, dtype)) return BM_ERR_ARG;
+    const int align = dtype == 0 ? 4 : 8;
+    if (Dk % align || Dv % align || q_stride % align || k_stride % align || v_stride % align ||
+        !aligned_to({q, k, v, out}, 16))
+        return BM_ERR_ARG;
+    if (side->n_rows == 0) return BM_OK;
+    const size_t need = batteries_neighbor_attention_workspace_bytes(side->n_parts, H, Dv);
+    if (workspace_bytes < need || (need && !workspace)) return BM_ERR_WORKSPACE;
+    AttnFwd a{};
+    a.side = side_args(*side, edge_id);
+    a.q = q; a.k = k; a.v = v; a.bias = bias; a.out = out; a.stats = stats;
+    a.part_o = (float*)workspace;
+    a.part_ml = a.part_o + (size_t)side->n_parts * H * kAttnRows * Dv;
+    a.qs = q_stride; a.ks = k_stride; a.vs = v_stride;
+    a.H = H; a.group = H / Hkv; a.Dk = Dk; a.Dv = Dv; a.scale = scale;
+    if (dtype == 0) attn_fwd_run<float>(a, side->n_parts, stream);
+    else attn_fwd_run<uint16_t>(a, side->n_parts, stream);
     return (int)hipGetLastError();
 }

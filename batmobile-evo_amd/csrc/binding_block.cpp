@@ -59,13 +59,74 @@ Tensor bytes_on(const Tensor& as, size_t n) {
 // attention
 // ---------------------------------------------------------------------------
 
-// [n, heads, D] with dense heads, any stride of the rows
-Tensor dense_heads(const Tensor& t) {
-    if (t.size(0) <= 1 || t.numel() == 0) return t.contiguous();
-    if (t.stride(2) == 1 && (t.size(1) == 1 || t.stride(1) == t.size(2)) &&
-        t.stride(0) >= t.size(1) * t.size(2))
-        return t;
-    return t.contiguous();
+// [n, heads, D] as the kernels read it: heads of a row dense, rows at any stride, everything in
+// units of 16 bytes.  Other layouts are copied; a head size that is no multiple of 16 bytes is
+// padded with zeros, which add nothing to a product.
+Tensor heads16(const Tensor& t) {
+    const int64_t unit = 16 / t.element_size(), D = t.size(2);
+    if (D % unit) return at::constant_pad_nd(t, {0, unit - D % unit}).contiguous();
+    const bool dense = t.stride(2) == 1 && (t.size(1) == 1 || t.stride(1) == D) &&
+                       (t.size(0) <= 1 || (t.stride(0) >= t.size(1) * D && t.stride(0) % unit == 0)) &&
+                       (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+    if (dense) return t;
+    const Tensor c = t.contiguous();
+    return reinterpret_cast<uintptr_t>(c.data_ptr()) & 15 ? c.clone(at::MemoryFormat::Contiguous)
+                                                          : c;
+}
+int64_t row_stride(const Tensor& t) {
+    return t.size(0) <= 1 ? t.size(1) * t.size(2) : t.stride(0);
+}
+// An output of head size D made in units of 16 bytes, and cut to D
+Tensor heads_like(const Tensor& as, int64_t n, int64_t heads, int64_t D) {
+    const int64_t unit = 16 / as.element_size();
+    return torch::empty({n, heads, (D + unit - 1) / unit * unit}, as.options());
+}
+Tensor cut_heads(const Tensor& t, int64_t D) {
+    return t.size(2) == D ? t : t.slice(2, 0, D).contiguous();
+}
+
+// A side of a plan: (plan, items, parts) as attention_plan returns them.
+batmobile_attention_side attn_side(const Tensor& plan, int64_t items, int64_t parts, int64_t rows,
+                                   int64_t cols, int64_t edges, const Tensor& as) {
+    TORCH_CHECK(plan.device() == as.device(), "the plan must be on ", as.device());
+    TORCH_CHECK(plan.scalar_type() == torch::kInt32 && plan.is_contiguous() &&
+                    (size_t)plan.numel() * 4 >= batteries_attention_plan_bytes(rows, edges),
+                "the plan is not one of this many rows and edges");
+    batmobile_attention_side s;
+    s.n_rows = rows, s.n_cols = cols, s.n_edges = edges;
+    s.plan = plan.data_ptr<int32_t>();
+    s.n_items = (int32_t)items, s.n_parts = (int32_t)parts;
+    return s;
+}
+const int32_t* opt_index32(const OptTensor& t, const Tensor& as, int64_t n, const char* name) {
+    if (!t) return nullptr;
+    TORCH_CHECK(t->device() == as.device() && t->scalar_type() == torch::kInt32 &&
+                    t->is_contiguous() && t->numel() == n,
+                name, " must be a contiguous int32 vector of ", n, " entries on ", as.device());
+    return t->data_ptr<int32_t>();
+}
+
+// (plan, items, parts, flags): waits for the GPU to read the numbers back
+std::tuple<Tensor, int64_t, int64_t, int64_t> attention_plan(const Tensor& row_ptr,
+                                                             const Tensor& col,
+                                                             const OptTensor& order,
+                                                             int64_t n_cols, bool check) {
+    TORCH_CHECK(row_ptr.is_cuda(), "row_ptr must be a CUDA tensor");
+    TORCH_CHECK(row_ptr.numel() >= 1, "row_ptr must have at least one entry");
+    const int64_t rows = row_ptr.numel() - 1, edges = col.numel();
+    const int64_t* rp = index_ptr(row_ptr, row_ptr, rows + 1, "row_ptr");
+    const int64_t* cp = index_ptr(col, row_ptr, edges, "col");
+    const int64_t* op = order ? index_ptr(*order, row_ptr, rows, "order") : nullptr;
+    const c10::DeviceGuard guard(row_ptr.device());
+    const size_t n = batteries_attention_plan_bytes(rows, edges);
+    TORCH_CHECK(n > 0 && n_cols >= 0, "attention_plan: up to 2^29 edges and 2^30 rows");
+    Tensor plan = torch::empty({(int64_t)(n / 4)}, row_ptr.options().dtype(torch::kInt32));
+    check_status(batteries_attention_plan(rp, cp, op, rows, n_cols, edges, check, plan.data_ptr(),
+                                          n, stream_of(row_ptr)),
+                 "attention_plan");
+    const Tensor head = plan.slice(0, 0, 4).cpu();
+    const int32_t* h = head.data_ptr<int32_t>();
+    return {plan, h[0], h[1], h[2]};
 }
 
 struct AttnShape {
@@ -100,35 +161,42 @@ AttnShape attn_shape(const Tensor& q, const Tensor& k, const Tensor& v, const Op
 }
 
 std::tuple<Tensor, Tensor> neighbor_attention(const Tensor& q_, const Tensor& k_, const Tensor& v_,
-                                              const OptTensor& bias_, const Tensor& row_ptr,
-                                              const Tensor& src, const OptTensor& eid,
-                                              double scale, bool keep_stats) {
-    const AttnShape s = attn_shape(q_, k_, v_, bias_, src.numel());
+                                              const OptTensor& bias_, const Tensor& plan,
+                                              int64_t items, int64_t parts, int64_t E,
+                                              const OptTensor& edge_id, double scale,
+                                              bool keep_stats) {
+    const AttnShape s = attn_shape(q_, k_, v_, bias_, E);
     const c10::DeviceGuard guard(q_.device());
-    const Tensor q = dense_heads(q_), k = dense_heads(k_), v = dense_heads(v_);
+    const batmobile_attention_side side = attn_side(plan, items, parts, s.n_dst, s.n_src, E, q_);
+    const int32_t* eid = opt_index32(edge_id, q_, E, "edge_id");
+    const Tensor q = heads16(q_), k = heads16(k_), v = heads16(v_);
     Tensor bias;
     if (bias_) bias = bias_->contiguous();
-    const int64_t* rp = index_ptr(row_ptr, q, s.n_dst + 1, "row_ptr");
-    const int64_t* col = index_ptr(src, q, s.E, "src");
-    const int64_t* ep = eid ? index_ptr(*eid, q, s.E, "edge_id") : nullptr;
-    Tensor out = torch::empty({s.n_dst, s.H, s.Dv}, q.options()), stats;
+    const Tensor out = heads_like(q, s.n_dst, s.H, s.Dv);
+    Tensor stats;
     if (keep_stats) stats = torch::empty({s.n_dst, s.H, 2}, q.options().dtype(torch::kFloat32));
+    const int Dk = (int)q.size(2), Dv = (int)v.size(2);
+    const size_t wsb = batteries_neighbor_attention_workspace_bytes(parts, s.H, Dv);
+    Tensor ws;
+    if (wsb) ws = bytes_on(q, wsb);
     check_status(batteries_neighbor_attention(
                      q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                     bias.defined() ? bias.data_ptr<float>() : nullptr, rp, col, ep,
-                     out.data_ptr(), keep_stats ? stats.data_ptr<float>() : nullptr, s.n_dst,
-                     s.n_src, s.E, s.H, s.Hkv, s.Dk, s.Dv, q.stride(0), k.stride(0), v.stride(0),
-                     (float)scale, s.dtype, stream_of(q)),
+                     bias.defined() ? bias.data_ptr<float>() : nullptr, eid, &side,
+                     out.data_ptr(), keep_stats ? stats.data_ptr<float>() : nullptr, s.H, s.Hkv,
+                     Dk, Dv, row_stride(q), row_stride(k), row_stride(v), (float)scale, s.dtype,
+                     wsb ? ws.data_ptr() : nullptr, wsb, stream_of(q)),
                  "neighbor_attention");
-    return {out, stats};
+    return {cut_heads(out, s.Dv), stats};
 }
 
+// src_*: the side of the sources, src_pos the position of its edges in the destinations' order
 std::tuple<Tensor, Tensor, Tensor, Tensor> neighbor_attention_backward(
     const Tensor& q_, const Tensor& k_, const Tensor& v_, const OptTensor& bias_,
-    const Tensor& stats, const Tensor& grad_, const Tensor& row_ptr, const Tensor& src,
-    const OptTensor& eid, const Tensor& src_ptr, const Tensor& src_dst, const Tensor& src_pos,
-    double scale, bool need_bias) {
-    const AttnShape s = attn_shape(q_, k_, v_, bias_, src.numel());
+    const Tensor& stats, const Tensor& grad_, const Tensor& row_ptr, const Tensor& plan,
+    int64_t items, int64_t parts, const OptTensor& edge_id, const Tensor& src_plan,
+    int64_t src_items, int64_t src_parts, const Tensor& src_pos, double scale, bool need_bias) {
+    const int64_t E = src_pos.numel();
+    const AttnShape s = attn_shape(q_, k_, v_, bias_, E);
     check_like(grad_, q_, "grad_out");
     TORCH_CHECK(grad_.dim() == 3 && grad_.size(0) == s.n_dst && grad_.size(1) == s.H &&
                     grad_.size(2) == s.Dv,
@@ -137,32 +205,33 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> neighbor_attention_backward(
     TORCH_CHECK(stats.is_contiguous() && stats.numel() == s.n_dst * s.H * 2,
                 "stats must be [N_dst, H, 2]");
     const c10::DeviceGuard guard(q_.device());
-    const Tensor q = dense_heads(q_), k = dense_heads(k_), v = dense_heads(v_),
-                 go = dense_heads(grad_);
+    const batmobile_attention_side dst = attn_side(plan, items, parts, s.n_dst, s.n_src, E, q_);
+    const batmobile_attention_side src =
+        attn_side(src_plan, src_items, src_parts, s.n_src, s.n_dst, E, q_);
+    const int32_t* eid = opt_index32(edge_id, q_, E, "edge_id");
+    const int32_t* pos = opt_index32(src_pos, q_, E, "src_pos");
+    const int64_t* rp = index_ptr(row_ptr, q_, s.n_dst + 1, "row_ptr");
+    const Tensor q = heads16(q_), k = heads16(k_), v = heads16(v_), go = heads16(grad_);
     Tensor bias, gbias;
     if (bias_) bias = bias_->contiguous();
     if (need_bias && bias_) gbias = torch::empty_like(bias);
-    const int64_t* rp = index_ptr(row_ptr, q, s.n_dst + 1, "row_ptr");
-    const int64_t* col = index_ptr(src, q, s.E, "src");
-    const int64_t* ep = eid ? index_ptr(*eid, q, s.E, "edge_id") : nullptr;
-    const int64_t* sp = index_ptr(src_ptr, q, s.n_src + 1, "src_ptr");
-    const int64_t* sd = index_ptr(src_dst, q, s.E, "src_dst");
-    const int64_t* ss = index_ptr(src_pos, q, s.E, "src_pos");
-    Tensor gq = torch::empty({s.n_dst, s.H, s.Dk}, q.options());
-    Tensor gk = torch::empty({s.n_src, s.Hkv, s.Dk}, q.options());
-    Tensor gv = torch::empty({s.n_src, s.Hkv, s.Dv}, q.options());
-    const size_t wsb = batteries_neighbor_attention_backward_workspace_bytes(s.E, s.H);
+    const Tensor gq = heads_like(q, s.n_dst, s.H, s.Dk);
+    const Tensor gk = heads_like(q, s.n_src, s.Hkv, s.Dk);
+    const Tensor gv = heads_like(q, s.n_src, s.Hkv, s.Dv);
+    const int Dk = (int)q.size(2), Dv = (int)v.size(2);
+    const size_t wsb = batteries_neighbor_attention_backward_workspace_bytes(
+        E, parts, src_parts, s.H, s.Hkv, Dk, Dv);
     const Tensor ws = bytes_on(q, wsb);
     check_status(
         batteries_neighbor_attention_backward(
             q.data_ptr(), k.data_ptr(), v.data_ptr(),
             bias.defined() ? bias.data_ptr<float>() : nullptr, stats.data_ptr<float>(),
-            go.data_ptr(), rp, col, ep, sp, sd, ss, gq.data_ptr(), gk.data_ptr(), gv.data_ptr(),
-            gbias.defined() ? gbias.data_ptr<float>() : nullptr, s.n_dst, s.n_src, s.E, s.H, s.Hkv,
-            s.Dk, s.Dv, q.stride(0), k.stride(0), v.stride(0), go.stride(0), (float)scale, s.dtype,
+            go.data_ptr(), rp, eid, &dst, &src, pos, gq.data_ptr(), gk.data_ptr(), gv.data_ptr(),
+            gbias.defined() ? gbias.data_ptr<float>() : nullptr, s.H, s.Hkv, Dk, Dv,
+            row_stride(q), row_stride(k), row_stride(v), row_stride(go), (float)scale, s.dtype,
             ws.data_ptr(), wsb, stream_of(q)),
         "neighbor_attention_backward");
-    return {gq, gk, gv, gbias};
+    return {cut_heads(gq, s.Dk), cut_heads(gk, s.Dk), cut_heads(gv, s.Dv), gbias};
 }
 
 // ---------------------------------------------------------------------------
@@ -356,14 +425,19 @@ std::tuple<Tensor, std::vector<Tensor>> clip_grad_norm(
 
 void register_block_ops(pybind11::module_& m) {
     namespace py = pybind11;
+    m.def("attention_plan", &attention_plan, py::arg("row_ptr"), py::arg("col"),
+          py::arg("order"), py::arg("n_cols"), py::arg("check") = true,
+          "tiles of a graph side for the attention -> (plan, items, parts, flags)");
     m.def("neighbor_attention", &neighbor_attention, py::arg("q"), py::arg("k"), py::arg("v"),
-          py::arg("bias"), py::arg("row_ptr"), py::arg("src"), py::arg("edge_id"),
-          py::arg("scale"), py::arg("keep_stats") = false,
+          py::arg("bias"), py::arg("plan"), py::arg("items"), py::arg("parts"),
+          py::arg("num_edges"), py::arg("edge_id"), py::arg("scale"),
+          py::arg("keep_stats") = false,
           "softmax attention over the edges of each row -> (out, stats or None)");
     m.def("neighbor_attention_backward", &neighbor_attention_backward, py::arg("q"), py::arg("k"),
           py::arg("v"), py::arg("bias"), py::arg("stats"), py::arg("grad_out"),
-          py::arg("row_ptr"), py::arg("src"), py::arg("edge_id"), py::arg("src_ptr"),
-          py::arg("src_dst"), py::arg("src_pos"), py::arg("scale"), py::arg("need_bias") = true,
+          py::arg("row_ptr"), py::arg("plan"), py::arg("items"), py::arg("parts"),
+          py::arg("edge_id"), py::arg("src_plan"), py::arg("src_items"), py::arg("src_parts"),
+          py::arg("src_pos"), py::arg("scale"), py::arg("need_bias") = true,
           "(grad_q, grad_k, grad_v, grad_bias or None)");
     m.def("gated_residual_norm", &gated_residual_norm, py::arg("x"), py::arg("y"),
           py::arg("gate"), py::arg("scale"), py::arg("weight_post"), py::arg("weight_pre"),

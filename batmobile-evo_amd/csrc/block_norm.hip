@@ -348,12 +348,6 @@ static bool norm_shape_ok(int64_t n, int C, int dtype) {
     return n >= 0 && C > 0 && C <= kNormMaxC && (dtype == 0 || dtype == 1) &&
            n < ((int64_t)1 << 31);
 }
-static bool aligned_to(std::initializer_list<const void*> ps, uintptr_t b) {
-    for (const void* p : ps)
-        if (reinterpret_cast<uintptr_t>(p) & (b - 1)) return false;
-    return true;
-}
-
 }  // namespace bmhip
 
 using namespace bmhip;

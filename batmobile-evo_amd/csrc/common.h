@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <initializer_list>
 #include <utility>
 
 #include "generated_tables.h"
@@ -429,6 +430,13 @@ constexpr int fwd_slot_pos(int q) {
 // small helpers
 // ---------------------------------------------------------------------------
 __host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Whether all pointers are multiples of b bytes (host).
+inline bool aligned_to(std::initializer_list<const void*> ps, uintptr_t b) {
+    for (const void* p : ps)
+        if (reinterpret_cast<uintptr_t>(p) & (b - 1)) return false;
+    return true;
+}
 
 // A wave-uniform 64-bit value in scalar registers.
 __device__ __forceinline__ int64_t uniform_i64(int64_t v) {

@@ -20,45 +20,45 @@ class AttentionPlan:
     """The edges of a graph as the attention kernels take them, made once per graph.
 
     src [E] int64 are the sources in the order of row_ptr [n_dst + 1] (edges grouped by
-    destination), ascending within a row.  order and src_order (permutations of the
-    destinations and of the sources; spatially near ones next to each other) only change the
-    speed.  from_edge_index takes edges in any order; bias rows are always in the caller's
-    order of the edges.  The arguments are checked on the GPU, which waits for it once.
+    destination), ascending within a row.  order and src_order are permutations of the
+    destinations and of the sources: 16 that follow each other form a tile, whose shared
+    neighbours are read once, so spatially near ones should be next to each other
+    (`spatial_order`); results only differ in the order of summation.  from_edge_index takes
+    edges in any order; bias rows are always in the caller's order of the edges.  Making a plan
+    waits for the GPU once.  validate=False leaves out the check of the arrays (the kernels then
+    rely on them).
     """
 
     def __init__(self, src, row_ptr, n_src=None, order=None, src_order=None, edge_id=None,
                  validate=True):
-        self.src, self.row_ptr, self.edge_id = src, row_ptr, edge_id
-        self.order, self.src_order = order, src_order
-        self.n_dst = row_ptr.numel() - 1
-        self.n_src = self.n_dst if n_src is None else int(n_src)
-        self._source_side = None
-        if validate:
-            self._validate()
-
-    def _validate(self):
-        for name in ("src", "row_ptr", "edge_id", "order", "src_order"):
-            t = getattr(self, name)
+        for name, t in (("src", src), ("row_ptr", row_ptr), ("order", order),
+                        ("src_order", src_order), ("edge_id", edge_id)):
             if t is None and name not in ("src", "row_ptr"):
                 continue
             if t.dtype != torch.int64 or t.dim() != 1 or not t.is_contiguous():
                 raise ValueError(f"AttentionPlan: {name} must be a contiguous int64 vector")
-            if t.device != self.src.device:
+            if t.device != src.device:
                 raise ValueError(f"AttentionPlan: {name} must be on the device of src")
-        e = self.src.numel()
-        step = self.row_ptr.diff()
-        ok = (step >= 0).all() & (self.row_ptr[0] == 0) & (self.row_ptr[-1] == e)
-        if e:
-            ok &= (self.src.min() >= 0) & (self.src.max() < self.n_src)
-        if not bool(ok):
-            raise ValueError("AttentionPlan: row_ptr must rise from 0 to E and src lie in "
-                             f"[0, {self.n_src})")
-        if e > 1:
-            first = torch.zeros(e + 1, dtype=torch.bool, device=self.src.device)
-            first[self.row_ptr] = True
-            if bool(((self.src[1:] < self.src[:-1]) & ~first[1:-1]).any()):
-                raise ValueError("AttentionPlan: src must ascend within a row (from_edge_index "
-                                 "takes edges in any order)")
+        self.src, self.row_ptr = src, row_ptr
+        self.n_dst = row_ptr.numel() - 1
+        self.n_src = self.n_dst if n_src is None else int(n_src)
+        self.edge_id = None if edge_id is None else edge_id.int()
+        self._src_order, self._source_side = src_order, None
+        if validate:
+            for name, t, n in (("order", order, self.n_dst), ("src_order", src_order, self.n_src)):
+                if t is not None and not torch.equal(t.sort()[0],
+                                                     torch.arange(n, device=t.device)):
+                    raise ValueError(f"AttentionPlan: {name} must be a permutation")
+        plan, items, parts, bad = _batmobile.attention_plan(row_ptr, src, order, self.n_src,
+                                                            validate)
+        if bad & 1:
+            raise ValueError("AttentionPlan: row_ptr must rise from 0 to the number of edges")
+        if bad & 2:
+            raise ValueError(f"AttentionPlan: src must lie in [0, {self.n_src})")
+        if bad & 4:
+            raise ValueError("AttentionPlan: src must ascend within a row (from_edge_index takes "
+                             "edges in any order)")
+        self.side = (plan, items, parts)
 
     @classmethod
     def from_edge_index(cls, edge_index, n_dst, n_src=None, order=None, src_order=None):
@@ -75,14 +75,17 @@ class AttentionPlan:
         return cls(src[edge_id], row_ptr, n_src, order, src_order, edge_id)
 
     def source_side(self):
-        """The edges grouped by source (for the backward; built on first use)."""
+        """The edges grouped by source, for the backward (built on first use): the side's plan
+        and the position of each of its edges among the destinations'."""
         if self._source_side is None:
             dst = torch.repeat_interleave(
                 torch.arange(self.n_dst, device=self.src.device), self.row_ptr.diff(),
                 output_size=self.src.numel())
             by, pos = torch.sort(self.src, stable=True)
             rows = torch.arange(self.n_src + 1, device=self.src.device)
-            self._source_side = (torch.searchsorted(by, rows), dst[pos], pos)
+            plan, items, parts, _ = _batmobile.attention_plan(
+                torch.searchsorted(by, rows), dst[pos], self._src_order, self.n_dst, False)
+            self._source_side = (plan, items, parts, pos.int())
         return self._source_side
 
 
@@ -92,7 +95,7 @@ class NeighborAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, plan, scale):
         train = any(ctx.needs_input_grad[:4])
-        out, stats = _batmobile.neighbor_attention(q, k, v, bias, plan.row_ptr, plan.src,
+        out, stats = _batmobile.neighbor_attention(q, k, v, bias, *plan.side, plan.src.numel(),
                                                    plan.edge_id, scale, train)
         ctx.save_for_backward(q, k, v, bias, stats)
         ctx.plan, ctx.scale = plan, scale
@@ -103,7 +106,7 @@ class NeighborAttentionFunction(torch.autograd.Function):
         q, k, v, bias, stats = ctx.saved_tensors
         plan = ctx.plan
         gq, gk, gv, gb = _batmobile.neighbor_attention_backward(
-            q, k, v, bias, stats, grad_out, plan.row_ptr, plan.src, plan.edge_id,
+            q, k, v, bias, stats, grad_out, plan.row_ptr, *plan.side, plan.edge_id,
             *plan.source_side(), ctx.scale, ctx.needs_input_grad[3])
         return gq, gk, gv, gb, None, None
 

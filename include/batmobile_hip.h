@@ -493,33 +493,54 @@ int batteries_mace_backward(const float* positions, const float* box, const floa
 /* ---------------------------------------------------------------------------
  * Softmax attention over the edges of a graph (no reference counterpart)
  *
- * Rows are destinations with their edges in row_ptr [n_dst + 1] order; col[e] is the source
- * (ascending within a row) and eid[e] (NULL: e) the row of `bias` and `grad_bias` of edge e.
- *   x_eh = scale <q[i,h], k[col e, h / (H / Hkv)]> + bias[eid e, h],   p = softmax over the row
- *   out[i,h] = sum_e p_eh v[col e, h / (H / Hkv)]
- * q [n_dst, H, Dk], k [n_src, Hkv, Dk], v [n_src, Hkv, Dv], out [n_dst, H, Dv] in fp32
- * (dtype 0) or bf16 (dtype 1), the strides of their rows in elements; bias [E, H] fp32 or
- * NULL.  An edge whose bias or logit is -inf is left out; a row without an edge gives 0.
- * stats [n_dst, H, 2] (NULL: not kept): the maximum of x and the sum of exp(x - max), which
- * the backward recomputes the probabilities from.  Dk, Dv <= 256.
+ * A side of the graph: n_rows rows (destinations, or sources) whose edges row_ptr [n_rows + 1]
+ * delimits, col[e] the other end, ascending within a row.  batteries_attention_plan cuts the
+ * rows, in the given order (a permutation, NULL: as they are; rows next to each other in it
+ * should share columns), into tiles and writes the plan (batteries_attention_plan_bytes, 64-byte
+ * aligned).  Its first ints are the number of items, the number of parts (items of cut tiles)
+ * and, with check, 0 or what is wrong with the arrays (1 row_ptr, 2 a column out of range, 4
+ * columns not ascending); the caller reads them back into the side's n_items and n_parts.
+ * n_edges < 2^29.
  * ------------------------------------------------------------------------- */
-int batteries_neighbor_attention(const void* q, const void* k, const void* v, const float* bias,
-                                 const int64_t* row_ptr, const int64_t* col, const int64_t* eid,
-                                 void* out, float* stats, int64_t n_dst, int64_t n_src,
-                                 int64_t n_edges, int H, int Hkv, int Dk, int Dv,
-                                 int64_t q_stride, int64_t k_stride, int64_t v_stride,
-                                 float scale, int dtype, hipStream_t stream);
+typedef struct batmobile_attention_side {
+    int64_t n_rows, n_cols, n_edges;
+    const int32_t* plan;
+    int32_t n_items, n_parts;
+} batmobile_attention_side;
 
-/* Gradients of the above: grad_q, grad_k, grad_v contiguous, grad_bias [E, H] or NULL.
- * src_ptr [n_src + 1], src_dst [E], src_pos [E]: the edges grouped by source, destinations
- * ascending, with each edge's position in the destinations' order. */
-size_t batteries_neighbor_attention_backward_workspace_bytes(int64_t n_edges, int H);
+size_t batteries_attention_plan_bytes(int64_t n_rows, int64_t n_edges);
+int batteries_attention_plan(const int64_t* row_ptr, const int64_t* col, const int64_t* order,
+                             int64_t n_rows, int64_t n_cols, int64_t n_edges, int check,
+                             void* plan, size_t plan_bytes, hipStream_t stream);
+
+/* With rows i (destinations) and sources j = col e:
+ *   x_eh = scale <q[i,h], k[j, h / (H / Hkv)]> + bias[edge_id e, h],   p = softmax over the row
+ *   out[i,h] = sum_e p_eh v[j, h / (H / Hkv)]
+ * q [n_dst, H, Dk], k [n_src, Hkv, Dk], v [n_src, Hkv, Dv], out [n_dst, H, Dv] in fp32
+ * (dtype 0) or bf16 (dtype 1), rows at strides (in elements), bias [E, H] fp32 or NULL,
+ * edge_id [E] or NULL (the edges' own order).  Dk, Dv <= 256; pointers 16-byte aligned, Dk, Dv
+ * and strides multiples of 16 bytes.  An edge whose bias or logit is -inf is left out; a row
+ * without an edge gives 0.  stats [n_dst, H, 2] (NULL: not kept): the maximum of x and the sum
+ * of exp(x - max), which the backward recomputes the probabilities from. */
+size_t batteries_neighbor_attention_workspace_bytes(int64_t n_parts, int H, int Dv);
+int batteries_neighbor_attention(const void* q, const void* k, const void* v, const float* bias,
+                                 const int32_t* edge_id, const batmobile_attention_side* dst,
+                                 void* out, float* stats, int H, int Hkv, int Dk, int Dv,
+                                 int64_t q_stride, int64_t k_stride, int64_t v_stride, float scale,
+                                 int dtype, void* workspace, size_t workspace_bytes,
+                                 hipStream_t stream);
+
+/* Gradients of the above: grad_q, grad_k, grad_v contiguous, grad_bias [E, H] or NULL.  src: the
+ * edges grouped by source, src_pos [E] each one's position in the destinations' order. */
+size_t batteries_neighbor_attention_backward_workspace_bytes(int64_t n_edges, int64_t dst_parts,
+                                                             int64_t src_parts, int H, int Hkv,
+                                                             int Dk, int Dv);
 int batteries_neighbor_attention_backward(
     const void* q, const void* k, const void* v, const float* bias, const float* stats,
-    const void* grad_out, const int64_t* row_ptr, const int64_t* col, const int64_t* eid,
-    const int64_t* src_ptr, const int64_t* src_dst, const int64_t* src_pos, void* grad_q,
-    void* grad_k, void* grad_v, float* grad_bias, int64_t n_dst, int64_t n_src, int64_t n_edges,
-    int H, int Hkv, int Dk, int Dv, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+    const void* grad_out, const int64_t* row_ptr, const int32_t* edge_id,
+    const batmobile_attention_side* dst, const batmobile_attention_side* src,
+    const int32_t* src_pos, void* grad_q, void* grad_k, void* grad_v, float* grad_bias, int H,
+    int Hkv, int Dk, int Dv, int64_t q_stride, int64_t k_stride, int64_t v_stride,
     int64_t go_stride, float scale, int dtype, void* workspace, size_t workspace_bytes,
     hipStream_t stream);
 
