@@ -25,7 +25,7 @@ constexpr int kAttnCols = 32;     // columns of a chunk
 // ---------------------------------------------------------------------------
 // the plan of one side, in one int32 array
 // ---------------------------------------------------------------------------
-constexpr int kPlanHead = 16;     // items, parts, longest row, flags
+constexpr int kPlanHead = 16;     // items, parts, what is wrong
 constexpr int kPlanItems = 0, kPlanParts = 1, kPlanBad = 2;
 
 struct PlanLayout {
@@ -33,13 +33,15 @@ struct PlanLayout {
     int64_t rows, tile_item, tile_chunk, tile_part, item_tile, items, base, masks, ids, total;
 };
 
-// An item takes up to 2048 edges and up to 256 of a row (512 if the row ends there).
-constexpr int kItemEdges = 2048, kItemRow = 256;
+// A tile of more than kTileEdges edges is cut into items of kCutEdges or more, one with a row of
+// more than kTileRow into items with kCutRow or more of that row.  An item that is a whole tile
+// so has at most kTileEdges, which is what the kernels keep of its edges in LDS.
+constexpr int kTileEdges = 2048, kCutEdges = 1024, kTileRow = 512, kCutRow = 256;
 
 inline PlanLayout plan_layout(int64_t n_rows, int64_t n_edges) {
     PlanLayout p;
     p.tiles = ceil_div(n_rows, kAttnRows);
-    p.max_items = p.tiles + n_edges / kItemEdges + n_edges / kItemRow;
+    p.max_items = p.tiles + n_edges / kCutEdges + n_edges / kCutRow;
     p.max_chunks = n_edges / kAttnCols + p.max_items;
     int64_t at = kPlanHead;
     auto take = [&](int64_t n) {
@@ -52,7 +54,7 @@ inline PlanLayout plan_layout(int64_t n_rows, int64_t n_edges) {
     p.tile_chunk = take(p.tiles + 1);
     p.tile_part = take(p.tiles + 1);
     p.items = take(p.max_items * 4);
-    p.base = take(p.max_items * kAttnRows);
+    p.base = take(p.max_items * 2 * kAttnRows);
     p.masks = take(p.max_chunks * kAttnRows);
     p.ids = take(p.max_chunks * kAttnCols);
     p.total = at;
@@ -63,7 +65,7 @@ struct AttnSide {
     const int* rows;          // [16 tiles], -1 past the end
     const int* tile_part;     // [tiles + 1] first part
     const int4* items;        // tile, first chunk, chunks, part (-1: the tile's only item)
-    const int* base;          // [16 items] each row's first edge in the item
+    const int* base;          // [items][2][16] each row's first edge in the item, and their number
     const uint32_t* masks;    // [16 chunks]
     const int* ids;           // [32 chunks] columns
     const int* eid;           // edge -> its place in the arrays per edge (NULL: itself)
@@ -82,15 +84,22 @@ __device__ __forceinline__ int tile_of_part(const AttnSide& s, int p, int& first
     return lo;
 }
 
-// The work unit of a wave: workgroup b runs on XCD b % 8, which takes a contiguous eighth of
-// the units, so that tiles that share columns meet in one L2.
-__device__ __forceinline__ int64_t attn_unit(int64_t n_units) {
-    const int64_t per = gridDim.x >> 3;
-    const int64_t b = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    const int64_t u = b * 4 + (threadIdx.x >> 6);
-    return u < n_units ? u : -1;
+// The work unit of a wave.  Workgroup b runs on XCD b % 8, which takes a contiguous eighth of
+// the items, so that tiles that share columns meet in one L2, and those head by head: the
+// columns of the tiles in flight are then one head's only, which fit the L2 (50,000 atoms, 8
+// heads of 256 in bf16: 1 KB a column against 8).
+__device__ __forceinline__ bool attn_unit(int n_items, int heads, int& item, int& head) {
+    const int x = blockIdx.x & 7;
+    const int i0 = (int)((int64_t)n_items * x >> 3), i1 = (int)((int64_t)n_items * (x + 1) >> 3);
+    const int64_t w = (int64_t)(blockIdx.x >> 3) * 4 + (threadIdx.x >> 6);
+    if (w >= (int64_t)(i1 - i0) * heads) return false;
+    head = __builtin_amdgcn_readfirstlane((int)((uint32_t)w / (uint32_t)(i1 - i0)));
+    item = __builtin_amdgcn_readfirstlane(i0 + (int)((uint32_t)w % (uint32_t)(i1 - i0)));
+    return true;
 }
-inline unsigned attn_grid(int64_t n_units) { return (unsigned)(ceil_div(n_units, 32) * 8); }
+inline unsigned attn_grid(int64_t n_items, int64_t heads) {
+    return (unsigned)(ceil_div(ceil_div(n_items, 8) * heads, 4) * 8);
+}
 
 // ---------------------------------------------------------------------------
 // Fragments.  l = lane, n = l % 16, g = l / 16.  A step takes kTiles tiles of 16 columns.
@@ -137,13 +146,15 @@ template <typename T, int P>
 struct RowFrag {
     static constexpr int kN = P / Attn<T>::kSteps;
     typename Attn<T>::Vec v[kN];
+    // No load is under a condition: a branch would make the waits for later loads wait for all.
+    template <bool FULL>
     __device__ __forceinline__ void load(const T* row, int D, int g) {
 #pragma unroll
         for (int s = 0; s < kN; ++s) {
             const int d = s * Attn<T>::kSteps + g * Attn<T>::kAlign;
-            typename Attn<T>::Vec z{};
-            if (d < D) z = *reinterpret_cast<const typename Attn<T>::Vec*>(row + d);
-            v[s] = z;
+            const bool in = FULL || d < D;
+            v[s] = *reinterpret_cast<const typename Attn<T>::Vec*>(row + (in ? d : 0));
+            if (!FULL && !in) v[s] = typename Attn<T>::Vec{};
         }
     }
     __device__ __forceinline__ void zero() {
@@ -164,7 +175,8 @@ __device__ __forceinline__ v4f row_product(const RowFrag<T, P>& a, const RowFrag
     return x + y;
 }
 
-// Column form of a step's columns: kW components a lane and block.
+// Column form of a step's columns: kW components a lane and block.  Past D a lane reads the
+// row's start: its results are never stored.
 template <typename T, int P>
 struct ColFrag;
 
@@ -180,7 +192,7 @@ struct ColFrag<float, P> {
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
                 const int d = b * 64 + 4 * n;
-                v[j][b] = d < D ? *reinterpret_cast<const float4*>(p + d) : make_float4(0, 0, 0, 0);
+                v[j][b] = *reinterpret_cast<const float4*>(p + (d < D ? d : 0));
             }
         }
     }
@@ -211,9 +223,7 @@ struct ColFrag<uint16_t, P> {
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
                 const int d = b * 16 * kW + kW * n;
-                Vec z{};
-                if (d < D) z = *reinterpret_cast<const Vec*>(p + d);
-                v[j][b] = z;
+                v[j][b] = *reinterpret_cast<const Vec*>(p + (d < D ? d : 0));
             }
         }
     }
@@ -257,7 +267,7 @@ __device__ __attribute__((noinline)) void mac_exact_mem(const float* w, const in
     for (int j = 0; j < Attn<T>::kRowsPerLane; ++j)
 #pragma unroll 1
         for (int gg = 0; gg < 4; ++gg) {
-            const float f = __shfl(w[j], gg * 16 + n);
+            const float f = __shfl(w[j], gg * 16 + n);   // (every lane takes part)
             const T* p = base + (int64_t)__shfl(cols[j], gg * 16) * stride;
             if (f == 0.0f) continue;
 #pragma unroll 1
@@ -349,6 +359,45 @@ struct Step {
     // place of pair (n, 16 t + 4 g + r) along row n's edges of this step
     __device__ __forceinline__ int nth(int bit) const {
         return __popc(mask & ((1u << bit) - 1u));
+    }
+};
+
+// ---------------------------------------------------------------------------
+// A wave's values per edge in LDS, in the order of the rows: read from memory once, contiguous,
+// instead of one gather per pair and step.
+// ---------------------------------------------------------------------------
+struct ItemEdges {
+    int base, count, off, total;           // tile row n (lane % 16): first edge, number, LDS place
+    __device__ __forceinline__ void load(const AttnSide& s, int item, int n) {
+        base = s.base[(int64_t)item * 2 * kAttnRows + n];
+        count = s.base[(int64_t)item * 2 * kAttnRows + kAttnRows + n];
+        // sum over lanes 0 .. n of a row of 16
+        int x = count;
+        x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+        off = x - count;
+        total = __builtin_amdgcn_readlane(x, 15);
+    }
+    // f(place in LDS, edge, tile row) for all edges of the item, 64 at a time
+    template <typename F>
+    __device__ __forceinline__ void each(F&& f) const {
+        int o[kAttnRows], d[kAttnRows];
+#pragma unroll
+        for (int r = 0; r < kAttnRows; ++r) {
+            o[r] = __builtin_amdgcn_readlane(off, r);
+            d[r] = __builtin_amdgcn_readlane(base, r) - o[r];
+        }
+        for (int i = threadIdx.x & 63; i < total; i += 64) {
+            int e = d[0], row = 0;
+#pragma unroll
+            for (int r = 1; r < kAttnRows; ++r) {
+                e = i >= o[r] ? d[r] : e;
+                row = i >= o[r] ? r : row;
+            }
+            f(i, i + e, row);
+        }
     }
 };
 

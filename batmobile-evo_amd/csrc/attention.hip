@@ -28,22 +28,33 @@ struct AttnFwd {
     float scale;
 };
 
-template <typename T, int KP, int VP>
-__global__ __launch_bounds__(256) void attn_fwd_kernel(AttnFwd a) {
-    constexpr int kT = Attn<T>::kTiles, kR = Attn<T>::kRowsPerLane;
+template <typename T, int KP, int VP, bool FULL, bool BIAS>
+__global__ __launch_bounds__(256, KP + VP <= 256 ? 2 : 1) void attn_fwd_kernel(AttnFwd a) {
+    constexpr int kT = Attn<T>::kTiles;
     constexpr float kInf = __builtin_inff();
-    const int64_t u = attn_unit((int64_t)a.side.n_items * a.H);
-    if (u < 0) return;
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int item = (int)(u / a.H), h = (int)(u % a.H), kv = h / a.group;
+    __shared__ float lds[BIAS ? 4 * kTileEdges : 1];
+    int item, h;
+    if (!attn_unit(a.side.n_items, a.H, item, h)) return;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, kv = h / a.group;
     const int4 it4 = a.side.items[item];
     const int row = a.side.rows[it4.x * kAttnRows + n];
     const int steps = it4.z * 2 / kT;
     const T* kbase = (const T*)a.k + (int64_t)kv * a.Dk;
     const T* vbase = (const T*)a.v + (int64_t)kv * a.Dv;
     RowFrag<T, KP> q;
-    q.zero();
-    if (row >= 0) q.load(row_of<T>(a.q, row, a.qs) + (int64_t)h * a.Dk, a.Dk, g);
+    // (a slot past the last row computes with row 0 and stores nothing)
+    q.template load<FULL>(row_of<T>(a.q, max(row, 0), a.qs) + (int64_t)h * a.Dk, a.Dk, g);
+    ItemEdges edges;
+    float* b_lds = lds + (BIAS ? (threadIdx.x >> 6) * kTileEdges : 0);
+    bool staged = true;
+    auto bias_of = [&](int e) {
+        return a.bias[(int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h];
+    };
+    if constexpr (BIAS) {
+        edges.load(a.side, item, n);
+        staged = edges.total <= kTileEdges;
+        if (staged) edges.each([&](int i, int e, int) { b_lds[i] = bias_of(e); });
+    }
 
     v4f acc[ColFrag<T, VP>::kAcc];
     float m, l;
@@ -52,36 +63,21 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(AttnFwd a) {
         l = 0.0f;
 #pragma unroll
         for (int i = 0; i < ColFrag<T, VP>::kAcc; ++i) acc[i] = v4f{0, 0, 0, 0};
-        int edge = a.side.base[item * kAttnRows + n];
-        Step<T> st;
+        int done = 0;                      // row n's edges of earlier steps
+        Step<T> st, next;
         RowFrag<T, KP> kf[kT];
         if (steps > 0) {
             st.load(a.side, it4.y, 0, n, g);
+            next.load(a.side, it4.y, min(1, steps - 1), n, g);
 #pragma unroll
-            for (int t = 0; t < kT; ++t) kf[t].load(row_of<T>(kbase, st.row[t], a.ks), a.Dk, g);
+            for (int t = 0; t < kT; ++t)
+                kf[t].template load<FULL>(row_of<T>(kbase, st.row[t], a.ks), a.Dk, g);
         }
         for (int i = 0; i < steps; ++i) {
-            // loads in flight: this step's v and bias over the first product, the next step's
-            // k over the softmax and the second product
+            // in flight: this step's v over the first product, the next step's k and the
+            // indices of the one after over the softmax and the second product
             ColFrag<T, VP> vf;
             vf.load([&](int j) { return row_of<T>(vbase, st.col[j], a.vs); }, a.Dv, n);
-            float b[4 * kT];
-#pragma unroll
-            for (int j = 0; j < 4 * kT; ++j) {
-                const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
-                b[j] = -kInf;
-                if ((st.mask >> bit) & 1) {
-                    b[j] = 0.0f;
-                    if (a.bias) {
-                        int e = edge + st.nth(bit);
-                        if (a.side.eid) e = a.side.eid[e];
-                        b[j] = a.bias[(int64_t)e * a.H + h];
-                    }
-                }
-            }
-            edge += __popc(st.mask);
-            Step<T> next;
-            next.load(a.side, it4.y, min(i + 1, steps - 1), n, g);
             float x[4 * kT];
 #pragma unroll
             for (int t = 0; t < kT; ++t) {
@@ -90,13 +86,25 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(AttnFwd a) {
                 for (int r = 0; r < 4; ++r) x[4 * t + r] = s[r];
             }
 #pragma unroll
-            for (int t = 0; t < kT; ++t) kf[t].load(row_of<T>(kbase, next.row[t], a.ks), a.Dk, g);
+            for (int t = 0; t < kT; ++t)
+                kf[t].template load<FULL>(row_of<T>(kbase, next.row[t], a.ks), a.Dk, g);
+            Step<T> after;
+            after.load(a.side, it4.y, min(i + 2, steps - 1), n, g);
             float top = m;
 #pragma unroll
             for (int j = 0; j < 4 * kT; ++j) {
-                x[j] = b[j] == -kInf ? -kInf : fmaf(x[j], a.scale, b[j]);
+                const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
+                const bool on = (st.mask >> bit) & 1;
+                float b = 0.0f;
+                if constexpr (BIAS) {
+                    const int at = done + st.nth(bit);
+                    if (staged) b = b_lds[min(edges.off + at, kTileEdges - 1)];
+                    else if (on) b = bias_of(edges.base + at);
+                }
+                x[j] = !on || b == -kInf ? -kInf : fmaf(x[j], a.scale, b);
                 top = fmaxf(top, x[j]);
             }
+            done += __popc(st.mask);
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
             const float ref = top == -kInf ? 0.0f : top;
@@ -116,6 +124,7 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(AttnFwd a) {
             if (exact) mac_exact<T, VP>(p, st.col, acc, vbase, a.vs, a.Dv);
             else vf.mac(p, acc);
             st = next;
+            next = after;
         }
         // infinities or NaN: the sums once more, each row over its own edges alone
         if (exact || !any_not_finite<ColFrag<T, VP>::kAcc>(acc)) break;
@@ -199,7 +208,12 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnFwd a) {
 
 template <typename T, int KP, int VP>
 static void attn_fwd_launch(const AttnFwd& a, hipStream_t s) {
-    attn_fwd_kernel<T, KP, VP><<<attn_grid((int64_t)a.side.n_items * a.H), 256, 0, s>>>(a);
+    const unsigned grid = attn_grid(a.side.n_items, a.H);
+    const bool full = a.Dk == KP;
+    if (a.bias && full) attn_fwd_kernel<T, KP, VP, true, true><<<grid, 256, 0, s>>>(a);
+    else if (a.bias) attn_fwd_kernel<T, KP, VP, false, true><<<grid, 256, 0, s>>>(a);
+    else if (full) attn_fwd_kernel<T, KP, VP, true, false><<<grid, 256, 0, s>>>(a);
+    else attn_fwd_kernel<T, KP, VP, false, false><<<grid, 256, 0, s>>>(a);
 }
 template <typename T, int KP>
 static void attn_fwd_pick_v(const AttnFwd& a, hipStream_t s) {

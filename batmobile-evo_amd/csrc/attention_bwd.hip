@@ -4,15 +4,17 @@
 //   gb = ds,  gq[i,h] = scale sum_e ds k[j,g],  gk[j,g] = scale sum ds q[i,h],
 //   gv[j,g] = sum p go[i,h]
 //
-// with p recomputed from the rows' maxima and sums.  Three kernels:
+// with p recomputed from the rows' maxima and sums.
 //
-//   attn_scores  a tile and head at a time, both products of its pairs: p and dp per edge
-//   attn_ds      a row and head at a time: D, ds (D from the same fp32 p and dp: formed from
-//                the rounded o it would put o's rounding into gb, which is fp32)
+//   attn_scores  a tile and head at a time, both products of its pairs: p and dp per edge, kept
+//                in LDS, D and ds; p and ds go to the workspace, ds to gb
+//   attn_ds      D and ds of the rows of cut tiles
 //   attn_sum     tiles of either side: gq (ds and k), gk (ds and q), gv (p and go)
 //
-// p and ds take 8 bytes an edge and head in the workspace; the source side would otherwise read
-// two rows and form both products again.  No atomics: sums run in the plan's order.
+// D comes from the same fp32 p and dp: formed from the rounded o it would put o's rounding into
+// gb, which is fp32.  p and ds take 8 bytes an edge and head in the workspace; the source side
+// would otherwise read two rows and form both products again.  No atomics: sums run in the
+// plan's order.
 #include "attention.h"
 
 namespace bmhip {
@@ -21,132 +23,136 @@ struct AttnScores {
     AttnSide side;
     const void *q, *k, *v, *go;
     const float *bias, *stats;
-    float2* ws;                            // [H][E]: p, dp
+    float* gbias;
+    float2* ws;                            // [H][E]: p, ds (of cut tiles first dp)
     int64_t qs, ks, vs, gs, edges;
     int H, group, Dk, Dv;
     float scale;
 };
 
-template <typename T, int KP, int VP>
-__global__ __launch_bounds__(256) void attn_scores_kernel(AttnScores a) {
+template <typename T, int KP, int VP, bool FULL>
+__global__ __launch_bounds__(256, KP + VP <= 256 ? 2 : 1) void attn_scores_kernel(AttnScores a) {
     constexpr int kT = Attn<T>::kTiles;
     constexpr float kInf = __builtin_inff();
-    const int64_t u = attn_unit((int64_t)a.side.n_items * a.H);
-    if (u < 0) return;
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int item = (int)(u / a.H), h = (int)(u % a.H), kv = h / a.group;
+    __shared__ float lds_p[4][kTileEdges];           // the bias, then p
+    __shared__ float lds_dp[4][kTileEdges];
+    __shared__ float lds_d[4][kAttnRows];
+    int item, h;
+    if (!attn_unit(a.side.n_items, a.H, item, h)) return;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, kv = h / a.group;
     const int4 it4 = a.side.items[item];
     const int row = a.side.rows[it4.x * kAttnRows + n];
     const int steps = it4.z * 2 / kT;
     if (steps == 0) return;
     const T* kbase = (const T*)a.k + (int64_t)kv * a.Dk;
     const T* vbase = (const T*)a.v + (int64_t)kv * a.Dv;
-    RowFrag<T, KP> q;
-    RowFrag<T, VP> go;
-    q.zero();
-    go.zero();
-    float ref = 0.0f, inv = 0.0f;
-    if (row >= 0) {
-        q.load(row_of<T>(a.q, row, a.qs) + (int64_t)h * a.Dk, a.Dk, g);
-        go.load(row_of<T>(a.go, row, a.gs) + (int64_t)h * a.Dv, a.Dv, g);
-        const float2 ml =
-            *reinterpret_cast<const float2*>(a.stats + ((int64_t)row * a.H + h) * 2);
-        ref = ml.x == -kInf ? 0.0f : ml.x;
-        inv = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
-    }
-    float2* ws = a.ws + (int64_t)h * a.edges;
-    int edge = a.side.base[item * kAttnRows + n];
-    Step<T> st;
+    Step<T> st, next;
     st.load(a.side, it4.y, 0, n, g);
-    RowFrag<T, KP> kf[kT];
+    next.load(a.side, it4.y, min(1, steps - 1), n, g);
+    RowFrag<T, KP> kf[kT], q;
+    RowFrag<T, VP> go;
 #pragma unroll
-    for (int t = 0; t < kT; ++t) kf[t].load(row_of<T>(kbase, st.row[t], a.ks), a.Dk, g);
+    for (int t = 0; t < kT; ++t)
+        kf[t].template load<FULL>(row_of<T>(kbase, st.row[t], a.ks), a.Dk, g);
+    q.template load<FULL>(row_of<T>(a.q, max(row, 0), a.qs) + (int64_t)h * a.Dk, a.Dk, g);
+    go.template load<FULL>(row_of<T>(a.go, max(row, 0), a.gs) + (int64_t)h * a.Dv, a.Dv, g);
+    const float2 ml =
+        *reinterpret_cast<const float2*>(a.stats + ((int64_t)max(row, 0) * a.H + h) * 2);
+    const float ref = ml.x == -kInf ? 0.0f : ml.x, inv = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
+    ItemEdges edges;
+    edges.load(a.side, item, n);
+    float* p_lds = lds_p[threadIdx.x >> 6];
+    float* dp_lds = lds_dp[threadIdx.x >> 6];
+    const bool staged = edges.total <= kTileEdges;
+    auto place = [&](int e) { return (int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h; };
+    if (staged && a.bias) edges.each([&](int i, int e, int) { p_lds[i] = a.bias[place(e)]; });
+    float2* ws = a.ws + (int64_t)h * a.edges;
+    float d = 0.0f;
+    int done = 0;                              // row n's edges of earlier steps
     for (int i = 0; i < steps; ++i) {
         RowFrag<T, VP> vf[kT];
 #pragma unroll
-        for (int t = 0; t < kT; ++t) vf[t].load(row_of<T>(vbase, st.row[t], a.vs), a.Dv, g);
-        float b[4 * kT];
-#pragma unroll
-        for (int j = 0; j < 4 * kT; ++j) {
-            const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
-            b[j] = 0.0f;
-            if (a.bias && ((st.mask >> bit) & 1)) {
-                int e = edge + st.nth(bit);
-                if (a.side.eid) e = a.side.eid[e];
-                b[j] = a.bias[(int64_t)e * a.H + h];
-            }
-        }
-        Step<T> next;
-        next.load(a.side, it4.y, min(i + 1, steps - 1), n, g);
+        for (int t = 0; t < kT; ++t)
+            vf[t].template load<FULL>(row_of<T>(vbase, st.row[t], a.vs), a.Dv, g);
         v4f s[kT], dp[kT];
 #pragma unroll
         for (int t = 0; t < kT; ++t) s[t] = row_product<T, KP>(kf[t], q);
 #pragma unroll
-        for (int t = 0; t < kT; ++t) kf[t].load(row_of<T>(kbase, next.row[t], a.ks), a.Dk, g);
+        for (int t = 0; t < kT; ++t)
+            kf[t].template load<FULL>(row_of<T>(kbase, next.row[t], a.ks), a.Dk, g);
+        Step<T> after;
+        after.load(a.side, it4.y, min(i + 2, steps - 1), n, g);
+        float p[4 * kT];
+#pragma unroll
+        for (int j = 0; j < 4 * kT; ++j) {
+            const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
+            const bool on = (st.mask >> bit) & 1;
+            const int at = done + st.nth(bit);
+            float b = 0.0f;
+            if (a.bias) {
+                if (staged) b = p_lds[min(edges.off + at, kTileEdges - 1)];
+                else if (on) b = a.bias[place(edges.base + at)];
+            }
+            const float x = fmaf(s[j >> 2][j & 3], a.scale, b);
+            p[j] = !on || b == -kInf || x == -kInf ? 0.0f : exp2f((x - ref) * kLog2e) * inv;
+        }
 #pragma unroll
         for (int t = 0; t < kT; ++t) dp[t] = row_product<T, VP>(vf[t], go);
 #pragma unroll
         for (int j = 0; j < 4 * kT; ++j) {
             const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
+            const float y = p[j] == 0.0f ? 0.0f : dp[j >> 2][j & 3];
+            d = fmaf(p[j], y, d);
             if ((st.mask >> bit) & 1) {
-                const float x = fmaf(s[j >> 2][j & 3], a.scale, b[j]);
-                const bool off = b[j] == -kInf || x == -kInf;
-                ws[edge + st.nth(bit)] =
-                    off ? make_float2(0.0f, 0.0f)
-                        : make_float2(exp2f((x - ref) * kLog2e) * inv, dp[j >> 2][j & 3]);
+                const int at = done + st.nth(bit);
+                if (staged) {
+                    p_lds[edges.off + at] = p[j];
+                    dp_lds[edges.off + at] = y;
+                } else {
+                    ws[edges.base + at] = make_float2(p[j], y);
+                }
             }
         }
-        edge += __popc(st.mask);
+        done += __popc(st.mask);
         st = next;
+        next = after;
     }
+    if (!staged) return;
+    if (it4.w >= 0) {                          // the rest once all parts of the row are there
+        edges.each([&](int i, int e, int) { ws[e] = make_float2(p_lds[i], dp_lds[i]); });
+        return;
+    }
+    d += __shfl_xor(d, 16);
+    d += __shfl_xor(d, 32);
+    float* d_lds = lds_d[threadIdx.x >> 6];
+    if (g == 0) d_lds[n] = d;
+    __builtin_amdgcn_wave_barrier();
+    edges.each([&](int i, int e, int r) {
+        const float p = p_lds[i], ds = p == 0.0f ? 0.0f : p * (dp_lds[i] - d_lds[r]);
+        ws[e] = make_float2(p, ds);
+        if (a.gbias) a.gbias[place(e)] = ds;
+    });
 }
 
 struct AttnDs {
+    AttnSide side;
     const int64_t* row_ptr;
-    const int* eid;
     float2* ws;
     float* gbias;
-    int64_t n_rows, edges;
+    int64_t edges;
     int H;
 };
 
-// 16 lanes a row and head; rows of more than 4096 edges: a workgroup.
-constexpr int kDsLong = 4096;
-
-__global__ __launch_bounds__(256) void attn_ds_kernel(AttnDs a) {
-    const int64_t u = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (u >= a.n_rows * a.H) return;
-    const int64_t row = u % a.n_rows;
-    const int h = (int)(u / a.n_rows), t = threadIdx.x & 15;
-    const int64_t e0 = a.row_ptr[row], e1 = a.row_ptr[row + 1];
-    if (e1 - e0 > kDsLong) return;
-    float2* ws = a.ws + (int64_t)h * a.edges;
-    float d = 0.0f;
-    for (int64_t e = e0 + t; e < e1; e += 16) {
-        const float2 w = ws[e];
-        d += w.x == 0.0f ? 0.0f : w.x * w.y;
-    }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) d += __shfl_xor(d, o);
-    for (int64_t e = e0 + t; e < e1; e += 16) {
-        const float2 w = ws[e];
-        const float ds = w.x == 0.0f ? 0.0f : w.x * (w.y - d);
-        ws[e].y = ds;
-        if (a.gbias) a.gbias[(a.eid ? a.eid[e] : e) * a.H + h] = ds;
-    }
-}
-
-// The long rows lie in cut tiles: workgroup p of the parts takes rows p, p + parts of its tile.
-__global__ __launch_bounds__(1024) void attn_ds_long_kernel(AttnDs a, AttnSide side) {
+// Rows of cut tiles: workgroup p of the parts takes rows p, p + parts of its tile, ...
+__global__ __launch_bounds__(1024) void attn_ds_kernel(AttnDs a) {
     __shared__ float sh[16];
     const int h = blockIdx.y;
     int first, parts;
-    const int tile = tile_of_part(side, blockIdx.x, first, parts);
+    const int tile = tile_of_part(a.side, blockIdx.x, first, parts);
     for (int slot = (int)blockIdx.x - first; slot < kAttnRows; slot += parts) {
-        const int row = side.rows[tile * kAttnRows + slot];
+        const int row = a.side.rows[tile * kAttnRows + slot];
         if (row < 0) continue;
         const int64_t e0 = a.row_ptr[row], e1 = a.row_ptr[row + 1];
-        if (e1 - e0 <= kDsLong) continue;
         float2* ws = a.ws + (int64_t)h * a.edges;
         float d = 0.0f;
         for (int64_t e = e0 + threadIdx.x; e < e1; e += 1024) {
@@ -164,7 +170,7 @@ __global__ __launch_bounds__(1024) void attn_ds_long_kernel(AttnDs a, AttnSide s
             const float2 w = ws[e];
             const float ds = w.x == 0.0f ? 0.0f : w.x * (w.y - d);
             ws[e].y = ds;
-            if (a.gbias) a.gbias[(a.eid ? a.eid[e] : e) * a.H + h] = ds;
+            if (a.gbias) a.gbias[(int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h] = ds;
         }
     }
 }
@@ -184,46 +190,68 @@ struct AttnSum {
 };
 
 template <typename T, int P>
-__global__ __launch_bounds__(256) void attn_sum_kernel(AttnSum a) {
+__global__ __launch_bounds__(256, 2) void attn_sum_kernel(AttnSum a) {
     constexpr int kT = Attn<T>::kTiles, kR = Attn<T>::kRowsPerLane;
-    const int64_t u = attn_unit((int64_t)a.side.n_items * a.heads);
-    if (u < 0) return;
+    __shared__ float lds[4][kTileEdges];
+    int item, head;
+    if (!attn_unit(a.side.n_items, a.heads, item, head)) return;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int item = (int)(u / a.heads), head = (int)(u % a.heads);
     const int4 it4 = a.side.items[item];
     const int row = a.side.rows[it4.x * kAttnRows + n];
     const int steps = it4.z * 2 / kT;
+    float* w_lds = lds[threadIdx.x >> 6];
+    ItemEdges edges;
+    edges.load(a.side, item, n);
+    const bool staged = edges.total <= kTileEdges;
     v4f acc[ColFrag<T, P>::kAcc];
     for (int exact = 0;; ++exact) {
 #pragma unroll
         for (int i = 0; i < ColFrag<T, P>::kAcc; ++i) acc[i] = v4f{0, 0, 0, 0};
-        for (int hh = head * a.group; hh < (head + 1) * a.group; ++hh) {
+        for (int hh = head * a.group; steps > 0 && hh < (head + 1) * a.group; ++hh) {
             const T* x = (const T*)a.x + (int64_t)(hh / a.x_div) * a.D;
             const float* ws = reinterpret_cast<const float*>(a.ws + (int64_t)hh * a.edges) +
                               a.second;
-            int edge = a.side.base[item * kAttnRows + n];
-            Step<T> st;
-            if (steps > 0) st.load(a.side, it4.y, 0, n, g);
-            for (int i = 0; i < steps; ++i) {
-                ColFrag<T, P> xf;
-                xf.load([&](int j) { return row_of<T>(x, st.col[j], a.xs); }, a.D, n);
+            auto factor = [&](int e) {
+                return ws[(int64_t)(a.side.eid ? a.side.eid[e] : e) * 2];
+            };
+            // two steps' rows in turn: one is read while the other is multiplied
+            Step<T> s0, s1;
+            ColFrag<T, P> x0, x1;
+            s0.load(a.side, it4.y, 0, n, g);
+            s1.load(a.side, it4.y, min(1, steps - 1), n, g);
+            if (steps == 1) s1.mask = 0;
+            x0.load([&](int j) { return row_of<T>(x, s0.col[j], a.xs); }, a.D, n);
+            __builtin_amdgcn_wave_barrier();
+            if (staged) edges.each([&](int i, int e, int) { w_lds[i] = factor(e); });
+            __builtin_amdgcn_wave_barrier();
+            int done = 0;                      // row n's edges of earlier steps
+            auto mac = [&](const Step<T>& s, const ColFrag<T, P>& f) {
                 float w[kR];
 #pragma unroll
                 for (int j = 0; j < kR; ++j) {
                     const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
-                    w[j] = 0.0f;
-                    if ((st.mask >> bit) & 1) {
-                        int e = edge + st.nth(bit);
-                        if (a.side.eid) e = a.side.eid[e];
-                        w[j] = ws[(int64_t)e * 2];
-                    }
+                    const int at = done + s.nth(bit);
+                    const bool on = (s.mask >> bit) & 1;
+                    float v = 0.0f;
+                    if (staged) v = w_lds[min(edges.off + at, kTileEdges - 1)];
+                    else if (on) v = factor(edges.base + at);
+                    w[j] = on ? v : 0.0f;
                 }
-                edge += __popc(st.mask);
-                Step<T> next;
-                next.load(a.side, it4.y, min(i + 1, steps - 1), n, g);
-                if (exact) mac_exact<T, P>(w, st.col, acc, x, a.xs, a.D);
-                else xf.mac(w, acc);
-                st = next;
+                done += __popc(s.mask);
+                if (exact) mac_exact<T, P>(w, s.col, acc, x, a.xs, a.D);
+                else f.mac(w, acc);
+            };
+            for (int i = 0; i < steps; i += 2) {
+                x1.load([&](int j) { return row_of<T>(x, s1.col[j], a.xs); }, a.D, n);
+                Step<T> s2, s3;
+                s2.load(a.side, it4.y, min(i + 2, steps - 1), n, g);
+                s3.load(a.side, it4.y, min(i + 3, steps - 1), n, g);
+                if (i + 3 >= steps) s3.mask = 0;
+                mac(s0, x0);
+                x0.load([&](int j) { return row_of<T>(x, s2.col[j], a.xs); }, a.D, n);
+                mac(s1, x1);
+                s0 = s2;
+                s1 = s3;
             }
         }
         if (exact || !any_not_finite<ColFrag<T, P>::kAcc>(acc)) break;
@@ -269,12 +297,17 @@ __global__ __launch_bounds__(256) void attn_sum_join_kernel(AttnSum a) {
     }
 }
 
+template <typename T, int KP, int VP>
+static void attn_scores_launch(const AttnScores& a, hipStream_t s) {
+    const unsigned grid = attn_grid(a.side.n_items, a.H);
+    if (a.Dk == KP && a.Dv == VP) attn_scores_kernel<T, KP, VP, true><<<grid, 256, 0, s>>>(a);
+    else attn_scores_kernel<T, KP, VP, false><<<grid, 256, 0, s>>>(a);
+}
 template <typename T, int KP>
 static void attn_scores_run_k(const AttnScores& a, hipStream_t s) {
-    const unsigned grid = attn_grid((int64_t)a.side.n_items * a.H);
-    if (a.Dv <= 64) attn_scores_kernel<T, KP, 64><<<grid, 256, 0, s>>>(a);
-    else if (a.Dv <= 128) attn_scores_kernel<T, KP, 128><<<grid, 256, 0, s>>>(a);
-    else attn_scores_kernel<T, KP, 256><<<grid, 256, 0, s>>>(a);
+    if (a.Dv <= 64) attn_scores_launch<T, KP, 64>(a, s);
+    else if (a.Dv <= 128) attn_scores_launch<T, KP, 128>(a, s);
+    else attn_scores_launch<T, KP, 256>(a, s);
 }
 template <typename T>
 static void attn_scores_run(const AttnScores& a, hipStream_t s) {
@@ -284,7 +317,7 @@ static void attn_scores_run(const AttnScores& a, hipStream_t s) {
 }
 template <typename T>
 static void attn_sum_run(const AttnSum& a, int parts, hipStream_t s) {
-    const unsigned grid = attn_grid((int64_t)a.side.n_items * a.heads);
+    const unsigned grid = attn_grid(a.side.n_items, a.heads);
     if (grid == 0) return;
     if (a.D <= 64) attn_sum_kernel<T, 64><<<grid, 256, 0, s>>>(a);
     else if (a.D <= 128) attn_sum_kernel<T, 128><<<grid, 256, 0, s>>>(a);
@@ -335,15 +368,15 @@ extern "C" int batteries_neighbor_attention_backward(
         AttnScores a{};
         a.side = side_args(*dst, edge_id);
         a.q = q; a.k = k; a.v = v; a.go = grad_out; a.bias = bias; a.stats = stats; a.ws = ws;
+        a.gbias = grad_bias;
         a.qs = q_stride; a.ks = k_stride; a.vs = v_stride; a.gs = go_stride; a.edges = E;
         a.H = H; a.group = H / Hkv; a.Dk = Dk; a.Dv = Dv; a.scale = scale;
         if (dtype == 0) attn_scores_run<float>(a, stream);
         else attn_scores_run<uint16_t>(a, stream);
-        AttnDs d{row_ptr, edge_id, ws, grad_bias, dst->n_rows, E, H};
-        attn_ds_kernel<<<(unsigned)ceil_div(dst->n_rows * H, 16), 256, 0, stream>>>(d);
-        if (dst->n_parts > 0)
-            attn_ds_long_kernel<<<dim3((unsigned)dst->n_parts, (unsigned)H), 1024, 0, stream>>>(
-                d, side_args(*dst, edge_id));
+        if (dst->n_parts > 0) {
+            AttnDs d{side_args(*dst, edge_id), row_ptr, ws, grad_bias, E, H};
+            attn_ds_kernel<<<dim3((unsigned)dst->n_parts, (unsigned)H), 1024, 0, stream>>>(d);
+        }
     }
     auto sum = [&](const batmobile_attention_side& side, const int32_t* at, const void* x,
                    int64_t xs, void* out, int heads, int group, int x_div, int D, int second,

@@ -7,9 +7,9 @@
 //                equal columns of different rows merged into one entry (a column that a row
 //                holds k times, parallel edges, gets k entries), masks from the entries
 //
-// A tile with more than kItemEdges edges, or a row of more than 2 kItemRow, is cut at column
-// values into items of equal edge counts, each found by searching for its first column.  A cut
-// with more edges than the LDS holds (one column thousands of times) is taken unmerged.
+// A tile with many edges or a long row is cut at column values into items of equal edge counts,
+// each found by searching for its first column.  A cut with more edges than the LDS holds (one
+// column thousands of times) is taken unmerged.
 #include "attention.h"
 
 namespace bmhip {
@@ -39,8 +39,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_tiles_kernel(PlanArgs a) {
         edges += len;
         longest = max(longest, len);
     }
-    const int64_t cuts = max(longest > 2 * kItemRow ? longest / kItemRow : 1,
-                             max((int64_t)1, edges / kItemEdges));
+    const int64_t cuts = max(longest > kTileRow ? longest / kCutRow : (int64_t)1,
+                             edges > kTileEdges ? edges / kCutEdges : (int64_t)1);
     a.plan[a.at.tile_item + t] = (int)cuts;
     a.plan[a.at.tile_chunk + t] = (int)(edges / kAttnCols + cuts);
     a.plan[a.at.tile_part + t] = cuts > 1 ? (int)cuts : 0;
@@ -168,7 +168,11 @@ __global__ __launch_bounds__(kPlanThreads) void plan_items_kernel(PlanArgs a) {
         }
         pre[kAttnRows] = n;
     }
-    if (tid < kAttnRows) a.plan[a.at.base + (int64_t)item * kAttnRows + tid] = (int)start[tid];
+    if (tid < kAttnRows) {
+        int* base = a.plan + a.at.base + (int64_t)item * 2 * kAttnRows;
+        base[tid] = (int)start[tid];
+        base[kAttnRows + tid] = (int)(stop[tid] - start[tid]);
+    }
     __syncthreads();
     const int n = pre[kAttnRows];
     uint32_t* masks = reinterpret_cast<uint32_t*>(a.plan) + a.at.masks + chunk0 * kAttnRows;
