@@ -10,9 +10,9 @@
 // again.  Edges of a row are numbered along the row: the k-th set bit of a row over the chunks
 // is its k-th edge, so the masks also give each pair's place in the arrays per edge.
 //
-// Every wave works on one (item, head): an item is a tile, or a part of one that has a long
-// row or many edges.  Nothing is shared between waves: the fragments come from global memory
-// in the layout the matrix instructions take.
+// Every wave works on one (item, head), an item being a tile, or a part of one that has a long
+// row or many edges, and is a workgroup of its own: nothing is shared, and there are no
+// barriers.
 #pragma once
 #include "common.h"
 #include "batmobile_hip.h"
@@ -36,7 +36,7 @@ struct PlanLayout {
 // A tile of more than kTileEdges edges is cut into items of kCutEdges or more, one with a row of
 // more than kTileRow into items with kCutRow or more of that row.  An item that is a whole tile
 // so has at most kTileEdges, which is what the kernels keep of its edges in LDS.
-constexpr int kTileEdges = 2048, kCutEdges = 1024, kTileRow = 512, kCutRow = 256;
+constexpr int kTileEdges = 1024, kCutEdges = 512, kTileRow = 512, kCutRow = 256;
 
 inline PlanLayout plan_layout(int64_t n_rows, int64_t n_edges) {
     PlanLayout p;
@@ -84,27 +84,29 @@ __device__ __forceinline__ int tile_of_part(const AttnSide& s, int p, int& first
     return lo;
 }
 
-// The work unit of a wave.  Workgroup b runs on XCD b % 8, which takes a contiguous eighth of
-// the items, so that tiles that share columns meet in one L2, and those head by head: the
-// columns of the tiles in flight are then one head's only, which fit the L2 (50,000 atoms, 8
-// heads of 256 in bf16: 1 KB a column against 8).
+// The work unit of workgroup b, which is one wave.  It runs on XCD b % 8, which takes a
+// contiguous eighth of the items, so that tiles that share columns meet in one L2, and those
+// head by head: the columns of the tiles in flight are then one head's only, which fit the L2
+// (50,000 atoms, 8 heads of 256 in bf16: 1 KB a column against 8).
 __device__ __forceinline__ bool attn_unit(int n_items, int heads, int& item, int& head) {
     const int x = blockIdx.x & 7;
     const int i0 = (int)((int64_t)n_items * x >> 3), i1 = (int)((int64_t)n_items * (x + 1) >> 3);
-    const int64_t w = (int64_t)(blockIdx.x >> 3) * 4 + (threadIdx.x >> 6);
-    if (w >= (int64_t)(i1 - i0) * heads) return false;
-    head = __builtin_amdgcn_readfirstlane((int)((uint32_t)w / (uint32_t)(i1 - i0)));
-    item = __builtin_amdgcn_readfirstlane(i0 + (int)((uint32_t)w % (uint32_t)(i1 - i0)));
+    const uint32_t w = blockIdx.x >> 3;
+    if (w >= (uint64_t)(i1 - i0) * heads) return false;
+    head = (int)(w / (uint32_t)(i1 - i0));
+    item = i0 + (int)(w % (uint32_t)(i1 - i0));
     return true;
 }
 inline unsigned attn_grid(int64_t n_items, int64_t heads) {
-    return (unsigned)(ceil_div(ceil_div(n_items, 8) * heads, 4) * 8);
+    return (unsigned)(ceil_div(n_items, 8) * heads * 8);
 }
 
 // ---------------------------------------------------------------------------
 // Fragments.  l = lane, n = l % 16, g = l / 16.  A step takes kTiles tiles of 16 columns.
 //
-// Row form (the contraction runs along a row's components): lane l holds row n.
+// Row form (the contraction runs along a row's components): lane l holds row n.  Read like that
+// from memory, 16 lanes in a row would ask for 16 cache lines (37 line accesses a load were
+// measured); the columns' rows go to LDS first, whole rows at a time (RowTile).
 //   bf16: components 32 s + 8 g + (0..7) in step s of v_mfma_f32_16x16x32_bf16
 //   fp32: components 16 s + 4 g + (0..3), one v_mfma_f32_16x16x4f32 for each of the four
 // Column form (the contraction runs over the step's columns j): lane l holds kW components
@@ -136,9 +138,31 @@ struct Attn<uint16_t> {
     }
 };
 
+// row of a matrix whose rows are `stride` bytes apart (one 32 x 32 -> 64-bit multiply-add)
 template <typename T>
-__device__ __forceinline__ const T* row_of(const void* p, int row, int64_t stride) {
-    return (const T*)p + (int64_t)row * stride;
+__device__ __forceinline__ const T* row_of(const void* p, int row, uint32_t stride) {
+    return (const T*)((const char*)p + (uint64_t)(uint32_t)row * stride);
+}
+
+// Over the lanes of the same n: the row pairs, then the halves, swapped and combined.
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
+template <typename F>
+__device__ __forceinline__ float over_groups(float x, F&& f) {
+    v2u r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_over_groups(float x) {
+    return over_groups(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float sum_over_groups(float x) {
+    return over_groups(x, [](float a, float b) { return a + b; });
+}
+
+// exp(x) of x <= 0 in natural units (v_exp_f32: a result below 2^-126 is 0)
+__device__ __forceinline__ float attn_exp(float x) {
+    return __builtin_amdgcn_exp2f(x * 1.4426950408889634f);
 }
 
 // Row form of one row: D components of at most P, zero past D.
@@ -157,9 +181,82 @@ struct RowFrag {
             if (!FULL && !in) v[s] = typename Attn<T>::Vec{};
         }
     }
-    __device__ __forceinline__ void zero() {
+};
+
+// The rows of a step's columns in LDS, moved there by loads that pass no registers: lane l of
+// load k brings the 16-byte piece l % kPieces of row k + kLoads (l / kPieces) to place 64 k + l.
+// Which piece of its row it brings is that number with the row's low bits flipped, so that the
+// 16 rows of a fragment read lie in different banks.
+template <typename T, int P>
+struct RowTile {
+    static constexpr int kRows = 16 * Attn<T>::kTiles, kPieces = P * (int)sizeof(T) / 16;
+    static constexpr int kPer = 64 / kPieces, kLoads = kRows / kPer;
+    static constexpr int kFlip = (kPieces < 16 ? kPieces : 16) - 1;
+    static constexpr int kBytes = kLoads * 1024;
+    // the columns of a step whose rows this lane brings pieces of
+    struct Ids {
+        int id[kLoads];
+        __device__ __forceinline__ void load(const int* ids, int lane) {
+            const int4* p = reinterpret_cast<const int4*>(ids + lane / kPieces * kLoads);
 #pragma unroll
-        for (int s = 0; s < kN; ++s) v[s] = typename Attn<T>::Vec{};
+            for (int k = 0; k < kLoads / 4; ++k) {
+                const int4 q = p[k];
+                id[4 * k] = q.x;
+                id[4 * k + 1] = q.y;
+                id[4 * k + 2] = q.z;
+                id[4 * k + 3] = q.w;
+            }
+        }
+    };
+    // Buffer loads, whose completion the compiler counts one by one (it takes the global form for
+    // an access to both memories and waits for everything); their offsets have 32 bits, so
+    // matrices of 2^32 bytes or more take the global form all the same.  Nothing tells the
+    // compiler that a fill writes what is read: arrived<LATER>() stands before the reads, LATER
+    // the number of loads issued after the fill that may still be under way (loads complete in
+    // order), and reads_done() after them.
+    template <int LATER>
+    static __device__ __forceinline__ void arrived() {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LATER) : "memory");
+    }
+    static __device__ __forceinline__ void reads_done() {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    template <bool FULL, bool WIDE>
+    static __device__ __forceinline__ void fill(char* lds, const Ids& ids, const T* base,
+                                                uint32_t stride, int D, int lane) {
+        const __amdgpu_buffer_rsrc_t rsrc =
+            buffer_rsrc(reinterpret_cast<const float*>(base), 0xffffffffu);
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k) {
+            const int piece = (lane % kPieces) ^ ((k + kLoads * (lane / kPieces)) & kFlip);
+            int off = piece * 16;
+            if (!FULL) off = off < D * (int)sizeof(T) ? off : 0;
+            __attribute__((address_space(3))) void* to =
+                (__attribute__((address_space(3))) void*)(lds + k * 1024);
+            if constexpr (WIDE)
+                __builtin_amdgcn_global_load_lds(
+                    (const __attribute__((address_space(1))) void*)((const char*)row_of<T>(
+                                                                        base, ids.id[k], stride) +
+                                                                    off),
+                    to, 16, 0, 0);
+            else
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    rsrc, to, 16, (int)((uint32_t)ids.id[k] * stride + (uint32_t)off), 0, 0, 0);
+        }
+        asm volatile("" ::: "memory");         // later loads stay later
+    }
+    template <bool FULL>
+    static __device__ __forceinline__ void read(RowFrag<T, P>& f, const char* lds, int t, int D,
+                                                int n, int g) {
+        const int row = 16 * t + n;
+        const char* at = lds + row % kLoads * 1024 + row / kLoads * kPieces * 16;
+#pragma unroll
+        for (int s = 0; s < RowFrag<T, P>::kN; ++s) {
+            f.v[s] = *reinterpret_cast<const typename Attn<T>::Vec*>(
+                at + ((4 * s + g) ^ (row & kFlip)) * 16);
+            if (!FULL && s * Attn<T>::kSteps + g * Attn<T>::kAlign >= D)
+                f.v[s] = typename Attn<T>::Vec{};
+        }
     }
 };
 
@@ -182,7 +279,7 @@ struct ColFrag;
 
 template <int P>
 struct ColFrag<float, P> {
-    static constexpr int kW = 4, kBlocks = P / 64, kAcc = kBlocks * kW;
+    static constexpr int kW = 4, kBlocks = P / 64, kAcc = kBlocks * kW, kLoads = 4 * kBlocks;
     float4 v[4][kBlocks];
     template <typename F>
     __device__ __forceinline__ void load(F&& row, int D, int n) {
@@ -213,6 +310,7 @@ struct ColFrag<float, P> {
 template <int P>
 struct ColFrag<uint16_t, P> {
     static constexpr int kW = P >= 128 ? 8 : 4, kBlocks = P / (16 * kW), kAcc = kBlocks * kW;
+    static constexpr int kLoads = 8 * kBlocks;
     using Vec = unsigned __attribute__((ext_vector_type(kW / 2)));
     Vec v[8][kBlocks];
     template <typename F>
@@ -252,45 +350,36 @@ struct ColFrag<uint16_t, P> {
     }
 };
 
+// For items with infinities or NaN in a row that not every tile row has an edge to (the matrix
+// product's 0 times them is NaN): f(edge, column) over the edges of one tile row, the whole wave
+// together.  Rare, so what uses it is only short.
+template <typename F>
+__device__ __forceinline__ void each_edge(const AttnSide& s, int item, int r, F&& f) {
+    const int4 it = s.items[item];
+    int e = s.base[(int64_t)item * 2 * kAttnRows + r];
+    for (int c = it.y; c < it.y + it.z; ++c)
+        for (uint32_t m = s.masks[(int64_t)c * kAttnRows + r]; m; m &= m - 1)
+            f(e++, s.ids[(int64_t)c * kAttnCols + __builtin_ctz(m)]);
+}
+
 __device__ __forceinline__ float attn_f32(float x) { return x; }
 __device__ __forceinline__ float attn_f32(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
-
-// The same sum with the columns of factor 0 left out, one column and component at a time: for
-// steps with infinities or NaN in a row that not every tile row has an edge to (0 times them
-// would be NaN).  Rare: it works on copies in memory, so that the callers' stay in registers.
-template <typename T, int P>
-__device__ __attribute__((noinline)) void mac_exact_mem(const float* w, const int* cols, float* acc,
-                                                        const T* base, int64_t stride, int D) {
-    constexpr int kW = ColFrag<T, P>::kW, kBlocks = ColFrag<T, P>::kBlocks;
-    const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
-#pragma unroll 1
-    for (int j = 0; j < Attn<T>::kRowsPerLane; ++j)
-#pragma unroll 1
-        for (int gg = 0; gg < 4; ++gg) {
-            const float f = __shfl(w[j], gg * 16 + n);   // (every lane takes part)
-            const T* p = base + (int64_t)__shfl(cols[j], gg * 16) * stride;
-            if (f == 0.0f) continue;
-#pragma unroll 1
-            for (int i = 0; i < kBlocks * kW * 4; ++i) {
-                const int b = i / (kW * 4), c = i / 4 % kW, r = i % 4;
-                const int d = b * 16 * kW + kW * (4 * g + r) + c;
-                if (d < D) acc[i] = fmaf(f, attn_f32(p[d]), acc[i]);
-            }
-        }
+__device__ __forceinline__ void attn_st(float* p, float v) { *p = v; }
+__device__ __forceinline__ void attn_st(uint16_t* p, float v) {
+    *p = (uint16_t)(bf16_pack(v, 0.0f) & 0xffffu);
 }
-template <typename T, int P>
-__device__ __forceinline__ void mac_exact(const float* w, const int* cols, v4f* acc, const T* base,
-                                          int64_t stride, int D) {
-    constexpr int kN = ColFrag<T, P>::kAcc, kR = Attn<T>::kRowsPerLane;
-    float t[kN * 4], tw[kR];
-    int tc[kR];
+__device__ __forceinline__ float attn_wave_sum(float v) {
 #pragma unroll
-    for (int i = 0; i < kN * 4; ++i) t[i] = acc[i / 4][i % 4];
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+// sum_e w x over a wave's lanes, components lane + 64 c
+template <typename T>
+__device__ __forceinline__ void add_row(float* acc, float w, const T* x, int D) {
 #pragma unroll
-    for (int i = 0; i < kR; ++i) tw[i] = w[i], tc[i] = cols[i];
-    mac_exact_mem<T, P>(tw, tc, t, base, stride, D);
-#pragma unroll
-    for (int i = 0; i < kN * 4; ++i) acc[i / 4][i % 4] = t[i];
+    for (int c = 0; c < 4; ++c)
+        if (c * 64 + (int)threadIdx.x < D)
+            acc[c] = fmaf(w, attn_f32(x[c * 64 + threadIdx.x]), acc[c]);
 }
 
 template <int N>
@@ -336,19 +425,22 @@ __device__ __forceinline__ void store_rows(O* row, const v4f* acc, float f, int 
 
 // A step of an item: columns it * 16 kTiles .. of the item's chunks.
 template <typename T>
-struct Step {
-    int row[Attn<T>::kTiles];               // column whose row form this lane holds, per tile
-    int col[Attn<T>::kRowsPerLane];         // columns whose column form this lane holds
-    uint32_t mask;                          // tile row n: the step's edges, bit 16 t + 4 g + r
-    __device__ __forceinline__ void load(const AttnSide& s, int chunk, int it, int n, int g) {
-        constexpr int kT = Attn<T>::kTiles;
-        const int c = chunk + it * kT / 2, half = kT == 2 ? 0 : it & 1;
-        const int* ids = s.ids + (int64_t)c * kAttnCols + half * 16;
-        const uint32_t m = s.masks[(int64_t)c * kAttnRows + n];
-        mask = kT == 2 ? m : (m >> (half * 16)) & 0xffffu;
+__device__ __forceinline__ const int* step_ids(const AttnSide& s, int chunk, int it) {
+    return s.ids + (int64_t)chunk * kAttnCols + it * (16 * Attn<T>::kTiles);
+}
+// Tile row n's edges of the step, bit 16 t + 4 g + r.
+template <typename T>
+__device__ __forceinline__ uint32_t step_mask(const AttnSide& s, int chunk, int it, int n) {
+    const uint32_t m = s.masks[((int64_t)chunk + it * Attn<T>::kTiles / 2) * kAttnRows + n];
+    return Attn<T>::kTiles == 2 ? m : (m >> ((it & 1) * 16)) & 0xffffu;
+}
+// The columns of the step whose column form this lane holds.
+template <typename T>
+struct StepCols {
+    int col[Attn<T>::kRowsPerLane];
+    __device__ __forceinline__ void load(const int* ids, int g) {
 #pragma unroll
-        for (int t = 0; t < kT; ++t) {
-            row[t] = ids[16 * t + n];
+        for (int t = 0; t < Attn<T>::kTiles; ++t) {
             const int4 q = *reinterpret_cast<const int4*>(ids + 16 * t + 4 * g);
             col[4 * t] = q.x;
             col[4 * t + 1] = q.y;
@@ -356,11 +448,11 @@ struct Step {
             col[4 * t + 3] = q.w;
         }
     }
-    // place of pair (n, 16 t + 4 g + r) along row n's edges of this step
-    __device__ __forceinline__ int nth(int bit) const {
-        return __popc(mask & ((1u << bit) - 1u));
-    }
 };
+// Place of the pair with bit `bit` along its row's edges of the step.
+__device__ __forceinline__ int nth_edge(uint32_t mask, int bit) {
+    return __popc(mask & ((1u << bit) - 1u));
+}
 
 // ---------------------------------------------------------------------------
 // A wave's values per edge in LDS, in the order of the rows: read from memory once, contiguous,
@@ -389,7 +481,7 @@ struct ItemEdges {
             o[r] = __builtin_amdgcn_readlane(off, r);
             d[r] = __builtin_amdgcn_readlane(base, r) - o[r];
         }
-        for (int i = threadIdx.x & 63; i < total; i += 64) {
+        for (int i = threadIdx.x; i < total; i += 64) {
             int e = d[0], row = 0;
 #pragma unroll
             for (int r = 1; r < kAttnRows; ++r) {
@@ -400,8 +492,6 @@ struct ItemEdges {
         }
     }
 };
-
-constexpr float kLog2e = 1.4426950408889634f;
 
 inline AttnSide side_args(const batmobile_attention_side& s, const int32_t* eid) {
     const PlanLayout p = plan_layout(s.n_rows, s.n_edges);
@@ -426,6 +516,17 @@ inline bool attn_shape_ok(const batmobile_attention_side& s, int H, int Hkv, int
            (s.n_edges == 0 || s.n_cols > 0) && s.n_rows < INT32_MAX / 2 &&
            s.n_edges < INT32_MAX / 4 &&
            (int64_t)s.n_items * H < (int64_t)1 << 32;
+}
+
+inline bool attn_strides_ok(std::initializer_list<int64_t> strides) {
+    for (int64_t s : strides)
+        if (s < 0 || s >= (int64_t)1 << 30) return false;
+    return true;
+}
+
+// Whether rows of n_src at these strides (bytes) lie within 32-bit offsets.
+inline bool attn_wide(int64_t rows, int64_t stride_bytes) {
+    return rows * stride_bytes >= (int64_t)1 << 32;
 }
 
 }  // namespace bmhip

@@ -23,61 +23,127 @@ struct AttnFwd {
     void* out;
     float *stats;                          // [n_dst, H, 2]
     float *part_o, *part_ml;               // [parts, H, 16, Dv], [parts, H, 16, 2]
-    int64_t qs, ks, vs;
+    uint32_t qs, ks, vs;                   // rows' strides in bytes
     int H, group, Dk, Dv;
     float scale;
 };
 
-template <typename T, int KP, int VP, bool FULL, bool BIAS>
-__global__ __launch_bounds__(256, KP + VP <= 256 ? 2 : 1) void attn_fwd_kernel(AttnFwd a) {
+// An item's rows one after the other, each over its own edges alone: infinities or NaN among the
+// values, or more edges than the LDS holds.
+template <typename T>
+__device__ __forceinline__ void attn_fwd_rows(const AttnFwd& a, int item, int h, int4 it4) {
+    constexpr float kInf = __builtin_inff();
+    const int kv = h / a.group;
+    for (int r = 0; r < kAttnRows; ++r) {
+        const int row = a.side.rows[it4.x * kAttnRows + r];
+        if (row < 0) continue;
+        const T* q = row_of<T>(a.q, row, a.qs) + (int64_t)h * a.Dk;
+        float m = -kInf, l = 0.0f, o[4] = {0, 0, 0, 0};
+        each_edge(a.side, item, r, [&](int e, int col) {
+            const float b =
+                a.bias ? a.bias[(int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h] : 0.0f;
+            const T* k = row_of<T>(a.k, col, a.ks) + (int64_t)kv * a.Dk;
+            float s = 0.0f;
+            for (int d = threadIdx.x; d < a.Dk; d += 64) s = fmaf(attn_f32(q[d]), attn_f32(k[d]), s);
+            const float x = fmaf(attn_wave_sum(s), a.scale, b);
+            if (b == -kInf || x == -kInf) return;
+            const float top = fmaxf(m, x), f = attn_exp(m - top);
+            const float p = attn_exp(x - top);
+            m = top;
+            l = l * f + p;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[c] *= f;
+            add_row<T>(o, p, row_of<T>(a.v, col, a.vs) + (int64_t)kv * a.Dv, a.Dv);
+        });
+        const int64_t part = ((int64_t)it4.w * a.H + h) * kAttnRows + r;
+        const int64_t at = (int64_t)row * a.H + h;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int d = c * 64 + threadIdx.x;
+            if (d >= a.Dv) continue;
+            if (it4.w >= 0) a.part_o[part * a.Dv + d] = o[c];
+            else attn_st((T*)a.out + at * a.Dv + d, o[c] * inv);
+        }
+        float* ml = it4.w >= 0 ? a.part_ml + part * 2 : a.stats ? a.stats + at * 2 : nullptr;
+        if (ml && threadIdx.x == 0) {
+            ml[0] = m;
+            ml[1] = l;
+        }
+    }
+}
+
+// A step's loads are in flight over most of the step before: k goes to LDS while the softmax and
+// the second product of the step before run, v to registers over the first product and the
+// softmax.  All reads from LDS stand before the loads to LDS.
+template <typename T, int KP, int VP, bool FULL, bool BIAS, bool WIDE>
+__global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_fwd_kernel(AttnFwd a) {
     constexpr int kT = Attn<T>::kTiles;
     constexpr float kInf = __builtin_inff();
-    __shared__ float lds[BIAS ? 4 * kTileEdges : 1];
+    using Rows = RowTile<T, KP>;
+    __shared__ __attribute__((aligned(1024))) char k_lds[Rows::kBytes];
+    __shared__ float b_lds[BIAS ? kTileEdges : 1];
     int item, h;
     if (!attn_unit(a.side.n_items, a.H, item, h)) return;
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, kv = h / a.group;
+    const int lane = threadIdx.x, n = lane & 15, g = lane >> 4, kv = h / a.group;
     const int4 it4 = a.side.items[item];
     const int row = a.side.rows[it4.x * kAttnRows + n];
-    const int steps = it4.z * 2 / kT;
+    const int steps = it4.z * 2 / kT, last = steps - 1;
     const T* kbase = (const T*)a.k + (int64_t)kv * a.Dk;
     const T* vbase = (const T*)a.v + (int64_t)kv * a.Dv;
     RowFrag<T, KP> q;
     // (a slot past the last row computes with row 0 and stores nothing)
     q.template load<FULL>(row_of<T>(a.q, max(row, 0), a.qs) + (int64_t)h * a.Dk, a.Dk, g);
     ItemEdges edges;
-    float* b_lds = lds + (BIAS ? (threadIdx.x >> 6) * kTileEdges : 0);
-    bool staged = true;
-    auto bias_of = [&](int e) {
-        return a.bias[(int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h];
-    };
     if constexpr (BIAS) {
         edges.load(a.side, item, n);
-        staged = edges.total <= kTileEdges;
-        if (staged) edges.each([&](int i, int e, int) { b_lds[i] = bias_of(e); });
+        if (__builtin_expect(edges.total > kTileEdges, 0)) {
+            attn_fwd_rows<T>(a, item, h, it4);
+            return;
+        }
+        edges.each([&](int i, int e, int) {
+            b_lds[i] = a.bias[(int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h];
+        });
     }
 
     v4f acc[ColFrag<T, VP>::kAcc];
-    float m, l;
-    for (int exact = 0;; ++exact) {
-        m = -kInf;
-        l = 0.0f;
+    float m = -kInf, l = 0.0f;
 #pragma unroll
-        for (int i = 0; i < ColFrag<T, VP>::kAcc; ++i) acc[i] = v4f{0, 0, 0, 0};
+    for (int i = 0; i < ColFrag<T, VP>::kAcc; ++i) acc[i] = v4f{0, 0, 0, 0};
+    {
         int done = 0;                      // row n's edges of earlier steps
-        Step<T> st, next;
-        RowFrag<T, KP> kf[kT];
+        typename Rows::Ids kid;
+        StepCols<T> vid;
+        ColFrag<T, VP> vf;
+        uint32_t mask = 0;
         if (steps > 0) {
-            st.load(a.side, it4.y, 0, n, g);
-            next.load(a.side, it4.y, min(1, steps - 1), n, g);
-#pragma unroll
-            for (int t = 0; t < kT; ++t)
-                kf[t].template load<FULL>(row_of<T>(kbase, st.row[t], a.ks), a.Dk, g);
+            kid.load(step_ids<T>(a.side, it4.y, 0), lane);
+            vid.load(step_ids<T>(a.side, it4.y, 0), g);
+            mask = step_mask<T>(a.side, it4.y, 0, n);
+            Rows::template fill<FULL, WIDE>(k_lds, kid, kbase, a.ks, a.Dk, lane);
+            vf.load([&](int j) { return row_of<T>(vbase, vid.col[j], a.vs); }, a.Dv, n);
+            kid.load(step_ids<T>(a.side, it4.y, min(1, last)), lane);
+            vid.load(step_ids<T>(a.side, it4.y, min(1, last)), g);
         }
         for (int i = 0; i < steps; ++i) {
-            // in flight: this step's v over the first product, the next step's k and the
-            // indices of the one after over the softmax and the second product
-            ColFrag<T, VP> vf;
-            vf.load([&](int j) { return row_of<T>(vbase, st.col[j], a.vs); }, a.Dv, n);
+            float b[4 * kT];
+            RowFrag<T, KP> kf[kT];
+            Rows::template arrived<ColFrag<T, VP>::kLoads>();
+#pragma unroll
+            for (int t = 0; t < kT; ++t) Rows::template read<FULL>(kf[t], k_lds, t, a.Dk, n, g);
+#pragma unroll
+            for (int j = 0; j < 4 * kT; ++j) {
+                b[j] = 0.0f;
+                if constexpr (BIAS) {
+                    const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
+                    const int at = done + nth_edge(mask, bit);
+                    b[j] = b_lds[min(edges.off + at, kTileEdges - 1)];
+                }
+            }
+            Rows::reads_done();
+            Rows::template fill<FULL, WIDE>(k_lds, kid, kbase, a.ks, a.Dk, lane);
+            const int* ids = step_ids<T>(a.side, it4.y, min(i + 2, last));
+            kid.load(ids, lane);
             float x[4 * kT];
 #pragma unroll
             for (int t = 0; t < kT; ++t) {
@@ -85,31 +151,19 @@ __global__ __launch_bounds__(256, KP + VP <= 256 ? 2 : 1) void attn_fwd_kernel(A
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x[4 * t + r] = s[r];
             }
-#pragma unroll
-            for (int t = 0; t < kT; ++t)
-                kf[t].template load<FULL>(row_of<T>(kbase, next.row[t], a.ks), a.Dk, g);
-            Step<T> after;
-            after.load(a.side, it4.y, min(i + 2, steps - 1), n, g);
             float top = m;
 #pragma unroll
             for (int j = 0; j < 4 * kT; ++j) {
                 const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
-                const bool on = (st.mask >> bit) & 1;
-                float b = 0.0f;
-                if constexpr (BIAS) {
-                    const int at = done + st.nth(bit);
-                    if (staged) b = b_lds[min(edges.off + at, kTileEdges - 1)];
-                    else if (on) b = bias_of(edges.base + at);
-                }
-                x[j] = !on || b == -kInf ? -kInf : fmaf(x[j], a.scale, b);
+                const bool on = ((mask >> bit) & 1) & (b[j] != -kInf);
+                x[j] = fmaf(x[j], a.scale, b[j]);
+                x[j] = on ? x[j] : -kInf;
                 top = fmaxf(top, x[j]);
             }
-            done += __popc(st.mask);
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
+            top = max_over_groups(top);
             const float ref = top == -kInf ? 0.0f : top;
             if (__any(top > m)) {
-                const float f = exp2f((m - ref) * kLog2e);
+                const float f = attn_exp(m - ref);
                 l *= f;
 #pragma unroll
                 for (int j = 0; j < ColFrag<T, VP>::kAcc; ++j) acc[j] *= f;
@@ -118,19 +172,21 @@ __global__ __launch_bounds__(256, KP + VP <= 256 ? 2 : 1) void attn_fwd_kernel(A
             float p[4 * kT];
 #pragma unroll
             for (int j = 0; j < 4 * kT; ++j) {
-                p[j] = exp2f((x[j] - ref) * kLog2e);
+                p[j] = attn_exp(x[j] - ref);
                 l += p[j];
             }
-            if (exact) mac_exact<T, VP>(p, st.col, acc, vbase, a.vs, a.Dv);
-            else vf.mac(p, acc);
-            st = next;
-            next = after;
+            vf.mac(p, acc);
+            done += __popc(mask);
+            mask = step_mask<T>(a.side, it4.y, min(i + 1, last), n);
+            vf.load([&](int j) { return row_of<T>(vbase, vid.col[j], a.vs); }, a.Dv, n);
+            vid.load(ids, g);
         }
-        // infinities or NaN: the sums once more, each row over its own edges alone
-        if (exact || !any_not_finite<ColFrag<T, VP>::kAcc>(acc)) break;
     }
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    l = sum_over_groups(l);
+    if (__builtin_expect(any_not_finite<ColFrag<T, VP>::kAcc>(acc), 0)) {
+        attn_fwd_rows<T>(a, item, h, it4);
+        return;
+    }
     if (row < 0) return;
     if (it4.w >= 0) {
         const int64_t at = ((int64_t)it4.w * a.H + h) * kAttnRows + n;
@@ -175,7 +231,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnFwd a) {
         float l = 0.0f, o[4] = {0, 0, 0, 0};
         for (int p = w; p < parts; p += 4) {
             const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at(p) * 2);
-            const float f = exp2f((ml.x - ref) * kLog2e);
+            const float f = attn_exp(ml.x - ref);
             l = fmaf(ml.y, f, l);
             if (4 * lane < a.Dv) {
                 const float4 x = *reinterpret_cast<const float4*>(a.part_o + at(p) * a.Dv + 4 * lane);
@@ -207,25 +263,27 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnFwd a) {
 }
 
 template <typename T, int KP, int VP>
-static void attn_fwd_launch(const AttnFwd& a, hipStream_t s) {
+static void attn_fwd_launch(const AttnFwd& a, bool wide, hipStream_t s) {
     const unsigned grid = attn_grid(a.side.n_items, a.H);
     const bool full = a.Dk == KP;
-    if (a.bias && full) attn_fwd_kernel<T, KP, VP, true, true><<<grid, 256, 0, s>>>(a);
-    else if (a.bias) attn_fwd_kernel<T, KP, VP, false, true><<<grid, 256, 0, s>>>(a);
-    else if (full) attn_fwd_kernel<T, KP, VP, true, false><<<grid, 256, 0, s>>>(a);
-    else attn_fwd_kernel<T, KP, VP, false, false><<<grid, 256, 0, s>>>(a);
+    if (wide && a.bias) attn_fwd_kernel<T, KP, VP, false, true, true><<<grid, 64, 0, s>>>(a);
+    else if (wide) attn_fwd_kernel<T, KP, VP, false, false, true><<<grid, 64, 0, s>>>(a);
+    else if (a.bias && full) attn_fwd_kernel<T, KP, VP, true, true, false><<<grid, 64, 0, s>>>(a);
+    else if (a.bias) attn_fwd_kernel<T, KP, VP, false, true, false><<<grid, 64, 0, s>>>(a);
+    else if (full) attn_fwd_kernel<T, KP, VP, true, false, false><<<grid, 64, 0, s>>>(a);
+    else attn_fwd_kernel<T, KP, VP, false, false, false><<<grid, 64, 0, s>>>(a);
 }
 template <typename T, int KP>
-static void attn_fwd_pick_v(const AttnFwd& a, hipStream_t s) {
-    if (a.Dv <= 64) attn_fwd_launch<T, KP, 64>(a, s);
-    else if (a.Dv <= 128) attn_fwd_launch<T, KP, 128>(a, s);
-    else attn_fwd_launch<T, KP, 256>(a, s);
+static void attn_fwd_pick_v(const AttnFwd& a, bool wide, hipStream_t s) {
+    if (a.Dv <= 64) attn_fwd_launch<T, KP, 64>(a, wide, s);
+    else if (a.Dv <= 128) attn_fwd_launch<T, KP, 128>(a, wide, s);
+    else attn_fwd_launch<T, KP, 256>(a, wide, s);
 }
 template <typename T>
-static void attn_fwd_run(const AttnFwd& a, int parts, hipStream_t s) {
-    if (a.Dk <= 64) attn_fwd_pick_v<T, 64>(a, s);
-    else if (a.Dk <= 128) attn_fwd_pick_v<T, 128>(a, s);
-    else attn_fwd_pick_v<T, 256>(a, s);
+static void attn_fwd_run(const AttnFwd& a, bool wide, int parts, hipStream_t s) {
+    if (a.Dk <= 64) attn_fwd_pick_v<T, 64>(a, wide, s);
+    else if (a.Dk <= 128) attn_fwd_pick_v<T, 128>(a, wide, s);
+    else attn_fwd_pick_v<T, 256>(a, wide, s);
     if (parts)
         attn_join_kernel<T><<<dim3((unsigned)parts, (unsigned)a.H), 256, 0, s>>>(a);
 }
@@ -249,7 +307,7 @@ extern "C" int batteries_neighbor_attention(const void* q, const void* k, const 
     if (!side || !attn_shape_ok(*side, H, Hkv, Dk, Dv, dtype)) return BM_ERR_ARG;
     const int align = dtype == 0 ? 4 : 8;
     if (Dk % align || Dv % align || q_stride % align || k_stride % align || v_stride % align ||
-        !aligned_to({q, k, v, out}, 16))
+        !attn_strides_ok({q_stride, k_stride, v_stride}) || !aligned_to({q, k, v, out}, 16))
         return BM_ERR_ARG;
     if (side->n_rows == 0) return BM_OK;
     const size_t need = batteries_neighbor_attention_workspace_bytes(side->n_parts, H, Dv);
@@ -259,9 +317,12 @@ extern "C" int batteries_neighbor_attention(const void* q, const void* k, const 
     a.q = q; a.k = k; a.v = v; a.bias = bias; a.out = out; a.stats = stats;
     a.part_o = (float*)workspace;
     a.part_ml = a.part_o + (size_t)side->n_parts * H * kAttnRows * Dv;
-    a.qs = q_stride; a.ks = k_stride; a.vs = v_stride;
+    const int64_t size = dtype == 0 ? 4 : 2;
+    a.qs = (uint32_t)(q_stride * size); a.ks = (uint32_t)(k_stride * size);
+    a.vs = (uint32_t)(v_stride * size);
     a.H = H; a.group = H / Hkv; a.Dk = Dk; a.Dv = Dv; a.scale = scale;
-    if (dtype == 0) attn_fwd_run<float>(a, side->n_parts, stream);
-    else attn_fwd_run<uint16_t>(a, side->n_parts, stream);
+    const bool wide = attn_wide(side->n_cols, k_stride * size);
+    if (dtype == 0) attn_fwd_run<float>(a, wide, side->n_parts, stream);
+    else attn_fwd_run<uint16_t>(a, wide, side->n_parts, stream);
     return (int)hipGetLastError();
 }

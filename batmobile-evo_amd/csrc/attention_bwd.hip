@@ -25,35 +25,84 @@ struct AttnScores {
     const float *bias, *stats;
     float* gbias;
     float2* ws;                            // [H][E]: p, ds (of cut tiles first dp)
-    int64_t qs, ks, vs, gs, edges;
+    uint32_t qs, ks, vs, gs;               // rows' strides in bytes
+    int64_t edges;
     int H, group, Dk, Dv;
     float scale;
 };
 
-template <typename T, int KP, int VP, bool FULL>
-__global__ __launch_bounds__(256, KP + VP <= 256 ? 2 : 1) void attn_scores_kernel(AttnScores a) {
+// An item's rows one after the other (more edges than the LDS holds): p and dp, and D and ds of a
+// tile that is not cut.
+template <typename T>
+__device__ __forceinline__ void attn_scores_rows(const AttnScores& a, int item, int h, int4 it4) {
+    constexpr float kInf = __builtin_inff();
+    const int kv = h / a.group;
+    float2* ws = a.ws + (int64_t)h * a.edges;
+    for (int r = 0; r < kAttnRows; ++r) {
+        const int row = a.side.rows[it4.x * kAttnRows + r];
+        if (row < 0) continue;
+        const T* q = row_of<T>(a.q, row, a.qs) + (int64_t)h * a.Dk;
+        const T* go = row_of<T>(a.go, row, a.gs) + (int64_t)h * a.Dv;
+        const float* ml = a.stats + ((int64_t)row * a.H + h) * 2;
+        const float ref = ml[0] == -kInf ? 0.0f : ml[0], inv = ml[1] == 0.0f ? 0.0f : 1.0f / ml[1];
+        float d = 0.0f;
+        each_edge(a.side, item, r, [&](int e, int col) {
+            const float b =
+                a.bias ? a.bias[(int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h] : 0.0f;
+            const T* k = row_of<T>(a.k, col, a.ks) + (int64_t)kv * a.Dk;
+            const T* v = row_of<T>(a.v, col, a.vs) + (int64_t)kv * a.Dv;
+            float s = 0.0f, y = 0.0f;
+            for (int c = threadIdx.x; c < a.Dk; c += 64) s = fmaf(attn_f32(q[c]), attn_f32(k[c]), s);
+            for (int c = threadIdx.x; c < a.Dv; c += 64)
+                y = fmaf(attn_f32(go[c]), attn_f32(v[c]), y);
+            const float x = fmaf(attn_wave_sum(s), a.scale, b);
+            const float p = b == -kInf || x == -kInf ? 0.0f : attn_exp(x - ref) * inv;
+            y = attn_wave_sum(y);
+            y = p == 0.0f ? 0.0f : y;
+            d = fmaf(p, y, d);
+            if (threadIdx.x == 0) ws[e] = make_float2(p, y);
+        });
+        if (it4.w >= 0) continue;
+        __threadfence_block();
+        each_edge(a.side, item, r, [&](int e, int) {
+            const float2 w = ws[e];
+            const float ds = w.x == 0.0f ? 0.0f : w.x * (w.y - d);
+            if (threadIdx.x != 0) return;
+            ws[e].y = ds;
+            if (a.gbias) a.gbias[(int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h] = ds;
+        });
+    }
+}
+
+// k and v of a step go to LDS while the products of the step before run; p and dp of the step
+// before are written to LDS first, as are all reads done (attn_fwd_kernel).
+template <typename T, int KP, int VP, bool FULL, bool WIDE>
+__global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_scores_kernel(AttnScores a) {
     constexpr int kT = Attn<T>::kTiles;
     constexpr float kInf = __builtin_inff();
-    __shared__ float lds_p[4][kTileEdges];           // the bias, then p
-    __shared__ float lds_dp[4][kTileEdges];
-    __shared__ float lds_d[4][kAttnRows];
+    using KRows = RowTile<T, KP>;
+    using VRows = RowTile<T, VP>;
+    __shared__ __attribute__((aligned(1024))) char k_lds[KRows::kBytes];
+    __shared__ __attribute__((aligned(1024))) char v_lds[VRows::kBytes];
+    __shared__ float p_lds[kTileEdges];              // the bias, then p
+    __shared__ float dp_lds[kTileEdges];
+    __shared__ float d_lds[kAttnRows];
     int item, h;
     if (!attn_unit(a.side.n_items, a.H, item, h)) return;
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, kv = h / a.group;
+    const int lane = threadIdx.x, n = lane & 15, g = lane >> 4, kv = h / a.group;
     const int4 it4 = a.side.items[item];
     const int row = a.side.rows[it4.x * kAttnRows + n];
-    const int steps = it4.z * 2 / kT;
+    const int steps = it4.z * 2 / kT, last = steps - 1;
     if (steps == 0) return;
     const T* kbase = (const T*)a.k + (int64_t)kv * a.Dk;
     const T* vbase = (const T*)a.v + (int64_t)kv * a.Dv;
-    Step<T> st, next;
-    st.load(a.side, it4.y, 0, n, g);
-    next.load(a.side, it4.y, min(1, steps - 1), n, g);
-    RowFrag<T, KP> kf[kT], q;
+    typename KRows::Ids kid;
+    typename VRows::Ids vid;
+    kid.load(step_ids<T>(a.side, it4.y, 0), lane);
+    vid.load(step_ids<T>(a.side, it4.y, 0), lane);
+    uint32_t mask = step_mask<T>(a.side, it4.y, 0, n);
+    RowFrag<T, KP> q;
     RowFrag<T, VP> go;
-#pragma unroll
-    for (int t = 0; t < kT; ++t)
-        kf[t].template load<FULL>(row_of<T>(kbase, st.row[t], a.ks), a.Dk, g);
     q.template load<FULL>(row_of<T>(a.q, max(row, 0), a.qs) + (int64_t)h * a.Dk, a.Dk, g);
     go.template load<FULL>(row_of<T>(a.go, max(row, 0), a.gs) + (int64_t)h * a.Dv, a.Dv, g);
     const float2 ml =
@@ -61,75 +110,92 @@ __global__ __launch_bounds__(256, KP + VP <= 256 ? 2 : 1) void attn_scores_kerne
     const float ref = ml.x == -kInf ? 0.0f : ml.x, inv = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
     ItemEdges edges;
     edges.load(a.side, item, n);
-    float* p_lds = lds_p[threadIdx.x >> 6];
-    float* dp_lds = lds_dp[threadIdx.x >> 6];
-    const bool staged = edges.total <= kTileEdges;
-    auto place = [&](int e) { return (int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h; };
-    if (staged && a.bias) edges.each([&](int i, int e, int) { p_lds[i] = a.bias[place(e)]; });
-    float2* ws = a.ws + (int64_t)h * a.edges;
-    float d = 0.0f;
-    int done = 0;                              // row n's edges of earlier steps
-    for (int i = 0; i < steps; ++i) {
-        RowFrag<T, VP> vf[kT];
-#pragma unroll
-        for (int t = 0; t < kT; ++t)
-            vf[t].template load<FULL>(row_of<T>(vbase, st.row[t], a.vs), a.Dv, g);
-        v4f s[kT], dp[kT];
-#pragma unroll
-        for (int t = 0; t < kT; ++t) s[t] = row_product<T, KP>(kf[t], q);
-#pragma unroll
-        for (int t = 0; t < kT; ++t)
-            kf[t].template load<FULL>(row_of<T>(kbase, next.row[t], a.ks), a.Dk, g);
-        Step<T> after;
-        after.load(a.side, it4.y, min(i + 2, steps - 1), n, g);
-        float p[4 * kT];
-#pragma unroll
-        for (int j = 0; j < 4 * kT; ++j) {
-            const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
-            const bool on = (st.mask >> bit) & 1;
-            const int at = done + st.nth(bit);
-            float b = 0.0f;
-            if (a.bias) {
-                if (staged) b = p_lds[min(edges.off + at, kTileEdges - 1)];
-                else if (on) b = a.bias[place(edges.base + at)];
-            }
-            const float x = fmaf(s[j >> 2][j & 3], a.scale, b);
-            p[j] = !on || b == -kInf || x == -kInf ? 0.0f : exp2f((x - ref) * kLog2e) * inv;
-        }
-#pragma unroll
-        for (int t = 0; t < kT; ++t) dp[t] = row_product<T, VP>(vf[t], go);
-#pragma unroll
-        for (int j = 0; j < 4 * kT; ++j) {
-            const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
-            const float y = p[j] == 0.0f ? 0.0f : dp[j >> 2][j & 3];
-            d = fmaf(p[j], y, d);
-            if ((st.mask >> bit) & 1) {
-                const int at = done + st.nth(bit);
-                if (staged) {
-                    p_lds[edges.off + at] = p[j];
-                    dp_lds[edges.off + at] = y;
-                } else {
-                    ws[edges.base + at] = make_float2(p[j], y);
-                }
-            }
-        }
-        done += __popc(st.mask);
-        st = next;
-        next = after;
+    if (__builtin_expect(edges.total > kTileEdges, 0)) {
+        attn_scores_rows<T>(a, item, h, it4);
+        return;
     }
-    if (!staged) return;
+    auto place = [&](int e) { return (int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h; };
+    edges.each([&](int i, int e, int) { p_lds[i] = a.bias ? a.bias[place(e)] : 0.0f; });
+    KRows::template fill<FULL, WIDE>(k_lds, kid, kbase, a.ks, a.Dk, lane);
+    VRows::template fill<FULL, WIDE>(v_lds, vid, vbase, a.vs, a.Dv, lane);
+    kid.load(step_ids<T>(a.side, it4.y, min(1, last)), lane);
+    vid.load(step_ids<T>(a.side, it4.y, min(1, last)), lane);
+    float2* ws = a.ws + (int64_t)h * a.edges;
+    float d = 0.0f, p[4 * kT], dp[4 * kT];
+    int done = 0, before = 0;                  // row n's edges of earlier steps
+    uint32_t mask_before = 0;
+    auto keep = [&]() {
+#pragma unroll
+        for (int j = 0; j < 4 * kT; ++j) {
+            const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
+            if ((mask_before >> bit) & 1) {
+                const int at = before + nth_edge(mask_before, bit);
+                p_lds[edges.off + at] = p[j];
+                dp_lds[edges.off + at] = dp[j];
+            }
+        }
+    };
+    for (int i = 0; i < steps; ++i) {
+        RowFrag<T, KP> kf[kT];
+        RowFrag<T, VP> vf[kT];
+        KRows::template arrived<0>();
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+            KRows::template read<FULL>(kf[t], k_lds, t, a.Dk, n, g);
+            VRows::template read<FULL>(vf[t], v_lds, t, a.Dv, n, g);
+        }
+        keep();
+        float b[4 * kT];
+#pragma unroll
+        for (int j = 0; j < 4 * kT; ++j) {
+            const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
+            const int at = done + nth_edge(mask, bit);
+            b[j] = p_lds[min(edges.off + at, kTileEdges - 1)];
+        }
+        KRows::reads_done();
+        KRows::template fill<FULL, WIDE>(k_lds, kid, kbase, a.ks, a.Dk, lane);
+        VRows::template fill<FULL, WIDE>(v_lds, vid, vbase, a.vs, a.Dv, lane);
+        const int* ids = step_ids<T>(a.side, it4.y, min(i + 2, last));
+        kid.load(ids, lane);
+        vid.load(ids, lane);
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+            const v4f s = row_product<T, KP>(kf[t], q);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int j = 4 * t + r, bit = 16 * t + 4 * g + r;
+                const float x = fmaf(s[r], a.scale, b[j]);
+                const bool on = ((mask >> bit) & 1) & (b[j] != -kInf) & (x != -kInf);
+                p[j] = attn_exp(x - ref) * inv;
+                p[j] = on ? p[j] : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+            const v4f y = row_product<T, VP>(vf[t], go);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int j = 4 * t + r;
+                dp[j] = p[j] == 0.0f ? 0.0f : y[r];
+                d = fmaf(p[j], dp[j], d);
+            }
+        }
+        before = done;
+        mask_before = mask;
+        done += __popc(mask);
+        mask = step_mask<T>(a.side, it4.y, min(i + 1, last), n);
+    }
+    keep();
     if (it4.w >= 0) {                          // the rest once all parts of the row are there
         edges.each([&](int i, int e, int) { ws[e] = make_float2(p_lds[i], dp_lds[i]); });
         return;
     }
-    d += __shfl_xor(d, 16);
-    d += __shfl_xor(d, 32);
-    float* d_lds = lds_d[threadIdx.x >> 6];
+    d = sum_over_groups(d);
     if (g == 0) d_lds[n] = d;
     __builtin_amdgcn_wave_barrier();
     edges.each([&](int i, int e, int r) {
-        const float p = p_lds[i], ds = p == 0.0f ? 0.0f : p * (dp_lds[i] - d_lds[r]);
-        ws[e] = make_float2(p, ds);
+        const float pe = p_lds[i], ds = pe == 0.0f ? 0.0f : pe * (dp_lds[i] - d_lds[r]);
+        ws[e] = make_float2(pe, ds);
         if (a.gbias) a.gbias[place(e)] = ds;
     });
 }
@@ -182,79 +248,108 @@ struct AttnSum {
     void* out;
     float* part;                           // [parts, heads, 16, D]
     const float2* ws;
-    int64_t xs, edges;
+    uint32_t xs;                           // row stride in bytes
+    int64_t edges;
     int heads, group, D, second;           // heads of out; heads of ws per head of out;
                                            // second: the factor is ws.y
     int x_div;                             // head of x = head of ws / x_div
     float f;
 };
 
+// An item's rows one after the other, each over its own edges of a factor other than 0.
+template <typename T>
+__device__ __forceinline__ void attn_sum_rows(const AttnSum& a, int item, int head, int4 it4) {
+    for (int r = 0; r < kAttnRows; ++r) {
+        const int row = a.side.rows[it4.x * kAttnRows + r];
+        if (row < 0) continue;
+        float o[4] = {0, 0, 0, 0};
+        for (int hh = head * a.group; hh < (head + 1) * a.group; ++hh)
+            each_edge(a.side, item, r, [&](int e, int col) {
+                const float2 pd =
+                    a.ws[(int64_t)hh * a.edges + (a.side.eid ? a.side.eid[e] : e)];
+                const float w = a.second ? pd.y : pd.x;
+                if (w != 0.0f)
+                    add_row<T>(o, w, row_of<T>(a.x, col, a.xs) + (int64_t)(hh / a.x_div) * a.D,
+                               a.D);
+            });
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int d = c * 64 + threadIdx.x;
+            if (d >= a.D) continue;
+            if (it4.w >= 0)
+                a.part[(((int64_t)it4.w * a.heads + head) * kAttnRows + r) * a.D + d] = o[c] * a.f;
+            else
+                attn_st((T*)a.out + ((int64_t)row * a.heads + head) * a.D + d, o[c] * a.f);
+        }
+    }
+}
+
 template <typename T, int P>
-__global__ __launch_bounds__(256, 2) void attn_sum_kernel(AttnSum a) {
+__global__ __launch_bounds__(64, P * sizeof(T) <= 256 || P == 64 ? 2 : 1) void attn_sum_kernel(AttnSum a) {
     constexpr int kT = Attn<T>::kTiles, kR = Attn<T>::kRowsPerLane;
-    __shared__ float lds[4][kTileEdges];
+    __shared__ float w_lds[kTileEdges];
     int item, head;
     if (!attn_unit(a.side.n_items, a.heads, item, head)) return;
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x, n = lane & 15, g = lane >> 4;
     const int4 it4 = a.side.items[item];
     const int row = a.side.rows[it4.x * kAttnRows + n];
-    const int steps = it4.z * 2 / kT;
-    float* w_lds = lds[threadIdx.x >> 6];
+    const int steps = it4.z * 2 / kT, last = steps - 1;
     ItemEdges edges;
     edges.load(a.side, item, n);
-    const bool staged = edges.total <= kTileEdges;
+    if (__builtin_expect(edges.total > kTileEdges, 0)) {
+        attn_sum_rows<T>(a, item, head, it4);
+        return;
+    }
     v4f acc[ColFrag<T, P>::kAcc];
-    for (int exact = 0;; ++exact) {
+    {
 #pragma unroll
         for (int i = 0; i < ColFrag<T, P>::kAcc; ++i) acc[i] = v4f{0, 0, 0, 0};
         for (int hh = head * a.group; steps > 0 && hh < (head + 1) * a.group; ++hh) {
             const T* x = (const T*)a.x + (int64_t)(hh / a.x_div) * a.D;
             const float* ws = reinterpret_cast<const float*>(a.ws + (int64_t)hh * a.edges) +
                               a.second;
-            auto factor = [&](int e) {
-                return ws[(int64_t)(a.side.eid ? a.side.eid[e] : e) * 2];
-            };
             // two steps' rows in turn: one is read while the other is multiplied
-            Step<T> s0, s1;
+            StepCols<T> s0, s1;
+            uint32_t m0 = step_mask<T>(a.side, it4.y, 0, n);
+            uint32_t m1 = step_mask<T>(a.side, it4.y, min(1, last), n);
             ColFrag<T, P> x0, x1;
-            s0.load(a.side, it4.y, 0, n, g);
-            s1.load(a.side, it4.y, min(1, steps - 1), n, g);
-            if (steps == 1) s1.mask = 0;
+            s0.load(step_ids<T>(a.side, it4.y, 0), g);
+            s1.load(step_ids<T>(a.side, it4.y, min(1, last)), g);
             x0.load([&](int j) { return row_of<T>(x, s0.col[j], a.xs); }, a.D, n);
+            s0.load(step_ids<T>(a.side, it4.y, min(2, last)), g);
             __builtin_amdgcn_wave_barrier();
-            if (staged) edges.each([&](int i, int e, int) { w_lds[i] = factor(e); });
+            edges.each([&](int i, int e, int) {
+                w_lds[i] = ws[(int64_t)(a.side.eid ? a.side.eid[e] : e) * 2];
+            });
             __builtin_amdgcn_wave_barrier();
             int done = 0;                      // row n's edges of earlier steps
-            auto mac = [&](const Step<T>& s, const ColFrag<T, P>& f) {
+            auto mac = [&](uint32_t mask, const ColFrag<T, P>& f) {
                 float w[kR];
 #pragma unroll
                 for (int j = 0; j < kR; ++j) {
                     const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
-                    const int at = done + s.nth(bit);
-                    const bool on = (s.mask >> bit) & 1;
-                    float v = 0.0f;
-                    if (staged) v = w_lds[min(edges.off + at, kTileEdges - 1)];
-                    else if (on) v = factor(edges.base + at);
-                    w[j] = on ? v : 0.0f;
+                    const int at = done + nth_edge(mask, bit);
+                    const float v = w_lds[min(edges.off + at, kTileEdges - 1)];
+                    w[j] = (mask >> bit) & 1 ? v : 0.0f;
                 }
-                done += __popc(s.mask);
-                if (exact) mac_exact<T, P>(w, s.col, acc, x, a.xs, a.D);
-                else f.mac(w, acc);
+                done += __popc(mask);
+                f.mac(w, acc);
             };
             for (int i = 0; i < steps; i += 2) {
                 x1.load([&](int j) { return row_of<T>(x, s1.col[j], a.xs); }, a.D, n);
-                Step<T> s2, s3;
-                s2.load(a.side, it4.y, min(i + 2, steps - 1), n, g);
-                s3.load(a.side, it4.y, min(i + 3, steps - 1), n, g);
-                if (i + 3 >= steps) s3.mask = 0;
-                mac(s0, x0);
-                x0.load([&](int j) { return row_of<T>(x, s2.col[j], a.xs); }, a.D, n);
-                mac(s1, x1);
-                s0 = s2;
-                s1 = s3;
+                s1.load(step_ids<T>(a.side, it4.y, min(i + 3, last)), g);
+                mac(m0, x0);
+                m0 = step_mask<T>(a.side, it4.y, min(i + 2, last), n);
+                x0.load([&](int j) { return row_of<T>(x, s0.col[j], a.xs); }, a.D, n);
+                s0.load(step_ids<T>(a.side, it4.y, min(i + 4, last)), g);
+                mac(i + 1 < steps ? m1 : 0, x1);
+                m1 = step_mask<T>(a.side, it4.y, min(i + 3, last), n);
             }
         }
-        if (exact || !any_not_finite<ColFrag<T, P>::kAcc>(acc)) break;
+    }
+    if (__builtin_expect(any_not_finite<ColFrag<T, P>::kAcc>(acc), 0)) {
+        attn_sum_rows<T>(a, item, head, it4);
+        return;
     }
     if (row < 0) return;
     if (it4.w >= 0)
@@ -298,30 +393,32 @@ __global__ __launch_bounds__(256) void attn_sum_join_kernel(AttnSum a) {
 }
 
 template <typename T, int KP, int VP>
-static void attn_scores_launch(const AttnScores& a, hipStream_t s) {
+static void attn_scores_launch(const AttnScores& a, bool wide, hipStream_t s) {
     const unsigned grid = attn_grid(a.side.n_items, a.H);
-    if (a.Dk == KP && a.Dv == VP) attn_scores_kernel<T, KP, VP, true><<<grid, 256, 0, s>>>(a);
-    else attn_scores_kernel<T, KP, VP, false><<<grid, 256, 0, s>>>(a);
+    if (wide) attn_scores_kernel<T, KP, VP, false, true><<<grid, 64, 0, s>>>(a);
+    else if (a.Dk == KP && a.Dv == VP)
+        attn_scores_kernel<T, KP, VP, true, false><<<grid, 64, 0, s>>>(a);
+    else attn_scores_kernel<T, KP, VP, false, false><<<grid, 64, 0, s>>>(a);
 }
 template <typename T, int KP>
-static void attn_scores_run_k(const AttnScores& a, hipStream_t s) {
-    if (a.Dv <= 64) attn_scores_launch<T, KP, 64>(a, s);
-    else if (a.Dv <= 128) attn_scores_launch<T, KP, 128>(a, s);
-    else attn_scores_launch<T, KP, 256>(a, s);
+static void attn_scores_run_k(const AttnScores& a, bool wide, hipStream_t s) {
+    if (a.Dv <= 64) attn_scores_launch<T, KP, 64>(a, wide, s);
+    else if (a.Dv <= 128) attn_scores_launch<T, KP, 128>(a, wide, s);
+    else attn_scores_launch<T, KP, 256>(a, wide, s);
 }
 template <typename T>
-static void attn_scores_run(const AttnScores& a, hipStream_t s) {
-    if (a.Dk <= 64) attn_scores_run_k<T, 64>(a, s);
-    else if (a.Dk <= 128) attn_scores_run_k<T, 128>(a, s);
-    else attn_scores_run_k<T, 256>(a, s);
+static void attn_scores_run(const AttnScores& a, bool wide, hipStream_t s) {
+    if (a.Dk <= 64) attn_scores_run_k<T, 64>(a, wide, s);
+    else if (a.Dk <= 128) attn_scores_run_k<T, 128>(a, wide, s);
+    else attn_scores_run_k<T, 256>(a, wide, s);
 }
 template <typename T>
 static void attn_sum_run(const AttnSum& a, int parts, hipStream_t s) {
     const unsigned grid = attn_grid(a.side.n_items, a.heads);
     if (grid == 0) return;
-    if (a.D <= 64) attn_sum_kernel<T, 64><<<grid, 256, 0, s>>>(a);
-    else if (a.D <= 128) attn_sum_kernel<T, 128><<<grid, 256, 0, s>>>(a);
-    else attn_sum_kernel<T, 256><<<grid, 256, 0, s>>>(a);
+    if (a.D <= 64) attn_sum_kernel<T, 64><<<grid, 64, 0, s>>>(a);
+    else if (a.D <= 128) attn_sum_kernel<T, 128><<<grid, 64, 0, s>>>(a);
+    else attn_sum_kernel<T, 256><<<grid, 64, 0, s>>>(a);
     if (parts)
         attn_sum_join_kernel<T><<<dim3((unsigned)parts, (unsigned)a.heads), 256, 0, s>>>(a);
 }
@@ -356,9 +453,10 @@ extern "C" int batteries_neighbor_attention_backward(
         return BM_ERR_ARG;
     const int align = dtype == 0 ? 4 : 8;
     if (Dk % align || Dv % align || q_stride % align || k_stride % align || v_stride % align ||
-        go_stride % align || !aligned_to({q, k, v, grad_out, grad_q, grad_k, grad_v, workspace}, 16))
+        go_stride % align || !attn_strides_ok({q_stride, k_stride, v_stride, go_stride}) ||
+        !aligned_to({q, k, v, grad_out, grad_q, grad_k, grad_v, workspace}, 16))
         return BM_ERR_ARG;
-    const int64_t E = dst->n_edges;
+    const int64_t E = dst->n_edges, size = dtype == 0 ? 4 : 2;
     const size_t need = batteries_neighbor_attention_backward_workspace_bytes(
         E, dst->n_parts, src->n_parts, H, Hkv, Dk, Dv);
     if (workspace_bytes < need || (need && !workspace)) return BM_ERR_WORKSPACE;
@@ -369,10 +467,12 @@ extern "C" int batteries_neighbor_attention_backward(
         a.side = side_args(*dst, edge_id);
         a.q = q; a.k = k; a.v = v; a.go = grad_out; a.bias = bias; a.stats = stats; a.ws = ws;
         a.gbias = grad_bias;
-        a.qs = q_stride; a.ks = k_stride; a.vs = v_stride; a.gs = go_stride; a.edges = E;
+        a.qs = (uint32_t)(q_stride * size); a.ks = (uint32_t)(k_stride * size);
+        a.vs = (uint32_t)(v_stride * size); a.gs = (uint32_t)(go_stride * size); a.edges = E;
         a.H = H; a.group = H / Hkv; a.Dk = Dk; a.Dv = Dv; a.scale = scale;
-        if (dtype == 0) attn_scores_run<float>(a, stream);
-        else attn_scores_run<uint16_t>(a, stream);
+        const bool wide = attn_wide(dst->n_cols, std::max(k_stride, v_stride) * size);
+        if (dtype == 0) attn_scores_run<float>(a, wide, stream);
+        else attn_scores_run<uint16_t>(a, wide, stream);
         if (dst->n_parts > 0) {
             AttnDs d{side_args(*dst, edge_id), row_ptr, ws, grad_bias, E, H};
             attn_ds_kernel<<<dim3((unsigned)dst->n_parts, (unsigned)H), 1024, 0, stream>>>(d);
@@ -384,7 +484,7 @@ extern "C" int batteries_neighbor_attention_backward(
         if (side.n_rows == 0) return;
         AttnSum a{};
         a.side = side_args(side, at);
-        a.x = x; a.xs = xs; a.out = out; a.part = part; a.ws = ws; a.edges = E; a.heads = heads;
+        a.x = x; a.xs = (uint32_t)(xs * size); a.out = out; a.part = part; a.ws = ws; a.edges = E; a.heads = heads;
         a.group = group; a.x_div = x_div; a.D = D; a.second = second; a.f = f;
         if (dtype == 0) attn_sum_run<float>(a, side.n_parts, stream);
         else attn_sum_run<uint16_t>(a, side.n_parts, stream);
