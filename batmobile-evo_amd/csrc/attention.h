@@ -193,21 +193,6 @@ struct RowTile {
     static constexpr int kPer = 64 / kPieces, kLoads = kRows / kPer;
     static constexpr int kFlip = (kPieces < 16 ? kPieces : 16) - 1;
     static constexpr int kBytes = kLoads * 1024;
-    // the columns of a step whose rows this lane brings pieces of
-    struct Ids {
-        int id[kLoads];
-        __device__ __forceinline__ void load(const int* ids, int lane) {
-            const int4* p = reinterpret_cast<const int4*>(ids + lane / kPieces * kLoads);
-#pragma unroll
-            for (int k = 0; k < kLoads / 4; ++k) {
-                const int4 q = p[k];
-                id[4 * k] = q.x;
-                id[4 * k + 1] = q.y;
-                id[4 * k + 2] = q.z;
-                id[4 * k + 3] = q.w;
-            }
-        }
-    };
     // Buffer loads, whose completion the compiler counts one by one (it takes the global form for
     // an access to both memories and waits for everything); their offsets have 32 bits, so
     // matrices of 2^32 bytes or more take the global form all the same.  Nothing tells the
@@ -222,8 +207,11 @@ struct RowTile {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     template <bool FULL, bool WIDE>
-    static __device__ __forceinline__ void fill(char* lds, const Ids& ids, const T* base,
+    static __device__ __forceinline__ void fill(char* lds, int ids, const T* base,
                                                 uint32_t stride, int D, int lane) {
+        int id[kLoads];
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k) id[k] = __shfl(ids, k + kLoads * (lane / kPieces));
         const __amdgpu_buffer_rsrc_t rsrc =
             buffer_rsrc(reinterpret_cast<const float*>(base), 0xffffffffu);
 #pragma unroll
@@ -236,12 +224,12 @@ struct RowTile {
             if constexpr (WIDE)
                 __builtin_amdgcn_global_load_lds(
                     (const __attribute__((address_space(1))) void*)((const char*)row_of<T>(
-                                                                        base, ids.id[k], stride) +
+                                                                        base, id[k], stride) +
                                                                     off),
                     to, 16, 0, 0);
             else
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                    rsrc, to, 16, (int)((uint32_t)ids.id[k] * stride + (uint32_t)off), 0, 0, 0);
+                    rsrc, to, 16, (int)((uint32_t)id[k] * stride + (uint32_t)off), 0, 0, 0);
         }
         asm volatile("" ::: "memory");         // later loads stay later
     }
@@ -423,30 +411,46 @@ __device__ __forceinline__ void store_rows(O* row, const v4f* acc, float f, int 
         }
 }
 
-// A step of an item: columns it * 16 kTiles .. of the item's chunks.
-template <typename T>
-__device__ __forceinline__ const int* step_ids(const AttnSide& s, int chunk, int it) {
-    return s.ids + (int64_t)chunk * kAttnCols + it * (16 * Attn<T>::kTiles);
+// Loads, and work on what earlier loads bring, stay on their side of it: loads complete in
+// order, so what is needed first must be issued first, and before waiting for others.
+__device__ __forceinline__ void load_fence() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
 }
-// Tile row n's edges of the step, bit 16 t + 4 g + r.
+
+// The steps of an item, as buffer loads (scalar base and step, the lane's own offset).
 template <typename T>
-__device__ __forceinline__ uint32_t step_mask(const AttnSide& s, int chunk, int it, int n) {
-    const uint32_t m = s.masks[((int64_t)chunk + it * Attn<T>::kTiles / 2) * kAttnRows + n];
-    return Attn<T>::kTiles == 2 ? m : (m >> ((it & 1) * 16)) & 0xffffu;
-}
-// The columns of the step whose column form this lane holds.
+struct Steps {
+    __amdgpu_buffer_rsrc_t ids_r, masks_r;
+    int chunk, last, lane4, n4;
+    __device__ __forceinline__ Steps(const AttnSide& s, int4 item, int lane)
+        : ids_r(buffer_rsrc(reinterpret_cast<const float*>(s.ids), 0xffffffffu)),
+          masks_r(buffer_rsrc(reinterpret_cast<const float*>(s.masks), 0xffffffffu)),
+          chunk(item.y), last(item.z * 2 / Attn<T>::kTiles - 1),
+          lane4(lane % (16 * Attn<T>::kTiles) * 4), n4((lane & 15) * 4) {}
+    // columns of step i, lane l the l-th (modulo their number); a lane that needs others takes
+    // them from there
+    __device__ __forceinline__ int ids(int i) const {
+        const uint32_t at = (uint32_t)chunk * (kAttnCols * 4) +
+                            (uint32_t)min(i, last) * (16 * Attn<T>::kTiles * 4);
+        return __builtin_amdgcn_raw_buffer_load_b32(ids_r, lane4, (int)at, 0);
+    }
+    // tile row n's edges of step i, bit 16 t + 4 g + r
+    __device__ __forceinline__ uint32_t mask(int i) const {
+        i = min(i, last);
+        const uint32_t at = (uint32_t)(chunk + i * Attn<T>::kTiles / 2) * (kAttnRows * 4);
+        const uint32_t m = __builtin_amdgcn_raw_buffer_load_b32(masks_r, n4, (int)at, 0);
+        return Attn<T>::kTiles == 2 ? m : (m >> ((i & 1) * 16)) & 0xffffu;
+    }
+};
+// The columns whose column form this lane holds.
 template <typename T>
 struct StepCols {
     int col[Attn<T>::kRowsPerLane];
-    __device__ __forceinline__ void load(const int* ids, int g) {
+    __device__ __forceinline__ StepCols(int ids, int g) {
 #pragma unroll
-        for (int t = 0; t < Attn<T>::kTiles; ++t) {
-            const int4 q = *reinterpret_cast<const int4*>(ids + 16 * t + 4 * g);
-            col[4 * t] = q.x;
-            col[4 * t + 1] = q.y;
-            col[4 * t + 2] = q.z;
-            col[4 * t + 3] = q.w;
-        }
+        for (int j = 0; j < Attn<T>::kRowsPerLane; ++j)
+            col[j] = __shfl(ids, (j >> 2) * 16 + 4 * g + (j & 3));
     }
 };
 // Place of the pair with bit `bit` along its row's edges of the step.

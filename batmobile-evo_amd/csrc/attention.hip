@@ -9,7 +9,8 @@
 //
 // An edge whose b or x is -inf is left out; a row without an edge gives o = 0.
 //
-// One pass over a tile's columns (attention.h) with the running maximum and sum.  x is formed in
+// One pass over a tile's columns (attention.h) with a running reference (the maximum, or up to 8
+// below it) and sum.  x is formed in
 // natural units and the maximum taken off before the factor log2 e, so that a bias of the
 // type's lowest value does not become infinite.
 #include "attention.h"
@@ -77,9 +78,9 @@ __device__ __forceinline__ void attn_fwd_rows(const AttnFwd& a, int item, int h,
 // the second product of the step before run, v to registers over the first product and the
 // softmax.  All reads from LDS stand before the loads to LDS.
 template <typename T, int KP, int VP, bool FULL, bool BIAS, bool WIDE>
-__global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_fwd_kernel(AttnFwd a) {
+__global__ __launch_bounds__(64, (KP + VP) * sizeof(T) <= 1536 ? 2 : 1) void attn_fwd_kernel(AttnFwd a) {
     constexpr int kT = Attn<T>::kTiles;
-    constexpr float kInf = __builtin_inff();
+    constexpr float kInf = __builtin_inff(), kSlack = 8.0f;
     using Rows = RowTile<T, KP>;
     __shared__ __attribute__((aligned(1024))) char k_lds[Rows::kBytes];
     __shared__ float b_lds[BIAS ? kTileEdges : 1];
@@ -88,7 +89,7 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_fwd_kernel(At
     const int lane = threadIdx.x, n = lane & 15, g = lane >> 4, kv = h / a.group;
     const int4 it4 = a.side.items[item];
     const int row = a.side.rows[it4.x * kAttnRows + n];
-    const int steps = it4.z * 2 / kT, last = steps - 1;
+    const int steps = it4.z * 2 / kT;
     const T* kbase = (const T*)a.k + (int64_t)kv * a.Dk;
     const T* vbase = (const T*)a.v + (int64_t)kv * a.Dv;
     RowFrag<T, KP> q;
@@ -112,25 +113,38 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_fwd_kernel(At
     for (int i = 0; i < ColFrag<T, VP>::kAcc; ++i) acc[i] = v4f{0, 0, 0, 0};
     {
         int done = 0;                      // row n's edges of earlier steps
-        typename Rows::Ids kid;
-        StepCols<T> vid;
         ColFrag<T, VP> vf;
         uint32_t mask = 0;
+        int ids = 0;
+        const Steps<T> step(a.side, it4, lane);
+        // v of step i, whose columns `ids` holds; then those of the next step
+        auto load_v = [&](int i) {
+            const StepCols<T> cols(ids, g);
+            ids = step.ids(i + 1);
+            load_fence();
+            vf.load([&](int j) { return row_of<T>(vbase, cols.col[j], a.vs); }, a.Dv, n);
+            load_fence();
+        };
         if (steps > 0) {
-            kid.load(step_ids<T>(a.side, it4.y, 0), lane);
-            vid.load(step_ids<T>(a.side, it4.y, 0), g);
-            mask = step_mask<T>(a.side, it4.y, 0, n);
-            Rows::template fill<FULL, WIDE>(k_lds, kid, kbase, a.ks, a.Dk, lane);
-            vf.load([&](int j) { return row_of<T>(vbase, vid.col[j], a.vs); }, a.Dv, n);
-            kid.load(step_ids<T>(a.side, it4.y, min(1, last)), lane);
-            vid.load(step_ids<T>(a.side, it4.y, min(1, last)), g);
+            ids = step.ids(0);
+            mask = step.mask(0);
+            Rows::template fill<FULL, WIDE>(k_lds, ids, kbase, a.ks, a.Dk, lane);
+            load_v(0);
         }
         for (int i = 0; i < steps; ++i) {
             float b[4 * kT];
-            RowFrag<T, KP> kf[kT];
+            float x[4 * kT];
             Rows::template arrived<ColFrag<T, VP>::kLoads>();
 #pragma unroll
-            for (int t = 0; t < kT; ++t) Rows::template read<FULL>(kf[t], k_lds, t, a.Dk, n, g);
+            for (int t = 0; t < kT; ++t) {
+                RowFrag<T, KP> kf;
+                Rows::template read<FULL>(kf, k_lds, t, a.Dk, n, g);
+                const v4f s = row_product<T, KP>(kf, q);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[4 * t + r] = s[r];
+                // two tiles' fragments at a time would leave no room for a second wave
+                if (kT > 1 && KP + VP > 256) asm volatile("" : "+v"(x[4 * t]) : : "memory");
+            }
 #pragma unroll
             for (int j = 0; j < 4 * kT; ++j) {
                 b[j] = 0.0f;
@@ -141,16 +155,7 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_fwd_kernel(At
                 }
             }
             Rows::reads_done();
-            Rows::template fill<FULL, WIDE>(k_lds, kid, kbase, a.ks, a.Dk, lane);
-            const int* ids = step_ids<T>(a.side, it4.y, min(i + 2, last));
-            kid.load(ids, lane);
-            float x[4 * kT];
-#pragma unroll
-            for (int t = 0; t < kT; ++t) {
-                const v4f s = row_product<T, KP>(kf[t], q);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) x[4 * t + r] = s[r];
-            }
+            Rows::template fill<FULL, WIDE>(k_lds, ids, kbase, a.ks, a.Dk, lane);
             float top = m;
 #pragma unroll
             for (int j = 0; j < 4 * kT; ++j) {
@@ -161,14 +166,17 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_fwd_kernel(At
                 top = fmaxf(top, x[j]);
             }
             top = max_over_groups(top);
-            const float ref = top == -kInf ? 0.0f : top;
-            if (__any(top > m)) {
-                const float f = attn_exp(m - ref);
+            // The sums are scaled to a new reference only where the maximum has left the old one by
+            // more than kSlack: p then stays below e^kSlack, which the fp32 sums have room for.
+            if (__any(top > m + kSlack)) {
+                const float to = top > m + kSlack ? top : m;
+                const float f = m == -kInf ? 0.0f : attn_exp(m - to);
                 l *= f;
 #pragma unroll
                 for (int j = 0; j < ColFrag<T, VP>::kAcc; ++j) acc[j] *= f;
-                m = top;
+                m = to;
             }
+            const float ref = m == -kInf ? 0.0f : m;
             float p[4 * kT];
 #pragma unroll
             for (int j = 0; j < 4 * kT; ++j) {
@@ -177,9 +185,8 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_fwd_kernel(At
             }
             vf.mac(p, acc);
             done += __popc(mask);
-            mask = step_mask<T>(a.side, it4.y, min(i + 1, last), n);
-            vf.load([&](int j) { return row_of<T>(vbase, vid.col[j], a.vs); }, a.Dv, n);
-            vid.load(ids, g);
+            mask = step.mask(i + 1);
+            load_v(i + 1);
         }
     }
     l = sum_over_groups(l);
@@ -207,55 +214,67 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_fwd_kernel(At
 }
 
 // Joins the parts of a cut tile, row by row: workgroup p of the parts takes rows p, p + parts of
-// its tile, ...; its waves take the parts in turn, a lane four components.
+// its tile, ...; groups of D / 4 lanes take the parts in turn, a lane four components.
 template <typename T>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnFwd a) {
-    __shared__ float sm[4], sl[4], so[4][256];
+__global__ __launch_bounds__(1024) void attn_join_kernel(AttnFwd a) {
+    constexpr float kInf = __builtin_inff();
+    __shared__ float sm[16], sl[16], so[1024][4];
     const int h = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int wide = a.Dv / 4, groups = 1024 / wide, k = threadIdx.x / wide, c4 = threadIdx.x % wide;
     int first, parts;
     const int tile = tile_of_part(a.side, blockIdx.x, first, parts);
     for (int slot = (int)blockIdx.x - first; slot < kAttnRows; slot += parts) {
         const int row = a.side.rows[tile * kAttnRows + slot];
         if (row < 0) continue;
-        __syncthreads();
-        constexpr float kInf = __builtin_inff();
         auto at = [&](int p) { return ((int64_t)(first + p) * a.H + h) * kAttnRows + slot; };
-        float m = -kInf;
-        for (int p = threadIdx.x; p < parts; p += 256) m = fmaxf(m, a.part_ml[at(p) * 2]);
-    #pragma unroll
+        float m = -kInf, l = 0.0f;
+        for (int p = threadIdx.x; p < parts; p += 1024) m = fmaxf(m, a.part_ml[at(p) * 2]);
+#pragma unroll
         for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        __syncthreads();
         if (lane == 0) sm[w] = m;
         __syncthreads();
-        m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = fmaxf(m, sm[i]);
         const float ref = m == -kInf ? 0.0f : m;
-        float l = 0.0f, o[4] = {0, 0, 0, 0};
-        for (int p = w; p < parts; p += 4) {
+        for (int p = threadIdx.x; p < parts; p += 1024) {
             const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at(p) * 2);
-            const float f = attn_exp(ml.x - ref);
-            l = fmaf(ml.y, f, l);
-            if (4 * lane < a.Dv) {
-                const float4 x = *reinterpret_cast<const float4*>(a.part_o + at(p) * a.Dv + 4 * lane);
+            l = fmaf(ml.y, attn_exp(ml.x - ref), l);
+        }
+        l = attn_wave_sum(l);
+        if (lane == 0) sl[w] = l;
+        float o[4] = {0, 0, 0, 0};
+        if (k < groups) {
+#pragma unroll 4
+            for (int p = k; p < parts; p += groups) {
                 // a part without an edge of this row holds zeros, and the factor 0
+                const float f = attn_exp(a.part_ml[at(p) * 2] - ref);
+                const float4 x = *reinterpret_cast<const float4*>(a.part_o + at(p) * a.Dv + 4 * c4);
                 o[0] = fmaf(x.x, f, o[0]);
                 o[1] = fmaf(x.y, f, o[1]);
                 o[2] = fmaf(x.z, f, o[2]);
                 o[3] = fmaf(x.w, f, o[3]);
             }
         }
-        if (lane == 0) sl[w] = l;
-    #pragma unroll
-        for (int c = 0; c < 4; ++c) so[w][4 * lane + c] = o[c];
+        *reinterpret_cast<float4*>(so[threadIdx.x]) = make_float4(o[0], o[1], o[2], o[3]);
         __syncthreads();
-        if (w != 0) continue;
-        l = sl[0] + sl[1] + sl[2] + sl[3];
+        if (k != 0) continue;
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) l += sl[i];
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        for (int i = 1; i < groups; ++i) {
+            const float4 x = *reinterpret_cast<const float4*>(so[i * wide + c4]);
+            o[0] += x.x;
+            o[1] += x.y;
+            o[2] += x.z;
+            o[3] += x.w;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[c] *= inv;
         const int64_t to = (int64_t)row * a.H + h;
-    #pragma unroll
-        for (int c = 0; c < 4; ++c)
-            o[c] = (so[0][4 * lane + c] + so[1][4 * lane + c] + so[2][4 * lane + c] +
-                    so[3][4 * lane + c]) * inv;
-        if (4 * lane < a.Dv) attn_store_w<4>((T*)a.out + to * a.Dv + 4 * lane, o);
-        if (a.stats && lane == 0) {
+        attn_store_w<4>((T*)a.out + to * a.Dv + 4 * c4, o);
+        if (a.stats && threadIdx.x == 0) {
             a.stats[to * 2] = m;
             a.stats[to * 2 + 1] = l;
         }
@@ -285,7 +304,7 @@ static void attn_fwd_run(const AttnFwd& a, bool wide, int parts, hipStream_t s) 
     else if (a.Dk <= 128) attn_fwd_pick_v<T, 128>(a, wide, s);
     else attn_fwd_pick_v<T, 256>(a, wide, s);
     if (parts)
-        attn_join_kernel<T><<<dim3((unsigned)parts, (unsigned)a.H), 256, 0, s>>>(a);
+        attn_join_kernel<T><<<dim3((unsigned)parts, (unsigned)a.H), 1024, 0, s>>>(a);
 }
 
 }  // namespace bmhip

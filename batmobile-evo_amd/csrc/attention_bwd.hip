@@ -92,15 +92,13 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_scores_kernel
     const int lane = threadIdx.x, n = lane & 15, g = lane >> 4, kv = h / a.group;
     const int4 it4 = a.side.items[item];
     const int row = a.side.rows[it4.x * kAttnRows + n];
-    const int steps = it4.z * 2 / kT, last = steps - 1;
+    const int steps = it4.z * 2 / kT;
     if (steps == 0) return;
     const T* kbase = (const T*)a.k + (int64_t)kv * a.Dk;
     const T* vbase = (const T*)a.v + (int64_t)kv * a.Dv;
-    typename KRows::Ids kid;
-    typename VRows::Ids vid;
-    kid.load(step_ids<T>(a.side, it4.y, 0), lane);
-    vid.load(step_ids<T>(a.side, it4.y, 0), lane);
-    uint32_t mask = step_mask<T>(a.side, it4.y, 0, n);
+    const Steps<T> step(a.side, it4, lane);
+    int ids = step.ids(0);
+    uint32_t mask = step.mask(0);
     RowFrag<T, KP> q;
     RowFrag<T, VP> go;
     q.template load<FULL>(row_of<T>(a.q, max(row, 0), a.qs) + (int64_t)h * a.Dk, a.Dk, g);
@@ -116,10 +114,9 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_scores_kernel
     }
     auto place = [&](int e) { return (int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h; };
     edges.each([&](int i, int e, int) { p_lds[i] = a.bias ? a.bias[place(e)] : 0.0f; });
-    KRows::template fill<FULL, WIDE>(k_lds, kid, kbase, a.ks, a.Dk, lane);
-    VRows::template fill<FULL, WIDE>(v_lds, vid, vbase, a.vs, a.Dv, lane);
-    kid.load(step_ids<T>(a.side, it4.y, min(1, last)), lane);
-    vid.load(step_ids<T>(a.side, it4.y, min(1, last)), lane);
+    KRows::template fill<FULL, WIDE>(k_lds, ids, kbase, a.ks, a.Dk, lane);
+    VRows::template fill<FULL, WIDE>(v_lds, ids, vbase, a.vs, a.Dv, lane);
+    ids = step.ids(1);
     float2* ws = a.ws + (int64_t)h * a.edges;
     float d = 0.0f, p[4 * kT], dp[4 * kT];
     int done = 0, before = 0;                  // row n's edges of earlier steps
@@ -153,11 +150,9 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_scores_kernel
             b[j] = p_lds[min(edges.off + at, kTileEdges - 1)];
         }
         KRows::reads_done();
-        KRows::template fill<FULL, WIDE>(k_lds, kid, kbase, a.ks, a.Dk, lane);
-        VRows::template fill<FULL, WIDE>(v_lds, vid, vbase, a.vs, a.Dv, lane);
-        const int* ids = step_ids<T>(a.side, it4.y, min(i + 2, last));
-        kid.load(ids, lane);
-        vid.load(ids, lane);
+        KRows::template fill<FULL, WIDE>(k_lds, ids, kbase, a.ks, a.Dk, lane);
+        VRows::template fill<FULL, WIDE>(v_lds, ids, vbase, a.vs, a.Dv, lane);
+        ids = step.ids(i + 2);
 #pragma unroll
         for (int t = 0; t < kT; ++t) {
             const v4f s = row_product<T, KP>(kf[t], q);
@@ -183,7 +178,7 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_scores_kernel
         before = done;
         mask_before = mask;
         done += __popc(mask);
-        mask = step_mask<T>(a.side, it4.y, min(i + 1, last), n);
+        mask = step.mask(i + 1);
     }
     keep();
     if (it4.w >= 0) {                          // the rest once all parts of the row are there
@@ -293,7 +288,7 @@ __global__ __launch_bounds__(64, P * sizeof(T) <= 256 || P == 64 ? 2 : 1) void a
     const int lane = threadIdx.x, n = lane & 15, g = lane >> 4;
     const int4 it4 = a.side.items[item];
     const int row = a.side.rows[it4.x * kAttnRows + n];
-    const int steps = it4.z * 2 / kT, last = steps - 1;
+    const int steps = it4.z * 2 / kT;
     ItemEdges edges;
     edges.load(a.side, item, n);
     if (__builtin_expect(edges.total > kTileEdges, 0)) {
@@ -309,14 +304,19 @@ __global__ __launch_bounds__(64, P * sizeof(T) <= 256 || P == 64 ? 2 : 1) void a
             const float* ws = reinterpret_cast<const float*>(a.ws + (int64_t)hh * a.edges) +
                               a.second;
             // two steps' rows in turn: one is read while the other is multiplied
-            StepCols<T> s0, s1;
-            uint32_t m0 = step_mask<T>(a.side, it4.y, 0, n);
-            uint32_t m1 = step_mask<T>(a.side, it4.y, min(1, last), n);
+            const Steps<T> step(a.side, it4, lane);
             ColFrag<T, P> x0, x1;
-            s0.load(step_ids<T>(a.side, it4.y, 0), g);
-            s1.load(step_ids<T>(a.side, it4.y, min(1, last)), g);
-            x0.load([&](int j) { return row_of<T>(x, s0.col[j], a.xs); }, a.D, n);
-            s0.load(step_ids<T>(a.side, it4.y, min(2, last)), g);
+            int s0 = step.ids(0), s1 = step.ids(1);
+            uint32_t m0 = step.mask(0), m1 = step.mask(1);
+            // the rows of the columns in `ids`; then the columns of step `then`
+            auto load = [&](ColFrag<T, P>& f, int& ids, int then) {
+                const StepCols<T> cols(ids, g);
+                ids = step.ids(then);
+                load_fence();
+                f.load([&](int j) { return row_of<T>(x, cols.col[j], a.xs); }, a.D, n);
+                load_fence();
+            };
+            load(x0, s0, 2);
             __builtin_amdgcn_wave_barrier();
             edges.each([&](int i, int e, int) {
                 w_lds[i] = ws[(int64_t)(a.side.eid ? a.side.eid[e] : e) * 2];
@@ -336,14 +336,12 @@ __global__ __launch_bounds__(64, P * sizeof(T) <= 256 || P == 64 ? 2 : 1) void a
                 f.mac(w, acc);
             };
             for (int i = 0; i < steps; i += 2) {
-                x1.load([&](int j) { return row_of<T>(x, s1.col[j], a.xs); }, a.D, n);
-                s1.load(step_ids<T>(a.side, it4.y, min(i + 3, last)), g);
+                load(x1, s1, i + 3);
                 mac(m0, x0);
-                m0 = step_mask<T>(a.side, it4.y, min(i + 2, last), n);
-                x0.load([&](int j) { return row_of<T>(x, s0.col[j], a.xs); }, a.D, n);
-                s0.load(step_ids<T>(a.side, it4.y, min(i + 4, last)), g);
+                m0 = step.mask(i + 2);
+                load(x0, s0, i + 4);
                 mac(i + 1 < steps ? m1 : 0, x1);
-                m1 = step_mask<T>(a.side, it4.y, min(i + 3, last), n);
+                m1 = step.mask(i + 3);
             }
         }
     }
@@ -361,34 +359,39 @@ __global__ __launch_bounds__(64, P * sizeof(T) <= 256 || P == 64 ? 2 : 1) void a
 
 // Adds the parts of a cut tile, row by row (as attn_join_kernel).
 template <typename T>
-__global__ __launch_bounds__(256) void attn_sum_join_kernel(AttnSum a) {
-    __shared__ float so[4][256];
-    const int head = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+__global__ __launch_bounds__(1024) void attn_sum_join_kernel(AttnSum a) {
+    __shared__ float so[1024][4];
+    const int head = blockIdx.y, wide = a.D / 4, groups = 1024 / wide;
+    const int k = threadIdx.x / wide, c4 = threadIdx.x % wide;
     int first, parts;
     const int tile = tile_of_part(a.side, blockIdx.x, first, parts);
     for (int slot = (int)blockIdx.x - first; slot < kAttnRows; slot += parts) {
         const int row = a.side.rows[tile * kAttnRows + slot];
         if (row < 0) continue;
         float o[4] = {0, 0, 0, 0};
-        if (4 * lane < a.D)
-            for (int p = w; p < parts; p += 4) {
+        if (k < groups) {
+#pragma unroll 4
+            for (int p = k; p < parts; p += groups) {
                 const int64_t at = ((int64_t)(first + p) * a.heads + head) * kAttnRows + slot;
-                const float4 x = *reinterpret_cast<const float4*>(a.part + at * a.D + 4 * lane);
+                const float4 x = *reinterpret_cast<const float4*>(a.part + at * a.D + 4 * c4);
                 o[0] += x.x;
                 o[1] += x.y;
                 o[2] += x.z;
                 o[3] += x.w;
             }
+        }
         __syncthreads();
-#pragma unroll
-        for (int c = 0; c < 4; ++c) so[w][4 * lane + c] = o[c];
+        *reinterpret_cast<float4*>(so[threadIdx.x]) = make_float4(o[0], o[1], o[2], o[3]);
         __syncthreads();
-        if (w != 0 || 4 * lane >= a.D) continue;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            o[c] = so[0][4 * lane + c] + so[1][4 * lane + c] + so[2][4 * lane + c] +
-                   so[3][4 * lane + c];
-        attn_store_w<4>((T*)a.out + ((int64_t)row * a.heads + head) * a.D + 4 * lane, o);
+        if (k != 0) continue;
+        for (int i = 1; i < groups; ++i) {
+            const float4 x = *reinterpret_cast<const float4*>(so[i * wide + c4]);
+            o[0] += x.x;
+            o[1] += x.y;
+            o[2] += x.z;
+            o[3] += x.w;
+        }
+        attn_store_w<4>((T*)a.out + ((int64_t)row * a.heads + head) * a.D + 4 * c4, o);
     }
 }
 
@@ -420,7 +423,7 @@ static void attn_sum_run(const AttnSum& a, int parts, hipStream_t s) {
     else if (a.D <= 128) attn_sum_kernel<T, 128><<<grid, 64, 0, s>>>(a);
     else attn_sum_kernel<T, 256><<<grid, 64, 0, s>>>(a);
     if (parts)
-        attn_sum_join_kernel<T><<<dim3((unsigned)parts, (unsigned)a.heads), 256, 0, s>>>(a);
+        attn_sum_join_kernel<T><<<dim3((unsigned)parts, (unsigned)a.heads), 1024, 0, s>>>(a);
 }
 
 }  // namespace bmhip
