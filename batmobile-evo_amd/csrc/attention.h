@@ -28,9 +28,13 @@ constexpr int kAttnCols = 32;     // columns of a chunk
 constexpr int kPlanHead = 16;     // items, parts, what is wrong
 constexpr int kPlanItems = 0, kPlanParts = 1, kPlanBad = 2;
 
+// An item, read by a wave with one load: tile, first chunk, chunks, part (-1: the tile's only
+// item); the tile's rows (-1 past the end); each row's first edge in the item; their number.
+constexpr int kItemInts = 64, kItemRows = 16, kItemBase = 32, kItemCount = 48;
+
 struct PlanLayout {
     int64_t tiles, max_items, max_chunks;
-    int64_t rows, tile_item, tile_chunk, tile_part, item_tile, items, base, masks, ids, total;
+    int64_t rows, tile_item, tile_chunk, tile_part, items, masks, ids, total;
 };
 
 // A tile of more than kTileEdges edges is cut into items of kCutEdges or more, one with a row of
@@ -53,8 +57,7 @@ inline PlanLayout plan_layout(int64_t n_rows, int64_t n_edges) {
     p.tile_item = take(p.tiles + 1);
     p.tile_chunk = take(p.tiles + 1);
     p.tile_part = take(p.tiles + 1);
-    p.items = take(p.max_items * 4);
-    p.base = take(p.max_items * 2 * kAttnRows);
+    p.items = take(p.max_items * kItemInts);
     p.masks = take(p.max_chunks * kAttnRows);
     p.ids = take(p.max_chunks * kAttnCols);
     p.total = at;
@@ -64,12 +67,11 @@ inline PlanLayout plan_layout(int64_t n_rows, int64_t n_edges) {
 struct AttnSide {
     const int* rows;          // [16 tiles], -1 past the end
     const int* tile_part;     // [tiles + 1] first part
-    const int4* items;        // tile, first chunk, chunks, part (-1: the tile's only item)
-    const int* base;          // [items][2][16] each row's first edge in the item, and their number
+    const int* items;         // [items][64]
     const uint32_t* masks;    // [16 chunks]
     const int* ids;           // [32 chunks] columns
     const int* eid;           // edge -> its place in the arrays per edge (NULL: itself)
-    int n_items, n_tiles;
+    int n_items, n_tiles, n_edges;
 };
 
 // The tile of part p, the tile's first part and their number.
@@ -343,9 +345,9 @@ struct ColFrag<uint16_t, P> {
 // together.  Rare, so what uses it is only short.
 template <typename F>
 __device__ __forceinline__ void each_edge(const AttnSide& s, int item, int r, F&& f) {
-    const int4 it = s.items[item];
-    int e = s.base[(int64_t)item * 2 * kAttnRows + r];
-    for (int c = it.y; c < it.y + it.z; ++c)
+    const int* it = s.items + (int64_t)item * kItemInts;
+    int e = it[kItemBase + r];
+    for (int c = it[1]; c < it[1] + it[2]; ++c)
         for (uint32_t m = s.masks[(int64_t)c * kAttnRows + r]; m; m &= m - 1)
             f(e++, s.ids[(int64_t)c * kAttnCols + __builtin_ctz(m)]);
 }
@@ -411,6 +413,66 @@ __device__ __forceinline__ void store_rows(O* row, const v4f* acc, float f, int 
         }
 }
 
+// ---------------------------------------------------------------------------
+// A wave's item, and its values per edge in LDS in the order of the rows: read from memory once,
+// contiguous along each row, instead of one gather per pair and step.
+// ---------------------------------------------------------------------------
+struct Item {
+    int tile, chunk, chunks, part;         // uniform
+    int row, base, count, off, total;      // of tile row n (lane % 16): its LDS place off; all
+    int longest;                           // uniform
+    __device__ __forceinline__ Item(const AttnSide& s, int item, int lane) {
+        const int v = s.items[(int64_t)item * kItemInts + lane];
+        tile = __builtin_amdgcn_readlane(v, 0);
+        chunk = __builtin_amdgcn_readlane(v, 1);
+        chunks = __builtin_amdgcn_readlane(v, 2);
+        part = __builtin_amdgcn_readlane(v, 3);
+        const int n = lane & 15;
+        row = __shfl(v, kItemRows + n);
+        base = __shfl(v, kItemBase + n);
+        count = __shfl(v, kItemCount + n);
+        // sum and maximum over lanes 0 .. n of a row of 16
+        int x = count, m = count;
+        x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+        m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x111, 0xf, 0xf, false));
+        m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x112, 0xf, 0xf, false));
+        m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x114, 0xf, 0xf, false));
+        m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x118, 0xf, 0xf, false));
+        off = x - count;
+        total = __builtin_amdgcn_readlane(x, 15);
+        longest = __builtin_amdgcn_readlane(m, 15);
+    }
+    // The item's edges, 16 lanes a row and kStage x 64 at a time: get(edge) for all of them (an
+    // edge that exists, also in lanes without one), then put(LDS place, edge, value, k) of tile row
+    // 4 k + g.
+    static constexpr int kStage = 12;      // rows of up to 48 edges in one go
+    template <typename V, typename G, typename P>
+    __device__ __forceinline__ void each(const AttnSide& s, int lane, G&& get, P&& put) const {
+        const int n = lane & 15, g = lane >> 4;
+        int b[4], c[4], o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            b[k] = __shfl(base, 4 * k + g);
+            c[k] = __shfl(count, 4 * k + g);
+            o[k] = __shfl(off, 4 * k + g);
+        }
+        for (int j = n; j - n < longest; j += 4 * kStage) {
+            V v[kStage];
+#pragma unroll
+            for (int u = 0; u < kStage; ++u)
+                v[u] = get(min(b[u & 3] + j + (u >> 2) * 16, s.n_edges - 1));
+#pragma unroll
+            for (int u = 0; u < kStage; ++u) {
+                const int i = j + (u >> 2) * 16;
+                if (i < c[u & 3]) put(o[u & 3] + i, b[u & 3] + i, v[u], u & 3);
+            }
+        }
+    }
+};
+
 // Loads, and work on what earlier loads bring, stay on their side of it: loads complete in
 // order, so what is needed first must be issued first, and before waiting for others.
 __device__ __forceinline__ void load_fence() {
@@ -423,10 +485,10 @@ template <typename T>
 struct Steps {
     __amdgpu_buffer_rsrc_t ids_r, masks_r;
     int chunk, last, lane4, n4;
-    __device__ __forceinline__ Steps(const AttnSide& s, int4 item, int lane)
+    __device__ __forceinline__ Steps(const AttnSide& s, const Item& item, int lane)
         : ids_r(buffer_rsrc(reinterpret_cast<const float*>(s.ids), 0xffffffffu)),
           masks_r(buffer_rsrc(reinterpret_cast<const float*>(s.masks), 0xffffffffu)),
-          chunk(item.y), last(item.z * 2 / Attn<T>::kTiles - 1),
+          chunk(item.chunk), last(item.chunks * 2 / Attn<T>::kTiles - 1),
           lane4(lane % (16 * Attn<T>::kTiles) * 4), n4((lane & 15) * 4) {}
     // columns of step i, lane l the l-th (modulo their number); a lane that needs others takes
     // them from there
@@ -458,57 +520,18 @@ __device__ __forceinline__ int nth_edge(uint32_t mask, int bit) {
     return __popc(mask & ((1u << bit) - 1u));
 }
 
-// ---------------------------------------------------------------------------
-// A wave's values per edge in LDS, in the order of the rows: read from memory once, contiguous,
-// instead of one gather per pair and step.
-// ---------------------------------------------------------------------------
-struct ItemEdges {
-    int base, count, off, total;           // tile row n (lane % 16): first edge, number, LDS place
-    __device__ __forceinline__ void load(const AttnSide& s, int item, int n) {
-        base = s.base[(int64_t)item * 2 * kAttnRows + n];
-        count = s.base[(int64_t)item * 2 * kAttnRows + kAttnRows + n];
-        // sum over lanes 0 .. n of a row of 16
-        int x = count;
-        x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
-        x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-        x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-        x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-        off = x - count;
-        total = __builtin_amdgcn_readlane(x, 15);
-    }
-    // f(place in LDS, edge, tile row) for all edges of the item, 64 at a time
-    template <typename F>
-    __device__ __forceinline__ void each(F&& f) const {
-        int o[kAttnRows], d[kAttnRows];
-#pragma unroll
-        for (int r = 0; r < kAttnRows; ++r) {
-            o[r] = __builtin_amdgcn_readlane(off, r);
-            d[r] = __builtin_amdgcn_readlane(base, r) - o[r];
-        }
-        for (int i = threadIdx.x; i < total; i += 64) {
-            int e = d[0], row = 0;
-#pragma unroll
-            for (int r = 1; r < kAttnRows; ++r) {
-                e = i >= o[r] ? d[r] : e;
-                row = i >= o[r] ? r : row;
-            }
-            f(i, i + e, row);
-        }
-    }
-};
-
 inline AttnSide side_args(const batmobile_attention_side& s, const int32_t* eid) {
     const PlanLayout p = plan_layout(s.n_rows, s.n_edges);
     AttnSide a;
     a.rows = s.plan + p.rows;
     a.tile_part = s.plan + p.tile_part;
-    a.items = reinterpret_cast<const int4*>(s.plan + p.items);
-    a.base = s.plan + p.base;
+    a.items = s.plan + p.items;
     a.masks = reinterpret_cast<const uint32_t*>(s.plan + p.masks);
     a.ids = s.plan + p.ids;
     a.eid = eid;
     a.n_items = s.n_items;
     a.n_tiles = (int)p.tiles;
+    a.n_edges = (int)s.n_edges;
     return a;
 }
 

@@ -32,11 +32,11 @@ struct AttnFwd {
 // An item's rows one after the other, each over its own edges alone: infinities or NaN among the
 // values, or more edges than the LDS holds.
 template <typename T>
-__device__ __forceinline__ void attn_fwd_rows(const AttnFwd& a, int item, int h, int4 it4) {
+__device__ __forceinline__ void attn_fwd_rows(const AttnFwd& a, int item, int h, int tile, int part_at) {
     constexpr float kInf = __builtin_inff();
     const int kv = h / a.group;
     for (int r = 0; r < kAttnRows; ++r) {
-        const int row = a.side.rows[it4.x * kAttnRows + r];
+        const int row = a.side.rows[tile * kAttnRows + r];
         if (row < 0) continue;
         const T* q = row_of<T>(a.q, row, a.qs) + (int64_t)h * a.Dk;
         float m = -kInf, l = 0.0f, o[4] = {0, 0, 0, 0};
@@ -56,17 +56,17 @@ __device__ __forceinline__ void attn_fwd_rows(const AttnFwd& a, int item, int h,
             for (int c = 0; c < 4; ++c) o[c] *= f;
             add_row<T>(o, p, row_of<T>(a.v, col, a.vs) + (int64_t)kv * a.Dv, a.Dv);
         });
-        const int64_t part = ((int64_t)it4.w * a.H + h) * kAttnRows + r;
+        const int64_t part = ((int64_t)part_at * a.H + h) * kAttnRows + r;
         const int64_t at = (int64_t)row * a.H + h;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             const int d = c * 64 + threadIdx.x;
             if (d >= a.Dv) continue;
-            if (it4.w >= 0) a.part_o[part * a.Dv + d] = o[c];
+            if (part_at >= 0) a.part_o[part * a.Dv + d] = o[c];
             else attn_st((T*)a.out + at * a.Dv + d, o[c] * inv);
         }
-        float* ml = it4.w >= 0 ? a.part_ml + part * 2 : a.stats ? a.stats + at * 2 : nullptr;
+        float* ml = part_at >= 0 ? a.part_ml + part * 2 : a.stats ? a.stats + at * 2 : nullptr;
         if (ml && threadIdx.x == 0) {
             ml[0] = m;
             ml[1] = l;
@@ -78,7 +78,7 @@ __device__ __forceinline__ void attn_fwd_rows(const AttnFwd& a, int item, int h,
 // the second product of the step before run, v to registers over the first product and the
 // softmax.  All reads from LDS stand before the loads to LDS.
 template <typename T, int KP, int VP, bool FULL, bool BIAS, bool WIDE>
-__global__ __launch_bounds__(64, (KP + VP) * sizeof(T) <= 1536 ? 2 : 1) void attn_fwd_kernel(AttnFwd a) {
+__global__ __launch_bounds__(64, KP + VP <= 256 ? 3 : (KP + VP) * sizeof(T) <= 1536 ? 2 : 1) void attn_fwd_kernel(AttnFwd a) {
     constexpr int kT = Attn<T>::kTiles;
     constexpr float kInf = __builtin_inff(), kSlack = 8.0f;
     using Rows = RowTile<T, KP>;
@@ -87,24 +87,24 @@ __global__ __launch_bounds__(64, (KP + VP) * sizeof(T) <= 1536 ? 2 : 1) void att
     int item, h;
     if (!attn_unit(a.side.n_items, a.H, item, h)) return;
     const int lane = threadIdx.x, n = lane & 15, g = lane >> 4, kv = h / a.group;
-    const int4 it4 = a.side.items[item];
-    const int row = a.side.rows[it4.x * kAttnRows + n];
-    const int steps = it4.z * 2 / kT;
+    const Item it(a.side, item, lane);
+    const int row = it.row, steps = it.chunks * 2 / kT;
     const T* kbase = (const T*)a.k + (int64_t)kv * a.Dk;
     const T* vbase = (const T*)a.v + (int64_t)kv * a.Dv;
     RowFrag<T, KP> q;
     // (a slot past the last row computes with row 0 and stores nothing)
     q.template load<FULL>(row_of<T>(a.q, max(row, 0), a.qs) + (int64_t)h * a.Dk, a.Dk, g);
-    ItemEdges edges;
     if constexpr (BIAS) {
-        edges.load(a.side, item, n);
-        if (__builtin_expect(edges.total > kTileEdges, 0)) {
-            attn_fwd_rows<T>(a, item, h, it4);
+        if (__builtin_expect(it.total > kTileEdges, 0)) {
+            attn_fwd_rows<T>(a, item, h, it.tile, it.part);
             return;
         }
-        edges.each([&](int i, int e, int) {
-            b_lds[i] = a.bias[(int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h];
-        });
+        auto keep = [&](int i, int, float b, int) { b_lds[i] = b; };
+        if (a.side.eid)
+            it.each<float>(a.side, lane,
+                           [&](int e) { return a.bias[(int64_t)a.side.eid[e] * a.H + h]; }, keep);
+        else
+            it.each<float>(a.side, lane, [&](int e) { return a.bias[(int64_t)e * a.H + h]; }, keep);
     }
 
     v4f acc[ColFrag<T, VP>::kAcc];
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(64, (KP + VP) * sizeof(T) <= 1536 ? 2 : 1) void att
         ColFrag<T, VP> vf;
         uint32_t mask = 0;
         int ids = 0;
-        const Steps<T> step(a.side, it4, lane);
+        const Steps<T> step(a.side, it, lane);
         // v of step i, whose columns `ids` holds; then those of the next step
         auto load_v = [&](int i) {
             const StepCols<T> cols(ids, g);
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(64, (KP + VP) * sizeof(T) <= 1536 ? 2 : 1) void att
                 if constexpr (BIAS) {
                     const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
                     const int at = done + nth_edge(mask, bit);
-                    b[j] = b_lds[min(edges.off + at, kTileEdges - 1)];
+                    b[j] = b_lds[min(it.off + at, kTileEdges - 1)];
                 }
             }
             Rows::reads_done();
@@ -191,12 +191,12 @@ __global__ __launch_bounds__(64, (KP + VP) * sizeof(T) <= 1536 ? 2 : 1) void att
     }
     l = sum_over_groups(l);
     if (__builtin_expect(any_not_finite<ColFrag<T, VP>::kAcc>(acc), 0)) {
-        attn_fwd_rows<T>(a, item, h, it4);
+        attn_fwd_rows<T>(a, item, h, it.tile, it.part);
         return;
     }
     if (row < 0) return;
-    if (it4.w >= 0) {
-        const int64_t at = ((int64_t)it4.w * a.H + h) * kAttnRows + n;
+    if (it.part >= 0) {
+        const int64_t at = ((int64_t)it.part * a.H + h) * kAttnRows + n;
         store_rows<T, VP>(a.part_o + at * a.Dv, acc, 1.0f, a.Dv, g);
         if (g == 0) {
             a.part_ml[at * 2] = m;

@@ -24,7 +24,9 @@ struct AttnScores {
     const void *q, *k, *v, *go;
     const float *bias, *stats;
     float* gbias;
-    float2* ws;                            // [H][E]: p, ds (of cut tiles first dp)
+    const int* place;                      // edge -> its place in the sources' order
+    float2* ws;                            // [H][E], sources' order: p, ds (of cut tiles first dp)
+    float* wd;                             // [H][E], destinations' order: ds
     uint32_t qs, ks, vs, gs;               // rows' strides in bytes
     int64_t edges;
     int H, group, Dk, Dv;
@@ -34,12 +36,13 @@ struct AttnScores {
 // An item's rows one after the other (more edges than the LDS holds): p and dp, and D and ds of a
 // tile that is not cut.
 template <typename T>
-__device__ __forceinline__ void attn_scores_rows(const AttnScores& a, int item, int h, int4 it4) {
+__device__ __forceinline__ void attn_scores_rows(const AttnScores& a, int item, int h,
+                                                 const Item& it) {
     constexpr float kInf = __builtin_inff();
     const int kv = h / a.group;
     float2* ws = a.ws + (int64_t)h * a.edges;
     for (int r = 0; r < kAttnRows; ++r) {
-        const int row = a.side.rows[it4.x * kAttnRows + r];
+        const int row = a.side.rows[it.tile * kAttnRows + r];
         if (row < 0) continue;
         const T* q = row_of<T>(a.q, row, a.qs) + (int64_t)h * a.Dk;
         const T* go = row_of<T>(a.go, row, a.gs) + (int64_t)h * a.Dv;
@@ -60,15 +63,15 @@ __device__ __forceinline__ void attn_scores_rows(const AttnScores& a, int item, 
             y = attn_wave_sum(y);
             y = p == 0.0f ? 0.0f : y;
             d = fmaf(p, y, d);
-            if (threadIdx.x == 0) ws[e] = make_float2(p, y);
+            if (threadIdx.x == 0) ws[a.place[e]] = make_float2(p, y);
         });
-        if (it4.w >= 0) continue;
-        __threadfence_block();
+        if (it.part >= 0) continue;
         each_edge(a.side, item, r, [&](int e, int) {
-            const float2 w = ws[e];
+            if (threadIdx.x != 0) return;      // reads what it wrote itself
+            const float2 w = ws[a.place[e]];
             const float ds = w.x == 0.0f ? 0.0f : w.x * (w.y - d);
-            if (threadIdx.x != 0) return;
-            ws[e].y = ds;
+            ws[a.place[e]].y = ds;
+            a.wd[(int64_t)h * a.edges + e] = ds;
             if (a.gbias) a.gbias[(int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h] = ds;
         });
     }
@@ -86,17 +89,15 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_scores_kernel
     __shared__ __attribute__((aligned(1024))) char v_lds[VRows::kBytes];
     __shared__ float p_lds[kTileEdges];              // the bias, then p
     __shared__ float dp_lds[kTileEdges];
-    __shared__ float d_lds[kAttnRows];
     int item, h;
     if (!attn_unit(a.side.n_items, a.H, item, h)) return;
     const int lane = threadIdx.x, n = lane & 15, g = lane >> 4, kv = h / a.group;
-    const int4 it4 = a.side.items[item];
-    const int row = a.side.rows[it4.x * kAttnRows + n];
-    const int steps = it4.z * 2 / kT;
+    const Item it(a.side, item, lane);
+    const int row = it.row, steps = it.chunks * 2 / kT;
     if (steps == 0) return;
     const T* kbase = (const T*)a.k + (int64_t)kv * a.Dk;
     const T* vbase = (const T*)a.v + (int64_t)kv * a.Dv;
-    const Steps<T> step(a.side, it4, lane);
+    const Steps<T> step(a.side, it, lane);
     int ids = step.ids(0);
     uint32_t mask = step.mask(0);
     RowFrag<T, KP> q;
@@ -106,17 +107,22 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_scores_kernel
     const float2 ml =
         *reinterpret_cast<const float2*>(a.stats + ((int64_t)max(row, 0) * a.H + h) * 2);
     const float ref = ml.x == -kInf ? 0.0f : ml.x, inv = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
-    ItemEdges edges;
-    edges.load(a.side, item, n);
-    if (__builtin_expect(edges.total > kTileEdges, 0)) {
-        attn_scores_rows<T>(a, item, h, it4);
+    if (__builtin_expect(it.total > kTileEdges, 0)) {
+        attn_scores_rows<T>(a, item, h, it);
         return;
     }
-    auto place = [&](int e) { return (int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h; };
-    edges.each([&](int i, int e, int) { p_lds[i] = a.bias ? a.bias[place(e)] : 0.0f; });
     KRows::template fill<FULL, WIDE>(k_lds, ids, kbase, a.ks, a.Dk, lane);
     VRows::template fill<FULL, WIDE>(v_lds, ids, vbase, a.vs, a.Dv, lane);
     ids = step.ids(1);
+    auto keep_bias = [&](int i, int, float b, int) { p_lds[i] = b; };
+    if (!a.bias)
+        it.each<float>(a.side, lane, [](int) { return 0.0f; }, keep_bias);
+    else if (a.side.eid)
+        it.each<float>(a.side, lane,
+                       [&](int e) { return a.bias[(int64_t)a.side.eid[e] * a.H + h]; }, keep_bias);
+    else
+        it.each<float>(a.side, lane, [&](int e) { return a.bias[(int64_t)e * a.H + h]; },
+                       keep_bias);
     float2* ws = a.ws + (int64_t)h * a.edges;
     float d = 0.0f, p[4 * kT], dp[4 * kT];
     int done = 0, before = 0;                  // row n's edges of earlier steps
@@ -127,8 +133,8 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_scores_kernel
             const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
             if ((mask_before >> bit) & 1) {
                 const int at = before + nth_edge(mask_before, bit);
-                p_lds[edges.off + at] = p[j];
-                dp_lds[edges.off + at] = dp[j];
+                p_lds[it.off + at] = p[j];
+                dp_lds[it.off + at] = dp[j];
             }
         }
     };
@@ -147,7 +153,7 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_scores_kernel
         for (int j = 0; j < 4 * kT; ++j) {
             const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
             const int at = done + nth_edge(mask, bit);
-            b[j] = p_lds[min(edges.off + at, kTileEdges - 1)];
+            b[j] = p_lds[min(it.off + at, kTileEdges - 1)];
         }
         KRows::reads_done();
         KRows::template fill<FULL, WIDE>(k_lds, ids, kbase, a.ks, a.Dk, lane);
@@ -181,25 +187,32 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_scores_kernel
         mask = step.mask(i + 1);
     }
     keep();
-    if (it4.w >= 0) {                          // the rest once all parts of the row are there
-        edges.each([&](int i, int e, int) { ws[e] = make_float2(p_lds[i], dp_lds[i]); });
+    auto place = [&](int e) { return a.place[e]; };
+    if (it.part >= 0) {                        // the rest once all parts of the row are there
+        it.each<int>(a.side, lane, place, [&](int i, int, int to, int) {
+            ws[to] = make_float2(p_lds[i], dp_lds[i]);
+        });
         return;
     }
     d = sum_over_groups(d);
-    if (g == 0) d_lds[n] = d;
-    __builtin_amdgcn_wave_barrier();
-    edges.each([&](int i, int e, int r) {
-        const float pe = p_lds[i], ds = pe == 0.0f ? 0.0f : pe * (dp_lds[i] - d_lds[r]);
-        ws[e] = make_float2(pe, ds);
-        if (a.gbias) a.gbias[place(e)] = ds;
+    float dr[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) dr[k] = __shfl(d, 4 * k + g);
+    float* wd = a.wd + (int64_t)h * a.edges;
+    it.each<int>(a.side, lane, place, [&](int i, int e, int to, int k) {
+        const float pe = p_lds[i], ds = pe == 0.0f ? 0.0f : pe * (dp_lds[i] - dr[k]);
+        ws[to] = make_float2(pe, ds);
+        wd[e] = ds;
+        if (a.gbias) a.gbias[(int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h] = ds;
     });
 }
 
 struct AttnDs {
     AttnSide side;
     const int64_t* row_ptr;
+    const int* place;
     float2* ws;
-    float* gbias;
+    float *wd, *gbias;
     int64_t edges;
     int H;
 };
@@ -217,7 +230,7 @@ __global__ __launch_bounds__(1024) void attn_ds_kernel(AttnDs a) {
         float2* ws = a.ws + (int64_t)h * a.edges;
         float d = 0.0f;
         for (int64_t e = e0 + threadIdx.x; e < e1; e += 1024) {
-            const float2 w = ws[e];
+            const float2 w = ws[a.place[e]];
             d += w.x == 0.0f ? 0.0f : w.x * w.y;
         }
 #pragma unroll
@@ -228,9 +241,10 @@ __global__ __launch_bounds__(1024) void attn_ds_kernel(AttnDs a) {
         d = 0.0f;
         for (int i = 0; i < 16; ++i) d += sh[i];
         for (int64_t e = e0 + threadIdx.x; e < e1; e += 1024) {
-            const float2 w = ws[e];
-            const float ds = w.x == 0.0f ? 0.0f : w.x * (w.y - d);
-            ws[e].y = ds;
+            float2* at = ws + a.place[e];
+            const float ds = at->x == 0.0f ? 0.0f : at->x * (at->y - d);
+            at->y = ds;
+            a.wd[(int64_t)h * a.edges + e] = ds;
             if (a.gbias) a.gbias[(int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h] = ds;
         }
     }
@@ -238,31 +252,30 @@ __global__ __launch_bounds__(1024) void attn_ds_kernel(AttnDs a) {
 
 // out[row, head] = f sum over the row's edges and the head's group of w x[column, head of x]
 struct AttnSum {
-    AttnSide side;                         // eid: edge -> its place in ws
+    AttnSide side;
     const void* x;
     void* out;
     float* part;                           // [parts, heads, 16, D]
-    const float2* ws;
+    const float* w;                        // [H][E], w_step apart, in the side's order
     uint32_t xs;                           // row stride in bytes
+    int w_step;
     int64_t edges;
-    int heads, group, D, second;           // heads of out; heads of ws per head of out;
-                                           // second: the factor is ws.y
+    int heads, group, D;                   // heads of out; heads of w per head of out
     int x_div;                             // head of x = head of ws / x_div
     float f;
 };
 
 // An item's rows one after the other, each over its own edges of a factor other than 0.
 template <typename T>
-__device__ __forceinline__ void attn_sum_rows(const AttnSum& a, int item, int head, int4 it4) {
+__device__ __forceinline__ void attn_sum_rows(const AttnSum& a, int item, int head,
+                                              const Item& it) {
     for (int r = 0; r < kAttnRows; ++r) {
-        const int row = a.side.rows[it4.x * kAttnRows + r];
+        const int row = a.side.rows[it.tile * kAttnRows + r];
         if (row < 0) continue;
         float o[4] = {0, 0, 0, 0};
         for (int hh = head * a.group; hh < (head + 1) * a.group; ++hh)
             each_edge(a.side, item, r, [&](int e, int col) {
-                const float2 pd =
-                    a.ws[(int64_t)hh * a.edges + (a.side.eid ? a.side.eid[e] : e)];
-                const float w = a.second ? pd.y : pd.x;
+                const float w = a.w[((int64_t)hh * a.edges + e) * a.w_step];
                 if (w != 0.0f)
                     add_row<T>(o, w, row_of<T>(a.x, col, a.xs) + (int64_t)(hh / a.x_div) * a.D,
                                a.D);
@@ -271,8 +284,8 @@ __device__ __forceinline__ void attn_sum_rows(const AttnSum& a, int item, int he
         for (int c = 0; c < 4; ++c) {
             const int d = c * 64 + threadIdx.x;
             if (d >= a.D) continue;
-            if (it4.w >= 0)
-                a.part[(((int64_t)it4.w * a.heads + head) * kAttnRows + r) * a.D + d] = o[c] * a.f;
+            if (it.part >= 0)
+                a.part[(((int64_t)it.part * a.heads + head) * kAttnRows + r) * a.D + d] = o[c] * a.f;
             else
                 attn_st((T*)a.out + ((int64_t)row * a.heads + head) * a.D + d, o[c] * a.f);
         }
@@ -286,13 +299,10 @@ __global__ __launch_bounds__(64, P * sizeof(T) <= 256 || P == 64 ? 2 : 1) void a
     int item, head;
     if (!attn_unit(a.side.n_items, a.heads, item, head)) return;
     const int lane = threadIdx.x, n = lane & 15, g = lane >> 4;
-    const int4 it4 = a.side.items[item];
-    const int row = a.side.rows[it4.x * kAttnRows + n];
-    const int steps = it4.z * 2 / kT;
-    ItemEdges edges;
-    edges.load(a.side, item, n);
-    if (__builtin_expect(edges.total > kTileEdges, 0)) {
-        attn_sum_rows<T>(a, item, head, it4);
+    const Item it(a.side, item, lane);
+    const int row = it.row, steps = it.chunks * 2 / kT;
+    if (__builtin_expect(it.total > kTileEdges, 0)) {
+        attn_sum_rows<T>(a, item, head, it);
         return;
     }
     v4f acc[ColFrag<T, P>::kAcc];
@@ -301,10 +311,9 @@ __global__ __launch_bounds__(64, P * sizeof(T) <= 256 || P == 64 ? 2 : 1) void a
         for (int i = 0; i < ColFrag<T, P>::kAcc; ++i) acc[i] = v4f{0, 0, 0, 0};
         for (int hh = head * a.group; steps > 0 && hh < (head + 1) * a.group; ++hh) {
             const T* x = (const T*)a.x + (int64_t)(hh / a.x_div) * a.D;
-            const float* ws = reinterpret_cast<const float*>(a.ws + (int64_t)hh * a.edges) +
-                              a.second;
+            const float* wh = a.w + (int64_t)hh * a.edges * a.w_step;
             // two steps' rows in turn: one is read while the other is multiplied
-            const Steps<T> step(a.side, it4, lane);
+            const Steps<T> step(a.side, it, lane);
             ColFrag<T, P> x0, x1;
             int s0 = step.ids(0), s1 = step.ids(1);
             uint32_t m0 = step.mask(0), m1 = step.mask(1);
@@ -318,9 +327,8 @@ __global__ __launch_bounds__(64, P * sizeof(T) <= 256 || P == 64 ? 2 : 1) void a
             };
             load(x0, s0, 2);
             __builtin_amdgcn_wave_barrier();
-            edges.each([&](int i, int e, int) {
-                w_lds[i] = ws[(int64_t)(a.side.eid ? a.side.eid[e] : e) * 2];
-            });
+            it.each<float>(a.side, lane, [&](int e) { return wh[(int64_t)e * a.w_step]; },
+                           [&](int i, int, float w, int) { w_lds[i] = w; });
             __builtin_amdgcn_wave_barrier();
             int done = 0;                      // row n's edges of earlier steps
             auto mac = [&](uint32_t mask, const ColFrag<T, P>& f) {
@@ -329,7 +337,7 @@ __global__ __launch_bounds__(64, P * sizeof(T) <= 256 || P == 64 ? 2 : 1) void a
                 for (int j = 0; j < kR; ++j) {
                     const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
                     const int at = done + nth_edge(mask, bit);
-                    const float v = w_lds[min(edges.off + at, kTileEdges - 1)];
+                    const float v = w_lds[min(it.off + at, kTileEdges - 1)];
                     w[j] = (mask >> bit) & 1 ? v : 0.0f;
                 }
                 done += __popc(mask);
@@ -346,12 +354,12 @@ __global__ __launch_bounds__(64, P * sizeof(T) <= 256 || P == 64 ? 2 : 1) void a
         }
     }
     if (__builtin_expect(any_not_finite<ColFrag<T, P>::kAcc>(acc), 0)) {
-        attn_sum_rows<T>(a, item, head, it4);
+        attn_sum_rows<T>(a, item, head, it);
         return;
     }
     if (row < 0) return;
-    if (it4.w >= 0)
-        store_rows<T, P>(a.part + (((int64_t)it4.w * a.heads + head) * kAttnRows + n) * a.D, acc,
+    if (it.part >= 0)
+        store_rows<T, P>(a.part + (((int64_t)it.part * a.heads + head) * kAttnRows + n) * a.D, acc,
                          a.f, a.D, g);
     else
         store_rows<T, P>((T*)a.out + ((int64_t)row * a.heads + head) * a.D, acc, a.f, a.D, g);
@@ -438,7 +446,7 @@ static size_t bwd_part_floats(int64_t dst_parts, int64_t src_parts, int H, int H
 extern "C" size_t batteries_neighbor_attention_backward_workspace_bytes(
     int64_t n_edges, int64_t dst_parts, int64_t src_parts, int H, int Hkv, int Dk, int Dv) {
     if (n_edges < 0 || dst_parts < 0 || src_parts < 0 || H <= 0 || Hkv <= 0) return 0;
-    return ((size_t)n_edges * H + 1) / 2 * 2 * sizeof(float2) +
+    return ((size_t)n_edges * H + 3) / 4 * 4 * 3 * sizeof(float) +
            bwd_part_floats(dst_parts, src_parts, H, Hkv, Dk, Dv) * sizeof(float);
 }
 
@@ -446,7 +454,7 @@ extern "C" int batteries_neighbor_attention_backward(
     const void* q, const void* k, const void* v, const float* bias, const float* stats,
     const void* grad_out, const int64_t* row_ptr, const int32_t* edge_id,
     const batmobile_attention_side* dst, const batmobile_attention_side* src,
-    const int32_t* src_pos, void* grad_q, void* grad_k, void* grad_v, float* grad_bias, int H,
+    const int32_t* src_place, void* grad_q, void* grad_k, void* grad_v, float* grad_bias, int H,
     int Hkv, int Dk, int Dv, int64_t q_stride, int64_t k_stride, int64_t v_stride,
     int64_t go_stride, float scale, int dtype, void* workspace, size_t workspace_bytes,
     hipStream_t stream) {
@@ -464,11 +472,13 @@ extern "C" int batteries_neighbor_attention_backward(
         E, dst->n_parts, src->n_parts, H, Hkv, Dk, Dv);
     if (workspace_bytes < need || (need && !workspace)) return BM_ERR_WORKSPACE;
     float2* ws = (float2*)workspace;
-    float* part = (float*)(ws + ((size_t)E * H + 1) / 2 * 2);
+    float* wd = (float*)(ws + ((size_t)E * H + 3) / 4 * 4);
+    float* part = wd + ((size_t)E * H + 3) / 4 * 4;
     if (E > 0) {
         AttnScores a{};
         a.side = side_args(*dst, edge_id);
         a.q = q; a.k = k; a.v = v; a.go = grad_out; a.bias = bias; a.stats = stats; a.ws = ws;
+        a.wd = wd; a.place = src_place;
         a.gbias = grad_bias;
         a.qs = (uint32_t)(q_stride * size); a.ks = (uint32_t)(k_stride * size);
         a.vs = (uint32_t)(v_stride * size); a.gs = (uint32_t)(go_stride * size); a.edges = E;
@@ -477,23 +487,23 @@ extern "C" int batteries_neighbor_attention_backward(
         if (dtype == 0) attn_scores_run<float>(a, wide, stream);
         else attn_scores_run<uint16_t>(a, wide, stream);
         if (dst->n_parts > 0) {
-            AttnDs d{side_args(*dst, edge_id), row_ptr, ws, grad_bias, E, H};
+            AttnDs d{side_args(*dst, edge_id), row_ptr, src_place, ws, wd, grad_bias, E, H};
             attn_ds_kernel<<<dim3((unsigned)dst->n_parts, (unsigned)H), 1024, 0, stream>>>(d);
         }
     }
-    auto sum = [&](const batmobile_attention_side& side, const int32_t* at, const void* x,
-                   int64_t xs, void* out, int heads, int group, int x_div, int D, int second,
-                   float f) {
+    auto sum = [&](const batmobile_attention_side& side, const void* x,
+                   int64_t xs, void* out, int heads, int group, int x_div, int D,
+                   const float* w, int w_step, float f) {
         if (side.n_rows == 0) return;
         AttnSum a{};
-        a.side = side_args(side, at);
-        a.x = x; a.xs = (uint32_t)(xs * size); a.out = out; a.part = part; a.ws = ws; a.edges = E; a.heads = heads;
-        a.group = group; a.x_div = x_div; a.D = D; a.second = second; a.f = f;
+        a.side = side_args(side, nullptr);
+        a.x = x; a.xs = (uint32_t)(xs * size); a.out = out; a.part = part; a.edges = E; a.heads = heads;
+        a.group = group; a.x_div = x_div; a.D = D; a.w = w; a.w_step = w_step; a.f = f;
         if (dtype == 0) attn_sum_run<float>(a, side.n_parts, stream);
         else attn_sum_run<uint16_t>(a, side.n_parts, stream);
     };
-    sum(*dst, nullptr, k, k_stride, grad_q, H, 1, H / Hkv, Dk, 1, scale);
-    sum(*src, src_pos, q, q_stride, grad_k, Hkv, H / Hkv, 1, Dk, 1, scale);
-    sum(*src, src_pos, grad_out, go_stride, grad_v, Hkv, H / Hkv, 1, Dv, 0, 1.0f);
+    sum(*dst, k, k_stride, grad_q, H, 1, H / Hkv, Dk, wd, 1, scale);
+    sum(*src, q, q_stride, grad_k, Hkv, H / Hkv, 1, Dk, &ws->y, 2, scale);
+    sum(*src, grad_out, go_stride, grad_v, Hkv, H / Hkv, 1, Dv, &ws->x, 2, 1.0f);
     return (int)hipGetLastError();
 }

@@ -168,16 +168,19 @@ __global__ __launch_bounds__(kPlanThreads) void plan_items_kernel(PlanArgs a) {
         }
         pre[kAttnRows] = n;
     }
+    int* out = a.plan + a.at.items + (int64_t)item * kItemInts;
     if (tid < kAttnRows) {
-        int* base = a.plan + a.at.base + (int64_t)item * 2 * kAttnRows;
-        base[tid] = (int)start[tid];
-        base[kAttnRows + tid] = (int)(stop[tid] - start[tid]);
+        out[kItemRows + tid] = a.plan[a.at.rows + (int64_t)tile * kAttnRows + tid];
+        out[kItemBase + tid] = (int)start[tid];
+        out[kItemCount + tid] = (int)(stop[tid] - start[tid]);
     }
     __syncthreads();
     const int n = pre[kAttnRows];
     uint32_t* masks = reinterpret_cast<uint32_t*>(a.plan) + a.at.masks + chunk0 * kAttnRows;
     int* ids = a.plan + a.at.ids + chunk0 * kAttnCols;
-    int4* out = reinterpret_cast<int4*>(a.plan + a.at.items) + item;
+    auto finish = [&](int chunks, int part_at) {
+        if (tid == 0) *reinterpret_cast<int4*>(out) = make_int4(tile, (int)chunk0, chunks, part_at);
+    };
     const int part_at = parts > 1 ? a.plan[a.at.tile_part + tile] + part : -1;
     auto column = [&](int i, int& r) {               // of the i-th edge, row by row
         r = 0;
@@ -201,7 +204,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_items_kernel(PlanArgs a) {
             for (int b = b0; b < b1; ++b) m |= 1u << b;
             masks[i] = m;
         }
-        if (tid == 0) *out = make_int4(tile, (int)chunk0, chunks, part_at);
+        finish(chunks, part_at);
         return;
     }
     int size = 64;
@@ -275,7 +278,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_items_kernel(PlanArgs a) {
     for (int i = tid; i < chunks * kAttnRows; i += kPlanThreads) masks[i] = mask[i];
     for (int i = total + tid; i < chunks * kAttnCols; i += kPlanThreads)
         ids[i] = (int)(key[n - 1] >> 20);             // read with factor 0
-    if (tid == 0) *out = make_int4(tile, (int)chunk0, chunks, part_at);
+    finish(chunks, part_at);
 }
 
 // A wave per row: offsets in order, columns in range and ascending.

@@ -189,13 +189,13 @@ std::tuple<Tensor, Tensor> neighbor_attention(const Tensor& q_, const Tensor& k_
     return {cut_heads(out, s.Dv), stats};
 }
 
-// src_*: the side of the sources, src_pos the position of its edges in the destinations' order
+// src_*: the side of the sources, src_place the place of every edge in its order
 std::tuple<Tensor, Tensor, Tensor, Tensor> neighbor_attention_backward(
     const Tensor& q_, const Tensor& k_, const Tensor& v_, const OptTensor& bias_,
     const Tensor& stats, const Tensor& grad_, const Tensor& row_ptr, const Tensor& plan,
     int64_t items, int64_t parts, const OptTensor& edge_id, const Tensor& src_plan,
-    int64_t src_items, int64_t src_parts, const Tensor& src_pos, double scale, bool need_bias) {
-    const int64_t E = src_pos.numel();
+    int64_t src_items, int64_t src_parts, const Tensor& src_place, double scale, bool need_bias) {
+    const int64_t E = src_place.numel();
     const AttnShape s = attn_shape(q_, k_, v_, bias_, E);
     check_like(grad_, q_, "grad_out");
     TORCH_CHECK(grad_.dim() == 3 && grad_.size(0) == s.n_dst && grad_.size(1) == s.H &&
@@ -209,7 +209,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> neighbor_attention_backward(
     const batmobile_attention_side src =
         attn_side(src_plan, src_items, src_parts, s.n_src, s.n_dst, E, q_);
     const int32_t* eid = opt_index32(edge_id, q_, E, "edge_id");
-    const int32_t* pos = opt_index32(src_pos, q_, E, "src_pos");
+    const int32_t* pos = opt_index32(src_place, q_, E, "src_place");
     const int64_t* rp = index_ptr(row_ptr, q_, s.n_dst + 1, "row_ptr");
     const Tensor q = heads16(q_), k = heads16(k_), v = heads16(v_), go = heads16(grad_);
     Tensor bias, gbias;
@@ -437,7 +437,7 @@ void register_block_ops(pybind11::module_& m) {
           py::arg("v"), py::arg("bias"), py::arg("stats"), py::arg("grad_out"),
           py::arg("row_ptr"), py::arg("plan"), py::arg("items"), py::arg("parts"),
           py::arg("edge_id"), py::arg("src_plan"), py::arg("src_items"), py::arg("src_parts"),
-          py::arg("src_pos"), py::arg("scale"), py::arg("need_bias") = true,
+          py::arg("src_place"), py::arg("scale"), py::arg("need_bias") = true,
           "(grad_q, grad_k, grad_v, grad_bias or None)");
     m.def("gated_residual_norm", &gated_residual_norm, py::arg("x"), py::arg("y"),
           py::arg("gate"), py::arg("scale"), py::arg("weight_post"), py::arg("weight_pre"),

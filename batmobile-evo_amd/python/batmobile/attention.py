@@ -76,7 +76,7 @@ class AttentionPlan:
 
     def source_side(self):
         """The edges grouped by source, for the backward (built on first use): the side's plan
-        and the position of each of its edges among the destinations'."""
+        and the place of every edge in its order."""
         if self._source_side is None:
             dst = torch.repeat_interleave(
                 torch.arange(self.n_dst, device=self.src.device), self.row_ptr.diff(),
@@ -85,7 +85,9 @@ class AttentionPlan:
             rows = torch.arange(self.n_src + 1, device=self.src.device)
             plan, items, parts, _ = _batmobile.attention_plan(
                 torch.searchsorted(by, rows), dst[pos], self._src_order, self.n_dst, False)
-            self._source_side = (plan, items, parts, pos.int())
+            place = torch.empty_like(pos, dtype=torch.int32)
+            place[pos] = torch.arange(pos.numel(), dtype=torch.int32, device=pos.device)
+            self._source_side = (plan, items, parts, place)
         return self._source_side
 
 

@@ -531,7 +531,7 @@ int batteries_neighbor_attention(const void* q, const void* k, const void* v, co
                                  hipStream_t stream);
 
 /* Gradients of the above: grad_q, grad_k, grad_v contiguous, grad_bias [E, H] or NULL.  src: the
- * edges grouped by source, src_pos [E] each one's position in the destinations' order. */
+ * edges grouped by source, src_place [E] each edge's place in that order. */
 size_t batteries_neighbor_attention_backward_workspace_bytes(int64_t n_edges, int64_t dst_parts,
                                                              int64_t src_parts, int H, int Hkv,
                                                              int Dk, int Dv);
@@ -539,7 +539,7 @@ int batteries_neighbor_attention_backward(
     const void* q, const void* k, const void* v, const float* bias, const float* stats,
     const void* grad_out, const int64_t* row_ptr, const int32_t* edge_id,
     const batmobile_attention_side* dst, const batmobile_attention_side* src,
-    const int32_t* src_pos, void* grad_q, void* grad_k, void* grad_v, float* grad_bias, int H,
+    const int32_t* src_place, void* grad_q, void* grad_k, void* grad_v, float* grad_bias, int H,
     int Hkv, int Dk, int Dv, int64_t q_stride, int64_t k_stride, int64_t v_stride,
     int64_t go_stride, float scale, int dtype, void* workspace, size_t workspace_bytes,
     hipStream_t stream);
