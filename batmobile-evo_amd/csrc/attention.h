@@ -70,7 +70,6 @@ struct AttnSide {
     const int* items;         // [items][64]
     const uint32_t* masks;    // [16 chunks]
     const int* ids;           // [32 chunks] columns
-    const int* eid;           // edge -> its place in the arrays per edge (NULL: itself)
     int n_items, n_tiles, n_edges;
 };
 
@@ -90,10 +89,11 @@ __device__ __forceinline__ int tile_of_part(const AttnSide& s, int p, int& first
 // contiguous eighth of the items, so that tiles that share columns meet in one L2, and those
 // head by head: the columns of the tiles in flight are then one head's only, which fit the L2
 // (50,000 atoms, 8 heads of 256 in bf16: 1 KB a column against 8).
-__device__ __forceinline__ bool attn_unit(int n_items, int heads, int& item, int& head) {
-    const int x = blockIdx.x & 7;
+__device__ __forceinline__ bool attn_unit(unsigned block, int n_items, int heads, int& item,
+                                          int& head) {
+    const int x = block & 7;
     const int i0 = (int)((int64_t)n_items * x >> 3), i1 = (int)((int64_t)n_items * (x + 1) >> 3);
-    const uint32_t w = blockIdx.x >> 3;
+    const uint32_t w = block >> 3;
     if (w >= (uint64_t)(i1 - i0) * heads) return false;
     head = (int)(w / (uint32_t)(i1 - i0));
     item = i0 + (int)(w % (uint32_t)(i1 - i0));
@@ -520,7 +520,23 @@ __device__ __forceinline__ int nth_edge(uint32_t mask, int bit) {
     return __popc(mask & ((1u << bit) - 1u));
 }
 
-inline AttnSide side_args(const batmobile_attention_side& s, const int32_t* eid) {
+// The bias of an edge and head: value[edge_id e][h] as the caller has it, or value[h][e] in the
+// side's order (edges_by_head).
+struct EdgeBias {
+    const float* value;
+    const int* eid;
+    int64_t edge_step, head_step;
+    __device__ __forceinline__ float at(int e, int h) const {
+        return value[(int64_t)(eid ? eid[e] : e) * edge_step + h * head_step];
+    }
+};
+inline EdgeBias edge_bias(const float* value, const int32_t* eid, int64_t n_edges, int H,
+                          bool by_head) {
+    if (by_head) return {value, nullptr, 1, n_edges};
+    return {value, eid, H, 1};
+}
+
+inline AttnSide side_args(const batmobile_attention_side& s) {
     const PlanLayout p = plan_layout(s.n_rows, s.n_edges);
     AttnSide a;
     a.rows = s.plan + p.rows;
@@ -528,7 +544,6 @@ inline AttnSide side_args(const batmobile_attention_side& s, const int32_t* eid)
     a.items = s.plan + p.items;
     a.masks = reinterpret_cast<const uint32_t*>(s.plan + p.masks);
     a.ids = s.plan + p.ids;
-    a.eid = eid;
     a.n_items = s.n_items;
     a.n_tiles = (int)p.tiles;
     a.n_edges = (int)s.n_edges;

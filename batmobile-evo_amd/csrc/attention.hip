@@ -20,7 +20,7 @@ namespace bmhip {
 struct AttnFwd {
     AttnSide side;
     const void *q, *k, *v;
-    const float* bias;
+    EdgeBias bias;
     void* out;
     float *stats;                          // [n_dst, H, 2]
     float *part_o, *part_ml;               // [parts, H, 16, Dv], [parts, H, 16, 2]
@@ -41,8 +41,7 @@ __device__ __forceinline__ void attn_fwd_rows(const AttnFwd& a, int item, int h,
         const T* q = row_of<T>(a.q, row, a.qs) + (int64_t)h * a.Dk;
         float m = -kInf, l = 0.0f, o[4] = {0, 0, 0, 0};
         each_edge(a.side, item, r, [&](int e, int col) {
-            const float b =
-                a.bias ? a.bias[(int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h] : 0.0f;
+            const float b = a.bias.value ? a.bias.at(e, h) : 0.0f;
             const T* k = row_of<T>(a.k, col, a.ks) + (int64_t)kv * a.Dk;
             float s = 0.0f;
             for (int d = threadIdx.x; d < a.Dk; d += 64) s = fmaf(attn_f32(q[d]), attn_f32(k[d]), s);
@@ -85,7 +84,7 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 3 : (KP + VP) * sizeof(T) <= 1
     __shared__ __attribute__((aligned(1024))) char k_lds[Rows::kBytes];
     __shared__ float b_lds[BIAS ? kTileEdges : 1];
     int item, h;
-    if (!attn_unit(a.side.n_items, a.H, item, h)) return;
+    if (!attn_unit(blockIdx.x, a.side.n_items, a.H, item, h)) return;
     const int lane = threadIdx.x, n = lane & 15, g = lane >> 4, kv = h / a.group;
     const Item it(a.side, item, lane);
     const int row = it.row, steps = it.chunks * 2 / kT;
@@ -100,11 +99,12 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 3 : (KP + VP) * sizeof(T) <= 1
             return;
         }
         auto keep = [&](int i, int, float b, int) { b_lds[i] = b; };
-        if (a.side.eid)
-            it.each<float>(a.side, lane,
-                           [&](int e) { return a.bias[(int64_t)a.side.eid[e] * a.H + h]; }, keep);
+        if (a.bias.eid)
+            it.each<float>(a.side, lane, [&](int e) { return a.bias.at(e, h); }, keep);
         else
-            it.each<float>(a.side, lane, [&](int e) { return a.bias[(int64_t)e * a.H + h]; }, keep);
+            it.each<float>(a.side, lane, [&](int e) {
+                return a.bias.value[(int64_t)e * a.bias.edge_step + h * a.bias.head_step];
+            }, keep);
     }
 
     v4f acc[ColFrag<T, VP>::kAcc];
@@ -285,10 +285,10 @@ template <typename T, int KP, int VP>
 static void attn_fwd_launch(const AttnFwd& a, bool wide, hipStream_t s) {
     const unsigned grid = attn_grid(a.side.n_items, a.H);
     const bool full = a.Dk == KP;
-    if (wide && a.bias) attn_fwd_kernel<T, KP, VP, false, true, true><<<grid, 64, 0, s>>>(a);
+    if (wide && a.bias.value) attn_fwd_kernel<T, KP, VP, false, true, true><<<grid, 64, 0, s>>>(a);
     else if (wide) attn_fwd_kernel<T, KP, VP, false, false, true><<<grid, 64, 0, s>>>(a);
-    else if (a.bias && full) attn_fwd_kernel<T, KP, VP, true, true, false><<<grid, 64, 0, s>>>(a);
-    else if (a.bias) attn_fwd_kernel<T, KP, VP, false, true, false><<<grid, 64, 0, s>>>(a);
+    else if (a.bias.value && full) attn_fwd_kernel<T, KP, VP, true, true, false><<<grid, 64, 0, s>>>(a);
+    else if (a.bias.value) attn_fwd_kernel<T, KP, VP, false, true, false><<<grid, 64, 0, s>>>(a);
     else if (full) attn_fwd_kernel<T, KP, VP, true, false, false><<<grid, 64, 0, s>>>(a);
     else attn_fwd_kernel<T, KP, VP, false, false, false><<<grid, 64, 0, s>>>(a);
 }
@@ -311,6 +311,45 @@ static void attn_fwd_run(const AttnFwd& a, bool wide, int parts, hipStream_t s) 
 
 using namespace bmhip;
 
+// in [E, H] (row edge_id e) <-> out [H, E]: 64 edges and up to 32 heads a workgroup, through LDS,
+// so that both sides are contiguous.
+template <bool TO_HEADS>
+__global__ __launch_bounds__(256) void attn_edges_kernel(const float* __restrict__ in,
+                                                         const int* __restrict__ eid,
+                                                         float* __restrict__ out, int64_t edges,
+                                                         int H) {
+    __shared__ float t[64][33];
+    const int64_t e0 = (int64_t)blockIdx.x * 64;
+    const int h0 = blockIdx.y * 32, n = (int)min((int64_t)64, edges - e0), w = min(32, H - h0);
+    // the [E, H] side: w values of an edge next to each other
+    auto rows = [&](auto&& f) {
+        for (int i = threadIdx.x; i < n * w; i += 256) {
+            const int e = i / w, h = i - e * w;
+            f(e, h, (eid ? (int64_t)eid[e0 + e] : e0 + e) * H + h0 + h);
+        }
+    };
+    auto cols = [&](auto&& f) {
+        for (int i = threadIdx.x; i < 64 * w; i += 256)
+            if ((i & 63) < n) f(i & 63, i >> 6, (int64_t)(h0 + (i >> 6)) * edges + e0 + (i & 63));
+    };
+    if (TO_HEADS) rows([&](int e, int h, int64_t at) { t[e][h] = in[at]; });
+    else cols([&](int e, int h, int64_t at) { t[e][h] = in[at]; });
+    __syncthreads();
+    if (TO_HEADS) cols([&](int e, int h, int64_t at) { out[at] = t[e][h]; });
+    else rows([&](int e, int h, int64_t at) { out[at] = t[e][h]; });
+}
+
+extern "C" int batteries_attention_edges_by_head(const float* values, const int32_t* edge_id,
+                                                 float* out, int64_t n_edges, int H, int back,
+                                                 hipStream_t stream) {
+    if (n_edges < 0 || H <= 0 || H > 65535 * 32 || n_edges >= INT32_MAX / 4) return BM_ERR_ARG;
+    if (n_edges == 0) return BM_OK;
+    const dim3 grid((unsigned)ceil_div(n_edges, 64), (unsigned)ceil_div(H, 32));
+    if (back) attn_edges_kernel<false><<<grid, 256, 0, stream>>>(values, edge_id, out, n_edges, H);
+    else attn_edges_kernel<true><<<grid, 256, 0, stream>>>(values, edge_id, out, n_edges, H);
+    return (int)hipGetLastError();
+}
+
 extern "C" size_t batteries_neighbor_attention_workspace_bytes(int64_t n_parts, int H, int Dv) {
     if (n_parts <= 0 || H <= 0 || Dv <= 0) return 0;
     return (size_t)n_parts * H * kAttnRows * (Dv + 2) * sizeof(float);
@@ -318,6 +357,7 @@ extern "C" size_t batteries_neighbor_attention_workspace_bytes(int64_t n_parts, 
 
 extern "C" int batteries_neighbor_attention(const void* q, const void* k, const void* v,
                                             const float* bias, const int32_t* edge_id,
+                                            int bias_by_head,
                                             const batmobile_attention_side* side, void* out,
                                             float* stats, int H, int Hkv, int Dk, int Dv,
                                             int64_t q_stride, int64_t k_stride, int64_t v_stride,
@@ -332,8 +372,10 @@ extern "C" int batteries_neighbor_attention(const void* q, const void* k, const 
     const size_t need = batteries_neighbor_attention_workspace_bytes(side->n_parts, H, Dv);
     if (workspace_bytes < need || (need && !workspace)) return BM_ERR_WORKSPACE;
     AttnFwd a{};
-    a.side = side_args(*side, edge_id);
-    a.q = q; a.k = k; a.v = v; a.bias = bias; a.out = out; a.stats = stats;
+    a.side = side_args(*side);
+    a.q = q; a.k = k; a.v = v; a.out = out;
+    a.bias = edge_bias(bias, edge_id, side->n_edges, H, bias_by_head != 0);
+    a.stats = stats;
     a.part_o = (float*)workspace;
     a.part_ml = a.part_o + (size_t)side->n_parts * H * kAttnRows * Dv;
     const int64_t size = dtype == 0 ? 4 : 2;

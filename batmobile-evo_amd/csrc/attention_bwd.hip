@@ -22,9 +22,10 @@ namespace bmhip {
 struct AttnScores {
     AttnSide side;
     const void *q, *k, *v, *go;
-    const float *bias, *stats;
-    float* gbias;
-    const int* place;                      // edge -> its place in the sources' order
+    EdgeBias bias;
+    const float* stats;
+    float* gbias;                          // [E, H], or NULL
+    const int *eid, *place;                // edge -> its row of gbias, its place among the sources'
     float2* ws;                            // [H][E], sources' order: p, ds (of cut tiles first dp)
     float* wd;                             // [H][E], destinations' order: ds
     uint32_t qs, ks, vs, gs;               // rows' strides in bytes
@@ -50,8 +51,7 @@ __device__ __forceinline__ void attn_scores_rows(const AttnScores& a, int item, 
         const float ref = ml[0] == -kInf ? 0.0f : ml[0], inv = ml[1] == 0.0f ? 0.0f : 1.0f / ml[1];
         float d = 0.0f;
         each_edge(a.side, item, r, [&](int e, int col) {
-            const float b =
-                a.bias ? a.bias[(int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h] : 0.0f;
+            const float b = a.bias.value ? a.bias.at(e, h) : 0.0f;
             const T* k = row_of<T>(a.k, col, a.ks) + (int64_t)kv * a.Dk;
             const T* v = row_of<T>(a.v, col, a.vs) + (int64_t)kv * a.Dv;
             float s = 0.0f, y = 0.0f;
@@ -72,7 +72,7 @@ __device__ __forceinline__ void attn_scores_rows(const AttnScores& a, int item, 
             const float ds = w.x == 0.0f ? 0.0f : w.x * (w.y - d);
             ws[a.place[e]].y = ds;
             a.wd[(int64_t)h * a.edges + e] = ds;
-            if (a.gbias) a.gbias[(int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h] = ds;
+            if (a.gbias) a.gbias[(int64_t)(a.eid ? a.eid[e] : e) * a.H + h] = ds;
         });
     }
 }
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_scores_kernel
     __shared__ float p_lds[kTileEdges];              // the bias, then p
     __shared__ float dp_lds[kTileEdges];
     int item, h;
-    if (!attn_unit(a.side.n_items, a.H, item, h)) return;
+    if (!attn_unit(blockIdx.x, a.side.n_items, a.H, item, h)) return;
     const int lane = threadIdx.x, n = lane & 15, g = lane >> 4, kv = h / a.group;
     const Item it(a.side, item, lane);
     const int row = it.row, steps = it.chunks * 2 / kT;
@@ -115,14 +115,14 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_scores_kernel
     VRows::template fill<FULL, WIDE>(v_lds, ids, vbase, a.vs, a.Dv, lane);
     ids = step.ids(1);
     auto keep_bias = [&](int i, int, float b, int) { p_lds[i] = b; };
-    if (!a.bias)
+    if (!a.bias.value)
         it.each<float>(a.side, lane, [](int) { return 0.0f; }, keep_bias);
-    else if (a.side.eid)
-        it.each<float>(a.side, lane,
-                       [&](int e) { return a.bias[(int64_t)a.side.eid[e] * a.H + h]; }, keep_bias);
+    else if (a.bias.eid)
+        it.each<float>(a.side, lane, [&](int e) { return a.bias.at(e, h); }, keep_bias);
     else
-        it.each<float>(a.side, lane, [&](int e) { return a.bias[(int64_t)e * a.H + h]; },
-                       keep_bias);
+        it.each<float>(a.side, lane, [&](int e) {
+            return a.bias.value[(int64_t)e * a.bias.edge_step + h * a.bias.head_step];
+        }, keep_bias);
     float2* ws = a.ws + (int64_t)h * a.edges;
     float d = 0.0f, p[4 * kT], dp[4 * kT];
     int done = 0, before = 0;                  // row n's edges of earlier steps
@@ -203,14 +203,14 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_scores_kernel
         const float pe = p_lds[i], ds = pe == 0.0f ? 0.0f : pe * (dp_lds[i] - dr[k]);
         ws[to] = make_float2(pe, ds);
         wd[e] = ds;
-        if (a.gbias) a.gbias[(int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h] = ds;
+        if (a.gbias) a.gbias[(int64_t)(a.eid ? a.eid[e] : e) * a.H + h] = ds;
     });
 }
 
 struct AttnDs {
     AttnSide side;
     const int64_t* row_ptr;
-    const int* place;
+    const int *eid, *place;
     float2* ws;
     float *wd, *gbias;
     int64_t edges;
@@ -245,7 +245,7 @@ __global__ __launch_bounds__(1024) void attn_ds_kernel(AttnDs a) {
             const float ds = at->x == 0.0f ? 0.0f : at->x * (at->y - d);
             at->y = ds;
             a.wd[(int64_t)h * a.edges + e] = ds;
-            if (a.gbias) a.gbias[(int64_t)(a.side.eid ? a.side.eid[e] : e) * a.H + h] = ds;
+            if (a.gbias) a.gbias[(int64_t)(a.eid ? a.eid[e] : e) * a.H + h] = ds;
         }
     }
 }
@@ -292,12 +292,21 @@ __device__ __forceinline__ void attn_sum_rows(const AttnSum& a, int item, int he
     }
 }
 
+// Up to three sums in one launch, so that one's last workgroups run beside the next one's first.
+struct AttnSums {
+    AttnSum sum[3];
+    unsigned first[4];                     // first workgroup of each, and their end
+};
+
 template <typename T, int P>
-__global__ __launch_bounds__(64, P * sizeof(T) <= 256 || P == 64 ? 2 : 1) void attn_sum_kernel(AttnSum a) {
+__global__ __launch_bounds__(64, P * sizeof(T) <= 256 || P == 64 ? 2 : 1) void attn_sum_kernel(
+    AttnSums all) {
+    const int which = (blockIdx.x >= all.first[1]) + (blockIdx.x >= all.first[2]);
+    const AttnSum& a = all.sum[which];
     constexpr int kT = Attn<T>::kTiles, kR = Attn<T>::kRowsPerLane;
     __shared__ float w_lds[kTileEdges];
     int item, head;
-    if (!attn_unit(a.side.n_items, a.heads, item, head)) return;
+    if (!attn_unit(blockIdx.x - all.first[which], a.side.n_items, a.heads, item, head)) return;
     const int lane = threadIdx.x, n = lane & 15, g = lane >> 4;
     const Item it(a.side, item, lane);
     const int row = it.row, steps = it.chunks * 2 / kT;
@@ -423,15 +432,28 @@ static void attn_scores_run(const AttnScores& a, bool wide, hipStream_t s) {
     else if (a.Dk <= 128) attn_scores_run_k<T, 128>(a, wide, s);
     else attn_scores_run_k<T, 256>(a, wide, s);
 }
+static int attn_sum_class(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+
+// The n sums of one size class, the later of their parts' joins.
 template <typename T>
-static void attn_sum_run(const AttnSum& a, int parts, hipStream_t s) {
-    const unsigned grid = attn_grid(a.side.n_items, a.heads);
+static void attn_sum_run(const AttnSum* sums, const int* parts, int n, hipStream_t s) {
+    AttnSums all{};
+    all.first[0] = 0;
+    for (int i = 0; i < 3; ++i) {
+        all.sum[i] = sums[std::min(i, n - 1)];
+        all.first[i + 1] =
+            all.first[i] + (i < n ? attn_grid(sums[i].side.n_items, sums[i].heads) : 0);
+    }
+    const unsigned grid = all.first[3];
     if (grid == 0) return;
-    if (a.D <= 64) attn_sum_kernel<T, 64><<<grid, 64, 0, s>>>(a);
-    else if (a.D <= 128) attn_sum_kernel<T, 128><<<grid, 64, 0, s>>>(a);
-    else attn_sum_kernel<T, 256><<<grid, 64, 0, s>>>(a);
-    if (parts)
-        attn_sum_join_kernel<T><<<dim3((unsigned)parts, (unsigned)a.heads), 1024, 0, s>>>(a);
+    const int P = attn_sum_class(sums[0].D);
+    if (P == 64) attn_sum_kernel<T, 64><<<grid, 64, 0, s>>>(all);
+    else if (P == 128) attn_sum_kernel<T, 128><<<grid, 64, 0, s>>>(all);
+    else attn_sum_kernel<T, 256><<<grid, 64, 0, s>>>(all);
+    for (int i = 0; i < n; ++i)
+        if (parts[i])
+            attn_sum_join_kernel<T><<<dim3((unsigned)parts[i], (unsigned)sums[i].heads), 1024, 0,
+                                      s>>>(sums[i]);
 }
 
 }  // namespace bmhip
@@ -439,8 +461,7 @@ static void attn_sum_run(const AttnSum& a, int parts, hipStream_t s) {
 using namespace bmhip;
 
 static size_t bwd_part_floats(int64_t dst_parts, int64_t src_parts, int H, int Hkv, int Dk, int Dv) {
-    return (size_t)kAttnRows *
-           std::max((size_t)dst_parts * H * Dk, (size_t)src_parts * Hkv * std::max(Dk, Dv));
+    return (size_t)kAttnRows * ((size_t)dst_parts * H * Dk + (size_t)src_parts * Hkv * (Dk + Dv));
 }
 
 extern "C" size_t batteries_neighbor_attention_backward_workspace_bytes(
@@ -453,7 +474,7 @@ extern "C" size_t batteries_neighbor_attention_backward_workspace_bytes(
 extern "C" int batteries_neighbor_attention_backward(
     const void* q, const void* k, const void* v, const float* bias, const float* stats,
     const void* grad_out, const int64_t* row_ptr, const int32_t* edge_id,
-    const batmobile_attention_side* dst, const batmobile_attention_side* src,
+    int bias_by_head, const batmobile_attention_side* dst, const batmobile_attention_side* src,
     const int32_t* src_place, void* grad_q, void* grad_k, void* grad_v, float* grad_bias, int H,
     int Hkv, int Dk, int Dv, int64_t q_stride, int64_t k_stride, int64_t v_stride,
     int64_t go_stride, float scale, int dtype, void* workspace, size_t workspace_bytes,
@@ -471,15 +492,19 @@ extern "C" int batteries_neighbor_attention_backward(
     const size_t need = batteries_neighbor_attention_backward_workspace_bytes(
         E, dst->n_parts, src->n_parts, H, Hkv, Dk, Dv);
     if (workspace_bytes < need || (need && !workspace)) return BM_ERR_WORKSPACE;
+    const bool by_head = bias_by_head != 0;
     float2* ws = (float2*)workspace;
     float* wd = (float*)(ws + ((size_t)E * H + 3) / 4 * 4);
     float* part = wd + ((size_t)E * H + 3) / 4 * 4;
     if (E > 0) {
         AttnScores a{};
-        a.side = side_args(*dst, edge_id);
-        a.q = q; a.k = k; a.v = v; a.go = grad_out; a.bias = bias; a.stats = stats; a.ws = ws;
+        a.side = side_args(*dst);
+        a.q = q; a.k = k; a.v = v; a.go = grad_out; a.stats = stats;
+        a.bias = edge_bias(bias, edge_id, E, H, by_head);
+        a.ws = ws;
         a.wd = wd; a.place = src_place;
-        a.gbias = grad_bias;
+        a.gbias = by_head ? nullptr : grad_bias;
+        a.eid = edge_id;
         a.qs = (uint32_t)(q_stride * size); a.ks = (uint32_t)(k_stride * size);
         a.vs = (uint32_t)(v_stride * size); a.gs = (uint32_t)(go_stride * size); a.edges = E;
         a.H = H; a.group = H / Hkv; a.Dk = Dk; a.Dv = Dv; a.scale = scale;
@@ -487,23 +512,39 @@ extern "C" int batteries_neighbor_attention_backward(
         if (dtype == 0) attn_scores_run<float>(a, wide, stream);
         else attn_scores_run<uint16_t>(a, wide, stream);
         if (dst->n_parts > 0) {
-            AttnDs d{side_args(*dst, edge_id), row_ptr, src_place, ws, wd, grad_bias, E, H};
+            AttnDs d{side_args(*dst), row_ptr, edge_id, src_place, ws, wd, a.gbias, E, H};
             attn_ds_kernel<<<dim3((unsigned)dst->n_parts, (unsigned)H), 1024, 0, stream>>>(d);
         }
     }
-    auto sum = [&](const batmobile_attention_side& side, const void* x,
-                   int64_t xs, void* out, int heads, int group, int x_div, int D,
-                   const float* w, int w_step, float f) {
+    if (grad_bias && by_head && E > 0) {
+        const int rc = batteries_attention_edges_by_head(wd, edge_id, grad_bias, E, H, 1, stream);
+        if (rc != BM_OK) return rc;
+    }
+    // the sums with the longest work per wave first; cut tiles' parts of each behind the last's
+    AttnSum sums[3];
+    int parts[3], n = 0;
+    auto sum = [&](const batmobile_attention_side& side, const void* x, int64_t xs, void* out,
+                   int heads, int group, int x_div, int D, const float* w, int w_step, float f) {
         if (side.n_rows == 0) return;
-        AttnSum a{};
-        a.side = side_args(side, nullptr);
-        a.x = x; a.xs = (uint32_t)(xs * size); a.out = out; a.part = part; a.edges = E; a.heads = heads;
-        a.group = group; a.x_div = x_div; a.D = D; a.w = w; a.w_step = w_step; a.f = f;
-        if (dtype == 0) attn_sum_run<float>(a, side.n_parts, stream);
-        else attn_sum_run<uint16_t>(a, side.n_parts, stream);
+        AttnSum& a = sums[n];
+        a.side = side_args(side);
+        a.x = x; a.xs = (uint32_t)(xs * size); a.out = out; a.part = part; a.edges = E;
+        a.heads = heads; a.group = group; a.x_div = x_div; a.D = D; a.w = w; a.w_step = w_step;
+        a.f = f;
+        part += (size_t)side.n_parts * heads * kAttnRows * D;
+        parts[n++] = side.n_parts;
     };
-    sum(*dst, k, k_stride, grad_q, H, 1, H / Hkv, Dk, wd, 1, scale);
+    auto run = [&]() {
+        if (n == 0) return;
+        if (dtype == 0) attn_sum_run<float>(sums, parts, n, stream);
+        else attn_sum_run<uint16_t>(sums, parts, n, stream);
+        n = 0;
+    };
     sum(*src, q, q_stride, grad_k, Hkv, H / Hkv, 1, Dk, &ws->y, 2, scale);
+    if (attn_sum_class(Dk) != attn_sum_class(Dv)) run();
     sum(*src, grad_out, go_stride, grad_v, Hkv, H / Hkv, 1, Dv, &ws->x, 2, 1.0f);
+    if (attn_sum_class(Dk) != attn_sum_class(Dv)) run();
+    sum(*dst, k, k_stride, grad_q, H, 1, H / Hkv, Dk, wd, 1, scale);
+    run();
     return (int)hipGetLastError();
 }

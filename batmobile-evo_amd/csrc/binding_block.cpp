@@ -160,18 +160,33 @@ AttnShape attn_shape(const Tensor& q, const Tensor& k, const Tensor& v, const Op
     return s;
 }
 
-std::tuple<Tensor, Tensor> neighbor_attention(const Tensor& q_, const Tensor& k_, const Tensor& v_,
-                                              const OptTensor& bias_, const Tensor& plan,
-                                              int64_t items, int64_t parts, int64_t E,
-                                              const OptTensor& edge_id, double scale,
-                                              bool keep_stats) {
+// Edges x heads from which the bias (and its gradient) is brought to [H, E] by a kernel of its
+// own: a wave takes one head of a tile, whose values lie H apart in [E, H], so every head reads
+// (writes) all cache lines of the array.  The extra launch pays from about here on.
+constexpr int64_t kByHead = 1 << 18;
+
+// (out, stats, bias by head): the last two for the backward, if kept
+std::tuple<Tensor, Tensor, Tensor> neighbor_attention(const Tensor& q_, const Tensor& k_,
+                                                      const Tensor& v_, const OptTensor& bias_,
+                                                      const Tensor& plan, int64_t items,
+                                                      int64_t parts, int64_t E,
+                                                      const OptTensor& edge_id, double scale,
+                                                      bool keep_stats) {
     const AttnShape s = attn_shape(q_, k_, v_, bias_, E);
     const c10::DeviceGuard guard(q_.device());
     const batmobile_attention_side side = attn_side(plan, items, parts, s.n_dst, s.n_src, E, q_);
     const int32_t* eid = opt_index32(edge_id, q_, E, "edge_id");
     const Tensor q = heads16(q_), k = heads16(k_), v = heads16(v_);
-    Tensor bias;
+    Tensor bias, by_head;
     if (bias_) bias = bias_->contiguous();
+    if (bias.defined() && s.H > 1 && E * s.H >= kByHead) {
+        by_head = torch::empty({s.H, E}, bias.options());
+        check_status(batteries_attention_edges_by_head(bias.data_ptr<float>(), eid,
+                                                       by_head.data_ptr<float>(), E, s.H, 0,
+                                                       stream_of(q)),
+                     "neighbor_attention");
+        bias = by_head;
+    }
     const Tensor out = heads_like(q, s.n_dst, s.H, s.Dv);
     Tensor stats;
     if (keep_stats) stats = torch::empty({s.n_dst, s.H, 2}, q.options().dtype(torch::kFloat32));
@@ -181,18 +196,19 @@ std::tuple<Tensor, Tensor> neighbor_attention(const Tensor& q_, const Tensor& k_
     if (wsb) ws = bytes_on(q, wsb);
     check_status(batteries_neighbor_attention(
                      q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                     bias.defined() ? bias.data_ptr<float>() : nullptr, eid, &side,
-                     out.data_ptr(), keep_stats ? stats.data_ptr<float>() : nullptr, s.H, s.Hkv,
-                     Dk, Dv, row_stride(q), row_stride(k), row_stride(v), (float)scale, s.dtype,
-                     wsb ? ws.data_ptr() : nullptr, wsb, stream_of(q)),
+                     bias.defined() ? bias.data_ptr<float>() : nullptr, eid, by_head.defined(),
+                     &side, out.data_ptr(), keep_stats ? stats.data_ptr<float>() : nullptr, s.H,
+                     s.Hkv, Dk, Dv, row_stride(q), row_stride(k), row_stride(v), (float)scale,
+                     s.dtype, wsb ? ws.data_ptr() : nullptr, wsb, stream_of(q)),
                  "neighbor_attention");
-    return {cut_heads(out, s.Dv), stats};
+    return {cut_heads(out, s.Dv), stats, keep_stats ? by_head : Tensor()};
 }
 
-// src_*: the side of the sources, src_place the place of every edge in its order
+// by_head: the forward's, in place of the bias.  src_*: the side of the sources, src_place the
+// place of every edge in its order.
 std::tuple<Tensor, Tensor, Tensor, Tensor> neighbor_attention_backward(
     const Tensor& q_, const Tensor& k_, const Tensor& v_, const OptTensor& bias_,
-    const Tensor& stats, const Tensor& grad_, const Tensor& row_ptr, const Tensor& plan,
+    const OptTensor& by_head, const Tensor& stats, const Tensor& grad_, const Tensor& row_ptr, const Tensor& plan,
     int64_t items, int64_t parts, const OptTensor& edge_id, const Tensor& src_plan,
     int64_t src_items, int64_t src_parts, const Tensor& src_place, double scale, bool need_bias) {
     const int64_t E = src_place.numel();
@@ -214,7 +230,15 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> neighbor_attention_backward(
     const Tensor q = heads16(q_), k = heads16(k_), v = heads16(v_), go = heads16(grad_);
     Tensor bias, gbias;
     if (bias_) bias = bias_->contiguous();
-    if (need_bias && bias_) gbias = torch::empty_like(bias);
+    if (by_head) {
+        check_f32(*by_head, q_, "bias by head");
+        TORCH_CHECK(by_head->is_contiguous() && by_head->dim() == 2 && by_head->size(0) == s.H &&
+                        by_head->size(1) == E,
+                    "bias by head must be [H, E]");
+        bias = *by_head;
+    }
+    if (need_bias && bias.defined())
+        gbias = torch::empty({E, s.H}, q.options().dtype(torch::kFloat32));
     const Tensor gq = heads_like(q, s.n_dst, s.H, s.Dk);
     const Tensor gk = heads_like(q, s.n_src, s.Hkv, s.Dk);
     const Tensor gv = heads_like(q, s.n_src, s.Hkv, s.Dv);
@@ -226,7 +250,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> neighbor_attention_backward(
         batteries_neighbor_attention_backward(
             q.data_ptr(), k.data_ptr(), v.data_ptr(),
             bias.defined() ? bias.data_ptr<float>() : nullptr, stats.data_ptr<float>(),
-            go.data_ptr(), rp, eid, &dst, &src, pos, gq.data_ptr(), gk.data_ptr(), gv.data_ptr(),
+            go.data_ptr(), rp, eid, by_head.has_value(), &dst, &src, pos, gq.data_ptr(), gk.data_ptr(), gv.data_ptr(),
             gbias.defined() ? gbias.data_ptr<float>() : nullptr, s.H, s.Hkv, Dk, Dv,
             row_stride(q), row_stride(k), row_stride(v), row_stride(go), (float)scale, s.dtype,
             ws.data_ptr(), wsb, stream_of(q)),
@@ -432,9 +456,9 @@ void register_block_ops(pybind11::module_& m) {
           py::arg("bias"), py::arg("plan"), py::arg("items"), py::arg("parts"),
           py::arg("num_edges"), py::arg("edge_id"), py::arg("scale"),
           py::arg("keep_stats") = false,
-          "softmax attention over the edges of each row -> (out, stats or None)");
+          "softmax attention over the edges of each row -> (out, stats or None, bias [H, E] or None)");
     m.def("neighbor_attention_backward", &neighbor_attention_backward, py::arg("q"), py::arg("k"),
-          py::arg("v"), py::arg("bias"), py::arg("stats"), py::arg("grad_out"),
+          py::arg("v"), py::arg("bias"), py::arg("by_head"), py::arg("stats"), py::arg("grad_out"),
           py::arg("row_ptr"), py::arg("plan"), py::arg("items"), py::arg("parts"),
           py::arg("edge_id"), py::arg("src_plan"), py::arg("src_items"), py::arg("src_parts"),
           py::arg("src_place"), py::arg("scale"), py::arg("need_bias") = true,

@@ -97,18 +97,19 @@ class NeighborAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, plan, scale):
         train = any(ctx.needs_input_grad[:4])
-        out, stats = _batmobile.neighbor_attention(q, k, v, bias, *plan.side, plan.src.numel(),
-                                                   plan.edge_id, scale, train)
-        ctx.save_for_backward(q, k, v, bias, stats)
+        out, stats, by_head = _batmobile.neighbor_attention(
+            q, k, v, bias, *plan.side, plan.src.numel(), plan.edge_id, scale, train)
+        # a bias brought to [H, E] takes the place of the caller's
+        ctx.save_for_backward(q, k, v, None if by_head is not None else bias, by_head, stats)
         ctx.plan, ctx.scale = plan, scale
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
-        q, k, v, bias, stats = ctx.saved_tensors
+        q, k, v, bias, by_head, stats = ctx.saved_tensors
         plan = ctx.plan
         gq, gk, gv, gb = _batmobile.neighbor_attention_backward(
-            q, k, v, bias, stats, grad_out, plan.row_ptr, *plan.side, plan.edge_id,
+            q, k, v, bias, by_head, stats, grad_out, plan.row_ptr, *plan.side, plan.edge_id,
             *plan.source_side(), ctx.scale, ctx.needs_input_grad[3])
         return gq, gk, gv, gb, None, None
 

@@ -513,24 +513,32 @@ int batteries_attention_plan(const int64_t* row_ptr, const int64_t* col, const i
                              int64_t n_rows, int64_t n_cols, int64_t n_edges, int check,
                              void* plan, size_t plan_bytes, hipStream_t stream);
 
+/* out [H, E] of values [E, H] (row edge_id e of edge e; edge_id NULL: e), or with `back`
+ * out [E, H] of values [H, E]. */
+int batteries_attention_edges_by_head(const float* values, const int32_t* edge_id, float* out,
+                                      int64_t n_edges, int H, int back, hipStream_t stream);
+
 /* With rows i (destinations) and sources j = col e:
  *   x_eh = scale <q[i,h], k[j, h / (H / Hkv)]> + bias[edge_id e, h],   p = softmax over the row
  *   out[i,h] = sum_e p_eh v[j, h / (H / Hkv)]
  * q [n_dst, H, Dk], k [n_src, Hkv, Dk], v [n_src, Hkv, Dv], out [n_dst, H, Dv] in fp32
  * (dtype 0) or bf16 (dtype 1), rows at strides (in elements), bias [E, H] fp32 or NULL,
- * edge_id [E] or NULL (the edges' own order).  Dk, Dv <= 256; pointers 16-byte aligned, Dk, Dv
+ * edge_id [E] or NULL (the edges' own order), or with bias_by_head [H, E] in the edges' order
+ * (then read contiguously; batteries_attention_edges_by_head makes it).  Dk, Dv <= 256; pointers 16-byte aligned, Dk, Dv
  * and strides multiples of 16 bytes.  An edge whose bias or logit is -inf is left out; a row
  * without an edge gives 0.  stats [n_dst, H, 2] (NULL: not kept): the maximum of x and the sum
  * of exp(x - max), which the backward recomputes the probabilities from. */
 size_t batteries_neighbor_attention_workspace_bytes(int64_t n_parts, int H, int Dv);
 int batteries_neighbor_attention(const void* q, const void* k, const void* v, const float* bias,
-                                 const int32_t* edge_id, const batmobile_attention_side* dst,
-                                 void* out, float* stats, int H, int Hkv, int Dk, int Dv,
+                                 const int32_t* edge_id, int bias_by_head,
+                                 const batmobile_attention_side* dst, void* out, float* stats,
+                                 int H, int Hkv, int Dk, int Dv,
                                  int64_t q_stride, int64_t k_stride, int64_t v_stride, float scale,
                                  int dtype, void* workspace, size_t workspace_bytes,
                                  hipStream_t stream);
 
-/* Gradients of the above: grad_q, grad_k, grad_v contiguous, grad_bias [E, H] or NULL.  src: the
+/* Gradients of the above: grad_q, grad_k, grad_v contiguous, grad_bias [E, H] or NULL (with
+ * bias_by_head it goes through [H, E] in the workspace: contiguous stores).  src: the
  * edges grouped by source, src_place [E] each edge's place in that order. */
 size_t batteries_neighbor_attention_backward_workspace_bytes(int64_t n_edges, int64_t dst_parts,
                                                              int64_t src_parts, int H, int Hkv,
@@ -538,7 +546,7 @@ size_t batteries_neighbor_attention_backward_workspace_bytes(int64_t n_edges, in
 int batteries_neighbor_attention_backward(
     const void* q, const void* k, const void* v, const float* bias, const float* stats,
     const void* grad_out, const int64_t* row_ptr, const int32_t* edge_id,
-    const batmobile_attention_side* dst, const batmobile_attention_side* src,
+    int bias_by_head, const batmobile_attention_side* dst, const batmobile_attention_side* src,
     const int32_t* src_place, void* grad_q, void* grad_k, void* grad_v, float* grad_bias, int H,
     int Hkv, int Dk, int Dv, int64_t q_stride, int64_t k_stride, int64_t v_stride,
     int64_t go_stride, float scale, int dtype, void* workspace, size_t workspace_bytes,
