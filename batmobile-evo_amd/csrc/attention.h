@@ -216,10 +216,11 @@ struct RowTile {
         for (int k = 0; k < kLoads; ++k) id[k] = __shfl(ids, k + kLoads * (lane / kPieces));
         const __amdgpu_buffer_rsrc_t rsrc =
             buffer_rsrc(reinterpret_cast<const float*>(base), 0xffffffffu);
+        int place = ((lane % kPieces) ^ (kLoads * (lane / kPieces) & kFlip)) * 16;
+        asm volatile("" : "+v"(place));        // kLoads offsets kept over the steps would not fit
 #pragma unroll
         for (int k = 0; k < kLoads; ++k) {
-            const int piece = (lane % kPieces) ^ ((k + kLoads * (lane / kPieces)) & kFlip);
-            int off = piece * 16;
+            int off = place ^ ((k & kFlip) * 16);
             if (!FULL) off = off < D * (int)sizeof(T) ? off : 0;
             __attribute__((address_space(3))) void* to =
                 (__attribute__((address_space(3))) void*)(lds + k * 1024);
@@ -242,8 +243,9 @@ struct RowTile {
         const char* at = lds + row % kLoads * 1024 + row / kLoads * kPieces * 16;
 #pragma unroll
         for (int s = 0; s < RowFrag<T, P>::kN; ++s) {
+            // the piece's bits above kFlip apart: a constant offset
             f.v[s] = *reinterpret_cast<const typename Attn<T>::Vec*>(
-                at + ((4 * s + g) ^ (row & kFlip)) * 16);
+                at + (((4 * s & kFlip) + g) ^ (row & kFlip)) * 16 + (4 * s & ~kFlip) * 16);
             if (!FULL && s * Attn<T>::kSteps + g * Attn<T>::kAlign >= D)
                 f.v[s] = typename Attn<T>::Vec{};
         }

@@ -80,7 +80,7 @@ __device__ __forceinline__ void attn_scores_rows(const AttnScores& a, int item, 
 // k and v of a step go to LDS while the products of the step before run; p and dp of the step
 // before are written to LDS first, as are all reads done (attn_fwd_kernel).
 template <typename T, int KP, int VP, bool FULL, bool WIDE>
-__global__ __launch_bounds__(64, KP + VP <= 256 ? 2 : 1) void attn_scores_kernel(AttnScores a) {
+__global__ __launch_bounds__(64, KP + VP < 512 ? 2 : 1) void attn_scores_kernel(AttnScores a) {
     constexpr int kT = Attn<T>::kTiles;
     constexpr float kInf = __builtin_inff();
     using KRows = RowTile<T, KP>;

@@ -399,8 +399,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> gated_residual_norm_b
 // ---------------------------------------------------------------------------
 
 // (norm, clipped): the norm as a tensor without dimensions; the clipped gradients in outs
-// (which may be the gradients) or in new tensors.  A strided view with gaps, or an out of
-// another layout than its gradient, goes through a dense copy.
+// (which may be the gradients; then nothing is returned for them) or in new tensors.  A strided
+// view with gaps, or an out of another layout than its gradient, goes through a dense copy.
 std::tuple<Tensor, std::vector<Tensor>> clip_grad_norm(
     const std::vector<Tensor>& grads, double max_norm,
     const c10::optional<std::vector<Tensor>>& outs) {
@@ -431,7 +431,9 @@ std::tuple<Tensor, std::vector<Tensor>> clip_grad_norm(
         in[i] = g.data_ptr(), out[i] = into[i].data_ptr(), numel[i] = g.numel();
     }
     Tensor norm = torch::empty({}, grads[0].options().dtype(torch::kFloat32));
-    const size_t wsb = batteries_clip_grad_norm_workspace_bytes((int64_t)n);
+    int64_t elements = 0;
+    for (const int64_t k : numel) elements += k;
+    const size_t wsb = batteries_clip_grad_norm_workspace_bytes((int64_t)n, elements);
     const Tensor ws = bytes_on(grads[0], wsb);
     check_status(batteries_clip_grad_norm(in.data(), out.data(), numel.data(), dt.data(),
                                           (int64_t)n, (float)max_norm, norm.data_ptr<float>(),
@@ -442,7 +444,7 @@ std::tuple<Tensor, std::vector<Tensor>> clip_grad_norm(
         Tensor o = (*outs)[i];
         if (!o.is_same(into[i])) o.copy_(into[i]);
     }
-    return {norm, *outs};
+    return {norm, {}};
 }
 
 }  // namespace

@@ -52,10 +52,14 @@ __device__ __forceinline__ void norm_st(uint16_t* p, float v) {
     *p = (uint16_t)(bf16_pack(v, 0.0f) & 0xffffu);
 }
 
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(
+        __builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
 template <int S0, int S1, int S2, int S3>
 __device__ __forceinline__ float quad(float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(
-        0, __float_as_int(v), S0 | (S1 << 2) | (S2 << 4) | (S3 << 6), 0xf, 0xf, true));
+    return dpp<S0 | (S1 << 2) | (S2 << 4) | (S3 << 6)>(v);
 }
 
 // Partial sums a (first component) and b (the other three) of the quad's lanes -> lane q: the
@@ -76,8 +80,13 @@ __device__ __forceinline__ float dot4(float4 a, float4 b, int q) {
 // takes part); the result in every lane of that q.  sh: two buffers used in turn.
 template <int W>
 __device__ __forceinline__ float row_sum(float v, float* sh, int& turn) {
-#pragma unroll
-    for (int o = 4; o < 64; o <<= 1) v += __shfl_xor(v, o);
+    v += dpp<0x124>(v);                        // row_ror:4 and :8 within 16 lanes
+    v += dpp<0x128>(v);
+    typedef unsigned v2u __attribute__((ext_vector_type(2)));
+    v2u r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     if constexpr (W > 1) {
         float* s = sh + turn * 4 * W;
         turn ^= 1;

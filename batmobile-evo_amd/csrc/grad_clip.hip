@@ -12,45 +12,47 @@
 
 namespace bmhip {
 
-constexpr int kClipTensors = 100;           // a launch's arguments stay under 4 KB
-constexpr int kClipChunk = 8192;            // elements of a tensor a workgroup takes at a time
+constexpr int kClipTensors = 160;           // a launch's arguments stay under 4 KB
 constexpr int kClipThreads = 256;
+constexpr int kClipLoads = 4;               // 16-byte loads a thread has under way
+constexpr int kClipBytes = kClipThreads * kClipLoads * 16;  // a workgroup's share at a time
 constexpr int kClipMaxBlocks = 1024;        // partial sums of a launch
 
 struct ClipArgs {
     const void* in[kClipTensors];
     void* out[kClipTensors];
-    int64_t numel[kClipTensors];
-    int first[kClipTensors + 1];            // first chunk of each tensor
+    uint32_t numel[kClipTensors];
+    int first[kClipTensors + 1];            // first share of each tensor
     uint8_t bf16[kClipTensors];
     int count;
 };
+static_assert(sizeof(ClipArgs) + 64 <= 4096, "kernel arguments");
 
-__device__ __forceinline__ float4 clip_ld4(const void* p, int64_t i, bool bf) {
-    if (!bf) return *reinterpret_cast<const float4*>((const float*)p + i);
-    const uint2 u = *reinterpret_cast<const uint2*>((const uint16_t*)p + i);
-    return make_float4(bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y));
-}
-__device__ __forceinline__ float clip_ld(const void* p, int64_t i, bool bf) {
+// 16 bytes at any address that an element may have (the hardware takes unaligned vectors)
+struct __attribute__((packed, aligned(2))) Clip16 {
+    uint32_t v[4];
+};
+
+__device__ __forceinline__ float clip_ld(const void* p, uint32_t i, bool bf) {
     return bf ? __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16) : ((const float*)p)[i];
 }
-__device__ __forceinline__ void clip_st(void* p, int64_t i, bool bf, float v) {
-    if (bf) ((uint16_t*)p)[i] = (uint16_t)(bf16_pack(v, 0.0f) & 0xffffu);
-    else ((float*)p)[i] = v;
-}
 
-// f(tensor, first element, element count) for every chunk of this workgroup
+// This workgroup's shares, the last first if `back`: f(tensor, first element, whole share?).
 template <typename F>
-__device__ __forceinline__ void clip_chunks(const ClipArgs& a, F&& f) {
-    const int total = a.first[a.count];
-    for (int c = blockIdx.x; c < total; c += gridDim.x) {
+__device__ __forceinline__ void clip_shares(const ClipArgs& a, bool back, F&& f) {
+    const int total = a.first[a.count], b = blockIdx.x, g = gridDim.x;
+    if (b >= total) return;
+    const int n = (total - b - 1) / g;
+    for (int i = 0; i <= n; ++i) {
+        const int c = b + (back ? n - i : i) * g;
         int lo = 0, hi = a.count - 1;
         while (lo < hi) {
             const int m = (lo + hi + 1) / 2;
             if (a.first[m] <= c) lo = m; else hi = m - 1;
         }
-        const int64_t i0 = (int64_t)(c - a.first[lo]) * kClipChunk;
-        f(lo, i0, (int)min((int64_t)kClipChunk, a.numel[lo] - i0));
+        const uint32_t per = a.bf16[lo] ? kClipBytes / 2 : kClipBytes / 4;
+        const uint32_t i0 = (uint32_t)(c - a.first[lo]) * per;
+        f(lo, i0, a.numel[lo] - i0 >= per);
     }
 }
 
@@ -68,18 +70,40 @@ __device__ __forceinline__ double block_sum(double v) {
 }
 
 __global__ __launch_bounds__(kClipThreads) void clip_norm_kernel(ClipArgs a, double* part) {
-    double s = 0.0;
-    clip_chunks(a, [&](int k, int64_t i0, int n) {
+    double s[2] = {0.0, 0.0};
+    clip_shares(a, false, [&](int k, uint32_t i0, bool whole) {
         const bool bf = a.bf16[k];
-        for (int i = threadIdx.x; i < n; i += kClipThreads) {
-            const double v = clip_ld(a.in[k], i0 + i, bf);
-            s = fma(v, v, s);
+        if (whole) {
+            const Clip16* p = reinterpret_cast<const Clip16*>(
+                (const char*)a.in[k] + (uint64_t)i0 * (bf ? 2 : 4)) + threadIdx.x;
+            Clip16 x[kClipLoads];
+#pragma unroll
+            for (int j = 0; j < kClipLoads; ++j) x[j] = p[j * kClipThreads];
+#pragma unroll
+            for (int j = 0; j < kClipLoads; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if (bf) {
+                        const double u = bf16_lo(x[j].v[c]), w = bf16_hi(x[j].v[c]);
+                        s[0] = fma(u, u, s[0]);
+                        s[1] = fma(w, w, s[1]);
+                    } else {
+                        const double u = __uint_as_float(x[j].v[c]);
+                        s[c & 1] = fma(u, u, s[c & 1]);
+                    }
+                }
+            return;
+        }
+        for (uint32_t i = i0 + threadIdx.x; i < a.numel[k]; i += kClipThreads) {
+            const double v = clip_ld(a.in[k], i, bf);
+            s[0] = fma(v, v, s[0]);
         }
     });
-    s = block_sum(s);
-    if (threadIdx.x == 0) part[blockIdx.x] = s;
+    const double total = block_sum(s[0] + s[1]);
+    if (threadIdx.x == 0) part[blockIdx.x] = total;
 }
 
+// The shares in the opposite order: the last ones read are still in the caches.
 __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(ClipArgs a, const double* part,
                                                                   int n_part, float max_norm,
                                                                   float* norm) {
@@ -89,11 +113,31 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(ClipArgs a, co
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
     // a norm that is not a number makes the factor, and every gradient, not a number
     const double r = (double)max_norm / (total + 1e-6);
-    const float c = r < 1.0 ? (float)r : (r != r ? (float)r : 1.0f);
-    clip_chunks(a, [&](int k, int64_t i0, int n) {
+    const float f = r < 1.0 ? (float)r : (r != r ? (float)r : 1.0f);
+    clip_shares(a, true, [&](int k, uint32_t i0, bool whole) {
         const bool bf = a.bf16[k];
-        for (int i = threadIdx.x; i < n; i += kClipThreads)
-            clip_st(a.out[k], i0 + i, bf, clip_ld(a.in[k], i0 + i, bf) * c);
+        if (whole) {
+            const uint64_t at = (uint64_t)i0 * (bf ? 2 : 4);
+            const Clip16* p = reinterpret_cast<const Clip16*>((const char*)a.in[k] + at) + threadIdx.x;
+            Clip16* q = reinterpret_cast<Clip16*>((char*)a.out[k] + at) + threadIdx.x;
+            Clip16 x[kClipLoads];
+#pragma unroll
+            for (int j = 0; j < kClipLoads; ++j) x[j] = p[j * kClipThreads];
+#pragma unroll
+            for (int j = 0; j < kClipLoads; ++j) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    x[j].v[c] = bf ? bf16_pack(bf16_lo(x[j].v[c]) * f, bf16_hi(x[j].v[c]) * f)
+                                   : __float_as_uint(__uint_as_float(x[j].v[c]) * f);
+                q[j * kClipThreads] = x[j];
+            }
+            return;
+        }
+        for (uint32_t i = i0 + threadIdx.x; i < a.numel[k]; i += kClipThreads) {
+            const float v = clip_ld(a.in[k], i, bf) * f;
+            if (bf) ((uint16_t*)a.out[k])[i] = (uint16_t)(bf16_pack(v, 0.0f) & 0xffffu);
+            else ((float*)a.out[k])[i] = v;
+        }
     });
 }
 
@@ -101,8 +145,12 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(ClipArgs a, co
 
 using namespace bmhip;
 
-extern "C" size_t batteries_clip_grad_norm_workspace_bytes(int64_t n_tensors) {
-    return (size_t)std::max<int64_t>(1, ceil_div(n_tensors, kClipTensors)) * kClipMaxBlocks *
+// Tensors of more than kClipMost elements travel as several entries.
+constexpr int64_t kClipMost = (int64_t)1 << 31;
+
+extern "C" size_t batteries_clip_grad_norm_workspace_bytes(int64_t n_tensors, int64_t n_elements) {
+    const int64_t entries = n_tensors + n_elements / kClipMost;
+    return (size_t)std::max<int64_t>(1, ceil_div(entries, kClipTensors)) * kClipMaxBlocks *
            sizeof(double);
 }
 
@@ -111,29 +159,36 @@ extern "C" int batteries_clip_grad_norm(const void* const* in, void* const* out,
                                         float max_norm, float* norm, void* workspace,
                                         size_t workspace_bytes, hipStream_t stream) {
     if (n_tensors < 0 || !norm || !(max_norm >= 0.0f)) return BM_ERR_ARG;
-    for (int64_t i = 0; i < n_tensors; ++i)
-        if (numel[i] < 0 || (dtype[i] != 0 && dtype[i] != 1) ||
-            (numel[i] > 0 && (!in[i] || !out[i])) ||
-            numel[i] > (int64_t)kClipChunk * (INT32_MAX / kClipTensors))
+    int64_t elements = 0;
+    for (int64_t i = 0; i < n_tensors; ++i) {
+        if (numel[i] < 0 || numel[i] > (int64_t)1 << 40 || (dtype[i] != 0 && dtype[i] != 1) ||
+            (numel[i] > 0 && (!in[i] || !out[i])))
             return BM_ERR_ARG;
-    if (!workspace || workspace_bytes < batteries_clip_grad_norm_workspace_bytes(n_tensors))
+        elements += numel[i];
+    }
+    if (!workspace || workspace_bytes < batteries_clip_grad_norm_workspace_bytes(n_tensors, elements))
         return BM_ERR_WORKSPACE;
     double* part = (double*)workspace;
     int n_part = 0;
     for (int pass = 0; pass < 2; ++pass) {
-        int64_t i = 0;
+        int64_t i = 0, done = 0;            // tensor, and elements of it in earlier entries
         do {
             ClipArgs a;
             a.count = 0;
             a.first[0] = 0;
-            for (; i < n_tensors && a.count < kClipTensors; ++i) {
-                if (numel[i] == 0) continue;
-                a.in[a.count] = in[i];
-                a.out[a.count] = out[i];
-                a.numel[a.count] = numel[i];
-                a.bf16[a.count] = dtype[i] == 1;
-                a.first[a.count + 1] = a.first[a.count] + (int)ceil_div(numel[i], kClipChunk);
-                ++a.count;
+            while (i < n_tensors && a.count < kClipTensors) {
+                const int64_t left = numel[i] - done, size = dtype[i] == 1 ? 2 : 4;
+                if (left > 0) {
+                    const int k = a.count++;
+                    a.in[k] = (const char*)in[i] + done * size;
+                    a.out[k] = (char*)out[i] + done * size;
+                    a.numel[k] = (uint32_t)std::min(left, kClipMost);
+                    a.bf16[k] = dtype[i] == 1;
+                    a.first[k + 1] =
+                        a.first[k] + (int)ceil_div((int64_t)a.numel[k] * size, kClipBytes);
+                }
+                if (left > kClipMost) done += kClipMost;
+                else ++i, done = 0;
             }
             const int blocks = std::max(1, std::min(kClipMaxBlocks, a.first[a.count]));
             if (pass == 0) {

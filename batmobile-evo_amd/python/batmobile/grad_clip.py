@@ -11,7 +11,8 @@ import _batmobile
 
 def clip_grad_norm(grads, max_norm, out=None):
     """(norm, clipped): the clipped gradients in `out` (a list like grads; None: new tensors)."""
-    return _batmobile.clip_grad_norm(grads, max_norm, out)
+    norm, clipped = _batmobile.clip_grad_norm(grads, max_norm, out)
+    return norm, clipped if out is None else out
 
 
 def clip_grad_norm_(parameters, max_norm):

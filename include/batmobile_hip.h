@@ -582,7 +582,7 @@ int batteries_gated_residual_norm_backward(
  * in, out (out[i] may be in[i]), numel and dtype (0 fp32, 1 bf16) are host arrays of
  * n_tensors; the tensors are dense and aligned to their element.
  * ------------------------------------------------------------------------- */
-size_t batteries_clip_grad_norm_workspace_bytes(int64_t n_tensors);
+size_t batteries_clip_grad_norm_workspace_bytes(int64_t n_tensors, int64_t n_elements);
 int batteries_clip_grad_norm(const void* const* in, void* const* out, const int64_t* numel,
                              const int* dtype, int64_t n_tensors, float max_norm, float* norm,
                              void* workspace, size_t workspace_bytes, hipStream_t stream);
