@@ -28,16 +28,32 @@ namespace bmhip {
 
 constexpr int kNormMaxC = 2048;
 
+// Four components as they lie in memory (bf16 takes half the registers until it is used)
 template <typename T>
-__device__ __forceinline__ float4 norm_ld4(const T* p);
+struct Raw4;
 template <>
-__device__ __forceinline__ float4 norm_ld4<float>(const float* p) {
-    return *reinterpret_cast<const float4*>(p);
-}
+struct Raw4<float> {
+    float4 v;
+    __device__ __forceinline__ void load(const float* p) { v = *reinterpret_cast<const float4*>(p); }
+    __device__ __forceinline__ void zero() { v = make_float4(0, 0, 0, 0); }
+    __device__ __forceinline__ float4 get() const { return v; }
+};
 template <>
-__device__ __forceinline__ float4 norm_ld4<uint16_t>(const uint16_t* p) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    return make_float4(bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y));
+struct Raw4<uint16_t> {
+    uint2 v;
+    __device__ __forceinline__ void load(const uint16_t* p) {
+        v = *reinterpret_cast<const uint2*>(p);
+    }
+    __device__ __forceinline__ void zero() { v = make_uint2(0, 0); }
+    __device__ __forceinline__ float4 get() const {
+        return make_float4(bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y));
+    }
+};
+template <typename T>
+__device__ __forceinline__ float4 norm_ld4(const T* p) {
+    Raw4<T> r;
+    r.load(p);
+    return r.get();
 }
 __device__ __forceinline__ void norm_st4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
 __device__ __forceinline__ void norm_st4(uint16_t* p, float4 v) {
@@ -77,7 +93,8 @@ __device__ __forceinline__ float dot4(float4 a, float4 b, int q) {
 }
 
 // Sum over the lanes of the same q, over the W waves of a row (every thread of the workgroup
-// takes part); the result in every lane of that q.  sh: two buffers used in turn.
+// takes part); the result in every lane of that q.  sh: two buffers of 4 floats a wave, used in
+// turn.
 template <int W>
 __device__ __forceinline__ float row_sum(float v, float* sh, int& turn) {
     v += dpp<0x124>(v);                        // row_ror:4 and :8 within 16 lanes
@@ -88,14 +105,14 @@ __device__ __forceinline__ float row_sum(float v, float* sh, int& turn) {
     r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     if constexpr (W > 1) {
-        float* s = sh + turn * 4 * W;
+        float* s = sh + turn * 4 * 16;
         turn ^= 1;
         const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
         if (lane < 4) s[w * 4 + lane] = v;
         __syncthreads();
         v = 0.0f;
 #pragma unroll
-        for (int i = 0; i < W; ++i) v += s[i * 4 + (lane & 3)];
+        for (int i = 0; i < W; ++i) v += s[(w / W * W + i) * 4 + (lane & 3)];
     }
     return v;
 }
@@ -113,43 +130,57 @@ struct NormArgs {
 // Rows per workgroup: 4 (W = 1) or 1.  BLOCK: h = x + f norm(y) first; else h = x.
 template <typename T, int NV, int W, bool BLOCK, bool GATE, bool PRE>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_fwd_kernel(NormArgs a) {
-    __shared__ float sh[2 * 4 * W];
+    __shared__ float sh[2 * 4 * 16];
     int turn = 0;
     const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
     if (row >= a.n) return;
     const int t = W == 1 ? (threadIdx.x & 63) : threadIdx.x, q = t & 3;
     const int64_t at = row * (int64_t)a.C * 16;
     const float cnt = 1.0f / ((float)a.C * (float)(2 * q + 1));
-    float4 h[NV], y[NV];
+    Raw4<T> x[NV], y[NV];
+    float4 h[NV];
     float f[NV];
+    // y, which the first sum waits for, before x
+    if constexpr (BLOCK) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            y[i].zero();
+            if (((i * 64 * W + t) >> 2) < a.C)
+                y[i].load((const T*)a.y + at + (int64_t)(i * 64 * W + t) * 4);
+        }
+    }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * 64 * W + t) >> 2;
-        const bool in = c < a.C;
-        const int64_t o = at + (int64_t)(i * 64 * W + t) * 4;
-        h[i] = in ? norm_ld4((const T*)a.x + o) : make_float4(0, 0, 0, 0);
-        if constexpr (BLOCK) {
-            y[i] = in ? norm_ld4((const T*)a.y + o) : make_float4(0, 0, 0, 0);
-            f[i] = in ? a.scale[c] * a.w_post[q * a.C + c] : 0.0f;
+        x[i].zero();
+        f[i] = 0.0f;
+        if (c < a.C) {
+            x[i].load((const T*)a.x + at + (int64_t)(i * 64 * W + t) * 4);
             if constexpr (GATE)
-                if (in) f[i] /= 1.0f + __expf(-norm_ld((const T*)a.gate + row * a.C * 4 +
-                                                        i * 64 * W + t));
+                f[i] = norm_ld((const T*)a.gate + row * a.C * 4 + i * 64 * W + t);
         }
     }
     if constexpr (BLOCK) {
         float s = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) s += dot4(y[i], y[i], q);
+        for (int i = 0; i < NV; ++i) s += dot4(y[i].get(), y[i].get(), q);
         const float r = 1.0f / sqrtf(fmaf(row_sum<W>(s, sh, turn), cnt, a.eps));
         if (a.rs && t < 4) a.rs[row * 8 + t] = r;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const float fa = first_of(f[i] * r), fb = others_of(f[i] * r);
-            h[i] = make_float4(fmaf(fa, y[i].x, h[i].x), fmaf(fb, y[i].y, h[i].y),
-                               fmaf(fb, y[i].z, h[i].z), fmaf(fb, y[i].w, h[i].w));
+            const int c = min((i * 64 * W + t) >> 2, a.C - 1);
+            float w = a.scale[c] * a.w_post[q * a.C + c] * r;
+            if constexpr (GATE) w /= 1.0f + __expf(-f[i]);
+            const float fa = first_of(w), fb = others_of(w);
+            const float4 yi = y[i].get(), xi = x[i].get();
+            h[i] = make_float4(fmaf(fa, yi.x, xi.x), fmaf(fb, yi.y, xi.y), fmaf(fb, yi.z, xi.z),
+                               fmaf(fb, yi.w, xi.w));
             if (((i * 64 * W + t) >> 2) < a.C)
                 norm_st4((T*)a.out_h + at + (int64_t)(i * 64 * W + t) * 4, h[i]);
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) h[i] = x[i].get();
     }
     if constexpr (PRE) {
         float s = 0.0f;
@@ -160,7 +191,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_fwd_kernel(NormArg
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * 64 * W + t) >> 2;
-            const float w = c < a.C ? a.w_pre[q * a.C + c] * r : 0.0f;
+            const float w = a.w_pre[q * a.C + min(c, a.C - 1)] * r;
             const float fa = first_of(w), fb = others_of(w);
             if (c < a.C)
                 norm_st4((T*)a.out_n + at + (int64_t)(i * 64 * W + t) * 4,
@@ -169,47 +200,64 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_fwd_kernel(NormArg
     }
 }
 
-// Every workgroup takes rows blockIdx.x, + gridDim.x, ... (4 at a time for W = 1) and keeps its
-// share of the weights' gradients in registers: part [gridDim.x, 9 C] (pre [4][C], post [4][C],
-// scale [C]), summed by norm_weights_kernel in workgroup order.
+// Every workgroup takes rows in turn (4 / W at a time, W waves each) and keeps its share of the
+// weights' gradients in registers: part [gridDim.x, 9 C] (pre [4][C], post [4][C], scale [C]),
+// summed by norm_weights_kernel.  A wave takes 64 channels of a row: with 128 the four arrays, the
+// weights and the sums would fill all registers of two waves.
 template <typename T, int NV, int W, bool BLOCK, bool GATE, bool PRE>
-__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_bwd_kernel(NormArgs a) {
-    __shared__ float sh[2 * 4 * W];
-    __shared__ float red[W == 1 ? 4 * 64 : 1];
+__global__ __launch_bounds__(W <= 4 ? 256 : 64 * W) void norm_bwd_kernel(NormArgs a) {
+    constexpr int kRows = W <= 4 ? 4 / W : 1;
+    __shared__ float sh[2 * 4 * 16];
+    __shared__ float red[kRows > 1 ? 256 : 1];
     int turn = 0;
-    const int wave = threadIdx.x >> 6;
-    const int t = W == 1 ? (threadIdx.x & 63) : threadIdx.x, q = t & 3;
+    const int group = threadIdx.x / (64 * W), t = threadIdx.x % (64 * W), q = t & 3;
     const float cnt = 1.0f / ((float)a.C * (float)(2 * q + 1));
     float aw_pre[NV], aw_post[NV], a_scale[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) aw_pre[i] = aw_post[i] = a_scale[i] = 0.0f;
-    for (int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x; row < a.n;
-         row += W == 1 ? gridDim.x * 4 : gridDim.x) {
+    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < a.n;
+         row0 += (int64_t)gridDim.x * kRows) {
+        const bool there = row0 + group < a.n;
+        const int64_t row = there ? row0 + group : a.n - 1;
         const int64_t at = row * (int64_t)a.C * 16;
-        float4 G[NV], h[NV], gn[NV];
-        float wp[NV];
+        float4 G[NV];
+        Raw4<T> gh[NV], h[NV], gn[NV], y[NV];
+        float sg[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * 64 * W + t) >> 2;
-            const bool in = c < a.C;
+            const bool in = there && ((i * 64 * W + t) >> 2) < a.C;
             const int64_t o = at + (int64_t)(i * 64 * W + t) * 4;
-            G[i] = h[i] = gn[i] = make_float4(0, 0, 0, 0);
-            wp[i] = 0.0f;
+            gh[i].zero();
+            h[i].zero();
+            gn[i].zero();
             if (in) {
-                if (a.gh) G[i] = norm_ld4((const T*)a.gh + o);
                 if constexpr (PRE) {
-                    h[i] = norm_ld4((const T*)a.h + o);
-                    gn[i] = norm_ld4((const T*)a.gn + o);
-                    wp[i] = a.w_pre[q * a.C + c];
+                    h[i].load((const T*)a.h + o);
+                    gn[i].load((const T*)a.gn + o);
+                }
+                if (a.gh) gh[i].load((const T*)a.gh + o);
+            }
+        }
+        if constexpr (BLOCK) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                y[i].zero();
+                sg[i] = 0.0f;
+                if (there && ((i * 64 * W + t) >> 2) < a.C) {
+                    y[i].load((const T*)a.y + at + (int64_t)(i * 64 * W + t) * 4);
+                    if constexpr (GATE)
+                        sg[i] = norm_ld((const T*)a.gate + row * a.C * 4 + i * 64 * W + t);
                 }
             }
         }
         if constexpr (PRE) {
             const float r = a.rs_in[row * 8 + 4 + q];
-            float s = 0.0f;
+            float s = 0.0f, wp[NV];
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const float v = dot4(gn[i], h[i], q);
+                const int c = (i * 64 * W + t) >> 2;
+                wp[i] = a.w_pre[q * a.C + min(c, a.C - 1)];
+                const float v = dot4(gn[i].get(), h[i].get(), q);   // 0 past C
                 aw_pre[i] = fmaf(r, v, aw_pre[i]);
                 s = fmaf(wp[i], v, s);
             }
@@ -218,55 +266,49 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_bwd_kernel(NormArg
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const float fa = first_of(wp[i] * r), fb = others_of(wp[i] * r);
-                G[i].x += fmaf(fa, gn[i].x, ka * h[i].x);
-                G[i].y += fmaf(fb, gn[i].y, kb * h[i].y);
-                G[i].z += fmaf(fb, gn[i].z, kb * h[i].z);
-                G[i].w += fmaf(fb, gn[i].w, kb * h[i].w);
+                const float4 gni = gn[i].get(), hi = h[i].get(), ghi = gh[i].get();
+                G[i] = make_float4(ghi.x + fmaf(fa, gni.x, ka * hi.x),
+                                   ghi.y + fmaf(fb, gni.y, kb * hi.y),
+                                   ghi.z + fmaf(fb, gni.z, kb * hi.z),
+                                   ghi.w + fmaf(fb, gni.w, kb * hi.w));
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) G[i] = gh[i].get();
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (((i * 64 * W + t) >> 2) < a.C)
+            if (there && ((i * 64 * W + t) >> 2) < a.C)
                 norm_st4((T*)a.gx + at + (int64_t)(i * 64 * W + t) * 4, G[i]);
         if constexpr (BLOCK) {
             const float r = a.rs_in[row * 8 + q];
             float s = 0.0f, f[NV];
-            float4 y[NV];
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = (i * 64 * W + t) >> 2;
-                f[i] = 0.0f;
-                y[i] = make_float4(0, 0, 0, 0);
-                float sg = 1.0f, sc = 0.0f, w = 0.0f;
-                if (c < a.C) {
-                    y[i] = norm_ld4((const T*)a.y + at + (int64_t)(i * 64 * W + t) * 4);
-                    if constexpr (GATE)
-                        sg = 1.0f / (1.0f + __expf(-norm_ld((const T*)a.gate + row * a.C * 4 +
-                                                            i * 64 * W + t)));
-                    sc = a.scale[c];
-                    w = a.w_post[q * a.C + c];
-                }
-                const float z = dot4(G[i], y[i], q), rz = r * z;
-                f[i] = sc * sg * w;
+                const float g = GATE ? 1.0f / (1.0f + __expf(-sg[i])) : 1.0f;
+                const float sc = a.scale[min(c, a.C - 1)], w = a.w_post[q * a.C + min(c, a.C - 1)];
+                const float z = dot4(G[i], y[i].get(), q), rz = r * z;   // 0 past C
+                f[i] = sc * g * w;
                 s = fmaf(f[i], z, s);
-                aw_post[i] = fmaf(sc * sg, rz, aw_post[i]);
-                a_scale[i] = fmaf(sg * w, rz, a_scale[i]);
+                aw_post[i] = fmaf(sc * g, rz, aw_post[i]);
+                a_scale[i] = fmaf(g * w, rz, a_scale[i]);
                 if constexpr (GATE)
-                    if (c < a.C)
+                    if (there && c < a.C)
                         norm_st((T*)a.ggate + row * a.C * 4 + i * 64 * W + t,
-                                f[i] * (1.0f - sg) * rz);
+                                f[i] * (1.0f - g) * rz);
             }
             const float k = -row_sum<W>(s, sh, turn) * cnt * r * r * r;
             const float ka = first_of(k), kb = others_of(k);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const float fa = first_of(f[i] * r), fb = others_of(f[i] * r);
-                if (((i * 64 * W + t) >> 2) < a.C)
+                const float4 yi = y[i].get();
+                if (there && ((i * 64 * W + t) >> 2) < a.C)
                     norm_st4((T*)a.gy + at + (int64_t)(i * 64 * W + t) * 4,
-                             make_float4(fmaf(fa, G[i].x, ka * y[i].x),
-                                         fmaf(fb, G[i].y, kb * y[i].y),
-                                         fmaf(fb, G[i].z, kb * y[i].z),
-                                         fmaf(fb, G[i].w, kb * y[i].w)));
+                             make_float4(fmaf(fa, G[i].x, ka * yi.x), fmaf(fb, G[i].y, kb * yi.y),
+                                         fmaf(fb, G[i].z, kb * yi.z),
+                                         fmaf(fb, G[i].w, kb * yi.w)));
             }
         }
     }
@@ -279,12 +321,14 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_bwd_kernel(NormArg
             if (k == 0 && !PRE) continue;
             if (k > 0 && !BLOCK) continue;
             if (k == 2) v = v + quad<1, 0, 3, 2>(v), v = v + quad<2, 3, 0, 1>(v);
-            if constexpr (W == 1) {
+            if constexpr (kRows > 1) {
                 __syncthreads();
-                red[wave * 64 + t] = v;
+                red[threadIdx.x] = v;
                 __syncthreads();
-                v = red[t] + red[64 + t] + red[128 + t] + red[192 + t];
-                if (wave != 0) continue;
+                v = 0.0f;
+#pragma unroll
+                for (int r = 0; r < kRows; ++r) v += red[r * 64 * W + t];
+                if (group != 0) continue;
             }
             const int c = (i * 64 * W + t) >> 2;
             if (c >= a.C) continue;
@@ -294,25 +338,29 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_bwd_kernel(NormArg
     }
 }
 
-// Column sums of part [rows, 9 C] over the workgroups' rows, in order: 16 columns a workgroup,
-// 16 threads a column, each over a contiguous run of the rows.
-__global__ __launch_bounds__(256) void norm_weights_kernel(const float* __restrict__ part,
-                                                           int rows, int C, float* gw_pre,
-                                                           float* gw_post, float* gscale) {
-    __shared__ float sh[16][17];
-    const int col = blockIdx.x * 16 + (threadIdx.x & 15), k = threadIdx.x >> 4;
-    const int per = (rows + 15) / 16;
-    float s = 0.0f;
+// Column sums of part [rows, 9 C] over the workgroups' rows: 16 columns a workgroup, 64 threads
+// a column, thread k rows k, k + 64, ...
+__global__ __launch_bounds__(1024) void norm_weights_kernel(const float* __restrict__ part,
+                                                            int rows, int C, float* gw_pre,
+                                                            float* gw_post, float* gscale) {
+    __shared__ float sh[64][17];
+    const int lane = threadIdx.x & 15, col = blockIdx.x * 16 + lane, k = threadIdx.x >> 4;
     const bool want = col < 9 * C && (col < 4 * C ? gw_pre != nullptr
                                                   : col < 8 * C ? gw_post != nullptr
                                                                 : gscale != nullptr);
-    if (want)
-        for (int r = k * per; r < min(rows, (k + 1) * per); ++r) s += part[(int64_t)r * 9 * C + col];
-    sh[k][threadIdx.x & 15] = s;
+    float s = 0.0f;
+    if (want) {
+#pragma unroll 8
+        for (int r = k; r < rows; r += 64) s += part[(int64_t)r * 9 * C + col];
+    }
+    sh[k][lane] = s;
     __syncthreads();
+    for (int o = 32; o > 0; o >>= 1) {
+        if (k < o) sh[k][lane] += sh[k + o][lane];
+        __syncthreads();
+    }
     if (k == 0 && want) {
-        s = 0.0f;
-        for (int i = 0; i < 16; ++i) s += sh[i][threadIdx.x];
+        s = sh[0][lane];
         if (col < 4 * C) gw_pre[col] = s;
         else if (col < 8 * C) gw_post[col - 4 * C] = s;
         else gscale[col - 8 * C] = s;
@@ -320,28 +368,39 @@ __global__ __launch_bounds__(256) void norm_weights_kernel(const float* __restri
 }
 
 static int norm_bwd_blocks(int64_t n, int C) {
-    return (int)std::min<int64_t>(C <= 128 ? ceil_div(n, 4) : n, C <= 512 ? 1024 : 512);
+    const int rows = C <= 64 ? 4 : C <= 128 ? 2 : 1;
+    return (int)std::min<int64_t>(ceil_div(n, rows), C <= 512 ? 1024 : 512);
 }
 
 template <typename T, int NV, int W, bool BLOCK, bool GATE, bool PRE>
-static void norm_launch(const NormArgs& a, bool bwd, hipStream_t s) {
-    const int threads = W == 1 ? 256 : 64 * W;
-    if (bwd)
-        norm_bwd_kernel<T, NV, W, BLOCK, GATE, PRE>
-            <<<norm_bwd_blocks(a.n, a.C), threads, 0, s>>>(a);
-    else
-        norm_fwd_kernel<T, NV, W, BLOCK, GATE, PRE>
-            <<<(unsigned)(W == 1 ? ceil_div(a.n, 4) : a.n), threads, 0, s>>>(a);
+static void norm_fwd_launch(const NormArgs& a, hipStream_t s) {
+    norm_fwd_kernel<T, NV, W, BLOCK, GATE, PRE>
+        <<<(unsigned)(W == 1 ? ceil_div(a.n, 4) : a.n), W == 1 ? 256 : 64 * W, 0, s>>>(a);
+}
+template <typename T, int NV, int W, bool BLOCK, bool GATE, bool PRE>
+static void norm_bwd_launch(const NormArgs& a, hipStream_t s) {
+    norm_bwd_kernel<T, NV, W, BLOCK, GATE, PRE>
+        <<<norm_bwd_blocks(a.n, a.C), W <= 4 ? 256 : 64 * W, 0, s>>>(a);
 }
 
 template <typename T, bool BLOCK, bool GATE, bool PRE>
 static void norm_pick(const NormArgs& a, bool bwd, hipStream_t s) {
-    if (a.C <= 16) norm_launch<T, 1, 1, BLOCK, GATE, PRE>(a, bwd, s);
-    else if (a.C <= 32) norm_launch<T, 2, 1, BLOCK, GATE, PRE>(a, bwd, s);
-    else if (a.C <= 64) norm_launch<T, 4, 1, BLOCK, GATE, PRE>(a, bwd, s);
-    else if (a.C <= 128) norm_launch<T, 8, 1, BLOCK, GATE, PRE>(a, bwd, s);
-    else if (a.C <= 512) norm_launch<T, 8, 4, BLOCK, GATE, PRE>(a, bwd, s);
-    else norm_launch<T, 8, 16, BLOCK, GATE, PRE>(a, bwd, s);
+    if (bwd) {
+        if (a.C <= 16) norm_bwd_launch<T, 1, 1, BLOCK, GATE, PRE>(a, s);
+        else if (a.C <= 32) norm_bwd_launch<T, 2, 1, BLOCK, GATE, PRE>(a, s);
+        else if (a.C <= 64) norm_bwd_launch<T, 4, 1, BLOCK, GATE, PRE>(a, s);
+        else if (a.C <= 128) norm_bwd_launch<T, 4, 2, BLOCK, GATE, PRE>(a, s);
+        else if (a.C <= 256) norm_bwd_launch<T, 4, 4, BLOCK, GATE, PRE>(a, s);
+        else if (a.C <= 512) norm_bwd_launch<T, 8, 4, BLOCK, GATE, PRE>(a, s);
+        else norm_bwd_launch<T, 8, 16, BLOCK, GATE, PRE>(a, s);
+        return;
+    }
+    if (a.C <= 16) norm_fwd_launch<T, 1, 1, BLOCK, GATE, PRE>(a, s);
+    else if (a.C <= 32) norm_fwd_launch<T, 2, 1, BLOCK, GATE, PRE>(a, s);
+    else if (a.C <= 64) norm_fwd_launch<T, 4, 1, BLOCK, GATE, PRE>(a, s);
+    else if (a.C <= 128) norm_fwd_launch<T, 8, 1, BLOCK, GATE, PRE>(a, s);
+    else if (a.C <= 512) norm_fwd_launch<T, 8, 4, BLOCK, GATE, PRE>(a, s);
+    else norm_fwd_launch<T, 8, 16, BLOCK, GATE, PRE>(a, s);
 }
 
 template <typename T>
@@ -404,7 +463,7 @@ extern "C" int batteries_gated_residual_norm_backward(
         if (dtype == 0) norm_run<float>(a, y != nullptr, w_pre != nullptr, true, stream);
         else norm_run<uint16_t>(a, y != nullptr, w_pre != nullptr, true, stream);
     }
-    norm_weights_kernel<<<(unsigned)ceil_div(9 * (int64_t)C, 16), 256, 0, stream>>>(
+    norm_weights_kernel<<<(unsigned)ceil_div(9 * (int64_t)C, 16), 1024, 0, stream>>>(
         a.part, N > 0 ? norm_bwd_blocks(N, C) : 0, C, w_pre ? gw_pre : nullptr,
         y ? gw_post : nullptr, y ? gscale : nullptr);
     return (int)hipGetLastError();
