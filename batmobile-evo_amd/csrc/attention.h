@@ -28,7 +28,7 @@ constexpr int kAttnCols = 32;     // columns of a chunk
 constexpr int kPlanHead = 16;     // items, parts, what is wrong
 constexpr int kPlanItems = 0, kPlanParts = 1, kPlanBad = 2;
 
-// An item, read by a wave with one load: tile, first chunk, chunks, part (-1: the tile's only
+// An item, read by a wave with one load: tile, first chunk, columns, part (-1: the tile's only
 // item); the tile's rows (-1 past the end); each row's first edge in the item; their number.
 constexpr int kItemInts = 64, kItemRows = 16, kItemBase = 32, kItemCount = 48;
 
@@ -189,9 +189,9 @@ struct RowFrag {
 // load k brings the 16-byte piece l % kPieces of row k + kLoads (l / kPieces) to place 64 k + l.
 // Which piece of its row it brings is that number with the row's low bits flipped, so that the
 // 16 rows of a fragment read lie in different banks.
-template <typename T, int P>
+template <typename T, int P, int TILES>
 struct RowTile {
-    static constexpr int kRows = 16 * Attn<T>::kTiles, kPieces = P * (int)sizeof(T) / 16;
+    static constexpr int kRows = 16 * TILES, kPieces = P * (int)sizeof(T) / 16;
     static constexpr int kPer = 64 / kPieces, kLoads = kRows / kPer;
     static constexpr int kFlip = (kPieces < 16 ? kPieces : 16) - 1;
     static constexpr int kBytes = kLoads * 1024;
@@ -349,7 +349,7 @@ template <typename F>
 __device__ __forceinline__ void each_edge(const AttnSide& s, int item, int r, F&& f) {
     const int* it = s.items + (int64_t)item * kItemInts;
     int e = it[kItemBase + r];
-    for (int c = it[1]; c < it[1] + it[2]; ++c)
+    for (int c = it[1]; c < it[1] + (it[2] + kAttnCols - 1) / kAttnCols; ++c)
         for (uint32_t m = s.masks[(int64_t)c * kAttnRows + r]; m; m &= m - 1)
             f(e++, s.ids[(int64_t)c * kAttnCols + __builtin_ctz(m)]);
 }
@@ -420,14 +420,14 @@ __device__ __forceinline__ void store_rows(O* row, const v4f* acc, float f, int 
 // contiguous along each row, instead of one gather per pair and step.
 // ---------------------------------------------------------------------------
 struct Item {
-    int tile, chunk, chunks, part;         // uniform
+    int tile, chunk, columns, part;        // uniform
     int row, base, count, off, total;      // of tile row n (lane % 16): its LDS place off; all
     int longest;                           // uniform
     __device__ __forceinline__ Item(const AttnSide& s, int item, int lane) {
         const int v = s.items[(int64_t)item * kItemInts + lane];
         tile = __builtin_amdgcn_readlane(v, 0);
         chunk = __builtin_amdgcn_readlane(v, 1);
-        chunks = __builtin_amdgcn_readlane(v, 2);
+        columns = __builtin_amdgcn_readlane(v, 2);
         part = __builtin_amdgcn_readlane(v, 3);
         const int n = lane & 15;
         row = __shfl(v, kItemRows + n);
@@ -446,6 +446,9 @@ struct Item {
         off = x - count;
         total = __builtin_amdgcn_readlane(x, 15);
         longest = __builtin_amdgcn_readlane(m, 15);
+    }
+    __device__ __forceinline__ int steps(int tiles) const {
+        return (columns + 16 * tiles - 1) / (16 * tiles);
     }
     // The item's edges, 16 lanes a row and kStage x 64 at a time: get(edge) for all of them (an
     // edge that exists, also in lanes without one), then put(LDS place, edge, value, k) of tile row
@@ -483,28 +486,28 @@ __device__ __forceinline__ void load_fence() {
 }
 
 // The steps of an item, as buffer loads (scalar base and step, the lane's own offset).
-template <typename T>
+template <int TILES>
 struct Steps {
     __amdgpu_buffer_rsrc_t ids_r, masks_r;
     int chunk, last, lane4, n4;
     __device__ __forceinline__ Steps(const AttnSide& s, const Item& item, int lane)
         : ids_r(buffer_rsrc(reinterpret_cast<const float*>(s.ids), 0xffffffffu)),
           masks_r(buffer_rsrc(reinterpret_cast<const float*>(s.masks), 0xffffffffu)),
-          chunk(item.chunk), last(item.chunks * 2 / Attn<T>::kTiles - 1),
-          lane4(lane % (16 * Attn<T>::kTiles) * 4), n4((lane & 15) * 4) {}
+          chunk(item.chunk), last(item.steps(TILES) - 1),
+          lane4(lane % (16 * TILES) * 4), n4((lane & 15) * 4) {}
     // columns of step i, lane l the l-th (modulo their number); a lane that needs others takes
     // them from there
     __device__ __forceinline__ int ids(int i) const {
         const uint32_t at = (uint32_t)chunk * (kAttnCols * 4) +
-                            (uint32_t)min(i, last) * (16 * Attn<T>::kTiles * 4);
+                            (uint32_t)min(i, last) * (16 * TILES * 4);
         return __builtin_amdgcn_raw_buffer_load_b32(ids_r, lane4, (int)at, 0);
     }
     // tile row n's edges of step i, bit 16 t + 4 g + r
     __device__ __forceinline__ uint32_t mask(int i) const {
         i = min(i, last);
-        const uint32_t at = (uint32_t)(chunk + i * Attn<T>::kTiles / 2) * (kAttnRows * 4);
+        const uint32_t at = (uint32_t)(chunk + i * TILES / 2) * (kAttnRows * 4);
         const uint32_t m = __builtin_amdgcn_raw_buffer_load_b32(masks_r, n4, (int)at, 0);
-        return Attn<T>::kTiles == 2 ? m : (m >> ((i & 1) * 16)) & 0xffffu;
+        return TILES == 2 ? m : (m >> ((i & 1) * 16)) & 0xffffu;
     }
 };
 // The columns whose column form this lane holds.
@@ -517,9 +520,19 @@ struct StepCols {
             col[j] = __shfl(ids, (j >> 2) * 16 + 4 * g + (j & 3));
     }
 };
-// Place of the pair with bit `bit` along its row's edges of the step.
-__device__ __forceinline__ int nth_edge(uint32_t mask, int bit) {
-    return __popc(mask & ((1u << bit) - 1u));
+// Place of pair (n, 16 t + 4 g + r) along row n's edges, r = 0..3, `done` of which lie before the
+// step; on[r]: whether it is an edge.
+__device__ __forceinline__ void edge_places(uint32_t mask, int t, int g, int done, int* at,
+                                            bool* on) {
+    const int bit = 16 * t + 4 * g;
+    int a = done + __popc(mask & ((1u << bit) - 1u));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const uint32_t m = (mask >> (bit + r)) & 1u;
+        on[r] = m != 0;
+        at[r] = a;
+        a += (int)m;
+    }
 }
 
 // The bias of an edge and head: value[edge_id e][h] as the caller has it, or value[h][e] in the

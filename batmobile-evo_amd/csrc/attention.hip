@@ -80,14 +80,14 @@ template <typename T, int KP, int VP, bool FULL, bool BIAS, bool WIDE>
 __global__ __launch_bounds__(64, KP + VP <= 256 ? 3 : (KP + VP) * sizeof(T) <= 1536 ? 2 : 1) void attn_fwd_kernel(AttnFwd a) {
     constexpr int kT = Attn<T>::kTiles;
     constexpr float kInf = __builtin_inff(), kSlack = 8.0f;
-    using Rows = RowTile<T, KP>;
+    using Rows = RowTile<T, KP, kT>;
     __shared__ __attribute__((aligned(1024))) char k_lds[Rows::kBytes];
-    __shared__ float b_lds[BIAS ? kTileEdges : 1];
+    __shared__ float b_lds[BIAS ? kTileEdges + 1 : 1];
     int item, h;
     if (!attn_unit(blockIdx.x, a.side.n_items, a.H, item, h)) return;
     const int lane = threadIdx.x, n = lane & 15, g = lane >> 4, kv = h / a.group;
     const Item it(a.side, item, lane);
-    const int row = it.row, steps = it.chunks * 2 / kT;
+    const int row = it.row, steps = it.steps(kT);
     const T* kbase = (const T*)a.k + (int64_t)kv * a.Dk;
     const T* vbase = (const T*)a.v + (int64_t)kv * a.Dv;
     RowFrag<T, KP> q;
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 3 : (KP + VP) * sizeof(T) <= 1
         ColFrag<T, VP> vf;
         uint32_t mask = 0;
         int ids = 0;
-        const Steps<T> step(a.side, it, lane);
+        const Steps<kT> step(a.side, it, lane);
         // v of step i, whose columns `ids` holds; then those of the next step
         auto load_v = [&](int i) {
             const StepCols<T> cols(ids, g);
@@ -132,8 +132,8 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 3 : (KP + VP) * sizeof(T) <= 1
             load_v(0);
         }
         for (int i = 0; i < steps; ++i) {
-            float b[4 * kT];
-            float x[4 * kT];
+            float b[4 * kT], x[4 * kT];
+            bool on[4 * kT];
             Rows::template arrived<ColFrag<T, VP>::kLoads>();
 #pragma unroll
             for (int t = 0; t < kT; ++t) {
@@ -146,23 +146,19 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 3 : (KP + VP) * sizeof(T) <= 1
                 if (kT > 1 && KP + VP > 256) asm volatile("" : "+v"(x[4 * t]) : : "memory");
             }
 #pragma unroll
-            for (int j = 0; j < 4 * kT; ++j) {
-                b[j] = 0.0f;
-                if constexpr (BIAS) {
-                    const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
-                    const int at = done + nth_edge(mask, bit);
-                    b[j] = b_lds[min(it.off + at, kTileEdges - 1)];
-                }
+            for (int t = 0; t < kT; ++t) {
+                int at[4];
+                edge_places(mask, t, g, it.off + done, at, on + 4 * t);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) b[4 * t + r] = BIAS ? b_lds[at[r]] : 0.0f;
             }
             Rows::reads_done();
             Rows::template fill<FULL, WIDE>(k_lds, ids, kbase, a.ks, a.Dk, lane);
             float top = m;
 #pragma unroll
             for (int j = 0; j < 4 * kT; ++j) {
-                const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
-                const bool on = ((mask >> bit) & 1) & (b[j] != -kInf);
-                x[j] = fmaf(x[j], a.scale, b[j]);
-                x[j] = on ? x[j] : -kInf;
+                // (b = -inf and a product that is infinite or NaN: the sums will tell)
+                x[j] = on[j] ? fmaf(x[j], a.scale, b[j]) : -kInf;
                 top = fmaxf(top, x[j]);
             }
             top = max_over_groups(top);

@@ -77,27 +77,28 @@ __device__ __forceinline__ void attn_scores_rows(const AttnScores& a, int item, 
     }
 }
 
+// A step takes 16 columns: with 32 the rows of k and v would leave LDS for 6 waves a CU only.
 // k and v of a step go to LDS while the products of the step before run; p and dp of the step
 // before are written to LDS first, as are all reads done (attn_fwd_kernel).
 template <typename T, int KP, int VP, bool FULL, bool WIDE>
 __global__ __launch_bounds__(64, KP + VP < 512 ? 2 : 1) void attn_scores_kernel(AttnScores a) {
-    constexpr int kT = Attn<T>::kTiles;
+    constexpr int kT = 1;                      // (see the kernel's head)
     constexpr float kInf = __builtin_inff();
-    using KRows = RowTile<T, KP>;
-    using VRows = RowTile<T, VP>;
+    using KRows = RowTile<T, KP, kT>;
+    using VRows = RowTile<T, VP, kT>;
     __shared__ __attribute__((aligned(1024))) char k_lds[KRows::kBytes];
     __shared__ __attribute__((aligned(1024))) char v_lds[VRows::kBytes];
-    __shared__ float p_lds[kTileEdges];              // the bias, then p
-    __shared__ float dp_lds[kTileEdges];
+    __shared__ float p_lds[kTileEdges + 1];          // the bias, then p
+    __shared__ float dp_lds[kTileEdges + 1];
     int item, h;
     if (!attn_unit(blockIdx.x, a.side.n_items, a.H, item, h)) return;
     const int lane = threadIdx.x, n = lane & 15, g = lane >> 4, kv = h / a.group;
     const Item it(a.side, item, lane);
-    const int row = it.row, steps = it.chunks * 2 / kT;
+    const int row = it.row, steps = it.steps(kT);
     if (steps == 0) return;
     const T* kbase = (const T*)a.k + (int64_t)kv * a.Dk;
     const T* vbase = (const T*)a.v + (int64_t)kv * a.Dv;
-    const Steps<T> step(a.side, it, lane);
+    const Steps<kT> step(a.side, it, lane);
     int ids = step.ids(0);
     uint32_t mask = step.mask(0);
     RowFrag<T, KP> q;
@@ -125,18 +126,16 @@ __global__ __launch_bounds__(64, KP + VP < 512 ? 2 : 1) void attn_scores_kernel(
         }, keep_bias);
     float2* ws = a.ws + (int64_t)h * a.edges;
     float d = 0.0f, p[4 * kT], dp[4 * kT];
-    int done = 0, before = 0;                  // row n's edges of earlier steps
-    uint32_t mask_before = 0;
+    int done = 0;                              // row n's edges of earlier steps
+    int at[4 * kT];
+    bool on[4 * kT], was[4 * kT] = {};
     auto keep = [&]() {
 #pragma unroll
-        for (int j = 0; j < 4 * kT; ++j) {
-            const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
-            if ((mask_before >> bit) & 1) {
-                const int at = before + nth_edge(mask_before, bit);
-                p_lds[it.off + at] = p[j];
-                dp_lds[it.off + at] = dp[j];
+        for (int j = 0; j < 4 * kT; ++j)
+            if (was[j]) {
+                p_lds[at[j]] = p[j];
+                dp_lds[at[j]] = dp[j];
             }
-        }
     };
     for (int i = 0; i < steps; ++i) {
         RowFrag<T, KP> kf[kT];
@@ -150,10 +149,10 @@ __global__ __launch_bounds__(64, KP + VP < 512 ? 2 : 1) void attn_scores_kernel(
         keep();
         float b[4 * kT];
 #pragma unroll
-        for (int j = 0; j < 4 * kT; ++j) {
-            const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
-            const int at = done + nth_edge(mask, bit);
-            b[j] = p_lds[min(it.off + at, kTileEdges - 1)];
+        for (int t = 0; t < kT; ++t) {
+            edge_places(mask, t, g, it.off + done, at + 4 * t, on + 4 * t);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) b[4 * t + r] = p_lds[at[4 * t + r]];
         }
         KRows::reads_done();
         KRows::template fill<FULL, WIDE>(k_lds, ids, kbase, a.ks, a.Dk, lane);
@@ -164,11 +163,11 @@ __global__ __launch_bounds__(64, KP + VP < 512 ? 2 : 1) void attn_scores_kernel(
             const v4f s = row_product<T, KP>(kf[t], q);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int j = 4 * t + r, bit = 16 * t + 4 * g + r;
+                const int j = 4 * t + r;
                 const float x = fmaf(s[r], a.scale, b[j]);
-                const bool on = ((mask >> bit) & 1) & (b[j] != -kInf) & (x != -kInf);
                 p[j] = attn_exp(x - ref) * inv;
-                p[j] = on ? p[j] : 0.0f;
+                p[j] = on[j] & (b[j] != -kInf) & (x != -kInf) ? p[j] : 0.0f;
+                was[j] = on[j];
             }
         }
 #pragma unroll
@@ -181,8 +180,6 @@ __global__ __launch_bounds__(64, KP + VP < 512 ? 2 : 1) void attn_scores_kernel(
                 d = fmaf(p[j], dp[j], d);
             }
         }
-        before = done;
-        mask_before = mask;
         done += __popc(mask);
         mask = step.mask(i + 1);
     }
@@ -304,12 +301,12 @@ __global__ __launch_bounds__(64, P * sizeof(T) <= 256 || P == 64 ? 2 : 1) void a
     const int which = (blockIdx.x >= all.first[1]) + (blockIdx.x >= all.first[2]);
     const AttnSum& a = all.sum[which];
     constexpr int kT = Attn<T>::kTiles, kR = Attn<T>::kRowsPerLane;
-    __shared__ float w_lds[kTileEdges];
+    __shared__ float w_lds[kTileEdges + 1];
     int item, head;
     if (!attn_unit(blockIdx.x - all.first[which], a.side.n_items, a.heads, item, head)) return;
     const int lane = threadIdx.x, n = lane & 15, g = lane >> 4;
     const Item it(a.side, item, lane);
-    const int row = it.row, steps = it.chunks * 2 / kT;
+    const int row = it.row, steps = it.steps(kT);
     if (__builtin_expect(it.total > kTileEdges, 0)) {
         attn_sum_rows<T>(a, item, head, it);
         return;
@@ -322,7 +319,7 @@ __global__ __launch_bounds__(64, P * sizeof(T) <= 256 || P == 64 ? 2 : 1) void a
             const T* x = (const T*)a.x + (int64_t)(hh / a.x_div) * a.D;
             const float* wh = a.w + (int64_t)hh * a.edges * a.w_step;
             // two steps' rows in turn: one is read while the other is multiplied
-            const Steps<T> step(a.side, it, lane);
+            const Steps<kT> step(a.side, it, lane);
             ColFrag<T, P> x0, x1;
             int s0 = step.ids(0), s1 = step.ids(1);
             uint32_t m0 = step.mask(0), m1 = step.mask(1);
@@ -343,11 +340,12 @@ __global__ __launch_bounds__(64, P * sizeof(T) <= 256 || P == 64 ? 2 : 1) void a
             auto mac = [&](uint32_t mask, const ColFrag<T, P>& f) {
                 float w[kR];
 #pragma unroll
-                for (int j = 0; j < kR; ++j) {
-                    const int bit = (j >> 2) * 16 + 4 * g + (j & 3);
-                    const int at = done + nth_edge(mask, bit);
-                    const float v = w_lds[min(it.off + at, kTileEdges - 1)];
-                    w[j] = (mask >> bit) & 1 ? v : 0.0f;
+                for (int t = 0; t < kT; ++t) {
+                    int at[4];
+                    bool on[4];
+                    edge_places(mask, t, g, it.off + done, at, on);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) w[4 * t + r] = on[r] ? w_lds[at[r]] : 0.0f;
                 }
                 done += __popc(mask);
                 f.mac(w, acc);

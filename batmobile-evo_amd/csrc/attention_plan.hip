@@ -178,10 +178,10 @@ __global__ __launch_bounds__(kPlanThreads) void plan_items_kernel(PlanArgs a) {
     const int n = pre[kAttnRows];
     uint32_t* masks = reinterpret_cast<uint32_t*>(a.plan) + a.at.masks + chunk0 * kAttnRows;
     int* ids = a.plan + a.at.ids + chunk0 * kAttnCols;
-    auto finish = [&](int chunks, int part_at) {
-        if (tid == 0) *reinterpret_cast<int4*>(out) = make_int4(tile, (int)chunk0, chunks, part_at);
-    };
     const int part_at = parts > 1 ? a.plan[a.at.tile_part + tile] + part : -1;
+    auto finish = [&](int columns) {
+        if (tid == 0) *reinterpret_cast<int4*>(out) = make_int4(tile, (int)chunk0, columns, part_at);
+    };
     auto column = [&](int i, int& r) {               // of the i-th edge, row by row
         r = 0;
 #pragma unroll
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_items_kernel(PlanArgs a) {
             for (int b = b0; b < b1; ++b) m |= 1u << b;
             masks[i] = m;
         }
-        finish(chunks, part_at);
+        finish(n);
         return;
     }
     int size = 64;
@@ -278,7 +278,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_items_kernel(PlanArgs a) {
     for (int i = tid; i < chunks * kAttnRows; i += kPlanThreads) masks[i] = mask[i];
     for (int i = total + tid; i < chunks * kAttnCols; i += kPlanThreads)
         ids[i] = (int)(key[n - 1] >> 20);             // read with factor 0
-    finish(chunks, part_at);
+    finish(total);
 }
 
 // A wave per row: offsets in order, columns in range and ascending.

@@ -215,49 +215,56 @@ __global__ __launch_bounds__(W <= 4 ? 256 : 64 * W) void norm_bwd_kernel(NormArg
     float aw_pre[NV], aw_post[NV], a_scale[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) aw_pre[i] = aw_post[i] = a_scale[i] = 0.0f;
-    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < a.n;
-         row0 += (int64_t)gridDim.x * kRows) {
+    // the next row's loads are under way while this one's sums are formed; lanes past C read the
+    // row's last channel and drop it
+    struct Row {
+        Raw4<T> gh[NV], h[NV], gn[NV], y[NV];
+        float sg[NV], r_pre, r_post;
+    };
+    auto load = [&](Row& x, int64_t row0) {
+        const int64_t row = min(row0 + group, a.n - 1);
+        const int64_t at = row * (int64_t)a.C * 16;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = min(i * 64 * W + t, a.C * 4 - 4 + q);
+            if constexpr (PRE) {
+                x.h[i].load((const T*)a.h + at + e * 4);
+                x.gn[i].load((const T*)a.gn + at + e * 4);
+            }
+            if (a.gh) x.gh[i].load((const T*)a.gh + at + e * 4);
+            else x.gh[i].zero();
+            if constexpr (BLOCK) {
+                x.y[i].load((const T*)a.y + at + e * 4);
+                if constexpr (GATE) x.sg[i] = norm_ld((const T*)a.gate + row * a.C * 4 + e);
+            }
+        }
+        if constexpr (PRE) x.r_pre = a.rs_in[row * 8 + 4 + q];
+        if constexpr (BLOCK) x.r_post = a.rs_in[row * 8 + q];
+    };
+    const int64_t step = (int64_t)gridDim.x * kRows;
+    Row next;
+    load(next, (int64_t)blockIdx.x * kRows);
+    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < a.n; row0 += step) {
         const bool there = row0 + group < a.n;
         const int64_t row = there ? row0 + group : a.n - 1;
         const int64_t at = row * (int64_t)a.C * 16;
+        Row x = next;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (!(there && ((i * 64 * W + t) >> 2) < a.C)) {
+                if constexpr (PRE) x.gn[i].zero();
+                if constexpr (BLOCK) x.y[i].zero();
+            }
+        if (row0 + step < a.n) load(next, row0 + step);
         float4 G[NV];
-        Raw4<T> gh[NV], h[NV], gn[NV], y[NV];
-        float sg[NV];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const bool in = there && ((i * 64 * W + t) >> 2) < a.C;
-            const int64_t o = at + (int64_t)(i * 64 * W + t) * 4;
-            gh[i].zero();
-            h[i].zero();
-            gn[i].zero();
-            if (in) {
-                if constexpr (PRE) {
-                    h[i].load((const T*)a.h + o);
-                    gn[i].load((const T*)a.gn + o);
-                }
-                if (a.gh) gh[i].load((const T*)a.gh + o);
-            }
-        }
-        if constexpr (BLOCK) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                y[i].zero();
-                sg[i] = 0.0f;
-                if (there && ((i * 64 * W + t) >> 2) < a.C) {
-                    y[i].load((const T*)a.y + at + (int64_t)(i * 64 * W + t) * 4);
-                    if constexpr (GATE)
-                        sg[i] = norm_ld((const T*)a.gate + row * a.C * 4 + i * 64 * W + t);
-                }
-            }
-        }
         if constexpr (PRE) {
-            const float r = a.rs_in[row * 8 + 4 + q];
+            const float r = x.r_pre;
             float s = 0.0f, wp[NV];
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = (i * 64 * W + t) >> 2;
                 wp[i] = a.w_pre[q * a.C + min(c, a.C - 1)];
-                const float v = dot4(gn[i].get(), h[i].get(), q);   // 0 past C
+                const float v = dot4(x.gn[i].get(), x.h[i].get(), q);   // 0 past C
                 aw_pre[i] = fmaf(r, v, aw_pre[i]);
                 s = fmaf(wp[i], v, s);
             }
@@ -266,7 +273,7 @@ __global__ __launch_bounds__(W <= 4 ? 256 : 64 * W) void norm_bwd_kernel(NormArg
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const float fa = first_of(wp[i] * r), fb = others_of(wp[i] * r);
-                const float4 gni = gn[i].get(), hi = h[i].get(), ghi = gh[i].get();
+                const float4 gni = x.gn[i].get(), hi = x.h[i].get(), ghi = x.gh[i].get();
                 G[i] = make_float4(ghi.x + fmaf(fa, gni.x, ka * hi.x),
                                    ghi.y + fmaf(fb, gni.y, kb * hi.y),
                                    ghi.z + fmaf(fb, gni.z, kb * hi.z),
@@ -274,21 +281,21 @@ __global__ __launch_bounds__(W <= 4 ? 256 : 64 * W) void norm_bwd_kernel(NormArg
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) G[i] = gh[i].get();
+            for (int i = 0; i < NV; ++i) G[i] = x.gh[i].get();
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i)
             if (there && ((i * 64 * W + t) >> 2) < a.C)
                 norm_st4((T*)a.gx + at + (int64_t)(i * 64 * W + t) * 4, G[i]);
         if constexpr (BLOCK) {
-            const float r = a.rs_in[row * 8 + q];
+            const float r = x.r_post;
             float s = 0.0f, f[NV];
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = (i * 64 * W + t) >> 2;
-                const float g = GATE ? 1.0f / (1.0f + __expf(-sg[i])) : 1.0f;
+                const float g = GATE ? __builtin_amdgcn_rcpf(1.0f + __expf(-x.sg[i])) : 1.0f;
                 const float sc = a.scale[min(c, a.C - 1)], w = a.w_post[q * a.C + min(c, a.C - 1)];
-                const float z = dot4(G[i], y[i].get(), q), rz = r * z;   // 0 past C
+                const float z = dot4(G[i], x.y[i].get(), q), rz = r * z;   // 0 past C
                 f[i] = sc * g * w;
                 s = fmaf(f[i], z, s);
                 aw_post[i] = fmaf(sc * g, rz, aw_post[i]);
@@ -303,7 +310,7 @@ __global__ __launch_bounds__(W <= 4 ? 256 : 64 * W) void norm_bwd_kernel(NormArg
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const float fa = first_of(f[i] * r), fb = others_of(f[i] * r);
-                const float4 yi = y[i].get();
+                const float4 yi = x.y[i].get();
                 if (there && ((i * 64 * W + t) >> 2) < a.C)
                     norm_st4((T*)a.gy + at + (int64_t)(i * 64 * W + t) * 4,
                              make_float4(fmaf(fa, G[i].x, ka * yi.x), fmaf(fb, G[i].y, kb * yi.y),
@@ -392,6 +399,7 @@ static void norm_pick(const NormArgs& a, bool bwd, hipStream_t s) {
         else if (a.C <= 128) norm_bwd_launch<T, 4, 2, BLOCK, GATE, PRE>(a, s);
         else if (a.C <= 256) norm_bwd_launch<T, 4, 4, BLOCK, GATE, PRE>(a, s);
         else if (a.C <= 512) norm_bwd_launch<T, 8, 4, BLOCK, GATE, PRE>(a, s);
+        else if (a.C <= 1024) norm_bwd_launch<T, 4, 16, BLOCK, GATE, PRE>(a, s);
         else norm_bwd_launch<T, 8, 16, BLOCK, GATE, PRE>(a, s);
         return;
     }
