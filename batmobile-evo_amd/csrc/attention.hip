@@ -90,23 +90,10 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 3 : (KP + VP) * sizeof(T) <= 1
     const int row = it.row, steps = it.steps(kT);
     const T* kbase = (const T*)a.k + (int64_t)kv * a.Dk;
     const T* vbase = (const T*)a.v + (int64_t)kv * a.Dv;
-    RowFrag<T, KP> q;
-    // (a slot past the last row computes with row 0 and stores nothing)
-    q.template load<FULL>(row_of<T>(a.q, max(row, 0), a.qs) + (int64_t)h * a.Dk, a.Dk, g);
-    if constexpr (BIAS) {
-        if (__builtin_expect(it.total > kTileEdges, 0)) {
-            attn_fwd_rows<T>(a, item, h, it.tile, it.part);
-            return;
-        }
-        auto keep = [&](int i, int, float b, int) { b_lds[i] = b; };
-        if (a.bias.eid)
-            it.each<float>(a.side, lane, [&](int e) { return a.bias.at(e, h); }, keep);
-        else
-            it.each<float>(a.side, lane, [&](int e) {
-                return a.bias.value[(int64_t)e * a.bias.edge_step + h * a.bias.head_step];
-            }, keep);
+    if (BIAS && __builtin_expect(it.total > kTileEdges, 0)) {
+        attn_fwd_rows<T>(a, item, h, it.tile, it.part);
+        return;
     }
-
     v4f acc[ColFrag<T, VP>::kAcc];
     float m = -kInf, l = 0.0f;
 #pragma unroll
@@ -128,8 +115,22 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 3 : (KP + VP) * sizeof(T) <= 1
         if (steps > 0) {
             ids = step.ids(0);
             mask = step.mask(0);
+        }
+        RowFrag<T, KP> q;
+        // (a slot past the last row computes with row 0 and stores nothing)
+        q.template load<FULL>(row_of<T>(a.q, max(row, 0), a.qs) + (int64_t)h * a.Dk, a.Dk, g);
+        if (steps > 0) {
             Rows::template fill<FULL, WIDE>(k_lds, ids, kbase, a.ks, a.Dk, lane);
             load_v(0);
+        }
+        if constexpr (BIAS) {
+            auto keep = [&](int i, int, float b, int) { b_lds[i] = b; };
+            if (a.bias.eid)
+                it.each<float>(a.side, lane, [&](int e) { return a.bias.at(e, h); }, keep);
+            else
+                it.each<float>(a.side, lane, [&](int e) {
+                    return a.bias.value[(int64_t)e * a.bias.edge_step + h * a.bias.head_step];
+                }, keep);
         }
         for (int i = 0; i < steps; ++i) {
             float b[4 * kT], x[4 * kT];

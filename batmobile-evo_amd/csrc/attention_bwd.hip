@@ -296,7 +296,7 @@ struct AttnSums {
 };
 
 template <typename T, int P>
-__global__ __launch_bounds__(64, P * sizeof(T) <= 256 || P == 64 ? 2 : 1) void attn_sum_kernel(
+__global__ __launch_bounds__(64, sizeof(T) == 4 || P <= 128 ? 2 : 1) void attn_sum_kernel(
     AttnSums all) {
     const int which = (blockIdx.x >= all.first[1]) + (blockIdx.x >= all.first[2]);
     const AttnSum& a = all.sum[which];
