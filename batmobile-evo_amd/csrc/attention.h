@@ -399,9 +399,9 @@ __device__ __forceinline__ void attn_store_w(float* p, const float* v) {
         *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
 }
 
-// f times a tile row's sums to its row of results (T, or fp32 for the parts of a cut tile).
-template <typename T, int P, typename O>
-__device__ __forceinline__ void store_rows(O* row, const v4f* acc, float f, int D, int g) {
+// f times a tile row's sums to its row of an fp32 part (a cut tile).
+template <typename T, int P>
+__device__ __forceinline__ void store_part(float* row, const v4f* acc, float f, int D, int g) {
     constexpr int kW = ColFrag<T, P>::kW, kBlocks = ColFrag<T, P>::kBlocks;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b)
@@ -414,6 +414,45 @@ __device__ __forceinline__ void store_rows(O* row, const v4f* acc, float f, int 
             if (d < D) attn_store_w<kW>(row + d, v);
         }
 }
+
+// f times the tile's sums to its rows of results, row i's at out + i * stride elements.  A lane
+// holds 16-byte pieces of one row; written as they are, a store would send 64 pieces to 64 cache
+// lines.  They go through LDS (the pieces' places with the row's low bits flipped, as in RowTile)
+// and leave as whole rows.
+template <typename T, int P>
+struct OutTile {
+    static constexpr int kPieces = P * (int)sizeof(T) / 16, kBytes = 16 * kPieces * 16;
+    static constexpr int kFlip = (kPieces < 16 ? kPieces : 16) - 1;
+    static __device__ __forceinline__ void store(char* lds, T* out, int64_t stride, int row,
+                                                 const v4f* acc, float f, int D, int lane) {
+        constexpr int kW = ColFrag<T, P>::kW, kBlocks = ColFrag<T, P>::kBlocks;
+        constexpr int kBytesW = kW * (int)sizeof(T);       // 16, or 8: half a piece
+        const int n = lane & 15, g = lane >> 4;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float v[kW];
+#pragma unroll
+                for (int c = 0; c < kW; ++c) v[c] = acc[b * kW + c][r] * f;
+                const int at = (b * 16 + 4 * g + r) * kBytesW;
+                attn_store_w<kW>(reinterpret_cast<T*>(lds + n * kPieces * 16 +
+                                                      ((at / 16) ^ (n & kFlip)) * 16 + at % 16),
+                                 v);
+            }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int k = 0; k < kPieces / 4; ++k) {
+            const int i = k * 64 + lane, to = i / kPieces, piece = i % kPieces;
+            const v4u v = *reinterpret_cast<const v4u*>(
+                lds + to * kPieces * 16 + (piece ^ (to & kFlip)) * 16);
+            const int at = __shfl(row, to);
+            if (at >= 0 && piece * 16 < D * (int)sizeof(T))
+                *reinterpret_cast<v4u*>((char*)(out + at * stride) + piece * 16) = v;
+        }
+    }
+};
 
 // ---------------------------------------------------------------------------
 // A wave's item, and its values per edge in LDS in the order of the rows: read from memory once,

@@ -81,7 +81,8 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 3 : (KP + VP) * sizeof(T) <= 1
     constexpr int kT = Attn<T>::kTiles;
     constexpr float kInf = __builtin_inff(), kSlack = 8.0f;
     using Rows = RowTile<T, KP, kT>;
-    __shared__ __attribute__((aligned(1024))) char k_lds[Rows::kBytes];
+    __shared__ __attribute__((aligned(1024))) char k_lds[
+        Rows::kBytes > OutTile<T, VP>::kBytes ? Rows::kBytes : OutTile<T, VP>::kBytes];
     __shared__ float b_lds[BIAS ? kTileEdges + 1 : 1];
     int item, h;
     if (!attn_unit(blockIdx.x, a.side.n_items, a.H, item, h)) return;
@@ -186,28 +187,28 @@ __global__ __launch_bounds__(64, KP + VP <= 256 ? 3 : (KP + VP) * sizeof(T) <= 1
             load_v(i + 1);
         }
     }
+    // (the last fill of k, which nothing read, must not land in the results)
+    Rows::template arrived<0>();
     l = sum_over_groups(l);
     if (__builtin_expect(any_not_finite<ColFrag<T, VP>::kAcc>(acc), 0)) {
         attn_fwd_rows<T>(a, item, h, it.tile, it.part);
         return;
     }
-    if (row < 0) return;
     if (it.part >= 0) {
+        if (row < 0) return;
         const int64_t at = ((int64_t)it.part * a.H + h) * kAttnRows + n;
-        store_rows<T, VP>(a.part_o + at * a.Dv, acc, 1.0f, a.Dv, g);
+        store_part<T, VP>(a.part_o + at * a.Dv, acc, 1.0f, a.Dv, g);
         if (g == 0) {
             a.part_ml[at * 2] = m;
             a.part_ml[at * 2 + 1] = l;
         }
         return;
     }
-    const int64_t at = (int64_t)row * a.H + h;
+    if (a.stats && g == 0 && row >= 0)
+        *reinterpret_cast<float2*>(a.stats + ((int64_t)row * a.H + h) * 2) = make_float2(m, l);
     // l is 0 only without an edge; a NaN stays one
-    store_rows<T, VP>((T*)a.out + at * a.Dv, acc, l == 0.0f ? 0.0f : 1.0f / l, a.Dv, g);
-    if (a.stats && g == 0) {
-        a.stats[at * 2] = m;
-        a.stats[at * 2 + 1] = l;
-    }
+    OutTile<T, VP>::store(k_lds, (T*)a.out + (int64_t)h * a.Dv, (int64_t)a.H * a.Dv, row, acc,
+                          l == 0.0f ? 0.0f : 1.0f / l, a.Dv, lane);
 }
 
 // Joins the parts of a cut tile, row by row: workgroup p of the parts takes rows p, p + parts of
@@ -308,40 +309,75 @@ static void attn_fwd_run(const AttnFwd& a, bool wide, int parts, hipStream_t s) 
 
 using namespace bmhip;
 
-// in [E, H] (row edge_id e) <-> out [H, E]: 64 edges and up to 32 heads a workgroup, through LDS,
-// so that both sides are contiguous.
+// in [E, H] (row edge_id e) <-> out [H, E]: 256 edges and up to 16 heads a workgroup, through LDS,
+// so that both sides are contiguous.  A thread takes up to 4 heads of an edge, 16 bytes where H
+// allows.
 template <bool TO_HEADS>
 __global__ __launch_bounds__(256) void attn_edges_kernel(const float* __restrict__ in,
                                                          const int* __restrict__ eid,
                                                          float* __restrict__ out, int64_t edges,
                                                          int H) {
-    __shared__ float t[64][33];
-    const int64_t e0 = (int64_t)blockIdx.x * 64;
-    const int h0 = blockIdx.y * 32, n = (int)min((int64_t)64, edges - e0), w = min(32, H - h0);
-    // the [E, H] side: w values of an edge next to each other
-    auto rows = [&](auto&& f) {
-        for (int i = threadIdx.x; i < n * w; i += 256) {
-            const int e = i / w, h = i - e * w;
-            f(e, h, (eid ? (int64_t)eid[e0 + e] : e0 + e) * H + h0 + h);
+    __shared__ float t[16][257];
+    const int64_t e0 = (int64_t)blockIdx.x * 256;
+    const int h0 = blockIdx.y * 16, n = (int)min((int64_t)256, edges - e0), w = min(16, H - h0);
+    const int groups = w <= 4 ? 1 : w <= 8 ? 2 : 4, g = threadIdx.x & (groups - 1);
+    const int per = 256 / groups, h = 4 * g, nh = min(4, w - h);
+    const bool vec = (H & 3) == 0;
+    auto rows = [&]() {
+        for (int k = 0; k < groups; ++k) {
+            const int e = k * per + threadIdx.x / groups;
+            if (e >= n || nh <= 0) continue;
+            const int64_t at = (eid ? (int64_t)eid[e0 + e] : e0 + e) * H + h0 + h;
+            if (TO_HEADS) {
+                float4 v = make_float4(0, 0, 0, 0);
+                if (vec) {
+                    v = *reinterpret_cast<const float4*>(in + at);
+                } else {
+                    v.x = in[at];
+                    if (nh > 1) v.y = in[at + 1];
+                    if (nh > 2) v.z = in[at + 2];
+                    if (nh > 3) v.w = in[at + 3];
+                }
+                t[h][e] = v.x;
+                t[h + 1][e] = v.y;
+                t[h + 2][e] = v.z;
+                t[h + 3][e] = v.w;
+            } else {
+                const float4 v = make_float4(t[h][e], t[h + 1][e], t[h + 2][e], t[h + 3][e]);
+                if (vec) {
+                    *reinterpret_cast<float4*>(out + at) = v;
+                } else {
+                    out[at] = v.x;
+                    if (nh > 1) out[at + 1] = v.y;
+                    if (nh > 2) out[at + 2] = v.z;
+                    if (nh > 3) out[at + 3] = v.w;
+                }
+            }
         }
     };
-    auto cols = [&](auto&& f) {
-        for (int i = threadIdx.x; i < 64 * w; i += 256)
-            if ((i & 63) < n) f(i & 63, i >> 6, (int64_t)(h0 + (i >> 6)) * edges + e0 + (i & 63));
+    auto cols = [&]() {
+        const int e = threadIdx.x;
+        if (e >= n) return;
+#pragma unroll 4
+        for (int i = 0; i < w; ++i) {
+            const int64_t at = (int64_t)(h0 + i) * edges + e0 + e;
+            if (TO_HEADS) out[at] = t[i][e];
+            else t[i][e] = in[at];
+        }
     };
-    if (TO_HEADS) rows([&](int e, int h, int64_t at) { t[e][h] = in[at]; });
-    else cols([&](int e, int h, int64_t at) { t[e][h] = in[at]; });
+    if (TO_HEADS) rows(); else cols();
     __syncthreads();
-    if (TO_HEADS) cols([&](int e, int h, int64_t at) { out[at] = t[e][h]; });
-    else rows([&](int e, int h, int64_t at) { out[at] = t[e][h]; });
+    if (TO_HEADS) cols(); else rows();
 }
 
 extern "C" int batteries_attention_edges_by_head(const float* values, const int32_t* edge_id,
                                                  float* out, int64_t n_edges, int H, int back,
                                                  hipStream_t stream) {
-    if (n_edges < 0 || H <= 0 || H > 65535 * 32 || n_edges >= INT32_MAX / 4) return BM_ERR_ARG;
+    if (n_edges < 0 || H <= 0 || H > 65535 || n_edges >= INT32_MAX / 4 ||
+        !aligned_to({values, out}, 16))
+        return BM_ERR_ARG;
     if (n_edges == 0) return BM_OK;
-    const dim3 grid((unsigned)ceil_div(n_edges, 64), (unsigned)ceil_div(H, 32));
+    const dim3 grid((unsigned)ceil_div(n_edges, 256), (unsigned)ceil_div(H, 16));
     if (back) attn_edges_kernel<false><<<grid, 256, 0, stream>>>(values, edge_id, out, n_edges, H);
     else attn_edges_kernel<true><<<grid, 256, 0, stream>>>(values, edge_id, out, n_edges, H);
     return (int)hipGetLastError();

@@ -184,6 +184,7 @@ __global__ __launch_bounds__(64, KP + VP < 512 ? 2 : 1) void attn_scores_kernel(
         mask = step.mask(i + 1);
     }
     keep();
+    KRows::template arrived<0>();              // the last fills, which nothing reads
     auto place = [&](int e) { return a.place[e]; };
     if (it.part >= 0) {                        // the rest once all parts of the row are there
         it.each<int>(a.side, lane, place, [&](int i, int, int to, int) {
@@ -301,7 +302,10 @@ __global__ __launch_bounds__(64, sizeof(T) == 4 || P <= 128 ? 2 : 1) void attn_s
     const int which = (blockIdx.x >= all.first[1]) + (blockIdx.x >= all.first[2]);
     const AttnSum& a = all.sum[which];
     constexpr int kT = Attn<T>::kTiles, kR = Attn<T>::kRowsPerLane;
-    __shared__ float w_lds[kTileEdges + 1];
+    constexpr int kBytes = (kTileEdges + 1) * 4;
+    __shared__ __attribute__((aligned(16))) char
+        lds[kBytes > OutTile<T, P>::kBytes ? kBytes : OutTile<T, P>::kBytes];
+    float* w_lds = reinterpret_cast<float*>(lds);
     int item, head;
     if (!attn_unit(blockIdx.x - all.first[which], a.side.n_items, a.heads, item, head)) return;
     const int lane = threadIdx.x, n = lane & 15, g = lane >> 4;
@@ -364,12 +368,15 @@ __global__ __launch_bounds__(64, sizeof(T) == 4 || P <= 128 ? 2 : 1) void attn_s
         attn_sum_rows<T>(a, item, head, it);
         return;
     }
-    if (row < 0) return;
-    if (it.part >= 0)
-        store_rows<T, P>(a.part + (((int64_t)it.part * a.heads + head) * kAttnRows + n) * a.D, acc,
-                         a.f, a.D, g);
-    else
-        store_rows<T, P>((T*)a.out + ((int64_t)row * a.heads + head) * a.D, acc, a.f, a.D, g);
+    if (it.part >= 0) {
+        if (row >= 0)
+            store_part<T, P>(
+                a.part + (((int64_t)it.part * a.heads + head) * kAttnRows + n) * a.D, acc, a.f,
+                a.D, g);
+        return;
+    }
+    OutTile<T, P>::store(lds, (T*)a.out + (int64_t)head * a.D, (int64_t)a.heads * a.D, row, acc,
+                         a.f, a.D, lane);
 }
 
 // Adds the parts of a cut tile, row by row (as attn_join_kernel).

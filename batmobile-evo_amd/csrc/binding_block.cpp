@@ -179,6 +179,8 @@ std::tuple<Tensor, Tensor, Tensor> neighbor_attention(const Tensor& q_, const Te
     const Tensor q = heads16(q_), k = heads16(k_), v = heads16(v_);
     Tensor bias, by_head;
     if (bias_) bias = bias_->contiguous();
+    if (bias.defined() && (reinterpret_cast<uintptr_t>(bias.data_ptr()) & 15))
+        bias = bias.clone(at::MemoryFormat::Contiguous);
     if (bias.defined() && s.H > 1 && E * s.H >= kByHead) {
         by_head = torch::empty({s.H, E}, bias.options());
         check_status(batteries_attention_edges_by_head(bias.data_ptr<float>(), eid,
