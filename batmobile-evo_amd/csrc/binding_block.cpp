@@ -165,6 +165,24 @@ AttnShape attn_shape(const Tensor& q, const Tensor& k, const Tensor& v, const Op
 // (writes) all cache lines of the array.  The extra launch pays from about here on.
 constexpr int64_t kByHead = 1 << 18;
 
+// values [E, H] -> [H, E] in the order of edge_id, or back
+Tensor attention_edges_by_head(const Tensor& values, const OptTensor& edge_id, bool back) {
+    TORCH_CHECK(values.is_cuda(), "values must be a CUDA tensor");
+    TORCH_CHECK(values.scalar_type() == torch::kFloat32 && values.dim() == 2 &&
+                    values.is_contiguous(),
+                "values must be a contiguous float32 matrix");
+    const int64_t E = values.size(back ? 1 : 0), H = values.size(back ? 0 : 1);
+    const c10::DeviceGuard guard(values.device());
+    const int32_t* eid = opt_index32(edge_id, values, E, "edge_id");
+    Tensor out = back ? torch::empty({E, H}, values.options()) : torch::empty({H, E}, values.options());
+    if (E == 0 || H == 0) return out;
+    check_status(batteries_attention_edges_by_head(values.data_ptr<float>(), eid,
+                                                   out.data_ptr<float>(), E, (int)H, back,
+                                                   stream_of(values)),
+                 "attention_edges_by_head");
+    return out;
+}
+
 // (out, stats, bias by head): the last two for the backward, if kept
 std::tuple<Tensor, Tensor, Tensor> neighbor_attention(const Tensor& q_, const Tensor& k_,
                                                       const Tensor& v_, const OptTensor& bias_,
@@ -456,6 +474,9 @@ void register_block_ops(pybind11::module_& m) {
     m.def("attention_plan", &attention_plan, py::arg("row_ptr"), py::arg("col"),
           py::arg("order"), py::arg("n_cols"), py::arg("check") = true,
           "tiles of a graph side for the attention -> (plan, items, parts, flags)");
+    m.def("attention_edges_by_head", &attention_edges_by_head, py::arg("values"),
+          py::arg("edge_id") = py::none(), py::arg("back") = false,
+          "values [E, H] (row edge_id[e] of edge e) -> [H, E]; back: the other way");
     m.def("neighbor_attention", &neighbor_attention, py::arg("q"), py::arg("k"), py::arg("v"),
           py::arg("bias"), py::arg("plan"), py::arg("items"), py::arg("parts"),
           py::arg("num_edges"), py::arg("edge_id"), py::arg("scale"),

@@ -7,6 +7,8 @@ names, re-exported from the compiled extension, plus the autograd wrappers.
 - 34-path Clebsch-Gordan tensor products (simple and channel-weighted)
 - Fused SH + tensor product, with scatter-add into destination nodes
 - CSR conversion and cell-list neighbor lists
+- Equivariant transformer blocks: attention over a graph's edges, norms by degree with gate and
+  residual, gradient clipping
 
 There is no CPU fallback: importing this package without the built extension
 raises ImportError.
@@ -65,6 +67,7 @@ from .attention import AttentionPlan, NeighborAttentionFunction, neighbor_attent
 from .block_norm import (  # noqa: E402
     GatedResidualNormFunction, equivariant_norm, gated_residual_norm)
 from .grad_clip import clip_grad_norm, clip_grad_norm_  # noqa: E402
+from .attention_block import AttentionBlock  # noqa: E402
 
 # Autograd-compatible wrappers (reference __init__.py:35-44)
 from .autograd import (  # noqa: E402
@@ -124,4 +127,5 @@ __all__ = [
     "gated_residual_norm",
     "clip_grad_norm",
     "clip_grad_norm_",
+    "AttentionBlock",
 ]

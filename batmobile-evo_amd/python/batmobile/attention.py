@@ -7,7 +7,9 @@ over the edges e: j -> i of the graph,
     out[i, h] = sum_e p_eh v[j, g],                g = h // (H / H_kv)
 
 Equivariant features [N, C, 16] go in as heads of C / H channels, `x.view(N, H, C // H * 16)`:
-the product over a channel's 16 components does not change under rotations.
+the product over a channel's 16 components does not change under rotations.  The backward
+recomputes the probabilities from each row's reference and sum; no sum's order varies, so results
+are the same from run to run.
 """
 import math
 

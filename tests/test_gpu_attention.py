@@ -341,3 +341,154 @@ def test_refusals(dev):
         batmobile.AttentionPlan(s.int(), r, 5)
     with pytest.raises(ValueError, match="destinations"):
         batmobile.AttentionPlan.from_edge_index(torch.stack([s, s]), 2, 5)
+
+
+def test_bias_by_head(dev):
+    """Enough edges and heads that the bias and its gradient go through [H, E]; edges in the
+    caller's own order as well.  The sums are checked on a part of the rows and sources."""
+    import batmobile
+    n, e, h, d = 900, 36000, 8, 8
+    g = gen(81)
+    assert e * h >= 1 << 18
+    ei = torch.stack([torch.randint(0, n, (e,), generator=g), torch.randint(0, n, (e,), generator=g)])
+    t = _inputs(n, n, e, h, 4, d, d, "f32", 82)
+    out, grads = _run(dev, batmobile.AttentionPlan.from_edge_index(ei.to(dev), n), t)
+    by = np.lexsort((ei[0].numpy(), ei[1].numpy()))
+    row_ptr = np.searchsorted(ei[1].numpy()[by], np.arange(n + 1))
+    want, wg = ob.attention(_np(t["q"]), _np(t["k"]), _np(t["v"]), ei[0].numpy()[by], row_ptr,
+                            _np(t["bias"])[by], go=_np(t["go"]))
+    back = np.empty_like(wg["bias"])
+    back[by] = wg["bias"]
+    _compare(out, grads, want, dict(wg, bias=back), "f32")
+
+
+@pytest.mark.parametrize("h", [1, 3, 5, 16, 17, 40])
+def test_edges_by_head(bm, dev, h):
+    """The transposition itself, whole and partial groups of edges and heads, with and without an
+    order, there and back: exact."""
+    for e in (1, 255, 256, 1000):
+        x = torch.randn(e, h, generator=gen(83))
+        order = torch.randperm(e, generator=gen(84))
+        q = torch.zeros(4, h, 4, device=dev)
+        for eid in (None, order):
+            got = bm.attention_edges_by_head(x.to(dev), None if eid is None else eid.int().to(dev))
+            want = x if eid is None else x[eid]
+            assert torch.equal(got.cpu(), want.t())
+            again = bm.attention_edges_by_head(got, None if eid is None else eid.int().to(dev), True)
+            assert torch.equal(again.cpu(), x)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_key_rows_past_32_bit_offsets(dev, dtype):
+    """Sources whose rows lie more than 2^32 bytes apart from the first: k and v are slices of a
+    wide table, read at 64-bit offsets."""
+    import batmobile
+    if torch.cuda.get_device_properties(0).total_memory < 40 << 30:
+        pytest.skip("needs 10 GB")
+    m, h, d = 300, 2, 32
+    size = 4 if dtype == "f32" else 2
+    wide = (1 << 24) // size                    # 16 MB a row: 300 rows are 5 GB
+    src, row_ptr = _edges([20] * 30, m, 85)
+    t = _inputs(30, m, len(src), h, h, d, d, dtype, 86)
+    plan = batmobile.AttentionPlan(torch.from_numpy(src).to(dev),
+                                   torch.from_numpy(row_ptr).to(dev), m)
+    want, wg = _run(dev, plan, t)
+    table = torch.zeros(m, wide, dtype=TYPES[dtype], device=dev)
+    k = table[:, 64:64 + h * d].view(m, h, d)
+    v = table[:, 4096:4096 + h * d].view(m, h, d)
+    k.copy_(t["k"].to(dev))
+    v.copy_(t["v"].to(dev))
+    s = {x: t[x].to(dev) for x in t}
+    leaf = [s["q"].requires_grad_(True), k.detach().requires_grad_(True),
+            v.detach().requires_grad_(True), s["bias"].requires_grad_(True)]
+    out = batmobile.neighbor_attention(*leaf[:3], plan, bias=leaf[3])
+    assert torch.equal(out, want)
+    for name, got in zip(("q", "k", "v", "bias"), torch.autograd.grad(out, leaf, s["go"])):
+        assert torch.equal(got, wg[name]), name
+
+
+def test_plan_covers_every_edge_once(bm, dev):
+    """The plan's masks, read back: every edge appears once, in its row's order, with its column;
+    tiles with many edges, long rows and parallel edges are cut within the limits."""
+    cases = [([5] * 40, 30, True), ([0] * 17, 5, True), ([1500, 3, 0, 40], 2000, True),
+             ([200] * 33, 220, True), ([1100] * 2 + [7] * 20, 9, False), ([3] * 100, 2, False)]
+    for seed, (degrees, m, distinct) in enumerate(cases):
+        src, row_ptr = _edges(degrees, m, 90 + seed, distinct)
+        n, e = len(degrees), len(src)
+        order = torch.randperm(n, generator=gen(95))
+        plan, items, parts, bad = bm.attention_plan(torch.from_numpy(row_ptr).to(dev),
+                                                    torch.from_numpy(src).to(dev), order.to(dev), m,
+                                                    True)
+        assert bad == 0
+        p = plan.cpu().numpy()
+        tiles = -(-n // 16)
+        max_items = tiles + e // 512 + e // 256
+        pad = lambda k: (k + 15) // 16 * 16
+        at = 16 + pad(tiles * 16) + 3 * pad(tiles + 1)
+        items_at, at = at, at + pad(max_items * 64)
+        masks_at, at = at, at + pad((e // 32 + max_items) * 16)
+        seen, of_tile = np.zeros(e, int), np.zeros(tiles, int)
+        for i in range(items):
+            rec = p[items_at + 64 * i:items_at + 64 * i + 64]
+            tile, chunk, cols, part = rec[:4]
+            of_tile[tile] += 1
+            edge, count = rec[32:48].copy(), np.zeros(16, int)
+            for c in range(-(-cols // 32)):
+                for r in range(16):
+                    mask = int(p[masks_at + (chunk + c) * 16 + r]) & 0xffffffff
+                    for bit in range(32):
+                        if mask >> bit & 1:
+                            row = int(order[tile * 16 + r])
+                            assert rec[16 + r] == row
+                            assert row_ptr[row] <= edge[r] < row_ptr[row + 1]
+                            assert 32 * c + bit < cols
+                            assert p[at + (chunk + c) * 32 + bit] == src[edge[r]]
+                            seen[edge[r]] += 1
+                            edge[r] += 1
+                            count[r] += 1
+            assert (count == rec[48:64]).all()
+        assert (seen == 1).all() and (of_tile >= 1).all()
+        assert parts == of_tile[of_tile > 1].sum()
+
+
+def test_plan_refuses_an_order_that_is_no_permutation(dev):
+    import batmobile
+    src, row_ptr = _edges([3] * 5, 6, 99)
+    args = [torch.from_numpy(x).to(dev) for x in (src, row_ptr)]
+    with pytest.raises(ValueError, match="permutation"):
+        batmobile.AttentionPlan(*args, 6, torch.tensor([0, 1, 2, 3, 3], device=dev))
+    with pytest.raises(ValueError, match="permutation"):
+        batmobile.AttentionPlan(*args, 6, None, torch.tensor([0, 1, 2, 3, 4, 9], device=dev))
+
+
+def test_memory_of_a_captured_pass(dev):
+    """Forward and backward recorded into a HIP graph and replayed three times with new inputs,
+    eager work between the replays: the eager bits."""
+    import batmobile
+    pos, cell = periodic_box(300, 101)
+    plan = batmobile.Graph(pos.to(dev), cell, 5.0, 8).attention_plan()
+    plan.source_side()
+    e = plan.src.numel()
+    s = {x: v.to(dev) for x, v in _inputs(300, 300, e, 4, 2, 64, 64, "f32", 102).items()}
+    leaf = [s[x].requires_grad_(True) for x in ("q", "k", "v", "bias")]
+
+    def step():
+        out = batmobile.neighbor_attention(*leaf[:3], plan, bias=leaf[3])
+        return [out] + list(torch.autograd.grad(out, leaf, s["go"]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for k in range(3):
+        with torch.no_grad():
+            leaf[0].copy_(torch.randn(300, 4, 64, generator=gen(103 + k)).to(dev))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, step()):
+            assert torch.equal(a, b)
