@@ -356,42 +356,42 @@ std::tuple<Tensor, Tensor, Tensor> gated_residual_norm(const Tensor& x_, const O
 
 // (gx, gy, ggate, gscale, gw_post, gw_pre)
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> gated_residual_norm_backward(
-    const OptTensor& gh_, const OptTensor& gn_, const Tensor& h_, const OptTensor& y_,
+    const OptTensor& gh_, const OptTensor& gn_, const Tensor& x_, const OptTensor& y_,
     const OptTensor& gate_, const OptTensor& scale_, const OptTensor& w_post_,
     const OptTensor& w_pre_, const Tensor& rs) {
-    const int dt = dtype_of(h_, "h");
-    check_features(h_, "h");
-    const int64_t N = h_.size(0);
-    const int C = (int)h_.size(1);
+    const int dt = dtype_of(x_, "x");
+    check_features(x_, "x");
+    const int64_t N = x_.size(0);
+    const int C = (int)x_.size(1);
     TORCH_CHECK(y_ || w_pre_, "one of y and weight_pre is needed");
     TORCH_CHECK(!w_pre_ || gn_, "weight_pre needs the gradient of n");
     TORCH_CHECK(w_pre_ || gh_, "the gradient of h is needed");
-    check_f32(rs, h_, "rs");
+    check_f32(rs, x_, "rs");
     TORCH_CHECK(rs.is_contiguous() && rs.numel() == N * 8, "rs must be [N, 8]");
-    const c10::DeviceGuard guard(h_.device());
-    const Tensor h = rows4(h_);
+    const c10::DeviceGuard guard(x_.device());
+    const Tensor x = rows4(x_);
     Tensor gh, gn, y, gate, scale, w_post, w_pre, gx, gy, ggate, gscale, gw_post, gw_pre;
-    gx = torch::empty_like(h);
-    if (gh_) check_same(*gh_, h_, "grad_h"), gh = rows4(*gh_);
+    gx = torch::empty_like(x);
+    if (gh_) check_same(*gh_, x_, "grad_h"), gh = rows4(*gh_);
     if (w_pre_) {
-        check_same(*gn_, h_, "grad_n");
+        check_same(*gn_, x_, "grad_n");
         gn = rows4(*gn_);
-        w_pre = weight4(*w_pre_, h_, "weight_pre");
+        w_pre = weight4(*w_pre_, x_, "weight_pre");
         gw_pre = torch::empty_like(w_pre);
     }
     if (y_) {
         TORCH_CHECK(scale_ && w_post_, "y needs scale and weight_post");
-        check_same(*y_, h_, "y");
+        check_same(*y_, x_, "y");
         y = rows4(*y_);
-        check_f32(*scale_, h_, "scale");
+        check_f32(*scale_, x_, "scale");
         TORCH_CHECK(scale_->numel() == C, "scale must be [C]");
         scale = scale_->contiguous();
-        w_post = weight4(*w_post_, h_, "weight_post");
+        w_post = weight4(*w_post_, x_, "weight_post");
         gy = torch::empty_like(y);
         gscale = torch::empty_like(scale);
         gw_post = torch::empty_like(w_post);
         if (gate_) {
-            check_like(*gate_, h_, "gate");
+            check_like(*gate_, x_, "gate");
             TORCH_CHECK(gate_->numel() == N * C * 4, "gate must be [N, C, 4]");
             gate = gate_->contiguous();
             ggate = torch::empty_like(gate);
@@ -403,13 +403,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> gated_residual_norm_b
         return {gx, gy, ggate, gscale, gw_post, gw_pre};
     }
     const size_t wsb = batteries_gated_residual_norm_backward_workspace_bytes(N, C);
-    const Tensor ws = bytes_on(h, wsb);
+    const Tensor ws = bytes_on(x, wsb);
     check_status(batteries_gated_residual_norm_backward(
-                     opt_ptr(gh), opt_ptr(gn), h.data_ptr(), opt_ptr(y), opt_ptr(gate),
+                     opt_ptr(gh), opt_ptr(gn), x.data_ptr(), opt_ptr(y), opt_ptr(gate),
                      opt_f32(scale), opt_f32(w_post), opt_f32(w_pre), rs.data_ptr<float>(),
                      gx.data_ptr(), opt_ptr(gy), opt_ptr(ggate), opt_f32(gscale),
                      opt_f32(gw_post), opt_f32(gw_pre), N, C, dt, ws.data_ptr(), wsb,
-                     stream_of(h)),
+                     stream_of(x)),
                  "gated_residual_norm_backward");
     return {gx, gy, ggate, gscale, gw_post, gw_pre};
 }
@@ -493,7 +493,7 @@ void register_block_ops(pybind11::module_& m) {
           py::arg("eps"), py::arg("keep_stats") = false,
           "h = x + scale sigmoid(gate) norm(y), n = norm(h) -> (h, n, rs); y None: n = norm(x)");
     m.def("gated_residual_norm_backward", &gated_residual_norm_backward, py::arg("grad_h"),
-          py::arg("grad_n"), py::arg("h"), py::arg("y"), py::arg("gate"), py::arg("scale"),
+          py::arg("grad_n"), py::arg("x"), py::arg("y"), py::arg("gate"), py::arg("scale"),
           py::arg("weight_post"), py::arg("weight_pre"), py::arg("rs"),
           "(grad_x, grad_y, grad_gate, grad_scale, grad_weight_post, grad_weight_pre)");
     m.def("clip_grad_norm", &clip_grad_norm, py::arg("grads"), py::arg("max_norm"),

@@ -7,7 +7,8 @@
 //   n = norm(h; w_pre)
 //
 // which commutes with rotations: the factors are the same for all components of a degree.
-// Backward, with gh and gn the gradients of h and n, M_l = C (2 l + 1), f = scale sigmoid(gate):
+// Backward, with gh and gn the gradients of h and n, M_l = C (2 l + 1), f = scale sigmoid(gate),
+// h formed again from x and y:
 //
 //   V[c, l] = sum_m gn h                     gw_pre[l, c] = sum over atoms of r_l(h) V
 //   G = gh + r w_pre gn - h r^3 / M sum_c w_pre V          (gx = G)
@@ -118,7 +119,7 @@ __device__ __forceinline__ float row_sum(float v, float* sh, int& turn) {
 }
 
 struct NormArgs {
-    const void *x, *y, *gate, *gh, *gn, *h;
+    const void *x, *y, *gate, *gh, *gn;
     const float *scale, *w_post, *w_pre, *rs_in;
     void *out_h, *out_n, *gx, *gy, *ggate;
     float *rs, *part;                  // rs [N, 8]: 1/rms of y by degree, then of h
@@ -218,7 +219,7 @@ __global__ __launch_bounds__(W <= 4 ? 256 : 64 * W) void norm_bwd_kernel(NormArg
     // the next row's loads are under way while this one's sums are formed; lanes past C read the
     // row's last channel and drop it
     struct Row {
-        Raw4<T> gh[NV], h[NV], gn[NV], y[NV];
+        Raw4<T> gh[NV], x[NV], gn[NV], y[NV];
         float sg[NV], r_pre, r_post;
     };
     auto load = [&](Row& x, int64_t row0) {
@@ -228,7 +229,7 @@ __global__ __launch_bounds__(W <= 4 ? 256 : 64 * W) void norm_bwd_kernel(NormArg
         for (int i = 0; i < NV; ++i) {
             const int e = min(i * 64 * W + t, a.C * 4 - 4 + q);
             if constexpr (PRE) {
-                x.h[i].load((const T*)a.h + at + e * 4);
+                x.x[i].load((const T*)a.x + at + e * 4);
                 x.gn[i].load((const T*)a.gn + at + e * 4);
             }
             if (a.gh) x.gh[i].load((const T*)a.gh + at + e * 4);
@@ -257,14 +258,32 @@ __global__ __launch_bounds__(W <= 4 ? 256 : 64 * W) void norm_bwd_kernel(NormArg
             }
         if (row0 + step < a.n) load(next, row0 + step);
         float4 G[NV];
+        float f[NV], sg[NV];
+        if constexpr (BLOCK) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = min((i * 64 * W + t) >> 2, a.C - 1);
+                sg[i] = GATE ? __builtin_amdgcn_rcpf(1.0f + __expf(-x.sg[i])) : 1.0f;
+                f[i] = a.scale[c] * sg[i] * a.w_post[q * a.C + c];
+            }
+        }
         if constexpr (PRE) {
             const float r = x.r_pre;
             float s = 0.0f, wp[NV];
+            // h as the forward had it before rounding: gw_pre is fp32 whatever the features' type
+            float4 h[NV];
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = (i * 64 * W + t) >> 2;
+                h[i] = x.x[i].get();
+                if constexpr (BLOCK) {
+                    const float fa = first_of(f[i] * x.r_post), fb = others_of(f[i] * x.r_post);
+                    const float4 yi = x.y[i].get();
+                    h[i] = make_float4(fmaf(fa, yi.x, h[i].x), fmaf(fb, yi.y, h[i].y),
+                                       fmaf(fb, yi.z, h[i].z), fmaf(fb, yi.w, h[i].w));
+                }
                 wp[i] = a.w_pre[q * a.C + min(c, a.C - 1)];
-                const float v = dot4(x.gn[i].get(), x.h[i].get(), q);   // 0 past C
+                const float v = dot4(x.gn[i].get(), h[i], q);       // 0 past C
                 aw_pre[i] = fmaf(r, v, aw_pre[i]);
                 s = fmaf(wp[i], v, s);
             }
@@ -273,11 +292,11 @@ __global__ __launch_bounds__(W <= 4 ? 256 : 64 * W) void norm_bwd_kernel(NormArg
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const float fa = first_of(wp[i] * r), fb = others_of(wp[i] * r);
-                const float4 gni = x.gn[i].get(), hi = x.h[i].get(), ghi = x.gh[i].get();
-                G[i] = make_float4(ghi.x + fmaf(fa, gni.x, ka * hi.x),
-                                   ghi.y + fmaf(fb, gni.y, kb * hi.y),
-                                   ghi.z + fmaf(fb, gni.z, kb * hi.z),
-                                   ghi.w + fmaf(fb, gni.w, kb * hi.w));
+                const float4 gni = x.gn[i].get(), ghi = x.gh[i].get();
+                G[i] = make_float4(ghi.x + fmaf(fa, gni.x, ka * h[i].x),
+                                   ghi.y + fmaf(fb, gni.y, kb * h[i].y),
+                                   ghi.z + fmaf(fb, gni.z, kb * h[i].z),
+                                   ghi.w + fmaf(fb, gni.w, kb * h[i].w));
             }
         } else {
 #pragma unroll
@@ -289,21 +308,19 @@ __global__ __launch_bounds__(W <= 4 ? 256 : 64 * W) void norm_bwd_kernel(NormArg
                 norm_st4((T*)a.gx + at + (int64_t)(i * 64 * W + t) * 4, G[i]);
         if constexpr (BLOCK) {
             const float r = x.r_post;
-            float s = 0.0f, f[NV];
+            float s = 0.0f;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = (i * 64 * W + t) >> 2;
-                const float g = GATE ? __builtin_amdgcn_rcpf(1.0f + __expf(-x.sg[i])) : 1.0f;
                 const float sc = a.scale[min(c, a.C - 1)], w = a.w_post[q * a.C + min(c, a.C - 1)];
-                const float z = dot4(G[i], x.y[i].get(), q), rz = r * z;   // 0 past C
-                f[i] = sc * g * w;
+                const float z = dot4(G[i], x.y[i].get(), q), rz = r * z;    // 0 past C
                 s = fmaf(f[i], z, s);
-                aw_post[i] = fmaf(sc * g, rz, aw_post[i]);
-                a_scale[i] = fmaf(g * w, rz, a_scale[i]);
+                aw_post[i] = fmaf(sc * sg[i], rz, aw_post[i]);
+                a_scale[i] = fmaf(sg[i] * w, rz, a_scale[i]);
                 if constexpr (GATE)
                     if (there && c < a.C)
                         norm_st((T*)a.ggate + row * a.C * 4 + i * 64 * W + t,
-                                f[i] * (1.0f - g) * rz);
+                                f[i] * (1.0f - sg[i]) * rz);
             }
             const float k = -row_sum<W>(s, sh, turn) * cnt * r * r * r;
             const float ka = first_of(k), kb = others_of(k);
@@ -452,19 +469,19 @@ extern "C" size_t batteries_gated_residual_norm_backward_workspace_bytes(int64_t
 }
 
 extern "C" int batteries_gated_residual_norm_backward(
-    const void* gh, const void* gn, const void* h, const void* y, const void* gate,
+    const void* gh, const void* gn, const void* x, const void* y, const void* gate,
     const float* scale, const float* w_post, const float* w_pre, const float* rs, void* gx,
     void* gy, void* ggate, float* gscale, float* gw_post, float* gw_pre, int64_t N, int C,
     int dtype, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     if (!norm_shape_ok(N, C, dtype) || (!y && !w_pre) || !gx ||
         (y && (!scale || !w_post || !gy || !gscale || !gw_post)) || (gate && !ggate) ||
-        (w_pre && (!gn || !h || !gw_pre)) || (!w_pre && !gh))
+        (w_pre && (!gn || !x || !gw_pre)) || (!w_pre && !gh))
         return BM_ERR_ARG;
-    if (!aligned_to({gh, gn, h, y, gx, gy}, dtype == 0 ? 16 : 8)) return BM_ERR_ARG;
+    if (!aligned_to({gh, gn, x, y, gx, gy}, dtype == 0 ? 16 : 8)) return BM_ERR_ARG;
     const size_t need = batteries_gated_residual_norm_backward_workspace_bytes(N, C);
     if (workspace_bytes < need || (need && !workspace)) return BM_ERR_WORKSPACE;
     NormArgs a{};
-    a.gh = gh; a.gn = gn; a.h = h; a.y = y; a.gate = gate; a.scale = scale; a.w_post = w_post;
+    a.gh = gh; a.gn = gn; a.x = x; a.y = y; a.gate = gate; a.scale = scale; a.w_post = w_post;
     a.w_pre = w_pre; a.rs_in = rs; a.gx = gx; a.gy = gy; a.ggate = ggate;
     a.part = (float*)workspace; a.n = N; a.C = C;
     if (N > 0) {

@@ -18,7 +18,7 @@ class GatedResidualNormFunction(torch.autograd.Function):
         train = any(ctx.needs_input_grad[:6])
         h, n, rs = _batmobile.gated_residual_norm(x, y, gate, scale, weight_post, weight_pre,
                                                   eps, train)
-        ctx.save_for_backward(x if y is None else h, y, gate, scale, weight_post, weight_pre, rs)
+        ctx.save_for_backward(x, y, gate, scale, weight_post, weight_pre, rs)
         ctx.set_materialize_grads(False)
         if y is None:
             return n
@@ -26,7 +26,7 @@ class GatedResidualNormFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
-        h, y, gate, scale, weight_post, weight_pre, rs = ctx.saved_tensors
+        x, y, gate, scale, weight_post, weight_pre, rs = ctx.saved_tensors
         if all(g is None for g in grads):
             return (None,) * 7
         gh = None if y is None else grads[0]
@@ -36,7 +36,7 @@ class GatedResidualNormFunction(torch.autograd.Function):
         else:
             weight_pre_used, gw_zero = weight_pre, False
         gx, gy, gg, gs, gpost, gpre = _batmobile.gated_residual_norm_backward(
-            gh, gn, h, y, gate, scale, weight_post, weight_pre_used, rs)
+            gh, gn, x, y, gate, scale, weight_post, weight_pre_used, rs)
         if gw_zero:
             gpre = torch.zeros_like(weight_pre)
         return gx, gy, gg, gs, gpost, gpre, None

@@ -567,10 +567,10 @@ int batteries_gated_residual_norm(const void* x, const void* y, const void* gate
                                   const float* scale, const float* w_post, const float* w_pre,
                                   void* h, void* n, float* rs, int64_t N, int C, float eps,
                                   int dtype, hipStream_t stream);
-/* Gradients from gh (NULL: zero) and gn; h is the forward's h (x where y was NULL). */
+/* Gradients from gh (NULL: zero) and gn (NULL without w_pre); h is formed again from x and y. */
 size_t batteries_gated_residual_norm_backward_workspace_bytes(int64_t N, int C);
 int batteries_gated_residual_norm_backward(
-    const void* gh, const void* gn, const void* h, const void* y, const void* gate,
+    const void* gh, const void* gn, const void* x, const void* y, const void* gate,
     const float* scale, const float* w_post, const float* w_pre, const float* rs, void* gx,
     void* gy, void* ggate, float* gscale, float* gw_post, float* gw_pre, int64_t N, int C,
     int dtype, void* workspace, size_t workspace_bytes, hipStream_t stream);
