@@ -370,6 +370,67 @@ __global__ __launch_bounds__(256) void attn_edges_kernel(const float* __restrict
     if (TO_HEADS) cols(); else rows();
 }
 
+// Heads of any size and strides <-> dense rows of heads padded with zeros to whole 16-byte pieces,
+// up to four matrices a launch (blockIdx.y).  Packing: a thread a piece; cutting: an element.
+struct AttnPacks {
+    batmobile_attention_pack m[4];
+};
+
+template <typename T, bool CUT>
+__global__ __launch_bounds__(256) void attn_pack_kernel(AttnPacks all) {
+    constexpr int kE = 16 / (int)sizeof(T);
+    const batmobile_attention_pack& a = all.m[blockIdx.y];
+    const uint32_t Dp = (uint32_t)(a.D + kE - 1) / kE * kE;
+    const int64_t step = (int64_t)gridDim.x * 256, i0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (CUT) {
+        const T* in = (const T*)a.in;
+        T* out = (T*)a.out;
+        const int64_t n = a.rows * a.heads * a.D;
+        for (int64_t i = i0; i < n; i += step) {
+            const int64_t rh = i / a.D;
+            out[i] = in[rh * Dp + (i - rh * a.D)];
+        }
+        return;
+    }
+    const uint32_t pieces = Dp / kE;
+    const int64_t n = a.rows * a.heads * pieces;
+    for (int64_t i = i0; i < n; i += step) {
+        const int64_t rh = i / pieces;
+        const int d0 = (int)(i - rh * pieces) * kE;
+        const int64_t row = rh / a.heads, head = rh - row * a.heads;
+        const T* in = (const T*)a.in + row * a.row_stride + head * a.head_stride;
+        T v[kE];
+#pragma unroll
+        for (int k = 0; k < kE; ++k) v[k] = d0 + k < a.D ? in[(d0 + k) * a.step] : (T)0;
+        v4u w;
+        __builtin_memcpy(&w, v, 16);
+        *reinterpret_cast<v4u*>((T*)a.out + i * kE) = w;
+    }
+}
+
+extern "C" int batteries_attention_pack(const batmobile_attention_pack* packs, int count,
+                                        int dtype, int cut, hipStream_t stream) {
+    if (count < 0 || count > 4 || (count > 0 && !packs) || (dtype != 0 && dtype != 1))
+        return BM_ERR_ARG;
+    AttnPacks all{};
+    int64_t most = 0;
+    for (int i = 0; i < count; ++i) {
+        const batmobile_attention_pack& p = packs[i];
+        if (p.rows < 0 || p.heads <= 0 || p.D <= 0 || p.D > 256 ||
+            (p.rows > 0 && (!p.in || !p.out)) || (!cut && !aligned_to({p.out}, 16)))
+            return BM_ERR_ARG;
+        all.m[i] = p;
+        most = std::max(most, p.rows * p.heads * (cut ? p.D : ceil_div(p.D * (dtype ? 2 : 4), 16)));
+    }
+    if (most == 0) return BM_OK;
+    const dim3 grid((unsigned)std::min<int64_t>(ceil_div(most, 256), 4096), (unsigned)count);
+    if (dtype == 0 && cut) attn_pack_kernel<float, true><<<grid, 256, 0, stream>>>(all);
+    else if (dtype == 0) attn_pack_kernel<float, false><<<grid, 256, 0, stream>>>(all);
+    else if (cut) attn_pack_kernel<uint16_t, true><<<grid, 256, 0, stream>>>(all);
+    else attn_pack_kernel<uint16_t, false><<<grid, 256, 0, stream>>>(all);
+    return (int)hipGetLastError();
+}
+
 extern "C" int batteries_attention_edges_by_head(const float* values, const int32_t* edge_id,
                                                  float* out, int64_t n_edges, int H, int back,
                                                  hipStream_t stream) {

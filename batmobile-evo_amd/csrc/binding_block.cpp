@@ -59,20 +59,41 @@ Tensor bytes_on(const Tensor& as, size_t n) {
 // attention
 // ---------------------------------------------------------------------------
 
-// [n, heads, D] as the kernels read it: heads of a row dense, rows at any stride, everything in
-// units of 16 bytes.  Other layouts are copied; a head size that is no multiple of 16 bytes is
-// padded with zeros, which add nothing to a product.
-Tensor heads16(const Tensor& t) {
-    const int64_t unit = 16 / t.element_size(), D = t.size(2);
-    if (D % unit) return at::constant_pad_nd(t, {0, unit - D % unit}).contiguous();
-    const bool dense = t.stride(2) == 1 && (t.size(1) == 1 || t.stride(1) == D) &&
-                       (t.size(0) <= 1 || (t.stride(0) >= t.size(1) * D && t.stride(0) % unit == 0)) &&
-                       (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
-    if (dense) return t;
-    const Tensor c = t.contiguous();
-    return reinterpret_cast<uintptr_t>(c.data_ptr()) & 15 ? c.clone(at::MemoryFormat::Contiguous)
-                                                          : c;
-}
+// Matrices [n, heads, D] as the kernels read them: heads of a row dense, rows at any stride,
+// everything in units of 16 bytes.  Others are packed (head sizes padded with zeros, which add
+// nothing to a product), all in one launch.
+class Packer {
+public:
+    Tensor add(const Tensor& t) {
+        const int64_t unit = 16 / t.element_size(), D = t.size(2);
+        const bool dense = t.stride(2) == 1 && (t.size(1) == 1 || t.stride(1) == D) &&
+                           (t.size(0) <= 1 ||
+                            (t.stride(0) >= t.size(1) * D && t.stride(0) % unit == 0)) &&
+                           (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+        if (D % unit == 0 && (dense || t.numel() == 0)) return t.numel() ? t : t.contiguous();
+        Tensor out = torch::empty({t.size(0), t.size(1), (D + unit - 1) / unit * unit}, t.options());
+        packs_[count_++] = {t.data_ptr(), out.data_ptr(), t.size(0), t.stride(0), t.stride(1),
+                            t.stride(2), (int32_t)t.size(1), (int32_t)D};
+        return out;
+    }
+    // padded results cut to D
+    Tensor cut(const Tensor& t, int64_t D) {
+        if (t.size(2) == D) return t;
+        Tensor out = torch::empty({t.size(0), t.size(1), D}, t.options());
+        packs_[count_++] = {t.data_ptr(), out.data_ptr(), t.size(0), 0, 0, 0, (int32_t)t.size(1),
+                            (int32_t)D};
+        return out;
+    }
+    void run(int dtype, bool cut, const Tensor& as, const char* what) {
+        if (count_)
+            check_status(batteries_attention_pack(packs_, count_, dtype, cut, stream_of(as)), what);
+        count_ = 0;
+    }
+
+private:
+    batmobile_attention_pack packs_[4];
+    int count_ = 0;
+};
 int64_t row_stride(const Tensor& t) {
     return t.size(0) <= 1 ? t.size(1) * t.size(2) : t.stride(0);
 }
@@ -81,10 +102,6 @@ Tensor heads_like(const Tensor& as, int64_t n, int64_t heads, int64_t D) {
     const int64_t unit = 16 / as.element_size();
     return torch::empty({n, heads, (D + unit - 1) / unit * unit}, as.options());
 }
-Tensor cut_heads(const Tensor& t, int64_t D) {
-    return t.size(2) == D ? t : t.slice(2, 0, D).contiguous();
-}
-
 // A side of a plan: (plan, items, parts) as attention_plan returns them.
 batmobile_attention_side attn_side(const Tensor& plan, int64_t items, int64_t parts, int64_t rows,
                                    int64_t cols, int64_t edges, const Tensor& as) {
@@ -194,7 +211,9 @@ std::tuple<Tensor, Tensor, Tensor> neighbor_attention(const Tensor& q_, const Te
     const c10::DeviceGuard guard(q_.device());
     const batmobile_attention_side side = attn_side(plan, items, parts, s.n_dst, s.n_src, E, q_);
     const int32_t* eid = opt_index32(edge_id, q_, E, "edge_id");
-    const Tensor q = heads16(q_), k = heads16(k_), v = heads16(v_);
+    Packer packer;
+    const Tensor q = packer.add(q_), k = packer.add(k_), v = packer.add(v_);
+    packer.run(s.dtype, false, q, "neighbor_attention");
     Tensor bias, by_head;
     if (bias_) bias = bias_->contiguous();
     if (bias.defined() && (reinterpret_cast<uintptr_t>(bias.data_ptr()) & 15))
@@ -221,7 +240,9 @@ std::tuple<Tensor, Tensor, Tensor> neighbor_attention(const Tensor& q_, const Te
                      s.Hkv, Dk, Dv, row_stride(q), row_stride(k), row_stride(v), (float)scale,
                      s.dtype, wsb ? ws.data_ptr() : nullptr, wsb, stream_of(q)),
                  "neighbor_attention");
-    return {cut_heads(out, s.Dv), stats, keep_stats ? by_head : Tensor()};
+    const Tensor result = packer.cut(out, s.Dv);
+    packer.run(s.dtype, true, q, "neighbor_attention");
+    return {result, stats, keep_stats ? by_head : Tensor()};
 }
 
 // by_head: the forward's, in place of the bias.  src_*: the side of the sources, src_place the
@@ -247,7 +268,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> neighbor_attention_backward(
     const int32_t* eid = opt_index32(edge_id, q_, E, "edge_id");
     const int32_t* pos = opt_index32(src_place, q_, E, "src_place");
     const int64_t* rp = index_ptr(row_ptr, q_, s.n_dst + 1, "row_ptr");
-    const Tensor q = heads16(q_), k = heads16(k_), v = heads16(v_), go = heads16(grad_);
+    Packer packer;
+    const Tensor q = packer.add(q_), k = packer.add(k_), v = packer.add(v_), go = packer.add(grad_);
+    packer.run(s.dtype, false, q, "neighbor_attention_backward");
     Tensor bias, gbias;
     if (bias_) bias = bias_->contiguous();
     if (by_head) {
@@ -275,7 +298,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> neighbor_attention_backward(
             row_stride(q), row_stride(k), row_stride(v), row_stride(go), (float)scale, s.dtype,
             ws.data_ptr(), wsb, stream_of(q)),
         "neighbor_attention_backward");
-    return {cut_heads(gq, s.Dk), cut_heads(gk, s.Dk), cut_heads(gv, s.Dv), gbias};
+    const Tensor rq = packer.cut(gq, s.Dk), rk = packer.cut(gk, s.Dk), rv = packer.cut(gv, s.Dv);
+    packer.run(s.dtype, true, q, "neighbor_attention_backward");
+    return {rq, rk, rv, gbias};
 }
 
 // ---------------------------------------------------------------------------

@@ -513,6 +513,18 @@ int batteries_attention_plan(const int64_t* row_ptr, const int64_t* col, const i
                              int64_t n_rows, int64_t n_cols, int64_t n_edges, int check,
                              void* plan, size_t plan_bytes, hipStream_t stream);
 
+/* Up to four matrices [rows, heads, D] at any strides (elements) to dense rows of heads padded with
+ * zeros to whole 16-byte units (out 16-byte aligned), or with `cut` dense padded ones to dense
+ * [rows, heads, D] (strides unused).  packs is a host array; D <= 256. */
+typedef struct batmobile_attention_pack {
+    const void* in;
+    void* out;
+    int64_t rows, row_stride, head_stride, step;
+    int32_t heads, D;
+} batmobile_attention_pack;
+int batteries_attention_pack(const batmobile_attention_pack* packs, int count, int dtype, int cut,
+                             hipStream_t stream);
+
 /* out [H, E] of values [E, H] (row edge_id e of edge e; edge_id NULL: e), or with `back`
  * out [E, H] of values [H, E]. */
 int batteries_attention_edges_by_head(const float* values, const int32_t* edge_id, float* out,
