@@ -37,15 +37,24 @@ struct PlanLayout {
     int64_t rows, tile_item, tile_chunk, tile_part, items, masks, ids, total;
 };
 
-// A tile of more than kTileEdges edges is cut into items of kCutEdges or more, one with a row of
-// more than kTileRow into items with kCutRow or more of that row.  An item that is a whole tile
-// so has at most kTileEdges, which is what the kernels keep of its edges in LDS.
-constexpr int kTileEdges = 1024, kCutEdges = 512, kTileRow = 512, kCutRow = 256;
+// A tile of more than kTileEdges edges, or with a row of more than kTileRow, is cut into items of
+// plan_cut edges or more, along its columns; their results are joined by a second kernel.  An item
+// so has at most kTileEdges edges (but for many edges between the same two), which is what the
+// kernels keep of them in LDS: twice that costs the training steps 3 to 14 % (its LDS).  Items of
+// 64 edges serve a graph too small to fill the card (one row of 1000 edges, 64 bf16 components:
+// 9.4 us against 14.5 with 256 edges and 22.0 uncut), but a large one pays for their number (100
+// rows of 500, 8 heads of 256 in bf16: 111 us with 256 edges, 92 with 512).
+constexpr int kTileEdges = 1024, kTileRow = 512;
+
+__host__ __device__ inline int64_t plan_cut(int64_t n_edges) {
+    const int64_t c = n_edges / 128;
+    return c < 64 ? 64 : c > 512 ? 512 : c;
+}
 
 inline PlanLayout plan_layout(int64_t n_rows, int64_t n_edges) {
     PlanLayout p;
     p.tiles = ceil_div(n_rows, kAttnRows);
-    p.max_items = p.tiles + n_edges / kCutEdges + n_edges / kCutRow;
+    p.max_items = p.tiles + n_edges / plan_cut(n_edges);
     p.max_chunks = n_edges / kAttnCols + p.max_items;
     int64_t at = kPlanHead;
     auto take = [&](int64_t n) {

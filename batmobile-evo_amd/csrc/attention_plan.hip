@@ -39,8 +39,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_tiles_kernel(PlanArgs a) {
         edges += len;
         longest = max(longest, len);
     }
-    const int64_t cuts = max(longest > kTileRow ? longest / kCutRow : (int64_t)1,
-                             edges > kTileEdges ? edges / kCutEdges : (int64_t)1);
+    const int64_t cuts = longest > kTileRow || edges > kTileEdges
+                             ? max(edges / plan_cut(a.n_edges), (int64_t)1)
+                             : 1;
     a.plan[a.at.tile_item + t] = (int)cuts;
     a.plan[a.at.tile_chunk + t] = (int)(edges / kAttnCols + cuts);
     a.plan[a.at.tile_part + t] = cuts > 1 ? (int)cuts : 0;

@@ -123,7 +123,7 @@ struct NormArgs {
     const float *scale, *w_post, *w_pre, *rs_in;
     void *out_h, *out_n, *gx, *gy, *ggate;
     float *rs, *part;                  // rs [N, 8]: 1/rms of y by degree, then of h
-    int64_t n;
+    int64_t n, row0;                   // rows; the launch's first
     int C;
     float eps;
 };
@@ -133,7 +133,8 @@ template <typename T, int NV, int W, bool BLOCK, bool GATE, bool PRE>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_fwd_kernel(NormArgs a) {
     __shared__ float sh[2 * 4 * 16];
     int turn = 0;
-    const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    const int64_t row =
+        a.row0 + (W == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x);
     if (row >= a.n) return;
     const int t = W == 1 ? (threadIdx.x & 63) : threadIdx.x, q = t & 3;
     const int64_t at = row * (int64_t)a.C * 16;
@@ -243,12 +244,14 @@ __global__ __launch_bounds__(W <= 4 ? 256 : 64 * W) void norm_bwd_kernel(NormArg
         if constexpr (BLOCK) x.r_post = a.rs_in[row * 8 + q];
     };
     const int64_t step = (int64_t)gridDim.x * kRows;
+    constexpr bool kAhead = W < 16;      // 16 waves have 128 registers each, too few for two rows
     Row next;
-    load(next, (int64_t)blockIdx.x * kRows);
+    if constexpr (kAhead) load(next, (int64_t)blockIdx.x * kRows);
     for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < a.n; row0 += step) {
         const bool there = row0 + group < a.n;
         const int64_t row = there ? row0 + group : a.n - 1;
         const int64_t at = row * (int64_t)a.C * 16;
+        if constexpr (!kAhead) load(next, row0);
         Row x = next;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -256,7 +259,7 @@ __global__ __launch_bounds__(W <= 4 ? 256 : 64 * W) void norm_bwd_kernel(NormArg
                 if constexpr (PRE) x.gn[i].zero();
                 if constexpr (BLOCK) x.y[i].zero();
             }
-        if (row0 + step < a.n) load(next, row0 + step);
+        if (kAhead && row0 + step < a.n) load(next, row0 + step);
         float4 G[NV];
         float f[NV], sg[NV];
         if constexpr (BLOCK) {
@@ -398,8 +401,12 @@ static int norm_bwd_blocks(int64_t n, int C) {
 
 template <typename T, int NV, int W, bool BLOCK, bool GATE, bool PRE>
 static void norm_fwd_launch(const NormArgs& a, hipStream_t s) {
-    norm_fwd_kernel<T, NV, W, BLOCK, GATE, PRE>
-        <<<(unsigned)(W == 1 ? ceil_div(a.n, 4) : a.n), W == 1 ? 256 : 64 * W, 0, s>>>(a);
+    constexpr int kRows = W == 1 ? 4 : 1, kThreads = W == 1 ? 256 : 64 * W;
+    constexpr int64_t kMost = (int64_t)1 << 20;     // workgroups of a launch (threads < 2^32)
+    NormArgs b = a;
+    for (b.row0 = 0; b.row0 < a.n; b.row0 += kMost * kRows)
+        norm_fwd_kernel<T, NV, W, BLOCK, GATE, PRE>
+            <<<(unsigned)std::min(ceil_div(a.n - b.row0, kRows), kMost), kThreads, 0, s>>>(b);
 }
 template <typename T, int NV, int W, bool BLOCK, bool GATE, bool PRE>
 static void norm_bwd_launch(const NormArgs& a, hipStream_t s) {
@@ -407,25 +414,28 @@ static void norm_bwd_launch(const NormArgs& a, hipStream_t s) {
         <<<norm_bwd_blocks(a.n, a.C), W <= 4 ? 256 : 64 * W, 0, s>>>(a);
 }
 
+template <typename T, int NV, int W, bool BLOCK, bool GATE, bool PRE>
+static void norm_launch(const NormArgs& a, bool bwd, hipStream_t s) {
+    if (bwd) norm_bwd_launch<T, NV, W, BLOCK, GATE, PRE>(a, s);
+    else norm_fwd_launch<T, NV, W, BLOCK, GATE, PRE>(a, s);
+}
+
+// Lanes of a row for its channels: four loads of each array a lane, and waves by the channels.
+// Eight loads a lane with fewer waves, at 6.4 M channels in us (four loads): gated block forward
+// bf16 128 channels 200 (162), 192: 284 (171), 512: 203 (169); f32 128 channels 327 (316); the
+// gain is occupancy.  One and two loads with more waves: bf16 128 channels 188 and 162, 100
+// channels (lanes idle) 233 and 193 (180); f32 within 6 %.  Past 1024 channels a workgroup has
+// no more waves.
 template <typename T, bool BLOCK, bool GATE, bool PRE>
 static void norm_pick(const NormArgs& a, bool bwd, hipStream_t s) {
-    if (bwd) {
-        if (a.C <= 16) norm_bwd_launch<T, 1, 1, BLOCK, GATE, PRE>(a, s);
-        else if (a.C <= 32) norm_bwd_launch<T, 2, 1, BLOCK, GATE, PRE>(a, s);
-        else if (a.C <= 64) norm_bwd_launch<T, 4, 1, BLOCK, GATE, PRE>(a, s);
-        else if (a.C <= 128) norm_bwd_launch<T, 4, 2, BLOCK, GATE, PRE>(a, s);
-        else if (a.C <= 256) norm_bwd_launch<T, 4, 4, BLOCK, GATE, PRE>(a, s);
-        else if (a.C <= 512) norm_bwd_launch<T, 8, 4, BLOCK, GATE, PRE>(a, s);
-        else if (a.C <= 1024) norm_bwd_launch<T, 4, 16, BLOCK, GATE, PRE>(a, s);
-        else norm_bwd_launch<T, 8, 16, BLOCK, GATE, PRE>(a, s);
-        return;
-    }
-    if (a.C <= 16) norm_fwd_launch<T, 1, 1, BLOCK, GATE, PRE>(a, s);
-    else if (a.C <= 32) norm_fwd_launch<T, 2, 1, BLOCK, GATE, PRE>(a, s);
-    else if (a.C <= 64) norm_fwd_launch<T, 4, 1, BLOCK, GATE, PRE>(a, s);
-    else if (a.C <= 128) norm_fwd_launch<T, 8, 1, BLOCK, GATE, PRE>(a, s);
-    else if (a.C <= 512) norm_fwd_launch<T, 8, 4, BLOCK, GATE, PRE>(a, s);
-    else norm_fwd_launch<T, 8, 16, BLOCK, GATE, PRE>(a, s);
+    if (a.C <= 16) norm_launch<T, 1, 1, BLOCK, GATE, PRE>(a, bwd, s);
+    else if (a.C <= 32) norm_launch<T, 2, 1, BLOCK, GATE, PRE>(a, bwd, s);
+    else if (a.C <= 64) norm_launch<T, 4, 1, BLOCK, GATE, PRE>(a, bwd, s);
+    else if (a.C <= 128) norm_launch<T, 4, 2, BLOCK, GATE, PRE>(a, bwd, s);
+    else if (a.C <= 256) norm_launch<T, 4, 4, BLOCK, GATE, PRE>(a, bwd, s);
+    else if (a.C <= 512) norm_launch<T, 4, 8, BLOCK, GATE, PRE>(a, bwd, s);
+    else if (a.C <= 1024) norm_launch<T, 4, 16, BLOCK, GATE, PRE>(a, bwd, s);
+    else norm_launch<T, 8, 16, BLOCK, GATE, PRE>(a, bwd, s);
 }
 
 template <typename T>
@@ -475,7 +485,8 @@ extern "C" int batteries_gated_residual_norm_backward(
     int dtype, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     if (!norm_shape_ok(N, C, dtype) || (!y && !w_pre) || !gx ||
         (y && (!scale || !w_post || !gy || !gscale || !gw_post)) || (gate && !ggate) ||
-        (w_pre && (!gn || !x || !gw_pre)) || (!w_pre && !gh))
+        (w_pre && (!gn || !x || !gw_pre)) || (!w_pre && !gh) ||
+        (N > 0 && !rs))
         return BM_ERR_ARG;
     if (!aligned_to({gh, gn, x, y, gx, gy}, dtype == 0 ? 16 : 8)) return BM_ERR_ARG;
     const size_t need = batteries_gated_residual_norm_backward_workspace_bytes(N, C);

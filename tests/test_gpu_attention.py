@@ -422,7 +422,7 @@ def test_plan_covers_every_edge_once(bm, dev):
         assert bad == 0
         p = plan.cpu().numpy()
         tiles = -(-n // 16)
-        max_items = tiles + e // 512 + e // 256
+        max_items = tiles + e // min(max(e // 128, 64), 512)
         pad = lambda k: (k + 15) // 16 * 16
         at = 16 + pad(tiles * 16) + 3 * pad(tiles + 1)
         items_at, at = at, at + pad(max_items * 64)
