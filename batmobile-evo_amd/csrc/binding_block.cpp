@@ -179,8 +179,11 @@ AttnShape attn_shape(const Tensor& q, const Tensor& k, const Tensor& v, const Op
 
 // Edges x heads from which the bias (and its gradient) is brought to [H, E] by a kernel of its
 // own: a wave takes one head of a tile, whose values lie H apart in [E, H], so every head reads
-// (writes) all cache lines of the array.  The extra launch pays from about here on.
-constexpr int64_t kByHead = 1 << 18;
+// (writes) all cache lines of the array, which shows once the array leaves the L2s.  A training
+// step, heads of 32 in f32, as it lies and by head: 20,000 rows of 28, 2 heads 60 and 66 us, 4
+// heads 96 and 98, 8 heads 191 and 170, 16 heads 517 and 354; 5000 rows, 8 heads 62 and 66, 16
+// heads 104 and 102.
+constexpr int64_t kByHead = 1 << 21;
 
 // values [E, H] -> [H, E] in the order of edge_id, or back
 Tensor attention_edges_by_head(const Tensor& values, const OptTensor& edge_id, bool back) {
