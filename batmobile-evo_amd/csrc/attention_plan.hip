@@ -10,6 +10,9 @@
 // A tile with many edges or a long row is cut at column values into items of equal edge counts,
 // each found by searching for its first column.  A cut with more edges than the LDS holds (one
 // column thousands of times) is taken unmerged.
+//
+// Once per graph: 5000 atoms with 28 neighbours take 55 us (35 of them plan_items, whose sort is
+// steps of LDS latency and barriers), 50,000 atoms 150 us.
 #include "attention.h"
 
 namespace bmhip {
