@@ -51,6 +51,8 @@ __host__ __device__ inline int64_t plan_cut(int64_t n_edges) {
     return c < 64 ? 64 : c > 512 ? 512 : c;
 }
 
+constexpr int64_t kPlanRows = ((int64_t)1 << 26) - 64;    // 64 threads a row, < 2^32 a launch
+
 inline PlanLayout plan_layout(int64_t n_rows, int64_t n_edges) {
     PlanLayout p;
     p.tiles = ceil_div(n_rows, kAttnRows);
@@ -618,9 +620,10 @@ inline bool attn_shape_ok(const batmobile_attention_side& s, int H, int Hkv, int
     return s.n_rows >= 0 && s.n_cols >= 0 && s.n_edges >= 0 && (s.n_rows == 0 || s.plan) &&
            s.n_items >= 0 && s.n_parts >= 0 && H > 0 && H <= 65535 && Hkv > 0 && H % Hkv == 0 &&
            Dk > 0 && Dv > 0 && Dk <= 256 && Dv <= 256 && (dtype == 0 || dtype == 1) &&
-           (s.n_edges == 0 || s.n_cols > 0) && s.n_rows < INT32_MAX / 2 &&
+           (s.n_edges == 0 || s.n_cols > 0) && s.n_rows < kPlanRows &&
            s.n_edges < INT32_MAX / 4 &&
-           ((int64_t)s.n_items + 8) * H < (int64_t)1 << 26;     // a launch has < 2^32 threads
+           // the three sums are one launch, of fewer than 2^32 threads
+           3 * ((int64_t)s.n_items + 8) * H < (int64_t)1 << 26;
 }
 
 inline bool attn_strides_ok(std::initializer_list<int64_t> strides) {

@@ -84,8 +84,8 @@ __device__ __forceinline__ void attn_fwd_rows(const AttnFwd& a, int item, int h,
 //                                                          time, 31 % for memory
 //   50,000, 8 heads of 256, bf16       353 us   2.5 TB/s   1.17 GB from HBM and Infinity Cache
 //   5000, random, 4 heads of 24 by 256 106 us   6.3 TB/s   of rows from Infinity Cache
-// Rows loaded straight to registers in row form took 79 us at the first size: 16 lanes ask for 16
-// cache lines.
+// Rows of k loaded straight to registers in row form, where 16 lanes ask for 16 cache lines, made an
+// earlier form take 79 us at the first size instead of 65.
 // Two waves a SIMD at least unless the tiles of k and v in f32 need more registers than that
 // leaves: 20,000 atoms, 8 heads of 256 in bf16 100 us against 122 without the bound, 5000 in f32
 // 66 us with it against 64.
@@ -481,6 +481,7 @@ extern "C" int batteries_neighbor_attention(const void* q, const void* k, const 
         !attn_strides_ok({q_stride, k_stride, v_stride}) || !aligned_to({q, k, v, out}, 16))
         return BM_ERR_ARG;
     if (side->n_rows == 0) return BM_OK;
+    if (!out || (side->n_edges > 0 && (!q || !k || !v))) return BM_ERR_ARG;
     const size_t need = batteries_neighbor_attention_workspace_bytes(side->n_parts, H, Dv);
     if (workspace_bytes < need || (need && !workspace)) return BM_ERR_WORKSPACE;
     AttnFwd a{};

@@ -508,6 +508,9 @@ extern "C" int batteries_neighbor_attention_backward(
         !aligned_to({q, k, v, grad_out, grad_q, grad_k, grad_v, workspace}, 16))
         return BM_ERR_ARG;
     const int64_t E = dst->n_edges, size = dtype == 0 ? 4 : 2;
+    if ((dst->n_rows > 0 && !grad_q) || (src->n_rows > 0 && (!grad_k || !grad_v)) ||
+        (E > 0 && (!q || !k || !v || !stats || !grad_out || !row_ptr || !src_place)))
+        return BM_ERR_ARG;
     const size_t need = batteries_neighbor_attention_backward_workspace_bytes(
         E, dst->n_parts, src->n_parts, H, Hkv, Dk, Dv);
     if (workspace_bytes < need || (need && !workspace)) return BM_ERR_WORKSPACE;

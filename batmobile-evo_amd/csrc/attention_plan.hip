@@ -313,7 +313,7 @@ __global__ void plan_head_kernel(int* plan) {
 using namespace bmhip;
 
 static bool plan_shape_ok(int64_t n_rows, int64_t n_cols, int64_t n_edges) {
-    return n_rows >= 0 && n_cols >= 0 && n_edges >= 0 && n_rows < INT32_MAX / 2 &&
+    return n_rows >= 0 && n_cols >= 0 && n_edges >= 0 && n_rows < kPlanRows &&
            n_cols < INT32_MAX && n_edges < INT32_MAX / 4 && (n_edges == 0 || n_cols > 0);
 }
 

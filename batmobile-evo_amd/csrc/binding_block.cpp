@@ -136,7 +136,7 @@ std::tuple<Tensor, int64_t, int64_t, int64_t> attention_plan(const Tensor& row_p
     const int64_t* op = order ? index_ptr(*order, row_ptr, rows, "order") : nullptr;
     const c10::DeviceGuard guard(row_ptr.device());
     const size_t n = batteries_attention_plan_bytes(rows, edges);
-    TORCH_CHECK(n > 0 && n_cols >= 0, "attention_plan: up to 2^29 edges and 2^30 rows");
+    TORCH_CHECK(n > 0 && n_cols >= 0, "attention_plan: up to 2^29 edges and 2^26 rows");
     Tensor plan = torch::empty({(int64_t)(n / 4)}, row_ptr.options().dtype(torch::kInt32));
     check_status(batteries_attention_plan(rp, cp, op, rows, n_cols, edges, check, plan.data_ptr(),
                                           n, stream_of(row_ptr)),
@@ -252,7 +252,8 @@ std::tuple<Tensor, Tensor, Tensor> neighbor_attention(const Tensor& q_, const Te
 // place of every edge in its order.
 std::tuple<Tensor, Tensor, Tensor, Tensor> neighbor_attention_backward(
     const Tensor& q_, const Tensor& k_, const Tensor& v_, const OptTensor& bias_,
-    const OptTensor& by_head, const Tensor& stats, const Tensor& grad_, const Tensor& row_ptr, const Tensor& plan,
+    const OptTensor& by_head, const Tensor& stats, const Tensor& grad_, const Tensor& row_ptr,
+    const Tensor& plan,
     int64_t items, int64_t parts, const OptTensor& edge_id, const Tensor& src_plan,
     int64_t src_items, int64_t src_parts, const Tensor& src_place, double scale, bool need_bias) {
     const int64_t E = src_place.numel();
@@ -296,7 +297,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> neighbor_attention_backward(
         batteries_neighbor_attention_backward(
             q.data_ptr(), k.data_ptr(), v.data_ptr(),
             bias.defined() ? bias.data_ptr<float>() : nullptr, stats.data_ptr<float>(),
-            go.data_ptr(), rp, eid, by_head.has_value(), &dst, &src, pos, gq.data_ptr(), gk.data_ptr(), gv.data_ptr(),
+            go.data_ptr(), rp, eid, by_head.has_value(), &dst, &src, pos, gq.data_ptr(),
+            gk.data_ptr(), gv.data_ptr(),
             gbias.defined() ? gbias.data_ptr<float>() : nullptr, s.H, s.Hkv, Dk, Dv,
             row_stride(q), row_stride(k), row_stride(v), row_stride(go), (float)scale, s.dtype,
             ws.data_ptr(), wsb, stream_of(q)),

@@ -85,10 +85,11 @@ class AttentionPlan:
                 output_size=self.src.numel())
             by, pos = torch.sort(self.src, stable=True)
             rows = torch.arange(self.n_src + 1, device=self.src.device)
-            plan, items, parts, _ = _batmobile.attention_plan(
-                torch.searchsorted(by, rows), dst[pos], self._src_order, self.n_dst, False)
             place = torch.empty_like(pos, dtype=torch.int32)
             place[pos] = torch.arange(pos.numel(), dtype=torch.int32, device=pos.device)
+            # last: it waits for the stream, so that any stream may use the result from here on
+            plan, items, parts, _ = _batmobile.attention_plan(
+                torch.searchsorted(by, rows), dst[pos], self._src_order, self.n_dst, False)
             self._source_side = (plan, items, parts, place)
         return self._source_side
 

@@ -500,7 +500,7 @@ int batteries_mace_backward(const float* positions, const float* box, const floa
  * aligned).  Its first ints are the number of items, the number of parts (items of cut tiles)
  * and, with check, 0 or what is wrong with the arrays (1 row_ptr, 2 a column out of range, 4
  * columns not ascending); the caller reads them back into the side's n_items and n_parts.
- * n_edges < 2^29.
+ * n_edges < 2^29, n_rows < 2^26 - 64.
  * ------------------------------------------------------------------------- */
 typedef struct batmobile_attention_side {
     int64_t n_rows, n_cols, n_edges;
@@ -536,8 +536,9 @@ int batteries_attention_edges_by_head(const float* values, const int32_t* edge_i
  * q [n_dst, H, Dk], k [n_src, Hkv, Dk], v [n_src, Hkv, Dv], out [n_dst, H, Dv] in fp32
  * (dtype 0) or bf16 (dtype 1), rows at strides (in elements), bias [E, H] fp32 or NULL,
  * edge_id [E] or NULL (the edges' own order), or with bias_by_head [H, E] in the edges' order
- * (then read contiguously; batteries_attention_edges_by_head makes it).  Dk, Dv <= 256; pointers 16-byte aligned, Dk, Dv
- * and strides multiples of 16 bytes.  An edge whose bias or logit is -inf is left out; a row
+ * (then read contiguously; batteries_attention_edges_by_head makes it).  Dk, Dv <= 256; pointers
+ * 16-byte aligned, Dk, Dv and strides multiples of 16 bytes, strides < 2^30; 3 H (n_items + 8) <
+ * 2^26 on either side.  An edge whose bias or logit is -inf is left out; a row
  * without an edge gives 0.  stats [n_dst, H, 2] (NULL: not kept): the maximum of x and the sum
  * of exp(x - max), which the backward recomputes the probabilities from. */
 size_t batteries_neighbor_attention_workspace_bytes(int64_t n_parts, int H, int Dv);

@@ -135,3 +135,37 @@ def test_python_refusals(bm):
     with pytest.raises(ValueError, match="edge_index"):
         batmobile.AttentionPlan.from_edge_index(torch.zeros(3, 2, dtype=torch.long), 4)
     assert float(batmobile.clip_grad_norm_([torch.zeros(3)], 1.0)) == 0.0
+
+
+def test_c_refusals_of_sizes_and_missing_arrays():
+    """Launches of 2^32 threads or more, and arrays that are needed and missing, are refused on
+    the host."""
+    lib = ctypes.CDLL(os.path.join(REPO, "batmobile-evo_amd", "lib", "libbatmobile_hip.so"))
+    i64, ptr, i32 = ctypes.c_int64, ctypes.c_void_p, ctypes.c_int
+    p = ctypes.c_void_p(256)            # never dereferenced: the checks come first
+    size = lib.batteries_attention_plan_bytes
+    size.restype, size.argtypes = ctypes.c_size_t, [i64, i64]
+    assert size((1 << 26) - 65, 0) > 0 and size((1 << 26) - 64, 0) == 0
+    assert size(10, 1 << 29) == 0
+
+    class Side(ctypes.Structure):
+        _fields_ = [("n_rows", i64), ("n_cols", i64), ("n_edges", i64), ("plan", ptr),
+                    ("n_items", ctypes.c_int32), ("n_parts", ctypes.c_int32)]
+
+    f = lib.batteries_neighbor_attention
+    f.argtypes = [ptr] * 5 + [i32, ctypes.POINTER(Side), ptr, ptr] + [i32] * 4 + [i64] * 3 + \
+        [ctypes.c_float, i32, ptr, ctypes.c_size_t, ptr]
+    side = Side(1 << 20, 1 << 20, 1 << 20, 256, 1 << 16, 0)
+    assert f(p, p, p, None, None, 0, side, p, None, 512, 512, 8, 8, 4096, 4096, 4096, 1.0, 0, None,
+             0, None) == -1             # 2^25 waves, and the backward's sums three times as many
+    assert f(p, p, p, None, None, 0, side, None, None, 8, 8, 8, 8, 64, 64, 64, 1.0, 0, None, 0,
+             None) == -1
+    assert f(None, p, p, None, None, 0, side, p, None, 8, 8, 8, 8, 64, 64, 64, 1.0, 0, None, 0,
+             None) == -1
+    back = lib.batteries_gated_residual_norm_backward
+    back.argtypes = [ptr] * 15 + [i64, i32, i32, ptr, ctypes.c_size_t, ptr]
+    args = [None, p, p, None, None, None, None, p, None, p, None, None, None, None, p]
+    assert back(*args, 5, 8, 0, p, 1 << 30, None) == -1        # rs
+    pack = lib.batteries_attention_pack
+    pack.argtypes = [ptr, i32, i32, i32, ptr]
+    assert pack(None, 1, 0, 0, None) == -1 and pack(p, 5, 0, 0, None) == -1
