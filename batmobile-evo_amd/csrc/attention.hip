@@ -453,7 +453,7 @@ extern "C" int batteries_attention_edges_by_head(const float* values, const int3
                                                  float* out, int64_t n_edges, int H, int back,
                                                  hipStream_t stream) {
     if (n_edges < 0 || H <= 0 || H > 65535 || n_edges >= INT32_MAX / 4 ||
-        !aligned_to({values, out}, 16))
+        !aligned_to({values, out}, 16) || (n_edges > 0 && (!values || !out)))
         return BM_ERR_ARG;
     if (n_edges == 0) return BM_OK;
     const dim3 grid((unsigned)ceil_div(n_edges, 256), (unsigned)ceil_div(H, 16));

@@ -326,7 +326,9 @@ extern "C" int batteries_attention_plan(const int64_t* row_ptr, const int64_t* c
                                         const int64_t* order, int64_t n_rows, int64_t n_cols,
                                         int64_t n_edges, int check, void* plan, size_t plan_bytes,
                                         hipStream_t stream) {
-    if (!plan_shape_ok(n_rows, n_cols, n_edges)) return BM_ERR_ARG;
+    if (!plan_shape_ok(n_rows, n_cols, n_edges) || (n_rows > 0 && !row_ptr) ||
+        (n_edges > 0 && !col))
+        return BM_ERR_ARG;
     if (!plan || (reinterpret_cast<uintptr_t>(plan) & 63) ||
         plan_bytes < batteries_attention_plan_bytes(n_rows, n_edges))
         return BM_ERR_WORKSPACE;

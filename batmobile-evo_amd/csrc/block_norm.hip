@@ -468,7 +468,7 @@ extern "C" int batteries_gated_residual_norm(const void* x, const void* y, const
                                              int64_t N, int C, float eps, int dtype,
                                              hipStream_t stream) {
     if (!norm_shape_ok(N, C, dtype) || (!y && !w_pre) || (y && (!scale || !w_post || !h)) ||
-        (w_pre && !n))
+        (w_pre && !n) || (N > 0 && !x))
         return BM_ERR_ARG;
     if (!aligned_to({x, y, h, n}, dtype == 0 ? 16 : 8)) return BM_ERR_ARG;
     if (N == 0) return BM_OK;

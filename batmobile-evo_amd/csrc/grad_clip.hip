@@ -161,7 +161,9 @@ extern "C" int batteries_clip_grad_norm(const void* const* in, void* const* out,
                                         const int64_t* numel, const int* dtype, int64_t n_tensors,
                                         float max_norm, float* norm, void* workspace,
                                         size_t workspace_bytes, hipStream_t stream) {
-    if (n_tensors < 0 || !norm || !(max_norm >= 0.0f)) return BM_ERR_ARG;
+    if (n_tensors < 0 || !norm || !(max_norm >= 0.0f) ||
+        (n_tensors > 0 && (!in || !out || !numel || !dtype)))
+        return BM_ERR_ARG;
     int64_t elements = 0;
     for (int64_t i = 0; i < n_tensors; ++i) {
         if (numel[i] < 0 || numel[i] > (int64_t)1 << 40 || (dtype[i] != 0 && dtype[i] != 1) ||

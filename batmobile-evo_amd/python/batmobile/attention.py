@@ -14,6 +14,7 @@ are the same from run to run.
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 import _batmobile
 
@@ -47,13 +48,14 @@ class AttentionPlan:
         self.edge_id = None if edge_id is None else edge_id.int()
         self._src_order, self._source_side = src_order, None
         if validate:
-            for name, t, n in (("order", order, self.n_dst), ("src_order", src_order, self.n_src)):
+            for name, t, n in (("order", order, self.n_dst), ("src_order", src_order, self.n_src),
+                               ("edge_id", edge_id, src.numel())):
                 if t is not None and not torch.equal(t.sort()[0],
                                                      torch.arange(n, device=t.device)):
                     raise ValueError(f"AttentionPlan: {name} must be a permutation")
         plan, items, parts, bad = _batmobile.attention_plan(row_ptr, src, order, self.n_src,
                                                             validate)
-        if bad & 1:
+        if bad & 1 or (self.n_dst == 0 and src.numel()):
             raise ValueError("AttentionPlan: row_ptr must rise from 0 to the number of edges")
         if bad & 2:
             raise ValueError(f"AttentionPlan: src must lie in [0, {self.n_src})")
@@ -74,7 +76,9 @@ class AttentionPlan:
         edge_id = torch.argsort(dst * n_src + src, stable=True)
         rows = torch.arange(n_dst + 1, device=dst.device)
         row_ptr = torch.searchsorted(dst[edge_id], rows)
-        return cls(src[edge_id], row_ptr, n_src, order, src_order, edge_id)
+        plan = cls(src[edge_id], row_ptr, n_src, order, src_order)
+        plan.edge_id = edge_id.int()       # a permutation as it comes, so not checked
+        return plan
 
     def source_side(self):
         """The edges grouped by source, for the backward (built on first use): the side's plan
@@ -108,6 +112,7 @@ class NeighborAttentionFunction(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out):
         q, k, v, bias, by_head, stats = ctx.saved_tensors
         plan = ctx.plan
@@ -123,7 +128,8 @@ def neighbor_attention(q, k, v, plan, bias=None, scale=None):
     q [n_dst, H, Dk], k [n_src, H_kv, Dk], v [n_src, H_kv, Dv] in float32 or bfloat16 (sums and
     softmax in float32), H a multiple of H_kv, Dk and Dv up to 256; rows may be strided (slices
     of one projection).  bias [E, H] float32: an edge with -inf is left out.  A row without an
-    edge gives zeros.  scale defaults to 1 / sqrt(Dk).  Gradients for q, k, v and bias.
+    edge gives zeros.  scale defaults to 1 / sqrt(Dk).  Gradients for q, k, v and bias,
+    which cannot be differentiated again (an error, not a missing term).
     """
     if q.dim() == 3 and (q.shape[0] != plan.n_dst or k.shape[0] != plan.n_src):
         raise RuntimeError(f"neighbor_attention: the plan has {plan.n_dst} destinations and "

@@ -8,6 +8,7 @@ every degree l of an atom is divided by its root mean square over channels and c
 float32 or bfloat16 features, float32 weights and sums, one pass over the data each way.
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 import _batmobile
 
@@ -25,6 +26,7 @@ class GatedResidualNormFunction(torch.autograd.Function):
         return h if n is None else (h, n)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grads):
         x, y, gate, scale, weight_post, weight_pre, rs = ctx.saved_tensors
         if all(g is None for g in grads):
@@ -54,6 +56,6 @@ def gated_residual_norm(x, y, gate, scale, weight_post, weight_pre=None, eps=1e-
 
     x (residual), y (the block's output) [N, C, 16], gate [N, C, 4] (None: no gate), scale [C],
     weights [4, C].  Returns (h, n), or h where weight_pre is None (after the last block).
-    Gradients for every tensor.
+    Gradients for every tensor, which cannot be differentiated again (an error).
     """
     return GatedResidualNormFunction.apply(x, y, gate, scale, weight_post, weight_pre, float(eps))

@@ -493,3 +493,34 @@ def test_memory_of_a_captured_pass(dev):
         torch.cuda.synchronize()
         for a, b in zip(held, step()):
             assert torch.equal(a, b)
+
+
+def test_plan_refuses_an_edge_id_that_is_no_permutation(dev):
+    """edge_id places the rows of the bias and of its gradient: a number past the edges would be
+    an access past them."""
+    import batmobile
+    src, row_ptr = _edges([3] * 5, 6, 110)
+    s, r = [torch.from_numpy(x).to(dev) for x in (src, row_ptr)]
+    ids = torch.arange(15, device=dev)
+    for at, to in ((0, 15), (0, -1), (0, 1)):
+        bad = ids.clone()
+        bad[at] = to
+        with pytest.raises(ValueError, match="permutation"):
+            batmobile.AttentionPlan(s, r, 6, edge_id=bad)
+    with pytest.raises(ValueError, match="permutation"):
+        batmobile.AttentionPlan(s, r, 6, edge_id=ids[:-1])
+    assert batmobile.AttentionPlan(s, r, 6, edge_id=ids.flip(0)).edge_id.dtype == torch.int32
+    with pytest.raises(ValueError, match="row_ptr"):
+        batmobile.AttentionPlan(s, r[:1], 6)             # edges without a row
+
+
+def test_second_derivative_is_refused(dev):
+    import batmobile
+    src, row_ptr = _edges([3] * 5, 6, 111)
+    plan = batmobile.AttentionPlan(torch.from_numpy(src).to(dev), torch.from_numpy(row_ptr).to(dev), 6)
+    q = torch.randn(5, 2, 8, generator=gen(112)).to(dev).requires_grad_(True)
+    k = torch.randn(6, 2, 8, generator=gen(113)).to(dev)
+    out = batmobile.neighbor_attention(q, k, k, plan)
+    grad, = torch.autograd.grad(out.square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        grad.sum().backward()

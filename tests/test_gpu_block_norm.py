@@ -304,3 +304,12 @@ def test_clip_refusals(dev):
         batmobile.clip_grad_norm([a], 1.0, [torch.ones(5, device=dev)])
     with pytest.raises(RuntimeError, match="type"):
         batmobile.clip_grad_norm([a], 1.0, [a.bfloat16()])
+
+
+def test_second_derivative_is_refused(dev):
+    import batmobile
+    x = torch.randn(3, 8, 16, generator=gen(90)).to(dev).requires_grad_(True)
+    n = batmobile.equivariant_norm(x, torch.ones(4, 8, device=dev))
+    grad, = torch.autograd.grad(n.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        grad.sum().backward()

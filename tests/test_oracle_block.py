@@ -169,3 +169,25 @@ def test_c_refusals_of_sizes_and_missing_arrays():
     pack = lib.batteries_attention_pack
     pack.argtypes = [ptr, i32, i32, i32, ptr]
     assert pack(None, 1, 0, 0, None) == -1 and pack(p, 5, 0, 0, None) == -1
+
+
+def test_c_refusals_of_missing_arrays_of_plans_norms_and_clipping():
+    lib = ctypes.CDLL(os.path.join(REPO, "batmobile-evo_amd", "lib", "libbatmobile_hip.so"))
+    i64, ptr, i32, f32 = ctypes.c_int64, ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+    size = ctypes.c_size_t
+    p = ctypes.c_void_p(256)            # never dereferenced: the checks come first
+    plan = lib.batteries_attention_plan
+    plan.argtypes = [ptr] * 3 + [i64] * 3 + [i32, ptr, size, ptr]
+    assert plan(None, p, None, 5, 5, 9, 1, p, 1 << 30, None) == -1
+    assert plan(p, None, None, 5, 5, 9, 1, p, 1 << 30, None) == -1
+    by_head = lib.batteries_attention_edges_by_head
+    by_head.argtypes = [ptr] * 3 + [i64, i32, i32, ptr]
+    assert by_head(None, None, p, 5, 2, 0, None) == -1 and by_head(p, None, None, 5, 2, 0, None) == -1
+    norm = lib.batteries_gated_residual_norm
+    norm.argtypes = [ptr] * 9 + [i64, i32, f32, i32, ptr]
+    assert norm(None, None, None, None, None, p, None, p, None, 5, 8, 1e-6, 0, None) == -1
+    clip = lib.batteries_clip_grad_norm
+    clip.argtypes = [ptr] * 4 + [i64, f32, ptr, ptr, size, ptr]
+    for at in range(4):
+        arrays = [None if i == at else p for i in range(4)]
+        assert clip(*arrays, 1, 1.0, p, p, 1 << 30, None) == -1
