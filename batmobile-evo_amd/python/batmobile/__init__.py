@@ -63,9 +63,8 @@ from _batteries import (  # noqa: E402
 )
 from .graph import Graph  # noqa: E402
 from .mace import MACEInteraction, MaceLayerFunction  # noqa: E402
-from .attention import AttentionPlan, NeighborAttentionFunction, neighbor_attention  # noqa: E402
-from .block_norm import (  # noqa: E402
-    GatedResidualNormFunction, equivariant_norm, gated_residual_norm)
+from .attention import AttentionPlan, neighbor_attention  # noqa: E402
+from .block_norm import equivariant_norm, gated_residual_norm  # noqa: E402
 from .grad_clip import clip_grad_norm, clip_grad_norm_  # noqa: E402
 from .attention_block import AttentionBlock  # noqa: E402
 
@@ -120,9 +119,7 @@ __all__ = [
     "MACEInteraction",
     "MaceLayerFunction",
     "AttentionPlan",
-    "NeighborAttentionFunction",
     "neighbor_attention",
-    "GatedResidualNormFunction",
     "equivariant_norm",
     "gated_residual_norm",
     "clip_grad_norm",

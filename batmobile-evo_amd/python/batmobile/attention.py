@@ -14,7 +14,6 @@ are the same from run to run.
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 import _batmobile
 
@@ -81,8 +80,8 @@ class AttentionPlan:
         return plan
 
     def source_side(self):
-        """The edges grouped by source, for the backward (built on first use): the side's plan
-        and the place of every edge in its order."""
+        """The edges grouped by source, for the backward (built when gradients are first wanted):
+        the side's plan and the place of every edge in its order."""
         if self._source_side is None:
             dst = torch.repeat_interleave(
                 torch.arange(self.n_dst, device=self.src.device), self.row_ptr.diff(),
@@ -98,30 +97,6 @@ class AttentionPlan:
         return self._source_side
 
 
-class NeighborAttentionFunction(torch.autograd.Function):
-    """out = attention(q, k, v, bias); the backward recomputes the probabilities."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, bias, plan, scale):
-        train = any(ctx.needs_input_grad[:4])
-        out, stats, by_head = _batmobile.neighbor_attention(
-            q, k, v, bias, *plan.side, plan.src.numel(), plan.edge_id, scale, train)
-        # a bias brought to [H, E] takes the place of the caller's
-        ctx.save_for_backward(q, k, v, None if by_head is not None else bias, by_head, stats)
-        ctx.plan, ctx.scale = plan, scale
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_out):
-        q, k, v, bias, by_head, stats = ctx.saved_tensors
-        plan = ctx.plan
-        gq, gk, gv, gb = _batmobile.neighbor_attention_backward(
-            q, k, v, bias, by_head, stats, grad_out, plan.row_ptr, *plan.side, plan.edge_id,
-            *plan.source_side(), ctx.scale, ctx.needs_input_grad[3])
-        return gq, gk, gv, gb, None, None
-
-
 def neighbor_attention(q, k, v, plan, bias=None, scale=None):
     """Attention of each destination over its edges: out [n_dst, H, Dv].
 
@@ -135,4 +110,6 @@ def neighbor_attention(q, k, v, plan, bias=None, scale=None):
         raise RuntimeError(f"neighbor_attention: the plan has {plan.n_dst} destinations and "
                            f"{plan.n_src} sources")
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
-    return NeighborAttentionFunction.apply(q, k, v, bias, plan, scale)
+    return _batmobile.neighbor_attention_autograd(q, k, v, bias, *plan.side, plan.src.numel(),
+                                                  plan.edge_id, plan.row_ptr, plan.source_side,
+                                                  scale)
