@@ -32,7 +32,7 @@ class AttentionPlan:
     """
 
     def __init__(self, src, row_ptr, n_src=None, order=None, src_order=None, edge_id=None,
-                 validate=True):
+                 validate=True, _sorted_here=False):
         for name, t in (("src", src), ("row_ptr", row_ptr), ("order", order),
                         ("src_order", src_order), ("edge_id", edge_id)):
             if t is None and name not in ("src", "row_ptr"):
@@ -48,10 +48,11 @@ class AttentionPlan:
         self._src_order, self._source_side = src_order, None
         if validate:
             for name, t, n in (("order", order, self.n_dst), ("src_order", src_order, self.n_src),
-                               ("edge_id", edge_id, src.numel())):
+                               ("edge_id", None if _sorted_here else edge_id, src.numel())):
                 if t is not None and not torch.equal(t.sort()[0],
                                                      torch.arange(n, device=t.device)):
                     raise ValueError(f"AttentionPlan: {name} must be a permutation")
+        # last: it waits for the stream, so that any stream may use the plan from here on
         plan, items, parts, bad = _batmobile.attention_plan(row_ptr, src, order, self.n_src,
                                                             validate)
         if bad & 1 or (self.n_dst == 0 and src.numel()):
@@ -75,9 +76,8 @@ class AttentionPlan:
         edge_id = torch.argsort(dst * n_src + src, stable=True)
         rows = torch.arange(n_dst + 1, device=dst.device)
         row_ptr = torch.searchsorted(dst[edge_id], rows)
-        plan = cls(src[edge_id], row_ptr, n_src, order, src_order)
-        plan.edge_id = edge_id.int()       # a permutation as it comes, so not checked
-        return plan
+        # (argsort's edge_id is a permutation as it comes, so not checked)
+        return cls(src[edge_id], row_ptr, n_src, order, src_order, edge_id, _sorted_here=True)
 
     def source_side(self):
         """The edges grouped by source, for the backward (built when gradients are first wanted):

@@ -524,3 +524,26 @@ def test_second_derivative_is_refused(dev):
     grad, = torch.autograd.grad(out.square().sum(), q, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         grad.sum().backward()
+
+
+def test_plan_made_on_one_stream_and_used_on_another(dev):
+    """A plan from edges in any order, made on a stream of its own; the bias and its gradient go
+    by its edge_id, forward and backward, on the current stream without a wait between."""
+    import batmobile
+    n, m, e, h = 300, 200, 9000, 2
+    g = gen(120)
+    ei = torch.stack([torch.randint(0, m, (e,), generator=g), torch.randint(0, n, (e,), generator=g)])
+    t = {x: None if v is None else v.to(dev) for x, v in
+         _inputs(n, m, e, h, h, 16, 16, "f32", 121).items()}
+    want, wg = _run(dev, batmobile.AttentionPlan.from_edge_index(ei.to(dev), n, m), t)
+    for _ in range(3):
+        stream = torch.cuda.Stream()
+        edges = ei.to(dev)
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            plan = batmobile.AttentionPlan.from_edge_index(edges, n, m)
+        out, grads = _run(dev, plan, t)
+        assert torch.equal(out, want)
+        for name in grads:
+            assert torch.equal(grads[name], wg[name]), name
+        torch.cuda.synchronize()
