@@ -481,7 +481,7 @@ extern "C" int batteries_neighbor_attention(const void* q, const void* k, const 
         !attn_strides_ok({q_stride, k_stride, v_stride}) || !aligned_to({q, k, v, out}, 16))
         return BM_ERR_ARG;
     if (side->n_rows == 0) return BM_OK;
-    if (!out || (side->n_edges > 0 && (!q || !k || !v))) return BM_ERR_ARG;
+    if (!q || !out || (side->n_edges > 0 && (!k || !v))) return BM_ERR_ARG;
     const size_t need = batteries_neighbor_attention_workspace_bytes(side->n_parts, H, Dv);
     if (workspace_bytes < need || (need && !workspace)) return BM_ERR_WORKSPACE;
     AttnFwd a{};

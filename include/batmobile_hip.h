@@ -538,9 +538,9 @@ int batteries_attention_edges_by_head(const float* values, const int32_t* edge_i
  * edge_id [E] or NULL (the edges' own order), or with bias_by_head [H, E] in the edges' order
  * (then read contiguously; batteries_attention_edges_by_head makes it).  Dk, Dv <= 256; pointers
  * 16-byte aligned, Dk, Dv and strides multiples of 16 bytes, strides < 2^30; 3 H (n_items + 8) <
- * 2^26 on either side.  An edge whose bias or logit is -inf is left out; a row
- * without an edge gives 0.  stats [n_dst, H, 2] (NULL: not kept): the maximum of x and the sum
- * of exp(x - max), which the backward recomputes the probabilities from. */
+ * 2^26 on either side.  Rows need q and out, edges k and v as well (others may be NULL).  An edge
+ * whose bias or logit is -inf is left out; a row without an edge gives 0.  stats [n_dst, H, 2]
+ * (NULL: not kept): the maximum of x and the sum of exp(x - max), which the backward recomputes the probabilities from. */
 size_t batteries_neighbor_attention_workspace_bytes(int64_t n_parts, int H, int Dv);
 int batteries_neighbor_attention(const void* q, const void* k, const void* v, const float* bias,
                                  const int32_t* edge_id, int bias_by_head,

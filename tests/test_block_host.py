@@ -1,10 +1,14 @@
 """Attention, norms and clipping without a GPU: what is refused on the host before anything runs,
 and the order of work around a plan's wait."""
+import ctypes
+import os
 import types
 
 import pytest
 import torch
 from torch.utils._python_dispatch import TorchDispatchMode
+
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 class _Ops(TorchDispatchMode):
@@ -50,3 +54,39 @@ def test_a_plan_is_complete_when_its_constructor_returns(plan_wait):
         AttentionPlan(plan.src, plan.row_ptr, 3, edge_id=torch.arange(5).flip(0))
         assert log.names[waits[-1]:] == []
     assert len(waits) == 3
+
+
+# ---------------------------------------------------------------------------
+# C entries: refused before anything is launched (the addresses are never read)
+# ---------------------------------------------------------------------------
+ERR_ARG = -1
+ADDR = ctypes.c_void_p(4096)
+
+
+class Side(ctypes.Structure):
+    _fields_ = [("n_rows", ctypes.c_int64), ("n_cols", ctypes.c_int64),
+                ("n_edges", ctypes.c_int64), ("plan", ctypes.c_void_p),
+                ("n_items", ctypes.c_int32), ("n_parts", ctypes.c_int32)]
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return ctypes.CDLL(os.path.join(REPO, "batmobile-evo_amd", "lib", "libbatmobile_hip.so"))
+
+
+def _attention(lib, side, **given):
+    """batteries_neighbor_attention with 2 heads of 16, f32."""
+    p = {**dict.fromkeys(("q", "k", "v", "out"), ADDR), **given}
+    i64, none = ctypes.c_int64, ctypes.c_void_p(None)
+    return lib.batteries_neighbor_attention(
+        p["q"], p["k"], p["v"], none, none, 0, ctypes.byref(side), p["out"], none, 2, 2, 16, 16,
+        i64(32), i64(32), i64(32), ctypes.c_float(1.0), 0, none, ctypes.c_size_t(0), none)
+
+
+@pytest.mark.parametrize("n_edges,missing", [(0, "q"), (0, "out"), (5, "q"), (5, "k"), (5, "v"),
+                                             (5, "out")])
+def test_attention_refuses_a_missing_array(lib, n_edges, missing):
+    """q and out are read and written for every row, also where no row has an edge; k and v only
+    along edges."""
+    side = Side(3, 4, n_edges, 4096, 1, 0)
+    assert _attention(lib, side, **{missing: None}) == ERR_ARG
