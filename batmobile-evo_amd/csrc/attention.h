@@ -25,8 +25,8 @@ constexpr int kAttnCols = 32;     // columns of a chunk
 // ---------------------------------------------------------------------------
 // the plan of one side, in one int32 array
 // ---------------------------------------------------------------------------
-constexpr int kPlanHead = 16;     // items, parts, what is wrong
-constexpr int kPlanItems = 0, kPlanParts = 1, kPlanBad = 2;
+constexpr int kPlanHead = 16;     // items, parts, what is wrong, edges of all tiles (64 bits)
+constexpr int kPlanItems = 0, kPlanParts = 1, kPlanBad = 2, kPlanEdges = 4;
 
 // An item, read by a wave with one load: tile, first chunk, columns, part (-1: the tile's only
 // item); the tile's rows (-1 past the end); each row's first edge in the item; their number.

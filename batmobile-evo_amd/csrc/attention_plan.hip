@@ -28,9 +28,8 @@ struct PlanArgs {
 
 __global__ __launch_bounds__(kPlanThreads) void plan_tiles_kernel(PlanArgs a) {
     const int64_t t = (int64_t)blockIdx.x * kPlanThreads + threadIdx.x;
-    if (t >= a.at.tiles) return;
     int64_t edges = 0, longest = 0;
-    for (int s = 0; s < kAttnRows; ++s) {
+    for (int s = 0; t < a.at.tiles && s < kAttnRows; ++s) {
         const int64_t i = t * kAttnRows + s;
         int64_t row = i < a.n_rows ? (a.order ? a.order[i] : i) : -1;
         if (row >= a.n_rows || row < 0) row = -1;
@@ -42,6 +41,13 @@ __global__ __launch_bounds__(kPlanThreads) void plan_tiles_kernel(PlanArgs a) {
         edges += len;
         longest = max(longest, len);
     }
+    long long all = edges;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o);
+    if ((threadIdx.x & 63) == 0)
+        atomicAdd(reinterpret_cast<unsigned long long*>(a.plan + kPlanEdges),
+                  (unsigned long long)all);
+    if (t >= a.at.tiles) return;
     const int64_t cuts = longest > kTileRow || edges > kTileEdges
                              ? max(edges / plan_cut(a.n_edges), (int64_t)1)
                              : 1;
@@ -50,7 +56,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_tiles_kernel(PlanArgs a) {
     a.plan[a.at.tile_part + t] = cuts > 1 ? (int)cuts : 0;
 }
 
-// Exclusive sums of the three arrays, in place; 1024 threads.
+// Exclusive sums of the three arrays, in place; 1024 threads.  The plan has room for the items and
+// chunks of n_edges edges: where the tiles hold more (a row_ptr that falls and rises again, an order
+// that names a row twice), there are no items, and nothing is written past it.
 __global__ __launch_bounds__(1024) void plan_scan_kernel(PlanArgs a) {
     __shared__ int sums[16];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -77,6 +85,12 @@ __global__ __launch_bounds__(1024) void plan_scan_kernel(PlanArgs a) {
             if (k == 0) a.plan[kPlanItems] = carry;
             if (k == 2) a.plan[kPlanParts] = carry;
         }
+    }
+    if (threadIdx.x == 0 &&
+        *reinterpret_cast<const unsigned long long*>(a.plan + kPlanEdges) >
+            (unsigned long long)a.n_edges) {
+        a.plan[kPlanItems] = a.plan[kPlanParts] = 0;
+        a.plan[kPlanBad] |= 8;
     }
 }
 

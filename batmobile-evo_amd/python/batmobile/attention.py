@@ -62,6 +62,9 @@ class AttentionPlan:
         if bad & 4:
             raise ValueError("AttentionPlan: src must ascend within a row (from_edge_index takes "
                              "edges in any order)")
+        if bad & 8:
+            raise ValueError("AttentionPlan: row_ptr and order give the rows more edges than there "
+                             "are")
         self.side = (plan, items, parts)
 
     @classmethod
@@ -91,8 +94,10 @@ class AttentionPlan:
             place = torch.empty_like(pos, dtype=torch.int32)
             place[pos] = torch.arange(pos.numel(), dtype=torch.int32, device=pos.device)
             # last: it waits for the stream, so that any stream may use the result from here on
-            plan, items, parts, _ = _batmobile.attention_plan(
+            plan, items, parts, bad = _batmobile.attention_plan(
                 torch.searchsorted(by, rows), dst[pos], self._src_order, self.n_dst, False)
+            if bad:
+                raise ValueError("AttentionPlan: src_order must be a permutation")
             self._source_side = (plan, items, parts, place)
         return self._source_side
 

@@ -498,8 +498,9 @@ int batteries_mace_backward(const float* positions, const float* box, const floa
  * rows, in the given order (a permutation, NULL: as they are; rows next to each other in it
  * should share columns), into tiles and writes the plan (batteries_attention_plan_bytes, 64-byte
  * aligned).  Its first ints are the number of items, the number of parts (items of cut tiles)
- * and, with check, 0 or what is wrong with the arrays (1 row_ptr, 2 a column out of range, 4
- * columns not ascending); the caller reads them back into the side's n_items and n_parts.
+ * and 0 or what is wrong with the arrays: with check 1 row_ptr, 2 a column out of range, 4
+ * columns not ascending; always 8 where the rows in this order hold more edges than n_edges (the
+ * plan then has no items).  The caller reads them back into the side's n_items and n_parts.
  * n_edges < 2^29, n_rows < 2^26 - 64.
  * ------------------------------------------------------------------------- */
 typedef struct batmobile_attention_side {

@@ -7,6 +7,9 @@ bits (2^-9 = 2e-3 of the largest), the probabilities and their gradients possibl
 they meet the rows, whose weighted sum of absolute values is at most 3 times the largest result
 for these inputs: 8e-3.  The bias gradient is fp32 in either case: 1e-5.
 """
+import ctypes
+import os
+
 import numpy as np
 import pytest
 import torch
@@ -547,3 +550,48 @@ def test_plan_made_on_one_stream_and_used_on_another(dev):
         for name in grads:
             assert torch.equal(grads[name], wg[name]), name
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("check", [0, 1])
+@pytest.mark.parametrize("what", ["row_ptr", "order"])
+def test_plan_of_arrays_that_name_edges_again_and_again(dev, what, check):
+    """A row_ptr that rises and falls, and an order that holds one row only: the rows together have
+    thousands of times the edges that the plan has room for.  Refused, with nothing written behind
+    the plan."""
+    import batmobile
+    lib = ctypes.CDLL(os.path.join(os.path.dirname(batmobile.__file__), "..", "..", "lib",
+                                   "libbatmobile_hip.so"))
+    lib.batteries_attention_plan_bytes.restype = ctypes.c_size_t
+    n, e, m = 4000, 400, 500
+    src = torch.arange(e, device=dev)
+    if what == "row_ptr":
+        row_ptr = torch.tensor([0, e], device=dev).repeat(n // 2 + 1)[:n + 1]
+        order = None
+    else:
+        row_ptr = torch.full((n + 1,), e, dtype=torch.long, device=dev)
+        row_ptr[0] = 0
+        order = torch.zeros(n, dtype=torch.long, device=dev)
+    size = lib.batteries_attention_plan_bytes(ctypes.c_int64(n), ctypes.c_int64(e))
+    plan = torch.full((size // 4 + 4096,), -7, dtype=torch.int32, device=dev)
+    torch.cuda.synchronize()
+    at = lambda t: ctypes.c_void_p(None if t is None else t.data_ptr())
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert lib.batteries_attention_plan(at(row_ptr), at(src), at(order), ctypes.c_int64(n),
+                                        ctypes.c_int64(m), ctypes.c_int64(e), check, at(plan),
+                                        ctypes.c_size_t(size), stream) == 0
+    head = plan[:3].tolist()
+    assert head[:2] == [0, 0] and head[2] == 8 + (check and what == "row_ptr")
+    assert (plan[size // 4:] == -7).all()
+    with pytest.raises(ValueError, match="row_ptr|permutation"):
+        batmobile.AttentionPlan(src, row_ptr, m, order, validate=bool(check))
+
+
+def test_source_side_refuses_an_order_that_repeats_a_source(dev):
+    import batmobile
+    src, row_ptr = _edges([9] * 200, 30, 122)
+    most = int(np.bincount(src).argmax())
+    plan = batmobile.AttentionPlan(torch.from_numpy(src).to(dev), torch.from_numpy(row_ptr).to(dev),
+                                   30, src_order=torch.full((30,), most, device=dev),
+                                   validate=False)
+    with pytest.raises(ValueError, match="src_order"):
+        plan.source_side()
