@@ -1,6 +1,7 @@
 // The operators of an equivariant transformer block in the _batmobile extension (registered by
 // binding.cpp): attention over the edges of a graph, norms by degree with gate and residual,
 // gradient clipping.  No reference counterpart.  Host code only, over include/batmobile_hip.h.
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -54,6 +55,18 @@ const int64_t* index_ptr(const Tensor& t, const Tensor& as, int64_t n, const cha
 Tensor bytes_on(const Tensor& as, size_t n) {
     return torch::empty({(int64_t)((n + 15) / 16 * 16)},
                         torch::TensorOptions().dtype(torch::kUInt8).device(as.device()));
+}
+
+const Tensor* ptr_of(const OptTensor& t) { return t ? &*t : nullptr; }
+// The kernels form no forward-mode derivatives: a tangent would be lost without a word, since a dual
+// tensor need not require a gradient.
+void refuse_tangent(const Tensor* t, const char* what) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->defined() || !t->_fw_grad(/*level=*/0).defined(), what,
+                                " has no forward-mode derivative");
+}
+void refuse_tangents(std::initializer_list<const Tensor*> all, const char* what) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor* t : all) refuse_tangent(t, what);
 }
 
 // ---------------------------------------------------------------------------
@@ -461,7 +474,6 @@ bool wants_grad(std::initializer_list<const Tensor*> all) {
         if (t && t->defined() && t->requires_grad()) return true;
     return false;
 }
-const Tensor* ptr_of(const OptTensor& t) { return t ? &*t : nullptr; }
 OptTensor opt_of(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 Tensor tensor_of(const OptTensor& t) { return t ? *t : Tensor(); }
 
@@ -500,6 +512,7 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const bool create_graph = at::GradMode::is_enabled();
         const torch::NoGradGuard no_grad;
+        refuse_tangents({&grads[0]}, "the gradient of neighbor_attention");
         const variable_list s = ctx->get_saved_variables();
         const std::vector<int64_t> n = ctx->saved_data["sizes"].toIntVector();
         auto [gq, gk, gv, gb] = neighbor_attention_backward(
@@ -518,6 +531,7 @@ Tensor neighbor_attention_autograd(const Tensor& q, const Tensor& k, const Tenso
                                    int64_t parts, int64_t E, const OptTensor& edge_id,
                                    const Tensor& row_ptr, const pybind11::function& source_side,
                                    double scale) {
+    refuse_tangents({&q, &k, &v, ptr_of(bias)}, "neighbor_attention");
     if (!wants_grad({&q, &k, &v, ptr_of(bias)}))
         return std::get<0>(neighbor_attention(q, k, v, bias, plan, items, parts, E, edge_id, scale,
                                               false));
@@ -544,6 +558,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const bool create_graph = at::GradMode::is_enabled();
         const torch::NoGradGuard no_grad;
+        refuse_tangents({&grads.front(), &grads.back()}, "the gradient of gated_residual_norm");
         const variable_list s = ctx->get_saved_variables();
         const Tensor gh = s[1].defined() ? grads.front() : Tensor();
         const Tensor gn = s[5].defined() ? grads.back() : Tensor();
@@ -566,6 +581,8 @@ variable_list gated_residual_norm_autograd(const Tensor& x, const OptTensor& y,
                                            const OptTensor& gate, const OptTensor& scale,
                                            const OptTensor& w_post, const OptTensor& w_pre,
                                            double eps) {
+    refuse_tangents({&x, ptr_of(y), ptr_of(gate), ptr_of(scale), ptr_of(w_post), ptr_of(w_pre)},
+                    "gated_residual_norm");
     if (wants_grad({&x, ptr_of(y), ptr_of(gate), ptr_of(scale), ptr_of(w_post), ptr_of(w_pre)}))
         return NormNode::apply(x, y, gate, scale, w_post, w_pre, eps);
     auto [h, n, rs] = gated_residual_norm(x, y, gate, scale, w_post, w_pre, eps, false);
@@ -587,6 +604,8 @@ std::tuple<Tensor, std::vector<Tensor>> clip_grad_norm(
     TORCH_CHECK(max_norm >= 0.0, "max_norm must not be negative");
     TORCH_CHECK(!grads.empty(), "at least one tensor is needed");
     TORCH_CHECK(!outs || outs->size() == grads.size(), "out must hold one tensor per gradient");
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        for (const Tensor& g : grads) refuse_tangent(&g, "clip_grad_norm");
     const torch::NoGradGuard no_grad;
     const size_t n = grads.size();
     std::vector<const void*> in(n);

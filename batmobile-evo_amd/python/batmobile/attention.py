@@ -109,7 +109,8 @@ def neighbor_attention(q, k, v, plan, bias=None, scale=None):
     softmax in float32), H a multiple of H_kv, Dk and Dv up to 256; rows may be strided (slices
     of one projection).  bias [E, H] float32: an edge with -inf is left out.  A row without an
     edge gives zeros.  scale defaults to 1 / sqrt(Dk).  Gradients for q, k, v and bias,
-    which cannot be differentiated again (an error, not a missing term).
+    which cannot be differentiated again, and no forward-mode derivatives (an error, not a
+    missing term).
     """
     if q.dim() == 3 and (q.shape[0] != plan.n_dst or k.shape[0] != plan.n_src):
         raise RuntimeError(f"neighbor_attention: the plan has {plan.n_dst} destinations and "

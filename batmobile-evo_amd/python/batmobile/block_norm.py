@@ -23,7 +23,8 @@ def gated_residual_norm(x, y, gate, scale, weight_post, weight_pre=None, eps=1e-
 
     x (residual), y (the block's output) [N, C, 16], gate [N, C, 4] (None: no gate), scale [C],
     weights [4, C].  Returns (h, n), or h where weight_pre is None (after the last block).
-    Gradients for every tensor, which cannot be differentiated again (an error).
+    Gradients for every tensor, which cannot be differentiated again, and no forward-mode
+    derivatives (an error).
     """
     res = _batmobile.gated_residual_norm_autograd(x, y, gate, scale, weight_post, weight_pre,
                                                   float(eps))

@@ -90,3 +90,41 @@ def test_attention_refuses_a_missing_array(lib, n_edges, missing):
     along edges."""
     side = Side(3, 4, n_edges, 4096, 1, 0)
     assert _attention(lib, side, **{missing: None}) == ERR_ARG
+
+
+# ---------------------------------------------------------------------------
+# forward-mode derivatives: refused before anything else, never dropped
+# ---------------------------------------------------------------------------
+
+def _attention_call(batmobile, q, k, v, bias):
+    plan = types.SimpleNamespace(n_dst=3, n_src=4, side=(torch.zeros(0, dtype=torch.int32), 0, 0),
+                                 src=torch.zeros(2), edge_id=None, row_ptr=torch.zeros(4),
+                                 source_side=lambda: None)
+    return batmobile.neighbor_attention(q, k, v, plan, bias=bias)
+
+
+TANGENT_CALLS = {
+    "neighbor_attention": (_attention_call, [(3, 2, 8), (4, 2, 8), (4, 2, 8), (2, 2)]),
+    "equivariant_norm": (lambda b, x, w: b.equivariant_norm(x, w), [(3, 5, 16), (4, 5)]),
+    "gated_residual_norm": (lambda b, *t: b.gated_residual_norm(*t),
+                            [(3, 5, 16), (3, 5, 16), (3, 5, 4), (5,), (4, 5), (4, 5)]),
+    "clip_grad_norm": (lambda b, *t: b.clip_grad_norm(list(t), 1.0), [(3,), (4, 5)]),
+}
+
+
+@pytest.mark.parametrize("name,at", [(n, i) for n, (_, s) in TANGENT_CALLS.items()
+                                     for i in range(len(s))])
+@pytest.mark.parametrize("others_need_grad", [False, True])
+def test_forward_mode_derivatives_are_refused(name, at, others_need_grad):
+    import batmobile
+    import torch.autograd.forward_ad as fw
+    call, shapes = TANGENT_CALLS[name]
+    args = [torch.ones(s, requires_grad=others_need_grad and i != at) for i, s in enumerate(shapes)]
+    with fw.dual_level():
+        args[at] = fw.make_dual(torch.ones(shapes[at]), torch.ones(shapes[at]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(batmobile, *args)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            call(batmobile, *args)
+    with pytest.raises(RuntimeError, match="CUDA"):      # without a tangent: the next check
+        call(batmobile, *[torch.ones(s) for s in shapes])

@@ -595,3 +595,18 @@ def test_source_side_refuses_an_order_that_repeats_a_source(dev):
                                    validate=False)
     with pytest.raises(ValueError, match="src_order"):
         plan.source_side()
+
+
+def test_forward_mode_of_the_backward_is_refused(dev):
+    """A tangent on the gradient that comes in would be lost in the one that goes out."""
+    import batmobile
+    import torch.autograd.forward_ad as fw
+    src, row_ptr = _edges([3] * 5, 6, 123)
+    plan = batmobile.AttentionPlan(torch.from_numpy(src).to(dev), torch.from_numpy(row_ptr).to(dev), 6)
+    q = torch.randn(5, 2, 8, generator=gen(124)).to(dev).requires_grad_(True)
+    k = torch.randn(6, 2, 8, generator=gen(125)).to(dev)
+    out = batmobile.neighbor_attention(q, k, k, plan)
+    with fw.dual_level():
+        go = fw.make_dual(torch.ones_like(out), torch.ones_like(out))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(out, q, go)

@@ -313,3 +313,18 @@ def test_second_derivative_is_refused(dev):
     grad, = torch.autograd.grad(n.square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         grad.sum().backward()
+
+
+@pytest.mark.parametrize("which", ["gh", "gn"])
+def test_forward_mode_of_the_backward_is_refused(dev, which):
+    """A tangent on a gradient that comes in would be lost in those that go out."""
+    import batmobile
+    import torch.autograd.forward_ad as fw
+    t = {x: v.to(dev) for x, v in _inputs(4, 8, "f32", 91).items()}
+    x = t["x"].requires_grad_(True)
+    h, n = batmobile.gated_residual_norm(x, *[t[k] for k in ("y", "gate", "scale", "w_post", "w_pre")])
+    with fw.dual_level():
+        go = {k: t[k] for k in ("gh", "gn")}
+        go[which] = fw.make_dual(go[which], torch.ones_like(h))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad([h, n], x, [go["gh"], go["gn"]])
