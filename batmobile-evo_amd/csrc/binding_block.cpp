@@ -503,7 +503,10 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
         const bool need_bias = bias && bias->requires_grad();
         // a bias brought to [H, E] takes the place of the caller's
         ctx->save_for_backward({q, k, v, by_head.defined() ? Tensor() : tensor_of(bias), by_head,
-                                stats, p.row_ptr, p.plan, p.edge_id, p.src_plan, p.src_place});
+                                stats});
+        // not saved variables: a plan may have been made under inference mode
+        ctx->saved_data["plan"] =
+            std::vector<Tensor>{p.row_ptr, p.plan, p.edge_id, p.src_plan, p.src_place};
         ctx->saved_data["sizes"] =
             std::vector<int64_t>{p.items, p.parts, p.src_items, p.src_parts, need_bias};
         ctx->saved_data["scale"] = scale;
@@ -514,10 +517,11 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
         const torch::NoGradGuard no_grad;
         refuse_tangents({&grads[0]}, "the gradient of neighbor_attention");
         const variable_list s = ctx->get_saved_variables();
+        const std::vector<Tensor> p = ctx->saved_data["plan"].toTensorVector();
         const std::vector<int64_t> n = ctx->saved_data["sizes"].toIntVector();
         auto [gq, gk, gv, gb] = neighbor_attention_backward(
-            s[0], s[1], s[2], opt_of(s[3]), opt_of(s[4]), s[5], grads[0], s[6], s[7], n[0], n[1],
-            opt_of(s[8]), s[9], n[2], n[3], s[10], ctx->saved_data["scale"].toDouble(), n[4] != 0);
+            s[0], s[1], s[2], opt_of(s[3]), opt_of(s[4]), s[5], grads[0], p[0], p[1], n[0], n[1],
+            opt_of(p[2]), p[3], n[2], n[3], p[4], ctx->saved_data["scale"].toDouble(), n[4] != 0);
         variable_list g =
             first_order({gq, gk, gv, gb}, create_graph, "neighbor_attention");
         g.resize(6);

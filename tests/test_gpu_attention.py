@@ -610,3 +610,22 @@ def test_forward_mode_of_the_backward_is_refused(dev):
         go = fw.make_dual(torch.ones_like(out), torch.ones_like(out))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(out, q, go)
+
+
+def test_plan_made_under_inference_mode_trains(dev):
+    """An evaluation pass makes the plan (and its sources' side) first, training follows on it."""
+    import batmobile
+    src, row_ptr = _edges([7] * 40, 30, 126)
+    t = _inputs(40, 30, len(src), 2, 1, 16, 16, "f32", 127)
+    s, r = torch.from_numpy(src).to(dev), torch.from_numpy(row_ptr).to(dev)
+    ids = torch.randperm(len(src), generator=gen(128)).to(dev)
+    want, wg = _run(dev, batmobile.AttentionPlan(s, r, 30, edge_id=ids), t)
+    for early in (False, True):
+        with torch.inference_mode():
+            plan = batmobile.AttentionPlan(s.clone(), r.clone(), 30, edge_id=ids)
+            if early:
+                plan.source_side()
+        out, grads = _run(dev, plan, t)
+        assert torch.equal(out, want)
+        for name in grads:
+            assert torch.equal(grads[name], wg[name]), name

@@ -114,3 +114,16 @@ def test_block_refusals(dev):
         batmobile.AttentionBlock(64, 2)
     with pytest.raises(ValueError, match="multiple"):
         batmobile.AttentionBlock(32, 4, 3)
+
+
+def test_block_trains_on_a_graph_of_an_evaluation_pass(dev):
+    import batmobile
+    block = batmobile.AttentionBlock(16, 2, device=dev, generator=gen(73))
+    x = torch.randn(120, 16, 16, generator=gen(74)).to(dev)
+    with torch.inference_mode():
+        graph = _graph(dev, 120, 75, 16)
+        want = block(graph, x)
+    out = block(graph, x)
+    assert torch.equal(out, want)
+    out.square().sum().backward()
+    assert all(torch.isfinite(p.grad).all() for p in block.parameters())
