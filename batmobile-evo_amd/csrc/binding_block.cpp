@@ -7,6 +7,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <tuple>
@@ -599,9 +600,40 @@ variable_list gated_residual_norm_autograd(const Tensor& x, const OptTensor& y,
 // gradient clipping
 // ---------------------------------------------------------------------------
 
+// Which outs share memory with another out, with another gradient, or with their own gradient at
+// another place: the kernels' workgroups read and write in no order, so those go through a buffer.
+// in, out: the addresses of dense tensors.
+std::vector<bool> overlapping_outs(const std::vector<const void*>& in,
+                                   const std::vector<void*>& out,
+                                   const std::vector<int64_t>& bytes) {
+    struct Range {
+        uintptr_t begin, end;
+        int64_t out;                       // -1: only read
+        bool operator<(const Range& o) const { return begin < o.begin; }
+    };
+    std::vector<Range> all;
+    all.reserve(2 * in.size());
+    for (size_t i = 0; i < in.size(); ++i) {
+        const uintptr_t r = reinterpret_cast<uintptr_t>(in[i]), w = reinterpret_cast<uintptr_t>(out[i]);
+        if (bytes[i] == 0) continue;
+        all.push_back({w, w + (uintptr_t)bytes[i], (int64_t)i});
+        if (w != r) all.push_back({r, r + (uintptr_t)bytes[i], -1});
+    }
+    std::sort(all.begin(), all.end());
+    std::vector<bool> overlaps(in.size(), false);
+    for (size_t i = 0, j; i < all.size(); i = j) {     // runs of ranges that overlap
+        uintptr_t end = all[i].end;
+        for (j = i + 1; j < all.size() && all[j].begin < end; ++j) end = std::max(end, all[j].end);
+        for (size_t k = i; j - i > 1 && k < j; ++k)
+            if (all[k].out >= 0) overlaps[all[k].out] = true;
+    }
+    return overlaps;
+}
+
 // (norm, clipped): the norm as a tensor without dimensions; the clipped gradients in outs
 // (which may be the gradients; then nothing is returned for them) or in new tensors.  A strided
-// view with gaps, or an out of another layout than its gradient, goes through a dense copy.
+// view with gaps, an out of another layout than its gradient, or one that shares memory with
+// others, goes through a dense copy: every gradient is read before any result is seen.
 std::tuple<Tensor, std::vector<Tensor>> clip_grad_norm(
     const std::vector<Tensor>& grads, double max_norm,
     const c10::optional<std::vector<Tensor>>& outs) {
@@ -614,7 +646,7 @@ std::tuple<Tensor, std::vector<Tensor>> clip_grad_norm(
     const size_t n = grads.size();
     std::vector<const void*> in(n);
     std::vector<void*> out(n);
-    std::vector<int64_t> numel(n);
+    std::vector<int64_t> numel(n), bytes(n);
     std::vector<int> dt(n);
     std::vector<Tensor> dense(n), into(n);
     TORCH_CHECK(grads[0].is_cuda(), "a gradient must be a CUDA tensor");
@@ -632,6 +664,12 @@ std::tuple<Tensor, std::vector<Tensor>> clip_grad_norm(
         }
         if (!into[i].defined()) into[i] = torch::empty_like(g);
         in[i] = g.data_ptr(), out[i] = into[i].data_ptr(), numel[i] = g.numel();
+        bytes[i] = numel[i] * g.element_size();
+    }
+    if (outs) {
+        const std::vector<bool> overlaps = overlapping_outs(in, out, bytes);
+        for (size_t i = 0; i < n; ++i)
+            if (overlaps[i]) into[i] = torch::empty_like(into[i]), out[i] = into[i].data_ptr();
     }
     Tensor norm = torch::empty({}, grads[0].options().dtype(torch::kFloat32));
     int64_t elements = 0;

@@ -10,16 +10,22 @@ import _batmobile
 
 
 def clip_grad_norm(grads, max_norm, out=None):
-    """(norm, clipped): the clipped gradients in `out` (a list like grads; None: new tensors)."""
+    """(norm, clipped): the clipped gradients in `out` (a list like grads; None: new tensors).
+
+    out may hold grads themselves, in any order, or other tensors that share memory with them: all
+    of grads is read first.  A tensor that is listed twice counts twice in the norm and is scaled
+    once.
+    """
     norm, clipped = _batmobile.clip_grad_norm(grads, max_norm, out)
     return norm, clipped if out is None else out
 
 
 def clip_grad_norm_(parameters, max_norm):
-    """Clips the gradients of `parameters` in place; returns their norm before clipping."""
+    """Clips the gradients of `parameters` in place; returns their norm before clipping.  A
+    parameter that is listed twice (tied weights) counts and is scaled once."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    grads = [p.grad for p in parameters if p.grad is not None]
+    grads = [p.grad for p in dict.fromkeys(parameters) if p.grad is not None]
     if not grads:
         return torch.zeros(())
     return clip_grad_norm(grads, max_norm, grads)[0]

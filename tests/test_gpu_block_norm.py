@@ -328,3 +328,63 @@ def test_forward_mode_of_the_backward_is_refused(dev, which):
         go[which] = fw.make_dual(go[which], torch.ones_like(h))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad([h, n], x, [go["gh"], go["gn"]])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_clip_of_tensors_that_share_memory(dev, dtype):
+    """A gradient listed twice in place, outs that are the gradients in another order, shifted
+    views, an out behind two gradients: each result is its gradient times the factor, whatever the
+    order of the writes.  Sizes of some hundred shares, tolerances as in test_clip."""
+    import batmobile
+    bound = 5e-7 if dtype == "f32" else 4e-3
+    n = 1 << 21
+    base = torch.randn(n + 64, generator=gen(92)).to(TYPES[dtype])
+
+    def check(grads, outs):
+        want = ob.clip([_np(x) for x in grads], 1.0)
+        norm, res = batmobile.clip_grad_norm(grads, 1.0, outs)
+        assert res is outs and abs(float(norm) - want[0]) <= 1e-6 * want[0]
+        return want[1]
+
+    for _ in range(3):
+        a = base[:n].to(dev)
+        want = check([a, a], [a, a])                      # twice in place
+        assert normwise_err(_np(a), want[0]) <= bound
+        a, b = base[:n].to(dev), base[64:].to(dev)
+        want = check([a, b], [b, a])                      # exchanged
+        assert normwise_err(_np(b), want[0]) <= bound
+        assert normwise_err(_np(a), want[1]) <= bound
+        a = base.to(dev)
+        want = check([a[:n]], [a[64:]])                   # shifted
+        assert normwise_err(_np(a[64:]), want[0]) <= bound
+        assert torch.equal(a[:64].cpu(), base[:64])
+        a, b = base.to(dev), base[5:4005].to(dev)
+        want = check([a[:n], b, a[n:]], [torch.empty(n, dtype=a.dtype, device=dev), a[n - 4000:n],
+                                         a[n:]])          # one gradient's end is another's out
+        assert normwise_err(_np(a[n - 4000:n]), want[1]) <= bound
+        assert normwise_err(_np(a[n:]), want[2]) <= bound
+    # parts of one buffer, in place: no copies, the bits of separate tensors
+    flat = base.to(dev)
+    parts, alone = list(flat.split(1000)), [x.clone() for x in flat.split(1000)]
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    batmobile.clip_grad_norm(parts, 1.0, parts)
+    assert torch.cuda.max_memory_allocated() - held < 1 << 18
+    _, want = batmobile.clip_grad_norm(alone, 1.0)
+    assert all(torch.equal(x, y) for x, y in zip(parts, want))
+
+
+def test_clip_of_a_parameter_listed_twice(dev):
+    """Tied weights in two lists: counted once, scaled once, from run to run the same."""
+    import batmobile
+    w = torch.nn.Parameter(torch.zeros(1 << 20, device=dev))
+    u = torch.nn.Parameter(torch.zeros(37, device=dev))
+    gw, gu = torch.randn(1 << 20, generator=gen(93)), torch.randn(37, generator=gen(94))
+    rn, want = ob.clip([_np(gw), _np(gu)], 2.0)
+    for _ in range(5):
+        w.grad, u.grad = gw.to(dev), gu.to(dev)
+        norm = batmobile.clip_grad_norm_([w, u, w], 2.0)
+        assert abs(float(norm) - rn) <= 1e-6 * rn
+        assert normwise_err(_np(w.grad), want[0]) <= 5e-7
+        assert normwise_err(_np(u.grad), want[1]) <= 5e-7
