@@ -682,8 +682,10 @@ std::tuple<Tensor, std::vector<Tensor>> clip_grad_norm(
                  "clip_grad_norm");
     if (!outs) return {norm, into};
     for (size_t i = 0; i < n; ++i) {
-        Tensor o = (*outs)[i];
+        const Tensor& o = (*outs)[i];
         if (!o.is_same(into[i])) o.copy_(into[i]);
+        // written by address: whoever saved it for a backward is told as by torch's own operators
+        else if (!o.is_inference()) torch::autograd::impl::bump_version(o);
     }
     return {norm, {}};
 }

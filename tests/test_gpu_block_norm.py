@@ -388,3 +388,30 @@ def test_clip_of_a_parameter_listed_twice(dev):
         assert abs(float(norm) - rn) <= 1e-6 * rn
         assert normwise_err(_np(w.grad), want[0]) <= 5e-7
         assert normwise_err(_np(u.grad), want[1]) <= 5e-7
+
+
+def test_clip_tells_autograd_what_it_writes(dev):
+    """Tensors that a graph has saved and clipping writes, dense or through a copy, raise in the
+    backward as with torch's own in-place operators; inference tensors have no versions."""
+    import batmobile
+    x = torch.ones(50, device=dev, requires_grad=True)
+    for g in (torch.full((50,), 2.0, device=dev), torch.full((100,), 2.0, device=dev)[::2]):
+        for write in (lambda: batmobile.clip_grad_norm([g], 1.0, [g]),
+                      lambda: batmobile.clip_grad_norm([torch.ones(50, device=dev)], 1.0, [g])):
+            y = (x * g).sum()
+            version = g._version
+            write()
+            assert g._version > version
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.backward()
+    p = torch.nn.Parameter(torch.ones(5, device=dev))
+    loss = (p ** 3).sum()
+    p.grad, = torch.autograd.grad(loss, p, create_graph=True)
+    z = (p.grad ** 2).sum()
+    batmobile.clip_grad_norm_([p], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    with torch.inference_mode():
+        g = torch.full((4,), 2.0, device=dev)
+        batmobile.clip_grad_norm([g], 1.0, [g])
+        assert torch.allclose(g, torch.full_like(g, 0.5))
