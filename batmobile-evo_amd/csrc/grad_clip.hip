@@ -116,7 +116,11 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(ClipArgs a, co
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
     // a norm that is not a number makes the factor, and every gradient, not a number
     const double r = (double)max_norm / (total + 1e-6);
-    const float f = r < 1.0 ? (float)r : (r != r ? (float)r : 1.0f);
+    // a factor near fp32's smallest number would keep few of its bits: taken in two steps, both exact
+    // in size (at 2^64 times its value it passes no element of 2^128 over fp32's range)
+    const bool tiny = r < 0x1p-100;
+    const float f = r < 1.0 ? (float)(tiny ? r * 0x1p64 : r) : (r != r ? (float)r : 1.0f);
+    const float f2 = tiny ? 0x1p-64f : 1.0f;
     clip_shares(a, true, [&](int k, uint32_t i0, bool whole) {
         const bool bf = a.bf16[k];
         if (whole) {
@@ -130,14 +134,15 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(ClipArgs a, co
             for (int j = 0; j < kClipLoads; ++j) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    x[j].v[c] = bf ? bf16_pack(bf16_lo(x[j].v[c]) * f, bf16_hi(x[j].v[c]) * f)
-                                   : __float_as_uint(__uint_as_float(x[j].v[c]) * f);
+                    x[j].v[c] = bf ? bf16_pack(bf16_lo(x[j].v[c]) * f * f2,
+                                               bf16_hi(x[j].v[c]) * f * f2)
+                                   : __float_as_uint(__uint_as_float(x[j].v[c]) * f * f2);
                 q[j * kClipThreads] = x[j];
             }
             return;
         }
         for (uint32_t i = i0 + threadIdx.x; i < a.numel[k]; i += kClipThreads) {
-            const float v = clip_ld(a.in[k], i, bf) * f;
+            const float v = clip_ld(a.in[k], i, bf) * f * f2;
             if (bf) ((uint16_t*)a.out[k])[i] = (uint16_t)(bf16_pack(v, 0.0f) & 0xffffu);
             else ((float*)a.out[k])[i] = v;
         }

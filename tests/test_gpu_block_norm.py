@@ -415,3 +415,17 @@ def test_clip_tells_autograd_what_it_writes(dev):
         g = torch.full((4,), 2.0, device=dev)
         batmobile.clip_grad_norm([g], 1.0, [g])
         assert torch.allclose(g, torch.full_like(g, 0.5))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("max_norm", [1.0, 1e-3, 1e-6])
+def test_clip_factor_below_the_normal_numbers(dev, dtype, max_norm):
+    """Gradients of 1e38, whose factor lies below 2^-126 (or below fp32's smallest number) though the
+    results do not: whole shares and a remainder, the bounds of test_clip."""
+    import batmobile
+    grads = _grads([(50,), (30011,)], [dtype] * 2, 95, 2e37)
+    norm, out = batmobile.clip_grad_norm([g.to(dev) for g in grads], max_norm)
+    rn, want = ob.clip([_np(g) for g in grads], float(np.float32(max_norm)))
+    assert max_norm / rn < 2.0 ** -126
+    for o, w in zip(out, want):
+        assert normwise_err(_np(o), w) <= (5e-7 if dtype == "f32" else 4e-3)
