@@ -119,6 +119,23 @@ __device__ __forceinline__ float row_sum(float v, float* sh, int& turn) {
     return v;
 }
 
+// sigmoid(g) and 1 - sigmoid(g), each to full relative precision at any g: the smaller one comes of the
+// exponential of -|g|, the larger is 1 less that.  One register: the smaller, with a minus if it is
+// 1 - sigmoid.
+__device__ __forceinline__ float sigmoid_pair(float g) {
+    const float a = fabsf(g) * 0.5f, x = a * -1.44269504f;        // log2 e, and what it leaves out
+    float e = __builtin_amdgcn_exp2f(x);                          // exp(-|g| / 2), to the square
+    e *= fmaf(fmaf(a, -1.44269504f, -x) - a * 1.92596299e-8f, 0.693147181f, 1.0f);
+    e *= e;
+    return copysignf(e * __builtin_amdgcn_rcpf(1.0f + e), -g);
+}
+__device__ __forceinline__ float sigmoid_on(float p) {
+    return __float_as_int(p) < 0 ? 1.0f + p : p;
+}
+__device__ __forceinline__ float sigmoid_off(float p) {
+    return __float_as_int(p) < 0 ? -p : 1.0f - p;
+}
+
 struct NormArgs {
     const void *x, *y, *gate, *gh, *gn;
     const float *scale, *w_post, *w_pre, *rs_in;
@@ -177,7 +194,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_fwd_kernel(NormArg
         for (int i = 0; i < NV; ++i) {
             const int c = min((i * 64 * W + t) >> 2, a.C - 1);
             float w = a.scale[c] * a.w_post[q * a.C + c] * r;
-            if constexpr (GATE) w /= 1.0f + __expf(-f[i]);
+            if constexpr (GATE) w *= sigmoid_on(sigmoid_pair(f[i]));
             const float fa = first_of(w), fb = others_of(w);
             const float4 yi = y[i].get(), xi = x[i].get();
             h[i] = make_float4(fmaf(fa, yi.x, xi.x), fmaf(fb, yi.y, xi.y), fmaf(fb, yi.z, xi.z),
@@ -266,15 +283,23 @@ __global__ __launch_bounds__(W <= 4 ? 256 : 64 * W) void norm_bwd_kernel(NormArg
                 if constexpr (PRE) x.gn[i].zero();
                 if constexpr (BLOCK) x.y[i].zero();
             }
+        float sg[NV];                    // before the next row takes registers
+        if constexpr (GATE) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) sg[i] = sigmoid_pair(x.sg[i]);
+        }
         if (kAhead && row0 + step < a.n) load(next, row0 + step);
         float4 G[NV];
-        float f[NV], sg[NV];
+        float f[NV];
         if constexpr (BLOCK) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = min((i * 64 * W + t) >> 2, a.C - 1);
-                sg[i] = GATE ? __builtin_amdgcn_rcpf(1.0f + __expf(-x.sg[i])) : 1.0f;
-                f[i] = a.scale[c] * sg[i] * a.w_post[q * a.C + c];
+                f[i] = a.scale[c] * a.w_post[q * a.C + c];
+                if constexpr (GATE) {
+                    f[i] *= sigmoid_on(sg[i]);
+                    asm volatile("" : "+v"(sg[i]));     // one register to the end, not two
+                }
             }
         }
         if constexpr (PRE) {
@@ -325,12 +350,13 @@ __global__ __launch_bounds__(W <= 4 ? 256 : 64 * W) void norm_bwd_kernel(NormArg
                 const float sc = a.scale[min(c, a.C - 1)], w = a.w_post[q * a.C + min(c, a.C - 1)];
                 const float z = dot4(G[i], x.y[i].get(), q), rz = r * z;    // 0 past C
                 s = fmaf(f[i], z, s);
-                aw_post[i] = fmaf(sc * sg[i], rz, aw_post[i]);
-                a_scale[i] = fmaf(sg[i] * w, rz, a_scale[i]);
+                const float on = GATE ? sigmoid_on(sg[i]) : 1.0f;
+                aw_post[i] = fmaf(sc * on, rz, aw_post[i]);
+                a_scale[i] = fmaf(on * w, rz, a_scale[i]);
                 if constexpr (GATE)
                     if (there && c < a.C)
                         norm_st((T*)a.ggate + row * a.C * 4 + i * 64 * W + t,
-                                f[i] * (1.0f - sg[i]) * rz);
+                                f[i] * sigmoid_off(sg[i]) * rz);
             }
             const float k = -row_sum<W>(s, sh, turn) * cnt * r * r * r;
             const float ka = first_of(k), kb = others_of(k);

@@ -75,6 +75,8 @@ def gated_residual_norm(x, y, gate, scale, w_post, w_pre, eps=1e-6, gh=None, gn=
         y = np.asarray(y, np.float64)
         s = 1 / (1 + np.exp(-np.asarray(gate, np.float64))) if gate is not None \
             else np.ones(x.shape[:2] + (4,))
+        # 1 - s, where s is next to 1 as well
+        off = 1 / (1 + np.exp(np.asarray(gate, np.float64))) if gate is not None else 0
         sc = np.asarray(scale, np.float64)[None, :, None]
         post, ry = norm(y, w_post, eps)
         h = x + sc * s[:, :, DEGREE] * post
@@ -89,7 +91,7 @@ def gated_residual_norm(x, y, gate, scale, w_post, w_pre, eps=1e-6, gh=None, gn=
     if y is not None:
         g["y"], g["w_post"] = _norm_grad(y, ry, w_post, G * sc * s[:, :, DEGREE])
         by = np.stack([(G * post)[:, :, DEGREE == l].sum(2) for l in range(4)], 2)
-        g["gate"] = by * sc * s * (1 - s)
+        g["gate"] = by * sc * s * off
         g["scale"] = (by * s).sum((0, 2))
     return h, n, g
 

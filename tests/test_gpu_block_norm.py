@@ -429,3 +429,20 @@ def test_clip_factor_below_the_normal_numbers(dev, dtype, max_norm):
     assert max_norm / rn < 2.0 ** -126
     for o, w in zip(out, want):
         assert normwise_err(_np(o), w) <= (5e-7 if dtype == "f32" else 4e-3)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("center", [-85.0, -30.0, -12.0, 12.0, 30.0, 85.0])
+def test_gates_far_from_zero(dev, dtype, center):
+    """Saturated gates: h is next to nothing of y or all of it, the gate's gradient next to nothing.
+    Each is compared with its own largest value (x = 0), which sigmoid or 1 - sigmoid scales."""
+    t = _inputs(19, 24, dtype, 96)
+    t["x"].zero_()
+    t["gate"] = (t["gate"].float() + center).to(TYPES[dtype])
+    pre = center > 0    # below, h is too small for a norm of it
+    h, _, grads = _block(dev, t, pre=pre, seeds=("gh", "gn") if pre else ("gh",))
+    rh, _, want = ob.gated_residual_norm(
+        *[_np(t[x]) for x in ("x", "y", "gate", "scale", "w_post")],
+        _np(t["w_pre"]) if pre else None, gh=_np(t["gh"]), gn=_np(t["gn"]) if pre else None)
+    assert normwise_err(_np(h), rh) <= BOUND[dtype]
+    _check(grads, want, dtype)
