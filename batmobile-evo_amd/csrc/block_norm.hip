@@ -123,7 +123,8 @@ __device__ __forceinline__ float row_sum(float v, float* sh, int& turn) {
 // exponential of -|g|, the larger is 1 less that.  One register: the smaller, with a minus if it is
 // 1 - sigmoid.
 __device__ __forceinline__ float sigmoid_pair(float g) {
-    const float a = fabsf(g) * 0.5f, x = a * -1.44269504f;        // log2 e, and what it leaves out
+    const float a = fabsf(g) > 256.0f ? 128.0f : fabsf(g) * 0.5f; // (infinities end at 0, NaN stays)
+    const float x = a * -1.44269504f;                             // log2 e, and what it leaves out
     float e = __builtin_amdgcn_exp2f(x);                          // exp(-|g| / 2), to the square
     e *= fmaf(fmaf(a, -1.44269504f, -x) - a * 1.92596299e-8f, 0.693147181f, 1.0f);
     e *= e;

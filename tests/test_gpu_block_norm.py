@@ -446,3 +446,27 @@ def test_gates_far_from_zero(dev, dtype, center):
         _np(t["w_pre"]) if pre else None, gh=_np(t["gh"]), gn=_np(t["gn"]) if pre else None)
     assert normwise_err(_np(h), rh) <= BOUND[dtype]
     _check(grads, want, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_infinite_and_nan_gates(dev, dtype):
+    """-inf closes a gate, inf opens it (factors 0 and 1, no gradient), the type's largest values as
+    well; a NaN stays in its row."""
+    t = _inputs(30, 20, dtype, 97)
+    big = torch.finfo(TYPES[dtype]).max
+    for i, g in enumerate((np.inf, -np.inf, big, -big)):
+        t["gate"][i::6, ::3, 1:3] = g
+    h, n, grads = _block(dev, t)
+    with np.errstate(over="ignore"):
+        rh, rn, want = ob.gated_residual_norm(
+            *[_np(t[x]) for x in ("x", "y", "gate", "scale", "w_post", "w_pre")],
+            gh=_np(t["gh"]), gn=_np(t["gn"]))
+    assert normwise_err(_np(h), rh) <= BOUND[dtype]
+    assert normwise_err(_np(n), rn) <= BOUND[dtype]
+    _check(grads, want, dtype)
+    assert not grads["gate"][0, ::3, 1:3].any() and not grads["gate"][1, ::3, 1:3].any()
+    t["gate"][4, 2, 1] = np.nan
+    h, n, grads = _block(dev, t)
+    rows = [i for i in range(30) if i != 4]
+    assert torch.isnan(h[4, 2, 1:4]).all() and torch.isfinite(h[rows]).all()
+    assert torch.isnan(grads["gate"][4]).any() and torch.isfinite(grads["gate"][rows]).all()
