@@ -74,8 +74,8 @@ void refuse_tangents(std::initializer_list<const Tensor*> all, const char* what)
 // attention
 // ---------------------------------------------------------------------------
 
-// Matrices [n, heads, D] as the kernels read them: heads of a row dense, rows at any stride,
-// everything in units of 16 bytes.  Others are packed (head sizes padded with zeros, which add
+// Matrices [n, heads, D] as the kernels read them: heads of a row dense, rows at any stride below
+// 2^30 elements, everything in units of 16 bytes.  Others are packed (head sizes padded with zeros, which add
 // nothing to a product), all in one launch.
 class Packer {
 public:
@@ -83,7 +83,8 @@ public:
         const int64_t unit = 16 / t.element_size(), D = t.size(2);
         const bool dense = t.stride(2) == 1 && (t.size(1) == 1 || t.stride(1) == D) &&
                            (t.size(0) <= 1 ||
-                            (t.stride(0) >= t.size(1) * D && t.stride(0) % unit == 0)) &&
+                            (t.stride(0) >= t.size(1) * D && t.stride(0) % unit == 0 &&
+                             t.stride(0) < (int64_t)1 << 30)) &&
                            (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
         if (D % unit == 0 && (dense || t.numel() == 0)) return t.numel() ? t : t.contiguous();
         Tensor out = torch::empty({t.size(0), t.size(1), (D + unit - 1) / unit * unit}, t.options());

@@ -629,3 +629,25 @@ def test_plan_made_under_inference_mode_trains(dev):
         assert torch.equal(out, want)
         for name in grads:
             assert torch.equal(grads[name], wg[name]), name
+
+
+def test_rows_2_30_elements_apart(dev):
+    """Strides past what the kernels take as they are: such rows are packed first, not refused."""
+    import batmobile
+    n, m, d = 2, 2, 16
+    src, row_ptr = np.array([0, 1, 1]), np.array([0, 2, 3])
+    t = _inputs(n, m, 3, 1, 1, d, d, "bf16", 129)
+    plan = batmobile.AttentionPlan(torch.from_numpy(src).to(dev),
+                                   torch.from_numpy(row_ptr).to(dev), m)
+    want, wg = _run(dev, plan, t)
+    store = torch.empty((1 << 30) + 4 * d, dtype=torch.bfloat16, device=dev)
+    far = {}
+    for i, x in enumerate(("q", "k", "v", "go")):
+        far[x] = store[i * d:].as_strided((2, 1, d), (1 << 30, d, 1))
+        far[x].copy_(t[x].to(dev))
+        far[x] = far[x].detach().requires_grad_(x != "go")
+    leaf = [far["q"], far["k"], far["v"], t["bias"].to(dev).requires_grad_(True)]
+    out = batmobile.neighbor_attention(*leaf[:3], plan, bias=leaf[3])
+    assert torch.equal(out, want)
+    for name, got in zip(("q", "k", "v", "bias"), torch.autograd.grad(out, leaf, far["go"])):
+        assert torch.equal(got, wg[name]), name
