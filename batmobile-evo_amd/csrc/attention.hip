@@ -29,7 +29,7 @@ struct AttnFwd {
 };
 
 // An item's rows one after the other, each over its own edges alone: infinities or NaN among the
-// values, or more edges than the LDS holds.
+// values.
 template <typename T>
 __device__ __forceinline__ void attn_fwd_rows(const AttnFwd& a, int item, int h, int tile,
                                               int part_at) {
@@ -105,10 +105,6 @@ __global__ __launch_bounds__(64, (KP + VP) * sizeof(T) <= 1536 ? 2 : 1) void att
     const int row = it.row, steps = it.steps(kT);
     const T* kbase = (const T*)a.k + (int64_t)kv * a.Dk;
     const T* vbase = (const T*)a.v + (int64_t)kv * a.Dv;
-    if (BIAS && __builtin_expect(it.total > kTileEdges, 0)) {
-        attn_fwd_rows<T>(a, item, h, it.tile, it.part);
-        return;
-    }
     v4f acc[ColFrag<T, VP>::kAcc];
     float m = -kInf, l = 0.0f;
 #pragma unroll

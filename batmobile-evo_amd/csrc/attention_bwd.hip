@@ -34,49 +34,6 @@ struct AttnScores {
     float scale;
 };
 
-// An item's rows one after the other (more edges than the LDS holds): p and dp, and D and ds of a
-// tile that is not cut.
-template <typename T>
-__device__ __forceinline__ void attn_scores_rows(const AttnScores& a, int item, int h,
-                                                 const Item& it) {
-    constexpr float kInf = __builtin_inff();
-    const int kv = h / a.group;
-    float2* ws = a.ws + (int64_t)h * a.edges;
-    for (int r = 0; r < kAttnRows; ++r) {
-        const int row = a.side.rows[it.tile * kAttnRows + r];
-        if (row < 0) continue;
-        const T* q = row_of<T>(a.q, row, a.qs) + (int64_t)h * a.Dk;
-        const T* go = row_of<T>(a.go, row, a.gs) + (int64_t)h * a.Dv;
-        const float* ml = a.stats + ((int64_t)row * a.H + h) * 2;
-        const float ref = ml[0] == -kInf ? 0.0f : ml[0], inv = ml[1] == 0.0f ? 0.0f : 1.0f / ml[1];
-        float d = 0.0f;
-        each_edge(a.side, item, r, [&](int e, int col) {
-            const float b = a.bias.value ? a.bias.at(e, h) : 0.0f;
-            const T* k = row_of<T>(a.k, col, a.ks) + (int64_t)kv * a.Dk;
-            const T* v = row_of<T>(a.v, col, a.vs) + (int64_t)kv * a.Dv;
-            float s = 0.0f, y = 0.0f;
-            for (int c = threadIdx.x; c < a.Dk; c += 64) s = fmaf(attn_f32(q[c]), attn_f32(k[c]), s);
-            for (int c = threadIdx.x; c < a.Dv; c += 64)
-                y = fmaf(attn_f32(go[c]), attn_f32(v[c]), y);
-            const float x = fmaf(attn_wave_sum(s), a.scale, b);
-            const float p = b == -kInf || x == -kInf ? 0.0f : attn_exp(x - ref) * inv;
-            y = attn_wave_sum(y);
-            y = p == 0.0f ? 0.0f : y;
-            d = fmaf(p, y, d);
-            if (threadIdx.x == 0) ws[a.place[e]] = make_float2(p, y);
-        });
-        if (it.part >= 0) continue;
-        each_edge(a.side, item, r, [&](int e, int) {
-            if (threadIdx.x != 0) return;      // reads what it wrote itself
-            const float2 w = ws[a.place[e]];
-            const float ds = w.x == 0.0f ? 0.0f : w.x * (w.y - d);
-            ws[a.place[e]].y = ds;
-            a.wd[(int64_t)h * a.edges + e] = ds;
-            if (a.gbias) a.gbias[(int64_t)(a.eid ? a.eid[e] : e) * a.H + h] = ds;
-        });
-    }
-}
-
 // A step takes 16 columns: with 32 the rows of k and v would leave LDS for 6 waves a CU only.
 // k and v of a step go to LDS while the products of the step before run; p and dp of the step
 // before are written to LDS first, as are all reads done (attn_fwd_kernel).
@@ -113,10 +70,6 @@ __global__ __launch_bounds__(64, 2) void attn_scores_kernel(AttnScores a) {
     const float2 ml =
         *reinterpret_cast<const float2*>(a.stats + ((int64_t)max(row, 0) * a.H + h) * 2);
     const float ref = ml.x == -kInf ? 0.0f : ml.x, inv = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
-    if (__builtin_expect(it.total > kTileEdges, 0)) {
-        attn_scores_rows<T>(a, item, h, it);
-        return;
-    }
     KRows::template fill<FULL, WIDE>(k_lds, ids, kbase, a.ks, a.Dk, lane);
     VRows::template fill<FULL, WIDE>(v_lds, ids, vbase, a.vs, a.Dv, lane);
     ids = step.ids(1);
@@ -325,10 +278,6 @@ __global__ __launch_bounds__(64, 2) void attn_sum_kernel(AttnSums all) {
     const int lane = threadIdx.x, n = lane & 15, g = lane >> 4;
     const Item it(a.side, item, lane);
     const int row = it.row, steps = it.steps(kT);
-    if (__builtin_expect(it.total > kTileEdges, 0)) {
-        attn_sum_rows<T>(a, item, head, it);
-        return;
-    }
     v4f acc[ColFrag<T, P>::kAcc];
     {
 #pragma unroll

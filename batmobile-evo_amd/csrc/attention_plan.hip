@@ -7,9 +7,8 @@
 //                equal columns of different rows merged into one entry (a column that a row
 //                holds k times, parallel edges, gets k entries), masks from the entries
 //
-// A tile with many edges or a long row is cut at column values into items of equal edge counts,
-// each found by searching for its first column.  A cut with more edges than the LDS holds (one
-// column thousands of times) is taken unmerged.
+// A tile with many edges or a long row is cut into items of equal edge counts, each found by
+// searching for its first column, and within a column that has very many.
 //
 // Once per graph: 5000 atoms with 28 neighbours take 55 us (35 of them plan_items, whose sort is
 // steps of LDS latency and barriers), 50,000 atoms 150 us.
@@ -17,7 +16,7 @@
 
 namespace bmhip {
 
-constexpr int kPlanThreads = 256, kPlanSort = 4096;
+constexpr int kPlanThreads = 256;
 
 struct PlanArgs {
     const int64_t *row_ptr, *col, *order;
@@ -106,12 +105,12 @@ __device__ __forceinline__ int64_t edges_below(const int64_t* col, int64_t e0, i
 }
 
 __global__ __launch_bounds__(kPlanThreads) void plan_items_kernel(PlanArgs a) {
-    __shared__ uint64_t key[kPlanSort];
-    __shared__ uint16_t before[kPlanSort + 1];       // entries before each sorted edge
-    __shared__ uint32_t mask[kPlanSort / kAttnCols * kAttnRows];
+    __shared__ uint64_t key[kTileEdges];
+    __shared__ uint16_t before[kTileEdges + 1];       // entries before each sorted edge
+    __shared__ uint32_t mask[kTileEdges / kAttnCols * kAttnRows];
     __shared__ int64_t start[kAttnRows], stop[kAttnRows], full[2][kAttnRows];
     __shared__ int pre[kAttnRows + 1], sums[kPlanThreads / 64];
-    __shared__ int64_t cut[2];
+    __shared__ int64_t cut[2], below[2][2][kAttnRows];
     __shared__ int count[16];
     const int item = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     if (item >= a.plan[kPlanItems]) return;
@@ -164,12 +163,24 @@ __global__ __launch_bounds__(kPlanThreads) void plan_items_kernel(PlanArgs a) {
             if (tid == 0) cut[side] = c0;
         }
         __syncthreads();
+        // a row's edges before the cut's column (0: the column before, which crosses the share)
+        if (tid < 4 * kAttnRows) {
+            const int r = tid & 15, side = (tid >> 4) & 1, k = tid >> 5;
+            below[k][side][r] = edges_below(a.col, full[0][r], full[1][r], cut[side] - 1 + k);
+        }
+        __syncthreads();
         if (tid < 2 * kAttnRows) {
             const int r = tid & 15, side = tid >> 4;
-            int64_t e = part + side == parts
-                            ? full[1][r]
-                            : full[0][r] + edges_below(a.col, full[0][r], full[1][r], cut[side]);
-            (side ? stop : start)[r] = e;
+            int64_t column = 0, left = edges * (part + side) / parts;
+            for (int i = 0; i < kAttnRows; ++i) {
+                const int64_t n = below[1][side][i] - below[0][side][i];
+                column += n;
+                left -= below[0][side][i] + (i < r ? n : 0);
+            }
+            int64_t e = below[1][side][r];
+            if (column > kCutColumn)                 // its edges row by row up to the share
+                e = below[0][side][r] + min(max(left, (int64_t)0), e - below[0][side][r]);
+            (side ? stop : start)[r] = part + side == parts ? full[1][r] : full[0][r] + e;
         }
         __syncthreads();
         if (tid < kAttnRows) stop[tid] = max(stop[tid], start[tid]);
@@ -208,21 +219,10 @@ __global__ __launch_bounds__(kPlanThreads) void plan_items_kernel(PlanArgs a) {
         const int64_t c = a.col[start[r] + (i - pre[r])];
         return (int)(c >= 0 && c < a.n_cols ? c : 0);
     };
-    if (n > kPlanSort) {
-        // one entry per edge
-        const int chunks = (n + kAttnCols - 1) / kAttnCols;
-        for (int i = tid; i < chunks * kAttnCols; i += kPlanThreads) {
-            int r;
-            ids[i] = column(min(i, n - 1), r);
-        }
-        for (int i = tid; i < chunks * kAttnRows; i += kPlanThreads) {
-            const int r = i & 15, c0 = (i >> 4) * kAttnCols;
-            const int b0 = max(pre[r] - c0, 0), b1 = min(pre[r + 1] - c0, kAttnCols);
-            uint32_t m = 0;
-            for (int b = b0; b < b1; ++b) m |= 1u << b;
-            masks[i] = m;
-        }
-        finish(n);
+    if (n > kTileEdges) {                            // only of columns that do not ascend
+        if (tid < kAttnRows) out[kItemCount + tid] = 0;
+        if (tid == 0) atomicOr(&a.plan[kPlanBad], 4);
+        finish(0);
         return;
     }
     int size = 64;
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_items_kernel(PlanArgs a) {
         }
         key[i] = k;
     }
-    for (int i = tid; i < kPlanSort / kAttnCols * kAttnRows; i += kPlanThreads) mask[i] = 0;
+    for (int i = tid; i < kTileEdges / kAttnCols * kAttnRows; i += kPlanThreads) mask[i] = 0;
     for (int k = 2; k <= size; k <<= 1)
         for (int j = k >> 1; j > 0; j >>= 1) {
             __syncthreads();

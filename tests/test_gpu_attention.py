@@ -651,3 +651,73 @@ def test_rows_2_30_elements_apart(dev):
     assert torch.equal(out, want)
     for name, got in zip(("q", "k", "v", "bias"), torch.autograd.grad(out, leaf, far["go"])):
         assert torch.equal(got, wg[name]), name
+
+
+def _crowded(count, seed, rows=(3,)):
+    """20 rows of 12 edges among 30 sources, `count` more of each of `rows` from source 4."""
+    src, row_ptr = _edges([12] * 20, 30, seed, distinct=False)
+    parts = [np.sort(np.concatenate([src[a:b], np.full(count if i in rows else 0, 4)]))
+             for i, (a, b) in enumerate(zip(row_ptr[:-1], row_ptr[1:]))]
+    return np.concatenate(parts), np.cumsum([0] + [len(x) for x in parts])
+
+
+CROWDS = [(1500, (3,)), (5000, (3,)), (20000, (17,)), (90, tuple(range(20))), (400, (0, 2, 15, 16)),
+          (13, tuple(range(16)))]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("count,rows", CROWDS)
+def test_more_parallel_edges_than_an_item_holds(dev, dtype, count, rows, bias):
+    """A column (from either side) with more edges than a part of a cut tile should have: it is cut
+    within the column, so that no sum runs over thousands of equal terms in fp32."""
+    src, row_ptr = _crowded(count, 130, rows)
+    t = _inputs(20, 30, len(src), 4, 2, 32, 48, dtype, 131, bias)
+    if bias:
+        t["bias"][row_ptr[3] + 5:row_ptr[3] + 9] = -np.inf
+    _check(dev, src, row_ptr, 30, t, dtype)
+
+
+@pytest.mark.parametrize("count,rows", CROWDS)
+def test_plan_of_crowded_columns_covers_every_edge_once(bm, dev, count, rows):
+    """As test_plan_covers_every_edge_once, and no item of more than 1024 edges."""
+    src, row_ptr = _crowded(count, 132, rows)
+    n, e = 20, len(src)
+    plan, items, parts, bad = bm.attention_plan(torch.from_numpy(row_ptr).to(dev),
+                                                torch.from_numpy(src).to(dev), None, 30, True)
+    p = plan.cpu().numpy()
+    tiles, pad = 2, lambda k: (k + 15) // 16 * 16
+    max_items = tiles + e // min(max(e // 128, 64), 512)
+    items_at = 16 + pad(tiles * 16) + 3 * pad(tiles + 1)
+    masks_at = items_at + pad(max_items * 64)
+    ids_at = masks_at + pad((e // 32 + max_items) * 16)
+    assert bad == 0 and items <= max_items
+    seen, chunk_end = np.zeros(e, int), 0
+    for rec in sorted(p[items_at:items_at + 64 * items].reshape(items, 64), key=lambda r: r[1]):
+        chunk, cols = rec[1], rec[2]
+        chunks = -(-cols // 32)
+        assert chunk >= chunk_end and chunk + chunks <= e // 32 + max_items
+        chunk_end = chunk + chunks
+        masks = p[masks_at + chunk * 16:masks_at + (chunk + chunks) * 16].view(np.uint32)
+        ids = p[ids_at + chunk * 32:ids_at + (chunk + chunks) * 32]
+        bits = (masks.reshape(chunks, 16)[:, :, None] >> np.arange(32, dtype=np.uint32)) & 1
+        bits = bits.transpose(1, 0, 2).reshape(16, chunks * 32)        # [row, column]
+        assert not bits[:, cols:].any() and (bits.sum(1) == rec[48:64]).all()
+        for r in range(16):
+            edges = np.arange(rec[32 + r], rec[32 + r] + rec[48 + r])
+            assert (src[edges] == ids[bits[r] == 1]).all()
+            if len(edges):
+                assert row_ptr[rec[16 + r]] <= edges[0] and edges[-1] < row_ptr[rec[16 + r] + 1]
+            seen[edges] += 1
+        assert rec[48:64].sum() <= 1024
+    assert (seen == 1).all()
+
+
+def test_plan_of_columns_in_no_order_is_refused(dev):
+    """Long rows whose columns do not ascend, with and without the check: the cuts, which are found by
+    searching, may come out anywhere in the row."""
+    import batmobile
+    src = torch.cat([torch.randint(0, 3, (6000,), generator=gen(133)) for _ in range(3)]).to(dev)
+    row_ptr = torch.tensor([0, 6000, 12000, 18000], device=dev)
+    with pytest.raises(ValueError, match="ascend"):
+        batmobile.AttentionPlan(src, row_ptr, 3)
