@@ -470,3 +470,38 @@ def test_infinite_and_nan_gates(dev, dtype):
     rows = [i for i in range(30) if i != 4]
     assert torch.isnan(h[4, 2, 1:4]).all() and torch.isfinite(h[rows]).all()
     assert torch.isnan(grads["gate"][4]).any() and torch.isfinite(grads["gate"][rows]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,c", [(5003, 100), (2501, 200), (2201, 400), (1301, 700), (1101, 1500)])
+def test_many_rows_of_many_channels(dev, dtype, n, c):
+    """2 to 16 waves a row, each workgroup of the backward taking two rows and more in turn."""
+    t = _inputs(n, c, dtype, n)
+    h, nn, grads = _block(dev, t)
+    rh, rn, want = ob.gated_residual_norm(*[_np(t[x]) for x in ("x", "y", "gate", "scale", "w_post",
+                                                                "w_pre")],
+                                          gh=_np(t["gh"]), gn=_np(t["gn"]))
+    assert normwise_err(_np(h), rh) <= BOUND[dtype]
+    assert normwise_err(_np(nn), rn) <= BOUND[dtype]
+    _check(grads, want, dtype)
+
+
+def test_clip_of_more_than_a_turn_of_the_workgroups(dev):
+    """70 MB of both types, every workgroup taking shares in turn, gradients and outs at odd elements;
+    the same bits as from aligned tensors."""
+    import batmobile
+    g = gen(98)
+    sizes = [(9_000_017, "f32"), (13_000_003, "bf16"), (3, "bf16"), (2_000_001, "f32")]
+    vals = [torch.randn(n, generator=g).to(TYPES[t]) for n, t in sizes]
+
+    def odd(v):
+        w = torch.empty(v.numel() + 1, dtype=v.dtype, device=dev)[1:]
+        return w.copy_(v.to(dev))
+    grads, outs = [odd(v) for v in vals], [odd(torch.zeros_like(v)) for v in vals]
+    norm, res = batmobile.clip_grad_norm(grads, 3.0, outs)
+    rn, want = ob.clip([_np(v) for v in vals], 3.0)
+    assert res is outs and abs(float(norm) - rn) <= 1e-6 * rn
+    for o, w, (_, t) in zip(outs, want, sizes):
+        assert normwise_err(_np(o), w) <= (5e-7 if t == "f32" else 4e-3)
+    norm2, aligned = batmobile.clip_grad_norm([v.to(dev) for v in vals], 3.0)
+    assert torch.equal(norm, norm2) and all(torch.equal(a, b) for a, b in zip(aligned, outs))
