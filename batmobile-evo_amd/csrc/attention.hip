@@ -100,7 +100,8 @@ __global__ __launch_bounds__(64, (KP + VP) * sizeof(T) <= 1536 ? 2 : 1) void att
     __shared__ float b_lds[BIAS ? kTileEdges + 1 : 1];
     int item, h;
     if (!attn_unit(blockIdx.x, a.side.n_items, a.H, item, h)) return;
-    const int lane = threadIdx.x, n = lane & 15, g = lane >> 4, kv = h / a.group;
+    const int lane = threadIdx.x, n = lane & 15, g = lane >> 4;
+    const int kv = uniform_quotient(h, a.group);
     const Item it(a.side, item, lane);
     const int row = it.row, steps = it.steps(kT);
     const T* kbase = (const T*)a.k + (int64_t)kv * a.Dk;

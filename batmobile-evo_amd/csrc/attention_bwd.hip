@@ -54,7 +54,8 @@ __global__ __launch_bounds__(64, 2) void attn_scores_kernel(AttnScores a) {
     __shared__ float dp_lds[kTileEdges + 1];
     int item, h;
     if (!attn_unit(blockIdx.x, a.side.n_items, a.H, item, h)) return;
-    const int lane = threadIdx.x, n = lane & 15, g = lane >> 4, kv = h / a.group;
+    const int lane = threadIdx.x, n = lane & 15, g = lane >> 4;
+    const int kv = uniform_quotient(h, a.group);
     const Item it(a.side, item, lane);
     const int row = it.row, steps = it.steps(kT);
     if (steps == 0) return;
