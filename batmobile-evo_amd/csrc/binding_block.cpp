@@ -602,31 +602,34 @@ variable_list gated_residual_norm_autograd(const Tensor& x, const OptTensor& y,
 // ---------------------------------------------------------------------------
 
 // Which outs share memory with another out, with another gradient, or with their own gradient at
-// another place: the kernels' workgroups read and write in no order, so those go through a buffer.
-// in, out: the addresses of dense tensors.
+// another place (empty: none): the kernels' workgroups read and write in no order, so those go through
+// a buffer.  in, out: the addresses of dense tensors.
 std::vector<bool> overlapping_outs(const std::vector<const void*>& in,
                                    const std::vector<void*>& out,
                                    const std::vector<int64_t>& bytes) {
     struct Range {
-        uintptr_t begin, end;
-        int64_t out;                       // -1: only read
-        bool operator<(const Range& o) const { return begin < o.begin; }
+        uintptr_t begin;
+        size_t i;                          // of a gradient, or behind those of an out
     };
+    const size_t n = in.size();
     std::vector<Range> all;
-    all.reserve(2 * in.size());
-    for (size_t i = 0; i < in.size(); ++i) {
-        const uintptr_t r = reinterpret_cast<uintptr_t>(in[i]), w = reinterpret_cast<uintptr_t>(out[i]);
+    all.reserve(2 * n);
+    for (size_t i = 0; i < n; ++i) {
         if (bytes[i] == 0) continue;
-        all.push_back({w, w + (uintptr_t)bytes[i], (int64_t)i});
-        if (w != r) all.push_back({r, r + (uintptr_t)bytes[i], -1});
+        all.push_back({reinterpret_cast<uintptr_t>(out[i]), n + i});
+        if (in[i] != out[i]) all.push_back({reinterpret_cast<uintptr_t>(in[i]), i});
     }
-    std::sort(all.begin(), all.end());
-    std::vector<bool> overlaps(in.size(), false);
+    std::sort(all.begin(), all.end(),
+              [](const Range& a, const Range& b) { return a.begin < b.begin; });
+    std::vector<bool> overlaps;
+    auto end_of = [&](size_t k) { return all[k].begin + (uintptr_t)bytes[all[k].i < n ? all[k].i : all[k].i - n]; };
     for (size_t i = 0, j; i < all.size(); i = j) {     // runs of ranges that overlap
-        uintptr_t end = all[i].end;
-        for (j = i + 1; j < all.size() && all[j].begin < end; ++j) end = std::max(end, all[j].end);
-        for (size_t k = i; j - i > 1 && k < j; ++k)
-            if (all[k].out >= 0) overlaps[all[k].out] = true;
+        uintptr_t end = end_of(i);
+        for (j = i + 1; j < all.size() && all[j].begin < end; ++j) end = std::max(end, end_of(j));
+        if (j - i == 1) continue;
+        overlaps.resize(n);
+        for (size_t k = i; k < j; ++k)
+            if (all[k].i >= n) overlaps[all[k].i - n] = true;
     }
     return overlaps;
 }
@@ -653,24 +656,24 @@ std::tuple<Tensor, std::vector<Tensor>> clip_grad_norm(
     TORCH_CHECK(grads[0].is_cuda(), "a gradient must be a CUDA tensor");
     const c10::DeviceGuard guard(grads[0].device());
     for (size_t i = 0; i < n; ++i) {
-        Tensor g = grads[i];
-        dt[i] = dtype_of(g, "a gradient");
-        TORCH_CHECK(g.device() == grads[0].device(), "the gradients must be on one device");
-        if (!g.is_non_overlapping_and_dense()) dense[i] = g = g.contiguous();
-        if (outs) {
-            const Tensor& o = (*outs)[i];
-            check_like(o, g, "out");
-            TORCH_CHECK(o.sizes() == g.sizes(), "out must have the shapes of the gradients");
-            if (o.strides() == g.strides()) into[i] = o;
+        const Tensor* g = &grads[i];
+        dt[i] = dtype_of(*g, "a gradient");
+        TORCH_CHECK(g->device() == grads[0].device(), "the gradients must be on one device");
+        if (!g->is_non_overlapping_and_dense()) dense[i] = g->contiguous(), g = &dense[i];
+        const Tensor* o = outs ? &(*outs)[i] : nullptr;
+        if (o) {
+            check_like(*o, *g, "out");
+            TORCH_CHECK(o->sizes() == g->sizes(), "out must have the shapes of the gradients");
         }
-        if (!into[i].defined()) into[i] = torch::empty_like(g);
-        in[i] = g.data_ptr(), out[i] = into[i].data_ptr(), numel[i] = g.numel();
-        bytes[i] = numel[i] * g.element_size();
+        if (!o || o->strides() != g->strides()) into[i] = torch::empty_like(*g), o = &into[i];
+        in[i] = g->data_ptr(), out[i] = o->data_ptr(), numel[i] = g->numel();
+        bytes[i] = numel[i] * (dt[i] ? 2 : 4);
     }
     if (outs) {
         const std::vector<bool> overlaps = overlapping_outs(in, out, bytes);
-        for (size_t i = 0; i < n; ++i)
-            if (overlaps[i]) into[i] = torch::empty_like(into[i]), out[i] = into[i].data_ptr();
+        for (size_t i = 0; i < overlaps.size(); ++i)
+            if (overlaps[i] && !into[i].defined())
+                into[i] = torch::empty_like((*outs)[i]), out[i] = into[i].data_ptr();
     }
     Tensor norm = torch::empty({}, grads[0].options().dtype(torch::kFloat32));
     int64_t elements = 0;
@@ -684,7 +687,7 @@ std::tuple<Tensor, std::vector<Tensor>> clip_grad_norm(
     if (!outs) return {norm, into};
     for (size_t i = 0; i < n; ++i) {
         const Tensor& o = (*outs)[i];
-        if (!o.is_same(into[i])) o.copy_(into[i]);
+        if (into[i].defined()) o.copy_(into[i]);
         // written by address: whoever saved it for a backward is told as by torch's own operators
         else if (!o.is_inference()) torch::autograd::impl::bump_version(o);
     }
