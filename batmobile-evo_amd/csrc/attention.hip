@@ -10,7 +10,7 @@
 // An edge whose b or x is -inf is left out; a row without an edge gives o = 0.
 //
 // One pass over a tile's columns (attention.h) with a running reference (the maximum, or up to 8
-// below it) and sum.  x is formed in natural units and the maximum taken off before the factor
+// below it) in m's place and the sum relative to it, which are kept for the backward.  x is formed in natural units and the maximum taken off before the factor
 // log2 e, so that a bias of the type's lowest value does not become infinite.
 #include "attention.h"
 
@@ -21,7 +21,7 @@ struct AttnFwd {
     const void *q, *k, *v;
     EdgeBias bias;
     void* out;
-    float *stats;                          // [n_dst, H, 2]
+    float *stats;                          // [n_dst, H, 2]: reference and sum
     float *part_o, *part_ml;               // [parts, H, 16, Dv], [parts, H, 16, 2]
     uint32_t qs, ks, vs;                   // rows' strides in bytes
     int H, group, Dk, Dv;
@@ -86,8 +86,8 @@ __device__ __forceinline__ void attn_fwd_rows(const AttnFwd& a, int item, int h,
 //   5000, random, 4 heads of 24 by 256 106 us   6.3 TB/s   of rows from Infinity Cache
 // Rows of k loaded straight to registers in row form, where 16 lanes ask for 16 cache lines, made an
 // earlier form take 79 us at the first size instead of 65.
-// Two waves a SIMD at least unless the tiles of k and v in f32 need more registers than that
-// leaves: 20,000 atoms, 8 heads of 256 in bf16 100 us against 122 without the bound, 5000 in f32
+// Registers for two waves a SIMD at least, unless the tiles of k and v in f32 need more than that
+// leaves (LDS holds 7 waves a CU at 256 by 256, 12 at 128 by 128): 20,000 atoms, 8 heads of 256 in bf16 100 us against 122 without the bound, 5000 in f32
 // 66 us with it against 64.
 template <typename T, int KP, int VP, bool FULL, bool BIAS, bool WIDE>
 __global__ __launch_bounds__(64, (KP + VP) * sizeof(T) <= 1536 ? 2 : 1) void attn_fwd_kernel(

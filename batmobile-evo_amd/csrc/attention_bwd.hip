@@ -4,7 +4,7 @@
 //   gb = ds,  gq[i,h] = scale sum_e ds k[j,g],  gk[j,g] = scale sum ds q[i,h],
 //   gv[j,g] = sum p go[i,h]
 //
-// with p recomputed from the rows' maxima and sums.
+// with p formed again from the rows' kept references and sums (attention.hip).
 //
 //   attn_scores  a tile and head at a time, both products of its pairs: p and dp per edge, kept
 //                in LDS, D and ds; p and ds go to the workspace, ds to gb
@@ -41,7 +41,8 @@ struct AttnScores {
 // Measured, atoms with 28 neighbours: 5000, 8 heads of 128 in f32 69 us; 20,011, 8 on 2 heads of
 // 128 in bf16 101 us (111 in steps of 32 columns), waves waiting 43 % of their time for memory
 // and 29 % for issue; 5000 with random neighbours, 4 heads of 24 by 256 in f32, 138 us (rows from
-// Infinity Cache).  The bound of two waves a SIMD gives 2 % at 128 components in bf16.
+// Infinity Cache).  Registers for two waves a SIMD give 2 % at 128 components in bf16; LDS
+// holds 9 waves a CU there, 6 at 128 in f32, 3 at 256 in f32 (less than one a SIMD).
 template <typename T, int KP, int VP, bool FULL, bool WIDE>
 __global__ __launch_bounds__(64, 2) void attn_scores_kernel(AttnScores a) {
     constexpr int kT = 1;                      // (see the kernel's head)
@@ -263,7 +264,7 @@ struct AttnSums {
 //
 // Measured, atoms with 28 neighbours, the three sums: 5000, 8 heads of 128 in f32 69 us; 20,011,
 // 8 on 2 heads of 128 in bf16 102 us, 34 % of the waves' time waiting for memory, 29 % for
-// issue.  Two waves a SIMD: a training step of 20,000 atoms, 8 heads of 256 in bf16, 369 us
+// issue.  Registers for two waves a SIMD (at 256 in bf16 with 8 bytes a lane of spill): a training step of 20,000 atoms, 8 heads of 256 in bf16, 369 us
 // against 418 without the bound; 8 heads of 64 125 against 134.
 template <typename T, int P>
 __global__ __launch_bounds__(64, 2) void attn_sum_kernel(AttnSums all) {

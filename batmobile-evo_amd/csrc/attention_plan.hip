@@ -10,8 +10,8 @@
 // A tile with many edges or a long row is cut into items of equal edge counts, each found by
 // searching for its first column, and within a column that has very many.
 //
-// Once per graph: 5000 atoms with 28 neighbours take 55 us (35 of them plan_items, whose sort is
-// steps of LDS latency and barriers), 50,000 atoms 150 us.
+// Once per graph and side: 5000 atoms with 28 neighbours take 53 us (35 of them plan_items, whose sort
+// is steps of LDS latency and barriers), 50,000 atoms 109 us.
 #include "attention.h"
 
 namespace bmhip {

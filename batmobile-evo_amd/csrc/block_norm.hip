@@ -229,8 +229,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_fwd_kernel(NormArg
 // weights' gradients in registers: part [gridDim.x, 9 C] (pre [4][C], post [4][C], scale [C]),
 // summed by norm_weights_kernel.
 //
-// Measured: 20,011 x 100 in f32 168 us, 5.0 TB/s; 50,000 x 128 in bf16 282 us; past 512 channels
-// registers spill (6250 x 1024 in f32 839 us, 512 us for the same elements at 512 channels).
+// Measured: 20,011 x 100 in f32 168 us, 5.0 TB/s; 50,000 x 128 in bf16 285 us; past 512 channels
+// registers spill (6250 x 1024 in f32 809 us, 512 us for the same elements at 512 channels).
 template <typename T, int NV, int W, bool BLOCK, bool GATE, bool PRE>
 __global__ __launch_bounds__(W <= 4 ? 256 : 64 * W) void norm_bwd_kernel(NormArgs a) {
     constexpr int kRows = W <= 4 ? 4 / W : 1;

@@ -11,7 +11,9 @@ Not a reference API.  Node features [N, C, 16] (degrees 0 to 3) pass through
 
 A head is heads' share of the channels with all their components, whose products do not change
 under rotations, so the block commutes with them.  The mixings are plain matrix products of the
-caller's torch; everything else runs in the HIP kernels.
+caller's torch; everything else runs in the HIP kernels.  The edge lengths come from the graph
+as numbers: gradients reach the features and the parameters, not the positions, so a model of this
+block alone has no forces (MACEInteraction gives those).
 """
 import math
 

@@ -499,8 +499,8 @@ int batteries_mace_backward(const float* positions, const float* box, const floa
  * should share columns), into tiles and writes the plan (batteries_attention_plan_bytes, 64-byte
  * aligned).  Its first ints are the number of items, the number of parts (items of cut tiles)
  * and 0 or what is wrong with the arrays: with check 1 row_ptr, 2 a column out of range, 4
- * columns not ascending; always 8 where the rows in this order hold more edges than n_edges (the
- * plan then has no items).  The caller reads them back into the side's n_items and n_parts.
+ * columns not ascending; without it too 8 where the rows in this order hold more edges than n_edges
+ * (the plan then has no items), and 4 where it shows in cutting a long row.  The caller reads them back into the side's n_items and n_parts.
  * n_edges < 2^29, n_rows < 2^26 - 64.
  * ------------------------------------------------------------------------- */
 typedef struct batmobile_attention_side {
@@ -541,7 +541,9 @@ int batteries_attention_edges_by_head(const float* values, const int32_t* edge_i
  * 16-byte aligned, Dk, Dv and strides multiples of 16 bytes, strides < 2^30; 3 H (n_items + 8) <
  * 2^26 on either side.  Rows need q and out, edges k and v as well (others may be NULL).  An edge
  * whose bias or logit is -inf is left out; a row without an edge gives 0.  stats [n_dst, H, 2]
- * (NULL: not kept): the maximum of x and the sum of exp(x - max), which the backward recomputes the probabilities from. */
+ * (NULL: not kept): a reference m, at most 8 below the row's maximum of x, and the sum of exp(x - m),
+ * from which the backward forms the probabilities again (the pair depends on the order of the edges,
+ * m + log(sum) does not; a row without an edge has -inf and 0). */
 size_t batteries_neighbor_attention_workspace_bytes(int64_t n_parts, int H, int Dv);
 int batteries_neighbor_attention(const void* q, const void* k, const void* v, const float* bias,
                                  const int32_t* edge_id, int bias_by_head,
