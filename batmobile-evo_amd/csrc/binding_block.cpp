@@ -1,11 +1,7 @@
 // The operators of an equivariant transformer block in the _batmobile extension (registered by
 // binding.cpp): attention over the edges of a graph, norms by degree with gate and residual,
 // gradient clipping.  No reference counterpart.  Host code only, over include/batmobile_hip.h.
-#include <c10/core/AutogradState.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/extension.h>
+#include "binding_ops.h"
 
 #include <algorithm>
 #include <cmath>
@@ -13,61 +9,16 @@
 #include <tuple>
 #include <vector>
 
-#include "batmobile_hip.h"
+using namespace bmops;
 
 namespace {
 
-using torch::Tensor;
-using OptTensor = c10::optional<Tensor>;
-
-hipStream_t stream_of(const Tensor& t) {
-    return c10::hip::getCurrentHIPStream(t.device().index()).stream();
-}
-
-void check_status(int rc, const char* what) {
-    if (rc == BATMOBILE_HIP_OK) return;
-    if (rc == BATMOBILE_HIP_ERR_ARG) TORCH_CHECK(false, what, ": invalid argument");
-    if (rc == BATMOBILE_HIP_ERR_WORKSPACE) TORCH_CHECK(false, what, ": workspace too small");
-    TORCH_CHECK(false, "HIP error in ", what, ": ", hipGetErrorString(static_cast<hipError_t>(rc)));
-}
-
-// 0 fp32, 1 bf16
-int dtype_of(const Tensor& t, const char* name) {
-    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
-    TORCH_CHECK(t.scalar_type() == torch::kFloat32 || t.scalar_type() == torch::kBFloat16, name,
-                " must be float32 or bfloat16");
-    return t.scalar_type() == torch::kBFloat16;
-}
-void check_like(const Tensor& t, const Tensor& as, const char* name) {
-    TORCH_CHECK(t.device() == as.device(), name, " must be on ", as.device());
-    TORCH_CHECK(t.scalar_type() == as.scalar_type(), name, " must have the type of the others");
-}
-void check_f32(const Tensor& t, const Tensor& as, const char* name) {
-    TORCH_CHECK(t.device() == as.device(), name, " must be on ", as.device());
-    TORCH_CHECK(t.scalar_type() == torch::kFloat32, name, " must be float32");
-}
 const int64_t* index_ptr(const Tensor& t, const Tensor& as, int64_t n, const char* name) {
     TORCH_CHECK(t.device() == as.device(), name, " must be on ", as.device());
     TORCH_CHECK(t.scalar_type() == torch::kInt64, name, " must be int64");
     TORCH_CHECK(t.is_contiguous() && t.dim() == 1, name, " must be contiguous and 1D");
     TORCH_CHECK(t.numel() == n, name, " must have ", n, " entries");
     return t.data_ptr<int64_t>();
-}
-Tensor bytes_on(const Tensor& as, size_t n) {
-    return torch::empty({(int64_t)((n + 15) / 16 * 16)},
-                        torch::TensorOptions().dtype(torch::kUInt8).device(as.device()));
-}
-
-const Tensor* ptr_of(const OptTensor& t) { return t ? &*t : nullptr; }
-// The kernels form no forward-mode derivatives: a tangent would be lost without a word, since a dual
-// tensor need not require a gradient.
-void refuse_tangent(const Tensor* t, const char* what) {
-    TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->defined() || !t->_fw_grad(/*level=*/0).defined(), what,
-                                " has no forward-mode derivative");
-}
-void refuse_tangents(std::initializer_list<const Tensor*> all, const char* what) {
-    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
-    for (const Tensor* t : all) refuse_tangent(t, what);
 }
 
 // ---------------------------------------------------------------------------
@@ -332,25 +283,12 @@ void check_features(const Tensor& x, const char* name) {
     TORCH_CHECK(x.dim() == 3 && x.size(2) == 16, name, " must be 3D [N, C, 16]");
     TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= 2048, name, " must have 1 to 2048 channels");
 }
-// contiguous and aligned for the kernels' 4-component loads
-Tensor rows4(const Tensor& t) {
-    const Tensor c = t.contiguous();
-    return reinterpret_cast<uintptr_t>(c.data_ptr()) & 15 ? c.clone(at::MemoryFormat::Contiguous)
-                                                          : c;
-}
 Tensor weight4(const Tensor& w, const Tensor& x, const char* name) {
     check_f32(w, x, name);
     TORCH_CHECK(w.dim() == 2 && w.size(0) == 4 && w.size(1) == x.size(1), name,
                 " must be [4, C]");
     return w.contiguous();
 }
-void check_same(const Tensor& t, const Tensor& x, const char* name) {
-    check_like(t, x, name);
-    TORCH_CHECK(t.sizes() == x.sizes(), name, " must have the shape of x");
-}
-void* opt_ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-float* opt_f32(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
-
 // (h, n, rs); y none: n = norm(x) alone, h undefined
 std::tuple<Tensor, Tensor, Tensor> gated_residual_norm(const Tensor& x_, const OptTensor& y_,
                                                        const OptTensor& gate_,
@@ -466,30 +404,6 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> gated_residual_norm_b
 // channels: 61 us against 83 with a node in Python, its two calls 15 us of either; attention of 39
 // atoms, 16 heads, 88 against 112; the norm of 1000 atoms without gradients 4.8 against 7.5).
 // ---------------------------------------------------------------------------
-
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-bool wants_grad(std::initializer_list<const Tensor*> all) {
-    if (!at::GradMode::is_enabled()) return false;
-    for (const Tensor* t : all)
-        if (t && t->defined() && t->requires_grad()) return true;
-    return false;
-}
-OptTensor opt_of(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
-Tensor tensor_of(const OptTensor& t) { return t ? *t : Tensor(); }
-
-// The gradients as the graph takes them: under create_graph an error waits for whoever
-// differentiates them again.
-variable_list first_order(variable_list grads, bool create_graph, const char* what) {
-    if (!create_graph) return grads;
-    for (Tensor& g : grads)
-        if (g.defined()) g = g.detach().set_requires_grad(true);
-    const auto node = std::make_shared<torch::autograd::DelayedError>(
-        std::string(what) + " is once_differentiable: its gradients have no gradients",
-        (int64_t)grads.size());
-    return node->apply(std::move(grads));
-}
 
 // A plan as the Python class holds it: both sides, (plan, items, parts), and its index arrays.
 struct PlanRef {
