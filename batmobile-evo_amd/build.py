@@ -31,7 +31,8 @@ EXT = os.path.join(PYDIR, "_batmobile" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 HIP_SOURCES = ["sh.hip", "tp.hip", "mp.hip", "nl.hip", "graph.hip", "mace.hip",
                "attention.hip", "attention_bwd.hip", "attention_plan.hip", "block_norm.hip",
-               "grad_clip.hip"]
+               "grad_clip.hip", "distance_bias.hip", "layer_norm.hip", "channel_mixing.hip",
+               "gate_activation.hip"]
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"
@@ -90,7 +91,8 @@ def build_ext(force=False):
     import torch
     from torch.utils import cpp_extension
 
-    srcs = [os.path.join(CSRC, f) for f in ("binding.cpp", "binding_block.cpp")]
+    srcs = [os.path.join(CSRC, f) for f in ("binding.cpp", "binding_block.cpp",
+                                           "binding_layers.cpp")]
     if not (force or _stale(EXT, srcs + [LIB] + _headers())):
         return EXT
     inc = cpp_extension.include_paths() + [os.path.join(ROCM, "include"), INCLUDE,
@@ -101,7 +103,7 @@ def build_ext(force=False):
              "-DTORCH_EXTENSION_NAME=_batmobile", "-DTORCH_API_INCLUDE_EXTENSION_H",
              "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-w"] + ["-I" + p for p in inc]
     objs = [os.path.join(BUILD, os.path.basename(f).replace(".cpp", ".o")) for f in srcs]
-    with cf.ThreadPoolExecutor(max_workers=2) as ex:
+    with cf.ThreadPoolExecutor(max_workers=3) as ex:
         list(ex.map(_run, [["g++"] + flags + ["-c", f, "-o", o] for f, o in zip(srcs, objs)]))
     _run(["g++", "-shared"] + objs + ["-o", EXT] + [
         "-L" + torch_lib, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python",

@@ -19,6 +19,7 @@
 #include "batmobile_hip.h"
 
 void register_block_ops(pybind11::module_& m);  // binding_block.cpp
+void register_layer_ops(pybind11::module_& m);  // binding_layers.cpp
 
 namespace {
 
@@ -1136,6 +1137,7 @@ PYBIND11_MODULE(_batmobile, m) {
           "gradient of the MACE-style layer w.r.t. positions (extension); order as for "
           "mace_forward");
     register_block_ops(m);
+    register_layer_ops(m);
     m.def("selftest_mfma_16x16x4", &selftest_mfma_16x16x4, py::arg("A"), py::arg("B"),
           "D = A @ B through one v_mfma_f32_16x16x4f32 (lane-layout self test)");
     m.def("selftest_mfma_4x4x1_bcast", &selftest_mfma_4x4x1_bcast, py::arg("A"), py::arg("B"),

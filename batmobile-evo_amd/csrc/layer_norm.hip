@@ -1,0 +1,358 @@
+// Layer norm of rows (no reference counterpart): x [rows, D], elements `step` apart,
+//
+//   m = mean x,  r = (mean (x - m)^2 + eps)^-1/2,  xh = (x - m) r,  y = xh w + b
+//   gx = r (u - mean u - xh mean(u xh)),  u = g w;   gw = sum over rows of g xh,  gb = sum g
+//
+// Memory bound: a row is read once each way into the registers of its lanes; the variance is that of
+// the differences from the mean, and the backward forms m and r again from the row, which costs
+// lane sums but no memory.  Sums are fp32.  A row of few elements takes a part of a wave, a long one up
+// to 16 waves.
+#include "sums.h"
+#include "batmobile_hip.h"
+
+namespace bmhip {
+
+constexpr int kLnMaxD = 8192;
+
+struct LnArgs {
+    const void *x, *g;
+    const float *w, *b;
+    void *y, *gx;
+    float* part;
+    int64_t rows, row_stride, step;
+    int D;
+    float eps, inv;                        // inv: 1 / D
+};
+
+// VEC elements in 16 bytes (or one element) as fp32
+template <typename T, int VEC>
+struct LnVec {
+    float v[VEC];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (VEC == 1) {
+            v[0] = norm_ld(p);
+        } else if constexpr (sizeof(T) == 4) {
+            const float4 t = *reinterpret_cast<const float4*>(p);
+            v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+        } else {
+            const uint4 t = *reinterpret_cast<const uint4*>(p);
+            v[0] = bf16_lo(t.x), v[1] = bf16_hi(t.x), v[2] = bf16_lo(t.y), v[3] = bf16_hi(t.y);
+            v[4] = bf16_lo(t.z), v[5] = bf16_hi(t.z), v[6] = bf16_lo(t.w), v[7] = bf16_hi(t.w);
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (VEC == 1) {
+            norm_st(p, v[0]);
+        } else if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+            *reinterpret_cast<uint4*>(p) = make_uint4(bf16_pack(v[0], v[1]), bf16_pack(v[2], v[3]),
+                                                      bf16_pack(v[4], v[5]), bf16_pack(v[6], v[7]));
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = 0.0f;
+    }
+};
+
+// Sum over a row: LPR lanes, or W whole waves (every thread of the workgroup takes part)
+template <int LPR, int W>
+__device__ __forceinline__ float ln_sum(float v, float* sh, int& turn) {
+    v = lanes_sum<LPR>(v);
+    if constexpr (W > 1) {
+        float* s = sh + turn * 16;
+        turn ^= 1;
+        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) v += s[i];
+    }
+    return v;
+}
+
+// Takes the mean m off a lane's part of a row and returns r.  The rounding of m, which is large next to
+// the differences of a row far from 0, shows in the differences' own mean: that is taken off as well.
+template <int LPR, int W, typename T, int VEC, int NV>
+__device__ __forceinline__ float ln_center(const LnArgs& a, int t, float m, LnVec<T, VEC> (&x)[NV],
+                                           float* sh, int& turn) {
+    constexpr int kLanes = W == 1 ? LPR : 64 * W;
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if ((i * kLanes + t) * VEC < a.D) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                x[i].v[j] -= m;
+                s1 += x[i].v[j];
+                s2 = fmaf(x[i].v[j], x[i].v[j], s2);
+            }
+        }
+    s1 = ln_sum<LPR, W>(s1, sh, turn) * a.inv;
+    s2 = ln_sum<LPR, W>(s2, sh, turn) * a.inv;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if ((i * kLanes + t) * VEC < a.D) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) x[i].v[j] -= s1;
+        }
+    return 1.0f / sqrtf(fmaxf(fmaf(-s1, s1, s2), 0.0f) + a.eps);
+}
+
+template <int W>
+constexpr int ln_threads() { return W == 1 ? 256 : 64 * W; }
+
+// A lane's part of a row: NV vectors, LPR * W vectors apart
+template <typename T, int VEC, int NV, int LPR, int W, int ROWS>
+__global__ __launch_bounds__(ln_threads<W>()) void ln_fwd_kernel(LnArgs a) {
+    __shared__ float sh[2 * 16];
+    int turn = 0;
+    constexpr int kGroups = W == 1 ? 4 * (64 / LPR) : 1, kLanes = W == 1 ? LPR : 64 * W;
+    const int t = W == 1 ? threadIdx.x % LPR : threadIdx.x;
+    const int group = W == 1 ? threadIdx.x / LPR : 0;
+    const int64_t row0 = (int64_t)blockIdx.x * kGroups * ROWS + group;
+    LnVec<T, VEC> x[ROWS][NV];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+        const int64_t row = min(row0 + k * kGroups, a.rows - 1);
+        const T* p = (const T*)a.x + row * a.row_stride;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * kLanes + t) * VEC;
+            if (c < a.D) x[k][i].load(p + (VEC == 1 ? c * a.step : c));
+            else x[k][i].zero();
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+        const int64_t row = row0 + k * kGroups;
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) s += x[k][i].v[j];
+        const float m = ln_sum<LPR, W>(s, sh, turn) * a.inv;
+        const float r = ln_center<LPR, W>(a, t, m, x[k], sh, turn);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * kLanes + t) * VEC;
+            if (c < a.D && row < a.rows) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    x[k][i].v[j] = fmaf(x[k][i].v[j] * r, a.w[c + j], a.b ? a.b[c + j] : 0.0f);
+                x[k][i].store((T*)a.y + row * a.D + c);
+            }
+        }
+    }
+}
+
+// Workgroups take rows in turn; a lane keeps its columns' sums of g xh and g in registers, which are
+// joined over the workgroup's rows at the end: part [gridDim.x, 2, D].
+template <typename T, int VEC, int NV, int LPR, int W>
+__global__ __launch_bounds__(ln_threads<W>()) void ln_bwd_kernel(LnArgs a) {
+    __shared__ float sh[2 * 16];
+    constexpr int kCols = NV * LPR * VEC;
+    __shared__ float red[W == 1 ? 4 * kCols : 1];
+    int turn = 0;
+    constexpr int kGroups = W == 1 ? 4 * (64 / LPR) : 1, kLanes = W == 1 ? LPR : 64 * W;
+    const int t = W == 1 ? threadIdx.x % LPR : threadIdx.x;
+    const int group = W == 1 ? threadIdx.x / LPR : 0;
+    float gw[NV][VEC], gb[NV][VEC];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) gw[i][j] = gb[i][j] = 0.0f;
+    for (int64_t row0 = (int64_t)blockIdx.x * kGroups; row0 < a.rows;
+         row0 += (int64_t)gridDim.x * kGroups) {
+        const bool there = row0 + group < a.rows;
+        const int64_t row = there ? row0 + group : a.rows - 1;
+        LnVec<T, VEC> x[NV], g[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * kLanes + t) * VEC;
+            x[i].zero();
+            g[i].zero();
+            if (c < a.D && there) {
+                x[i].load((const T*)a.x + row * a.row_stride + (VEC == 1 ? c * a.step : c));
+                g[i].load((const T*)a.g + row * a.D + c);
+            }
+        }
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) s += x[i].v[j];
+        const float m = ln_sum<LPR, W>(s, sh, turn) * a.inv;
+        const float r = ln_center<LPR, W>(a, t, m, x, sh, turn);
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * kLanes + t) * VEC;
+            if (c < a.D) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float xh = x[i].v[j] * r;
+                    gw[i][j] = fmaf(g[i].v[j], xh, gw[i][j]);
+                    gb[i][j] += g[i].v[j];
+                    x[i].v[j] = xh;
+                    g[i].v[j] *= a.w[c + j];
+                    s1 += g[i].v[j];
+                    s2 = fmaf(g[i].v[j], xh, s2);
+                }
+            }
+        }
+        s1 = ln_sum<LPR, W>(s1, sh, turn) * a.inv;
+        s2 = ln_sum<LPR, W>(s2, sh, turn) * a.inv;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * kLanes + t) * VEC;
+            if (c < a.D && there) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    g[i].v[j] = r * (g[i].v[j] - s1 - x[i].v[j] * s2);
+                g[i].store((T*)a.gx + row * a.D + c);
+            }
+        }
+    }
+    float* part = a.part + (int64_t)blockIdx.x * 2 * a.D;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        if constexpr (W == 1) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                float v = k ? gb[i][j] : gw[i][j];
+                if constexpr (W == 1) {
+#pragma unroll
+                    for (int o = LPR; o < 64; o <<= 1) v += __shfl_xor(v, o);
+                    if ((threadIdx.x & 63) < LPR)
+                        red[(threadIdx.x >> 6) * kCols + (i * LPR + t) * VEC + j] = v;
+                } else {
+                    const int c = (i * kLanes + t) * VEC + j;
+                    if (c < a.D) part[k * a.D + c] = v;
+                }
+            }
+        if constexpr (W == 1) {
+            __syncthreads();
+            for (int c = threadIdx.x; c < a.D; c += 256)
+                part[k * a.D + c] = (red[c] + red[kCols + c]) + (red[2 * kCols + c] + red[3 * kCols + c]);
+        }
+    }
+}
+
+__global__ __launch_bounds__(1024) void ln_weights_kernel(const float* part, int rows, int D,
+                                                          float* gw, float* gb) {
+    const int col = blockIdx.x * 16 + (threadIdx.x & 15);
+    const bool there = col < (gb ? 2 * D : D);
+    const float s =
+        column_sum(there ? rows : 0, [&](int r) { return part[(int64_t)r * 2 * D + col]; });
+    if (threadIdx.x < 16 && there) {
+        if (col < D) gw[col] = s;
+        else gb[col - D] = s;
+    }
+}
+
+// Workgroups of the backward: enough to fill the card, and few enough that the partial sums stay a
+// small part of the data
+static int ln_parts(int64_t rows, int D) {
+    const int64_t groups = D <= 64 ? 8 : D <= 256 ? 4 : 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, 8 * groups), 1024));
+}
+
+template <typename T, int VEC, int NV, int LPR, int W>
+static void ln_launch(const LnArgs& a, bool bwd, hipStream_t s) {
+    constexpr int kGroups = W == 1 ? 4 * (64 / LPR) : 1;
+    constexpr int kRows = W > 1 ? 1 : NV * VEC <= 8 ? 4 : NV * VEC <= 16 ? 2 : 1;
+    if (bwd) {
+        ln_bwd_kernel<T, VEC, NV, LPR, W><<<ln_parts(a.rows, a.D), ln_threads<W>(), 0, s>>>(a);
+        return;
+    }
+    constexpr int64_t kMost = (int64_t)1 << 20;     // workgroups of a launch
+    LnArgs b = a;
+    for (int64_t row = 0; row < a.rows; row += kMost * kGroups * kRows) {
+        b.x = (const T*)a.x + row * a.row_stride;
+        b.y = (T*)a.y + row * a.D;
+        b.rows = std::min(a.rows - row, kMost * kGroups * kRows);
+        ln_fwd_kernel<T, VEC, NV, LPR, W, kRows>
+            <<<(unsigned)ceil_div(b.rows, kGroups * kRows), ln_threads<W>(), 0, s>>>(b);
+    }
+}
+
+template <typename T, int VEC>
+static void ln_pick(const LnArgs& a, bool bwd, hipStream_t s) {
+    const int units = (a.D + VEC - 1) / VEC;
+    if (units <= 8) ln_launch<T, VEC, 1, 8, 1>(a, bwd, s);
+    else if (units <= 16) ln_launch<T, VEC, 1, 16, 1>(a, bwd, s);
+    else if (units <= 32) ln_launch<T, VEC, 1, 32, 1>(a, bwd, s);
+    else if (units <= 64) ln_launch<T, VEC, 1, 64, 1>(a, bwd, s);
+    else if (units <= 128) ln_launch<T, VEC, 2, 64, 1>(a, bwd, s);
+    else if (units <= 256) ln_launch<T, VEC, 4, 64, 1>(a, bwd, s);
+    else if (units <= 512) ln_launch<T, VEC, 2, 64, 4>(a, bwd, s);
+    else if (units <= 1024) ln_launch<T, VEC, 4, 64, 4>(a, bwd, s);
+    else if constexpr (kLnMaxD / VEC > 1024) {
+        if (units <= 2048) ln_launch<T, VEC, 2, 64, 16>(a, bwd, s);
+        else if constexpr (kLnMaxD / VEC > 2048) ln_launch<T, VEC, 8, 64, 16>(a, bwd, s);
+    }
+}
+
+template <typename T>
+static void ln_run(const LnArgs& a, bool bwd, hipStream_t s) {
+    constexpr int VEC = 16 / sizeof(T);
+    const bool vec = a.D % VEC == 0 && a.step == 1 && (a.row_stride % VEC == 0 || a.rows <= 1) &&
+                     aligned_to({a.x, a.g, a.y, a.gx}, 16);
+    if (vec) ln_pick<T, VEC>(a, bwd, s);
+    else ln_pick<T, 1>(a, bwd, s);
+}
+
+static bool ln_shape_ok(int64_t rows, int D, int dtype) {
+    return rows >= 0 && rows < ((int64_t)1 << 38) && D >= 1 && D <= kLnMaxD &&
+           (dtype == 0 || dtype == 1);
+}
+}  // namespace bmhip
+
+using namespace bmhip;
+
+extern "C" int batteries_layer_norm(const void* x, const float* weight, const float* bias, void* y,
+                                    int64_t rows, int D, int64_t row_stride, int64_t step, float eps,
+                                    int dtype, hipStream_t stream) {
+    if (!ln_shape_ok(rows, D, dtype) || !weight || (rows > 0 && (!x || !y)) || !(eps >= 0.0f))
+        return BM_ERR_ARG;
+    if (!aligned_to({x, y}, dtype == 0 ? 4 : 2)) return BM_ERR_ARG;
+    if (rows == 0) return BM_OK;
+    LnArgs a{};
+    a.x = x; a.w = weight; a.b = bias; a.y = y; a.rows = rows; a.row_stride = row_stride;
+    a.step = step; a.D = D; a.eps = eps; a.inv = 1.0f / (float)D;
+    if (dtype == 0) ln_run<float>(a, false, stream);
+    else ln_run<uint16_t>(a, false, stream);
+    return (int)hipGetLastError();
+}
+
+extern "C" size_t batteries_layer_norm_backward_workspace_bytes(int64_t rows, int D) {
+    if (!ln_shape_ok(rows, D, 0)) return 0;
+    return (size_t)ln_parts(rows, D) * 2 * D * sizeof(float);
+}
+
+extern "C" int batteries_layer_norm_backward(const void* x, const float* weight, const void* g,
+                                             void* gx, float* gweight, float* gbias, int64_t rows,
+                                             int D, int64_t row_stride, int64_t step, float eps,
+                                             int dtype, void* workspace, size_t workspace_bytes,
+                                             hipStream_t stream) {
+    if (!ln_shape_ok(rows, D, dtype) || !weight || !gweight || (rows > 0 && (!x || !g || !gx)) ||
+        !(eps >= 0.0f))
+        return BM_ERR_ARG;
+    if (!aligned_to({x, g, gx}, dtype == 0 ? 4 : 2)) return BM_ERR_ARG;
+    if (workspace_bytes < batteries_layer_norm_backward_workspace_bytes(rows, D) || !workspace)
+        return BM_ERR_WORKSPACE;
+    LnArgs a{};
+    a.x = x; a.w = weight; a.g = g; a.gx = gx; a.part = (float*)workspace; a.rows = rows;
+    a.row_stride = row_stride; a.step = step; a.D = D; a.eps = eps; a.inv = 1.0f / (float)D;
+    if (rows > 0) {
+        if (dtype == 0) ln_run<float>(a, true, stream);
+        else ln_run<uint16_t>(a, true, stream);
+    }
+    ln_weights_kernel<<<(unsigned)ceil_div(gbias ? 2 * D : D, 16), 1024, 0, stream>>>(
+        a.part, rows > 0 ? ln_parts(rows, D) : 0, D, gweight, gbias);
+    return (int)hipGetLastError();
+}

@@ -8,7 +8,8 @@ names, re-exported from the compiled extension, plus the autograd wrappers.
 - Fused SH + tensor product, with scatter-add into destination nodes
 - CSR conversion and cell-list neighbor lists
 - Equivariant transformer blocks: attention over a graph's edges, norms by degree with gate and
-  residual, gradient clipping
+  residual, gradient clipping; a learned bias by distance, layer norm, channel mixing and gated
+  activation with 8-bit checkpoints
 
 There is no CPU fallback: importing this package without the built extension
 raises ImportError.
@@ -66,6 +67,15 @@ from .mace import MACEInteraction, MaceLayerFunction  # noqa: E402
 from .attention import AttentionPlan, neighbor_attention  # noqa: E402
 from .block_norm import equivariant_norm, gated_residual_norm  # noqa: E402
 from .grad_clip import clip_grad_norm, clip_grad_norm_  # noqa: E402
+from .distance_bias import distance_bias  # noqa: E402
+from .layer_norm import layer_norm  # noqa: E402
+from .feed_forward import (  # noqa: E402
+    FeedForwardBlock,
+    channel_mixing,
+    checkpoint_decode,
+    checkpoint_encode,
+    gate_activation,
+)
 from .attention_block import AttentionBlock  # noqa: E402
 
 # Autograd-compatible wrappers (reference __init__.py:35-44)
@@ -125,4 +135,11 @@ __all__ = [
     "clip_grad_norm",
     "clip_grad_norm_",
     "AttentionBlock",
+    "distance_bias",
+    "layer_norm",
+    "channel_mixing",
+    "gate_activation",
+    "checkpoint_encode",
+    "checkpoint_decode",
+    "FeedForwardBlock",
 ]

@@ -604,6 +604,89 @@ int batteries_clip_grad_norm(const void* const* in, void* const* out, const int6
                              void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Learned bias of attention by distance (no reference counterpart)
+ *
+ *   bias[e, h] = table[k, h] + log max(0, 1 - (r / cutoff)^2),   r = lengths[e],
+ *   k = number of boundaries <= r
+ * lengths [E], boundaries [B - 1] ascending (any values give a bucket in [0, B)), table [B, H], bias
+ * [E, H], all fp32; cutoff 0: without the second term, which from the cutoff on is -inf.  A length
+ * that is NaN gives NaN.  buckets [E] (NULL: not kept) takes k for the backward.  B <= 4096,
+ * H <= 1024, E < 2^38.
+ * ------------------------------------------------------------------------- */
+int batteries_distance_bias(const float* lengths, const float* boundaries, const float* table,
+                            float* bias, uint16_t* buckets, int64_t E, int H, int B, float cutoff,
+                            hipStream_t stream);
+/* gtable [B, H] (NULL: not wanted; it needs buckets and the workspace) and glengths [E] (NULL: not
+ * wanted; 0 without a cutoff and from the cutoff on) from g [E, H].  Sums have a fixed order. */
+size_t batteries_distance_bias_backward_workspace_bytes(int64_t E, int H, int B);
+int batteries_distance_bias_backward(const float* lengths, const uint16_t* buckets, const float* g,
+                                     float* gtable, float* glengths, int64_t E, int H, int B,
+                                     float cutoff, void* workspace, size_t workspace_bytes,
+                                     hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Layer norm of rows (no reference counterpart)
+ *
+ *   y = (x - mean) / sqrt(mean of (x - mean)^2 + eps) * weight + bias
+ * x: `rows` rows of D elements in fp32 (dtype 0) or bf16 (dtype 1), at row_stride, the elements of a
+ * row `step` apart (both in elements); y dense, weight [D] and bias [D] (NULL: 0) fp32.
+ * D <= 8192, rows < 2^38.  Rows of whole 16-byte units at such strides and addresses are read 16
+ * bytes a lane, others element by element.
+ * ------------------------------------------------------------------------- */
+int batteries_layer_norm(const void* x, const float* weight, const float* bias, void* y, int64_t rows,
+                         int D, int64_t row_stride, int64_t step, float eps, int dtype,
+                         hipStream_t stream);
+/* gx (dense), gweight and gbias (NULL: not wanted) from g (dense); the rows' means are formed again. */
+size_t batteries_layer_norm_backward_workspace_bytes(int64_t rows, int D);
+int batteries_layer_norm_backward(const void* x, const float* weight, const void* g, void* gx,
+                                  float* gweight, float* gbias, int64_t rows, int D,
+                                  int64_t row_stride, int64_t step, float eps, int dtype,
+                                  void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Activations in 8 bits (no reference counterpart)
+ *
+ * Features x [N, C, 16] as codes [N, C, 16] (e4m3, no infinities, largest 448) and exps
+ * [N, ceil(C / 8)]: the 8 channels x 16 components of a block share 2^(exps - 127), the least power
+ * with max |x| <= 448 times it, within [2^-110, 2^120]; codes are rounded to nearest even.  A value
+ * that is not finite becomes NaN and has no part in the maximum; what would round to 2^128 becomes
+ * 240 * 2^120.  fp32 (dtype 0) or bf16 (dtype 1);
+ * x 16-byte, codes 8-byte aligned; C <= 2048, N ceil(C / 8) < 2^31.
+ * ------------------------------------------------------------------------- */
+int batteries_checkpoint_encode(const void* x, uint8_t* codes, uint8_t* exps, int64_t N, int C,
+                                int dtype, hipStream_t stream);
+int batteries_checkpoint_decode(const uint8_t* codes, const uint8_t* exps, void* x, int64_t N, int C,
+                                int dtype, hipStream_t stream);
+
+/* Gated activation: y[n, c, m] = sigmoid(x[n, c, 0]) x[n, c, m]; codes and exps (NULL: not kept) take
+ * the 8-bit form of x.  The backward takes x, or with x NULL its 8-bit form.  Limits as above. */
+int batteries_gate_activation(const void* x, void* y, uint8_t* codes, uint8_t* exps, int64_t N, int C,
+                              int dtype, hipStream_t stream);
+int batteries_gate_activation_backward(const void* x, const uint8_t* codes, const uint8_t* exps,
+                                       const void* g, void* gx, int64_t N, int C, int dtype,
+                                       hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Channels mixed degree by degree (no reference counterpart)
+ *
+ *   y[n, o, m] = sum_c x[n, c, m] weight[l(m), c, o],  l(m) the degree of component m
+ * x [N, C, 16] to y [N, O, 16] in fp32 (dtype 0) or bf16 (dtype 1), 16-byte aligned, weight
+ * [4, C, O] fp32; transposed: x [N, O, 16] to y [N, C, 16], the sum over o.  fp32 accuracy of the
+ * products in fp32; with bf16 features the weight is rounded to 16 bits of mantissa.  C, O <= 2048,
+ * N < 2^31.
+ * ------------------------------------------------------------------------- */
+size_t batteries_channel_mixing_workspace_bytes(int C, int O, int transposed, int dtype);
+int batteries_channel_mixing(const void* x, const float* weight, void* y, int64_t N, int C, int O,
+                             int transposed, int dtype, void* workspace, size_t workspace_bytes,
+                             hipStream_t stream);
+/* gweight [4, C, O] fp32 from g [N, O, 16] and x, or with x NULL its 8-bit form. */
+size_t batteries_channel_mixing_weight_grad_workspace_bytes(int64_t N, int C, int O);
+int batteries_channel_mixing_weight_grad(const void* x, const uint8_t* codes, const uint8_t* exps,
+                                         const void* g, float* gweight, int64_t N, int C, int O,
+                                         int dtype, void* workspace, size_t workspace_bytes,
+                                         hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Self test (no reference counterpart): D[16,16] = A[16,4] B[4,16] through one
  * v_mfma_f32_16x16x4f32 with the lane layout the kernels above assume.
  * ------------------------------------------------------------------------- */
