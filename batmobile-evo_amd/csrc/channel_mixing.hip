@@ -6,7 +6,7 @@
 //   gW[l, c, o] = sum_n sum_{m of degree l} x[n, c, m] g[n, o, m]  (x as it was, or from its 8-bit form)
 //
 // All on the bf16 matrix cores with fp32 sums.  fp32 features and weights go in three parts and six
-// products, as exact as fp32 products; the fp32 weight of bf16 features goes in two (off by 2^-16 of it
+// products, as exact as fp32 products; the fp32 weight of bf16 features goes in two (off by 2^-15 of it
 // at most), bf16 features in one, which is exact; an 8-bit form is exact in bf16, so against it only g is
 // split.
 //
@@ -69,17 +69,6 @@ struct Mix8<uint16_t> {
     }
 };
 
-// 0xffff in the halves of p that are infinite
-__device__ __forceinline__ unsigned mix_infinity(unsigned p) {
-    return ((p & 0x7fff0000u) == 0x7f800000u ? 0xffff0000u : 0u) |
-           ((p & 0x7fffu) == 0x7f80u ? 0xffffu : 0u);
-}
-__device__ __forceinline__ unsigned mix_max(unsigned a, unsigned b) {
-    typedef unsigned short v2s __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(v2s, a),
-                                                                  __builtin_bit_cast(v2s, b)));
-}
-
 // acc += A B in the products that PA and PB parts need, the small ones first
 template <int PA, int PB>
 __device__ __forceinline__ v4f mix_mfma(const v4u* a, const v4u* b, v4f acc) {
@@ -91,6 +80,18 @@ __device__ __forceinline__ v4f mix_mfma(const v4u* a, const v4u* b, v4f acc) {
             if (j >= 0 && j < PB) acc = mfma_bf16(a[i], b[j], acc);
         }
     return acc;
+}
+
+// v in two parts of one sign, the leading bits (upper half of the result) and the rest (lower half, to
+// nearest).  A feature's infinity then ends as one of the same sign in both products; so that it does where
+// nothing is left over, the least number of that sign stands in for it.  An infinite v is all in the
+// first part.
+__device__ __forceinline__ unsigned mix_two_parts(float v) {
+    const unsigned bits = __float_as_uint(v), h = bits & 0xffff0000u;
+    if (v != v) return 0x7fc00000u;
+    unsigned m = bf16_pack(v - __uint_as_float(h), 0.0f) & 0xffffu;
+    if ((m & 0x7fffu) == 0 || (m & 0x7fffu) >= 0x7f80u) m = v == 0.0f ? 0u : (h >> 16 & 0x8000u) | 1u;
+    return h | m;
 }
 
 // W (element W[l][k][m] at l K M + k sk + m sm) as the matrix operands of its parts: 16 bytes a lane,
@@ -109,15 +110,20 @@ __global__ __launch_bounds__(256) void mix_pack_kernel(const float* __restrict__
         const int k = step * 32 + 4 * j + q;
         v[j] = k < K && m < M ? w[(int64_t)l * K * M + (int64_t)k * sk + (int64_t)m * sm] : 0.0f;
     }
-    Bf3 s = bf16_split8(v);
-    if constexpr (PW < 3) {                // an infinity, which the split has in its last part
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s.h[j] |= mix_infinity(s.l[j]) & s.l[j];
-    }
     v4u* p = out + (int64_t)(i >> 6) * PW * 64 + lane;
-    p[0] = s.h;
-    p[64] = s.m;
-    if constexpr (PW > 2) p[128] = s.l;
+    if constexpr (PW == 3) {
+        const Bf3 s = bf16_split8(v);
+        p[0] = s.h, p[64] = s.m, p[128] = s.l;
+    } else {
+        v4u h, m;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned a = mix_two_parts(v[2 * j]), b = mix_two_parts(v[2 * j + 1]);
+            h[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            m[j] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+        }
+        p[0] = h, p[64] = m;
+    }
 }
 
 struct MixArgs {
@@ -185,47 +191,21 @@ __global__ __launch_bounds__(512) void mix_kernel(MixArgs a) {
             x.template operand<3>(f[3][k]);
         }
         const v4u* w = a.w + (int64_t)(s * 4 * a.tiles + tile0) * PW * 64 + lane;
-        auto products = [&](auto infinite) {
 #pragma unroll
-            for (int o = 0; o < OT; ++o) {
-                v4u w0[PW], w1[PW];
+        for (int o = 0; o < OT; ++o) {
+            v4u w0[PW], w1[PW];
 #pragma unroll
-                for (int p = 0; p < PW; ++p) {
-                    w0[p] = w[((int64_t)d0 * a.tiles + o) * PW * 64 + p * 64];
-                    w1[p] = w[((int64_t)d1 * a.tiles + o) * PW * 64 + p * 64];
-                }
-#pragma unroll
-                for (int k = 0; k < NT; ++k)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const v4u* wi = i ? w1 : w0;
-                        if constexpr (decltype(infinite)::value) {
-                            v4u g = f[i][k][0];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) g[j] &= ~mix_infinity(g[j]);
-                            acc[i][k][o] = mfma_bf16(wi[1], g, acc[i][k][o]);
-                            acc[i][k][o] = mfma_bf16(wi[0], f[i][k][0], acc[i][k][o]);
-                        } else {
-                            acc[i][k][o] = mix_mfma<PW, PX>(wi, f[i][k], acc[i][k][o]);
-                        }
-                    }
+            for (int p = 0; p < PW; ++p) {
+                w0[p] = w[((int64_t)d0 * a.tiles + o) * PW * 64 + p * 64];
+                w1[p] = w[((int64_t)d1 * a.tiles + o) * PW * 64 + p * 64];
             }
-        };
-        if constexpr (PX == 1) {
-            // an infinite feature meets the weight's first part alone: with the second, of any sign or 0,
-            // it would end as NaN (fp32 features have it in a part that meets one part only)
-            unsigned top = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int k = 0; k < NT; ++k) {
+                acc[0][k][o] = mix_mfma<PW, PX>(w0, f[0][k], acc[0][k][o]);
 #pragma unroll
-                for (int k = 0; k < NT; ++k)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) top = mix_max(top, f[i][k][0][j] & 0x7fff7fffu);
-            const bool any = max(top >> 16, top & 0xffffu) >= 0x7f80u;
-            if (__builtin_expect(__any(any), 0)) products(std::true_type{});
-            else products(std::false_type{});
-        } else {
-            products(std::false_type{});
+                for (int i = 1; i < 4; ++i)
+                    acc[i][k][o] = mix_mfma<PW, PX>(w1, f[i][k], acc[i][k][o]);
+            }
         }
     }
     // the four waves' components of 16 atoms x 16 outputs together, and out as whole lines
