@@ -17,6 +17,7 @@
 // channels, so a cache line is read by all of them at about the same time, and a wave meets two
 // degrees at most.  The order of the sum is free as long as both operands have the same one: value j of lane
 // group q is channel (atom) 4 j + q, so that a load covers neighbours.
+#include <atomic>
 #include <type_traits>
 
 #include "checkpoint.h"
@@ -26,6 +27,9 @@
 namespace bmhip {
 
 constexpr int kMixMaxC = 2048;
+// channels up to which the weight stays in registers
+template <typename T>
+constexpr int kStayMost = sizeof(T) == 4 ? 64 : 256;
 constexpr int kMixFar = 0x7fffff00;        // a buffer offset past every buffer here: reads 0
 
 // degrees of a wave's first component and of its other three
@@ -42,6 +46,7 @@ struct Mix8<float> {
     __device__ __forceinline__ void load(int j, __amdgpu_buffer_rsrc_t b, int off) {
         r[j] = buffer_ld4(b, off, 0);
     }
+    __device__ __forceinline__ void zero(int j) { r[j] = make_float4(0, 0, 0, 0); }
     template <int I>
     __device__ __forceinline__ void operand(v4u* f) const {
         float v[8];
@@ -60,6 +65,7 @@ struct Mix8<uint16_t> {
         const auto v = __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, 0);
         r[j][0] = v[0], r[j][1] = v[1];
     }
+    __device__ __forceinline__ void zero(int j) { r[j][0] = r[j][1] = 0; }
     template <int I>
     __device__ __forceinline__ void operand(v4u* f) const {
         constexpr unsigned kSel = I % 2 ? 0x07060302u : 0x05040100u;
@@ -87,11 +93,28 @@ __device__ __forceinline__ v4f mix_mfma(const v4u* a, const v4u* b, v4f acc) {
 // nothing is left over, the least number of that sign stands in for it.  An infinite v is all in the
 // first part.
 __device__ __forceinline__ unsigned mix_two_parts(float v) {
-    const unsigned bits = __float_as_uint(v), h = bits & 0xffff0000u;
-    if (v != v) return 0x7fc00000u;
-    unsigned m = bf16_pack(v - __uint_as_float(h), 0.0f) & 0xffffu;
-    if ((m & 0x7fffu) == 0 || (m & 0x7fffu) >= 0x7f80u) m = v == 0.0f ? 0u : (h >> 16 & 0x8000u) | 1u;
-    return h | m;
+    const unsigned h = __float_as_uint(v) & 0xffff0000u;
+    const unsigned m = bf16_pack(v - __uint_as_float(h), 0.0f) & 0xffffu;
+    const unsigned least = v == 0.0f ? 0u : (h >> 16 & 0x8000u) | 1u;
+    // (nothing left over, or an infinite v)
+    const unsigned rest = (m & 0x7fffu) - 1u >= 0x7f7fu ? least : m;
+    return v != v ? 0x7fc00000u : h | rest;
+}
+
+// Eight fp32 values as the operands of their parts
+template <int PW>
+__device__ __forceinline__ void mix_split(const float* v, v4u* p) {
+    if constexpr (PW == 3) {
+        const Bf3 s = bf16_split8(v);
+        p[0] = s.h, p[1] = s.m, p[2] = s.l;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned a = mix_two_parts(v[2 * j]), b = mix_two_parts(v[2 * j + 1]);
+            p[0][j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            p[1][j] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+        }
+    }
 }
 
 // W (element W[l][k][m] at l K M + k sk + m sm) as the matrix operands of its parts: 16 bytes a lane,
@@ -110,31 +133,23 @@ __global__ __launch_bounds__(256) void mix_pack_kernel(const float* __restrict__
         const int k = step * 32 + 4 * j + q;
         v[j] = k < K && m < M ? w[(int64_t)l * K * M + (int64_t)k * sk + (int64_t)m * sm] : 0.0f;
     }
-    v4u* p = out + (int64_t)(i >> 6) * PW * 64 + lane;
-    if constexpr (PW == 3) {
-        const Bf3 s = bf16_split8(v);
-        p[0] = s.h, p[64] = s.m, p[128] = s.l;
-    } else {
-        v4u h, m;
+    v4u f[PW];
+    mix_split<PW>(v, f);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const unsigned a = mix_two_parts(v[2 * j]), b = mix_two_parts(v[2 * j + 1]);
-            h[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-            m[j] = __builtin_amdgcn_perm(b, a, 0x05040100u);
-        }
-        p[0] = h, p[64] = m;
-    }
+    for (int p = 0; p < PW; ++p) out[((int64_t)(i >> 6) * PW + p) * 64 + lane] = f[p];
 }
 
 struct MixArgs {
     const void *x, *g;
     const uint8_t *codes, *exps;
-    const v4u* w;
+    const v4u* w;                          // in parts (mix_pack_kernel)
+    const float* weight;                   // as given: element l K M + k sk + m sm
+    int sk, sm;
     void* y;
     float* part;
     int64_t n;
     int K, M;                              // channels in, out
-    int tiles, chunks, groups;             // tiles of 16 outputs (padded), chunks of them; waves / 4
+    int tiles, chunks;                     // tiles of 16 outputs (padded), chunks of them
     int64_t units;                         // workgroups of atoms
     int splits, per_split;                 // gW: ranges of atoms, steps of 32 atoms in one
 };
@@ -150,23 +165,54 @@ __device__ __forceinline__ bool mix_place(int64_t units, int per, int64_t& unit,
 }
 static unsigned mix_grid(int64_t units, int per) { return (unsigned)(ceil_div(units, 8) * 8 * per); }
 
-// y: 16 NT atoms, OT tiles of outputs for each group of four waves
-template <typename T, int PW, int NT, int OT>
-__global__ __launch_bounds__(512) void mix_kernel(MixArgs a) {
+// y of 16 NT NG atoms and OT tiles of outputs: NG groups of four waves take 16 NT atoms each.
+//
+// A step is 32 channels.  Its weights (4 degrees x OT tiles x PW parts, 1 KB each) go to LDS by direct
+// loads a step ahead, in two buffers, and its features to registers a step ahead: what a wave waits
+// for at the end of a step are the weights alone, which were asked for first.
+template <typename T, int PW, int NT, int OT, int NG>
+__global__ __launch_bounds__(256 * NG) void mix_kernel(MixArgs a) {
     constexpr int PX = Mix8<T>::kParts, kB = Mix8<T>::kBytes;
     constexpr int kPitch = 16 * 16 + 4;    // floats of an atom in LDS
-    __shared__ __attribute__((aligned(16))) float sh[2][16 * kPitch];
+    constexpr int kW = 4 * OT * PW * 64;   // 16-byte pieces of a step's weights
+    constexpr int kOut = NG * 16 * kPitch * 4;
+    __shared__ __attribute__((aligned(16))) char sh[2 * kW * 16 > kOut ? 2 * kW * 16 : kOut];
     int64_t unit;
     int chunk;
     if (!mix_place(a.units, a.chunks, unit, chunk)) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quarter = wave & 3, group = wave >> 2;
-    const int q = lane >> 4, at = lane & 15;
-    const int64_t n0 = unit * 16 * NT;
-    const int tile0 = (chunk * a.groups + group) * OT;
-    const int rows = (int)min((int64_t)16 * NT, a.n - n0);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int quarter = wave & 3, group = wave >> 2, q = lane >> 4, at = lane & 15;
+    const int64_t n0 = (unit * NG + group) * 16 * NT;
+    const int tile0 = chunk * OT;
+    const int rows = (int)max((int64_t)0, min((int64_t)16 * NT, a.n - n0));
     const __amdgpu_buffer_rsrc_t xb =
         buffer_rsrc((const float*)((const char*)a.x + n0 * a.K * 16 * kB), rows * a.K * 16 * kB);
     const int d0 = mix_degree0(quarter), d1 = mix_degree1(quarter);
+    const int steps = (a.K + 31) / 32;
+    // weights of a step: [l][tile][part][lane], OT tiles of a.tiles
+    const __amdgpu_buffer_rsrc_t wb = buffer_rsrc(
+        (const float*)(a.w + (int64_t)tile0 * PW * 64), (uint32_t)((steps * 4 * a.tiles - tile0) * PW * 1024));
+    auto weights = [&](int s, char* to) {
+#pragma unroll
+        for (int i = 0; i < kW / 64 / (4 * NG); ++i) {
+            const int f = i * 4 * NG + wave;               // 1 KB: degree f / (OT PW)
+            const int from = ((s * 4 + f / (OT * PW)) * a.tiles * PW + f % (OT * PW)) * 1024;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                wb, (__attribute__((address_space(3))) void*)(to + f * 1024), 16, lane * 16, from, 0, 0);
+        }
+        asm volatile("" ::: "memory");                     // what follows is asked for later
+    };
+    Mix8<T> x[NT];
+    const int off = ((at * a.K + q) * 16 + quarter * 4) * kB;
+    auto features = [&](int s) {
+#pragma unroll
+        for (int k = 0; k < NT; ++k) {
+            // (all in the lane's offset, which the buffer's bounds are checked against)
+            const int at0 = off + (k * 16 * a.K + s * 32) * 16 * kB;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[k].load(j, xb, at0 + j * 64 * kB);
+        }
+    };
     v4f acc[4][NT][OT];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -174,50 +220,63 @@ __global__ __launch_bounds__(512) void mix_kernel(MixArgs a) {
         for (int k = 0; k < NT; ++k)
 #pragma unroll
             for (int o = 0; o < OT; ++o) acc[i][k][o] = v4f{0, 0, 0, 0};
-    const int steps = (a.K + 31) / 32;
+    weights(0, sh);
+    features(0);
     for (int s = 0; s < steps; ++s) {
+        // this step's weights have arrived, in every wave's part
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NT * 8) : "memory");
+        __syncthreads();
+        if ((a.K & 31) && s == steps - 1) {                // past K the loads gave the next atom's
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (s * 32 + 4 * j + q >= a.K) {
+#pragma unroll
+                    for (int k = 0; k < NT; ++k) x[k].zero(j);
+                }
+        }
         v4u f[4][NT][PX];
 #pragma unroll
         for (int k = 0; k < NT; ++k) {
-            Mix8<T> x;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int c = s * 32 + 4 * j + q;
-                x.load(j, xb, c < a.K ? (((k * 16 + at) * a.K + c) * 16 + quarter * 4) * kB : kMixFar);
-            }
-            x.template operand<0>(f[0][k]);
-            x.template operand<1>(f[1][k]);
-            x.template operand<2>(f[2][k]);
-            x.template operand<3>(f[3][k]);
+            x[k].template operand<0>(f[0][k]);
+            x[k].template operand<1>(f[1][k]);
+            x[k].template operand<2>(f[2][k]);
+            x[k].template operand<3>(f[3][k]);
         }
-        const v4u* w = a.w + (int64_t)(s * 4 * a.tiles + tile0) * PW * 64 + lane;
+        const v4u* w = reinterpret_cast<const v4u*>(sh) + (s & 1) * kW + lane;
+        if (s + 1 < steps) {
+            weights(s + 1, sh + ((s + 1) & 1) * kW * 16);
+            features(s + 1);
+            asm volatile("" ::: "memory");
+        }
 #pragma unroll
         for (int o = 0; o < OT; ++o) {
             v4u w0[PW], w1[PW];
 #pragma unroll
-            for (int p = 0; p < PW; ++p) {
-                w0[p] = w[((int64_t)d0 * a.tiles + o) * PW * 64 + p * 64];
-                w1[p] = w[((int64_t)d1 * a.tiles + o) * PW * 64 + p * 64];
-            }
+            for (int p = 0; p < PW; ++p) w0[p] = w[((d0 * OT + o) * PW + p) * 64];
 #pragma unroll
-            for (int k = 0; k < NT; ++k) {
-                acc[0][k][o] = mix_mfma<PW, PX>(w0, f[0][k], acc[0][k][o]);
+            for (int k = 0; k < NT; ++k) acc[0][k][o] = mix_mfma<PW, PX>(w0, f[0][k], acc[0][k][o]);
 #pragma unroll
-                for (int i = 1; i < 4; ++i)
+            for (int p = 0; p < PW; ++p) w1[p] = w[((d1 * OT + o) * PW + p) * 64];
+#pragma unroll
+            for (int i = 1; i < 4; ++i)
+#pragma unroll
+                for (int k = 0; k < NT; ++k)
                     acc[i][k][o] = mix_mfma<PW, PX>(w1, f[i][k], acc[i][k][o]);
-            }
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __syncthreads();                                   // the buffer is free
     }
     // the four waves' components of 16 atoms x 16 outputs together, and out as whole lines
     const int t = threadIdx.x & 255;
+    float* out = reinterpret_cast<float*>(sh) + group * 16 * kPitch;
 #pragma unroll
     for (int k = 0; k < NT; ++k)
 #pragma unroll
         for (int o = 0; o < OT; ++o) {
-            __syncthreads();
+            if (k + o) __syncthreads();
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                *reinterpret_cast<float4*>(&sh[group][at * kPitch + (4 * q + r) * 16 + quarter * 4]) =
+                *reinterpret_cast<float4*>(&out[at * kPitch + (4 * q + r) * 16 + quarter * 4]) =
                     make_float4(acc[0][k][o][r], acc[1][k][o][r], acc[2][k][o][r], acc[3][k][o][r]);
             __syncthreads();
             const int m0 = (tile0 + o) * 16;
@@ -226,18 +285,322 @@ __global__ __launch_bounds__(512) void mix_kernel(MixArgs a) {
             for (int i = 0; i < 16 * kPer / 256; ++i) {
                 const int p = i * 256 + t, node = p / kPer, e = p % kPer * kUnit;
                 if (k * 16 + node >= rows || m0 + e / 16 >= a.M) continue;
-                const float4 u = *reinterpret_cast<const float4*>(&sh[group][node * kPitch + e]);
+                const float4 u = *reinterpret_cast<const float4*>(&out[node * kPitch + e]);
                 const int64_t to = ((n0 + k * 16 + node) * a.M + m0) * 16 + e;
                 if constexpr (kB == 4) {
                     *reinterpret_cast<float4*>((float*)a.y + to) = u;
                 } else {
-                    const float4 v = *reinterpret_cast<const float4*>(&sh[group][node * kPitch + e + 4]);
+                    const float4 v = *reinterpret_cast<const float4*>(&out[node * kPitch + e + 4]);
                     *reinterpret_cast<uint4*>((uint16_t*)a.y + to) =
                         make_uint4(bf16_pack(u.x, u.y), bf16_pack(u.z, u.w), bf16_pack(v.x, v.y),
                                    bf16_pack(v.z, v.w));
                 }
             }
         }
+}
+
+// ---------------------------------------------------------------------------
+// The same with the weight in registers, for up to 32 KS channels: a workgroup stays, takes tiles of 16
+// atoms in turn and reads nothing but features.
+//
+// A step's features (32 channels of 16 atoms) come to LDS by direct loads of 16 bytes a lane, whole lines,
+// kAhead steps ahead; straight to registers a wave would ask for 8 or 16 bytes of every 32 or 64,
+// whose rate is the address units' (3.6 TB/s with every line in L1).  A wave takes 8 of the 16 components,
+// those of degrees 1 and 2 (1..8) or of 3 and 0 (9..15, 0), so two degrees of the weight, for OT tiles
+// of outputs: 2 KS OT PW registers x 4.  In LDS the 16-byte pieces of an atom are permuted by its
+// number, so that 16 atoms' reads meet no bank twice.
+// The two kinds of wave run code of their own, barrier for barrier alike.
+// ---------------------------------------------------------------------------
+template <typename T>
+struct StayRead;
+// Of 8 channels components 1..7 of one half of the 16 and the first of the other half, a part at a time
+// (all at once they would not fit beside the weight)
+template <>
+struct StayRead<uint16_t> {
+    static constexpr int kPieces = 64;     // 16-byte pieces of an atom's 32 channels
+    static constexpr int kParts = 2, kFrom[3] = {0, 7, 8};     // the parts' first components
+    v4u m[8];
+    __device__ __forceinline__ static int first(int at, int q, int half) {
+        return at * 1024 + ((2 * q + half) ^ at) * 16;
+    }
+    template <int PART>
+    __device__ __forceinline__ void load(const char* x, int main, int other) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (PART == 0)
+                m[j] = *reinterpret_cast<const v4u*>(x + (main ^ (j & 1) * 128) + (j >> 1) * 256);
+            else
+                m[j][0] = *reinterpret_cast<const unsigned*>(x + (other ^ (j & 1) * 128) + (j >> 1) * 256);
+        }
+    }
+    __device__ __forceinline__ void cut(int j) { m[j] = v4u{0, 0, 0, 0}; }
+    template <int I>                       // component I + 1 of the half; 7: the other's first
+    __device__ __forceinline__ void operand(v4u* o) const {
+        constexpr int kAt = I < 7 ? I + 1 : 0;
+        constexpr unsigned kSel = kAt % 2 ? 0x07060302u : 0x05040100u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            o[0][j] = __builtin_amdgcn_perm(m[2 * j + 1][kAt / 2], m[2 * j][kAt / 2], kSel);
+    }
+};
+template <>
+struct StayRead<float> {
+    static constexpr int kPieces = 128;
+    static constexpr int kParts = 3, kFrom[4] = {0, 3, 7, 8};
+    float4 m[8];
+    __device__ __forceinline__ static int first(int at, int q, int half) {
+        return at * 2048 + ((4 * q + 2 * half) ^ at) * 16;
+    }
+    template <int PART>
+    __device__ __forceinline__ void load(const char* x, int main, int other) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (PART < 2)
+                m[j] = *reinterpret_cast<const float4*>(x + (main ^ PART * 16) + j * 256);
+            else
+                m[j].x = *reinterpret_cast<const float*>(x + other + j * 256);
+        }
+    }
+    __device__ __forceinline__ void cut(int j) { m[j] = make_float4(0, 0, 0, 0); }
+    template <int I>
+    __device__ __forceinline__ float value(int j) const {
+        constexpr int kAt = I < 7 ? (I + 1) % 4 : 0;
+        return kAt == 0 ? m[j].x : kAt == 1 ? m[j].y : kAt == 2 ? m[j].z : m[j].w;
+    }
+};
+
+// The weight of 32 channels and 16 outputs, and acc[i][o] += its products with a part of the components
+template <typename T>
+struct StayWeight;
+template <>
+struct StayWeight<uint16_t> {
+    v4u p[2];
+    __device__ __forceinline__ void set(const float* v) { mix_split<2>(v, p); }
+};
+template <>
+struct StayWeight<float> {
+    float v[8];
+    __device__ __forceinline__ void set(const float* t) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = t[j];
+    }
+};
+// Successive products go to different sums: one that waits for the last result waits for all its cycles
+template <int FROM, int TO, int SECOND, int OT>
+__device__ __forceinline__ void stay_products(const StayRead<uint16_t>& x,
+                                              const StayWeight<uint16_t>* const (&w)[2], v4f (&acc)[8][OT]) {
+    constexpr int kAtOnce = OT == 1 ? 2 : 1;
+    static_for<(TO - FROM + kAtOnce - 1) / kAtOnce>([&](auto kk) {
+        constexpr int I0 = FROM + decltype(kk)::value * kAtOnce, kN = std::min(kAtOnce, TO - I0);
+        v4u f[kN];
+        static_for<kN>([&](auto ii) {
+            x.template operand<I0 + decltype(ii)::value>(&f[decltype(ii)::value]);
+        });
+#pragma unroll
+        for (int p = 1; p >= 0; --p)
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+#pragma unroll
+                for (int o = 0; o < OT; ++o)
+                    acc[I0 + i][o] = mfma_bf16(w[I0 + i >= SECOND][o].p[p], f[i], acc[I0 + i][o]);
+    });
+}
+template <int FROM, int TO, int SECOND, int OT>
+__device__ __forceinline__ void stay_products(const StayRead<float>& x,
+                                              const StayWeight<float>* const (&w)[2], v4f (&acc)[8][OT]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        static_for<TO - FROM>([&](auto ii) {
+            constexpr int I = FROM + decltype(ii)::value;
+#pragma unroll
+            for (int o = 0; o < OT; ++o)
+                acc[I][o] = mfma1(w[I >= SECOND][o].v[j], x.template value<I>(j), acc[I][o]);
+        });
+}
+
+template <typename T>
+struct StayShape {
+    static constexpr int kRing = sizeof(T) == 4 ? 2 : 3, kAhead = kRing - 1;
+    static constexpr int kStep = StayRead<T>::kPieces * 16 * 16;       // bytes of a step
+    static constexpr int kOut = 16 * 8 * 16 * 4;       // of a group's 16 atoms x 8 outputs on the way out
+    static constexpr int bytes(int groups) { return kRing * kStep + groups * kOut; }
+};
+
+// Until at most LATER loads and `tiles` tiles' stores are under way: what was asked for before them is
+// there (loads complete in order; a store that completes early only lengthens the wait)
+template <int LATER, int STORES, int MOST>
+__device__ __forceinline__ void stay_wait(int tiles) {
+    static_for<MOST + 1>([&](auto ii) {
+        constexpr int I = decltype(ii)::value;
+        static_assert(LATER + I * STORES < 64, "the counter's range");
+        if (tiles == I)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LATER + I * STORES) : "memory");
+    });
+}
+
+template <typename T, int KS, int OT, int OG, int HALF>
+__device__ __forceinline__ void mix_stay(const MixArgs& a, char* sh) {
+    using S = StayShape<T>;
+    constexpr int kB = sizeof(T), kWaves = 2 * OG;
+    constexpr int kPieces = StayRead<T>::kPieces, kLoads = kPieces / 4 / kWaves;   // of a wave and step
+    constexpr int kStores = OT * 4 * kB / 2;                                       // of a wave and tile
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = wave >> 1, q = lane >> 4, at = lane & 15;
+    const int slot = blockIdx.x >> 3, chunk = slot % a.chunks;
+    const int64_t tiles = ceil_div(a.n, 16), streams = gridDim.x / a.chunks;
+    const int64_t first = (int64_t)(slot / a.chunks) * 8 + (blockIdx.x & 7);
+    if (first >= tiles) return;
+    const int steps = (a.K + 31) / 32;
+    const int m0 = (chunk * OG + group) * OT * 16;
+
+    // steps of this workgroup one after the other; past the last tile the last one again, so that
+    // the number of loads under way is always the same.  Lanes past the tile's last atom or (after the last
+    // step of K) its last channel read the next one's or, past the buffer's bounds, nothing: no result
+    // takes them.
+    int offset[kLoads];                    // of a load's lane in its tile
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int load = i * kWaves + wave;                // 64 pieces of one atom
+        const int node = load * 64 / kPieces, p = (load * 64 % kPieces + lane) ^ node;
+        offset[i] = node * a.K * 16 * kB + p * 16;
+    }
+    int64_t ask_tile = first;
+    int ask_step = 0, ask_place = 0;
+    auto ask = [&]() {
+        const int64_t n0 = min(ask_tile, tiles - 1) * 16;
+        const int rows = (int)min((int64_t)16, a.n - n0);
+        const __amdgpu_buffer_rsrc_t xb =
+            buffer_rsrc((const float*)((const char*)a.x + n0 * a.K * 16 * kB), rows * a.K * 16 * kB);
+        char* to = sh + ask_place * S::kStep + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                xb, (__attribute__((address_space(3))) void*)(to + i * kWaves * 1024), 16,
+                offset[i] + ask_step * 512 * kB, 0, 0, 0);
+        asm volatile("" ::: "memory");
+        ask_place = ask_place + 1 == S::kRing ? 0 : ask_place + 1;
+        if (++ask_step == steps) ask_step = 0, ask_tile += streams;
+    };
+#pragma unroll
+    for (int i = 0; i < S::kAhead; ++i) ask();
+
+    // degrees of this wave: 1 2 (half 0) or 3 0
+    StayWeight<T> w[2][KS][OT];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const __amdgpu_buffer_rsrc_t wb = buffer_rsrc(
+            a.weight + (int64_t)(HALF ? 3 - 3 * u : 1 + u) * a.K * a.M, (uint32_t)(a.K * a.M * 4));
+        float v[KS][OT][8];
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int o = 0; o < OT; ++o)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int k = s * 32 + 4 * j + q, m = m0 + o * 16 + at;
+                    v[s][o][j] = buffer_ld(wb, k < a.K && m < a.M ? (k * a.sk + m * a.sm) * 4 : kMixFar, 0);
+                }
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int o = 0; o < OT; ++o) w[u][s][o].set(v[s][o]);
+        asm volatile("" ::: "memory");                     // one degree at a time: registers
+    }
+    const int main = StayRead<T>::first(at, q, HALF), other = StayRead<T>::first(at, q, 1 - HALF);
+    char* out = sh + S::kRing * S::kStep + group * S::kOut;
+    int place = 0;
+    unsigned ends = 0;                     // bit i: a tile ended i steps ago
+    for (int64_t tile = first; tile < tiles; tile += streams) {
+        v4f acc[8][OT];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int o = 0; o < OT; ++o) acc[i][o] = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            if (s >= steps) break;
+            // this step's loads are in, those of every wave; the step before is read
+            constexpr int kMost = std::min(S::kAhead, (63 - (S::kAhead - 1) * kLoads) / kStores);
+            stay_wait<(S::kAhead - 1) * kLoads, kStores, kMost>(
+                min(__builtin_popcount(ends & ((1u << S::kAhead) - 1)), kMost));
+            ends <<= 1;
+            __syncthreads();
+            ask();
+            const char* from = sh + place * S::kStep;
+            place = place + 1 == S::kRing ? 0 : place + 1;
+            const bool cut = s == steps - 1 && (a.K & 31);
+            StayRead<T> x;
+            const StayWeight<T>* const ws[2] = {w[0][s], w[1][s]};
+            static_for<StayRead<T>::kParts>([&](auto ii) {
+                constexpr int P = decltype(ii)::value;
+                if constexpr (P > 0) asm volatile("" ::: "memory");
+                x.template load<P>(from, main, other);
+                if (cut) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (s * 32 + 4 * j + q >= a.K) x.cut(j);
+                }
+                constexpr int kFrom = StayRead<T>::kFrom[P], kTo = StayRead<T>::kFrom[P + 1];
+                stay_products<kFrom, kTo, (HALF ? 7 : 3)>(x, ws, acc);
+            });
+        }
+        ends |= 1;
+        // the two waves' components of 16 atoms x 8 outputs together, and out as whole lines
+        const int64_t n0 = tile * 16;
+        const int rows = (int)min((int64_t)16, a.n - n0);
+        const __amdgpu_buffer_rsrc_t yb =
+            buffer_rsrc((const float*)((const char*)a.y + n0 * a.M * 16 * kB), rows * a.M * 16 * kB);
+#pragma unroll
+        for (int o = 0; o < OT; ++o)
+#pragma unroll
+            for (int rp = 0; rp < 2; ++rp) {
+                int mine = (at * 32 + (q * 8 ^ at)) * 16;
+                asm volatile("" : "+v"(mine));             // the places are formed again, not kept
+                __syncthreads();
+#pragma unroll
+                for (int rr = 0; rr < 2; ++rr) {
+                    // pieces of four components, permuted by the atom's number
+                    auto to = [&](int piece) {
+                        return reinterpret_cast<float*>(out + (mine ^ (rr * 4 + piece) * 16));
+                    };
+                    const int r = rp * 2 + rr;
+                    to(HALF * 2)[1] = acc[0][o][r];
+                    *reinterpret_cast<float2*>(to(HALF * 2) + 2) = make_float2(acc[1][o][r], acc[2][o][r]);
+                    *reinterpret_cast<float4*>(to(HALF * 2 + 1)) =
+                        make_float4(acc[3][o][r], acc[4][o][r], acc[5][o][r], acc[6][o][r]);
+                    to(2 - HALF * 2)[0] = acc[7][o][r];
+                }
+                __syncthreads();
+                constexpr int kUnit = 16 / kB, kPer = 128 / kUnit;     // 16-byte pieces of an atom
+#pragma unroll
+                for (int i = 0; i < 16 * kPer / 128; ++i) {
+                    const int p = i * 128 + (threadIdx.x & 127), node = p / kPer, e = p % kPer * kUnit;
+                    const int row = e / 16, m = m0 + o * 16 + (row >> 1) * 4 + rp * 2 + (row & 1);
+                    // (every store is issued, those past the end dropped by the buffer's bounds: the
+                    // waits count them)
+                    const int to = m < a.M ? ((node * a.M + m) * 16 + e % 16) * kB : kMixFar;
+                    const float4 u =
+                        *reinterpret_cast<const float4*>(out + (node * 32 + (e / 4 ^ node)) * 16);
+                    v4u piece;
+                    if constexpr (kB == 4) {
+                        piece = __builtin_bit_cast(v4u, u);
+                    } else {
+                        const float4 v = *reinterpret_cast<const float4*>(
+                            out + (node * 32 + ((e / 4 + 1) ^ node)) * 16);
+                        piece = v4u{bf16_pack(u.x, u.y), bf16_pack(u.z, u.w), bf16_pack(v.x, v.y),
+                                    bf16_pack(v.z, v.w)};
+                    }
+                    __builtin_amdgcn_raw_buffer_store_b128(piece, yb, to, 0, 0);
+                }
+            }
+    }
+}
+
+template <typename T, int KS, int OT, int OG>
+__global__ __launch_bounds__(128 * OG, 2) void mix_stay_kernel(MixArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char sh[];
+    if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 1) mix_stay<T, KS, OT, OG, 1>(a, sh);
+    else mix_stay<T, KS, OT, OG, 0>(a, sh);
 }
 
 // The 8-bit form of eight atoms: the code's value is exact in bf16
@@ -366,32 +729,68 @@ static bool mix_shape_ok(int64_t N, int C, int O, int dtype) {
            (dtype == 0 || dtype == 1);
 }
 
-// Tiles of outputs of a wave, and groups of four waves
+// Atoms and outputs of a workgroup, parts of the weight
 template <typename T>
 struct MixShape {
-    static constexpr int kNT = 2, kOT = sizeof(T) == 4 ? 2 : 4, kPW = sizeof(T) == 4 ? 3 : 2;
+    static constexpr int kNT = 1, kOT = 4, kNG = 2, kPW = sizeof(T) == 4 ? 3 : 2;
 };
 template <typename T>
 static void mix_tiles(int M, MixArgs& a) {
     constexpr int kOT = MixShape<T>::kOT;
-    a.groups = M <= kOT * 16 ? 1 : 2;
-    a.chunks = (M + kOT * a.groups * 16 - 1) / (kOT * a.groups * 16);
-    a.tiles = a.chunks * a.groups * kOT;
+    a.chunks = (M + kOT * 16 - 1) / (kOT * 16);
+    a.tiles = a.chunks * kOT;
 }
 template <typename T>
 static size_t mix_bytes(int K, int M) {
+    if (K <= kStayMost<T>) return 16;
     MixArgs a{};
     mix_tiles<T>(M, a);
     return (size_t)((K + 31) / 32) * 4 * a.tiles * MixShape<T>::kPW * 64 * 16;
 }
 
+template <typename T, int KS, int OT, int OG>
+static int stay_launch(MixArgs a, hipStream_t s) {
+    constexpr int kBytes = StayShape<T>::bytes(OG), kPer = std::min(8 / (2 * OG), 163840 / kBytes);
+    auto kernel = mix_stay_kernel<T, KS, OT, OG>;
+    // more than 64 KB of LDS, allowed once on each device
+    static std::atomic<uint64_t> allowed{0};
+    int device = 0;
+    hipError_t rc = hipGetDevice(&device);
+    if (rc != hipSuccess) return (int)rc;
+    const uint64_t bit = device < 64 ? (uint64_t)1 << device : 0;
+    if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+        rc = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+        if (rc != hipSuccess) return (int)rc;
+        allowed.fetch_or(bit, std::memory_order_relaxed);
+    }
+    a.chunks = (a.M + OG * OT * 16 - 1) / (OG * OT * 16);
+    const int64_t tiles = ceil_div(a.n, 16), most = std::max(1, 32 * kPer / a.chunks);
+    const int64_t streams = 8 * std::min(most, ceil_div(tiles, 8));
+    kernel<<<(unsigned)(streams * a.chunks), 128 * OG, kBytes, s>>>(a);
+    return (int)hipGetLastError();
+}
+template <typename T, int KS, int OT>
+static int stay_groups(const MixArgs& a, hipStream_t s) {
+    if (a.M <= OT * 16) return stay_launch<T, KS, OT, 1>(a, s);
+    return stay_launch<T, KS, OT, 2>(a, s);
+}
 template <typename T>
-static void mix_run(MixArgs a, const float* w, int sk, int sm, void* ws, hipStream_t s) {
+static int stay_run(const MixArgs& a, hipStream_t s) {
+    if constexpr (sizeof(T) == 2) {
+        if (a.K > 128) return stay_groups<T, 8, 1>(a, s);
+        if (a.K > 64) return stay_groups<T, 4, 2>(a, s);
+    }
+    return stay_groups<T, 2, 2>(a, s);
+}
+
+template <typename T>
+static int mix_run(MixArgs a, void* ws, hipStream_t s) {
+    if (a.K <= kStayMost<T>) return stay_run<T>(a, s);
     using S = MixShape<T>;
     mix_tiles<T>(a.M, a);
     const int total = (a.K + 31) / 32 * 4 * a.tiles * 64;
-    mix_pack_kernel<S::kPW><<<(total + 255) / 256, 256, 0, s>>>(w, (v4u*)ws, a.K, a.M, sk, sm, a.tiles,
-                                                               total);
+    mix_pack_kernel<S::kPW><<<(total + 255) / 256, 256, 0, s>>>(a.weight, (v4u*)ws, a.K, a.M, a.sk,
+                                                               a.sm, a.tiles, total);
     a.w = (const v4u*)ws;
     constexpr int64_t kAtoms = (int64_t)1 << 24;     // of a launch
     const int64_t n = a.n;
@@ -401,10 +800,11 @@ static void mix_run(MixArgs a, const float* w, int sk, int sm, void* ws, hipStre
         a.x = x + n0 * a.K * 16 * (int64_t)sizeof(T);
         a.y = y + n0 * a.M * 16 * (int64_t)sizeof(T);
         a.n = std::min(n - n0, kAtoms);
-        a.units = ceil_div(a.n, 16 * S::kNT);
-        mix_kernel<T, S::kPW, S::kNT, S::kOT>
-            <<<mix_grid(a.units, a.chunks), 256 * a.groups, 0, s>>>(a);
+        a.units = ceil_div(a.n, 16 * S::kNT * S::kNG);
+        mix_kernel<T, S::kPW, S::kNT, S::kOT, S::kNG>
+            <<<mix_grid(a.units, a.chunks), 256 * S::kNG, 0, s>>>(a);
     }
+    return (int)hipGetLastError();
 }
 
 // Ranges of atoms of gW: about 1024 workgroups of at least four steps, 64 MB of partial sums at most
@@ -443,10 +843,8 @@ extern "C" int batteries_channel_mixing(const void* x, const float* weight, void
         return BM_ERR_WORKSPACE;
     MixArgs a{};
     a.x = x; a.y = y; a.n = N; a.K = transposed ? O : C; a.M = transposed ? C : O;
-    const int sk = transposed ? 1 : O, sm = transposed ? O : 1;
-    if (dtype == 0) mix_run<float>(a, weight, sk, sm, workspace, stream);
-    else mix_run<uint16_t>(a, weight, sk, sm, workspace, stream);
-    return (int)hipGetLastError();
+    a.weight = weight; a.sk = transposed ? 1 : O; a.sm = transposed ? O : 1;
+    return dtype == 0 ? mix_run<float>(a, workspace, stream) : mix_run<uint16_t>(a, workspace, stream);
 }
 
 extern "C" size_t batteries_channel_mixing_weight_grad_workspace_bytes(int64_t N, int C, int O) {

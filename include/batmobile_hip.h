@@ -672,7 +672,7 @@ int batteries_gate_activation_backward(const void* x, const uint8_t* codes, cons
  *   y[n, o, m] = sum_c x[n, c, m] weight[l(m), c, o],  l(m) the degree of component m
  * x [N, C, 16] to y [N, O, 16] in fp32 (dtype 0) or bf16 (dtype 1), 16-byte aligned, weight
  * [4, C, O] fp32; transposed: x [N, O, 16] to y [N, C, 16], the sum over o.  fp32 accuracy of the
- * products in fp32; with bf16 features the weight is rounded to 16 bits of mantissa.  C, O <= 2048,
+ * products in fp32; with bf16 features the weight is rounded to 15 bits.  C, O <= 2048,
  * N < 2^31.
  * ------------------------------------------------------------------------- */
 size_t batteries_channel_mixing_workspace_bytes(int C, int O, int transposed, int dtype);
