@@ -265,7 +265,8 @@ void check_codes(const Tensor& codes, const Tensor& exps) {
     check_features(codes, "codes");
     TORCH_CHECK(codes.scalar_type() == torch::kFloat8_e4m3fn && codes.is_contiguous(),
                 "codes must be contiguous float8_e4m3fn");
-    TORCH_CHECK((reinterpret_cast<uintptr_t>(codes.data_ptr()) & 7) == 0, "codes must be aligned to 8 bytes");
+    TORCH_CHECK((reinterpret_cast<uintptr_t>(codes.data_ptr()) & 15) == 0,
+                "codes must be aligned to 16 bytes");
     TORCH_CHECK(exps.device() == codes.device() && exps.scalar_type() == torch::kUInt8 &&
                     exps.is_contiguous() && exps.dim() == 2 && exps.size(0) == codes.size(0) &&
                     exps.size(1) == (codes.size(1) + 7) / 8,

@@ -21,7 +21,6 @@
 #include <type_traits>
 
 #include "checkpoint.h"
-#include "sums.h"
 #include "batmobile_hip.h"
 
 namespace bmhip {
@@ -36,7 +35,7 @@ constexpr int kMixFar = 0x7fffff00;        // a buffer offset past every buffer 
 __device__ __forceinline__ int mix_degree0(int quarter) { return (0x3220 >> (4 * quarter)) & 15; }
 __device__ __forceinline__ int mix_degree1(int quarter) { return (0x3321 >> (4 * quarter)) & 15; }
 
-// Four components of eight rows, and from them the operand of each component, in PARTS parts
+// Four components of eight channels, and from them the operand of each component, in its parts
 template <typename T>
 struct Mix8;
 template <>
@@ -151,7 +150,7 @@ struct MixArgs {
     int K, M;                              // channels in, out
     int tiles, chunks;                     // tiles of 16 outputs (padded), chunks of them
     int64_t units;                         // workgroups of atoms
-    int splits, per_split;                 // gW: ranges of atoms, steps of 32 atoms in one
+    int splits, per_split;                 // gW: ranges of atoms, steps in one
 };
 
 // Workgroup b of `units` times `per`: those of a unit follow each other on one XCD (b % 8), which
@@ -603,125 +602,260 @@ __global__ __launch_bounds__(128 * OG, 2) void mix_stay_kernel(MixArgs a) {
     else mix_stay<T, KS, OT, OG, 0>(a, sh);
 }
 
-// The 8-bit form of eight atoms: the code's value is exact in bf16
-struct MixKept {
-    static constexpr int kParts = 1, kBytes = 1;
+// ---------------------------------------------------------------------------
+// gW: a workgroup takes 32 CT channels in and 64 out over a range of atoms.  A step is 16 atoms in bf16 (8
+// in fp32, whose products run on the fp32 matrix cores, 4 atoms each), features and gradients brought to
+// LDS by direct loads while the step before is worked on.  A wave takes four components (two degrees at
+// most) and half of the channels in: lane l holds channel l % 16 and atoms l / 16 + 4 j.  part [splits,
+// 4, K, M].
+// ---------------------------------------------------------------------------
+typedef short v4s __attribute__((ext_vector_type(4)));
+
+template <typename T, bool KEPT, int CT>
+struct GradShape {
+    static constexpr int kB = sizeof(T), kAtoms = kB == 2 ? 16 : 8;
+    static constexpr int kIn = 32 * CT, kOut = 64;                 // channels
+    static constexpr int kXB = KEPT ? 1 : kB;                      // bytes of a value of x
+    static constexpr int kX = kAtoms * kIn * 16 * kXB, kG = kAtoms * kOut * 16 * kB;
+    static constexpr int kStep = kX + kG, kBytes = 2 * kStep;
+    static constexpr int kExps = KEPT ? kAtoms * 2 * CT / 64 + (kAtoms * 2 * CT % 64 != 0) : 0;
 };
-__device__ __forceinline__ void mix_decode(unsigned code, int e, unsigned* r) {
-    const float4 v = ckpt_decode4(code, ckpt_up(e));
-    r[0] = bf16_pack(v.x, v.y);
-    r[1] = bf16_pack(v.z, v.w);
+
+// Where piece p (16 bytes) of an atom lies in LDS: 16 neighbouring channels' pieces of the same
+// components in different banks (its own inverse)
+template <int BYTES>
+__device__ __forceinline__ int grad_place(int p) {
+    return BYTES == 4 ? p ^ (p >> 4 & 3) : BYTES == 2 ? p ^ (p >> 4 & 1) : p;
 }
 
-// gW: a workgroup takes CT x OT tiles of (c, o) over a range of atoms.  part [splits, 6, K, M]: the
-// sums of the quarters' degrees 0 1 | 2 | 2 3 | 3.
-template <typename X, typename G, int CT, int OT>
-__global__ __launch_bounds__(256) void mix_weight_kernel(MixArgs a) {
-    constexpr bool kKept = X::kBytes == 1;
-    constexpr int PX = X::kParts, PG = G::kParts;
+// Four components of a channel and atom
+template <typename T>
+struct Four;
+template <>
+struct Four<float> {
+    float4 v;
+    __device__ __forceinline__ void load(const char* p) { v = *reinterpret_cast<const float4*>(p); }
+    __device__ __forceinline__ void decode(unsigned code, float up) { v = ckpt_decode4(code, up); }
+    __device__ __forceinline__ void zero() { v = make_float4(0, 0, 0, 0); }
+    template <int I>
+    __device__ __forceinline__ float get() const {
+        return I == 0 ? v.x : I == 1 ? v.y : I == 2 ? v.z : v.w;
+    }
+};
+template <>
+struct Four<uint16_t> {
+    unsigned v[2];
+    __device__ __forceinline__ void load(const char* p) {
+        const uint2 t = *reinterpret_cast<const uint2*>(p);
+        v[0] = t.x, v[1] = t.y;
+    }
+    __device__ __forceinline__ void decode(unsigned code, float up) {
+        const float4 t = ckpt_decode4(code, up);               // exact in bf16
+        v[0] = bf16_pack(t.x, t.y), v[1] = bf16_pack(t.z, t.w);
+    }
+    __device__ __forceinline__ void zero() { v[0] = v[1] = 0; }
+};
+// acc[k][o] += sum over the step's atoms of component I
+template <int I, int CT>
+__device__ __forceinline__ void grad_products(const Four<uint16_t> (&x)[CT][4], const Four<uint16_t> (&g)[4][4],
+                                              v4f (&acc)[CT][4]) {
+    constexpr unsigned kSel = I % 2 ? 0x07060302u : 0x05040100u;
+    auto operand = [&](const Four<uint16_t>(&r)[4]) {
+        return __builtin_bit_cast(v4s, uint2{__builtin_amdgcn_perm(r[1].v[I / 2], r[0].v[I / 2], kSel),
+                                             __builtin_amdgcn_perm(r[3].v[I / 2], r[2].v[I / 2], kSel)});
+    };
+    v4s f[4];
+#pragma unroll
+    for (int o = 0; o < 4; ++o) f[o] = operand(g[o]);
+#pragma unroll
+    for (int k = 0; k < CT; ++k) {
+        const v4s e = operand(x[k]);
+#pragma unroll
+        for (int o = 0; o < 4; ++o)
+            acc[k][o] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(e, f[o], acc[k][o], 0, 0, 0);
+    }
+}
+template <int I, int CT>
+__device__ __forceinline__ void grad_products(const Four<float> (&x)[CT][2], const Four<float> (&g)[4][2],
+                                              v4f (&acc)[CT][4]) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int k = 0; k < CT; ++k)
+#pragma unroll
+            for (int o = 0; o < 4; ++o)
+                acc[k][o] = mfma1(x[k][j].template get<I>(), g[o][j].template get<I>(), acc[k][o]);
+}
+
+template <typename T, bool KEPT, int CT>
+__global__ __launch_bounds__(512, 2) void mix_weight_kernel(MixArgs a) {
+    using S = GradShape<T, KEPT, CT>;
+    constexpr int kJ = S::kAtoms / 4, kXPieces = S::kIn * S::kXB, kGPieces = S::kOut * S::kB;   // of an atom
+    extern __shared__ __attribute__((aligned(16))) char sh[];
     int64_t split;
     int which;
     if (!mix_place(a.splits, a.tiles * a.chunks, split, which)) return;
-    const int lane = threadIdx.x & 63, quarter = threadIdx.x >> 6;
-    const int q = lane >> 4, at = lane & 15;
-    const int c0 = which % a.tiles * CT * 16, o0 = which / a.tiles * OT * 16;
-    v4f acc[2][CT][OT];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int quarter = wave & 3, side = wave >> 2, q = lane >> 4, at = lane & 15;
+    const int c0 = which % a.tiles * S::kIn, o0 = which / a.tiles * S::kOut;
+    const int exps = ckpt_blocks(a.K);
+    const int64_t begin = split * a.per_split * S::kAtoms;
+    const int64_t end = min(a.n, begin + (int64_t)a.per_split * S::kAtoms);
+
+    // channels past K or M read what lies there (the next atom's, past the buffer nothing): no result
+    // that is stored takes them
+    int code[S::kExps ? S::kExps : 1];
+    auto ask = [&](int64_t n0, char* to) {
+        const int rows = (int)min((int64_t)S::kAtoms, a.n - n0);
+        const void* xs = KEPT ? (const void*)(a.codes + n0 * a.K * 16)
+                              : (const void*)((const char*)a.x + n0 * a.K * 16 * S::kB);
+        const __amdgpu_buffer_rsrc_t xb = buffer_rsrc((const float*)xs, rows * a.K * 16 * S::kXB);
+        const __amdgpu_buffer_rsrc_t gb = buffer_rsrc(
+            (const float*)((const char*)a.g + n0 * a.M * 16 * S::kB), rows * a.M * 16 * S::kB);
+#pragma unroll
+        for (int i = 0; i < S::kX / 8192; ++i) {
+            const int at0 = (i * 8 + wave) * 64 + lane;            // place in the step
+            const int off = (at0 / kXPieces * a.K + c0) * 16 * S::kXB +
+                            grad_place<S::kXB>(at0 % kXPieces) * 16;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                xb, (__attribute__((address_space(3))) void*)(to + (i * 8 + wave) * 1024), 16, off, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < S::kG / 8192; ++i) {
+            const int at0 = (i * 8 + wave) * 64 + lane;
+            const int off = (at0 / kGPieces * a.M + o0) * 16 * S::kB +
+                            grad_place<S::kB>(at0 % kGPieces) * 16;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                gb, (__attribute__((address_space(3))) void*)(to + S::kX + (i * 8 + wave) * 1024), 16, off,
+                0, 0, 0);
+        }
+        if constexpr (KEPT) {
+            // exponent e of the wave's 2 CT blocks of atom n in lane (n 2 CT + e) % 64 of a register
+            const __amdgpu_buffer_rsrc_t eb = buffer_rsrc((const float*)(a.exps + n0 * exps), rows * exps);
+#pragma unroll
+            for (int i = 0; i < S::kExps; ++i) {
+                const int e = i * 64 + lane;
+                code[i] = __builtin_amdgcn_raw_buffer_load_b8(
+                    eb, e / (2 * CT) * exps + (c0 + side * CT * 16) / 8 + e % (2 * CT), 0, 0);
+            }
+        }
+        asm volatile("" ::: "memory");
+    };
+
+    v4f acc[2][CT][4];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int k = 0; k < CT; ++k)
 #pragma unroll
-            for (int o = 0; o < OT; ++o) acc[i][k][o] = v4f{0, 0, 0, 0};
-    const int exps = ckpt_blocks(a.K);
-    const int64_t last = min(a.n, (split + 1) * a.per_split * 32);
-    for (int64_t n0 = split * a.per_split * 32; n0 < last; n0 += 32) {
-        const int rows = (int)min((int64_t)32, a.n - n0);
-        const __amdgpu_buffer_rsrc_t gb = buffer_rsrc(
-            (const float*)((const char*)a.g + n0 * a.M * 16 * G::kBytes), rows * a.M * 16 * G::kBytes);
-        const void* xs = kKept ? (const void*)(a.codes + n0 * a.K * 16)
-                               : (const void*)((const char*)a.x + n0 * a.K * 16 * X::kBytes);
-        const __amdgpu_buffer_rsrc_t xb = buffer_rsrc((const float*)xs, rows * a.K * 16 * X::kBytes);
-        typename std::conditional<kKept, Mix8<uint16_t>, X>::type x[CT];
-        G g[OT];
-        if constexpr (kKept) {
-            const __amdgpu_buffer_rsrc_t eb =
-                buffer_rsrc((const float*)(a.exps + n0 * exps), rows * exps);
-            unsigned code[CT][8];
-            int e[CT][8];
+            for (int o = 0; o < 4; ++o) acc[i][k][o] = v4f{0, 0, 0, 0};
+    if (begin < end) ask(begin, sh);
+    int turn = 0;
+    for (int64_t n0 = begin; n0 < end; n0 += S::kAtoms, turn ^= 1) {
+        // this step's loads are in, those of every wave; the step before is read
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        int now[S::kExps ? S::kExps : 1];
+        if constexpr (KEPT) {
 #pragma unroll
-            for (int k = 0; k < CT; ++k)
+            for (int i = 0; i < S::kExps; ++i) now[i] = code[i];
+        }
+        __syncthreads();
+        if (n0 + S::kAtoms < end) ask(n0 + S::kAtoms, sh + (turn ^ 1) * S::kStep);
+        const char* from = sh + turn * S::kStep;
+        Four<T> x[CT][kJ], g[4][kJ];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int c = c0 + k * 16 + at, n = 4 * j + q;
-                    code[k][j] = __builtin_amdgcn_raw_buffer_load_b32(
-                        xb, c < a.K ? (n * a.K + c) * 16 + quarter * 4 : kMixFar, 0, 0);
-                    e[k][j] = __builtin_amdgcn_raw_buffer_load_b8(
-                        eb, c < a.K ? n * exps + c / kCkptChannels : kMixFar, 0, 0);
+        for (int k = 0; k < CT; ++k)
+#pragma unroll
+            for (int j = 0; j < kJ; ++j) {
+                const int c = (side * CT + k) * 16 + at, n = 4 * j + q;
+                if constexpr (KEPT) {
+                    const int e = (4 * j * 2 * CT) % 64 + q * 2 * CT + 2 * k + (at >> 3);
+                    const int exponent = __builtin_amdgcn_ds_bpermute(e * 4, now[4 * j * 2 * CT / 64]);
+                    x[k][j].decode(*reinterpret_cast<const unsigned*>(from + (n * S::kIn + c) * 16 + quarter * 4),
+                                   ckpt_up(exponent));
+                } else {
+                    const int p = c * S::kB + quarter * S::kB / 4;
+                    x[k][j].load(from + (n * kXPieces + grad_place<S::kB>(p)) * 16 +
+                                 (S::kB == 2 ? quarter % 2 * 8 : 0));
                 }
+            }
 #pragma unroll
-            for (int k = 0; k < CT; ++k)
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) mix_decode(code[k][j], e[k][j], x[k].r[j]);
-        } else {
+            for (int j = 0; j < kJ; ++j) {
+                const int p = (k * 16 + at) * S::kB + quarter * S::kB / 4;
+                g[k][j].load(from + S::kX + ((4 * j + q) * kGPieces + grad_place<S::kB>(p)) * 16 +
+                             (S::kB == 2 ? quarter % 2 * 8 : 0));
+            }
+        if (n0 + S::kAtoms > a.n) {                        // atoms past the last add nothing
 #pragma unroll
-            for (int k = 0; k < CT; ++k)
+            for (int j = 0; j < kJ; ++j)
+                if (n0 + 4 * j + q >= a.n) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int c = c0 + k * 16 + at;
-                    x[k].load(j, xb, c < a.K ? (((4 * j + q) * a.K + c) * 16 + quarter * 4) * X::kBytes
-                                             : kMixFar);
+                    for (int k = 0; k < CT; ++k) x[k][j].zero();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) g[k][j].zero();
                 }
         }
+        grad_products<0>(x, g, acc[0]);
+        grad_products<1>(x, g, acc[1]);
+        grad_products<2>(x, g, acc[1]);
+        grad_products<3>(x, g, acc[1]);
+    }
+    // degrees of the quarters: 0 1 | 2 2 | 2 3 | 3 3.  The third hands its sums to the others.
+    v4f* give = reinterpret_cast<v4f*>(sh) + side * 2 * CT * 4 * 64 + lane;
+    __syncthreads();
+    if (quarter == 2) {
 #pragma unroll
-        for (int k = 0; k < OT; ++k)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int o = o0 + k * 16 + at;
-                g[k].load(j, gb, o < a.M ? (((4 * j + q) * a.M + o) * 16 + quarter * 4) * G::kBytes
-                                         : kMixFar);
-            }
-        static_for<4>([&](auto ii) {
-            constexpr int I = decltype(ii)::value;
-            v4u fx[CT][PX], fg[OT][PG];
-#pragma unroll
-            for (int k = 0; k < CT; ++k) x[k].template operand<I>(fx[k]);
-#pragma unroll
-            for (int k = 0; k < OT; ++k) g[k].template operand<I>(fg[k]);
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int k = 0; k < CT; ++k)
 #pragma unroll
-                for (int o = 0; o < OT; ++o)
-                    acc[I > 0][k][o] = mix_mfma<PX, PG>(fx[k], fg[o], acc[I > 0][k][o]);
-        });
+                for (int o = 0; o < 4; ++o) give[((i * CT + k) * 4 + o) * 64] = acc[i][k][o];
     }
-    const int slab = quarter + (quarter + 1) / 2;          // 0 2 3 5
-    const bool one = quarter & 1;                          // one degree: the two sums together
-    float* part = a.part + ((int64_t)split * 6 + slab) * a.K * a.M;
+    __syncthreads();
+    if (quarter == 2) return;
 #pragma unroll
     for (int k = 0; k < CT; ++k)
 #pragma unroll
-        for (int o = 0; o < OT; ++o)
+        for (int o = 0; o < 4; ++o) {
+            v4f u = acc[0][k][o], v = acc[1][k][o];
+            if (quarter) u += v + give[((quarter / 2 * CT + k) * 4 + o) * 64];
+            const int l = quarter ? quarter / 2 + 2 : 0;
+            float* part = a.part + (split * 4 + l) * a.K * a.M;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int c = c0 + k * 16 + 4 * q + r, m = o0 + o * 16 + at;
+                const int c = c0 + (side * CT + k) * 16 + 4 * q + r, m = o0 + o * 16 + at;
                 if (c >= a.K || m >= a.M) continue;
-                const float u = acc[0][k][o][r], v = acc[1][k][o][r];
-                part[(int64_t)c * a.M + m] = one ? u + v : u;
-                if (!one) part[((int64_t)a.K + c) * a.M + m] = v;
+                part[(int64_t)c * a.M + m] = u[r];
+                if (!quarter) part[((int64_t)a.K + c) * a.M + m] = v[r];
             }
+        }
 }
 
-__global__ __launch_bounds__(1024) void mix_weight_sum_kernel(const float* __restrict__ part, int splits,
-                                                              int64_t cells, float* out) {
-    const int64_t col = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
-    const bool there = col < 4 * cells;
-    const int l = there ? (int)(col / cells) : 0;
-    const float* p = part + (l < 2 ? l : 2 * l - 2) * cells + (col - l * cells);
-    const float s = column_sum(there ? splits : 0, [&](int r) {
-        const float* v = p + r * 6 * cells;
-        return l < 2 ? v[0] : v[0] + v[cells];
-    });
-    if (threadIdx.x < 16 && there) out[col] = s;
+// Sums of part over the splits: 64 columns of four a workgroup, four threads a column
+__global__ __launch_bounds__(256) void mix_weight_sum_kernel(const float* __restrict__ part, int splits,
+                                                             int64_t cols, float* __restrict__ out) {
+    __shared__ float4 sh[4][64];
+    const int lane = threadIdx.x & 63, k = threadIdx.x >> 6;
+    const int64_t col = ((int64_t)blockIdx.x * 64 + lane) * 4;
+    float4 s = make_float4(0, 0, 0, 0);
+    if (col < cols) {
+#pragma unroll 8
+        for (int r = k; r < splits; r += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(part + r * cols + col);
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+    }
+    sh[k][lane] = s;
+    __syncthreads();
+    if (k || col >= cols) return;
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+        const float4 v = sh[i][lane];
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    *reinterpret_cast<float4*>(out + col) = s;
 }
 
 static bool mix_shape_ok(int64_t N, int C, int O, int dtype) {
@@ -748,21 +882,25 @@ static size_t mix_bytes(int K, int M) {
     return (size_t)((K + 31) / 32) * 4 * a.tiles * MixShape<T>::kPW * 64 * 16;
 }
 
-template <typename T, int KS, int OT, int OG>
-static int stay_launch(MixArgs a, hipStream_t s) {
-    constexpr int kBytes = StayShape<T>::bytes(OG), kPer = std::min(8 / (2 * OG), 163840 / kBytes);
-    auto kernel = mix_stay_kernel<T, KS, OT, OG>;
-    // more than 64 KB of LDS, allowed once on each device
-    static std::atomic<uint64_t> allowed{0};
+// More than 64 KB of LDS for a kernel, allowed once on each device
+static int mix_allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& allowed) {
     int device = 0;
     hipError_t rc = hipGetDevice(&device);
     if (rc != hipSuccess) return (int)rc;
     const uint64_t bit = device < 64 ? (uint64_t)1 << device : 0;
-    if (!(allowed.load(std::memory_order_relaxed) & bit)) {
-        rc = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-        if (rc != hipSuccess) return (int)rc;
-        allowed.fetch_or(bit, std::memory_order_relaxed);
-    }
+    if (allowed.load(std::memory_order_relaxed) & bit) return 0;
+    rc = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (rc != hipSuccess) return (int)rc;
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+    return 0;
+}
+
+template <typename T, int KS, int OT, int OG>
+static int stay_launch(MixArgs a, hipStream_t s) {
+    constexpr int kBytes = StayShape<T>::bytes(OG), kPer = std::min(8 / (2 * OG), 163840 / kBytes);
+    auto kernel = mix_stay_kernel<T, KS, OT, OG>;
+    static std::atomic<uint64_t> allowed{0};
+    if (const int rc = mix_allow_lds((const void*)kernel, kBytes, allowed)) return rc;
     a.chunks = (a.M + OG * OT * 16 - 1) / (OG * OT * 16);
     const int64_t tiles = ceil_div(a.n, 16), most = std::max(1, 32 * kPer / a.chunks);
     const int64_t streams = 8 * std::min(most, ceil_div(tiles, 8));
@@ -807,21 +945,30 @@ static int mix_run(MixArgs a, void* ws, hipStream_t s) {
     return (int)hipGetLastError();
 }
 
-// Ranges of atoms of gW: about 1024 workgroups of at least four steps, 64 MB of partial sums at most
+// Ranges of atoms of gW: about a workgroup for each compute unit, of one or two steps at least, 64 MB of partial
+// sums at most
 static int mix_splits(int64_t N, int C, int O) {
-    const int64_t tiles = ceil_div(C, 64) * ceil_div(O, 32);
-    const int64_t most = std::max<int64_t>(1, ((int64_t)1 << 24) / ((int64_t)6 * C * O));
-    return (int)std::max<int64_t>(
-        1, std::min({ceil_div(1024, tiles), ceil_div(N, 128), most}));
+    const int64_t tiles = ceil_div(C, C > 64 ? 128 : 64) * ceil_div(O, 64);
+    const int64_t most = std::max<int64_t>(1, ((int64_t)1 << 24) / ((int64_t)4 * C * O));
+    return (int)std::max<int64_t>(1, std::min({ceil_div(256, tiles), ceil_div(N, 16), most}));
 }
 
-template <typename X, typename G, int CT, int OT>
-static void mix_weight_run(MixArgs a, hipStream_t s) {
-    a.tiles = (a.K + 16 * CT - 1) / (16 * CT);
-    a.chunks = (a.M + 16 * OT - 1) / (16 * OT);
-    a.per_split = (int)ceil_div(ceil_div(a.n, 32), a.splits);
-    mix_weight_kernel<X, G, CT, OT>
-        <<<mix_grid(a.splits, a.tiles * a.chunks), 256, 0, s>>>(a);
+template <typename T, bool KEPT, int CT>
+static int mix_weight_run(MixArgs a, hipStream_t s) {
+    using S = GradShape<T, KEPT, CT>;
+    auto kernel = mix_weight_kernel<T, KEPT, CT>;
+    static std::atomic<uint64_t> allowed{0};
+    if (const int rc = mix_allow_lds((const void*)kernel, S::kBytes, allowed)) return rc;
+    a.tiles = (a.K + S::kIn - 1) / S::kIn;
+    a.chunks = (a.M + S::kOut - 1) / S::kOut;
+    a.per_split = (int)ceil_div(ceil_div(a.n, S::kAtoms), a.splits);
+    kernel<<<mix_grid(a.splits, a.tiles * a.chunks), 512, S::kBytes, s>>>(a);
+    return (int)hipGetLastError();
+}
+template <typename T>
+static int mix_weight_pick(const MixArgs& a, hipStream_t s) {
+    if (a.x) return mix_weight_run<T, false, 2>(a, s);
+    return a.K > 64 ? mix_weight_run<T, true, 4>(a, s) : mix_weight_run<T, true, 2>(a, s);
 }
 }  // namespace bmhip
 
@@ -849,7 +996,7 @@ extern "C" int batteries_channel_mixing(const void* x, const float* weight, void
 
 extern "C" size_t batteries_channel_mixing_weight_grad_workspace_bytes(int64_t N, int C, int O) {
     if (!mix_shape_ok(N, C, O, 0)) return 0;
-    return (size_t)mix_splits(N, C, O) * 6 * C * O * sizeof(float);
+    return (size_t)mix_splits(N, C, O) * 4 * C * O * sizeof(float);
 }
 
 extern "C" int batteries_channel_mixing_weight_grad(const void* x, const uint8_t* codes,
@@ -858,25 +1005,18 @@ extern "C" int batteries_channel_mixing_weight_grad(const void* x, const uint8_t
                                                     size_t workspace_bytes, hipStream_t stream) {
     if (!mix_shape_ok(N, C, O, dtype) || !gweight || (N > 0 && (!g || (!x && (!codes || !exps)))))
         return BM_ERR_ARG;
-    if (!aligned_to({x, g}, 16) || !aligned_to({codes}, 4)) return BM_ERR_ARG;
+    if (!aligned_to({x, g, codes, gweight, workspace}, 16)) return BM_ERR_ARG;
     if (workspace_bytes < batteries_channel_mixing_weight_grad_workspace_bytes(N, C, O) || !workspace)
         return BM_ERR_WORKSPACE;
     MixArgs a{};
     a.x = x; a.codes = codes; a.exps = exps; a.g = g; a.part = (float*)workspace; a.n = N; a.K = C;
     a.M = O; a.splits = mix_splits(N, C, O);
     if (N > 0) {
-        using F = Mix8<float>;
-        using B = Mix8<uint16_t>;
-        if (dtype == 0) {
-            if (x) mix_weight_run<F, F, 2, 2>(a, stream);
-            else mix_weight_run<MixKept, F, 4, 2>(a, stream);
-        } else {
-            if (x) mix_weight_run<B, B, 4, 2>(a, stream);
-            else mix_weight_run<MixKept, B, 4, 2>(a, stream);
-        }
+        const int rc = dtype == 0 ? mix_weight_pick<float>(a, stream) : mix_weight_pick<uint16_t>(a, stream);
+        if (rc) return rc;
     }
-    const int64_t cells = (int64_t)C * O;
-    mix_weight_sum_kernel<<<(unsigned)ceil_div(4 * cells, 16), 1024, 0, stream>>>(
-        a.part, N > 0 ? a.splits : 0, cells, gweight);
+    const int64_t cols = (int64_t)4 * C * O;
+    mix_weight_sum_kernel<<<(unsigned)ceil_div(cols, 256), 256, 0, stream>>>(
+        a.part, N > 0 ? a.splits : 0, cols, gweight);
     return (int)hipGetLastError();
 }

@@ -651,7 +651,7 @@ int batteries_layer_norm_backward(const void* x, const float* weight, const void
  * with max |x| <= 448 times it, within [2^-110, 2^120]; codes are rounded to nearest even.  A value
  * that is not finite becomes NaN and has no part in the maximum; what would round to 2^128 becomes
  * 240 * 2^120.  fp32 (dtype 0) or bf16 (dtype 1);
- * x 16-byte, codes 8-byte aligned; C <= 2048, N ceil(C / 8) < 2^31.
+ * x 16-byte, codes 8-byte aligned (16-byte for the mixing's gradient below); C <= 2048, N ceil(C / 8) < 2^31.
  * ------------------------------------------------------------------------- */
 int batteries_checkpoint_encode(const void* x, uint8_t* codes, uint8_t* exps, int64_t N, int C,
                                 int dtype, hipStream_t stream);
