@@ -24,6 +24,11 @@ struct LnArgs {
     float eps, inv;                        // inv: 1 / D
 };
 
+// 16 bytes at any address that an element may have (the hardware takes unaligned vectors)
+struct __attribute__((packed, aligned(2))) Ln16 {
+    uint32_t v[4];
+};
+
 // VEC elements in 16 bytes (or one element) as fp32
 template <typename T, int VEC>
 struct LnVec {
@@ -31,23 +36,26 @@ struct LnVec {
     __device__ __forceinline__ void load(const T* p) {
         if constexpr (VEC == 1) {
             v[0] = norm_ld(p);
-        } else if constexpr (sizeof(T) == 4) {
-            const float4 t = *reinterpret_cast<const float4*>(p);
-            v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
         } else {
-            const uint4 t = *reinterpret_cast<const uint4*>(p);
-            v[0] = bf16_lo(t.x), v[1] = bf16_hi(t.x), v[2] = bf16_lo(t.y), v[3] = bf16_hi(t.y);
-            v[4] = bf16_lo(t.z), v[5] = bf16_hi(t.z), v[6] = bf16_lo(t.w), v[7] = bf16_hi(t.w);
+            const Ln16 t = *reinterpret_cast<const Ln16*>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (VEC == 4) v[i] = __uint_as_float(t.v[i]);
+                else v[2 * i] = bf16_lo(t.v[i]), v[2 * i + 1] = bf16_hi(t.v[i]);
+            }
         }
     }
     __device__ __forceinline__ void store(T* p) const {
         if constexpr (VEC == 1) {
             norm_st(p, v[0]);
-        } else if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
         } else {
-            *reinterpret_cast<uint4*>(p) = make_uint4(bf16_pack(v[0], v[1]), bf16_pack(v[2], v[3]),
-                                                      bf16_pack(v[4], v[5]), bf16_pack(v[6], v[7]));
+            Ln16 t;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (VEC == 4) t.v[i] = __float_as_uint(v[i]);
+                else t.v[i] = bf16_pack(v[2 * i], v[2 * i + 1]);
+            }
+            *reinterpret_cast<Ln16*>(p) = t;
         }
     }
     __device__ __forceinline__ void zero() {
@@ -72,76 +80,103 @@ __device__ __forceinline__ float ln_sum(float v, float* sh, int& turn) {
     return v;
 }
 
-// Takes the mean m off a lane's part of a row and returns r.  The rounding of m, which is large next to
-// the differences of a row far from 0, shows in the differences' own mean: that is taken off as well.
-template <int LPR, int W, typename T, int VEC, int NV>
-__device__ __forceinline__ float ln_center(const LnArgs& a, int t, float m, LnVec<T, VEC> (&x)[NV],
-                                           float* sh, int& turn) {
+// Where a lane's vector i of a row lies.  The last one of a row that is no whole number of vectors
+// begins earlier (TAIL), so that it ends with the row: its first `skip` elements are another lane's, are worked
+// out twice, and have no part in the sums.
+template <int VEC, bool TAIL>
+struct LnAt {
+    int c, skip;
+    bool there;
+    __device__ __forceinline__ LnAt(int unit, int D) {
+        const int first = unit * VEC;
+        there = first < D;
+        c = TAIL ? min(first, D - VEC) : first;
+        skip = TAIL ? first - c : 0;
+    }
+    __device__ __forceinline__ bool counts(int j) const { return there && (!TAIL || j >= skip); }
+};
+
+// Takes the mean off a lane's part of a row and returns r.  The rounding of the mean, which is large next
+// to the differences of a row far from 0, shows in the differences' own mean: that is taken off as well.
+template <int LPR, int W, bool TAIL, typename T, int VEC, int NV>
+__device__ __forceinline__ float ln_center(const LnArgs& a, int t, LnVec<T, VEC> (&x)[NV], float* sh,
+                                           int& turn) {
     constexpr int kLanes = W == 1 ? LPR : 64 * W;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const LnAt<VEC, TAIL> at(i * kLanes + t, a.D);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s += !TAIL || at.counts(j) ? x[i].v[j] : 0.0f;
+    }
+    const float m = ln_sum<LPR, W>(s, sh, turn) * a.inv;
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if ((i * kLanes + t) * VEC < a.D) {
+    for (int i = 0; i < NV; ++i) {
+        const LnAt<VEC, TAIL> at(i * kLanes + t, a.D);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                x[i].v[j] -= m;
-                s1 += x[i].v[j];
-                s2 = fmaf(x[i].v[j], x[i].v[j], s2);
-            }
+        for (int j = 0; j < VEC; ++j) {
+            x[i].v[j] -= m;
+            const float d = at.counts(j) ? x[i].v[j] : 0.0f;
+            s1 += d;
+            s2 = fmaf(d, d, s2);
         }
+    }
     s1 = ln_sum<LPR, W>(s1, sh, turn) * a.inv;
     s2 = ln_sum<LPR, W>(s2, sh, turn) * a.inv;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-        if ((i * kLanes + t) * VEC < a.D) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) x[i].v[j] -= s1;
-        }
+        for (int j = 0; j < VEC; ++j) x[i].v[j] -= s1;
     return 1.0f / sqrtf(fmaxf(fmaf(-s1, s1, s2), 0.0f) + a.eps);
 }
 
 template <int W>
 constexpr int ln_threads() { return W == 1 ? 256 : 64 * W; }
 
-// A lane's part of a row: NV vectors, LPR * W vectors apart
-template <typename T, int VEC, int NV, int LPR, int W, int ROWS>
+// Workgroups take rows in turn, ROWS at a time for a group of lanes, whose loads are all asked for first;
+// the weights stay in registers.
+template <typename T, int VEC, int NV, int LPR, int W, int ROWS, bool TAIL>
 __global__ __launch_bounds__(ln_threads<W>()) void ln_fwd_kernel(LnArgs a) {
     __shared__ float sh[2 * 16];
     int turn = 0;
     constexpr int kGroups = W == 1 ? 4 * (64 / LPR) : 1, kLanes = W == 1 ? LPR : 64 * W;
     const int t = W == 1 ? threadIdx.x % LPR : threadIdx.x;
     const int group = W == 1 ? threadIdx.x / LPR : 0;
-    const int64_t row0 = (int64_t)blockIdx.x * kGroups * ROWS + group;
-    LnVec<T, VEC> x[ROWS][NV];
+    float w[NV][VEC], b[NV][VEC];
 #pragma unroll
-    for (int k = 0; k < ROWS; ++k) {
-        const int64_t row = min(row0 + k * kGroups, a.rows - 1);
-        const T* p = (const T*)a.x + row * a.row_stride;
+    for (int i = 0; i < NV; ++i) {
+        const LnAt<VEC, TAIL> at(i * kLanes + t, a.D);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * kLanes + t) * VEC;
-            if (c < a.D) x[k][i].load(p + (VEC == 1 ? c * a.step : c));
-            else x[k][i].zero();
+        for (int j = 0; j < VEC; ++j) {
+            w[i][j] = at.there ? a.w[at.c + j] : 0.0f;
+            b[i][j] = at.there && a.b ? a.b[at.c + j] : 0.0f;
         }
     }
+    for (int64_t row0 = (int64_t)blockIdx.x * kGroups * ROWS + group; row0 - group < a.rows;
+         row0 += (int64_t)gridDim.x * kGroups * ROWS) {
+        LnVec<T, VEC> x[ROWS][NV];
 #pragma unroll
-    for (int k = 0; k < ROWS; ++k) {
-        const int64_t row = row0 + k * kGroups;
-        float s = 0.0f;
+        for (int k = 0; k < ROWS; ++k) {
+            const int64_t row = min(row0 + k * kGroups, a.rows - 1);
+            const T* p = (const T*)a.x + row * a.row_stride;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+            for (int i = 0; i < NV; ++i) {
+                const LnAt<VEC, TAIL> at(i * kLanes + t, a.D);
+                x[k][i].zero();
+                if (at.there) x[k][i].load(p + (VEC == 1 ? at.c * a.step : at.c));
+            }
+        }
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) s += x[k][i].v[j];
-        const float m = ln_sum<LPR, W>(s, sh, turn) * a.inv;
-        const float r = ln_center<LPR, W>(a, t, m, x[k], sh, turn);
+        for (int k = 0; k < ROWS; ++k) {
+            const int64_t row = row0 + k * kGroups;
+            const float r = ln_center<LPR, W, TAIL>(a, t, x[k], sh, turn);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * kLanes + t) * VEC;
-            if (c < a.D && row < a.rows) {
+            for (int i = 0; i < NV; ++i) {
+                const LnAt<VEC, TAIL> at(i * kLanes + t, a.D);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    x[k][i].v[j] = fmaf(x[k][i].v[j] * r, a.w[c + j], a.b ? a.b[c + j] : 0.0f);
-                x[k][i].store((T*)a.y + row * a.D + c);
+                for (int j = 0; j < VEC; ++j) x[k][i].v[j] = fmaf(x[k][i].v[j] * r, w[i][j], b[i][j]);
+                if (at.there && row < a.rows) x[k][i].store((T*)a.y + row * a.D + at.c);
             }
         }
     }
@@ -149,7 +184,7 @@ __global__ __launch_bounds__(ln_threads<W>()) void ln_fwd_kernel(LnArgs a) {
 
 // Workgroups take rows in turn; a lane keeps its columns' sums of g xh and g in registers, which are
 // joined over the workgroup's rows at the end: part [gridDim.x, 2, D].
-template <typename T, int VEC, int NV, int LPR, int W>
+template <typename T, int VEC, int NV, int LPR, int W, bool TAIL>
 __global__ __launch_bounds__(ln_threads<W>()) void ln_bwd_kernel(LnArgs a) {
     __shared__ float sh[2 * 16];
     constexpr int kCols = NV * LPR * VEC;
@@ -170,35 +205,30 @@ __global__ __launch_bounds__(ln_threads<W>()) void ln_bwd_kernel(LnArgs a) {
         LnVec<T, VEC> x[NV], g[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * kLanes + t) * VEC;
+            const LnAt<VEC, TAIL> at(i * kLanes + t, a.D);
             x[i].zero();
             g[i].zero();
-            if (c < a.D && there) {
-                x[i].load((const T*)a.x + row * a.row_stride + (VEC == 1 ? c * a.step : c));
-                g[i].load((const T*)a.g + row * a.D + c);
+            if (at.there && there) {
+                x[i].load((const T*)a.x + row * a.row_stride + (VEC == 1 ? at.c * a.step : at.c));
+                g[i].load((const T*)a.g + row * a.D + at.c);
             }
         }
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) s += x[i].v[j];
-        const float m = ln_sum<LPR, W>(s, sh, turn) * a.inv;
-        const float r = ln_center<LPR, W>(a, t, m, x, sh, turn);
+        const float r = ln_center<LPR, W, TAIL>(a, t, x, sh, turn);
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * kLanes + t) * VEC;
-            if (c < a.D) {
+            const LnAt<VEC, TAIL> at(i * kLanes + t, a.D);
+            if (at.there) {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
                     const float xh = x[i].v[j] * r;
                     gw[i][j] = fmaf(g[i].v[j], xh, gw[i][j]);
                     gb[i][j] += g[i].v[j];
                     x[i].v[j] = xh;
-                    g[i].v[j] *= a.w[c + j];
-                    s1 += g[i].v[j];
-                    s2 = fmaf(g[i].v[j], xh, s2);
+                    g[i].v[j] *= a.w[at.c + j];
+                    const float u = at.counts(j) ? g[i].v[j] : 0.0f;
+                    s1 += u;
+                    s2 = fmaf(u, xh, s2);
                 }
             }
         }
@@ -206,12 +236,12 @@ __global__ __launch_bounds__(ln_threads<W>()) void ln_bwd_kernel(LnArgs a) {
         s2 = ln_sum<LPR, W>(s2, sh, turn) * a.inv;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * kLanes + t) * VEC;
-            if (c < a.D && there) {
+            const LnAt<VEC, TAIL> at(i * kLanes + t, a.D);
+            if (at.there && there) {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j)
                     g[i].v[j] = r * (g[i].v[j] - s1 - x[i].v[j] * s2);
-                g[i].store((T*)a.gx + row * a.D + c);
+                g[i].store((T*)a.gx + row * a.D + at.c);
             }
         }
     }
@@ -220,20 +250,21 @@ __global__ __launch_bounds__(ln_threads<W>()) void ln_bwd_kernel(LnArgs a) {
     for (int k = 0; k < 2; ++k) {
         if constexpr (W == 1) __syncthreads();
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            const LnAt<VEC, TAIL> at(i * kLanes + t, a.D);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 float v = k ? gb[i][j] : gw[i][j];
                 if constexpr (W == 1) {
 #pragma unroll
                     for (int o = LPR; o < 64; o <<= 1) v += __shfl_xor(v, o);
-                    if ((threadIdx.x & 63) < LPR)
-                        red[(threadIdx.x >> 6) * kCols + (i * LPR + t) * VEC + j] = v;
-                } else {
-                    const int c = (i * kLanes + t) * VEC + j;
-                    if (c < a.D) part[k * a.D + c] = v;
+                    if ((threadIdx.x & 63) < LPR && at.counts(j))
+                        red[(threadIdx.x >> 6) * kCols + at.c + j] = v;
+                } else if (at.counts(j)) {
+                    part[k * a.D + at.c + j] = v;
                 }
             }
+        }
         if constexpr (W == 1) {
             __syncthreads();
             for (int c = threadIdx.x; c < a.D; c += 256)
@@ -261,49 +292,43 @@ static int ln_parts(int64_t rows, int D) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, 8 * groups), 1024));
 }
 
-template <typename T, int VEC, int NV, int LPR, int W>
+template <typename T, int VEC, int NV, int LPR, int W, bool TAIL>
 static void ln_launch(const LnArgs& a, bool bwd, hipStream_t s) {
     constexpr int kGroups = W == 1 ? 4 * (64 / LPR) : 1;
     constexpr int kRows = W > 1 ? 1 : NV * VEC <= 8 ? 4 : NV * VEC <= 16 ? 2 : 1;
     if (bwd) {
-        ln_bwd_kernel<T, VEC, NV, LPR, W><<<ln_parts(a.rows, a.D), ln_threads<W>(), 0, s>>>(a);
+        ln_bwd_kernel<T, VEC, NV, LPR, W, TAIL><<<ln_parts(a.rows, a.D), ln_threads<W>(), 0, s>>>(a);
         return;
     }
-    constexpr int64_t kMost = (int64_t)1 << 20;     // workgroups of a launch
-    LnArgs b = a;
-    for (int64_t row = 0; row < a.rows; row += kMost * kGroups * kRows) {
-        b.x = (const T*)a.x + row * a.row_stride;
-        b.y = (T*)a.y + row * a.D;
-        b.rows = std::min(a.rows - row, kMost * kGroups * kRows);
-        ln_fwd_kernel<T, VEC, NV, LPR, W, kRows>
-            <<<(unsigned)ceil_div(b.rows, kGroups * kRows), ln_threads<W>(), 0, s>>>(b);
-    }
+    const int64_t most = W == 16 ? 512 : 2048;      // workgroups: what the card holds at once
+    ln_fwd_kernel<T, VEC, NV, LPR, W, kRows, TAIL>
+        <<<(unsigned)std::min(ceil_div(a.rows, kGroups * kRows), most), ln_threads<W>(), 0, s>>>(a);
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool TAIL>
 static void ln_pick(const LnArgs& a, bool bwd, hipStream_t s) {
     const int units = (a.D + VEC - 1) / VEC;
-    if (units <= 8) ln_launch<T, VEC, 1, 8, 1>(a, bwd, s);
-    else if (units <= 16) ln_launch<T, VEC, 1, 16, 1>(a, bwd, s);
-    else if (units <= 32) ln_launch<T, VEC, 1, 32, 1>(a, bwd, s);
-    else if (units <= 64) ln_launch<T, VEC, 1, 64, 1>(a, bwd, s);
-    else if (units <= 128) ln_launch<T, VEC, 2, 64, 1>(a, bwd, s);
-    else if (units <= 256) ln_launch<T, VEC, 4, 64, 1>(a, bwd, s);
-    else if (units <= 512) ln_launch<T, VEC, 2, 64, 4>(a, bwd, s);
-    else if (units <= 1024) ln_launch<T, VEC, 4, 64, 4>(a, bwd, s);
+    if (units <= 8) ln_launch<T, VEC, 1, 8, 1, TAIL>(a, bwd, s);
+    else if (units <= 16) ln_launch<T, VEC, 1, 16, 1, TAIL>(a, bwd, s);
+    else if (units <= 32) ln_launch<T, VEC, 1, 32, 1, TAIL>(a, bwd, s);
+    else if (units <= 64) ln_launch<T, VEC, 1, 64, 1, TAIL>(a, bwd, s);
+    else if (units <= 128) ln_launch<T, VEC, 2, 64, 1, TAIL>(a, bwd, s);
+    else if (units <= 256) ln_launch<T, VEC, 4, 64, 1, TAIL>(a, bwd, s);
+    else if (units <= 512) ln_launch<T, VEC, 2, 64, 4, TAIL>(a, bwd, s);
+    else if (units <= 1024) ln_launch<T, VEC, 4, 64, 4, TAIL>(a, bwd, s);
     else if constexpr (kLnMaxD / VEC > 1024) {
-        if (units <= 2048) ln_launch<T, VEC, 2, 64, 16>(a, bwd, s);
-        else if constexpr (kLnMaxD / VEC > 2048) ln_launch<T, VEC, 8, 64, 16>(a, bwd, s);
+        if (units <= 2048) ln_launch<T, VEC, 2, 64, 16, TAIL>(a, bwd, s);
+        else if constexpr (kLnMaxD / VEC > 2048) ln_launch<T, VEC, 8, 64, 16, TAIL>(a, bwd, s);
     }
 }
 
+// 16 bytes a lane where a row's elements follow each other, at any alignment; else one element
 template <typename T>
 static void ln_run(const LnArgs& a, bool bwd, hipStream_t s) {
     constexpr int VEC = 16 / sizeof(T);
-    const bool vec = a.D % VEC == 0 && a.step == 1 && (a.row_stride % VEC == 0 || a.rows <= 1) &&
-                     aligned_to({a.x, a.g, a.y, a.gx}, 16);
-    if (vec) ln_pick<T, VEC>(a, bwd, s);
-    else ln_pick<T, 1>(a, bwd, s);
+    if (a.step != 1 || a.D < VEC) ln_pick<T, 1, false>(a, bwd, s);
+    else if (a.D % VEC == 0) ln_pick<T, VEC, false>(a, bwd, s);
+    else ln_pick<T, VEC, true>(a, bwd, s);
 }
 
 static bool ln_shape_ok(int64_t rows, int D, int dtype) {

@@ -630,8 +630,8 @@ int batteries_distance_bias_backward(const float* lengths, const uint16_t* bucke
  *   y = (x - mean) / sqrt(mean of (x - mean)^2 + eps) * weight + bias
  * x: `rows` rows of D elements in fp32 (dtype 0) or bf16 (dtype 1), at row_stride, the elements of a
  * row `step` apart (both in elements); y dense, weight [D] and bias [D] (NULL: 0) fp32.
- * D <= 8192, rows < 2^38.  Rows of whole 16-byte units at such strides and addresses are read 16
- * bytes a lane, others element by element.
+ * D <= 8192, rows < 2^38.  Rows with step 1 are read 16 bytes a lane at any alignment, others element
+ * by element.
  * ------------------------------------------------------------------------- */
 int batteries_layer_norm(const void* x, const float* weight, const float* bias, void* y, int64_t rows,
                          int D, int64_t row_stride, int64_t step, float eps, int dtype,
