@@ -10,6 +10,8 @@
 //
 // (c - r) (c + r) in place of c^2 - r^2: next to the cutoff the difference is exact.  A length that is
 // not a number gives a bias that is none.
+#include <type_traits>
+
 #include "sums.h"
 #include "batmobile_hip.h"
 
@@ -89,13 +91,15 @@ __global__ __launch_bounds__(256) void bias_fwd_kernel(BiasArgs a) {
 }
 
 // Table gradient.  A wave holds 64 columns of sums in LDS for each of its (at most 64) buckets; lane
-// (slot s, head h) adds the values of its edges to its own column alone, so no two lanes meet, the order
-// is the edges', and a step costs one LDS addition.  More than 64 buckets: the waves of a workgroup take
-// ranges of 64 and read the same edges; more than 256: gridDim.y ranges of 256.  The columns' sums go
-// to part [gridDim.x, B, H].  Heads past 64: gridDim.z.
+// (slot s, head h) adds the values of its edges to its own column alone, so no two lanes meet and the order
+// is the edges'.  It reads, adds and writes: the LDS's own addition takes 3 cycles a lane (1.4 M edges x 8
+// heads in 64 buckets 66 us, so 18).  More than 64 buckets: the waves of a workgroup take ranges of 64 and
+// read the same edges, of which each adds a part (256 buckets 40 us); more than 256: gridDim.y ranges of
+// 256.  The columns' sums go to part [gridDim.x, B, H].  Heads past 64: gridDim.z.
+template <bool RANGES>
 __global__ __launch_bounds__(256) void bias_bwd_kernel(BiasArgs a, int range_waves) {
     extern __shared__ __attribute__((aligned(16))) float sh[];
-    const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+    const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int h0 = blockIdx.z * 64, H = min(64, a.H - h0), slots = 64 / H;
     const int range = w % range_waves, sub = w / range_waves, subs = 4 / range_waves;
     const int b0 = (blockIdx.y * range_waves + range) * kBiasRange, per = min(a.B, kBiasRange);
@@ -104,26 +108,54 @@ __global__ __launch_bounds__(256) void bias_bwd_kernel(BiasArgs a, int range_wav
     const int s = lane / H, h = lane - s * H;
     const int64_t share = (a.edges + gridDim.x - 1) / gridDim.x;
     const int64_t first = blockIdx.x * share, last = min(a.edges, first + share);
-    const int step = slots * subs;
-    constexpr int kAhead = 8;
-    if (s < slots) {
-        for (int64_t e = first + sub * slots + s; e < last; e += (int64_t)step * kAhead) {
-            float v[kAhead];
-            int k[kAhead];
+    const int step = slots * subs, from = sub * slots + s;
+    // steps whose loads are under way, and steps that read, add and write together
+    constexpr int kAhead = RANGES ? 16 : 8, kTogether = RANGES ? 2 : 1;
+    auto batch = [&](int64_t e0, auto whole) {             // kAhead steps from edge e0 on
+        const float* g = a.g + e0 * a.H + h0;
+        const uint16_t* bucket = a.bucket + e0;
+        const int left = (int)min(last - e0, (int64_t)1 << 20);
+        float v[kAhead];
+        int k[kAhead];
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const int64_t ei = min(e + (int64_t)i * step, last - 1);
-                k[i] = a.bucket[ei];
-                v[i] = a.g[ei * a.H + h0 + h];
-            }
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const int b = k[i] - b0;
-                if (e + (int64_t)i * step < last && b >= 0 && b < per)
-                    __hip_atomic_fetch_add(&mine[b * 64 + lane], v[i], __ATOMIC_RELAXED,
-                                           __HIP_MEMORY_SCOPE_WORKGROUP);
-            }
+        for (int i = 0; i < kAhead; ++i) {
+            int e = from + i * step;
+            if (!decltype(whole)::value) e = min(e, left - 1);
+            k[i] = bucket[(uint32_t)e];
+            v[i] = g[(uint32_t)(e * a.H + h)];
         }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            // an edge of another range, or past the last, adds 0 to some bucket
+            bool there = true;
+            if (RANGES) k[i] -= b0, there = (unsigned)k[i] < (unsigned)per;
+            if (!decltype(whole)::value) there = there && from + i * step < left;
+            if (RANGES || !decltype(whole)::value) {
+                k[i] = there ? k[i] : 0;
+                v[i] = there ? v[i] : 0.0f;
+            }
+            k[i] = k[i] * 64 + lane;
+        }
+#pragma unroll
+        for (int i0 = 0; i0 < kAhead; i0 += kTogether) {
+            float sum[kTogether];
+#pragma unroll
+            for (int i = 0; i < kTogether; ++i) sum[i] = mine[k[i0 + i]];
+#pragma unroll
+            for (int i = 0; i < kTogether; ++i) {
+                // a bucket that came before in the group goes on from there
+#pragma unroll
+                for (int j = 0; j < i; ++j) sum[i] = k[i0 + j] == k[i0 + i] ? sum[j] : sum[i];
+                sum[i] += v[i0 + i];
+            }
+#pragma unroll
+            for (int i = 0; i < kTogether; ++i) mine[k[i0 + i]] = sum[i];
+        }
+    };
+    if (s < slots) {
+        int64_t e = first;
+        for (; e + kAhead * step <= last; e += kAhead * step) batch(e, std::true_type{});
+        if (e < last) batch(e, std::false_type{});
     }
     __syncthreads();
     for (int i = t; i < range_waves * per * H; i += 256) {
@@ -145,24 +177,49 @@ __global__ __launch_bounds__(1024) void bias_table_kernel(const float* part, int
     if (threadIdx.x < 16 && col < cols) out[col] = s;
 }
 
-// A lane an edge
-template <bool VEC>
+// LANES lanes an edge
+template <bool VEC, int LANES>
 __global__ __launch_bounds__(256) void bias_lengths_kernel(BiasArgs a) {
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t e = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
     if (e >= a.edges) return;
+    const int lane = threadIdx.x % LANES;
     const float r = a.lengths[e];
     float s = 0.0f;
     if constexpr (VEC) {
         const float4* p = reinterpret_cast<const float4*>(a.g + e * a.H);
-        for (int i = 0; i < a.H / 4; ++i) {
+        for (int i = lane; i < a.H / 4; i += LANES) {
             const float4 v = p[i];
             s += (v.x + v.y) + (v.z + v.w);
         }
     } else {
-        for (int i = 0; i < a.H; ++i) s += a.g[e * a.H + i];
+        for (int i = lane; i < a.H; i += LANES) s += a.g[e * a.H + i];
     }
+    if constexpr (LANES > 1) s = lanes_sum<LANES>(s);
     const bool in = fabsf(r) < a.cutoff;
-    a.glengths[e] = in ? s * (-2.0f * r / ((a.cutoff - r) * (a.cutoff + r))) : r != r ? r : 0.0f;
+    if (lane == 0)
+        a.glengths[e] = in ? s * (-2.0f * r / ((a.cutoff - r) * (a.cutoff + r))) : r != r ? r : 0.0f;
+}
+
+template <bool VEC, int LANES>
+static void bias_lengths_launch(const BiasArgs& a, hipStream_t s) {
+    constexpr int64_t kEdges = ((int64_t)1 << 22) * (256 / LANES);     // of a launch
+    for (int64_t e = 0; e < a.edges; e += kEdges) {
+        BiasArgs b = a;
+        b.lengths = a.lengths + e;
+        b.g = a.g + e * a.H;
+        b.glengths = a.glengths + e;
+        b.edges = std::min(a.edges - e, kEdges);
+        bias_lengths_kernel<VEC, LANES><<<(unsigned)ceil_div(b.edges, 256 / LANES), 256, 0, s>>>(b);
+    }
+}
+// One or two loads a lane (500,000 edges of 64 heads with a lane an edge: 97 us, with
+// 16 lanes 22)
+template <bool VEC>
+static void bias_lengths_run(const BiasArgs& a, hipStream_t s) {
+    const int loads = VEC ? a.H / 4 : a.H;
+    if (loads <= 2) bias_lengths_launch<VEC, 1>(a, s);
+    else if (loads <= 8) bias_lengths_launch<VEC, 4>(a, s);
+    else bias_lengths_launch<VEC, 16>(a, s);
 }
 
 static bool bias_shape_ok(int64_t E, int H, int B) {
@@ -229,25 +286,17 @@ extern "C" int batteries_distance_bias_backward(const float* lengths, const uint
         if (parts) {
             const dim3 grid((unsigned)parts, (unsigned)ceil_div(B, kBiasRange * rw),
                             (unsigned)ceil_div(H, 64));
-            bias_bwd_kernel<<<grid, 256, 4 * std::min(B, kBiasRange) * 64 * sizeof(float), stream>>>(
-                a, rw);
+            const size_t lds = 4 * std::min(B, kBiasRange) * 64 * sizeof(float);
+            if (rw > 1) bias_bwd_kernel<true><<<grid, 256, lds, stream>>>(a, rw);
+            else bias_bwd_kernel<false><<<grid, 256, lds, stream>>>(a, rw);
         }
         const int64_t cols = (int64_t)B * H;
         bias_table_kernel<<<(unsigned)ceil_div(cols, 16), 1024, 0, stream>>>(a.part, parts, cols,
                                                                             gtable);
     }
     if (glengths && E > 0) {
-        constexpr int64_t kMost = (int64_t)1 << 22;     // workgroups of a launch
-        for (int64_t e = 0; e < E; e += kMost * 256) {
-            BiasArgs b = a;
-            b.lengths = lengths + e;
-            b.g = g + e * H;
-            b.glengths = glengths + e;
-            b.edges = std::min(E - e, kMost * 256);
-            const unsigned grid = (unsigned)ceil_div(b.edges, 256);
-            if (H % 4 == 0 && aligned_to({g}, 16)) bias_lengths_kernel<true><<<grid, 256, 0, stream>>>(b);
-            else bias_lengths_kernel<false><<<grid, 256, 0, stream>>>(b);
-        }
+        if (H % 4 == 0 && aligned_to({g}, 16)) bias_lengths_run<true>(a, stream);
+        else bias_lengths_run<false>(a, stream);
     }
     return (int)hipGetLastError();
 }
