@@ -613,7 +613,7 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 
 template <typename T, bool KEPT, int CT>
 struct GradShape {
-    static constexpr int kB = sizeof(T), kAtoms = kB == 2 ? 16 : 8;
+    static constexpr int kB = sizeof(T), kAtoms = kB == 2 || KEPT ? 16 : 8;
     static constexpr int kIn = 32 * CT, kOut = 64;                 // channels
     static constexpr int kXB = KEPT ? 1 : kB;                      // bytes of a value of x
     static constexpr int kX = kAtoms * kIn * 16 * kXB, kG = kAtoms * kOut * 16 * kB;
@@ -635,7 +635,6 @@ template <>
 struct Four<float> {
     float4 v;
     __device__ __forceinline__ void load(const char* p) { v = *reinterpret_cast<const float4*>(p); }
-    __device__ __forceinline__ void decode(unsigned code, float up) { v = ckpt_decode4(code, up); }
     __device__ __forceinline__ void zero() { v = make_float4(0, 0, 0, 0); }
     template <int I>
     __device__ __forceinline__ float get() const {
@@ -673,6 +672,38 @@ __device__ __forceinline__ void grad_products(const Four<uint16_t> (&x)[CT][4], 
 #pragma unroll
         for (int o = 0; o < 4; ++o)
             acc[k][o] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(e, f[o], acc[k][o], 0, 0, 0);
+    }
+}
+template <int I, int CT>
+__device__ __forceinline__ void grad_products(const Four<uint16_t> (&x)[CT][4], const Four<float> (&g)[4][4],
+                                              v4f (&acc)[CT][4]) {
+    constexpr unsigned kSel = I % 2 ? 0x07060302u : 0x05040100u, kHigh = 0x07060302u;
+    v4s e[CT];
+#pragma unroll
+    for (int k = 0; k < CT; ++k)
+        e[k] = __builtin_bit_cast(v4s, uint2{__builtin_amdgcn_perm(x[k][1].v[I / 2], x[k][0].v[I / 2], kSel),
+                                             __builtin_amdgcn_perm(x[k][3].v[I / 2], x[k][2].v[I / 2], kSel)});
+#pragma unroll
+    for (int o = 0; o < 4; ++o) {
+        uint2 f[3];
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = g[o][j].template get<I>();
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {                      // the leading bits, and what is left
+            f[p].x = __builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), kHigh);
+            f[p].y = __builtin_amdgcn_perm(__float_as_uint(v[3]), __float_as_uint(v[2]), kHigh);
+            if (p < 2) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] -= __uint_as_float(__float_as_uint(v[j]) & 0xffff0000u);
+            }
+        }
+#pragma unroll
+        for (int p = 2; p >= 0; --p)
+#pragma unroll
+            for (int k = 0; k < CT; ++k)
+                acc[k][o] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
+                    e[k], __builtin_bit_cast(v4s, f[p]), acc[k][o], 0, 0, 0);
     }
 }
 template <int I, int CT>
@@ -762,7 +793,8 @@ __global__ __launch_bounds__(512, 2) void mix_weight_kernel(MixArgs a) {
         __syncthreads();
         if (n0 + S::kAtoms < end) ask(n0 + S::kAtoms, sh + (turn ^ 1) * S::kStep);
         const char* from = sh + turn * S::kStep;
-        Four<T> x[CT][kJ], g[4][kJ];
+        Four<typename std::conditional<KEPT, uint16_t, T>::type> x[CT][kJ];
+        Four<T> g[4][kJ];
 #pragma unroll
         for (int k = 0; k < CT; ++k)
 #pragma unroll
@@ -945,8 +977,8 @@ static int mix_run(MixArgs a, void* ws, hipStream_t s) {
     return (int)hipGetLastError();
 }
 
-// Ranges of atoms of gW: about a workgroup for each compute unit, of one or two steps at least, 64 MB of partial
-// sums at most
+// Most ranges of atoms of gW: a workgroup for each compute unit, of one or two steps at least, 64 MB of
+// partial sums at most
 static int mix_splits(int64_t N, int C, int O) {
     const int64_t tiles = ceil_div(C, C > 64 ? 128 : 64) * ceil_div(O, 64);
     const int64_t most = std::max<int64_t>(1, ((int64_t)1 << 24) / ((int64_t)4 * C * O));
@@ -954,21 +986,24 @@ static int mix_splits(int64_t N, int C, int O) {
 }
 
 template <typename T, bool KEPT, int CT>
-static int mix_weight_run(MixArgs a, hipStream_t s) {
+static int mix_weight_run(MixArgs& a, hipStream_t s) {
     using S = GradShape<T, KEPT, CT>;
     auto kernel = mix_weight_kernel<T, KEPT, CT>;
     static std::atomic<uint64_t> allowed{0};
     if (const int rc = mix_allow_lds((const void*)kernel, S::kBytes, allowed)) return rc;
     a.tiles = (a.K + S::kIn - 1) / S::kIn;
     a.chunks = (a.M + S::kOut - 1) / S::kOut;
+    a.splits = std::min(a.splits, (int)ceil_div(256, a.tiles * a.chunks));
     a.per_split = (int)ceil_div(ceil_div(a.n, S::kAtoms), a.splits);
     kernel<<<mix_grid(a.splits, a.tiles * a.chunks), 512, S::kBytes, s>>>(a);
     return (int)hipGetLastError();
 }
 template <typename T>
-static int mix_weight_pick(const MixArgs& a, hipStream_t s) {
+static int mix_weight_pick(MixArgs& a, hipStream_t s) {
     if (a.x) return mix_weight_run<T, false, 2>(a, s);
-    return a.K > 64 ? mix_weight_run<T, true, 4>(a, s) : mix_weight_run<T, true, 2>(a, s);
+    if constexpr (sizeof(T) == 2)
+        if (a.K > 64) return mix_weight_run<T, true, 4>(a, s);
+    return mix_weight_run<T, true, 2>(a, s);
 }
 }  // namespace bmhip
 
