@@ -62,23 +62,26 @@ std::tuple<Tensor, Tensor> distance_bias(const Tensor& lengths_, const Tensor& b
 }
 
 // (grad_table, grad_lengths), each if wanted
-std::tuple<Tensor, Tensor> distance_bias_backward(const Tensor& lengths_, const Tensor& buckets,
+std::tuple<Tensor, Tensor> distance_bias_backward(const OptTensor& lengths_, const OptTensor& buckets,
                                                   const Tensor& grad_, int64_t B, double cutoff,
                                                   bool need_table, bool need_lengths) {
     TORCH_CHECK(grad_.is_cuda(), "grad must be a CUDA tensor");
     check_f32(grad_, grad_, "grad");
     TORCH_CHECK(grad_.dim() == 2 && B >= 1, "grad must be [E, H]");
-    check_f32(lengths_, grad_, "lengths");
     const int64_t E = grad_.size(0), H = grad_.size(1);
-    TORCH_CHECK(lengths_.dim() == 1 && lengths_.size(0) == E, "lengths must be [E]");
     if (need_table)
-        TORCH_CHECK(buckets.defined() && buckets.device() == grad_.device() &&
-                        buckets.scalar_type() == torch::kInt16 && buckets.is_contiguous() &&
-                        buckets.numel() == E,
+        TORCH_CHECK(buckets && buckets->device() == grad_.device() &&
+                        buckets->scalar_type() == torch::kInt16 && buckets->is_contiguous() &&
+                        buckets->numel() == E,
                     "buckets must be int16 [E]");
     const c10::DeviceGuard guard(grad_.device());
-    const Tensor grad = rows4(grad_), lengths = lengths_.contiguous();
-    Tensor gt, gl, ws;
+    const Tensor grad = rows4(grad_);
+    Tensor lengths, gt, gl, ws;
+    if (need_lengths) {
+        TORCH_CHECK(lengths_ && lengths_->dim() == 1 && lengths_->size(0) == E, "lengths must be [E]");
+        check_f32(*lengths_, grad_, "lengths");
+        lengths = lengths_->contiguous();
+    }
     size_t wsb = 0;
     if (need_table) {
         gt = torch::empty({B, H}, grad.options());
@@ -87,7 +90,7 @@ std::tuple<Tensor, Tensor> distance_bias_backward(const Tensor& lengths_, const 
     }
     if (need_lengths) gl = torch::empty({E}, grad.options());
     check_status(batteries_distance_bias_backward(
-                     opt_f32(lengths), need_table ? (const uint16_t*)opt_ptr(buckets) : nullptr,
+                     opt_f32(lengths), need_table ? (const uint16_t*)buckets->data_ptr() : nullptr,
                      opt_f32(grad), opt_f32(gt), opt_f32(gl), E, (int)H, (int)B, (float)cutoff,
                      opt_ptr(ws), wsb, stream_of(grad)),
                  "distance_bias_backward");
@@ -99,7 +102,8 @@ struct BiasNode : torch::autograd::Function<BiasNode> {
                           const Tensor& table, c10::optional<double> cutoff) {
         const bool need_table = table.requires_grad(), need_lengths = lengths.requires_grad();
         auto [bias, buckets] = distance_bias(lengths, boundaries, table, cutoff, need_table);
-        ctx->save_for_backward({lengths, buckets});
+        const bool by_cutoff = need_lengths && cutoff.has_value();
+        ctx->save_for_backward({by_cutoff ? lengths : Tensor(), buckets});
         ctx->saved_data["cutoff"] = cutoff.value_or(0.0);
         ctx->saved_data["sizes"] = std::vector<int64_t>{table.size(0), need_table, need_lengths};
         return bias;
@@ -111,9 +115,9 @@ struct BiasNode : torch::autograd::Function<BiasNode> {
         const variable_list s = ctx->get_saved_variables();
         const std::vector<int64_t> n = ctx->saved_data["sizes"].toIntVector();
         const double cutoff = ctx->saved_data["cutoff"].toDouble();
-        auto [gt, gl] = distance_bias_backward(s[0], s[1], grads[0], n[0], cutoff, n[1] != 0,
-                                               n[2] != 0 && cutoff > 0.0);
-        if (n[2] && !gl.defined()) gl = torch::zeros_like(s[0]);
+        auto [gt, gl] = distance_bias_backward(opt_of(s[0]), opt_of(s[1]), grads[0], n[0], cutoff,
+                                               n[1] != 0, n[2] != 0 && cutoff > 0.0);
+        if (n[2] && !gl.defined()) gl = torch::zeros({grads[0].size(0)}, grads[0].options());
         variable_list g = first_order({gl, Tensor(), gt}, create_graph, "distance_bias");
         g.resize(4);
         return g;

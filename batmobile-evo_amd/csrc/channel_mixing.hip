@@ -42,9 +42,7 @@ template <>
 struct Mix8<float> {
     static constexpr int kParts = 3, kBytes = 4;
     float4 r[8];
-    __device__ __forceinline__ void load(int j, __amdgpu_buffer_rsrc_t b, int off) {
-        r[j] = buffer_ld4(b, off, 0);
-    }
+    __device__ __forceinline__ void load(int j, const char* p) { r[j] = *reinterpret_cast<const float4*>(p); }
     __device__ __forceinline__ void zero(int j) { r[j] = make_float4(0, 0, 0, 0); }
     template <int I>
     __device__ __forceinline__ void operand(v4u* f) const {
@@ -52,17 +50,29 @@ struct Mix8<float> {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             v[j] = I == 0 ? r[j].x : I == 1 ? r[j].y : I == 2 ? r[j].z : r[j].w;
-        const Bf3 s = bf16_split8(v);
-        f[0] = s.h, f[1] = s.m, f[2] = s.l;
+        // the leading bits, of the rest the leading ones to nearest, and what is left, at most 8 bits.  Of a
+        // product second part times third is dropped twice, 2^-22 of it at most and of either sign.  An
+        // infinity ends as NaN: mix_again.
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned a = __float_as_uint(v[2 * j]), b = __float_as_uint(v[2 * j + 1]);
+            const float ra = v[2 * j] - __uint_as_float(a & 0xffff0000u);
+            const float rb = v[2 * j + 1] - __uint_as_float(b & 0xffff0000u);
+            const unsigned m = bf16_pack(ra, rb);
+            f[0][j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            f[1][j] = m;
+            f[2][j] = __builtin_amdgcn_perm(__float_as_uint(rb - bf16_hi(m)),
+                                            __float_as_uint(ra - bf16_lo(m)), 0x07060302u);
+        }
     }
 };
 template <>
 struct Mix8<uint16_t> {
     static constexpr int kParts = 1, kBytes = 2;
     unsigned r[8][2];
-    __device__ __forceinline__ void load(int j, __amdgpu_buffer_rsrc_t b, int off) {
-        const auto v = __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, 0);
-        r[j][0] = v[0], r[j][1] = v[1];
+    __device__ __forceinline__ void load(int j, const char* p) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        r[j][0] = v.x, r[j][1] = v.y;
     }
     __device__ __forceinline__ void zero(int j) { r[j][0] = r[j][1] = 0; }
     template <int I>
@@ -73,19 +83,6 @@ struct Mix8<uint16_t> {
             f[0][j] = __builtin_amdgcn_perm(r[2 * j + 1][I / 2], r[2 * j][I / 2], kSel);
     }
 };
-
-// acc += A B in the products that PA and PB parts need, the small ones first
-template <int PA, int PB>
-__device__ __forceinline__ v4f mix_mfma(const v4u* a, const v4u* b, v4f acc) {
-#pragma unroll
-    for (int s = 2; s >= 0; --s)
-#pragma unroll
-        for (int i = PA - 1; i >= 0; --i) {
-            const int j = s - i;
-            if (j >= 0 && j < PB) acc = mfma_bf16(a[i], b[j], acc);
-        }
-    return acc;
-}
 
 // v in two parts of one sign, the leading bits (upper half of the result) and the rest (lower half, to
 // nearest).  A feature's infinity then ends as one of the same sign in both products; so that it does where
@@ -164,26 +161,57 @@ __device__ __forceinline__ bool mix_place(int64_t units, int per, int64_t& unit,
 }
 static unsigned mix_grid(int64_t units, int per) { return (unsigned)(ceil_div(units, 8) * 8 * per); }
 
-// y of 16 NT NG atoms and OT tiles of outputs: NG groups of four waves take 16 NT atoms each.
+// Four components, from `comp` on, of one fp32 result: those that are not finite again in plain fp32
+__device__ __forceinline__ float4 mix_again(const MixArgs& a, int64_t n, int m, int comp, float4 u) {
+    const float* x = (const float*)a.x + n * a.K * 16 + comp;
+    const float* w0 = a.weight + (int64_t)mix_degree0(comp / 4) * a.K * a.M + (int64_t)m * a.sm;
+    const float* w1 = a.weight + (int64_t)mix_degree1(comp / 4) * a.K * a.M + (int64_t)m * a.sm;
+    float4 s = make_float4(0, 0, 0, 0);
+#pragma unroll 1
+    for (int k = 0; k < a.K; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(x + k * 16);
+        const float f = w0[(int64_t)k * a.sk], g = w1[(int64_t)k * a.sk];
+        s.x = fmaf(v.x, f, s.x);
+        s.y = fmaf(v.y, g, s.y);
+        s.z = fmaf(v.z, g, s.z);
+        s.w = fmaf(v.w, g, s.w);
+    }
+    const float inf = __builtin_inff();
+    return make_float4(fabsf(u.x) < inf ? u.x : s.x, fabsf(u.y) < inf ? u.y : s.y,
+                       fabsf(u.z) < inf ? u.z : s.z, fabsf(u.w) < inf ? u.w : s.w);
+}
+
+// y of 16 NG atoms and OT tiles of outputs: NG groups of four waves take 16 atoms each, a wave four
+// components.
 //
-// A step is 32 channels.  Its weights (4 degrees x OT tiles x PW parts, 1 KB each) go to LDS by direct
-// loads a step ahead, in two buffers, and its features to registers a step ahead: what a wave waits
-// for at the end of a step are the weights alone, which were asked for first.
-template <typename T, int PW, int NT, int OT, int NG>
-__global__ __launch_bounds__(256 * NG) void mix_kernel(MixArgs a) {
-    constexpr int PX = Mix8<T>::kParts, kB = Mix8<T>::kBytes;
-    constexpr int kPitch = 16 * 16 + 4;    // floats of an atom in LDS
-    constexpr int kW = 4 * OT * PW * 64;   // 16-byte pieces of a step's weights
-    constexpr int kOut = NG * 16 * kPitch * 4;
-    __shared__ __attribute__((aligned(16))) char sh[2 * kW * 16 > kOut ? 2 * kW * 16 : kOut];
+// A step is 32 channels.  Its weights (4 degrees x OT tiles x PW parts, 1 KB each) and its features come to LDS
+// by direct loads while the step before is worked on, the weights into two buffers, the features into one: a
+// wave takes its share to registers first.  Loaded to registers from memory, 16 bytes of every 64 a lane, each
+// wave had its lines to itself: 64 KB of a step do not stay in L1 until the other three waves ask for them
+// (20,011 x 100 to 200 in f32 207 us, so 196).
+template <typename T>
+struct MixTile {
+    static constexpr int kB = sizeof(T), kPW = kB == 4 ? 3 : 2, kOT = 4, kNG = 2;
+    static constexpr int kAtom = 512 * kB;                         // bytes of an atom's 32 channels
+    static constexpr int kW = 4 * kOT * kPW * 1024, kX = 16 * kNG * kAtom;
+    static constexpr int kBytes = 2 * kW + kX;
+    static constexpr int kPitch = 16 * 16 + 4;                     // floats of an atom on the way out
+    static_assert(kNG * 16 * kPitch * 4 <= kBytes, "the results take the buffers' place");
+};
+
+template <typename T>
+__device__ __forceinline__ void mix_general(const MixArgs& a, char* sh) {      // sh: weights, weights, features
+    using S = MixTile<T>;
+    constexpr int PW = S::kPW, PX = Mix8<T>::kParts, OT = S::kOT, kB = S::kB, kWaves = 4 * S::kNG;
+    constexpr int kPitch = S::kPitch, kPieces = S::kAtom / 16;
     int64_t unit;
     int chunk;
     if (!mix_place(a.units, a.chunks, unit, chunk)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int quarter = wave & 3, group = wave >> 2, q = lane >> 4, at = lane & 15;
-    const int64_t n0 = (unit * NG + group) * 16 * NT;
+    const int64_t n0 = unit * S::kNG * 16;
     const int tile0 = chunk * OT;
-    const int rows = (int)max((int64_t)0, min((int64_t)16 * NT, a.n - n0));
+    const int rows = (int)min((int64_t)16 * S::kNG, a.n - n0);
     const __amdgpu_buffer_rsrc_t xb =
         buffer_rsrc((const float*)((const char*)a.x + n0 * a.K * 16 * kB), rows * a.K * 16 * kB);
     const int d0 = mix_degree0(quarter), d1 = mix_degree1(quarter);
@@ -191,111 +219,116 @@ __global__ __launch_bounds__(256 * NG) void mix_kernel(MixArgs a) {
     // weights of a step: [l][tile][part][lane], OT tiles of a.tiles
     const __amdgpu_buffer_rsrc_t wb = buffer_rsrc(
         (const float*)(a.w + (int64_t)tile0 * PW * 64), (uint32_t)((steps * 4 * a.tiles - tile0) * PW * 1024));
-    auto weights = [&](int s, char* to) {
+    // lanes past the last atom or, after the last step of K, past the last channel bring what lies there
+    // (past the buffer nothing): no result that is stored takes them
+    auto ask = [&](int s, char* lds) {
+        char* to = lds + (s & 1) * S::kW;
 #pragma unroll
-        for (int i = 0; i < kW / 64 / (4 * NG); ++i) {
-            const int f = i * 4 * NG + wave;               // 1 KB: degree f / (OT PW)
+        for (int i = 0; i < S::kW / 1024 / kWaves; ++i) {
+            const int f = i * kWaves + wave;               // 1 KB: degree f / (OT PW)
             const int from = ((s * 4 + f / (OT * PW)) * a.tiles * PW + f % (OT * PW)) * 1024;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                wb, (__attribute__((address_space(3))) void*)(to + f * 1024), 16, lane * 16, from, 0, 0);
+                wb, (__attribute__((address_space(3))) void*)(to + f * 1024), 16, lane * 16 + from, 0, 0, 0);
         }
-        asm volatile("" ::: "memory");                     // what follows is asked for later
-    };
-    Mix8<T> x[NT];
-    const int off = ((at * a.K + q) * 16 + quarter * 4) * kB;
-    auto features = [&](int s) {
 #pragma unroll
-        for (int k = 0; k < NT; ++k) {
-            // (all in the lane's offset, which the buffer's bounds are checked against)
-            const int at0 = off + (k * 16 * a.K + s * 32) * 16 * kB;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[k].load(j, xb, at0 + j * 64 * kB);
+        for (int i = 0; i < S::kX / 1024 / kWaves; ++i) {
+            const int load = i * kWaves + wave, node = load * 64 / kPieces;
+            const int p = (load * 64 % kPieces + lane) ^ (node & 15);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                xb, (__attribute__((address_space(3))) void*)(lds + 2 * S::kW + load * 1024), 16,
+                node * a.K * 16 * kB + s * S::kAtom + p * 16, 0, 0, 0);
         }
+        asm volatile("" ::: "memory");
     };
-    v4f acc[4][NT][OT];
+    // this lane's pieces: (4 j + q) kB + quarter kB / 4, permuted by the atom's number
+    const char* mine = sh + 2 * S::kW + (group * 16 + at) * S::kAtom;
+    const int piece = q * kB + quarter * kB / 4;
+    v4f acc[4][OT];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int k = 0; k < NT; ++k)
-#pragma unroll
-            for (int o = 0; o < OT; ++o) acc[i][k][o] = v4f{0, 0, 0, 0};
-    weights(0, sh);
-    features(0);
+        for (int o = 0; o < OT; ++o) acc[i][o] = v4f{0, 0, 0, 0};
+    ask(0, sh);
     for (int s = 0; s < steps; ++s) {
-        // this step's weights have arrived, in every wave's part
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NT * 8) : "memory");
+        // this step's loads are in, those of every wave; the step before is worked off
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __syncthreads();
-        if ((a.K & 31) && s == steps - 1) {                // past K the loads gave the next atom's
+        Mix8<T> x;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            x.load(j, mine + ((piece + 4 * j * kB) ^ at) * 16 + (kB == 2 ? quarter % 2 * 8 : 0));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __syncthreads();                                   // the features' buffer is free
+        if (s + 1 < steps) ask(s + 1, sh);
+        if ((a.K & 31) && s == steps - 1) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (s * 32 + 4 * j + q >= a.K) {
-#pragma unroll
-                    for (int k = 0; k < NT; ++k) x[k].zero(j);
-                }
+                if (s * 32 + 4 * j + q >= a.K) x.zero(j);
         }
-        v4u f[4][NT][PX];
-#pragma unroll
-        for (int k = 0; k < NT; ++k) {
-            x[k].template operand<0>(f[0][k]);
-            x[k].template operand<1>(f[1][k]);
-            x[k].template operand<2>(f[2][k]);
-            x[k].template operand<3>(f[3][k]);
-        }
-        const v4u* w = reinterpret_cast<const v4u*>(sh) + (s & 1) * kW + lane;
-        if (s + 1 < steps) {
-            weights(s + 1, sh + ((s + 1) & 1) * kW * 16);
-            features(s + 1);
-            asm volatile("" ::: "memory");
-        }
+        v4u f[4][PX];
+        x.template operand<0>(f[0]);
+        x.template operand<1>(f[1]);
+        x.template operand<2>(f[2]);
+        x.template operand<3>(f[3]);
+        const v4u* w = reinterpret_cast<const v4u*>(sh + (s & 1) * S::kW) + lane;
 #pragma unroll
         for (int o = 0; o < OT; ++o) {
             v4u w0[PW], w1[PW];
 #pragma unroll
             for (int p = 0; p < PW; ++p) w0[p] = w[((d0 * OT + o) * PW + p) * 64];
 #pragma unroll
-            for (int k = 0; k < NT; ++k) acc[0][k][o] = mix_mfma<PW, PX>(w0, f[0][k], acc[0][k][o]);
-#pragma unroll
             for (int p = 0; p < PW; ++p) w1[p] = w[((d1 * OT + o) * PW + p) * 64];
+            // the small products first, successive ones to different sums
 #pragma unroll
-            for (int i = 1; i < 4; ++i)
+            for (int sum = 2; sum >= 0; --sum)
 #pragma unroll
-                for (int k = 0; k < NT; ++k)
-                    acc[i][k][o] = mix_mfma<PW, PX>(w1, f[i][k], acc[i][k][o]);
+                for (int p = PW - 1; p >= 0; --p) {
+                    const int r = sum - p;
+                    if (r < 0 || r >= PX) continue;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        acc[i][o] = mfma_bf16(i ? w1[p] : w0[p], f[i][r], acc[i][o]);
+                }
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __syncthreads();                                   // the buffer is free
     }
     // the four waves' components of 16 atoms x 16 outputs together, and out as whole lines
     const int t = threadIdx.x & 255;
     float* out = reinterpret_cast<float*>(sh) + group * 16 * kPitch;
 #pragma unroll
-    for (int k = 0; k < NT; ++k)
+    for (int o = 0; o < OT; ++o) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __syncthreads();
 #pragma unroll
-        for (int o = 0; o < OT; ++o) {
-            if (k + o) __syncthreads();
+        for (int r = 0; r < 4; ++r)
+            *reinterpret_cast<float4*>(&out[at * kPitch + (4 * q + r) * 16 + quarter * 4]) =
+                make_float4(acc[0][o][r], acc[1][o][r], acc[2][o][r], acc[3][o][r]);
+        __syncthreads();
+        const int m0 = (tile0 + o) * 16;
+        constexpr int kUnit = 16 / kB, kPer = 256 / kUnit;     // 16-byte pieces of an atom
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                *reinterpret_cast<float4*>(&out[at * kPitch + (4 * q + r) * 16 + quarter * 4]) =
-                    make_float4(acc[0][k][o][r], acc[1][k][o][r], acc[2][k][o][r], acc[3][k][o][r]);
-            __syncthreads();
-            const int m0 = (tile0 + o) * 16;
-            constexpr int kUnit = 16 / kB, kPer = 256 / kUnit;     // 16-byte pieces of an atom
-#pragma unroll
-            for (int i = 0; i < 16 * kPer / 256; ++i) {
-                const int p = i * 256 + t, node = p / kPer, e = p % kPer * kUnit;
-                if (k * 16 + node >= rows || m0 + e / 16 >= a.M) continue;
-                const float4 u = *reinterpret_cast<const float4*>(&out[node * kPitch + e]);
-                const int64_t to = ((n0 + k * 16 + node) * a.M + m0) * 16 + e;
-                if constexpr (kB == 4) {
-                    *reinterpret_cast<float4*>((float*)a.y + to) = u;
-                } else {
-                    const float4 v = *reinterpret_cast<const float4*>(&out[node * kPitch + e + 4]);
-                    *reinterpret_cast<uint4*>((uint16_t*)a.y + to) =
-                        make_uint4(bf16_pack(u.x, u.y), bf16_pack(u.z, u.w), bf16_pack(v.x, v.y),
-                                   bf16_pack(v.z, v.w));
-                }
+        for (int i = 0; i < 16 * kPer / 256; ++i) {
+            const int p = i * 256 + t, node = p / kPer, e = p % kPer * kUnit;
+            if (group * 16 + node >= rows || m0 + e / 16 >= a.M) continue;
+            float4 u = *reinterpret_cast<const float4*>(&out[node * kPitch + e]);
+            const int64_t n = n0 + group * 16 + node, to = (n * a.M + m0) * 16 + e;
+            if constexpr (kB == 4) {
+                if (!(fabsf((u.x + u.y) + (u.z + u.w)) < __builtin_inff()))
+                    u = mix_again(a, n, m0 + e / 16, e % 16, u);
+                *reinterpret_cast<float4*>((float*)a.y + to) = u;
+            } else {
+                const float4 v = *reinterpret_cast<const float4*>(&out[node * kPitch + e + 4]);
+                *reinterpret_cast<uint4*>((uint16_t*)a.y + to) =
+                    make_uint4(bf16_pack(u.x, u.y), bf16_pack(u.z, u.w), bf16_pack(v.x, v.y),
+                               bf16_pack(v.z, v.w));
             }
         }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256 * MixTile<T>::kNG) void mix_kernel(MixArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char sh[];
+    mix_general<T>(a, sh);
 }
 
 // ---------------------------------------------------------------------------
@@ -895,14 +928,9 @@ static bool mix_shape_ok(int64_t N, int C, int O, int dtype) {
            (dtype == 0 || dtype == 1);
 }
 
-// Atoms and outputs of a workgroup, parts of the weight
-template <typename T>
-struct MixShape {
-    static constexpr int kNT = 1, kOT = 4, kNG = 2, kPW = sizeof(T) == 4 ? 3 : 2;
-};
 template <typename T>
 static void mix_tiles(int M, MixArgs& a) {
-    constexpr int kOT = MixShape<T>::kOT;
+    constexpr int kOT = MixTile<T>::kOT;
     a.chunks = (M + kOT * 16 - 1) / (kOT * 16);
     a.tiles = a.chunks * kOT;
 }
@@ -911,7 +939,7 @@ static size_t mix_bytes(int K, int M) {
     if (K <= kStayMost<T>) return 16;
     MixArgs a{};
     mix_tiles<T>(M, a);
-    return (size_t)((K + 31) / 32) * 4 * a.tiles * MixShape<T>::kPW * 64 * 16;
+    return (size_t)((K + 31) / 32) * 4 * a.tiles * MixTile<T>::kPW * 64 * 16;
 }
 
 // More than 64 KB of LDS for a kernel, allowed once on each device
@@ -956,23 +984,25 @@ static int stay_run(const MixArgs& a, hipStream_t s) {
 template <typename T>
 static int mix_run(MixArgs a, void* ws, hipStream_t s) {
     if (a.K <= kStayMost<T>) return stay_run<T>(a, s);
-    using S = MixShape<T>;
+    using S = MixTile<T>;
+    static std::atomic<uint64_t> allowed{0};
+    if (const int rc = mix_allow_lds((const void*)&mix_kernel<T>, S::kBytes, allowed)) return rc;
     mix_tiles<T>(a.M, a);
     const int total = (a.K + 31) / 32 * 4 * a.tiles * 64;
     mix_pack_kernel<S::kPW><<<(total + 255) / 256, 256, 0, s>>>(a.weight, (v4u*)ws, a.K, a.M, a.sk,
                                                                a.sm, a.tiles, total);
     a.w = (const v4u*)ws;
-    constexpr int64_t kAtoms = (int64_t)1 << 24;     // of a launch
+    // atoms of a launch: 2^22 workgroups (threads < 2^32)
+    const int64_t most = ((int64_t)1 << 22) / a.chunks * 16 * S::kNG;
     const int64_t n = a.n;
     const char *x = (const char*)a.x;
     char* y = (char*)a.y;
-    for (int64_t n0 = 0; n0 < n; n0 += kAtoms) {
+    for (int64_t n0 = 0; n0 < n; n0 += most) {
         a.x = x + n0 * a.K * 16 * (int64_t)sizeof(T);
         a.y = y + n0 * a.M * 16 * (int64_t)sizeof(T);
-        a.n = std::min(n - n0, kAtoms);
-        a.units = ceil_div(a.n, 16 * S::kNT * S::kNG);
-        mix_kernel<T, S::kPW, S::kNT, S::kOT, S::kNG>
-            <<<mix_grid(a.units, a.chunks), 256 * S::kNG, 0, s>>>(a);
+        a.n = std::min(n - n0, most);
+        a.units = ceil_div(a.n, 16 * S::kNG);
+        mix_kernel<T><<<mix_grid(a.units, a.chunks), 256 * S::kNG, S::kBytes, s>>>(a);
     }
     return (int)hipGetLastError();
 }

@@ -129,6 +129,7 @@ __global__ __launch_bounds__(256) void bias_bwd_kernel(BiasArgs a, int range_wav
             // an edge of another range, or past the last, adds 0 to some bucket
             bool there = true;
             if (RANGES) k[i] -= b0, there = (unsigned)k[i] < (unsigned)per;
+            else k[i] = min(k[i], per - 1);                // (no array of buckets leads out of the LDS)
             if (!decltype(whole)::value) there = there && from + i * step < left;
             if (RANGES || !decltype(whole)::value) {
                 k[i] = there ? k[i] : 0;

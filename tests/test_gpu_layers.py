@@ -289,7 +289,8 @@ def _check_mixing(dev, n, c, o, dtype, kept, seed):
 @pytest.mark.parametrize("kept", [None, "e4m3"])
 @pytest.mark.parametrize("n,c,o", [(1, 1, 1), (2, 3, 5), (15, 16, 16), (16, 31, 33), (17, 32, 32),
                                    (33, 64, 64), (100, 40, 100), (31, 100, 200), (65, 128, 64),
-                                   (32, 130, 129), (40, 256, 8), (200, 8, 256), (129, 33, 65)])
+                                   (32, 130, 129), (40, 256, 8), (200, 8, 256), (129, 33, 65),
+                                   (21, 300, 70), (50, 70, 300)])
 def test_channel_mixing(dev, dtype, kept, n, c, o):
     _check_mixing(dev, n, c, o, dtype, kept, n + c + o)
 
@@ -342,25 +343,74 @@ def test_channel_mixing_strides(dev, dtype):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
-def test_channel_mixing_infinities(dev):
+@pytest.mark.parametrize("c", [33, 70, 300])
+def test_channel_mixing_infinities(dev, c):
     """An infinity or NaN reaches what it is a term of, and nothing else."""
     import batmobile
     for dtype in (torch.float32, torch.bfloat16):
-        x = torch.randn(40, 33, 16, generator=gen(8)).to(dev, dtype)
-        w = (torch.rand(4, 33, 20, generator=gen(9)) + 0.5).to(dev)
+        x = torch.randn(40, c, 16, generator=gen(8)).to(dev, dtype)
+        w = (torch.rand(4, c, 20, generator=gen(9)) + 0.5).to(dev)
         want = batmobile.channel_mixing(x, w)
-        x[5, 7, 3], x[33, 32, 9] = float("inf"), float("nan")
+        x[5, 7, 3], x[33, c - 1, 9] = float("inf"), float("nan")
         y = batmobile.channel_mixing(x, w)
         assert torch.isinf(y[5, :, 3]).all() and torch.isnan(y[33, :, 9]).all()
         y[5, :, 3], y[33, :, 9] = want[5, :, 3], want[33, :, 9]
         assert torch.equal(y, want)
-        x = torch.rand(40, 33, 16, generator=gen(8)).to(dev, dtype) + 0.5
+        x = torch.rand(40, c, 16, generator=gen(8)).to(dev, dtype) + 0.5
         want = batmobile.channel_mixing(x, w)
         w[1, 6, 4] = -float("inf")
         y = batmobile.channel_mixing(x, w)
         assert torch.isneginf(y[:, 4, 1:4]).all()
         y[:, 4, 1:4] = want[:, 4, 1:4]
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("kept", [None, "e4m3"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_weight_gradient_with_nan(dev, dtype, kept):
+    """A NaN in x or in the gradient reaches its channel's row or column of its degree alone."""
+    import batmobile
+    x, g = _features(37, 20, dtype, 12).to(dev), _features(37, 70, dtype, 13).to(dev)
+    w = torch.randn(4, 20, 70, generator=gen(14)).to(dev).requires_grad_(True)
+    want, = torch.autograd.grad(batmobile.channel_mixing(x, w, kept), w, g)
+    x[36, 19, 5], g[20, 69, 12] = float("nan"), float("nan")
+    got, = torch.autograd.grad(batmobile.channel_mixing(x, w, kept), w, g)
+    bad = torch.isnan(got)
+    hit = torch.zeros_like(bad)
+    hit[2, 19], hit[3, :, 69] = True, True
+    assert torch.equal(bad, hit)
+    # the 8-bit block that holds the NaN is another one: its largest value may have gone
+    hit[:, 16:] = hit[:, 16:] | (kept is not None)
+    assert torch.equal(got[~hit], want[~hit])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_channel_mixing_single_gradients(dev, dtype):
+    """Only the gradient that is wanted, the same as with both; nothing is kept for the other."""
+    import batmobile
+    x, g = _features(33, 24, dtype, 15).to(dev), _features(33, 10, dtype, 16).to(dev)
+    w = torch.randn(4, 24, 10, generator=gen(17)).to(dev)
+    both = [x.clone().requires_grad_(True), w.clone().requires_grad_(True)]
+    want = torch.autograd.grad(batmobile.channel_mixing(*both), both, g)
+    y = batmobile.channel_mixing(both[0], w)
+    z = batmobile.channel_mixing(x, both[1])
+    w.mul_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(y, both[0], g)
+    assert torch.equal(torch.autograd.grad(z, both[1], g)[0], want[1])
+    y = batmobile.channel_mixing(both[0], w)
+    both[0].detach().zero_()                           # its values are not needed
+    assert torch.equal(torch.autograd.grad(y, both[0], g)[0], want[0])
+
+
+def test_buckets_of_the_backward_stay_in_bounds(dev):
+    """Buckets that no forward gave are taken to the last one, or left out; nothing is written past."""
+    k = torch.tensor([0, 1, 5, 300, -1], dtype=torch.int16, device=dev)
+    g = torch.ones(5, 2, device=dev)
+    for buckets in (2, 200):
+        gt, gl = _batmobile.distance_bias_backward(None, k, g, buckets, 0.0, True, False)
+        assert gl is None and gt.shape == (buckets, 2) and torch.isfinite(gt).all()
+        assert gt[0, 0] >= 1 and gt.sum() <= 10
 
 
 def test_channel_mixing_past_32_bits(dev):
