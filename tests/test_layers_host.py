@@ -92,9 +92,16 @@ def _mix(lib, n=3, c=8, o=8, dtype=0, x=ADDR, w=ADDR, y=ADDR, ws=ADDR, b=1 << 30
     (dict(n=-1), ERR_ARG), (dict(n=1 << 31), ERR_ARG), (dict(c=0), ERR_ARG), (dict(o=2049), ERR_ARG),
     (dict(dtype=2), ERR_ARG), (dict(x=NONE), ERR_ARG), (dict(w=NONE), ERR_ARG), (dict(y=NONE), ERR_ARG),
     (dict(x=ODD), ERR_ARG), (dict(y=ODD), ERR_ARG), (dict(ws=NONE), ERR_WORKSPACE),
-    (dict(b=64), ERR_WORKSPACE)])
+    (dict(b=8), ERR_WORKSPACE)])
 def test_channel_mixing_refuses(lib, given, want):
     assert _mix(lib, **given) == want
+
+
+@pytest.mark.parametrize("c", [8, 64, 65, 128, 256, 257, 2048])
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_channel_mixing_refuses_a_byte_too_few(lib, c, dtype):
+    need = lib.batteries_channel_mixing_workspace_bytes(c, 8, 0, dtype)
+    assert need >= 16 and _mix(lib, c=c, dtype=dtype, b=need - 1) == ERR_WORKSPACE
 
 
 def _mix_weight(lib, n=3, x=ADDR, codes=NONE, exps=NONE, g=ADDR, gw=ADDR, ws=ADDR, b=1 << 30):
@@ -152,7 +159,8 @@ def test_workspaces_stay_small(lib):
             assert 4 * h * b <= n <= max(17 << 20, 4 * h * b)
         for c, o in ((1, 1), (64, 64), (128, 256), (2048, 2048)):
             n = lib.batteries_channel_mixing_weight_grad_workspace_bytes(i64(e), c, o)
-            assert 24 * c * o <= n <= max(64 << 20, 24 * c * o)
+            # a partial sum: 4 degrees of c x o in 4 bytes
+            assert 16 * c * o <= n <= max(64 << 20, 16 * c * o)
     assert lib.batteries_layer_norm_backward_workspace_bytes(i64(10), 9000) == 0
     assert lib.batteries_channel_mixing_workspace_bytes(4000, 8, 0, 0) == 0
 
