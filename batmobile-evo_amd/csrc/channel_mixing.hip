@@ -5,18 +5,22 @@
 //   gx[n, c, m] = sum_o g[n, o, m] W[l(m), c, o]                   (the same kernel, W transposed)
 //   gW[l, c, o] = sum_n sum_{m of degree l} x[n, c, m] g[n, o, m]  (x as it was, or from its 8-bit form)
 //
-// All on the bf16 matrix cores with fp32 sums.  fp32 features and weights go in three parts and six
-// products, as exact as fp32 products; the fp32 weight of bf16 features goes in two (off by 2^-15 of it
-// at most), bf16 features in one, which is exact; an 8-bit form is exact in bf16, so against it only g is
-// split.
+// Sums are fp32.  bf16 features go to the bf16 matrix cores as they are; their weight, which is fp32, goes in
+// two parts (off by 2^-15 of it at most).  fp32 features run on the fp32 matrix cores (up to 64 channels in,
+// and for gW) or, three parts each, in six products on the bf16 ones, as exact as fp32 products.  An 8-bit
+// form is exact in bf16, so against it only g is split.
 //
 // The features lie [N, C, 16], 16 components together, and a matrix operand wants 8 values along the sum
-// for one component.  A lane therefore loads the same four components of 8 channels (or of 8 atoms,
-// for gW), and the operand of each component is its values of the eight: in bf16 one v_perm for two of
-// them.  The four waves of a workgroup take four components each of the same atoms and
-// channels, so a cache line is read by all of them at about the same time, and a wave meets two
-// degrees at most.  The order of the sum is free as long as both operands have the same one: value j of lane
-// group q is channel (atom) 4 j + q, so that a load covers neighbours.
+// for one component.  Whole lines come to LDS by direct loads; from there a lane takes the same components
+// of 8 channels (for gW of 4 atoms), and the operand of each component is its values of the eight: in bf16
+// one v_perm for two of them.  A wave takes 4 or 8 of the components, which have two degrees at most.  The
+// order of the sum is free as long as both operands have the same one: value j of lane group q is channel
+// (atom) 4 j + q.
+//
+// Measured, us (what the bytes take at a copy's 5 TB/s): 50,000 atoms 128 to 128 in bf16 104 (82), its gW 122 to 136,
+// from the 8-bit form 94 (62); 64 to 64 in bf16 43 (41), in fp32 104 (82); 20,011 atoms 100 to 200 in fp32
+// 196 (77), 200 to 100 148, gW 234, from the 8-bit form 146.  bf16 is bound by memory and by reads and
+// writes that take turns; fp32 by the matrix cores and the splitting.
 #include <atomic>
 #include <type_traits>
 
@@ -26,7 +30,9 @@
 namespace bmhip {
 
 constexpr int kMixMaxC = 2048;
-// channels up to which the weight stays in registers
+// Channels up to which the weight stays in registers.  Against the general kernel, us: fp32 50,000 atoms 64
+// to 64 104 and 114, but 20,011 100 to 200 250 and 196; bf16 50,000 128 to 128 104 and 162, 20,011 200 to
+// 256 174 and 178.  Above 256 in bf16 a degree's weight no longer fits.
 template <typename T>
 constexpr int kStayMost = sizeof(T) == 4 ? 64 : 256;
 constexpr int kMixFar = 0x7fffff00;        // a buffer offset past every buffer here: reads 0
@@ -51,7 +57,7 @@ struct Mix8<float> {
         for (int j = 0; j < 8; ++j)
             v[j] = I == 0 ? r[j].x : I == 1 ? r[j].y : I == 2 ? r[j].z : r[j].w;
         // the leading bits, of the rest the leading ones to nearest, and what is left, at most 8 bits.  Of a
-        // product second part times third is dropped twice, 2^-22 of it at most and of either sign.  An
+        // product second part times third is dropped twice, 2^-23 of it at most and of either sign.  An
         // infinity ends as NaN: mix_again.
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -1031,6 +1037,7 @@ static int mix_weight_run(MixArgs& a, hipStream_t s) {
 template <typename T>
 static int mix_weight_pick(MixArgs& a, hipStream_t s) {
     if (a.x) return mix_weight_run<T, false, 2>(a, s);
+    // 128 channels in for 64 out where g would else be read once more (50,000 x 128 x 128: 94 against 106 us)
     if constexpr (sizeof(T) == 2)
         if (a.K > 64) return mix_weight_run<T, true, 4>(a, s);
     return mix_weight_run<T, true, 2>(a, s);

@@ -7,6 +7,10 @@
 // the differences from the mean, and the backward forms m and r again from the row, which costs
 // lane sums but no memory.  Sums are fp32.  A row of few elements takes a part of a wave, a long one up
 // to 16 waves.
+//
+// Measured, us (the bytes at 5 TB/s): 560,308 x 64 in bf16 forward 28 (29), backward 43 (43) and 4 for the
+// weights; 50,000 x 1000 in fp32 78 (80) and 120 (120); 300,000 x 37 in fp32 17 (18) and 36 (27).  Invariants
+// that lie 16 apart cost their lines: 20,011 x 100 in fp32 21 and 24, 6 TB/s of whole lines.
 #include "sums.h"
 #include "batmobile_hip.h"
 
