@@ -465,7 +465,7 @@ struct StayShape {
 };
 
 // Until at most LATER loads and `tiles` tiles' stores are under way: what was asked for before them is
-// there (loads complete in order; a store that completes early only lengthens the wait)
+// there (the counter goes down in the order of issue, loads and stores alike)
 template <int LATER, int STORES, int MOST>
 __device__ __forceinline__ void stay_wait(int tiles) {
     static_for<MOST + 1>([&](auto ii) {
@@ -632,6 +632,8 @@ __device__ __forceinline__ void mix_stay(const MixArgs& a, char* sh) {
                 }
             }
     }
+    // the loads past the last tile, before the LDS that they write goes to another workgroup
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 template <typename T, int KS, int OT, int OG>
