@@ -222,7 +222,7 @@ __global__ __launch_bounds__(ln_threads<W>()) void ln_bwd_kernel(LnArgs a) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const LnAt<VEC, TAIL> at(i * kLanes + t, a.D);
-            if (at.there) {
+            if (at.there && there) {                       // (without eps r of no row is infinite)
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
                     const float xh = x[i].v[j] * r;

@@ -194,6 +194,16 @@ def test_layer_norm(dev, dtype, rows, d):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,d", [(1, 8), (3, 33), (5, 100), (33, 64), (7, 500), (2, 2048)])
+def test_layer_norm_without_eps(dev, dtype, rows, d):
+    """eps = 0: a workgroup's places without a row have no part in the weights' gradient."""
+    g = gen(rows + d)
+    x = (torch.randn(rows, d, generator=g) + 0.5).to(TYPES[dtype]).to(dev)
+    _check_ln(dev, x, torch.randn(d, generator=g), torch.randn(d, generator=g),
+              torch.randn(rows, d, generator=g).to(TYPES[dtype]), dtype, eps=0.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("form", ["scalars", "columns", "rows", "offset", "three", "expanded", "packed"])
 def test_layer_norm_strides(dev, dtype, form):
     g = gen(11)
