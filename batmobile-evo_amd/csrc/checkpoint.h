@@ -6,7 +6,7 @@
 // most 2^-4 of the value down to 2^-15 of the block's largest.  The power is exact in fp32 and bf16, and so is
 // a decoded value, so the factors of the backward's products lose nothing more.  codes [N, C, 16]
 // and exps [N, ceil(C / 8)] are bytes, an exponent kept as E + 127.  A value that is not finite is kept
-// as NaN and has no part in the maximum.  At E = 120 the code 256 would be 2^128: values over 248 take 240,
+// as NaN and has no part in the maximum.  At E = 120 the code 256 would be 2^128: values from 248 on take 240,
 // which is within the same 2^-4.
 #pragma once
 
@@ -29,7 +29,7 @@ __device__ __forceinline__ float ckpt_finite(float v) {
 }
 // A value of a block of E = 120 as it goes to its code
 __device__ __forceinline__ float ckpt_limit(float v) {
-    return fabsf(v) > 0x1.fp127f ? copysignf(0x1.ep127f, v) : v;
+    return fabsf(v) >= 0x1.fp127f ? copysignf(0x1.ep127f, v) : v;
 }
 // Four values divided by 2^E as four codes
 __device__ __forceinline__ unsigned ckpt_encode4(float a, float b, float c, float d, float down) {

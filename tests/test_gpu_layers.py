@@ -476,6 +476,24 @@ def test_checkpoint(dev, dtype, n, c):
         assert np.array_equal(_np(back), want, equal_nan=True)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_checkpoint_largest(dev, dtype):
+    """Where codes end: the halves between 240, 256 and 448 times 2^120, and the largest numbers."""
+    import batmobile
+    big = torch.finfo(TYPES[dtype]).max
+    x = torch.zeros(2, 8, 16)
+    x[0, 0, :6] = torch.tensor([248.0, -248.0, 232.0, 224.0, 249.0, 1.0]) * 2.0 ** 120
+    x[1, 3, :4] = torch.tensor([big, -big, 240 * 2.0 ** 120, 216 * 2.0 ** 120])
+    x = x.to(TYPES[dtype])
+    codes, exps = batmobile.checkpoint_encode(x.to(dev))
+    wc, we = ol.encode(_np(x))
+    assert torch.equal(exps.cpu(), torch.from_numpy(we))
+    assert np.array_equal(codes.view(torch.uint8).cpu().numpy(), wc)
+    back = batmobile.checkpoint_decode(codes, exps)
+    assert torch.isfinite(back).all()
+    assert (np.abs(_np(back) - _np(x)) <= 2.0 ** -4 * np.abs(_np(x))).all()
+
+
 def test_checkpoint_empty(dev):
     import batmobile
     codes, exps = batmobile.checkpoint_encode(torch.zeros(0, 9, 16, device=dev))
