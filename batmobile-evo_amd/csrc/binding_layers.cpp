@@ -3,7 +3,6 @@
 // activations.  No reference counterpart.  Host code only, over include/batmobile_hip.h.
 #include "binding_ops.h"
 
-#include <cmath>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -38,8 +37,8 @@ void check_bias(const Tensor& lengths, const Tensor& boundaries, const Tensor& t
                 "table must be [B, H], up to 4096 buckets and 1024 heads");
     TORCH_CHECK(boundaries.dim() == 1 && boundaries.size(0) == table.size(0) - 1,
                 "boundaries must be [B - 1]");
-    TORCH_CHECK(!cutoff || (*cutoff > 0.0 && (float)*cutoff > 0.0f && std::isfinite((float)*cutoff)),
-                "cutoff must be positive and finite");
+    TORCH_CHECK(!cutoff || ((float)*cutoff >= 1e-30f && (float)*cutoff <= 1e30f),
+                "cutoff must be positive and finite (1e-30 to 1e30)");
 }
 
 // (bias [E, H], buckets [E] int16 or none)

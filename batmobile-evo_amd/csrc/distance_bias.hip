@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void bias_fwd_kernel(BiasArgs a) {
 
 // Table gradient.  A wave holds 64 columns of sums in LDS for each of its (at most 64) buckets; lane
 // (slot s, head h) adds the values of its edges to its own column alone, so no two lanes meet and the order
-// is the edges'.  It reads, adds and writes: the LDS's own addition takes 3 cycles a lane (1.4 M edges x 8
+// is the edges'.  It reads, adds and writes: the LDS's own addition takes longer (1.4 M edges x 8
 // heads in 64 buckets 66 us, so 18).  More than 64 buckets: the waves of a workgroup take ranges of 64 and
 // read the same edges, of which each adds a part (256 buckets 40 us); more than 256: gridDim.y ranges of
 // 256.  The columns' sums go to part [gridDim.x, B, H].  Heads past 64: gridDim.z.
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(256) void bias_lengths_kernel(BiasArgs a) {
     if constexpr (LANES > 1) s = lanes_sum<LANES>(s);
     const bool in = fabsf(r) < a.cutoff;
     if (lane == 0)
-        a.glengths[e] = in ? s * (-2.0f * r / ((a.cutoff - r) * (a.cutoff + r))) : r != r ? r : 0.0f;
+        a.glengths[e] = in ? s * (-2.0f * r / (a.cutoff - r) / (a.cutoff + r)) : r != r ? r : 0.0f;
 }
 
 template <bool VEC, int LANES>
@@ -223,6 +223,8 @@ static void bias_lengths_run(const BiasArgs& a, hipStream_t s) {
     else bias_lengths_launch<VEC, 16>(a, s);
 }
 
+// A cutoff whose inverse, and whose products with a length, stay in fp32's range; 0: none
+static bool bias_cutoff_ok(float c) { return c == 0.0f || (c >= 1e-30f && c <= 1e30f); }
 static bool bias_shape_ok(int64_t E, int H, int B) {
     return E >= 0 && E < ((int64_t)1 << 38) && H >= 1 && H <= kBiasMaxHeads && B >= 1 &&
            B <= kBiasMaxBuckets;
@@ -245,7 +247,7 @@ using namespace bmhip;
 extern "C" int batteries_distance_bias(const float* lengths, const float* boundaries,
                                        const float* table, float* bias, uint16_t* buckets,
                                        int64_t E, int H, int B, float cutoff, hipStream_t stream) {
-    if (!bias_shape_ok(E, H, B) || !(cutoff >= 0.0f) || cutoff == __builtin_inff() ||
+    if (!bias_shape_ok(E, H, B) || !bias_cutoff_ok(cutoff) ||
         (B > 1 && !boundaries) || !table || (E > 0 && (!lengths || !bias)))
         return BM_ERR_ARG;
     if (E == 0) return BM_OK;
@@ -274,7 +276,7 @@ extern "C" int batteries_distance_bias_backward(const float* lengths, const uint
                                                 int64_t E, int H, int B, float cutoff,
                                                 void* workspace, size_t workspace_bytes,
                                                 hipStream_t stream) {
-    if (!bias_shape_ok(E, H, B) || !(cutoff >= 0.0f) || cutoff == __builtin_inff() ||
+    if (!bias_shape_ok(E, H, B) || !bias_cutoff_ok(cutoff) ||
         (E > 0 && (!g || (gtable && !buckets) || (glengths && !lengths))))
         return BM_ERR_ARG;
     BiasArgs a{};

@@ -609,8 +609,8 @@ int batteries_clip_grad_norm(const void* const* in, void* const* out, const int6
  *   bias[e, h] = table[k, h] + log max(0, 1 - (r / cutoff)^2),   r = lengths[e],
  *   k = number of boundaries <= r
  * lengths [E], boundaries [B - 1] ascending (any values give a bucket in [0, B)), table [B, H], bias
- * [E, H], all fp32; cutoff 0: without the second term, which from the cutoff on is -inf.  A length
- * that is NaN gives NaN.  buckets [E] (NULL: not kept) takes k for the backward.  B <= 4096,
+ * [E, H], all fp32; cutoff 1e-30 to 1e30, or 0: without the second term, which from the cutoff on is
+ * -inf.  A length that is NaN gives NaN.  buckets [E] (NULL: not kept) takes k for the backward.  B <= 4096,
  * H <= 1024, E < 2^38.
  * ------------------------------------------------------------------------- */
 int batteries_distance_bias(const float* lengths, const float* boundaries, const float* table,

@@ -120,6 +120,21 @@ def test_distance_bias_strided_inputs(dev):
     assert all(torch.equal(x, y) for x, y in zip(one, full))
 
 
+@pytest.mark.parametrize("k", [-90, 90])
+def test_distance_bias_scaled(dev, k):
+    """All lengths times 2^k: the same bias, and the gradient times 2^-k, bit for bit."""
+    import batmobile
+    r, bound, table, g = [t.to(dev) for t in _bias_inputs(600, 40, 8, 3)]
+
+    def run(scale):
+        a = (r * scale).requires_grad_(True)
+        out = batmobile.distance_bias(a, bound * scale, table, 5.0 * scale)
+        return out, torch.autograd.grad(out, a, g)[0] * scale
+
+    for got, want in zip(run(2.0 ** k), run(1.0)):
+        assert torch.equal(got, want)
+
+
 def test_distance_bias_single_gradients(dev):
     """Only the gradient that is wanted."""
     import batmobile

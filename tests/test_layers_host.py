@@ -41,6 +41,7 @@ def _bias(lib, e=10, h=4, b=8, cutoff=5.0, lengths=ADDR, bounds=ADDR, table=ADDR
 
 @pytest.mark.parametrize("given", [dict(e=-1), dict(e=1 << 38), dict(h=0), dict(h=1025), dict(b=0),
                                    dict(b=4097), dict(cutoff=-1.0), dict(cutoff=float("nan")),
+                                   dict(cutoff=1e-31), dict(cutoff=2e30),
                                    dict(cutoff=float("inf")), dict(lengths=NONE), dict(bounds=NONE),
                                    dict(table=NONE), dict(out=NONE)])
 def test_distance_bias_refuses(lib, given):
