@@ -672,14 +672,15 @@ int batteries_gate_activation_backward(const void* x, const uint8_t* codes, cons
  *   y[n, o, m] = sum_c x[n, c, m] weight[l(m), c, o],  l(m) the degree of component m
  * x [N, C, 16] to y [N, O, 16] in fp32 (dtype 0) or bf16 (dtype 1), 16-byte aligned, weight
  * [4, C, O] fp32; transposed: x [N, O, 16] to y [N, C, 16], the sum over o.  fp32 accuracy of the
- * products in fp32; with bf16 features the weight is rounded to 15 bits.  C, O <= 2048,
- * N < 2^31.
+ * products in fp32 (a feature below 2^-110 counts to 2^-133 only); with bf16 features the weight is
+ * rounded to 15 bits.  C, O <= 2048, N < 2^31.
  * ------------------------------------------------------------------------- */
 size_t batteries_channel_mixing_workspace_bytes(int C, int O, int transposed, int dtype);
 int batteries_channel_mixing(const void* x, const float* weight, void* y, int64_t N, int C, int O,
                              int transposed, int dtype, void* workspace, size_t workspace_bytes,
                              hipStream_t stream);
-/* gweight [4, C, O] fp32 from g [N, O, 16] and x, or with x NULL its 8-bit form. */
+/* gweight [4, C, O] fp32 from g [N, O, 16] and x, or with x NULL its 8-bit form (an infinite g in fp32
+ * then gives NaN, and one below 2^-110 counts to 2^-133 only). */
 size_t batteries_channel_mixing_weight_grad_workspace_bytes(int64_t N, int C, int O);
 int batteries_channel_mixing_weight_grad(const void* x, const uint8_t* codes, const uint8_t* exps,
                                          const void* g, float* gweight, int64_t N, int C, int O,
