@@ -22,7 +22,7 @@ struct GateArgs {
     const uint8_t *codes_in, *exps_in;
     void *y;
     uint8_t *codes, *exps;
-    uint32_t blocks;                       // N * ckpt_blocks(C)
+    uint32_t blocks;                       // of a launch: atoms * ckpt_blocks(C)
     int C;
 };
 
@@ -182,9 +182,29 @@ __global__ __launch_bounds__(256) void gate_bwd_kernel(GateArgs a) {
     }
 }
 
+// Blocks of a launch: 2^31 threads at most (8 threads a block and turn in fp32, 4 in bf16).  A grid of 2^32
+// threads and more is not refused by the runtime: it leaves results unwritten.
+constexpr int64_t kGateLaunch = (int64_t)1 << 28;
+
 template <typename T>
-static unsigned gate_grid(uint32_t blocks) {
-    return (unsigned)ceil_div(blocks, 256 / (128 / Chan<T>::kN) * kGateAhead);
+static int gate_run(void (*kernel)(GateArgs), const GateArgs& all, int64_t N, hipStream_t s) {
+    const int64_t per = ckpt_blocks(all.C), most = kGateLaunch / per;
+    auto move = [](auto* p, int64_t n) { return p ? p + n : p; };
+    for (int64_t n = 0; n < N; n += most) {
+        GateArgs a = all;
+        const int64_t at = n * a.C * 16;
+        a.x = move((const T*)all.x, at);
+        a.g = move((const T*)all.g, at);
+        a.y = move((T*)all.y, at);
+        a.codes_in = move(all.codes_in, at);
+        a.exps_in = move(all.exps_in, n * per);
+        a.codes = move(all.codes, at);
+        a.exps = move(all.exps, n * per);
+        a.blocks = (uint32_t)(std::min(N - n, most) * per);
+        const int64_t grid = ceil_div(a.blocks, 256 / (128 / Chan<T>::kN) * kGateAhead);
+        kernel<<<(unsigned)grid, 256, 0, s>>>(a);
+    }
+    return (int)hipGetLastError();
 }
 static bool gate_shape_ok(int64_t N, int C, int dtype) {
     return N >= 0 && C >= 1 && C <= kGateMaxC && (dtype == 0 || dtype == 1) &&
@@ -201,15 +221,11 @@ extern "C" int batteries_gate_activation(const void* x, void* y, uint8_t* codes,
     if (N == 0) return BM_OK;
     GateArgs a{};
     a.x = x; a.y = y; a.codes = codes; a.exps = exps; a.C = C;
-    a.blocks = (uint32_t)(N * ckpt_blocks(C));
-    if (dtype == 0) {
-        if (codes) gate_fwd_kernel<float, true, true><<<gate_grid<float>(a.blocks), 256, 0, stream>>>(a);
-        else gate_fwd_kernel<float, true, false><<<gate_grid<float>(a.blocks), 256, 0, stream>>>(a);
-    } else {
-        if (codes) gate_fwd_kernel<uint16_t, true, true><<<gate_grid<uint16_t>(a.blocks), 256, 0, stream>>>(a);
-        else gate_fwd_kernel<uint16_t, true, false><<<gate_grid<uint16_t>(a.blocks), 256, 0, stream>>>(a);
-    }
-    return (int)hipGetLastError();
+    if (dtype == 0)
+        return gate_run<float>(codes ? gate_fwd_kernel<float, true, true> : gate_fwd_kernel<float, true, false>,
+                               a, N, stream);
+    return gate_run<uint16_t>(
+        codes ? gate_fwd_kernel<uint16_t, true, true> : gate_fwd_kernel<uint16_t, true, false>, a, N, stream);
 }
 
 extern "C" int batteries_gate_activation_backward(const void* x, const uint8_t* codes,
@@ -221,15 +237,11 @@ extern "C" int batteries_gate_activation_backward(const void* x, const uint8_t* 
     if (N == 0) return BM_OK;
     GateArgs a{};
     a.x = x; a.g = g; a.y = gx; a.codes_in = codes; a.exps_in = exps; a.C = C;
-    a.blocks = (uint32_t)(N * ckpt_blocks(C));
-    if (dtype == 0) {
-        if (!x) gate_bwd_kernel<float, true, true><<<gate_grid<float>(a.blocks), 256, 0, stream>>>(a);
-        else gate_bwd_kernel<float, false, true><<<gate_grid<float>(a.blocks), 256, 0, stream>>>(a);
-    } else {
-        if (!x) gate_bwd_kernel<uint16_t, true, true><<<gate_grid<uint16_t>(a.blocks), 256, 0, stream>>>(a);
-        else gate_bwd_kernel<uint16_t, false, true><<<gate_grid<uint16_t>(a.blocks), 256, 0, stream>>>(a);
-    }
-    return (int)hipGetLastError();
+    if (dtype == 0)
+        return gate_run<float>(x ? gate_bwd_kernel<float, false, true> : gate_bwd_kernel<float, true, true>, a,
+                               N, stream);
+    return gate_run<uint16_t>(
+        x ? gate_bwd_kernel<uint16_t, false, true> : gate_bwd_kernel<uint16_t, true, true>, a, N, stream);
 }
 
 extern "C" int batteries_checkpoint_encode(const void* x, uint8_t* codes, uint8_t* exps, int64_t N,
@@ -239,10 +251,8 @@ extern "C" int batteries_checkpoint_encode(const void* x, uint8_t* codes, uint8_
     if (N == 0) return BM_OK;
     GateArgs a{};
     a.x = x; a.codes = codes; a.exps = exps; a.C = C;
-    a.blocks = (uint32_t)(N * ckpt_blocks(C));
-    if (dtype == 0) gate_fwd_kernel<float, false, true><<<gate_grid<float>(a.blocks), 256, 0, stream>>>(a);
-    else gate_fwd_kernel<uint16_t, false, true><<<gate_grid<uint16_t>(a.blocks), 256, 0, stream>>>(a);
-    return (int)hipGetLastError();
+    return dtype == 0 ? gate_run<float>(gate_fwd_kernel<float, false, true>, a, N, stream)
+                      : gate_run<uint16_t>(gate_fwd_kernel<uint16_t, false, true>, a, N, stream);
 }
 
 extern "C" int batteries_checkpoint_decode(const uint8_t* codes, const uint8_t* exps, void* x, int64_t N,
@@ -252,8 +262,6 @@ extern "C" int batteries_checkpoint_decode(const uint8_t* codes, const uint8_t* 
     if (N == 0) return BM_OK;
     GateArgs a{};
     a.codes_in = codes; a.exps_in = exps; a.y = x; a.C = C;
-    a.blocks = (uint32_t)(N * ckpt_blocks(C));
-    if (dtype == 0) gate_bwd_kernel<float, true, false><<<gate_grid<float>(a.blocks), 256, 0, stream>>>(a);
-    else gate_bwd_kernel<uint16_t, true, false><<<gate_grid<uint16_t>(a.blocks), 256, 0, stream>>>(a);
-    return (int)hipGetLastError();
+    return dtype == 0 ? gate_run<float>(gate_bwd_kernel<float, true, false>, a, N, stream)
+                      : gate_run<uint16_t>(gate_bwd_kernel<uint16_t, true, false>, a, N, stream);
 }
