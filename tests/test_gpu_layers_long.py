@@ -4,6 +4,9 @@ range, batches of edges, launches after the first.  Every row differs from every
 Bounds, u = 2^-24:
   mixing    a sum of K products, each as exact as one of fp32: (K + 16) u sum |x w|; bf16: the weight to
             2^-15, the result to 2^-8 of itself more
+  gW        a sum of n (2 l + 1) products of exact values: (n (2 l + 1) + 16) u sum |x g|; as a whole 3e-6, as
+            roundings do not add up one way
+  gtable    a sum of n terms in any order: (n + 8) u sum |g|
 """
 import pytest
 import torch
@@ -36,6 +39,14 @@ def _mixed(x, w):
     """[N, O, 16] in float64, one product for each component."""
     x, w = x.double(), w.double()
     return torch.stack([x[:, :, m].contiguous() @ w[l] for m, l in enumerate(DEGREE)], 2)
+
+
+def _weight_gradient(x, g):
+    x, g = x.double(), g.double()
+    out = torch.zeros(4, x.shape[1], g.shape[1], dtype=torch.float64, device=x.device)
+    for m, l in enumerate(DEGREE):
+        out[l] += x[:, :, m].t().contiguous() @ g[:, :, m].contiguous()
+    return out
 
 
 # ---------------------------------------------------------------------------
@@ -72,11 +83,56 @@ def test_mixing_takes_many_tiles(dev, dtype, k, m, transposed):
 
 def test_the_reference_here_is_the_oracle(dev):
     from oracle import layers as ol
-    x = _features(dev, 30, 5, "f32", 1)
+    x, g = _features(dev, 30, 5, "f32", 1), _features(dev, 30, 7, "f32", 2)
     w = torch.randn(4, 5, 7, generator=_gen(dev, 3), device=dev)
-    y = ol.channel_mixing(x.cpu().numpy(), w.cpu().numpy())
-    # float64 both, sums of 5 terms in another order
+    y, _, gw = ol.channel_mixing(x.cpu().numpy(), w.cpu().numpy(), g.cpu().numpy())
+    # float64 both, sums of up to 210 terms in another order
     assert (_mixed(x, w).cpu() - torch.from_numpy(y)).abs().max() <= 1e-12
+    assert (_weight_gradient(x, g).cpu() - torch.from_numpy(gw)).abs().max() <= 1e-12
+
+
+# ---------------------------------------------------------------------------
+# the weight's gradient: steps after the first of a range of atoms
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kept", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,c,o", [(12345, 64, 64), (12295, 20, 40), (1003, 128, 1024), (2501, 70, 300),
+                                   (1507, 200, 300), (1001, 1024, 65), (4101, 100, 200)])
+def test_weight_gradient_takes_many_steps(dev, dtype, kept, n, c, o):
+    """At most 256 workgroups take 64 or 128 channels by 64 each over ranges of steps of 16 atoms (8 in
+    fp32): three steps of a range at least here, and an odd end."""
+    x, g = _features(dev, n, c, dtype, c), _features(dev, n, o, dtype, o + 1)
+    if kept:
+        codes, exps = _batmobile.checkpoint_encode(x)
+        x = _batmobile.checkpoint_decode(codes, exps, torch.float32)
+        gw = _batmobile.channel_mixing_weight_grad(None, codes, exps, g)
+    else:
+        gw = _batmobile.channel_mixing_weight_grad(x, None, None, g)
+    want, size = _weight_gradient(x, g), _weight_gradient(x.abs(), g.abs())
+    terms = n * torch.tensor([1.0, 3, 5, 7], device=dev, dtype=torch.float64)[:, None, None]
+    _within(gw, want, size * (terms + 16) * U)
+    assert (gw - want).abs().max() <= 3e-6 * want.abs().max()
+
+
+# ---------------------------------------------------------------------------
+# the bias's table: batches of edges after the first of a share
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("e,b,h", [(900_001, 64, 8), (450_007, 65, 8), (450_003, 128, 8),
+                                   (260_011, 200, 8), (260_005, 300, 8), (70_003, 200, 40),
+                                   (40_009, 150, 64), (40_013, 300, 70), (900_009, 7, 8)])
+def test_table_gradient_takes_many_batches(dev, e, b, h):
+    """At most 512 workgroups share the edges; a batch is 16 steps (8 up to 64 buckets) of each wave."""
+    gen = _gen(dev, b + h)
+    k = torch.randint(0, b, (e,), generator=gen, device=dev)
+    g = torch.randn(e, h, generator=gen, device=dev)
+    gt, _ = _batmobile.distance_bias_backward(None, k.short(), g, b, 0.0, True, False)
+    zero = torch.zeros(b, h, dtype=torch.float64)
+    k, g = k.cpu(), g.cpu().double()
+    want, size = zero.index_add(0, k, g), zero.index_add(0, k, g.abs())
+    _within(gt.cpu(), want, (torch.bincount(k, minlength=b)[:, None] + 8) * U * size)
+    assert (gt.cpu() - want).abs().max() <= 3e-6 * size.max()
 
 
 # ---------------------------------------------------------------------------
