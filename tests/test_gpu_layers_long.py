@@ -7,6 +7,7 @@ Bounds, u = 2^-24:
   gW        a sum of n (2 l + 1) products of exact values: (n (2 l + 1) + 16) u sum |x g|; as a whole 3e-6, as
             roundings do not add up one way
   gtable    a sum of n terms in any order: (n + 8) u sum |g|
+  glengths  a sum of H terms, and six roundings of the factor: (H + 8) u sum |g| |factor|
 """
 import pytest
 import torch
@@ -138,6 +139,19 @@ def test_table_gradient_takes_many_batches(dev, e, b, h):
 # ---------------------------------------------------------------------------
 # launches after the first
 # ---------------------------------------------------------------------------
+
+def test_lengths_gradient_takes_a_second_launch(dev):
+    """A launch takes 2^26 edges with 16 lanes an edge."""
+    e, h, c = (1 << 26) + 77, 9, 5.0
+    gen = _gen(dev, 4)
+    r, g = 6 * torch.rand(e, generator=gen, device=dev), torch.empty(e, h, device=dev)
+    g.normal_(generator=gen)
+    _, gl = _batmobile.distance_bias_backward(r, None, g, 1, c, False, True)
+    for part in (slice(0, 500), slice((1 << 26) - 500, e)):
+        q, gq = r[part].double(), g[part].double()
+        factor = torch.where(q < c, -2 * q / ((c - q) * (c + q)), 0.0)
+        _within(gl[part], factor * gq.sum(1), (h + 8) * U * factor.abs() * gq.abs().sum(1))
+
 
 def _rows_that_count(n, chunk):
     """The ends of launches, and of what 2^32 threads take."""
