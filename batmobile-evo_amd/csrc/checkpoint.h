@@ -2,8 +2,9 @@
 //
 // Eight channels of an atom's features [N, C, 16] (128 values; the last block of an atom may have fewer)
 // share a power of two 2^E, the least with max |x| <= 448 * 2^E, E in [-110, 120], and hold x / 2^E as
-// e4m3 (sign, 4 bits of exponent, 3 of mantissa, largest value 448), rounded to nearest even: off by at
-// most 2^-4 of the value down to 2^-15 of the block's largest.  The power is exact in fp32 and bf16, and so is
+// e4m3 (sign, 4 bits of exponent, 3 of mantissa, largest value 448), rounded to nearest even: a value of
+// 2^-6 2^E or more is off by 2^-4 of itself at most, a smaller one by 2^-10 2^E.  The block's largest lies
+// above 224 2^E (E > -110), so 2^-4 holds down to 2^-13.8 of it.  The power is exact in fp32 and bf16, and so is
 // a decoded value, so the factors of the backward's products lose nothing more.  codes [N, C, 16]
 // and exps [N, ceil(C / 8)] are bytes, an exponent kept as E + 127.  A value that is not finite is kept
 // as NaN and has no part in the maximum.  At E = 120 the code 256 would be 2^128: values from 248 on take 240,

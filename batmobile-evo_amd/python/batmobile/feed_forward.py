@@ -8,8 +8,8 @@ what mixes channels within a degree, or scales all components of one, commutes w
 
 With checkpoint="e4m3" a layer keeps its input for the backward pass in 8 bits instead of 16 or 32:
 blocks of 8 channels of an atom share a power of two, the least with max |x| <= 448 times it
-(2^-110 to 2^120), and hold x over it as e4m3, off by at most 2^-4 of a value (down to 2^-15 of
-the block's largest).  The output and what the gradient passes on through a mixing do not change; the
+(2^-110 to 2^120), and hold x over it as e4m3: a value is off by 2^-4 of itself at most, one below
+2^-6 times the power (2^-13.8 of the block's largest) by 2^-10 times the power.  The output and what the gradient passes on through a mixing do not change; the
 weight's gradient, and the activation's, are those at the input so kept.  A value that is not
 finite is kept as NaN.
 """

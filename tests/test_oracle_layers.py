@@ -111,3 +111,21 @@ def test_encode():
     assert e[0, 0] == 127 - 7 and e[0, 1] == 127 - 110
     v = ol.decode(c, e)
     assert np.isnan(v[0, 0, 0]) and np.isnan(v[0, 1, 1]) and v[0, 2, 2] == 3.0
+
+
+@pytest.mark.parametrize("top", [225.0, 300.0, 448.0])
+def test_how_far_codes_are_off(top):
+    """A value of 2^-6 2^E or more by 2^-4 of itself at most, a smaller one by 2^-10 2^E; in a block whose
+    largest is just above 224 2^E, 2^-4 holds down to 2^-13.8 of it and no further."""
+    rng = _rng(7)
+    for k in (-100, 0, 100):
+        x = np.exp2(rng.uniform(-16, 0, (40, 8, 16))) * rng.choice([-1, 1], (40, 8, 16)) * top * 2.0 ** k
+        x[:, 0, 0] = top * 2.0 ** k
+        c, e = ol.encode(x)
+        assert (e == k + 127).all()
+        off, unit = np.abs(ol.decode(c, e) - x), 2.0 ** k
+        large = np.abs(x) >= 2.0 ** -6 * unit
+        assert (off <= 2.0 ** -4 * np.abs(x))[large].all() and (off <= 2.0 ** -10 * unit)[~large].all()
+        assert large[np.abs(x) >= 2.0 ** -13.8 * top * unit].all()
+        small = ~large & (np.abs(x) >= 2.0 ** -15 * top * unit)
+        assert (off > 2.0 ** -4 * np.abs(x))[small].any()
