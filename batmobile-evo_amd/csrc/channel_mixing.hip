@@ -950,6 +950,15 @@ static size_t mix_bytes(int K, int M) {
     return (size_t)((K + 31) / 32) * 4 * a.tiles * MixTile<T>::kPW * 64 * 16;
 }
 
+// The general kernel's launch: at most 2^22 workgroups (and the last 8 units' of a chunk) of 512 threads.  Beyond
+// that features and results do not fit a card's memory.
+template <typename T>
+static bool mix_launch_ok(int64_t n, int K, int M) {
+    MixArgs a{};
+    mix_tiles<T>(M, a);
+    return K <= kStayMost<T> || n * a.chunks <= (int64_t)1 << 27;
+}
+
 // More than 64 KB of LDS for a kernel, allowed once on each device
 static int mix_allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& allowed) {
     int device = 0;
@@ -1000,18 +1009,8 @@ static int mix_run(MixArgs a, void* ws, hipStream_t s) {
     mix_pack_kernel<S::kPW><<<(total + 255) / 256, 256, 0, s>>>(a.weight, (v4u*)ws, a.K, a.M, a.sk,
                                                                a.sm, a.tiles, total);
     a.w = (const v4u*)ws;
-    // atoms of a launch: 2^22 workgroups (threads < 2^32)
-    const int64_t most = ((int64_t)1 << 22) / a.chunks * 16 * S::kNG;
-    const int64_t n = a.n;
-    const char *x = (const char*)a.x;
-    char* y = (char*)a.y;
-    for (int64_t n0 = 0; n0 < n; n0 += most) {
-        a.x = x + n0 * a.K * 16 * (int64_t)sizeof(T);
-        a.y = y + n0 * a.M * 16 * (int64_t)sizeof(T);
-        a.n = std::min(n - n0, most);
-        a.units = ceil_div(a.n, 16 * S::kNG);
-        mix_kernel<T><<<mix_grid(a.units, a.chunks), 256 * S::kNG, S::kBytes, s>>>(a);
-    }
+    a.units = ceil_div(a.n, 16 * S::kNG);
+    mix_kernel<T><<<mix_grid(a.units, a.chunks), 256 * S::kNG, S::kBytes, s>>>(a);
     return (int)hipGetLastError();
 }
 
@@ -1059,11 +1058,13 @@ extern "C" int batteries_channel_mixing(const void* x, const float* weight, void
                                         size_t workspace_bytes, hipStream_t stream) {
     if (!mix_shape_ok(N, C, O, dtype) || (N > 0 && (!x || !weight || !y))) return BM_ERR_ARG;
     if (!aligned_to({x, y, workspace}, 16) || !aligned_to({weight}, 4)) return BM_ERR_ARG;
+    const int K = transposed ? O : C, M = transposed ? C : O;
+    if (!(dtype == 0 ? mix_launch_ok<float>(N, K, M) : mix_launch_ok<uint16_t>(N, K, M))) return BM_ERR_ARG;
     if (N == 0) return BM_OK;
     if (workspace_bytes < batteries_channel_mixing_workspace_bytes(C, O, transposed, dtype) || !workspace)
         return BM_ERR_WORKSPACE;
     MixArgs a{};
-    a.x = x; a.y = y; a.n = N; a.K = transposed ? O : C; a.M = transposed ? C : O;
+    a.x = x; a.y = y; a.n = N; a.K = K; a.M = M;
     a.weight = weight; a.sk = transposed ? 1 : O; a.sm = transposed ? O : 1;
     return dtype == 0 ? mix_run<float>(a, workspace, stream) : mix_run<uint16_t>(a, workspace, stream);
 }

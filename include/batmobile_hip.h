@@ -673,7 +673,8 @@ int batteries_gate_activation_backward(const void* x, const uint8_t* codes, cons
  * x [N, C, 16] to y [N, O, 16] in fp32 (dtype 0) or bf16 (dtype 1), 16-byte aligned, weight
  * [4, C, O] fp32; transposed: x [N, O, 16] to y [N, C, 16], the sum over o.  fp32 accuracy of the
  * products in fp32 (a feature below 2^-110 counts to 2^-133 only); with bf16 features the weight is
- * rounded to 15 bits.  C, O <= 2048, N < 2^31.
+ * rounded to 15 bits.  C, O <= 2048, N < 2^31, and N ceil(channels of y / 64) <= 2^27 where x has more than
+ * 64 (bf16: 256) channels.
  * ------------------------------------------------------------------------- */
 size_t batteries_channel_mixing_workspace_bytes(int C, int O, int transposed, int dtype);
 int batteries_channel_mixing(const void* x, const float* weight, void* y, int64_t N, int C, int O,

@@ -217,3 +217,21 @@ def test_an_attention_block_without_the_options_is_as_it_was():
     for n, s in (("w_qkv", (4, 16, 32)), ("w_out", (4, 16, 16)), ("w_gate", (16, 64)), ("w1", (8, 32)),
                  ("w2", (32, 4))):
         assert torch.equal(getattr(block, n).detach(), torch.randn(*s, generator=g) / s[-2] ** 0.5)
+
+
+# ---------------------------------------------------------------------------
+# launches
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("c,o,dtype,n", [(128, 64, 0, (1 << 27) + 1), (65, 65, 0, (1 << 26) + 1),
+                                         (300, 2048, 1, (1 << 22) + 1)])
+def test_channel_mixing_refuses_more_than_a_launch_takes(lib, c, o, dtype, n):
+    """One launch of the kernel for many channels: N ceil(outputs / 64) <= 2^27, more than any memory holds."""
+    assert _mix(lib, n=n, c=c, o=o, dtype=dtype) == ERR_ARG
+    assert n * (16 * (4 >> dtype)) * (c + o) > 288 * 2 ** 30
+
+
+@pytest.mark.parametrize("c,o,dtype", [(64, 2048, 0), (256, 2048, 1)])
+def test_channel_mixing_of_few_channels_has_no_such_limit(lib, c, o, dtype):
+    """(a workspace too small is what is refused next)"""
+    assert _mix(lib, n=(1 << 31) - 1, c=c, o=o, dtype=dtype, b=15) == ERR_WORKSPACE
