@@ -78,7 +78,8 @@ class AttentionBlock(torch.nn.Module):
             self.table = None
             self.w1, self.w2 = normal(N_BASIS, HIDDEN), normal(HIDDEN, heads)
         else:
-            self.table = normal(buckets, heads)
+            # the size of what the MLP begins with, whatever the number of buckets
+            self.table = torch.nn.Parameter((0.1 * torch.randn(buckets, heads, generator=g)).to(device))
             self.register_buffer("boundaries", torch.arange(1, buckets, device=device)
                                  * (self.cutoff / buckets))
 

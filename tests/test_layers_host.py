@@ -235,3 +235,16 @@ def test_channel_mixing_refuses_more_than_a_launch_takes(lib, c, o, dtype, n):
 def test_channel_mixing_of_few_channels_has_no_such_limit(lib, c, o, dtype):
     """(a workspace too small is what is refused next)"""
     assert _mix(lib, n=(1 << 31) - 1, c=c, o=o, dtype=dtype, b=15) == ERR_WORKSPACE
+
+
+def test_a_table_begins_the_same_size_for_any_number_of_buckets():
+    """A lookup adds nothing up: its entries do not get smaller as buckets get finer.  The spread of 4096
+    normal numbers is known to 1 / sqrt(2 * 4096) = 1.1 %; four times that of each."""
+    import batmobile
+
+    def spread(buckets, heads):
+        g = torch.Generator().manual_seed(buckets)
+        return float(batmobile.AttentionBlock(heads, heads, generator=g, buckets=buckets).table.detach().std())
+
+    few, many = spread(4, 1024), spread(1024, 4)
+    assert abs(few / many - 1) <= 0.09
