@@ -83,6 +83,11 @@ class AttentionBlock(torch.nn.Module):
             self.register_buffer("boundaries", torch.arange(1, buckets, device=device)
                                  * (self.cutoff / buckets))
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "checkpoint" not in self.__dict__:            # pickled before the options were there
+            self.table = self.checkpoint = None
+
     def edge_bias(self, lengths):
         """[E, H]: a function of the edge length, -inf from the cutoff on."""
         if self.table is not None:

@@ -248,3 +248,19 @@ def test_a_table_begins_the_same_size_for_any_number_of_buckets():
 
     few, many = spread(4, 1024), spread(1024, 4)
     assert abs(few / many - 1) <= 0.09
+
+
+def test_an_attention_block_kept_before_it_had_the_options_still_runs():
+    """A pickled module is its attributes: one without a table and checkpoints has neither."""
+    import pickle
+    import batmobile
+    block = batmobile.AttentionBlock(16, 4, 2)
+    want = block.edge_bias(torch.linspace(0.5, 6.0, 9))
+    state = {k: v for k, v in block.__dict__.items() if k not in ("table", "checkpoint")}
+    old = batmobile.AttentionBlock.__new__(batmobile.AttentionBlock)
+    old.__setstate__(pickle.loads(pickle.dumps(state)))
+    x, w = torch.randn(3, 16, 16), block.w_out
+    assert torch.equal(old.edge_bias(torch.linspace(0.5, 6.0, 9)), want)
+    assert torch.equal(old.mix(x, w), block.mix(x, w))
+    new = pickle.loads(pickle.dumps(batmobile.AttentionBlock(16, 4, buckets=5, checkpoint="e4m3")))
+    assert new.table.shape == (5, 4) and new.checkpoint == "e4m3"
