@@ -390,6 +390,27 @@ def test_channel_mixing_infinities(dev, c):
         assert torch.equal(y, want)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("c", [20, 64, 70, 128, 200, 256, 300])
+def test_channel_mixing_infinities_times_round_weights(dev, dtype, c):
+    """Weights of which nothing is left behind their leading bits, zeros among them: an infinity times
+    zero is no number, any other weight gives its sign's infinity."""
+    import batmobile
+    x = torch.randint(-4, 5, (35, c, 16), generator=gen(41)).to(TYPES[dtype])
+    w = torch.tensor([1.0, -2.0, 0.5, -(2.0 ** -100), 1.5, 0.0, -0.0, 2.0 ** 100])
+    w = w[torch.randint(0, 8, (4, c, 24), generator=gen(42))]
+    w[:, 1, :8] = torch.tensor([1.0, -2.0, 0.5, -(2.0 ** -100), 1.5, 0.0, -0.0, 2.0 ** 100])
+    x[3, 1, 0], x[20, 1, 5], x[34, 1, 15] = float("inf"), -float("inf"), float("inf")
+    y = _np(batmobile.channel_mixing(x.to(dev), w.to(dev)))
+    with np.errstate(invalid="ignore"):
+        for n, m, l in ((3, 0, 0), (20, 5, 2), (34, 15, 3)):
+            want = np.float64(x[n, 1, m]) * w[l, 1].double().numpy()
+            assert np.array_equal(y[n, :, m], want, equal_nan=True)
+    assert np.isfinite(np.delete(y, [3, 20, 34], 0)).all()
+    back = _np(_batmobile.channel_mixing(x.to(dev), w.transpose(1, 2).contiguous().to(dev), True))
+    assert np.array_equal(back, y, equal_nan=True)
+
+
 @pytest.mark.parametrize("kept", [None, "e4m3"])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_weight_gradient_with_nan(dev, dtype, kept):
