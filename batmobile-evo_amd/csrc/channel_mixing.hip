@@ -6,7 +6,9 @@
 //   gW[l, c, o] = sum_n sum_{m of degree l} x[n, c, m] g[n, o, m]  (x as it was, or from its 8-bit form)
 //
 // Sums are fp32.  bf16 features go to the bf16 matrix cores as they are; their weight, which is fp32, goes in
-// two parts (off by 2^-15 of it at most).  fp32 features run on the fp32 matrix cores (up to 64 channels in,
+// two parts (off by 2^-15 of it at most): a third would make a wave's 128 registers of weight 192, for results
+// that are rounded to 8 bits.  At 128 to 128 channels 0.45 % of them round the other way than with all 24 bits, and
+// the error against 64 bits is the same, 1.659e-3.  fp32 features run on the fp32 matrix cores (up to 64 channels in,
 // and for gW) or, three parts each, in six products on the bf16 ones, as exact as fp32 products.  An 8-bit
 // form is exact in bf16, so against it only g is split.
 //
@@ -17,10 +19,11 @@
 // order of the sum is free as long as both operands have the same one: value j of lane group q is channel
 // (atom) 4 j + q.
 //
-// Measured, us (what the bytes take at a copy's 5 TB/s): 50,000 atoms 128 to 128 in bf16 104 (82), its gW 122 to 136,
-// from the 8-bit form 94 (62); 64 to 64 in bf16 43 (41), in fp32 104 (82); 20,011 atoms 100 to 200 in fp32
-// 196 (77), 200 to 100 148, gW 234, from the 8-bit form 146.  bf16 is bound by memory and by reads and
-// writes that take turns; fp32 by the matrix cores and the splitting.
+// Measured, us (what the bytes take at a copy's 5 TB/s): 50,000 atoms 128 to 128 in bf16 104 to 112 (82), its gW
+// 122 to 136, from the 8-bit form 94 (62); 256 to 128 200 (123); 64 to 64 in bf16 38 (41), in fp32 101 (82); 20,011
+// atoms 100 to 200 in fp32 184 (77), 200 to 100 141, gW 234, from the 8-bit form 146.  bf16 is bound by memory and
+// by waits for all of it at barriers (stay_wait), above 128 channels by features read again for each 32 outputs;
+// fp32 by the matrix cores and the splitting.
 #include <atomic>
 #include <type_traits>
 
@@ -31,8 +34,10 @@ namespace bmhip {
 
 constexpr int kMixMaxC = 2048;
 // Channels up to which the weight stays in registers.  Against the general kernel, us: fp32 50,000 atoms 64
-// to 64 104 and 114, but 20,011 100 to 200 250 and 196; bf16 50,000 128 to 128 104 and 162, 20,011 200 to
-// 256 174 and 178.  Above 256 in bf16 a degree's weight no longer fits.
+// to 64 101 and 114, 33 to 100 162 and 158; bf16 50,000 64 to 64 38 and 52, 128 to 128 104 to 112 and 151, 128 to
+// 256 188 and 266, 256 to 128 200 and 222; 20,011 160 to 160 72 and 72, 200 to 256 162 and 159, 256 to 64 47 and 62.
+// fp32 above 64 in registers took 250 at 20,011 100 to 200 (184 as it is); above 256 in bf16 a degree's weight does
+// not fit.
 template <typename T>
 constexpr int kStayMost = sizeof(T) == 4 ? 64 : 256;
 constexpr int kMixFar = 0x7fffff00;        // a buffer offset past every buffer here: reads 0
@@ -342,10 +347,11 @@ __global__ __launch_bounds__(256 * MixTile<T>::kNG) void mix_kernel(MixArgs a) {
 // atoms in turn and reads nothing but features.
 //
 // A step's features (32 channels of 16 atoms) come to LDS by direct loads of 16 bytes a lane, whole lines,
-// kAhead steps ahead; straight to registers a wave would ask for 8 or 16 bytes of every 32 or 64,
+// asked for kAhead steps ahead (1 in fp32, 2 in bf16; but see stay_wait); straight to registers a wave would ask for 8 or 16 bytes of every 32 or 64,
 // whose rate is the address units' (3.6 TB/s with every line in L1).  A wave takes 8 of the 16 components,
 // those of degrees 1 and 2 (1..8) or of 3 and 0 (9..15, 0), so two degrees of the weight, for OT tiles
-// of outputs: 2 KS OT PW registers x 4.  In LDS the 16-byte pieces of an atom are permuted by its
+// of outputs: 2 KS OT PW registers x 4, 128 at most.  With 65 to 128 channels that and the sums do not quite fit: to
+// more than 32 outputs 12 bytes a lane lie in scratch memory, to 32 and fewer 84, read back in a tile's last step.  In LDS the 16-byte pieces of an atom are permuted by its
 // number, so that 16 atoms' reads meet no bank twice.
 // The two kinds of wave run code of their own, barrier for barrier alike.
 // ---------------------------------------------------------------------------
@@ -465,7 +471,10 @@ struct StayShape {
 };
 
 // Until at most LATER loads and `tiles` tiles' stores are under way: what was asked for before them is
-// there (the counter goes down in the order of issue, loads and stores alike)
+// there (the counter goes down in the order of issue, loads and stores alike).  The wave's own loads, that is: the
+// __syncthreads() behind it orders them for the other waves, and for that the compiler has it wait for all vector
+// memory, at every step of a tile but the first and at the first barrier of the way out.  So only the first step's
+// count lets anything go on: in effect loads have one step, and a tile's stores end within the next one's first.
 template <int LATER, int STORES, int MOST>
 __device__ __forceinline__ void stay_wait(int tiles) {
     static_for<MOST + 1>([&](auto ii) {

@@ -27,7 +27,8 @@ def channel_mixing(x, weight, checkpoint=None):
     """y [N, C_out, 16] of x [N, C_in, 16] (float32 or bfloat16) and weight [4, C_in, C_out]
     (float32), up to 2048 channels.  float32 features have float32 accuracy
     (numbers below 2^-110 only that of 2^-133); with bfloat16 ones the weight is taken to 15 bits and
-    sums are float32.  Gradients for both, which cannot be differentiated
+    sums are float32, which leaves the error of the result's own rounding.  With "e4m3" an infinite
+    float32 gradient makes its column of the weight's gradient NaN.  Gradients for both, which cannot be differentiated
     again, and no forward-mode derivatives (an error).  checkpoint: None, or "e4m3".
     """
     return _batmobile.channel_mixing_autograd(x, weight, checkpoint)
