@@ -5,12 +5,12 @@
 //   gx[n, c, m] = sum_o g[n, o, m] W[l(m), c, o]                   (the same kernel, W transposed)
 //   gW[l, c, o] = sum_n sum_{m of degree l} x[n, c, m] g[n, o, m]  (x as it was, or from its 8-bit form)
 //
-// Sums are fp32.  bf16 features go to the bf16 matrix cores as they are; their weight, which is fp32, goes in
-// two parts (off by 2^-15 of it at most): a third would make a wave's 128 registers of weight 192, for results
-// that are rounded to 8 bits.  At 128 to 128 channels 0.45 % of them round the other way than with all 24 bits, and
-// the error against 64 bits is the same, 1.659e-3.  fp32 features run on the fp32 matrix cores (up to 64 channels in,
-// and for gW) or, three parts each, in six products on the bf16 ones, as exact as fp32 products.  An 8-bit
-// form is exact in bf16, so against it only g is split.
+// Sums are fp32. bf16 features go to the bf16 matrix cores as they are; their weight, which is fp32, goes
+// in two parts (off by 2^-15 of it at most): a third would make a wave's 128 registers of weight 192, for
+// results that are rounded to 8 bits. At 128 to 128 channels 0.45 % of them round the other way than with
+// all 24 bits, and the error against 64 bits is the same, 1.659e-3. fp32 features run on the fp32 matrix
+// cores (up to 64 channels in, and for gW) or, three parts each, in six products on the bf16 ones, as exact
+// as fp32 products. An 8-bit form is exact in bf16, so against it only g is split.
 //
 // The features lie [N, C, 16], 16 components together, and a matrix operand wants 8 values along the sum
 // for one component.  Whole lines come to LDS by direct loads; from there a lane takes the same components
@@ -347,12 +347,13 @@ __global__ __launch_bounds__(256 * MixTile<T>::kNG) void mix_kernel(MixArgs a) {
 // atoms in turn and reads nothing but features.
 //
 // A step's features (32 channels of 16 atoms) come to LDS by direct loads of 16 bytes a lane, whole lines,
-// asked for kAhead steps ahead (1 in fp32, 2 in bf16; but see stay_wait); straight to registers a wave would ask for 8 or 16 bytes of every 32 or 64,
-// whose rate is the address units' (3.6 TB/s with every line in L1).  A wave takes 8 of the 16 components,
-// those of degrees 1 and 2 (1..8) or of 3 and 0 (9..15, 0), so two degrees of the weight, for OT tiles
-// of outputs: 2 KS OT PW registers x 4, 128 at most.  With 65 to 128 channels that and the sums do not quite fit: to
-// more than 32 outputs 12 bytes a lane lie in scratch memory, to 32 and fewer 84, read back in a tile's last step.  In LDS the 16-byte pieces of an atom are permuted by its
-// number, so that 16 atoms' reads meet no bank twice.
+// asked for kAhead steps ahead (1 in fp32, 2 in bf16; but see stay_wait); straight to registers a wave would
+// ask for 8 or 16 bytes of every 32 or 64, whose rate is the address units' (3.6 TB/s with every line in L1). A
+// wave takes 8 of the 16 components, those of degrees 1 and 2 (1..8) or of 3 and 0 (9..15, 0), so two degrees
+// of the weight, for OT tiles of outputs: 2 KS OT PW registers x 4, 128 at most. With 65 to 128 channels that
+// and the sums do not quite fit: to more than 32 outputs 12 bytes a lane lie in scratch memory, to 32 and fewer
+// 84, read back in a tile's last step. In LDS the 16-byte pieces of an atom are permuted by its number, so that
+// 16 atoms' reads meet no bank twice.
 // The two kinds of wave run code of their own, barrier for barrier alike.
 // ---------------------------------------------------------------------------
 template <typename T>

@@ -7,11 +7,11 @@ what mixes channels within a degree, or scales all components of one, commutes w
     gate_activation:  y[c, m] = sigmoid(x[c, 0]) x[c, m]        (silu of the invariant)
 
 With checkpoint="e4m3" a layer keeps its input for the backward pass in 8 bits instead of 16 or 32:
-blocks of 8 channels of an atom share a power of two, the least with max |x| <= 448 times it
-(2^-110 to 2^120), and hold x over it as e4m3: a value is off by 2^-4 of itself at most, one below
-2^-6 times the power (2^-13.8 of the block's largest) by 2^-10 times the power.  The output and what the gradient passes on through a mixing do not change; the
-weight's gradient, and the activation's, are those at the input so kept.  A value that is not
-finite is kept as NaN.
+blocks of 8 channels of an atom share a power of two, the least with max |x| <= 448 times it (2^-110
+to 2^120), and hold x over it as e4m3: a value is off by 2^-4 of itself at most, one below 2^-6
+times the power (2^-13.8 of the block's largest) by 2^-10 times the power. The output and what the
+gradient passes on through a mixing do not change; the weight's gradient, and the activation's, are
+those at the input so kept. A value that is not finite is kept as NaN.
 """
 import math
 
@@ -25,11 +25,11 @@ from .layer_norm import layer_norm
 
 def channel_mixing(x, weight, checkpoint=None):
     """y [N, C_out, 16] of x [N, C_in, 16] (float32 or bfloat16) and weight [4, C_in, C_out]
-    (float32), up to 2048 channels.  float32 features have float32 accuracy
-    (numbers below 2^-110 only that of 2^-133); with bfloat16 ones the weight is taken to 15 bits and
-    sums are float32, which leaves the error of the result's own rounding.  With "e4m3" an infinite
-    float32 gradient makes its column of the weight's gradient NaN.  Gradients for both, which cannot be differentiated
-    again, and no forward-mode derivatives (an error).  checkpoint: None, or "e4m3".
+    (float32), up to 2048 channels.  float32 features have float32 accuracy (numbers below 2^-110
+    only that of 2^-133); with bfloat16 ones the weight is taken to 15 bits and sums are float32,
+    which leaves the error of the result's own rounding.  Gradients for both, which cannot be
+    differentiated again, and no forward-mode derivatives (an error).  checkpoint: None, or "e4m3",
+    with which an infinite float32 gradient makes its column of the weight's gradient NaN.
     """
     return _batmobile.channel_mixing_autograd(x, weight, checkpoint)
 
